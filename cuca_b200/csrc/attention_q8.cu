@@ -1,0 +1,596 @@
+// Causal grouped-query attention over 8-bit pages for few query rows: single tokens, short portions, and the 32-bit mode.
+// (Scales, weights and their exactness: attention_q8.cuh.)
+//
+// Both products run turned round on mma.sync.m16n8k16 (16-bit floats, 32-bit sums): the 16 rows are keys (then dimensions of
+// the values), the 8 columns are query rows, i.e. (token, head) pairs of one key head; S^T = K Q^T, O^T = V^T W^T. So a key
+// head's few query rows fill half an instruction instead of a quarter, and in 32-bit mode a row's two 16-bit parts are simply
+// two neighbouring columns: the same instructions serve both types.
+//
+// A block (4 warps) takes one tile of rows, one key head and a share of the keys; its warps take the groups of 16 keys in
+// turn, each through a ring of its own (16-byte asynchronous copies straight from the pages, no barrier in the loop), and are
+// joined at the end; shares of a tile's keys are joined by a second small launch. A thread's values sit in shared memory so
+// that it reads its fragments 16 bytes at a time without bank conflicts (`place`), and the order of dimensions and keys
+// within an instruction is chosen to match: a contraction may be summed in any order.
+//
+// Decoding is bound by the pages' bytes: 16 keys of 128 are 4.2 KB and some 270 warp instructions (176 of them turn codes into
+// 16-bit floats).
+#include "attention_q8.cuh"
+
+namespace {
+
+constexpr int GROUP = 16;     // keys of a step
+constexpr int STAGES = 4;     // of a warp's ring
+constexpr int WARPS = 4;
+
+__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {  // zeros where not ok
+  const int n = ok ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 shared_16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 shared_8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ float shared_f(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turned_8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// DP: the head size rounded up to 64, 128 or 256 (what is beyond d stays zero).
+template <int DP>
+struct Ring {
+  static constexpr int CHUNKS = DP / 16;                 // 16-byte pieces of a row
+  static constexpr int TENSOR = GROUP * DP;              // bytes of a group's keys
+  static constexpr int STAGE = 2 * TENSOR + 2 * GROUP * 4;  // keys, values, their scales
+  static constexpr int WARP = STAGES * STAGE;
+  // Where piece c of key k stands. A thread (g, t) of a warp reads keys g and g + 8 at pieces t, t + 4, .. and, for the values,
+  // keys 2t, 2t + 1, 2t + 8, 2t + 9 at piece g (half a piece with DP = 64): the eight lanes that are served together must find
+  // their pieces in eight different places of 128 bytes, for both.
+  static __device__ __forceinline__ uint32_t place(int k, int c) {
+    const int k0 = k & 1, k1 = (k >> 1) & 1, k2 = (k >> 2) & 1;
+    if (DP == 64) return (uint32_t)(((k & ~1) | (k0 ^ k1)) * 64 + ((c ^ (k2 << 1)) * 16));
+    return (uint32_t)(k * DP + ((c ^ (((k0 ^ k2) << 2) | (k1 << 1))) * 16));
+  }
+};
+
+// NT: tiles of 8 columns. PARTS: 1: bfloat16 rows, a column each; 2: 32-bit rows, two columns each. OPT: score cap, sink and
+// distance bias.
+template <int DP, int NT, int PARTS, bool OPT>
+__global__ void __launch_bounds__(WARPS * 32)
+attention_q8_kernel(const Q8Params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  using R = Ring<DP>;
+  using T = typename std::conditional<PARTS == 2, float, __nv_bfloat16>::type;
+  constexpr int CHUNKS = R::CHUNKS;
+  constexpr int QC = CHUNKS / 4;         // pieces of a key row that a thread reads
+  constexpr int TILES = DP / 16;         // of 16 dimensions
+  constexpr int COLS = NT * 8 / PARTS;   // query rows
+  constexpr int LC = 2 / PARTS;          // of a thread and column tile
+  constexpr bool Q_SHARED = NT * DP > 256;  // the queries' fragments do not fit the registers: they are read from shared memory
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  pdl_trigger();
+  pdl_wait();
+
+  // ---------------------------------------------------------------- rows, heads, keys
+  int row0, n_tok;
+  if (!q8_rows_of_tile(p, blockIdx.z, row0, n_tok)) return;
+  const int kvh = blockIdx.y / p.head_parts, hp = blockIdx.y % p.head_parts;
+  const int group_heads = p.nh / p.nkv;
+  const int head0 = kvh * group_heads + hp * p.heads_per_cta;
+  const int heads = min(p.heads_per_cta, group_heads - hp * p.heads_per_cta);
+  const int seq = p.seq_of_row[row0];
+  const int pos0 = p.positions[row0];
+  const int n_cols = n_tok * heads;
+  const bool nothing = seq < 0 || pos0 < 0;  // rows of no request
+  if (nothing) {
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i < n_cols * p.d; i += WARPS * 32) {
+        const int c = i / p.d;
+        ((T*)p.out)[(size_t)(row0 + c / heads) * p.out_stride + (size_t)(head0 + c % heads) * p.d + i % p.d] = from_f32<T>(0.f);
+      }
+    return;
+  }
+  const Q8Keys keys = q8_keys<GROUP>(p, pos0, n_tok);
+  const int share = p.chunk > 0 ? p.chunk / GROUP : keys.groups;
+  const int first = blockIdx.x * share;
+  const int last = (int)blockIdx.x == p.n_splits - 1 ? keys.groups : min(keys.groups, first + share);
+  if (first >= last) return;  // a share that this tile does not have
+  const bool alone = share >= keys.groups || p.n_splits == 1;
+  const int* table = p.tables + (size_t)seq * p.table_stride;
+
+  // ---------------------------------------------------------------- queries: the second operand's fragments
+  // column c of tile j is query row (8 j + c) / PARTS: token (..) / heads, head (..) % heads
+  uint8_t* my_ring = smem + warp * R::WARP;
+  uint32_t* q_shared = reinterpret_cast<uint32_t*>(smem + WARPS * R::WARP);  // [TILES][NT][32 lanes][2]
+  uint32_t qf[Q_SHARED ? 1 : TILES][Q_SHARED ? 1 : NT][2];
+  float q_down[NT][LC];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int col = (8 * j + g) / PARTS;
+    const bool ok = col < n_cols;
+    const T* src = (const T*)p.q + (size_t)(row0 + (ok ? col / heads : 0)) * p.q_stride + (size_t)(head0 + (ok ? col % heads : 0)) * p.d;
+    float v[QC][16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < QC; ++i) {
+      const int e0 = (t + 4 * i) * 16;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        v[i][e] = ok && e0 < p.d ? to_f32(src[e0 + e]) : 0.f;
+        top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+      }
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float up, down;
+    q8_query_scale(top, up, down);
+#pragma unroll
+    for (int c = 0; c < LC; ++c) q_down[j][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
+#pragma unroll
+    for (int i = 0; i < QC; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = top >= 0x7f800000u ? 0.f : v[i][4 * w + e] * up;
+          if (PARTS == 2 && (g & 1)) x[e] -= __half2float(__float2half_rn(x[e]));  // the second part
+        }
+        const uint32_t lo = q8_pack(x[0], x[1]), hi = q8_pack(x[2], x[3]);
+        if (Q_SHARED) {
+          if (warp == 0) *reinterpret_cast<uint2*>(q_shared + (((4 * i + w) * NT + j) * 32 + lane) * 2) = make_uint2(lo, hi);
+        } else {
+          qf[Q_SHARED ? 0 : 4 * i + w][Q_SHARED ? 0 : j][0] = lo;
+          qf[Q_SHARED ? 0 : 4 * i + w][Q_SHARED ? 0 : j][1] = hi;
+        }
+      }
+  }
+  // positions that bound what a column sees
+  int col_pos[NT][LC], col_lo[NT][LC], col_head[NT][LC];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int c = 0; c < LC; ++c) {
+      const int col = 8 * j / PARTS + LC * t + c;
+      const bool ok = col < n_cols;
+      col_pos[j][c] = ok ? pos0 + col / heads : -1;
+      col_lo[j][c] = p.window > 0 ? col_pos[j][c] - (p.window - 1) : 0;
+      col_head[j][c] = head0 + (ok ? col % heads : 0);
+    }
+  const int least_pos = pos0, most_lo = p.window > 0 ? pos0 + n_tok - 1 - (p.window - 1) : 0;
+
+  // ---------------------------------------------------------------- the ring
+  const uint32_t ring = shared_at(my_ring);
+  if (p.d < DP) {
+    for (int i = lane; i < R::WARP / 16; i += 32) reinterpret_cast<uint4*>(my_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
+  }
+  // Lane k of 16: where key k of a group stands in the pools, as a row number (-1: nowhere), looked up a step before its use.
+  auto lookup = [&](int j) -> long long {
+    if (j >= last) return -1;
+    const int kp = keys.at(j) * GROUP + (lane & 15);
+    if (kp >= keys.hi) return -1;
+    const int entry = kp / p.bs;
+    const int blk = entry < p.table_stride ? table[entry] : -1;
+    if (blk < 0 || blk >= p.n_blocks) {
+      // pages behind a window may have gone back; their keys are masked. Anything else is an error.
+      if ((kp >= (p.window > 0 ? pos0 - (p.window - 1) : 0) || kp < p.keep) && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+      return -1;
+    }
+    return ((long long)blk * p.nkv + kvh) * p.bs + kp % p.bs;
+  };
+  constexpr int KEYS_AT_ONCE = 32 / CHUNKS;
+  auto fetch = [&](int stage, long long mine) {
+    const uint32_t at = ring + stage * R::STAGE;
+    const int c = lane % CHUNKS;
+#pragma unroll
+    for (int i = 0; i < GROUP / KEYS_AT_ONCE; ++i) {
+      const int k = i * KEYS_AT_ONCE + lane / CHUNKS;
+      const long long row = __shfl_sync(0xffffffffu, mine, k);
+      const bool ok = row >= 0;
+      const size_t off = (size_t)(ok ? row : 0) * p.d + c * 16;
+      if (c * 16 < p.d) {
+        copy16(at + R::place(k, c), p.kpool + off, ok);
+        copy16(at + R::TENSOR + R::place(k, c), p.vpool + off, ok);
+      }
+    }
+    const float* scales = lane < 16 ? p.kscale : p.vscale;
+    copy4(at + 2 * R::TENSOR + lane * 4, scales + (mine >= 0 ? mine : 0), mine >= 0);
+  };
+
+  float acc[TILES][NT][4];
+#pragma unroll
+  for (int i = 0; i < TILES; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+  float m[NT][LC], l[NT][LC];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int c = 0; c < LC; ++c) { m[j][c] = -INFINITY; l[j][c] = 0.f; }
+
+  long long next;
+  {
+    long long at[STAGES - 1];
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) at[s] = lookup(first + warp + WARPS * s);
+    next = lookup(first + warp + WARPS * (STAGES - 1));
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+      if (first + warp + WARPS * s < last) fetch(s, at[s]);
+      copies_commit();
+    }
+  }
+  if (Q_SHARED) __syncthreads();
+
+  int stage = 0;
+  for (int j0 = first + warp; j0 < last; j0 += WARPS) {
+    copies_wait<STAGES - 2>();
+    __syncwarp();
+    {  // the stage that was read in the last turn
+      const int ahead = stage == 0 ? STAGES - 1 : stage - 1;
+      if (j0 + WARPS * (STAGES - 1) < last) fetch(ahead, next);
+      copies_commit();
+      next = lookup(j0 + WARPS * STAGES);
+    }
+    const uint32_t at = ring + stage * R::STAGE;
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+    // ------------------------------------------------ raw scores: rows g and g + 8 are the group's keys, columns query rows
+    float s[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[j][c] = 0.f;
+#pragma unroll
+    for (int i = 0; i < QC; ++i) {
+      const uint4 a4 = shared_16(at + R::place(g, t + 4 * i)), b4 = shared_16(at + R::place(g + 8, t + 4 * i));
+      const uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t x = a[w] ^ 0x80808080u, y = b[w] ^ 0x80808080u;
+        const uint32_t a0 = q8_pair_lo(x), a1 = q8_pair_lo(y), a2 = q8_pair_hi(x), a3 = q8_pair_hi(y);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint32_t b0, b1;
+          if (Q_SHARED) {
+            const uint2 f = *reinterpret_cast<const uint2*>(q_shared + (((4 * i + w) * NT + j) * 32 + lane) * 2);
+            b0 = f.x; b1 = f.y;
+          } else {
+            b0 = qf[Q_SHARED ? 0 : 4 * i + w][Q_SHARED ? 0 : j][0];
+            b1 = qf[Q_SHARED ? 0 : 4 * i + w][Q_SHARED ? 0 : j][1];
+          }
+          mma_f16(s[j], a0, a1, a2, a3, b0, b1);
+        }
+      }
+    }
+
+    // ------------------------------------------------ scores in log2 units with the values' scales, masks
+    const int key0 = keys.at(j0) * GROUP;
+    float ks[2], ve[2], vf[2], vi[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      ks[r] = shared_f(at + 2 * R::TENSOR + (g + 8 * r) * 4) * (OPT && p.cap > 0.f ? p.scale : p.scale_log2e);
+      q8_value_scale(shared_f(at + 2 * R::TENSOR + GROUP * 4 + (g + 8 * r) * 4), ve[r], vf[r], vi[r]);
+    }
+    const bool whole = key0 + GROUP - 1 <= least_pos && (p.window <= 0 || key0 >= most_lo || key0 + GROUP <= p.keep);
+    float z[NT][LC][2];
+    bool higher = false;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < LC; ++c)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float raw = PARTS == 2 ? s[j][2 * r] + s[j][2 * r + 1] : s[j][2 * r + c];
+          const float f = ks[r] * q_down[j][c];
+          float x;
+          if (OPT) {
+            x = raw * f;
+            if (p.cap > 0.f) x = q8_capped<PARTS == 2>(x, p.cap);
+            if (p.slopes) x -= p.slopes[col_head[j][c]] * CUCA_LOG2E * (float)(col_pos[j][c] - (key0 + g + 8 * r));
+            x += ve[r];
+          } else {
+            x = fmaf(raw, f, ve[r]);
+          }
+          if (!whole) {
+            const int kp = key0 + g + 8 * r;
+            if (!(kp <= col_pos[j][c] && (kp >= col_lo[j][c] || kp < p.keep))) x = -INFINITY;
+          }
+          z[j][c][r] = x;
+          higher |= x > m[j][c] + Q8_LAG;
+        }
+    if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float corr[LC];
+#pragma unroll
+        for (int c = 0; c < LC; ++c) {
+          float top = fmaxf(z[j][c][0], z[j][c][1]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const bool moves = top > m[j][c] + Q8_LAG;  // (each column by its own scores alone)
+          corr[c] = moves ? q8_exp2(m[j][c] - top) : 1.f;
+          if (moves) m[j][c] = top;
+          l[j][c] *= corr[c];
+        }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+          acc[i][j][0] *= corr[0]; acc[i][j][1] *= corr[LC - 1];
+          acc[i][j][2] *= corr[0]; acc[i][j][3] *= corr[LC - 1];
+        }
+      }
+    }
+
+    // ------------------------------------------------ weights, as the second operand of the values' product
+    uint32_t wb[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float w[LC];
+#pragma unroll
+        for (int c = 0; c < LC; ++c) {
+          w[c] = q8_exp2(z[j][c][r] - (m[j][c] == -INFINITY ? 0.f : m[j][c] - Q8_LIFT));
+          l[j][c] = fmaf(w[c], vi[r], l[j][c]);
+          w[c] *= vf[r];
+        }
+        uint32_t packed;
+        if (PARTS == 2) {
+          const float hi = __half2float(__float2half_rn(w[0]));
+          packed = q8_pack(hi, w[0] - hi);
+        } else {
+          packed = q8_pack(w[0], w[LC - 1]);
+        }
+        wb[j][r] = turned_8x8(packed);
+      }
+    // ------------------------------------------------ values: rows are dimensions, from keys 2t, 2t + 1, 2t + 8, 2t + 9
+    const uint32_t vat = at + R::TENSOR;
+    auto products = [&](int tile0, uint32_t ka, uint32_t kb, uint32_t kc, uint32_t kd) {  // four dimensions: two tiles
+      ka ^= 0x80808080u; kb ^= 0x80808080u; kc ^= 0x80808080u; kd ^= 0x80808080u;
+      const uint32_t ab0 = __byte_perm(ka, kb, 0x5140), ab1 = __byte_perm(ka, kb, 0x7362);
+      const uint32_t cd0 = __byte_perm(kc, kd, 0x5140), cd1 = __byte_perm(kc, kd, 0x7362);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        mma_f16(acc[tile0][j], q8_pair_lo(ab0), q8_pair_hi(ab0), q8_pair_lo(cd0), q8_pair_hi(cd0), wb[j][0], wb[j][1]);
+        mma_f16(acc[tile0 + 1][j], q8_pair_lo(ab1), q8_pair_hi(ab1), q8_pair_lo(cd1), q8_pair_hi(cd1), wb[j][0], wb[j][1]);
+      }
+    };
+    if (DP == 64) {
+      uint2 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = shared_8(vat + R::place(2 * t + (i & 1) + 8 * (i >> 1), g >> 1) + (g & 1) * 8);
+      products(0, x[0].x, x[1].x, x[2].x, x[3].x);
+      products(2, x[0].y, x[1].y, x[2].y, x[3].y);
+    } else {
+#pragma unroll
+      for (int h = 0; h < DP / 128; ++h) {
+        uint4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = shared_16(vat + R::place(2 * t + (i & 1) + 8 * (i >> 1), g + 8 * h));
+        products(8 * h, x[0].x, x[1].x, x[2].x, x[3].x);
+        products(8 * h + 2, x[0].y, x[1].y, x[2].y, x[3].y);
+        products(8 * h + 4, x[0].z, x[1].z, x[2].z, x[3].z);
+        products(8 * h + 6, x[0].w, x[1].w, x[2].w, x[3].w);
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- the warps' results joined, in their order
+  copies_wait<0>();
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int c = 0; c < LC; ++c) {
+      l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], 4);
+      l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], 8);
+      l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], 16);
+    }
+  __syncthreads();  // the rings are free
+  constexpr int OS = DP + 4;  // floats between columns
+  float* o_s = reinterpret_cast<float*>(smem);             // [WARPS][COLS][OS]
+  float* ml_s = o_s + WARPS * COLS * OS;                   // [WARPS][COLS][2]
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int c = 0; c < LC; ++c) {
+      const int col = 8 * j / PARTS + LC * t + c;
+      float* dst = o_s + (warp * COLS + col) * OS;
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        // dimensions of the thread: DP / 8 from piece (half a piece) g, eight tiles a piece
+        const int e = DP == 64 ? 8 * g + 2 * i : 128 * (i / 8) + 16 * g + 2 * (i % 8);
+        const float lo = PARTS == 2 ? acc[i][j][0] + acc[i][j][1] : acc[i][j][c];
+        const float hi = PARTS == 2 ? acc[i][j][2] + acc[i][j][3] : acc[i][j][2 + c];
+        *reinterpret_cast<float2*>(dst + e) = make_float2(lo, hi);
+      }
+      if (g == 0) {
+        ml_s[(warp * COLS + col) * 2] = m[j][c];
+        ml_s[(warp * COLS + col) * 2 + 1] = l[j][c];
+      }
+    }
+  __syncthreads();
+  const int per_col = p.d / 4;
+  for (int i = threadIdx.x; i < n_cols * per_col; i += WARPS * 32) {
+    const int col = i / per_col, e = (i % per_col) * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml_s[(w * COLS + col) * 2]);
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float mw = ml_s[(w * COLS + col) * 2];
+      const float f = mw == top ? 1.f : q8_exp2(mw - top);  // (a warp without keys has zeros)
+      const float4 v = *reinterpret_cast<const float4*>(o_s + (w * COLS + col) * OS + e);
+      o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
+      den += f * ml_s[(w * COLS + col) * 2 + 1];
+    }
+    const int head = head0 + col % heads;
+    if (alone) {
+      if (OPT && p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
+      const float inv = den == 0.f ? 0.f : 1.f / den;  // (a column that saw nothing has zeros)
+      T* dst = (T*)p.out + (size_t)(row0 + col / heads) * p.out_stride + (size_t)head * p.d + e;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) dst[k] = from_f32<T>(o[k] * inv);
+    } else {
+      float* dst = p.part + ((((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.n_splits + blockIdx.x) * COLS + col) * (p.d + 2);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) dst[e + k] = o[k];
+      if (e == 0) { dst[p.d] = top; dst[p.d + 1] = den; }
+    }
+  }
+}
+
+// Joins the shares of a tile's keys, in their order: a block per tile and key head, a warp per query row.
+template <typename T>
+__global__ void __launch_bounds__(WARPS * 32) join_q8_kernel(const Q8Params p, int cols) {
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int row0, n_tok;
+  if (!q8_rows_of_tile(p, blockIdx.z, row0, n_tok)) return;
+  const int kvh = blockIdx.y / p.head_parts, hp = blockIdx.y % p.head_parts;
+  const int group_heads = p.nh / p.nkv;
+  const int head0 = kvh * group_heads + hp * p.heads_per_cta;
+  const int heads = min(p.heads_per_cta, group_heads - hp * p.heads_per_cta);
+  const int pos0 = p.positions[row0];
+  if (p.seq_of_row[row0] < 0 || pos0 < 0) return;
+  const Q8Keys keys = q8_keys<GROUP>(p, pos0, n_tok);
+  const int share = p.chunk / GROUP, used = min(p.n_splits, (keys.groups + share - 1) / share);
+  if (used <= 1) return;  // written already
+  for (int col = warp; col < n_tok * heads; col += WARPS) {
+    const float* src = p.part + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.n_splits * cols + col) * (p.d + 2);
+    const size_t step = (size_t)cols * (p.d + 2);
+    float top = -INFINITY;
+    for (int s = 0; s < used; ++s) top = fmaxf(top, src[s * step + p.d]);
+    float o[8], den = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = 0.f;
+    for (int s = 0; s < used; ++s) {
+      const float* a = src + s * step;
+      const float ms = a[p.d], f = ms == top ? 1.f : q8_exp2(ms - top);
+      den += f * a[p.d + 1];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (lane + 32 * k < p.d) o[k] += f * a[lane + 32 * k];
+    }
+    const int head = head0 + col % heads;
+    if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    T* dst = (T*)p.out + (size_t)(row0 + col / heads) * p.out_stride + (size_t)head * p.d;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (lane + 32 * k < p.d) dst[lane + 32 * k] = from_f32<T>(o[k] * inv);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+template <int DP, int NT, int PARTS>
+constexpr int smem_bytes() {
+  const int ring = WARPS * Ring<DP>::WARP + (NT * DP > 256 ? (DP / 16) * NT * 32 * 8 : 0);
+  const int cols = NT * 8 / PARTS;
+  const int join = WARPS * cols * (DP + 4 + 2) * 4;
+  return ring > join ? ring : join;
+}
+
+template <int DP, int NT, int PARTS, bool OPT>
+int launch_q8(const Q8Params& p, int n_tiles, cudaStream_t stream) {
+  constexpr int smem = smem_bytes<DP, NT, PARTS>();
+  auto kernel = attention_q8_kernel<DP, NT, PARTS, OPT>;
+  static cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  CUCA_REQUIRE(configured == cudaSuccess, "attention_q8: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(configured));
+  cuca_launch(kernel, dim3(p.n_splits, p.nkv * p.head_parts, n_tiles), dim3(WARPS * 32), smem, stream, true, p);
+  CUCA_CHECK_LAUNCH("attention_q8");
+  if (p.n_splits > 1) {
+    auto join = join_q8_kernel<typename std::conditional<PARTS == 2, float, __nv_bfloat16>::type>;
+    cuca_launch(join, dim3(1, p.nkv * p.head_parts, n_tiles), dim3(WARPS * 32), 0, stream, true, p, NT * 8 / PARTS);
+    CUCA_CHECK_LAUNCH("attention_q8 (join)");
+  }
+  return 0;
+}
+template <int DP, int NT, int PARTS>
+int launch_q8_opt(const Q8Params& p, int n_tiles, cudaStream_t stream) {
+  return p.cap > 0.f || p.sink || p.slopes ? launch_q8<DP, NT, PARTS, true>(p, n_tiles, stream)
+                                           : launch_q8<DP, NT, PARTS, false>(p, n_tiles, stream);
+}
+template <int DP, int PARTS>
+int launch_q8_nt(const Q8Params& p, int nt, int n_tiles, cudaStream_t stream) {
+  if (nt == 1) return launch_q8_opt<DP, 1, PARTS>(p, n_tiles, stream);
+  if constexpr (DP <= 128) {
+    if (nt == 4) return launch_q8_opt<DP, 4, PARTS>(p, n_tiles, stream);
+  }
+  return launch_q8_opt<DP, 2, PARTS>(p, n_tiles, stream);
+}
+
+}  // namespace
+
+
+// Requests that bring count_lo .. count_hi rows (req_count null: every request one), tile_tokens rows of a request and
+// heads_per_cta query heads to a block of `nt` column tiles; keys in shares of `chunk`, n_splits of them at most (the last has
+// the rest). part: [n_tiles][nkv * pieces of a group][n_splits][8 nt / parts][d + 2] floats where n_splits > 1.
+CUCA_API int cuca_attention_q8(const void* q, int q_stride, void* out, int out_stride, int dtype, const void* kpool,
+                               const void* vpool, const float* kscale, const float* vscale, int n_blocks, int bs,
+                               const int* positions, const int* seq_of_row, const int* tables, int table_stride,
+                               const int* req_row0, const int* req_count, int n_seqs, int count_lo, int count_hi, int tile_tokens,
+                               int n_tiles, int nh, int nkv, int d, const CucaAttnOptions* opt, int heads_per_cta, int nt,
+                               int chunk, int n_splits, float* part, int* err, cudaStream_t stream) {
+  if (n_tiles == 0) return 0;
+  CUCA_REQUIRE(dtype == CUCA_F32 || dtype == CUCA_BF16, "attention_q8: unknown dtype %d", dtype);
+  CUCA_REQUIRE(opt != nullptr && opt->window >= 0 && opt->keep >= 0, "attention_q8: bad options");
+  CUCA_REQUIRE(opt->gate == nullptr && opt->key_scale == nullptr, "attention_q8: no output gate and no shared rows over 8-bit pages");
+  CUCA_REQUIRE(nkv > 0 && nh > 0 && nh % nkv == 0 && d >= 16 && d <= 256 && d % 16 == 0,
+               "attention_q8: unsupported shape (heads %d/%d, head size %d)", nh, nkv, d);
+  CUCA_REQUIRE(bs > 0 && n_blocks > 0 && table_stride > 0, "attention_q8: empty pages or tables");
+  CUCA_REQUIRE((((uintptr_t)kpool | (uintptr_t)vpool) & 15) == 0, "attention_q8: pools must be 16-byte aligned");
+  CUCA_REQUIRE(nt == 1 || nt == 2 || (nt == 4 && d <= 128), "attention_q8: %d column tiles", nt);
+  const int parts = dtype == CUCA_F32 ? 2 : 1, group = nh / nkv;
+  CUCA_REQUIRE(heads_per_cta > 0 && heads_per_cta <= group && tile_tokens > 0 && (long long)tile_tokens * heads_per_cta * parts <= 8 * nt,
+               "attention_q8: %d rows of %d heads do not fit %d columns", tile_tokens, heads_per_cta, 8 * nt / parts);
+  CUCA_REQUIRE(chunk >= 0 && chunk % 64 == 0 && n_splits >= 1 && (n_splits == 1 || (chunk > 0 && part)), "attention_q8: bad shares of the keys");
+  const int head_parts = (group + heads_per_cta - 1) / heads_per_cta;
+  CUCA_REQUIRE(n_tiles <= 65535 && (long long)nkv * head_parts <= 65535, "attention_q8: too many tiles or heads");
+  Q8Params p;
+  p.q = q; p.q_stride = q_stride; p.out = out; p.out_stride = out_stride;
+  p.kpool = (const int8_t*)kpool; p.vpool = (const int8_t*)vpool; p.kscale = kscale; p.vscale = vscale;
+  p.n_blocks = n_blocks; p.bs = bs; p.tables = tables; p.table_stride = table_stride; p.positions = positions;
+  p.seq_of_row = seq_of_row; p.req_row0 = req_row0; p.req_count = req_count; p.n_seqs = n_seqs; p.count_lo = count_lo;
+  p.count_hi = count_hi; p.tile_tokens = tile_tokens; p.nh = nh; p.nkv = nkv; p.d = d;
+  p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E; p.cap = opt->softcap; p.sink = opt->sink ? 1 : 0;
+  p.sink_val = opt->sink ? opt->sink_val : nullptr; p.window = opt->window; p.keep = opt->window > 0 ? opt->keep : 0;
+  p.slopes = opt->slopes; p.heads_per_cta = heads_per_cta; p.head_parts = head_parts; p.chunk = n_splits > 1 ? chunk : 0;
+  p.n_splits = n_splits; p.part = part; p.err = err;
+  if (parts == 2) {
+    if (d <= 64) return launch_q8_nt<64, 2>(p, nt, n_tiles, stream);
+    if (d <= 128) return launch_q8_nt<128, 2>(p, nt, n_tiles, stream);
+    return launch_q8_nt<256, 2>(p, nt, n_tiles, stream);
+  }
+  if (d <= 64) return launch_q8_nt<64, 1>(p, nt, n_tiles, stream);
+  if (d <= 128) return launch_q8_nt<128, 1>(p, nt, n_tiles, stream);
+  return launch_q8_nt<256, 1>(p, nt, n_tiles, stream);
+}

@@ -1,0 +1,164 @@
+// What the attention kernels over 8-bit pages share: their parameters, which rows a block takes, scores and codes.
+//
+// A cached row is d signed codes and a 32-bit scale (csrc/cache_q8.cu). Codes are whole numbers of at most 127, exact in
+// 16-bit floats, and a query times a power of two is too where it came in bfloat16 (in 32-bit mode it goes in two 16-bit
+// parts), so the raw score q . codes is as exact as a 32-bit sum of exact products. The scales never touch the codes:
+//
+//   s_j = raw_j ks_j (scale log2 e)                 the key's scale multiplies its score (log2 units)
+//   vs_j = f_j 2^e_j, 1 <= f_j < 2                  the value's scale goes into the weight: its exponent into the softmax's,
+//   z_j = s_j + e_j, u_j = 2^(z_j - max z + LIFT)   its fraction times the weight u_j f_j, which is bounded whatever the scales
+//   o   = sum_j (u_j f_j) vcode_j / sum_j u_j 2^-e_j  are, so it fits a 16-bit float
+//
+// The weights are rounded to 16-bit floats (11 bits; in 32-bit mode to two of them, 22 bits) because the tensor cores take
+// them so; every sum, the maximum and the denominator are in 32 bits.
+#pragma once
+#include "attention_options.cuh"
+#include "common.cuh"
+#include <cuda_fp16.h>
+#include <math.h>
+
+namespace {
+
+// Weights are less than 2^(LIFT + LAG + 1): the running maximum follows a larger one only when it is exceeded by more than LAG
+// (rescaling is rare then), and LIFT puts the weights' 29 binades of full precision below 2^15.
+constexpr float Q8_LIFT = 7.f, Q8_LAG = 7.f;
+
+struct Q8Params {
+  const void* q;
+  int q_stride;  // values between rows
+  void* out;
+  int out_stride;
+  const int8_t* kpool;
+  const int8_t* vpool;
+  const float* kscale;
+  const float* vscale;
+  int n_blocks, bs;
+  const int* tables;
+  int table_stride;
+  const int* positions;
+  const int* seq_of_row;
+  const int* req_row0;
+  const int* req_count;  // null: every request brings one row
+  int n_seqs;
+  int count_lo, count_hi;  // requests with so many rows are this launch's
+  int tile_tokens;         // rows of a request that a tile takes
+  int nh, nkv, d;
+  float scale_log2e;
+  float cap;       // > 0: a score s becomes cap tanh(s / cap) ...
+  float scale;     // ... of the score with this scale
+  int sink;        // the denominator holds one more term exp(0) ...
+  const float* sink_val;  // ... or exp(sink_val[head])
+  int window, keep;
+  const float* slopes;  // slopes[head] * distance is taken off a score
+  int heads_per_cta, head_parts;  // a key head's query heads in `head_parts` pieces
+  int chunk;       // keys of a block's share (a multiple of 64); 0: all of them
+  int n_splits;
+  float* part;     // [tiles][kv heads * head parts][splits][columns][d + 2] where a tile's keys are shared out
+  int* err;
+};
+
+// Which rows tile number `tile` of a launch takes: those of the requests that are the launch's, tile_tokens at a time, a
+// request's last ones (which see most keys) first. By every warp for itself.
+__device__ __forceinline__ bool q8_rows_of_tile(const Q8Params& p, int tile, int& row0, int& n) {
+  if (p.req_count == nullptr) {
+    row0 = p.req_row0[tile];
+    n = 1;
+    return true;
+  }
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+    const int s = s0 + lane;
+    const int count = s < p.n_seqs ? p.req_count[s] : 0;
+    const int tiles = count >= p.count_lo && count <= p.count_hi ? (count + p.tile_tokens - 1) / p.tile_tokens : 0;
+    int upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + upto > tile);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      const int its = __shfl_sync(0xffffffffu, tiles, at), its_count = __shfl_sync(0xffffffffu, count, at);
+      const int k = its - 1 - (tile - before - (__shfl_sync(0xffffffffu, upto, at) - its));
+      row0 = p.req_row0[s0 + at] + k * p.tile_tokens;
+      n = min(p.tile_tokens, its_count - k * p.tile_tokens);
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
+}
+
+// The keys that some of the rows at positions pos0 .. pos0 + n - 1 see, in groups of U positions counted without the gap
+// between the first `keep` and the window: `kept` groups from 0, then those from number `low` on.
+struct Q8Keys {
+  int kept, low, groups, hi;  // (hi: one past the last position)
+  __device__ __forceinline__ int at(int j) const { return j < kept ? j : low + j - kept; }
+};
+template <int U>
+__device__ __forceinline__ Q8Keys q8_keys(const Q8Params& p, int pos0, int n) {
+  Q8Keys k;
+  k.hi = pos0 + n;
+  const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
+  k.low = lo / U;
+  k.kept = min((p.keep + U - 1) / U, k.low);
+  k.groups = k.kept + (k.hi - 1) / U - k.low + 1;
+  return k;
+}
+
+// Four codes as two pairs of 16-bit floats: x + 128 in the low bits of 1024 (ulp 1), less 1152.
+__device__ __forceinline__ uint32_t q8_minus(uint32_t a) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x64806480u));
+  return r;
+}
+__device__ __forceinline__ uint32_t q8_pair_lo(uint32_t biased) { return q8_minus(__byte_perm(biased, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t q8_pair_hi(uint32_t biased) { return q8_minus(__byte_perm(biased, 0x64646464u, 0x4342)); }
+
+__device__ __forceinline__ float q8_exp2(float x) {  // 2^x; 0 at -infinity
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t q8_pack(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// A value scale as f 2^e (e as a float), and 2^-e for the denominator. e is -60 at least, so that u 2^-e does not leave 32 bits
+// where scales are far apart; f is smaller than 1 then, 0 for a row of zeros. A scale that is not finite (2^123 and more, which
+// no row has, count as that) makes e, so the weight, NaN where the key is seen; the factors are numbers, so that a masked key's
+// weight of zero stays zero.
+__device__ __forceinline__ void q8_value_scale(float vs, float& e, float& f, float& inv) {
+  const uint32_t bits = (__float_as_uint(vs) >> 23) & 255u, x = max(bits, 67u);
+  const bool fine = bits < 250u;
+  e = fine ? (float)((int)x - 127) : __uint_as_float(0x7fc00000u);
+  inv = fine ? __uint_as_float((254u - x) << 23) : 1.f;
+  f = fine ? vs * inv : 1.f;
+}
+// The power of two that puts magnitudes up to the one with these bits below 2^14, and its inverse (NaN where the row is not
+// finite: its scores are NaN then, as they should be).
+__device__ __forceinline__ void q8_query_scale(uint32_t top, float& up, float& down) {
+  if (top >= 0x7f800000u) {
+    up = 0.f;
+    down = __uint_as_float(0x7fc00000u);
+    return;
+  }
+  const uint32_t e = max(top >> 23, 14u);
+  up = __uint_as_float((267u - e) << 23);
+  down = __uint_as_float((e - 13u) << 23);
+}
+// cap tanh(s / cap) in log2 units. EXACT: for the 32-bit mode; else 1 - 2 / (e^2y + 1), right at both ends.
+template <bool EXACT>
+__device__ __forceinline__ float q8_capped(float s, float cap) {
+  if (EXACT) return cap * CUCA_LOG2E * tanhf(s / cap);
+  const float e = q8_exp2(s * (2.f * CUCA_LOG2E) / cap);
+  return cap * CUCA_LOG2E * (1.f - __fdividef(2.f, e + 1.f));
+}
+// What a sink adds to a denominator that is relative to the reference m.
+__device__ __forceinline__ float q8_sink_term(const Q8Params& p, int head, float m) {
+  return q8_exp2((p.sink_val ? p.sink_val[head] * CUCA_LOG2E : 0.f) - m + Q8_LIFT);
+}
+
+}  // namespace

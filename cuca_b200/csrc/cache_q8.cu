@@ -1,0 +1,302 @@
+// The key/value cache in 8 bits: quantising rows as they are written, and reading them back.
+//
+// A row (the d keys or values of one position and key head) is d signed 8-bit codes and a 32-bit scale. With a = max |x|,
+//
+//   scale = a / 127,   code = round(x * (127 / a)) to the nearest, ties to even,   and the row stands for code * scale.
+//
+// A row with a < 2^-100 is kept as zeros (scale 0). A row that is not finite gets the scale NaN and codes 0, so it reads back
+// as NaN whole and never as something plausible; codes are finite whatever happens, so a masked row can be multiplied by zero.
+// The rotation, the quotients and the products are rounded one by one in 32 bits (no fused multiply-adds), so the codes do not
+// depend on the form that made them. Rounding to 8 bits here is the cache's own choice: against bfloat16 pages it halves the
+// bytes a decode step reads; the error of a value is at most half a 127th of its row's largest.
+//
+// Both kernels do a few operations per byte and are bound by memory, or by latency when there are few rows.
+#include "common.cuh"
+
+namespace {
+
+constexpr float CUCA_Q8_TINY = 7.888609052210118e-31f;  // 2^-100
+constexpr int STORE_THREADS = 256;
+
+struct StoreParams {
+  const void* qkv;
+  int row_stride;  // values between rows; q heads, k heads, v heads from a row's start
+  void* q_out;
+  int q_stride;
+  const int* positions;
+  const int* seq_of_row;
+  const int* tables;
+  int table_stride;
+  const float* cos_t;
+  const float* sin_t;
+  int table_rows, rot, adjacent;
+  int8_t* kpool;
+  int8_t* vpool;
+  float* kscale;
+  float* vscale;
+  int n_blocks, bs, n_rows, nh, nkv, d;
+  int seg;  // lanes of a head: d / 8, rounded up to a power of two
+  int* err;
+};
+
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const float4 x = *reinterpret_cast<const float4*>(p);
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&v)[4]) {
+  const uint2 x = *reinterpret_cast<const uint2*>(p);
+  v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
+  v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
+  __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+}
+
+__device__ __forceinline__ uint32_t codes4(const float (&v)[4], float inv) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = max(-127, min(127, __float2int_rn(__fmul_rn(v[i], inv))));
+    w |= (uint32_t)(c & 0xff) << (8 * i);
+  }
+  return w;
+}
+
+// A group of `seg` lanes takes one head of one row; a lane has values 4 l .. 4 l + 3 of each half of the head, which are the
+// rotation's pairs where the whole head is rotated in halves (VEC: 8- or 16-byte accesses). Else (part of the head rotated,
+// neighbours as pairs, rows that are not aligned) the same values are fetched one by one with their partners. A head stays
+// within a warp, and everything is read before anything is written: q_out may be the rows themselves.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(STORE_THREADS) rope_store_q8_kernel(const StoreParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int heads = p.nh + 2 * p.nkv;
+  const long long unit = ((long long)blockIdx.x * STORE_THREADS + threadIdx.x) / p.seg;
+  const int l = threadIdx.x & (p.seg - 1);
+  const int row = (int)(unit / heads), head = (int)(unit % heads);
+  const int half = p.d / 2;
+  const bool lane_ok = row < p.n_rows && 4 * l < half;
+  const int seq = row < p.n_rows ? p.seq_of_row[row] : -1;
+  const int pos = seq >= 0 ? p.positions[row] : 0;
+  const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+  const bool rotate = !is_v && p.rot > 0;
+  const bool in_table = pos >= 0 && pos < p.table_rows;
+  const bool live = lane_ok && seq >= 0;
+  float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    if (rotate && !in_table && l == 0 && p.err) atomicExch(p.err, CUCA_ERR_TOKEN_RANGE);
+    const T* src = (const T*)p.qkv + (size_t)row * p.row_stride + (size_t)head * p.d;
+    const float* cr = p.cos_t + (size_t)(in_table ? pos : 0) * (p.rot / 2);
+    const float* sr = p.sin_t + (size_t)(in_table ? pos : 0) * (p.rot / 2);
+    if (VEC) {
+      load4(src + 4 * l, a);
+      load4(src + half + 4 * l, b);
+      if (rotate && in_table) {
+        float c[4], s[4];
+        load4(cr + 4 * l, c);
+        load4(sr + 4 * l, s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = a[i], y = b[i];
+          a[i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
+          b[i] = __fadd_rn(__fmul_rn(x, s[i]), __fmul_rn(y, c[i]));
+        }
+      }
+    } else {
+      auto value = [&](int e) {
+        const float x = to_f32(src[e]);
+        if (!rotate || !in_table || e >= p.rot) return x;
+        const int hr = p.rot / 2;
+        const int i = p.adjacent ? e / 2 : (e < hr ? e : e - hr);
+        const bool first = p.adjacent ? (e & 1) == 0 : e < hr;
+        const float c = cr[i], s = sr[i];
+        const float y = to_f32(src[p.adjacent ? e ^ 1 : (first ? e + hr : i)]);
+        return first ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)) : __fadd_rn(__fmul_rn(y, s), __fmul_rn(x, c));
+      };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { a[i] = value(4 * l + i); b[i] = value(half + 4 * l + i); }
+    }
+  }
+  // the largest magnitude of the head, as bits: anything not finite compares above every number
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    top = max(top, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
+  for (int o = p.seg >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));  // (also: all has been read)
+  if (!live) return;
+  if (is_q) {
+    T* dst = (T*)p.q_out + (size_t)row * p.q_stride + (size_t)head * p.d;
+    if (VEC) {
+      store4(dst + 4 * l, a);
+      store4(dst + half + 4 * l, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { dst[4 * l + i] = from_f32<T>(a[i]); dst[half + 4 * l + i] = from_f32<T>(b[i]); }
+    }
+    return;
+  }
+  const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
+  const int entry = pos / p.bs;
+  const int blk = pos >= 0 && entry < p.table_stride ? p.tables[(size_t)seq * p.table_stride + entry] : -1;
+  if (blk < 0 || blk >= p.n_blocks) {
+    if (l == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+    return;
+  }
+  const size_t at = ((size_t)blk * p.nkv + kvh) * p.bs + pos % p.bs;
+  const float most = __uint_as_float(top);
+  float scale, inv;
+  if (top >= 0x7f800000u) {
+    scale = __uint_as_float(0x7fc00000u);
+    inv = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = b[i] = 0.f;
+  } else if (most < CUCA_Q8_TINY) {
+    scale = inv = 0.f;
+  } else {
+    scale = __fdiv_rn(most, 127.f);
+    inv = __fdiv_rn(127.f, most);
+  }
+  int8_t* dst = (is_v ? p.vpool : p.kpool) + at * p.d;
+  *reinterpret_cast<uint32_t*>(dst + 4 * l) = codes4(a, inv);
+  *reinterpret_cast<uint32_t*>(dst + half + 4 * l) = codes4(b, inv);
+  if (l == 0) (is_v ? p.vscale : p.kscale)[at] = scale;
+}
+
+// ------------------------------------------------------------------ reading back
+constexpr int READ_THREADS = 256, READ_UNROLL = 4;
+
+template <typename T> struct Piece;  // what a thread writes at once: 16 bytes
+template <> struct Piece<float> { static constexpr int N = 4; };
+template <> struct Piece<__nv_bfloat16> { static constexpr int N = 8; };
+
+struct ReadParams {
+  const int8_t* pool[2];
+  const float* scale[2];
+  void* out[2];
+  int out_stride[2];
+  const int* positions;
+  const int* seq_of_row;
+  const int* tables;
+  int table_stride, n_blocks, bs, n_rows, nkv, d, rows_per_block;
+  int* err;
+};
+
+// A block takes `rows_per_block` rows of one tensor; a thread writes 16 bytes at a time, four of them requested together.
+template <typename T>
+__global__ void __launch_bounds__(READ_THREADS) read_q8_kernel(const ReadParams p) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int N = Piece<T>::N;
+  const int which = blockIdx.y;
+  T* out = (T*)p.out[which];
+  if (!out) return;
+  const int8_t* pool = p.pool[which];
+  const float* scales = p.scale[which];
+  const int row0 = blockIdx.x * p.rows_per_block;
+  const unsigned per_head = p.d / N, per_row = per_head * p.nkv;
+  const unsigned total = per_row * (unsigned)min(p.rows_per_block, p.n_rows - row0);
+  for (unsigned first = threadIdx.x; first < total; first += READ_THREADS * READ_UNROLL) {
+    uint2 w[READ_UNROLL];
+    float s[READ_UNROLL];
+    T* dst[READ_UNROLL];
+#pragma unroll
+    for (int u = 0; u < READ_UNROLL; ++u) {
+      const unsigned idx = first + u * READ_THREADS;
+      dst[u] = nullptr;
+      if (idx >= total) continue;
+      const int row = row0 + (int)(idx / per_row);
+      const unsigned rest = idx % per_row;
+      const int kvh = (int)(rest / per_head), e = (int)(rest % per_head) * N;
+      dst[u] = out + (size_t)row * p.out_stride[which] + (size_t)kvh * p.d + e;
+      w[u] = make_uint2(0u, 0u);
+      s[u] = 0.f;
+      const int seq = p.seq_of_row[row];
+      if (seq < 0) continue;  // a row of no request: zeros
+      const int pos = p.positions[row], entry = pos / p.bs;
+      const int blk = pos >= 0 && entry < p.table_stride ? p.tables[(size_t)seq * p.table_stride + entry] : -1;
+      if (blk < 0 || blk >= p.n_blocks) {
+        if (p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+        continue;
+      }
+      const size_t at = ((size_t)blk * p.nkv + kvh) * p.bs + pos % p.bs;
+      s[u] = scales[at];
+      if (N == 8) w[u] = *reinterpret_cast<const uint2*>(pool + at * p.d + e);
+      else w[u].x = *reinterpret_cast<const uint32_t*>(pool + at * p.d + e);
+    }
+#pragma unroll
+    for (int u = 0; u < READ_UNROLL; ++u) {
+      if (!dst[u]) continue;
+      float v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = (float)(int8_t)((i < 4 ? w[u].x : w[u].y) >> (8 * (i & 3))) * s[u];
+      if constexpr (N == 4) {
+        *reinterpret_cast<float4*>(dst[u]) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          o[i] = *reinterpret_cast<uint32_t*>(&t);
+        }
+        *reinterpret_cast<uint4*>(dst[u]) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+// Rotates q (into q_out, which may be the rows themselves) and k, quantises k and v and writes them to their pages.
+// `adjacent`: neighbouring values are the rotation's pairs instead of the halves of the first `rot`.
+CUCA_API int cuca_rope_store_q8(const void* qkv, int row_stride, void* q_out, int q_stride, int dtype, const int* positions,
+                                const int* seq_of_row, const int* tables, int table_stride, const float* cos_t,
+                                const float* sin_t, int table_rows, int rot, int adjacent, void* kpool, void* vpool,
+                                float* kscale, float* vscale, int n_blocks, int bs, int n_rows, int nh, int nkv, int d,
+                                int* err, cudaStream_t stream) {
+  CUCA_REQUIRE(dtype == CUCA_F32 || dtype == CUCA_BF16, "rope_store_q8: unknown dtype %d", dtype);
+  CUCA_REQUIRE(nh > 0 && nkv > 0 && bs > 0 && n_blocks > 0 && table_stride > 0, "rope_store_q8: empty heads, pages or tables");
+  CUCA_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "rope_store_q8: head size %d is not a multiple of 16 up to 256", d);
+  CUCA_REQUIRE(rot >= 0 && rot <= d && rot % 2 == 0 && (rot == 0 || (cos_t && sin_t)), "rope_store_q8: %d rotated values of %d", rot, d);
+  CUCA_REQUIRE(((uintptr_t)kpool & 3) == 0 && ((uintptr_t)vpool & 3) == 0, "rope_store_q8: pools must be 4-byte aligned");
+  if (n_rows == 0) return 0;
+  StoreParams p{qkv, row_stride, q_out, q_stride, positions, seq_of_row, tables, table_stride, cos_t, sin_t, table_rows, rot,
+                adjacent, (int8_t*)kpool, (int8_t*)vpool, kscale, vscale, n_blocks, bs, n_rows, nh, nkv, d, 1, err};
+  while (p.seg * 8 < d) p.seg *= 2;
+  const long long threads = (long long)n_rows * (nh + 2 * nkv) * p.seg;
+  const long long blocks = (threads + STORE_THREADS - 1) / STORE_THREADS;
+  CUCA_REQUIRE(blocks < (1ll << 31), "rope_store_q8: too many rows");
+  const uintptr_t align = dtype == CUCA_F32 ? 15 : 7;
+  const bool vec = (rot == d || rot == 0) && !adjacent && d % 8 == 0 && row_stride % 4 == 0 && q_stride % 4 == 0 &&
+                   (((uintptr_t)qkv | (uintptr_t)q_out) & align) == 0 && (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15) == 0;
+  auto kernel = dtype == CUCA_F32 ? (vec ? rope_store_q8_kernel<float, true> : rope_store_q8_kernel<float, false>)
+                                  : (vec ? rope_store_q8_kernel<__nv_bfloat16, true> : rope_store_q8_kernel<__nv_bfloat16, false>);
+  cuca_launch(kernel, dim3((unsigned)blocks), dim3(STORE_THREADS), 0, stream, true, p);
+  CUCA_CHECK_LAUNCH("rope_store_q8");
+  return 0;
+}
+
+// Rows of k_out / v_out (either may be null): the values that the codes of (seq_of_row, positions) stand for; zeros for a row
+// of no request (seq < 0).
+CUCA_API int cuca_read_q8(const void* kpool, const void* vpool, const float* kscale, const float* vscale, int n_blocks, int bs,
+                          const int* positions, const int* seq_of_row, const int* tables, int table_stride, void* k_out,
+                          int k_stride, void* v_out, int v_stride, int dtype, int n_rows, int nkv, int d, int* err,
+                          cudaStream_t stream) {
+  CUCA_REQUIRE(dtype == CUCA_F32 || dtype == CUCA_BF16, "read_q8: unknown dtype %d", dtype);
+  CUCA_REQUIRE(nkv > 0 && bs > 0 && n_blocks > 0 && table_stride > 0, "read_q8: empty heads, pages or tables");
+  CUCA_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "read_q8: head size %d is not a multiple of 16 up to 256", d);
+  const int n = dtype == CUCA_F32 ? 4 : 8;
+  CUCA_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0 && (!k_out || k_stride % n == 0) && (!v_out || v_stride % n == 0) &&
+               (((uintptr_t)kpool | (uintptr_t)vpool) & 7) == 0, "read_q8: rows must start on 16 bytes, pools on 8");
+  if (n_rows == 0 || (!k_out && !v_out)) return 0;
+  ReadParams p{{(const int8_t*)kpool, (const int8_t*)vpool}, {kscale, vscale}, {k_out, v_out}, {k_stride, v_stride}, positions,
+               seq_of_row, tables, table_stride, n_blocks, bs, n_rows, nkv, d, 1, err};
+  const int pieces = nkv * d / n;  // of a row
+  p.rows_per_block = READ_THREADS * READ_UNROLL / pieces > 1 ? READ_THREADS * READ_UNROLL / pieces : 1;
+  const int blocks = (n_rows + p.rows_per_block - 1) / p.rows_per_block;
+  auto kernel = dtype == CUCA_F32 ? read_q8_kernel<float> : read_q8_kernel<__nv_bfloat16>;
+  cuca_launch(kernel, dim3(blocks, 2), dim3(READ_THREADS), 0, stream, true, p);
+  CUCA_CHECK_LAUNCH("read_q8");
+  return 0;
+}

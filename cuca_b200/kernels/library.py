@@ -190,6 +190,11 @@ _SIGNATURES = {
     "cuca_sum_norm_shift": [_P, _P, _P, _P, _F, _F, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P],
     "cuca_shift_rows": [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P],
     "cuca_moe_glu_capped_dense": [_P, _P, _I, _P, _I, _I, _I, _I, _I, _F, _F, _F, _P],
+    "cuca_rope_store_q8": [_P, _I, _P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P,
+                           _P],
+    "cuca_read_q8": [_P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P],
+    "cuca_attention_q8": [_P, _I, _P, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P,
+                          _I, _I, _I, _I, _P, _P, _P],
 }
 
 _lock = threading.Lock()

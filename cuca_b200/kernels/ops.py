@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from dataclasses import dataclass
 
 import torch
 
@@ -1537,3 +1538,211 @@ def shift_rows(x, mix, kept, out, step) -> None:
     library.check(library.load().cuca_shift_rows(_p(x), _p(mix), _p(kept), _p(out), dtype_code(out.dtype),
                                                  _p(step.seq_of_row), _p(step.req_row0), _p(step.req_count), _p(step.slots),
                                                  x.shape[0], step.n_seqs, x.shape[1], _stream()), "shift_rows")
+
+
+# ------------------------------------------------------------------ the cache in 8 bits
+@dataclass
+class QuantizedPages:
+    """Keys and values in 8 bits: a row (one position and key head) is `head_dim` signed codes and a 32-bit scale, and stands
+    for codes * scale (`csrc/cache_q8.cu`). Zeroed pages stand for zeros."""
+
+    k: torch.Tensor  # int8 [pages, kv heads, positions of a page, head_dim]
+    v: torch.Tensor
+    k_scale: torch.Tensor  # float32 [pages, kv heads, positions of a page]
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, n_pages: int, n_kv_heads: int, block_size: int, head_dim: int, device) -> "QuantizedPages":
+        """Pages that hold zeros."""
+        shape = (n_pages, n_kv_heads, block_size, head_dim)
+        return cls(*(torch.zeros(shape, dtype=torch.int8, device=device) for _ in range(2)),
+                   *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+
+    def check(self, n_kv_heads: int, head_dim: int) -> None:
+        shape = self.k.shape
+        if len(shape) != 4 or shape[1] != n_kv_heads or shape[3] != head_dim or self.v.shape != shape \
+                or self.k_scale.shape != shape[:3] or self.v_scale.shape != shape[:3]:
+            raise library.KernelError(f"8-bit pages of {n_kv_heads} heads of {head_dim}: codes are [pages, heads, positions, head "
+                                      f"size], scales the same without the last; given {tuple(shape)}, {tuple(self.v.shape)}, "
+                                      f"{tuple(self.k_scale.shape)}, {tuple(self.v_scale.shape)}")
+        for t, dtype in ((self.k, torch.int8), (self.v, torch.int8), (self.k_scale, torch.float32), (self.v_scale, torch.float32)):
+            if t.dtype != dtype or not t.is_contiguous():
+                raise library.KernelError("8-bit pages are contiguous int8 codes and contiguous float32 scales")
+        _cuda(self.k, self.v, self.k_scale, self.v_scale)
+
+
+Q8_MAX_HEAD_DIM = 256
+
+
+def q8_supported(head_dim: int) -> bool:
+    """Whether rows of this size can be kept in 8-bit pages."""
+    return 16 <= head_dim <= Q8_MAX_HEAD_DIM and head_dim % 16 == 0
+
+
+def _q8_head_dim(head_dim: int) -> None:
+    if not q8_supported(head_dim):
+        raise library.KernelError(f"8-bit pages take head sizes that are multiples of 16 up to {Q8_MAX_HEAD_DIM}, not {head_dim}")
+
+
+def _ints(n, *tensors) -> None:
+    """32-bit whole numbers on the device, `n` of them at least (None: of any number), without gaps."""
+    for t in tensors:
+        _cuda(t)
+        if t.dtype != torch.int32 or not t.is_contiguous() or (n is not None and t.numel() < n):
+            raise library.KernelError("positions, slots and page tables are contiguous int32 tensors, one number per row")
+
+
+def _rows(t, n_rows: int, width: int, what: str) -> None:
+    if t.dim() != 2 or t.shape[0] != n_rows or t.shape[1] < width or (t.stride(1) != 1 and width > 1):
+        raise library.KernelError(f"{what} are [{n_rows}, {width} or more] with contiguous rows, not {tuple(t.shape)}")
+
+
+def rope_store_q8(qkv, q_out, positions, seq_of_row, tables, cos, sin, rotary_dim, pages: QuantizedPages, n_heads, n_kv_heads,
+                  head_dim, err, adjacent: bool = False) -> None:
+    """Rows q | k | v: q, rotated, into `q_out` (which may be the rows themselves), k, rotated, and v quantised into their
+    pages. The first `rotary_dim` values of a head are rotated (cos None: none), in halves or as neighbouring pairs. A row that is
+    not finite reads back as NaN. Rows with seq_of_row < 0 are left out."""
+    _cuda(qkv, q_out, cos, sin)
+    code, n = dtype_code(qkv.dtype), qkv.shape[0]
+    _q8_head_dim(head_dim)
+    pages.check(n_kv_heads, head_dim)
+    _rows(qkv, n, (n_heads + 2 * n_kv_heads) * head_dim, "projected rows")
+    _rows(q_out, n, n_heads * head_dim, "rotated queries")
+    if q_out.dtype != qkv.dtype:
+        raise library.KernelError(f"rotated queries have the rows' dtype {qkv.dtype}, not {q_out.dtype}")
+    _ints(n, positions, seq_of_row)
+    _ints(None, tables)
+    rot = int(rotary_dim) if cos is not None else 0
+    if cos is not None:
+        for x in (cos, sin):
+            if x is None or x.dtype != torch.float32 or not x.is_contiguous() or x.shape != cos.shape or x.shape[1] * 2 != rot:
+                raise library.KernelError(f"cosines and sines are contiguous float32 [positions, {rot // 2}]")
+    library.check(library.load().cuca_rope_store_q8(
+        _p(qkv), qkv.stride(0), _p(q_out), q_out.stride(0), code, _p(positions), _p(seq_of_row), _p(tables), tables.shape[1],
+        _p(cos), _p(sin), cos.shape[0] if cos is not None else 0, rot, int(bool(adjacent)), _p(pages.k), _p(pages.v),
+        _p(pages.k_scale), _p(pages.v_scale), pages.k.shape[0], pages.k.shape[2], n, n_heads, n_kv_heads, head_dim, _p(err),
+        _stream()), "rope_store_q8")
+
+
+def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, err) -> None:
+    """k_out[r], v_out[r] ([rows, kv heads, head_dim] in bfloat16 or float32; either may be None) = what the pages hold for
+    position positions[r] of the request with page table seq_of_row[r]; zeros where seq_of_row < 0."""
+    nkv, d, n = pages.k.shape[1], pages.k.shape[3], positions.shape[0]
+    _q8_head_dim(d)
+    pages.check(nkv, d)
+    outs = [t for t in (k_out, v_out) if t is not None]
+    if not outs:
+        return
+    _cuda(*outs)
+    for t in outs:
+        if t.shape != (n, nkv, d) or t.dtype != outs[0].dtype or t.stride(2) != 1 or t.stride(1) != d:
+            raise library.KernelError(f"rows read back are [{n}, {nkv}, {d}], contiguous but for the rows' stride and of one dtype")
+    _ints(n, positions, seq_of_row)
+    _ints(None, tables)
+    library.check(library.load().cuca_read_q8(
+        _p(pages.k), _p(pages.v), _p(pages.k_scale), _p(pages.v_scale), pages.k.shape[0], pages.k.shape[2], _p(positions),
+        _p(seq_of_row), _p(tables), tables.shape[1], _p(k_out), 0 if k_out is None else k_out.stride(0), _p(v_out),
+        0 if v_out is None else v_out.stride(0), dtype_code(outs[0].dtype), n, nkv, d, _p(err), _stream()), "read_q8")
+
+
+class QuantizedPlan:
+    """How a step's requests are handed to the attention over 8-bit pages: counts and lengths from the step's per-request lists
+    on the host; which rows a block takes is worked out on the device. One plan serves every layer of a step."""
+
+    def __init__(self, step):
+        self.static = step.static_max_len is not None
+        if self.static:
+            self.counts, self.lengths = [1] * step.n_rows, [int(step.static_max_len)] * step.n_rows
+        else:
+            self.counts = [int(c) for c in step.host["counts"]]
+            self.lengths = [int(s) + c for s, c in zip(step.host["starts"], self.counts)]
+        self.all_single = all(c == 1 for c in self.counts)
+        self.longest = max(self.counts, default=0)
+        self._launches: dict = {}
+
+    def launches(self, n_heads, n_kv_heads, head_dim, dtype, window, keep):
+        """[(least count, most count, rows of a tile, tiles, heads of a block, column tiles, keys of a share, shares)]"""
+        key = (n_heads, n_kv_heads, head_dim, dtype, window, keep)
+        if key not in self._launches:
+            out = []
+            if 1 in self.counts:
+                out.append(self._few(1, 1, *key))
+            if self.longest > 1:
+                out.append(self._few(2, self.longest, *key))
+            self._launches[key] = out
+        return self._launches[key]
+
+    def _few(self, lo, hi, n_heads, n_kv_heads, head_dim, dtype, window, keep):
+        parts, group = (2 if dtype == torch.float32 else 1), n_heads // n_kv_heads
+        most = 2 if head_dim > 128 else 4
+        nt = next((n for n in (1, 2) if min(hi, 8) * group * parts <= 8 * n), most)
+        cap = 8 * nt // parts
+        heads = min(group, cap)
+        tokens = cap // heads if heads == group else 1
+        pieces = n_kv_heads * -(-group // heads)
+        tiles = keys = longest = 0
+        for c, length in zip(self.counts, self.lengths):
+            if lo <= c <= hi:
+                n = -(-c // tokens)
+                seen = length if window is None else min(length, window + min(c, tokens) - 1 + keep)
+                tiles += n
+                keys += n * seen
+                longest = max(longest, seen)
+        share, shares = _q8_shares(tiles * pieces, keys * pieces, longest, head_dim, nt)
+        return lo, hi, tokens, tiles, heads, nt, share, shares
+
+
+def _q8_shares(blocks: int, keys: int, longest: int, head_dim: int, nt: int, sms: int | None = None):
+    """(keys of a block's share, shares of the longest tile): enough blocks to fill the GPU, none with less than 128 keys."""
+    if sms is None:
+        sms = sm_count()
+    resident = sms * max(1, 3 * 128 // (max(64, head_dim) * nt))
+    share = max(128, -(-keys // max(1, resident) // 64) * 64)
+    share = max(share, -(-longest // 64 // 64) * 64)  # at most 64 shares
+    if blocks == 0 or share >= longest:
+        return 0, 1
+    return share, -(-(longest + 16) // share)
+
+
+def attention_q8_plan(step) -> QuantizedPlan:
+    plan = step.plans.get("paged_attention_q8")
+    if plan is None:
+        plan = step.plans["paged_attention_q8"] = QuantizedPlan(step)
+    return plan
+
+
+def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_heads, head_dim, scale, window, err, softcap=0.0,
+                 sink=False, sink_values=None, keep_first=0, slopes=None) -> None:
+    """Paged causal attention of every row of the step over 8-bit pages: q stands at the head of each row of `q`, `out` is
+    [rows, heads * head_dim] in q's dtype (bfloat16 or float32). `step` describes the rows (`StepBatch`: positions, seq_of_row,
+    req_row0, req_count, counts and starts on the host). Rows of no request (seq_of_row < 0) get zeros. The other options: see
+    `attention_options`."""
+    _cuda(q, out, tables)
+    code, n = dtype_code(q.dtype), step.n_rows
+    _q8_head_dim(head_dim)
+    if n_kv_heads < 1 or n_heads % n_kv_heads:
+        raise library.KernelError(f"{n_kv_heads} key heads must divide {n_heads} query heads")
+    pages.check(n_kv_heads, head_dim)
+    _rows(q, n, n_heads * head_dim, "queries")
+    _rows(out, n, n_heads * head_dim, "results")
+    if out.dtype != q.dtype:
+        raise library.KernelError(f"results have the queries' dtype {q.dtype}, not {out.dtype}")
+    _ints(n, step.positions, step.seq_of_row)
+    _ints(step.n_seqs, step.req_row0)
+    _ints(None, tables)
+    if window is not None and window < 0 or keep_first < 0 or softcap < 0:
+        raise library.KernelError("a window, kept first keys and a score cap are not negative")
+    plan = attention_q8_plan(step)
+    opt = attention_options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
+    lib = library.load()
+    for lo, hi, tokens, tiles, heads, nt, share, shares in plan.launches(n_heads, n_kv_heads, head_dim, q.dtype, window or None, opt.keep):
+        part = None
+        if shares > 1:
+            cols = 8 * nt // (2 if code == F32 else 1)
+            part = torch.empty(tiles * n_kv_heads * -(-(n_heads // n_kv_heads) // heads) * shares * cols * (head_dim + 2),
+                               dtype=torch.float32, device=q.device)
+        library.check(lib.cuca_attention_q8(
+            _p(q), q.stride(0), _p(out), out.stride(0), code, _p(pages.k), _p(pages.v), _p(pages.k_scale), _p(pages.v_scale),
+            pages.k.shape[0], pages.k.shape[2], _p(step.positions), _p(step.seq_of_row), _p(tables), tables.shape[1],
+            _p(step.req_row0), None if plan.all_single else _p(step.req_count), step.n_seqs, lo, hi, tokens, tiles, n_heads,
+            n_kv_heads, head_dim, ctypes.addressof(opt), heads, nt, share, shares, _p(part), _p(err), _stream()), "attention_q8")
