@@ -312,7 +312,7 @@ attention_q8_kernel(const Q8Params p) {
           float x;
           if (OPT) {
             x = raw * f;
-            if (p.cap > 0.f) x = q8_capped<PARTS == 2>(x, p.cap);
+            if (p.cap > 0.f) x = q8_capped<PARTS == 2>(x, p);
             if (p.slopes) x -= p.slopes[col_head[j][c]] * CUCA_LOG2E * (float)(col_pos[j][c] - (key0 + g + 8 * r));
             x += ve[r];
           } else {
@@ -581,7 +581,7 @@ CUCA_API int cuca_attention_q8(const void* q, int q_stride, void* out, int out_s
   p.n_blocks = n_blocks; p.bs = bs; p.tables = tables; p.table_stride = table_stride; p.positions = positions;
   p.seq_of_row = seq_of_row; p.req_row0 = req_row0; p.req_count = req_count; p.n_seqs = n_seqs; p.count_lo = count_lo;
   p.count_hi = count_hi; p.tile_tokens = tile_tokens; p.nh = nh; p.nkv = nkv; p.d = d;
-  p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E; p.cap = opt->softcap; p.sink = opt->sink ? 1 : 0;
+  p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E; p.cap = opt->softcap; p.cap_arg = opt->softcap > 0.f ? 2.f * CUCA_LOG2E / opt->softcap : 0.f; p.sink = opt->sink ? 1 : 0;
   p.sink_val = opt->sink ? opt->sink_val : nullptr; p.window = opt->window; p.keep = opt->window > 0 ? opt->keep : 0;
   p.slopes = opt->slopes; p.heads_per_cta = heads_per_cta; p.head_parts = head_parts; p.chunk = n_splits > 1 ? chunk : 0;
   p.n_splits = n_splits; p.part = part; p.err = err;

@@ -46,6 +46,7 @@ struct Q8Params {
   float scale_log2e;
   float cap;       // > 0: a score s becomes cap tanh(s / cap) ...
   float scale;     // ... of the score with this scale
+  float cap_arg;   // 2 log2 e / cap
   int sink;        // the denominator holds one more term exp(0) ...
   const float* sink_val;  // ... or exp(sink_val[head])
   int window, keep;
@@ -149,12 +150,12 @@ __device__ __forceinline__ void q8_query_scale(uint32_t top, float& up, float& d
   up = __uint_as_float((267u - e) << 23);
   down = __uint_as_float((e - 13u) << 23);
 }
-// cap tanh(s / cap) in log2 units. EXACT: for the 32-bit mode; else 1 - 2 / (e^2y + 1), right at both ends.
+// cap tanh(s / cap) in log2 units. EXACT: for the 32-bit mode; else 1 - 2 / (e^2y + 1), right at both ends, and without a branch
+// (a quotient that is rounded right has one, which leaves a warp's threads apart).
 template <bool EXACT>
-__device__ __forceinline__ float q8_capped(float s, float cap) {
-  if (EXACT) return cap * CUCA_LOG2E * tanhf(s / cap);
-  const float e = q8_exp2(s * (2.f * CUCA_LOG2E) / cap);
-  return cap * CUCA_LOG2E * (1.f - __fdividef(2.f, e + 1.f));
+__device__ __forceinline__ float q8_capped(float s, const Q8Params& p) {
+  if (EXACT) return p.cap * CUCA_LOG2E * tanhf(s / p.cap);
+  return p.cap * CUCA_LOG2E * (1.f - __fdividef(2.f, q8_exp2(s * p.cap_arg) + 1.f));
 }
 // What a sink adds to a denominator that is relative to the reference m.
 __device__ __forceinline__ float q8_sink_term(const Q8Params& p, int head, float m) {

@@ -195,6 +195,8 @@ _SIGNATURES = {
     "cuca_read_q8": [_P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P],
     "cuca_attention_q8": [_P, _I, _P, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P,
                           _I, _I, _I, _I, _P, _P, _P],
+    "cuca_attention_q8_tc": [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _I,
+                             _I, _P, _P, _P],
 }
 
 _lock = threading.Lock()

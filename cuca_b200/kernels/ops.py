@@ -1645,6 +1645,9 @@ def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, 
         0 if v_out is None else v_out.stride(0), dtype_code(outs[0].dtype), n, nkv, d, _p(err), _stream()), "read_q8")
 
 
+Q8_FEW_ROWS = 32  # query rows of a key head that the form for few rows takes of a portion
+
+
 class QuantizedPlan:
     """How a step's requests are handed to the attention over 8-bit pages: counts and lengths from the step's per-request lists
     on the host; which rows a block takes is worked out on the device. One plan serves every layer of a step."""
@@ -1661,16 +1664,41 @@ class QuantizedPlan:
         self._launches: dict = {}
 
     def launches(self, n_heads, n_kv_heads, head_dim, dtype, window, keep):
-        """[(least count, most count, rows of a tile, tiles, heads of a block, column tiles, keys of a share, shares)]"""
+        """[(form, least count, most count, rows of a tile, tiles, heads of a block, column tiles, keys of a share, shares)];
+        form 0: few rows a block, 1: tcgen05 (there `column tiles` are query tiles of 128)"""
         key = (n_heads, n_kv_heads, head_dim, dtype, window, keep)
         if key not in self._launches:
-            out = []
+            group, out, few = n_heads // n_kv_heads, [], self.longest
+            if dtype == torch.bfloat16 and head_dim <= 128 and group <= 128:
+                few = Q8_FEW_ROWS // group
             if 1 in self.counts:
                 out.append(self._few(1, 1, *key))
-            if self.longest > 1:
-                out.append(self._few(2, self.longest, *key))
+            if any(1 < c <= few for c in self.counts):
+                out.append(self._few(2, few, *key))
+            if self.longest > max(few, 1):
+                out.append(self._many(max(few, 1) + 1, self.longest, *key))
             self._launches[key] = out
         return self._launches[key]
+
+    def _many(self, lo, hi, n_heads, n_kv_heads, head_dim, dtype, window, keep):
+        sms, fixed, best = sm_count(), 4, None
+        tokens = 128 // (n_heads // n_kv_heads)
+
+        def lengths(n):  # key tiles of 64 of every tile of n rows
+            return [-(-(e if window is None else min(e, window + n + keep)) // 64) for c, length in zip(self.counts, self.lengths)
+                    if lo <= c <= hi for e in range(length, length - c, -n)]
+        query_tiles = 1 if len(lengths(tokens)) * n_kv_heads <= sms else 2
+        tiles = lengths(tokens * query_tiles)
+        longest = max(tiles)
+        for shares in range(1, min(16, -(-longest // 4)) + 1):
+            share = -(-longest // shares)
+            blocks = sum(-(-t // share) for t in tiles) * n_kv_heads
+            rounds = -(-blocks // sms)
+            cost = max(share + fixed, rounds * (sum(tiles) * n_kv_heads / blocks + fixed) if rounds > 1 else 0) + (fixed if shares > 1 else 0)
+            if best is None or cost < best[0]:
+                best = cost, share, -(-longest // share)
+        _, share, shares = best
+        return 1, lo, hi, tokens * query_tiles, len(tiles), 0, query_tiles, share * 64, shares
 
     def _few(self, lo, hi, n_heads, n_kv_heads, head_dim, dtype, window, keep):
         parts, group = (2 if dtype == torch.float32 else 1), n_heads // n_kv_heads
@@ -1689,7 +1717,7 @@ class QuantizedPlan:
                 keys += n * seen
                 longest = max(longest, seen)
         share, shares = _q8_shares(tiles * pieces, keys * pieces, longest, head_dim, nt)
-        return lo, hi, tokens, tiles, heads, nt, share, shares
+        return 0, lo, hi, tokens, tiles, heads, nt, share, shares
 
 
 def _q8_shares(blocks: int, keys: int, longest: int, head_dim: int, nt: int, sms: int | None = None):
@@ -1735,14 +1763,24 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
     plan = attention_q8_plan(step)
     opt = attention_options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
     lib = library.load()
-    for lo, hi, tokens, tiles, heads, nt, share, shares in plan.launches(n_heads, n_kv_heads, head_dim, q.dtype, window or None, opt.keep):
+    rows = (_p(pages.k), _p(pages.v), _p(pages.k_scale), _p(pages.v_scale), pages.k.shape[0], pages.k.shape[2], _p(step.positions),
+            _p(step.seq_of_row), _p(tables), tables.shape[1], _p(step.req_row0), None if plan.all_single else _p(step.req_count),
+            step.n_seqs)
+    for form, lo, hi, tokens, tiles, heads, nt, share, shares in plan.launches(n_heads, n_kv_heads, head_dim, q.dtype, window or None,
+                                                                               opt.keep):
         part = None
+        if form == 1:
+            if shares > 1:
+                part = torch.empty(tiles * n_kv_heads * shares * (256 * (64 if head_dim <= 64 else 128) + 512), dtype=torch.float32,
+                                   device=q.device)
+            library.check(lib.cuca_attention_q8_tc(_p(q), q.stride(0), _p(out), out.stride(0), *rows, lo, hi, nt, tiles, n_heads,
+                                                   n_kv_heads, head_dim, ctypes.addressof(opt), share, shares, _p(part), _p(err),
+                                                   _stream()), "attention_q8")
+            continue
         if shares > 1:
             cols = 8 * nt // (2 if code == F32 else 1)
             part = torch.empty(tiles * n_kv_heads * -(-(n_heads // n_kv_heads) // heads) * shares * cols * (head_dim + 2),
                                dtype=torch.float32, device=q.device)
-        library.check(lib.cuca_attention_q8(
-            _p(q), q.stride(0), _p(out), out.stride(0), code, _p(pages.k), _p(pages.v), _p(pages.k_scale), _p(pages.v_scale),
-            pages.k.shape[0], pages.k.shape[2], _p(step.positions), _p(step.seq_of_row), _p(tables), tables.shape[1],
-            _p(step.req_row0), None if plan.all_single else _p(step.req_count), step.n_seqs, lo, hi, tokens, tiles, n_heads,
-            n_kv_heads, head_dim, ctypes.addressof(opt), heads, nt, share, shares, _p(part), _p(err), _stream()), "attention_q8")
+        library.check(lib.cuca_attention_q8(_p(q), q.stride(0), _p(out), out.stride(0), code, *rows, lo, hi, tokens, tiles, n_heads,
+                                            n_kv_heads, head_dim, ctypes.addressof(opt), heads, nt, share, shares, _p(part), _p(err),
+                                            _stream()), "attention_q8")

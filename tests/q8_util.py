@@ -118,7 +118,7 @@ class Case:
                     den = den + torch.exp((sink_values[h].double() if sink_values is not None else 0.0) - s.amax(-1, keepdim=True))
                 w = e / den
                 out[rows, h], size[rows, h] = w @ vh, w @ vh.abs()
-                most[rows, h] = (w * vh.abs().amax(-1)).amax(-1) * see.sum(-1)
+                most[rows, h] = (w * vh.abs().amax(-1).clamp_min(127 * 2.0 ** -60)).amax(-1) * see.sum(-1)
                 work[rows, h] = ((q.abs() @ kh.abs().T) * abs(scale)).masked_fill(~see, 0.0).amax(-1)
             row0 += count
         return out, size, work, most
@@ -127,7 +127,8 @@ class Case:
         """How far a result may be: its own rounding; the weights' (11 bits, in 32-bit mode 22; the exponent of 2 and the value
         scale's logarithm are good to 2^-21); the scores' 32-bit sums of d products in steps of 16 in each of two parts, whose
         error e changes a weight by a factor of e^e above and below the line. A 16-bit float has no steps under 2^-24, and the
-        largest weight is 2^7 or more: each key's weight may be off by 2^-32 of that."""
+        largest weight is 2^7 or more: each key's weight may be off by 2^-32 of that (a value
+        scale counts as 2^-60 at least there)."""
         f32 = self.dtype == torch.float32
         steps = (2 if f32 else 1) * self.dim / 16 + 4
         score = steps * 2.0 ** -23 * work[..., None]
