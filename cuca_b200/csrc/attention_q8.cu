@@ -22,32 +22,6 @@ constexpr int GROUP = 16;     // keys of a step
 constexpr int STAGES = 4;     // of a warp's ring
 constexpr int WARPS = 4;
 
-__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {  // zeros where not ok
-  const int n = ok ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool ok) {
-  const int n = ok ? 4 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 shared_16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ uint2 shared_8(uint32_t at) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ float shared_f(uint32_t at) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
-  return v;
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -127,6 +101,7 @@ attention_q8_kernel(const Q8Params p) {
   uint32_t* q_shared = reinterpret_cast<uint32_t*>(smem + WARPS * R::WARP);  // [TILES][NT][32 lanes][2]
   uint32_t qf[Q_SHARED ? 1 : TILES][Q_SHARED ? 1 : NT][2];
   float q_down[NT][LC];
+  const bool q_aligned = ((uintptr_t)p.q & 15) == 0 && p.q_stride % (16 / (int)sizeof(T)) == 0;
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int col = (8 * j + g) / PARTS;
@@ -137,11 +112,29 @@ attention_q8_kernel(const Q8Params p) {
 #pragma unroll
     for (int i = 0; i < QC; ++i) {
       const int e0 = (t + 4 * i) * 16;
+      const bool mine = ok && e0 < p.d;
+      if (q_aligned) {
+        constexpr int N = 16 / sizeof(T);  // values of 16 bytes
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        v[i][e] = ok && e0 < p.d ? to_f32(src[e0 + e]) : 0.f;
-        top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+        for (int n = 0; n < 16 / N; ++n) {
+          const uint4 w = mine ? *reinterpret_cast<const uint4*>(src + e0 + n * N) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (PARTS == 2) {
+              v[i][n * N + e] = __uint_as_float(x[e]);
+            } else {
+              v[i][n * N + (2 * e) % N] = __uint_as_float(x[e] << 16);
+              v[i][n * N + (2 * e + 1) % N] = __uint_as_float(x[e] & 0xffff0000u);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[i][e] = mine ? to_f32(src[e0 + e]) : 0.f;
       }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
     }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -183,29 +176,49 @@ attention_q8_kernel(const Q8Params p) {
   const int least_pos = pos0, most_lo = p.window > 0 ? pos0 + n_tok - 1 - (p.window - 1) : 0;
 
   // ---------------------------------------------------------------- the ring
-  const uint32_t ring = shared_at(my_ring);
+  const uint32_t ring = q8_shared(my_ring);
   if (p.d < DP) {
     for (int i = lane; i < R::WARP / 16; i += 32) reinterpret_cast<uint4*>(my_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncwarp();
   }
-  // Lane k of 16: where key k of a group stands in the pools, as a row number (-1: nowhere), looked up a step before its use.
-  auto lookup = [&](int j) -> long long {
-    if (j >= last) return -1;
-    const int kp = keys.at(j) * GROUP + (lane & 15);
-    if (kp >= keys.hi) return -1;
-    const int entry = kp / p.bs;
-    const int blk = entry < p.table_stride ? table[entry] : -1;
-    if (blk < 0 || blk >= p.n_blocks) {
-      // pages behind a window may have gone back; their keys are masked. Anything else is an error.
-      if ((kp >= (p.window > 0 ? pos0 - (p.window - 1) : 0) || kp < p.keep) && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
-      return -1;
-    }
-    return ((long long)blk * p.nkv + kvh) * p.bs + kp % p.bs;
-  };
+  // Groups that lie within a page (its size a power of two, 16 at least) and whose rows have no gap: one look at the table and two
+  // runs of bytes a group. `find` gives the page, `fetch` checks it and asks for the rows; the look goes out a step before.
+  const bool in_page = p.run_shift >= 4 && p.d == DP;
   constexpr int KEYS_AT_ONCE = 32 / CHUNKS;
-  auto fetch = [&](int stage, long long mine) {
+  const int lo = p.window > 0 ? pos0 - (p.window - 1) : 0;
+  // Else lane k of 16: the page of key k of the group.
+  auto find = [&](int j) -> int {
+    if (j >= last) return -1;
+    if (in_page) {
+      const int entry = (keys.at(j) * GROUP) >> p.run_shift;
+      return entry < p.table_stride ? table[entry] : -1;
+    }
+    const int kp = keys.at(j) * GROUP + (lane & 15), entry = kp / p.bs;
+    return kp < keys.hi && entry < p.table_stride ? table[entry] : -1;
+  };
+  auto fetch = [&](int j, int stage, int blk) {
     const uint32_t at = ring + stage * R::STAGE;
+    const int key0 = keys.at(j) * GROUP;
+    const bool paged = blk >= 0 && blk < p.n_blocks;
     const int c = lane % CHUNKS;
+    if (in_page) {
+      // (pages behind a window may have gone back; their keys are masked. Any other that is not there is an error.)
+      if (!paged && (key0 + GROUP > lo || key0 < p.keep) && lane == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+      const size_t row = ((size_t)(paged ? blk : 0) * p.nkv + kvh) * p.bs + (key0 & (p.bs - 1));
+      const int8_t* kr = p.kpool + row * DP + lane * 16;
+      const int8_t* vr = p.vpool + row * DP + lane * 16;
+#pragma unroll
+      for (int i = 0; i < GROUP / KEYS_AT_ONCE; ++i) {
+        const int k = i * KEYS_AT_ONCE + lane / CHUNKS;
+        copy16(at + R::place(k, c), kr + i * 512, paged);
+        copy16(at + R::TENSOR + R::place(k, c), vr + i * 512, paged);
+      }
+      copy4(at + 2 * R::TENSOR + lane * 4, (lane < 16 ? p.kscale : p.vscale) + row + (lane & 15), paged);
+      return;
+    }
+    const int kp = key0 + (lane & 15);
+    if (!paged && kp < keys.hi && (kp >= lo || kp < p.keep) && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+    const long long mine = paged ? ((long long)blk * p.nkv + kvh) * p.bs + kp % p.bs : -1;
 #pragma unroll
     for (int i = 0; i < GROUP / KEYS_AT_ONCE; ++i) {
       const int k = i * KEYS_AT_ONCE + lane / CHUNKS;
@@ -234,15 +247,15 @@ attention_q8_kernel(const Q8Params p) {
 #pragma unroll
     for (int c = 0; c < LC; ++c) { m[j][c] = -INFINITY; l[j][c] = 0.f; }
 
-  long long next;
+  int next;
   {
-    long long at[STAGES - 1];
+    int at[STAGES - 1];
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) at[s] = lookup(first + warp + WARPS * s);
-    next = lookup(first + warp + WARPS * (STAGES - 1));
+    for (int s = 0; s < STAGES - 1; ++s) at[s] = find(first + warp + WARPS * s);
+    next = find(first + warp + WARPS * (STAGES - 1));
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-      if (first + warp + WARPS * s < last) fetch(s, at[s]);
+      if (first + warp + WARPS * s < last) fetch(first + warp + WARPS * s, s, at[s]);
       copies_commit();
     }
   }
@@ -254,9 +267,9 @@ attention_q8_kernel(const Q8Params p) {
     __syncwarp();
     {  // the stage that was read in the last turn
       const int ahead = stage == 0 ? STAGES - 1 : stage - 1;
-      if (j0 + WARPS * (STAGES - 1) < last) fetch(ahead, next);
+      if (j0 + WARPS * (STAGES - 1) < last) fetch(j0 + WARPS * (STAGES - 1), ahead, next);
       copies_commit();
-      next = lookup(j0 + WARPS * STAGES);
+      next = find(j0 + WARPS * STAGES);
     }
     const uint32_t at = ring + stage * R::STAGE;
     stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -459,20 +472,21 @@ attention_q8_kernel(const Q8Params p) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) dst[k] = from_f32<T>(o[k] * inv);
     } else {
-      float* dst = p.part + ((((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.n_splits + blockIdx.x) * COLS + col) * (p.d + 2);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) dst[e + k] = o[k];
-      if (e == 0) { dst[p.d] = top; dst[p.d + 1] = den; }
+      float* part = p.part + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.n_splits + blockIdx.x) * (COLS * (p.d + 2));
+      *reinterpret_cast<float4*>(part + col * p.d + e) = make_float4(o[0], o[1], o[2], o[3]);
+      if (e == 0) *reinterpret_cast<float2*>(part + COLS * p.d + 2 * col) = make_float2(top, den);
     }
   }
 }
 
-// Joins the shares of a tile's keys, in their order: a block per tile and key head, a warp per query row.
+// Joins the shares of a tile's keys, in their order: a warp per query row. Its lanes take two shares' maxima and sums each, then
+// four dimensions (of each 128).
+constexpr int MOST_SHARES = 64;
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32) join_q8_kernel(const Q8Params p, int cols) {
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = blockIdx.x * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   int row0, n_tok;
   if (!q8_rows_of_tile(p, blockIdx.z, row0, n_tok)) return;
   const int kvh = blockIdx.y / p.head_parts, hp = blockIdx.y % p.head_parts;
@@ -480,33 +494,42 @@ __global__ void __launch_bounds__(WARPS * 32) join_q8_kernel(const Q8Params p, i
   const int head0 = kvh * group_heads + hp * p.heads_per_cta;
   const int heads = min(p.heads_per_cta, group_heads - hp * p.heads_per_cta);
   const int pos0 = p.positions[row0];
-  if (p.seq_of_row[row0] < 0 || pos0 < 0) return;
+  if (p.seq_of_row[row0] < 0 || pos0 < 0 || col >= n_tok * heads) return;
   const Q8Keys keys = q8_keys<GROUP>(p, pos0, n_tok);
   const int share = p.chunk / GROUP, used = min(p.n_splits, (keys.groups + share - 1) / share);
   if (used <= 1) return;  // written already
-  for (int col = warp; col < n_tok * heads; col += WARPS) {
-    const float* src = p.part + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.n_splits * cols + col) * (p.d + 2);
-    const size_t step = (size_t)cols * (p.d + 2);
-    float top = -INFINITY;
-    for (int s = 0; s < used; ++s) top = fmaxf(top, src[s * step + p.d]);
-    float o[8], den = 0.f;
+  const size_t step = (size_t)cols * (p.d + 2);
+  const float* part = p.part + ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.n_splits * step;
+  float2 ml[2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] = 0.f;
+  for (int h = 0; h < 2; ++h)
+    ml[h] = lane + 32 * h < used ? *reinterpret_cast<const float2*>(part + (lane + 32 * h) * step + cols * p.d + 2 * col)
+                                 : make_float2(-INFINITY, 0.f);
+  const float top = warp_max(fmaxf(ml[0].x, ml[1].x));
+  float f[2], den = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    f[h] = lane + 32 * h < used ? (ml[h].x == top ? 1.f : q8_exp2(ml[h].x - top)) : 0.f;
+    den += lane + 32 * h < used ? f[h] * ml[h].y : 0.f;
+  }
+  den = warp_sum(den);
+  const int head = head0 + col % heads;
+  if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  for (int e0 = 0; e0 < p.d; e0 += 128) {
+    const int e = e0 + 4 * lane;
+    const float* src = part + col * p.d + (e < p.d ? e : 0);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
     for (int s = 0; s < used; ++s) {
-      const float* a = src + s * step;
-      const float ms = a[p.d], f = ms == top ? 1.f : q8_exp2(ms - top);
-      den += f * a[p.d + 1];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (lane + 32 * k < p.d) o[k] += f * a[lane + 32 * k];
+      const float fs = __shfl_sync(0xffffffffu, s < 32 ? f[0] : f[1], s & 31);
+      const float4 v = *reinterpret_cast<const float4*>(src + s * step);
+      o.x += fs * v.x; o.y += fs * v.y; o.z += fs * v.z; o.w += fs * v.w;
     }
-    const int head = head0 + col % heads;
-    if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    T* dst = (T*)p.out + (size_t)(row0 + col / heads) * p.out_stride + (size_t)head * p.d;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (lane + 32 * k < p.d) dst[lane + 32 * k] = from_f32<T>(o[k] * inv);
+    if (e >= p.d) continue;
+    T* dst = (T*)p.out + (size_t)(row0 + col / heads) * p.out_stride + (size_t)head * p.d + e;
+    dst[0] = from_f32<T>(o.x * inv); dst[1] = from_f32<T>(o.y * inv);
+    dst[2] = from_f32<T>(o.z * inv); dst[3] = from_f32<T>(o.w * inv);
   }
 }
 
@@ -529,7 +552,7 @@ int launch_q8(const Q8Params& p, int n_tiles, cudaStream_t stream) {
   CUCA_CHECK_LAUNCH("attention_q8");
   if (p.n_splits > 1) {
     auto join = join_q8_kernel<typename std::conditional<PARTS == 2, float, __nv_bfloat16>::type>;
-    cuca_launch(join, dim3(1, p.nkv * p.head_parts, n_tiles), dim3(WARPS * 32), 0, stream, true, p, NT * 8 / PARTS);
+    cuca_launch(join, dim3((p.tile_tokens * p.heads_per_cta + WARPS - 1) / WARPS, p.nkv * p.head_parts, n_tiles), dim3(WARPS * 32), 0, stream, true, p, NT * 8 / PARTS);
     CUCA_CHECK_LAUNCH("attention_q8 (join)");
   }
   return 0;
@@ -572,7 +595,8 @@ CUCA_API int cuca_attention_q8(const void* q, int q_stride, void* out, int out_s
   const int parts = dtype == CUCA_F32 ? 2 : 1, group = nh / nkv;
   CUCA_REQUIRE(heads_per_cta > 0 && heads_per_cta <= group && tile_tokens > 0 && (long long)tile_tokens * heads_per_cta * parts <= 8 * nt,
                "attention_q8: %d rows of %d heads do not fit %d columns", tile_tokens, heads_per_cta, 8 * nt / parts);
-  CUCA_REQUIRE(chunk >= 0 && chunk % 64 == 0 && n_splits >= 1 && (n_splits == 1 || (chunk > 0 && part)), "attention_q8: bad shares of the keys");
+  CUCA_REQUIRE(chunk >= 0 && chunk % 64 == 0 && n_splits >= 1 && n_splits <= MOST_SHARES &&
+               (n_splits == 1 || (chunk > 0 && part && ((uintptr_t)part & 15) == 0)), "attention_q8: bad shares of the keys");
   const int head_parts = (group + heads_per_cta - 1) / heads_per_cta;
   CUCA_REQUIRE(n_tiles <= 65535 && (long long)nkv * head_parts <= 65535, "attention_q8: too many tiles or heads");
   Q8Params p;
@@ -584,7 +608,7 @@ CUCA_API int cuca_attention_q8(const void* q, int q_stride, void* out, int out_s
   p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E; p.cap = opt->softcap; p.cap_arg = opt->softcap > 0.f ? 2.f * CUCA_LOG2E / opt->softcap : 0.f; p.sink = opt->sink ? 1 : 0;
   p.sink_val = opt->sink ? opt->sink_val : nullptr; p.window = opt->window; p.keep = opt->window > 0 ? opt->keep : 0;
   p.slopes = opt->slopes; p.heads_per_cta = heads_per_cta; p.head_parts = head_parts; p.chunk = n_splits > 1 ? chunk : 0;
-  p.n_splits = n_splits; p.part = part; p.err = err;
+  p.n_splits = n_splits; p.part = part; p.err = err; p.run_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
   if (parts == 2) {
     if (d <= 64) return launch_q8_nt<64, 2>(p, nt, n_tiles, stream);
     if (d <= 128) return launch_q8_nt<128, 2>(p, nt, n_tiles, stream);

@@ -33,6 +33,7 @@ struct Q8Params {
   const float* kscale;
   const float* vscale;
   int n_blocks, bs;
+  int run_shift;  // log2 of bs where it is a power of two, else -1
   const int* tables;
   int table_stride;
   const int* positions;
@@ -109,6 +110,34 @@ __device__ __forceinline__ Q8Keys q8_keys(const Q8Params& p, int pos0, int n) {
   return k;
 }
 
+// Asynchronous copies into shared memory, and loads from it by address.
+__device__ __forceinline__ uint32_t q8_shared(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {  // zeros where not ok
+  const int n = ok ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 shared_16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 shared_8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ float shared_f(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+
 // Four codes as two pairs of 16-bit floats: x + 128 in the low bits of 1024 (ulp 1), less 1152.
 __device__ __forceinline__ uint32_t q8_minus(uint32_t a) {
   uint32_t r;
@@ -126,6 +155,9 @@ __device__ __forceinline__ float q8_exp2(float x) {  // 2^x; 0 at -infinity
 __device__ __forceinline__ uint32_t q8_pack(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float q8_pow2(float e) {  // 2^e, e a whole number of -126 .. 127
+  return __uint_as_float((uint32_t)((int)e + 127) << 23);
 }
 // A value scale as f 2^e (e as a float), and 2^-e for the denominator. e is -60 at least, so that u 2^-e does not leave 32 bits
 // where scales are far apart; f is smaller than 1 then, 0 for a row of zeros. A scale that is not finite (2^123 and more, which

@@ -10,13 +10,19 @@
 // Four warps fetch the codes (into registers, a tile ahead), turn them into 16-bit floats and store them as operand tiles, with
 // each key's factors beside them; four warps per query tile own a row per thread (a lane of tensor memory) and turn scores into
 // weights; a warp per query tile issues its products. Where the two query tiles share a converted tile, the conversion is a
-// seventh of the block's instructions. Bound by the exponent unit, instruction issue and the tensor pipe, which need about the
-// same time for a tile.
+// seventh of the block's instructions.
+//
+// A value scale goes into the operand tile here: V = code vs 2^(7 - E) with E the largest exponent of the tile's scales, rounded
+// to 11 bits, factor and product, so that z = s + E for every key of the tile and one multiplication a tile brings the sum of
+// the weights to the denominator's unit. Per-key factors in the softmax would each cost 16 loads of 512 bytes a warp and tile:
+// with three of them a tile of 64 keys took 3,900 clocks, 2,048 of them of shared memory's bandwidth. Where a tile's scales are
+// more than 2^20 apart the exponents stay with the keys (`wide`). The keys' scales multiply the scores, so codes of keys are exact.
 //
 // Every wait is bounded; when one runs out the kernel records CUCA_ERR_WAIT_TIMEOUT, all roles stop, tensor memory is freed and
 // the kernel returns.
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
+#include <type_traits>
 
 namespace {
 
@@ -25,18 +31,33 @@ constexpr int KEYS = 64;   // keys of a tile
 constexpr int NQ = 2;      // query tiles of a block
 constexpr int SOFT_WARPS = 4 * NQ, CONV_WARPS = 4;
 constexpr int CONV = CONV_WARPS * 32;
-constexpr int NTHREADS = (SOFT_WARPS + CONV_WARPS + NQ) * 32;  // softmax, conversion, issue
-constexpr int STAGES = 4;
+constexpr int NTHREADS = (SOFT_WARPS + CONV_WARPS + 4) * 32;  // softmax, conversion, issue (two warps of four)
+// Registers a thread: 128 at launch, then by role; the sum, 2 x 176 + 88 + 64 over groups of 128 threads, is within the 4 x 128
+// of the launch.
+constexpr int SOFT_REGS = 176, CONV_REGS = 88, ISSUE_REGS = 64;
+constexpr int STAGES = 3;         // of operand tiles
+constexpr int RAW = 3;            // tiles of codes on their way
+constexpr float V_LIFT = 7.f;     // values are 2^7 larger in the operand tile: 127 2^7 2 is the most that fits
+constexpr int WIDE = 20;
 constexpr int TMEM_COLS = 512;  // two score buffers per query tile (4 x 64 columns), results of both (2 x DP)
+
+__device__ __forceinline__ uint32_t q8_times(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
 template <int DP>
 struct Shape {
   static constexpr int HALVES = DP / 64;
   static constexpr int Q_HALF = ROWS * 128, Q_BYTES = HALVES * Q_HALF;
   static constexpr int KV_HALF = KEYS * 128, KV_TILE = HALVES * KV_HALF;
-  static constexpr int FACTORS = 4 * KEYS * 4;  // of a stage: the keys' factors, the value scales' exponents, 2^-exponents, fractions
+  static constexpr int FACTORS = (3 * KEYS + 4) * 4;  // of a stage: the keys' factors; the value scales' exponents less E and their
+                                                      // inverse (of a wide tile); E, its inverse, and whether the tile is wide
   static constexpr int STAGE = 2 * KV_TILE;
-  static constexpr int TILES = NQ * Q_BYTES + STAGES * (STAGE + FACTORS);
+  static constexpr int PER = KEYS * (DP / 16) / CONV;  // 16-byte pieces of keys, and of values, that a thread converts
+  static constexpr int RAW_STAGE = CONV * (2 * PER * 16 + 16);  // codes of a tile and four scales a thread, each thread's its own
+  static constexpr int TILES = NQ * Q_BYTES + STAGES * (STAGE + FACTORS) + RAW * RAW_STAGE;
   static constexpr int SMEM = TILES + 256 + 1024;  // + barriers, + alignment
 };
 
@@ -67,21 +88,23 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[2][32]) 
 }
 
 template <int DP, bool OPT>
-__global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Params p, const int bs_shift) {
+__global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Params p) {
   using SH = Shape<DP>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  // (by an offset, so that the compiler still knows it for shared memory)
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* q_s = smem;
   uint8_t* kv_s = q_s + NQ * SH::Q_BYTES;
   float* factor_s = (float*)(kv_s + STAGES * SH::STAGE);
-  uint64_t* bars = (uint64_t*)((uint8_t*)factor_s + STAGES * SH::FACTORS);
+  uint8_t* raw_s = (uint8_t*)factor_s + STAGES * SH::FACTORS;
+  uint64_t* bars = (uint64_t*)(raw_s + RAW * SH::RAW_STAGE);
   uint64_t* q_full = bars;                   // [NQ]
   uint64_t* kv_full = q_full + NQ;           // [STAGES]
   uint64_t* kv_empty = kv_full + STAGES;     // [STAGES]
   uint64_t* s_full = kv_empty + STAGES;      // [NQ][2]
   uint64_t* p_full = s_full + 2 * NQ;        // [NQ]
-  uint64_t* pv_done = p_full + NQ;           // [NQ]
-  uint32_t* tmem_slot = (uint32_t*)(pv_done + NQ);
+  uint64_t* pv_done = p_full + NQ;           // [NQ][2]
+  uint32_t* tmem_slot = (uint32_t*)(pv_done + 2 * NQ);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   uint32_t* q_top = tmem_slot + 2;           // the largest magnitude of the block's queries, as bits
 
@@ -121,11 +144,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       mbar_init(&q_full[x], 128);
       mbar_init(&s_full[2 * x], 1);
       mbar_init(&s_full[2 * x + 1], 1);
-      mbar_init(&p_full[x], 128);
-      mbar_init(&pv_done[x], 1);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&pv_done[2 * x], 1);
+      mbar_init(&pv_done[2 * x + 1], 1);
     }
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&kv_full[s], CONV);
+      mbar_init(&kv_full[s], CONV_WARPS);
       mbar_init(&kv_empty[s], nq);
     }
     *abort_flag = 0;
@@ -141,6 +165,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 
   if (warp < SOFT_WARPS) {
     // ------------------------------------------------ a query row per thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
     const int x = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;  // row of the query tile
     const uint32_t lane_bits = (uint32_t)(quarter * 32) << 16;
@@ -199,43 +224,50 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const float slope2 = OPT && p.slopes ? p.slopes[head] * CUCA_LOG2E : 0.f;
     float m = -INFINITY, l = 0.f;
     bool ok = x < nq;
+    // The product of tile j - 1. Not every one is waited for and two can be on their way, so even and odd tiles have a barrier
+    // each: tile j - 3's product was done before tile j - 1's scores were, so this one's is a phase behind at most.
+    auto product_done = [&](int j) {
+      return warp_wait(&pv_done[2 * x + ((j - 1) & 1)], ((j - 1) >> 1) & 1, p.err, abort_flag);
+    };
     for (int j = 0; ok && j < n_tiles; ++j) {
       const int st = j % STAGES;
       if (!warp_wait(&s_full[2 * x + (j & 1)], (j >> 1) & 1, p.err, abort_flag)) { ok = false; break; }
       tc_fence_after();
       // (long complete: the scores were made from the tile; for the factors that came with it)
       if (!warp_wait(&kv_full[st], (j / STAGES) & 1, p.err, abort_flag)) { ok = false; break; }
-      const float4* factor = reinterpret_cast<const float4*>(factor_s + st * 4 * KEYS);
+      const float* factor = factor_s + st * (SH::FACTORS / 4);
+      const float4* kf4 = reinterpret_cast<const float4*>(factor);
+      const float4 tile_e = kf4[3 * KEYS / 4];  // E, 2^-E, wide
       const int key0 = keys.at(first + j) * KEYS;
       const bool whole = key0 + KEYS - 1 <= least_pos && (p.window <= 0 || key0 >= most_lo || key0 + KEYS <= p.keep);
       uint32_t raw[2][32];
       tmem_ld64(tmem_s(x, j) + lane_bits, raw);
-      // z = s + e
+      // scores in log2 units
       const float bias0 = OPT ? slope2 * (float)(key0 - row_pos) : 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 kf = factor[c * 8 + i], ve = factor[KEYS / 4 + c * 8 + i];
-          const float f[4] = {kf.x, kf.y, kf.z, kf.w}, e[4] = {ve.x, ve.y, ve.z, ve.w};
+          const float4 kf = kf4[c * 8 + i];
+          const float f[4] = {kf.x, kf.y, kf.z, kf.w};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int k = 4 * i + 2 * h;
-            const float2 r2 = make_float2(__uint_as_float(raw[c][k]), __uint_as_float(raw[c][k + 1]));
-            const float2 f2 = make_float2(f[2 * h], f[2 * h + 1]), e2 = make_float2(e[2 * h], e[2 * h + 1]);
-            float2 z;
+            float2 s2 = __fmul2_rn(make_float2(__uint_as_float(raw[c][k]), __uint_as_float(raw[c][k + 1])), make_float2(f[2 * h], f[2 * h + 1]));
             if (OPT) {
-              float2 s2 = __fmul2_rn(r2, f2);
               if (p.cap > 0.f) s2 = make_float2(q8_capped<false>(s2.x, p), q8_capped<false>(s2.y, p));
               s2 = __fadd2_rn(s2, make_float2(fmaf(slope2, (float)(c * 32 + k), bias0), fmaf(slope2, (float)(c * 32 + k + 1), bias0)));
-              z = __fadd2_rn(s2, e2);
-            } else {
-              z = __ffma2_rn(r2, f2, e2);
             }
-            raw[c][k] = __float_as_uint(z.x);
-            raw[c][k + 1] = __float_as_uint(z.y);
+            raw[c][k] = __float_as_uint(s2.x);
+            raw[c][k + 1] = __float_as_uint(s2.y);
           }
         }
+      if (tile_e.z != 0.f) {  // a wide tile
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) raw[c][i] = __float_as_uint(__uint_as_float(raw[c][i]) + factor[KEYS + c * 32 + i]);
+      }
       if (!whole) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -251,38 +283,37 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 #pragma unroll
         for (int i = 0; i < 32; i += 2)
           mx4[(i >> 1) & 3] = fmaxf(fmaxf(mx4[(i >> 1) & 3], __uint_as_float(raw[c][i])), __uint_as_float(raw[c][i + 1]));
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) + tile_e.x;
       const bool moves = mx > m + Q8_LAG;
       const float corr = moves ? q8_exp2(m - mx) : 1.f;
       if (moves) m = mx;
-      const float ref = m == -INFINITY ? 0.f : m - Q8_LIFT;
+      const float ref = (m == -INFINITY ? 0.f : m - Q8_LIFT) - tile_e.x;
       const float2 neg2 = make_float2(-ref, -ref);
       float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       uint32_t pw[KEYS / 2];
+      auto weights = [&](auto wide) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 vi = factor[2 * KEYS / 4 + c * 8 + i], vf = factor[3 * KEYS / 4 + c * 8 + i];
-          const float v[4] = {vi.x, vi.y, vi.z, vi.w}, f[4] = {vf.x, vf.y, vf.z, vf.w};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = 4 * i + 2 * h;
-            const float2 x2 = __fadd2_rn(make_float2(__uint_as_float(raw[c][k]), __uint_as_float(raw[c][k + 1])), neg2);
+          for (int e = 0; e < 16; ++e) {
+            const float2 x2 = __fadd2_rn(make_float2(__uint_as_float(raw[c][2 * e]), __uint_as_float(raw[c][2 * e + 1])), neg2);
             const float2 u2 = make_float2(q8_exp2(x2.x), q8_exp2(x2.y));
-            sum2[h] = __ffma2_rn(u2, make_float2(v[2 * h], v[2 * h + 1]), sum2[h]);
-            const float2 w2 = __fmul2_rn(u2, make_float2(f[2 * h], f[2 * h + 1]));
-            pw[c * 16 + 2 * i + h] = q8_pack(w2.x, w2.y);
+            if (decltype(wide)::value)
+              sum2[e & 1] = __ffma2_rn(u2, *reinterpret_cast<const float2*>(factor + 2 * KEYS + c * 32 + 2 * e), sum2[e & 1]);
+            else
+              sum2[e & 1] = __fadd2_rn(sum2[e & 1], u2);
+            pw[c * 16 + e] = q8_pack(u2.x, u2.y);
           }
-        }
+      };
+      if (tile_e.z != 0.f) weights(std::true_type{});
+      else weights(std::false_type{});
       static_assert(KEYS == 64, "one 32-column store holds a row's weights of a tile");
       __syncwarp();
       tmem_st32_raw(tmem_s(x, j) + lane_bits, pw);
-      l = l * corr + (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-      // O is made smaller where a row's maximum moved; only then must the product before have finished (its barrier is never
-      // more than a phase ahead: the next product waits for this tile's weights)
+      l = fmaf((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y), tile_e.y, l * corr);
+      // O is made smaller where a row's maximum moved; only then must the product before have finished
       if (j > 0 && __any_sync(0xffffffffu, moves)) {
-        if (!warp_wait(&pv_done[x], (j - 1) & 1, p.err, abort_flag)) { ok = false; break; }
+        if (!product_done(j)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
@@ -295,13 +326,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[x]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[x]);
     }
-    if (ok && warp_wait(&pv_done[x], (n_tiles - 1) & 1, p.err, abort_flag)) {
+    if (ok && product_done(n_tiles)) {
       tc_fence_after();
       if (alone) {
         if (OPT && p.sink && m != -INFINITY) l += q8_sink_term(p, head, m);
-        const float inv = bad ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : 1.f / l;
+        const float inv = bad ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : q8_pow2(-V_LIFT) / l;
         __nv_bfloat16* dst = out + (size_t)(row0 + tok) * p.out_stride + (size_t)head * p.d;
         const bool aligned = ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0;
 #pragma unroll
@@ -340,114 +372,151 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         }
         float* ml = part + NQ * ROWS * DP + x * 2 * ROWS;
         ml[r] = m;
-        ml[ROWS + r] = bad ? __uint_as_float(0x7fc00000u) : l;
+        ml[ROWS + r] = bad ? __uint_as_float(0x7fc00000u) : l * q8_pow2(V_LIFT);
       }
     }
   } else if (warp < SOFT_WARPS + CONV_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONV_REGS));
     // ------------------------------------------------ codes to operand tiles
-    const int tid = threadIdx.x - SOFT_WARPS * 32;
-    constexpr int CHUNKS = DP / 16;                // 16-byte pieces of a row
-    constexpr int PER = KEYS * CHUNKS / CONV;      // of a thread, in keys and in values
-    constexpr int STEP = CONV / CHUNKS;            // rows between a thread's pieces
-    const int c = tid % CHUNKS, r0 = tid / CHUNKS;
-    const bool piece = c * 16 < p.d;
+    // Every warp works for itself. Its lanes stand for the tile's keys lane and lane + 32 (pages, scales, the tile's exponent) and
+    // hand rows and factors round; it converts every fourth set of rows. A page is looked up a tile before its rows are asked for,
+    // and they three tiles before they are used, by asynchronous copies into places that are each thread's own: a load takes
+    // 1,700 to 2,700 clocks here, and with one tile on its way in registers a tile took as long.
+    const int cw = warp - SOFT_WARPS;
+    constexpr int ROWS_AT_ONCE = DP == 128 ? 4 : 8;         // of a warp: 16-byte pieces of keys or values
+    constexpr int STEP = CONV_WARPS * ROWS_AT_ONCE, PER = KEYS / STEP;
+    // Eight lanes that store together have two rows of four pieces, and find eight places.
+    const int half = DP == 128 ? lane >> 4 : 0, quad = lane & 3, r0 = cw * ROWS_AT_ONCE + ((lane >> 2) & (ROWS_AT_ONCE - 1));
+    const int c = half * 4 + quad;
+    const int c_at = c * 16 < p.d ? c * 16 : 0;  // (beyond the head's size anything will do: the queries are zeros there, and
+                                                 // the results are not stored)
+    const int place0 = half * SH::KV_HALF + r0 * 128 + (((2 * quad) ^ (r0 & 7)) << 4);
+    const int place1 = half * SH::KV_HALF + r0 * 128 + (((2 * quad + 1) ^ (r0 & 7)) << 4);
     const int* table = p.tables + (size_t)seq * p.table_stride;
     const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
-    // where key number i of tile j stands in the pools, as a row number (-1: nowhere)
-    auto entry_of = [&](int j, int i) {  // its page
-      if (j >= n_tiles) return -1;
-      const int kp = keys.at(first + j) * KEYS + i;
-      if (kp >= keys.hi) return -1;
-      const int at = bs_shift >= 0 ? kp >> bs_shift : kp / p.bs;
-      int blk = at < p.table_stride ? table[at] : -1;
-      if (blk < 0 || blk >= p.n_blocks) {
-        if ((kp >= lo || kp < p.keep) && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
-        blk = -1;
-      }
-      return blk;
-    };
-    auto row_of = [&](int blk, int j, int i) -> size_t {
-      const int kp = keys.at(first + j) * KEYS + i;
-      const int off = bs_shift >= 0 ? kp & (p.bs - 1) : kp % p.bs;
-      return ((size_t)blk * p.nkv + kvh) * p.bs + off;
-    };
-    int blk[PER], blk_f;
-    uint4 kn[PER], vn[PER];  // of the tile ahead
-    float ksn = 0.f, vsn = 0.f;
+    constexpr uint32_t NOWHERE = 0xffffffffu;
+    int page[2];                // of the tile that is asked for next
+    const uint32_t raw = q8_shared(raw_s) + (threadIdx.x - SOFT_WARPS * 32) * 16;
     auto look = [&](int j) {
+      const int key0 = keys.at(first + min(j, n_tiles - 1)) * KEYS;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) blk[i] = entry_of(j, r0 + i * STEP);
-      blk_f = tid < KEYS ? entry_of(j, tid) : -1;
+      for (int h = 0; h < 2; ++h) {
+        const int kp = min(key0 + lane + 32 * h, keys.hi - 1);
+        page[h] = __ldg(table + min(p.run_shift >= 0 ? kp >> p.run_shift : kp / p.bs, p.table_stride - 1));
+      }
     };
     auto fetch = [&](int j) {
+      if (j < n_tiles) {
+        const int key0 = keys.at(first + j) * KEYS;
+        const uint32_t to = raw + (j % RAW) * SH::RAW_STAGE;
+        bool wrong = false;
+        uint32_t key_row[2];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        kn[i] = vn[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (blk[i] >= 0 && piece) {
-          const size_t at = row_of(blk[i], j, r0 + i * STEP) * p.d + c * 16;
-          kn[i] = __ldg(reinterpret_cast<const uint4*>(p.kpool + at));
-          vn[i] = __ldg(reinterpret_cast<const uint4*>(p.vpool + at));
+        for (int h = 0; h < 2; ++h) {
+          const int kp = key0 + lane + 32 * h, off = p.run_shift >= 0 ? kp & (p.bs - 1) : kp % p.bs;
+          const bool mine = kp < keys.hi, paged = page[h] >= 0 && page[h] < p.n_blocks;
+          wrong |= mine && !paged && (kp >= lo || kp < p.keep);  // (pages behind a window may have gone back)
+          key_row[h] = mine && paged ? ((uint32_t)page[h] * p.nkv + kvh) * p.bs + off : NOWHERE;
+          const bool ok = key_row[h] != NOWHERE;
+          copy4(to + 2 * PER * CONV * 16 + 8 * h, p.vscale + (ok ? key_row[h] : 0u), ok);
+          copy4(to + 2 * PER * CONV * 16 + 8 * h + 4, p.kscale + (ok ? key_row[h] : 0u), ok);
+        }
+        if (wrong && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const uint32_t row = __shfl_sync(0xffffffffu, key_row[(i * STEP) / 32], (r0 + i * STEP) & 31);
+          const size_t at = (size_t)(row == NOWHERE ? 0u : row) * p.d + c_at;  // (a key that is not there: zeros, scales 0, masked)
+          copy16(to + 2 * i * CONV * 16, p.kpool + at, row != NOWHERE);
+          copy16(to + (2 * i + 1) * CONV * 16, p.vpool + at, row != NOWHERE);
         }
       }
-      ksn = vsn = 0.f;
-      if (blk_f >= 0) {
-        const size_t at = row_of(blk_f, j, tid);
-        ksn = __ldg(p.kscale + at);
-        vsn = __ldg(p.vscale + at);
-      }
+      copies_commit();
     };
     look(0);
-    fetch(0);
-    look(1);
+#pragma unroll
+    for (int j = 0; j < RAW; ++j) {
+      fetch(j);
+      look(j + 1);
+    }
     asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
     float up, down;
     q8_query_scale(*q_top, up, down);
     const float key_factor = down * (OPT && p.cap > 0.f ? p.scale : p.scale_log2e);
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j % STAGES;
-      uint4 k[PER], v[PER];
-      const float ks = ksn, vs = vsn;
+      copies_wait<RAW - 1>();  // the thread's own copies of the tile
+      const uint32_t from = raw + (j % RAW) * SH::RAW_STAGE;
+      const uint4 scales = shared_16(from + 2 * PER * CONV * 16);
+      const float vs[2] = {__uint_as_float(scales.x), __uint_as_float(scales.z)}, ks[2] = {__uint_as_float(scales.y), __uint_as_float(scales.w)};
+      // the tile's exponent: the largest of its finite scales other than 0
+      float e[2], f, inv;
+      bool fine[2];
+      int hi = -60, least = 1000;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) { k[i] = kn[i]; v[i] = vn[i]; }
-      if (j + 1 < n_tiles) {
-        fetch(j + 1);
-        look(j + 2);
+      for (int h = 0; h < 2; ++h) {
+        q8_value_scale(vs[h], e[h], f, inv);
+        fine[h] = e[h] == e[h];
+        if (fine[h] && vs[h] != 0.f) { hi = max(hi, (int)e[h]); least = min(least, (int)e[h]); }
+      }
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      least = __reduce_min_sync(0xffffffffu, least);
+      const bool wide = hi - least > WIDE;
+      uint32_t factor2[2];  // what a key's value codes are multiplied by, twice
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = fine[h] ? vs[h] * q8_pow2(V_LIFT - (wide ? e[h] : (float)hi)) : 0.f;
+        factor2[h] = q8_pack(x, x);
       }
       if (j >= STAGES && !warp_wait(&kv_empty[st], ((j / STAGES) & 1) ^ 1, p.err, abort_flag)) break;
       uint8_t* kt = kv_s + st * SH::STAGE;
-      auto put = [&](uint8_t* tile, int row, const uint4& w4) {
-        // 16 dimensions: two pieces of a 128-byte row of 64. Eight lanes, a row's eight pieces (or two rows' four), must find
-        // eight places: lanes of the second half of a wide row go the other way round.
-        const int swap = DP == 128 ? c >> 2 : 0;
-        const uint32_t w[4] = {(swap ? w4.z : w4.x) ^ 0x80808080u, (swap ? w4.w : w4.y) ^ 0x80808080u,
-                               (swap ? w4.x : w4.z) ^ 0x80808080u, (swap ? w4.y : w4.w) ^ 0x80808080u};
-        uint8_t* dst = tile + (c / 4) * SH::KV_HALF + row * 128;
-        *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + swap) ^ (row & 7)) << 4)) =
-            make_uint4(q8_pair_lo(w[0]), q8_pair_hi(w[0]), q8_pair_lo(w[1]), q8_pair_hi(w[1]));
-        *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1 - swap) ^ (row & 7)) << 4)) =
-            make_uint4(q8_pair_lo(w[2]), q8_pair_hi(w[2]), q8_pair_lo(w[3]), q8_pair_hi(w[3]));
-      };
+      if (cw == j % CONV_WARPS) {
+        float* factor = factor_s + st * (SH::FACTORS / 4);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) put(kt, r0 + i * STEP, k[i]);
+        for (int h = 0; h < 2; ++h) {
+          const int key = lane + 32 * h;
+          // (a value row that is not finite: its scores are NaN for those who see it)
+          factor[key] = fine[h] ? ks[h] * key_factor : __uint_as_float(0x7fc00000u);
+          if (wide) {
+            factor[KEYS + key] = fine[h] ? e[h] - (float)hi : 0.f;
+            factor[2 * KEYS + key] = fine[h] ? q8_pow2(fmaxf(-126.f, fminf(127.f, (float)hi - e[h]))) : 1.f;
+          }
+        }
+        if (lane == 0) *reinterpret_cast<float4*>(factor + 3 * KEYS) = make_float4((float)hi, q8_pow2(-(float)hi), wide ? 1.f : 0.f, 0.f);
+      }
 #pragma unroll
-      for (int i = 0; i < PER; ++i) put(kt + SH::KV_TILE, r0 + i * STEP, v[i]);
-      if (tid < KEYS) {
-        float* f = factor_s + st * 4 * KEYS + tid;
-        float e, frac, inv;
-        q8_value_scale(vs, e, frac, inv);
-        f[0] = ks * key_factor;
-        f[KEYS] = e;
-        f[2 * KEYS] = inv;
-        f[3 * KEYS] = frac;
+      for (int i = 0; i < PER; ++i) {
+        const uint4 k = shared_16(from + 2 * i * CONV * 16);
+        const uint32_t w[4] = {k.x ^ 0x80808080u, k.y ^ 0x80808080u, k.z ^ 0x80808080u, k.w ^ 0x80808080u};
+        *reinterpret_cast<uint4*>(kt + place0 + i * STEP * 128) = make_uint4(q8_pair_lo(w[0]), q8_pair_hi(w[0]), q8_pair_lo(w[1]), q8_pair_hi(w[1]));
+        *reinterpret_cast<uint4*>(kt + place1 + i * STEP * 128) = make_uint4(q8_pair_lo(w[2]), q8_pair_hi(w[2]), q8_pair_lo(w[3]), q8_pair_hi(w[3]));
+      }
+      uint8_t* vt = kt + SH::KV_TILE;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t times = __shfl_sync(0xffffffffu, factor2[(i * STEP) / 32], (r0 + i * STEP) & 31);
+        const uint4 v = shared_16(from + (2 * i + 1) * CONV * 16);
+        const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+        uint32_t h[8];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) { h[2 * n] = q8_times(q8_pair_lo(w[n]), times); h[2 * n + 1] = q8_times(q8_pair_hi(w[n]), times); }
+        *reinterpret_cast<uint4*>(vt + place0 + i * STEP * 128) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(vt + place1 + i * STEP * 128) = make_uint4(h[4], h[5], h[6], h[7]);
       }
       fence_proxy_async();
-      mbar_arrive(&kv_full[st]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[st]);
+      fetch(j + RAW);  // where the codes were that have just been converted
+      look(j + RAW + 1);
     }
+    copies_wait<0>();
   } else {
     // ------------------------------------------------ products: a warp per query tile; scores run a tile ahead
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ISSUE_REGS));
     const int x = warp - SOFT_WARPS - CONV_WARPS;
     constexpr uint32_t idesc_qk = desc_f16(false, KEYS), idesc_pv = desc_f16(true, DP);
     bool ok = x < nq && warp_wait(&q_full[x], 0, p.err, abort_flag);
+    // The second query tile starts half a tile behind the first, so that one's exponents run beside the other's maxima and sums.
+    if (ok && x == 1) ok = warp_wait(&p_full[0], 0, p.err, abort_flag);
     const uint64_t q_desc = smem_desc(smem_u32(q_s + x * SH::Q_BYTES));
     const uint32_t kv_at = smem_u32(kv_s);
     auto scores = [&](int t) {
@@ -476,7 +545,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         for (int k = 0; k < KEYS / 16; ++k)
           umma_bf16_tmem_a(tmem_o(x), tmem_s(x, j) + k * 8, vd + (uint64_t)((k * 2048) >> 4), idesc_pv, j > 0 || k > 0);
         umma_commit(&kv_empty[st]);
-        umma_commit(&pv_done[x]);
+        umma_commit(&pv_done[2 * x + (j & 1)]);
       }
       __syncwarp();
       if (j + 2 < n_tiles && !scores(j + 2)) break;
@@ -547,8 +616,7 @@ int launch_q8_tc(const Q8Params& p, int n_tiles, cudaStream_t stream) {
   auto kernel = attention_q8_tc_kernel<DP, OPT>;
   static cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   CUCA_REQUIRE(configured == cudaSuccess, "attention_q8_tc: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(configured));
-  const int bs_shift = (p.bs & (p.bs - 1)) == 0 ? __builtin_ctz(p.bs) : -1;
-  cuca_launch(kernel, dim3(p.nkv * p.n_splits, n_tiles), dim3(NTHREADS), smem, stream, true, p, bs_shift);
+  cuca_launch(kernel, dim3(p.nkv * p.n_splits, n_tiles), dim3(NTHREADS), smem, stream, true, p);
   CUCA_CHECK_LAUNCH("attention_q8_tc");
   if (p.n_splits > 1) {
     cuca_launch(join_q8_tc_kernel<DP>, dim3(NQ * DP / 8, p.nkv, n_tiles), dim3(ROWS), 0, stream, true, p);
@@ -575,6 +643,7 @@ CUCA_API int cuca_attention_q8_tc(const void* q, int q_stride, void* out, int ou
                "attention_q8_tc: unsupported shape (heads %d/%d, head size %d)", nh, nkv, d);
   CUCA_REQUIRE(bs > 0 && n_blocks > 0 && table_stride > 0, "attention_q8_tc: empty pages or tables");
   CUCA_REQUIRE((((uintptr_t)kpool | (uintptr_t)vpool) & 15) == 0, "attention_q8_tc: pools must be 16-byte aligned");
+  CUCA_REQUIRE((long long)n_blocks * nkv * bs < 0xffffffffll, "attention_q8_tc: more than 2^32 rows in the pools");
   CUCA_REQUIRE(query_tiles == 1 || query_tiles == NQ, "attention_q8_tc: %d query tiles", query_tiles);
   CUCA_REQUIRE(chunk >= 0 && chunk % KEYS == 0 && n_splits >= 1 && (n_splits == 1 || (chunk > 0 && part && ((uintptr_t)part & 15) == 0)),
                "attention_q8_tc: bad shares of the keys");
@@ -588,7 +657,7 @@ CUCA_API int cuca_attention_q8_tc(const void* q, int q_stride, void* out, int ou
   p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E; p.cap = opt->softcap; p.cap_arg = opt->softcap > 0.f ? 2.f * CUCA_LOG2E / opt->softcap : 0.f; p.sink = opt->sink ? 1 : 0;
   p.sink_val = opt->sink ? opt->sink_val : nullptr; p.window = opt->window; p.keep = opt->window > 0 ? opt->keep : 0;
   p.slopes = opt->slopes; p.heads_per_cta = nh / nkv; p.head_parts = 1; p.chunk = n_splits > 1 ? chunk : 0;
-  p.n_splits = n_splits; p.part = part; p.err = err;
+  p.n_splits = n_splits; p.part = part; p.err = err; p.run_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
   const bool extra = p.cap > 0.f || p.sink || p.slopes;
   if (d <= 64) return extra ? launch_q8_tc<64, true>(p, n_tiles, stream) : launch_q8_tc<64, false>(p, n_tiles, stream);
   return extra ? launch_q8_tc<128, true>(p, n_tiles, stream) : launch_q8_tc<128, false>(p, n_tiles, stream);
