@@ -29,7 +29,7 @@ namespace {
 constexpr int ROWS = 128;  // query rows of a tile = lanes of tensor memory
 constexpr int KEYS = 64;   // keys of a tile
 constexpr int NQ = 2;      // query tiles of a block
-constexpr int SOFT_WARPS = 4 * NQ, CONV_WARPS = 4;
+constexpr int SOFT_WARPS = 4 * NQ, CONV_WARPS = 4;  // (8 that convert, with 144 registers for the softmax: a prompt of 2,048 76 us, not 70)
 constexpr int CONV = CONV_WARPS * 32;
 constexpr int NTHREADS = (SOFT_WARPS + CONV_WARPS + 4) * 32;  // softmax, conversion, issue (two warps of four)
 // Registers a thread: 128 at launch, then by role; the sum, 2 x 176 + 88 + 64 over groups of 128 threads, is within the 4 x 128
@@ -87,6 +87,21 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[2][32]) 
       : "r"(taddr) : "memory");
 }
 
+// The same for 32 columns.
+__device__ __forceinline__ void tmem_ld32_done(uint32_t taddr, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31"
+      "}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      :
+        "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr) : "memory");
+}
+
 template <int DP, bool OPT>
 __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Params p) {
   using SH = Shape<DP>;
@@ -102,9 +117,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   uint64_t* kv_full = q_full + NQ;           // [STAGES]
   uint64_t* kv_empty = kv_full + STAGES;     // [STAGES]
   uint64_t* s_full = kv_empty + STAGES;      // [NQ][2]
-  uint64_t* p_full = s_full + 2 * NQ;        // [NQ]
-  uint64_t* pv_done = p_full + NQ;           // [NQ][2]
-  uint32_t* tmem_slot = (uint32_t*)(pv_done + 2 * NQ);
+  // (a warp can be a tile ahead of the others, so even and odd tiles have a barrier each: its two arrivals must not count for one)
+  uint64_t* p_full = s_full + 2 * NQ;        // [NQ][2]
+  uint64_t* pv_done = p_full + 2 * NQ;       // [NQ][2]
+  uint64_t* ahead = pv_done + 2 * NQ;        // the first query tile has handed over its first weights
+  uint32_t* tmem_slot = (uint32_t*)(ahead + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   uint32_t* q_top = tmem_slot + 2;           // the largest magnitude of the block's queries, as bits
 
@@ -144,7 +161,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       mbar_init(&q_full[x], 128);
       mbar_init(&s_full[2 * x], 1);
       mbar_init(&s_full[2 * x + 1], 1);
-      mbar_init(&p_full[x], 4);
+      mbar_init(&p_full[2 * x], 4);
+      mbar_init(&p_full[2 * x + 1], 4);
       mbar_init(&pv_done[2 * x], 1);
       mbar_init(&pv_done[2 * x + 1], 1);
     }
@@ -152,6 +170,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       mbar_init(&kv_full[s], CONV_WARPS);
       mbar_init(&kv_empty[s], nq);
     }
+    mbar_init(ahead, 4);
     *abort_flag = 0;
     *q_top = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -240,85 +259,76 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       const float4 tile_e = kf4[3 * KEYS / 4];  // E, 2^-E, wide
       const int key0 = keys.at(first + j) * KEYS;
       const bool whole = key0 + KEYS - 1 <= least_pos && (p.window <= 0 || key0 >= most_lo || key0 + KEYS <= p.keep);
-      uint32_t raw[2][32];
-      tmem_ld64(tmem_s(x, j) + lane_bits, raw);
-      // scores in log2 units
       const float bias0 = OPT ? slope2 * (float)(key0 - row_pos) : 0.f;
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 kf = kf4[c * 8 + i];
-          const float f[4] = {kf.x, kf.y, kf.z, kf.w};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = 4 * i + 2 * h;
-            float2 s2 = __fmul2_rn(make_float2(__uint_as_float(raw[c][k]), __uint_as_float(raw[c][k + 1])), make_float2(f[2 * h], f[2 * h + 1]));
-            if (OPT) {
-              if (p.cap > 0.f) s2 = make_float2(q8_capped<false>(s2.x, p), q8_capped<false>(s2.y, p));
-              s2 = __fadd2_rn(s2, make_float2(fmaf(slope2, (float)(c * 32 + k), bias0), fmaf(slope2, (float)(c * 32 + k + 1), bias0)));
-            }
-            raw[c][k] = __float_as_uint(s2.x);
-            raw[c][k + 1] = __float_as_uint(s2.y);
-          }
-        }
-      if (tile_e.z != 0.f) {  // a wide tile
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) raw[c][i] = __float_as_uint(__uint_as_float(raw[c][i]) + factor[KEYS + c * 32 + i]);
-      }
-      if (!whole) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int kp = key0 + c * 32 + i;
-            if (!(kp <= row_pos && (kp >= row_lo || kp < p.keep))) raw[c][i] = 0xff800000u;
-          }
-      }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; i += 2)
-          mx4[(i >> 1) & 3] = fmaxf(fmaxf(mx4[(i >> 1) & 3], __uint_as_float(raw[c][i])), __uint_as_float(raw[c][i + 1]));
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) + tile_e.x;
-      const bool moves = mx > m + Q8_LAG;
-      const float corr = moves ? q8_exp2(m - mx) : 1.f;
-      if (moves) m = mx;
-      const float ref = (m == -INFINITY ? 0.f : m - Q8_LIFT) - tile_e.x;
-      const float2 neg2 = make_float2(-ref, -ref);
-      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      // Weights relative to the maximum of the tiles before, with this tile's maximum beside them, so that the exponents need not
+      // wait for it; only where a row exceeds the reference by more than 2^LAG is the tile's row read and worked out again.
+      float corr = 1.f;
+      bool moved = false;
+      float2 sum2[2];
       uint32_t pw[KEYS / 2];
-      auto weights = [&](auto wide) {
+#pragma unroll 1
+      for (;;) {
+        uint32_t raw[2][32];
+        tmem_ld64(tmem_s(x, j) + lane_bits, raw);
+        const float ref = (m == -INFINITY ? 0.f : m - Q8_LIFT) - tile_e.x;
+        const float2 neg2 = make_float2(-ref, -ref);
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        sum2[0] = sum2[1] = make_float2(0.f, 0.f);
+        auto row = [&](auto masked, auto wide) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+          for (int i = 0; i < KEYS / 4; ++i) {
+            const float4 kf = kf4[i];
+            const float f[4] = {kf.x, kf.y, kf.z, kf.w};
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 x2 = __fadd2_rn(make_float2(__uint_as_float(raw[c][2 * e]), __uint_as_float(raw[c][2 * e + 1])), neg2);
-            const float2 u2 = make_float2(q8_exp2(x2.x), q8_exp2(x2.y));
-            if (decltype(wide)::value)
-              sum2[e & 1] = __ffma2_rn(u2, *reinterpret_cast<const float2*>(factor + 2 * KEYS + c * 32 + 2 * e), sum2[e & 1]);
-            else
-              sum2[e & 1] = __fadd2_rn(sum2[e & 1], u2);
-            pw[c * 16 + e] = q8_pack(u2.x, u2.y);
+            for (int h = 0; h < 2; ++h) {
+              const int k = 4 * i + 2 * h;
+              // scores in log2 units
+              float2 s2 = __fmul2_rn(make_float2(__uint_as_float(raw[k / 32][k % 32]), __uint_as_float(raw[k / 32][k % 32 + 1])), make_float2(f[2 * h], f[2 * h + 1]));
+              if (OPT) {
+                if (p.cap > 0.f) s2 = make_float2(q8_capped<false>(s2.x, p), q8_capped<false>(s2.y, p));
+                s2 = __fadd2_rn(s2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
+              }
+              if (decltype(wide)::value) s2 = __fadd2_rn(s2, *reinterpret_cast<const float2*>(factor + KEYS + k));
+              if (decltype(masked)::value) {
+                const int kp = key0 + k;
+                if (!(kp <= row_pos && (kp >= row_lo || kp < p.keep))) s2.x = -INFINITY;
+                if (!(kp + 1 <= row_pos && (kp + 1 >= row_lo || kp + 1 < p.keep))) s2.y = -INFINITY;
+              }
+              const float2 x2 = __fadd2_rn(s2, neg2);
+              const float2 u2 = make_float2(q8_exp2(x2.x), q8_exp2(x2.y));
+              mx4[k / 2 & 3] = fmaxf(fmaxf(mx4[k / 2 & 3], s2.x), s2.y);
+              if (decltype(wide)::value)
+                sum2[h] = __ffma2_rn(u2, *reinterpret_cast<const float2*>(factor + 2 * KEYS + k), sum2[h]);
+              else
+                sum2[h] = __fadd2_rn(sum2[h], u2);
+              pw[k / 2] = q8_pack(u2.x, u2.y);
+            }
           }
-      };
-      if (tile_e.z != 0.f) weights(std::true_type{});
-      else weights(std::false_type{});
+        };
+        if (tile_e.z != 0.f) row(std::true_type{}, std::true_type{});
+        else if (!whole) row(std::true_type{}, std::false_type{});
+        else row(std::false_type{}, std::false_type{});
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) + tile_e.x;
+        const bool moves = mx > m + Q8_LAG;
+        if (!__any_sync(0xffffffffu, moves)) break;
+        if (moves) {
+          corr = q8_exp2(m - mx);
+          m = mx;
+        }
+        moved = true;
+      }
       static_assert(KEYS == 64, "one 32-column store holds a row's weights of a tile");
       __syncwarp();
       tmem_st32_raw(tmem_s(x, j) + lane_bits, pw);
       l = fmaf((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y), tile_e.y, l * corr);
       // O is made smaller where a row's maximum moved; only then must the product before have finished
-      if (j > 0 && __any_sync(0xffffffffu, moves)) {
+      if (j > 0 && moved) {
         if (!product_done(j)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
           float o[32];
-          tmem_ld32(tmem_o(x) + lane_bits + c * 32, o);
+          tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] *= corr;
           tmem_st32(tmem_o(x) + lane_bits + c * 32, o);
@@ -327,7 +337,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x]);
+      if (lane == 0) {
+        mbar_arrive(&p_full[2 * x + (j & 1)]);
+        if (j == 0 && x == 0) mbar_arrive(ahead);
+      }
     }
     if (ok && product_done(n_tiles)) {
       tc_fence_after();
@@ -339,7 +352,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
           float o[32];
-          tmem_ld32(tmem_o(x) + lane_bits + c * 32, o);  // (the whole warp reads)
+          tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);  // (the whole warp reads)
           if (row_ok) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -366,7 +379,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
           float o[32];
-          tmem_ld32(tmem_o(x) + lane_bits + c * 32, o);
+          tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);
 #pragma unroll
           for (int q = 0; q < 8; ++q) dst[(c * 8 + q) * ROWS] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
         }
@@ -385,6 +398,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const int cw = warp - SOFT_WARPS;
     constexpr int ROWS_AT_ONCE = DP == 128 ? 4 : 8;         // of a warp: 16-byte pieces of keys or values
     constexpr int STEP = CONV_WARPS * ROWS_AT_ONCE, PER = KEYS / STEP;
+    // (a warp's rows of a set are all among the tile's first 32 keys or all among its last)
     // Eight lanes that store together have two rows of four pieces, and find eight places.
     const int half = DP == 128 ? lane >> 4 : 0, quad = lane & 3, r0 = cw * ROWS_AT_ONCE + ((lane >> 2) & (ROWS_AT_ONCE - 1));
     const int c = half * 4 + quad;
@@ -424,7 +438,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         if (wrong && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const uint32_t row = __shfl_sync(0xffffffffu, key_row[(i * STEP) / 32], (r0 + i * STEP) & 31);
+          const uint32_t row = __shfl_sync(0xffffffffu, r0 + i * STEP < 32 ? key_row[0] : key_row[1], (r0 + i * STEP) & 31);
           const size_t at = (size_t)(row == NOWHERE ? 0u : row) * p.d + c_at;  // (a key that is not there: zeros, scales 0, masked)
           copy16(to + 2 * i * CONV * 16, p.kpool + at, row != NOWHERE);
           copy16(to + (2 * i + 1) * CONV * 16, p.vpool + at, row != NOWHERE);
@@ -493,7 +507,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       uint8_t* vt = kt + SH::KV_TILE;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const uint32_t times = __shfl_sync(0xffffffffu, factor2[(i * STEP) / 32], (r0 + i * STEP) & 31);
+        const uint32_t times = __shfl_sync(0xffffffffu, r0 + i * STEP < 32 ? factor2[0] : factor2[1], (r0 + i * STEP) & 31);
         const uint4 v = shared_16(from + (2 * i + 1) * CONV * 16);
         const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
         uint32_t h[8];
@@ -516,7 +530,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     constexpr uint32_t idesc_qk = desc_f16(false, KEYS), idesc_pv = desc_f16(true, DP);
     bool ok = x < nq && warp_wait(&q_full[x], 0, p.err, abort_flag);
     // The second query tile starts half a tile behind the first, so that one's exponents run beside the other's maxima and sums.
-    if (ok && x == 1) ok = warp_wait(&p_full[0], 0, p.err, abort_flag);
+    if (ok && x == 1) ok = warp_wait(ahead, 0, p.err, abort_flag);
     const uint64_t q_desc = smem_desc(smem_u32(q_s + x * SH::Q_BYTES));
     const uint32_t kv_at = smem_u32(kv_s);
     auto scores = [&](int t) {
@@ -537,7 +551,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     ok = ok && scores(0) && (n_tiles < 2 || scores(1));
     for (int j = 0; ok && j < n_tiles; ++j) {
       const int st = j % STAGES;
-      if (!warp_wait(&p_full[x], j & 1, p.err, abort_flag)) break;
+      if (!warp_wait(&p_full[2 * x + (j & 1)], (j >> 1) & 1, p.err, abort_flag)) break;
       tc_fence_after();
       const uint64_t vd = desc_mnmajor(kv_at + st * SH::STAGE + SH::KV_TILE, SH::KV_HALF, 1024);
       if (elect_one()) {

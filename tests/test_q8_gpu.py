@@ -371,3 +371,13 @@ def test_a_page_that_is_not_there_is_recorded():
             call()
             assert int(c.err) == 2 and torch.equal(before, c.k)
             c.err.zero_()
+
+
+@pytest.mark.parametrize("heads,kv,dim,counts,starts", [(32, 8, 128, [300], [2000]), (32, 8, 128, [700], [3000]), (8, 2, 64, [200, 90], [700, 1]),
+                                                         (6, 1, 96, [256, 3], [1500, 900])])
+def test_portions_give_the_same_bits_in_every_run(heads, kv, dim, counts, starts):
+    """Warps of a block run apart from one another; what they hand over does not depend on by how much."""
+    c = Case(heads, kv, dim, 16, counts, starts, torch.bfloat16, seed=dim, level=4.0)
+    first = _check(c)
+    for _ in range(60):
+        assert torch.equal(first, _attend(c))
