@@ -270,8 +270,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       for (;;) {
         uint32_t raw[2][32];
         tmem_ld64(tmem_s(x, j) + lane_bits, raw);
-        const float ref = (m == -INFINITY ? 0.f : m - Q8_LIFT) - tile_e.x;
-        const float2 neg2 = make_float2(-ref, -ref);
+        const float ref = m == -INFINITY ? 0.f : m - Q8_LIFT;  // the exponents are z - ref
+        const float2 neg2 = make_float2(tile_e.x - ref, tile_e.x - ref);
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         sum2[0] = sum2[1] = make_float2(0.f, 0.f);
         auto row = [&](auto masked, auto wide) {
@@ -282,21 +282,24 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int k = 4 * i + 2 * h;
-              // scores in log2 units
-              float2 s2 = __fmul2_rn(make_float2(__uint_as_float(raw[k / 32][k % 32]), __uint_as_float(raw[k / 32][k % 32 + 1])), make_float2(f[2 * h], f[2 * h + 1]));
+              float2 x2 = make_float2(__uint_as_float(raw[k / 32][k % 32]), __uint_as_float(raw[k / 32][k % 32 + 1]));
+              const float2 f2 = make_float2(f[2 * h], f[2 * h + 1]);
               if (OPT) {
-                if (p.cap > 0.f) s2 = make_float2(q8_capped<false>(s2.x, p), q8_capped<false>(s2.y, p));
-                s2 = __fadd2_rn(s2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
+                x2 = __fmul2_rn(x2, f2);
+                if (p.cap > 0.f) x2 = make_float2(q8_capped<false>(x2.x, p), q8_capped<false>(x2.y, p));
+                x2 = __fadd2_rn(x2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
+                x2 = __fadd2_rn(x2, neg2);
+              } else {
+                x2 = __ffma2_rn(x2, f2, neg2);
               }
-              if (decltype(wide)::value) s2 = __fadd2_rn(s2, *reinterpret_cast<const float2*>(factor + KEYS + k));
+              if (decltype(wide)::value) x2 = __fadd2_rn(x2, *reinterpret_cast<const float2*>(factor + KEYS + k));
               if (decltype(masked)::value) {
                 const int kp = key0 + k;
-                if (!(kp <= row_pos && (kp >= row_lo || kp < p.keep))) s2.x = -INFINITY;
-                if (!(kp + 1 <= row_pos && (kp + 1 >= row_lo || kp + 1 < p.keep))) s2.y = -INFINITY;
+                if (!(kp <= row_pos && (kp >= row_lo || kp < p.keep))) x2.x = -INFINITY;
+                if (!(kp + 1 <= row_pos && (kp + 1 >= row_lo || kp + 1 < p.keep))) x2.y = -INFINITY;
               }
-              const float2 x2 = __fadd2_rn(s2, neg2);
               const float2 u2 = make_float2(q8_exp2(x2.x), q8_exp2(x2.y));
-              mx4[k / 2 & 3] = fmaxf(fmaxf(mx4[k / 2 & 3], s2.x), s2.y);
+              mx4[k / 2 & 3] = fmaxf(fmaxf(mx4[k / 2 & 3], x2.x), x2.y);
               if (decltype(wide)::value)
                 sum2[h] = __ffma2_rn(u2, *reinterpret_cast<const float2*>(factor + 2 * KEYS + k), sum2[h]);
               else
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         if (tile_e.z != 0.f) row(std::true_type{}, std::true_type{});
         else if (!whole) row(std::true_type{}, std::false_type{});
         else row(std::false_type{}, std::false_type{});
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) + tile_e.x;
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) + ref;
         const bool moves = mx > m + Q8_LAG;
         if (!__any_sync(0xffffffffu, moves)) break;
         if (moves) {
