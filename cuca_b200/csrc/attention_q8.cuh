@@ -71,7 +71,7 @@ __device__ __forceinline__ bool q8_rows_of_tile(const Q8Params& p, int tile, int
   int before = 0;
   for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
     const int s = s0 + lane;
-    const int count = s < p.n_seqs ? p.req_count[s] : 0;
+    const int count = s < p.n_seqs ? p.req_count[s] : 0, first = s < p.n_seqs ? p.req_row0[s] : 0;
     const int tiles = count >= p.count_lo && count <= p.count_hi ? (count + p.tile_tokens - 1) / p.tile_tokens : 0;
     int upto = tiles;
 #pragma unroll
@@ -84,7 +84,7 @@ __device__ __forceinline__ bool q8_rows_of_tile(const Q8Params& p, int tile, int
       const int at = __ffs(past) - 1;
       const int its = __shfl_sync(0xffffffffu, tiles, at), its_count = __shfl_sync(0xffffffffu, count, at);
       const int k = its - 1 - (tile - before - (__shfl_sync(0xffffffffu, upto, at) - its));
-      row0 = p.req_row0[s0 + at] + k * p.tile_tokens;
+      row0 = __shfl_sync(0xffffffffu, first, at) + k * p.tile_tokens;
       n = min(p.tile_tokens, its_count - k * p.tile_tokens);
       return true;
     }

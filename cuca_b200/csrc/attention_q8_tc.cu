@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   const int n_tiles = last - first;
   const int tile_tok = ROWS / G;             // tokens of a query tile
   const int nq = n_tok > tile_tok ? 2 : 1;
+  const uint32_t per_head = (65536u + G - 1) / G;  // a row of a query tile over G: right for up to 128 of both
+  auto token_of = [&](int row) { return (int)(((uint32_t)row * per_head) >> 16); };
 
   if (warp == SOFT_WARPS + CONV_WARPS) {
     tmem_alloc(tmem_slot, TMEM_COLS);
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   }
   if (threadIdx.x == 0) {
     for (int x = 0; x < NQ; ++x) {
-      mbar_init(&q_full[x], 128);
+      mbar_init(&q_full[x], 4);
       mbar_init(&s_full[2 * x], 1);
       mbar_init(&s_full[2 * x + 1], 1);
       mbar_init(&p_full[2 * x], 4);
@@ -188,53 +190,90 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const int x = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;  // row of the query tile
     const uint32_t lane_bits = (uint32_t)(quarter * 32) << 16;
-    const int tok = x * tile_tok + r / G, head = head0 + r % G;
-    const bool row_ok = x < nq && r < tile_tok * G && tok < n_tok;
-    uint4 raw_q[DP / 8];
-    uint32_t top = 0;
+    const int tok = x * tile_tok + token_of(r), head = head0 + r - token_of(r) * G;
+    // The warp's 32 rows of queries: DP / 8 lanes a row, so that a request for them is whole lines.
+    constexpr int LANES = DP / 8, AT_ONCE = 32 / LANES, SETS = 32 / AT_ONCE;
+    const int c = lane % LANES;  // 16 bytes of a row
+    uint32_t* bad_s = q_top + 1;  // [8]: rows that are not finite, a bit each
     {
-      const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + (size_t)(row0 + (row_ok ? tok : 0)) * p.q_stride + (size_t)head * p.d;
+      uint4 raw_q[SETS];
+      uint32_t top = 0, bad_rows = 0;
       const bool aligned = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 8 == 0;
+      auto at = [&](int i, bool& ok) {  // where the lane's piece of set i stands (of rows that are not there: another's)
+        const int row = quarter * 32 + i * AT_ONCE + lane / LANES, t0 = token_of(row), its_tok = x * tile_tok + t0;
+        ok = x < nq && row < tile_tok * G && its_tok < n_tok && c * 8 < p.d;
+        return (const __nv_bfloat16*)p.q + (size_t)(row0 + (ok ? its_tok : 0)) * p.q_stride + (size_t)(head0 + (ok ? row - t0 * G : 0)) * p.d + (ok ? c * 8 : 0);
+      };
+      if (aligned) {
 #pragma unroll
-      for (int c = 0; c < DP / 8; ++c) {
-        raw_q[c] = make_uint4(0u, 0u, 0u, 0u);
-        if (row_ok && c * 8 < p.d) {
-          if (aligned) {
-            raw_q[c] = *reinterpret_cast<const uint4*>(src + c * 8);
+        for (int i = 0; i < SETS; ++i) {
+          bool ok;
+          const uint4 w = *reinterpret_cast<const uint4*>(at(i, ok));
+          raw_q[i] = ok ? w : make_uint4(0u, 0u, 0u, 0u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) {
+          bool ok;
+          const unsigned short* h = reinterpret_cast<const unsigned short*>(at(i, ok));
+          raw_q[i] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+          if (!ok) raw_q[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+      auto top_of = [&](const uint4& q) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = max(m, max((w[k] << 16) & 0x7fffffffu, w[k] & 0x7fff0000u));
+        return m;
+      };
+#pragma unroll
+      for (int i = 0; i < SETS; ++i) top = max(top, top_of(raw_q[i]));
+      if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {
+        // a row that is not finite goes in as zeros and comes out as NaN
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) {
+          const uint32_t its = top_of(raw_q[i]);
+          const uint32_t hit = __ballot_sync(0xffffffffu, its >= 0x7f800000u);
+          const uint32_t mates = (LANES == 32 ? 0xffffffffu : (1u << (LANES & 31)) - 1) << (lane / LANES * LANES);
+          if (hit & mates) {
+            bad_rows |= 1u << (i * AT_ONCE + lane / LANES);
+            raw_q[i] = make_uint4(0u, 0u, 0u, 0u);
           } else {
-            const unsigned short* h = reinterpret_cast<const unsigned short*>(src + c * 8);
-            raw_q[c] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+            top = max(top, its);
           }
         }
-        const uint32_t w[4] = {raw_q[c].x, raw_q[c].y, raw_q[c].z, raw_q[c].w};
+        bad_rows = __reduce_or_sync(0xffffffffu, bad_rows);
+      }
+      // One power of two for the block's rows: what it costs rows much smaller than the largest is far below what a score can
+      // show.
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) {
+        atomicMax(q_top, top);
+        bad_s[warp] = bad_rows;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
+      float up, down;
+      q8_query_scale(*q_top, up, down);
+      if (x < nq) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+        for (int i = 0; i < SETS; ++i) {
+          const int row = quarter * 32 + i * AT_ONCE + lane / LANES;
+          const uint32_t w[4] = {raw_q[i].x, raw_q[i].y, raw_q[i].z, raw_q[i].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            h[k] = q8_pack(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xffff0000u) * up);
+          *reinterpret_cast<uint4*>(q_s + x * SH::Q_BYTES + (c / 8) * SH::Q_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+              make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[x]);
       }
     }
-    // One power of two for the block's rows: what it costs rows much smaller than the largest is far below what a score can
-    // show. A row that is not finite goes in as zeros and comes out as NaN.
-    const bool bad = top >= 0x7f800000u;
-    uint32_t top_w = bad ? 0u : top;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top_w = max(top_w, __shfl_xor_sync(0xffffffffu, top_w, o));
-    if (lane == 0) atomicMax(q_top, top_w);
-    asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
-    float up, down;
-    q8_query_scale(*q_top, up, down);
-    if (x < nq) {
-      uint8_t* dst = q_s + x * SH::Q_BYTES + r * 128;
-#pragma unroll
-      for (int c = 0; c < DP / 8; ++c) {
-        const uint32_t w[4] = {raw_q[c].x, raw_q[c].y, raw_q[c].z, raw_q[c].w};
-        uint32_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          h[i] = bad ? 0u : q8_pack(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
-        *reinterpret_cast<uint4*>(dst + (c / 8) * SH::Q_HALF + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-      }
-      fence_proxy_async();
-      mbar_arrive(&q_full[x]);
-    }
+    const bool bad = (bad_s[warp] >> lane) & 1u;
 
     const int row_pos = pos0 + tok;
     const int row_lo = p.window > 0 ? row_pos - (p.window - 1) : 0;
@@ -350,31 +389,45 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       if (alone) {
         if (OPT && p.sink && m != -INFINITY) l += q8_sink_term(p, head, m);
         const float inv = bad ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : q8_pow2(-V_LIFT) / l;
-        __nv_bfloat16* dst = out + (size_t)(row0 + tok) * p.out_stride + (size_t)head * p.d;
-        const bool aligned = ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0;
+        // Through shared memory, where the queries were (every product that read them is done), so that what is stored is whole
+        // lines; a row's pieces are turned round by its number, as in the operand tiles.
+        uint8_t* mine = q_s + x * SH::Q_BYTES + quarter * 32 * (DP * 2);
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
+        for (int c0 = 0; c0 < DP / 32; ++c0) {
           float o[32];
-          tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);  // (the whole warp reads)
-          if (row_ok) {
+          tmem_ld32_done(tmem_o(x) + lane_bits + c0 * 32, o);  // (the whole warp reads)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if (c * 32 + q * 8 >= p.d) break;
-              uint32_t w[4];
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const __nv_bfloat162 t2 = __floats2bfloat162_rn(o[q * 8 + 2 * i] * inv, o[q * 8 + 2 * i + 1] * inv);
-                w[i] = *reinterpret_cast<const uint32_t*>(&t2);
-              }
-              if (aligned) {
-                *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int i = 0; i < 4; ++i) {
+              const __nv_bfloat162 t2 = __floats2bfloat162_rn(o[q * 8 + 2 * i] * inv, o[q * 8 + 2 * i + 1] * inv);
+              w[i] = *reinterpret_cast<const uint32_t*>(&t2);
+            }
+            *reinterpret_cast<uint4*>(mine + lane * (DP * 2) + (((c0 * 4 + q) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        __syncwarp();
+        const bool aligned = ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0;
+        auto store = [&](auto whole_lines) {
+#pragma unroll
+          for (int i = 0; i < SETS; ++i) {
+            const int its = i * AT_ONCE + lane / LANES, row = quarter * 32 + its, t0 = token_of(row), its_tok = x * tile_tok + t0;
+            const uint4 w = *reinterpret_cast<const uint4*>(mine + its * (DP * 2) + ((c ^ (its & 7)) << 4));
+            __nv_bfloat16* dst = out + (size_t)(row0 + its_tok) * p.out_stride + (size_t)(head0 + row - t0 * G) * p.d + c * 8;
+            if (row < tile_tok * G && its_tok < n_tok && c * 8 < p.d) {
+              if (decltype(whole_lines)::value) {
+                *reinterpret_cast<uint4*>(dst) = w;
               } else {
+                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dst[c * 32 + q * 8 + i] = __ushort_as_bfloat16((unsigned short)(w[i / 2] >> (16 * (i & 1))));
+                for (int k = 0; k < 8; ++k) dst[k] = __ushort_as_bfloat16((unsigned short)(v[k / 2] >> (16 * (k & 1))));
               }
             }
           }
-        }
+        };
+        if (aligned) store(std::true_type{});
+        else store(std::false_type{});
       } else {
         // [NQ][DP / 4][ROWS][4], then m and l [NQ][2][ROWS]: rows side by side
         float* part = p.part + (((size_t)blockIdx.y * p.nkv + kvh) * p.n_splits + split) * (size_t)(NQ * ROWS * (DP + 2));
