@@ -13,6 +13,8 @@
 // Both kernels do a few operations per byte and are bound by memory, or by latency when there are few rows.
 #include "common.cuh"
 
+int cuca_device_sms();
+
 namespace {
 
 constexpr float CUCA_Q8_TINY = 7.888609052210118e-31f;  // 2^-100
@@ -35,7 +37,7 @@ struct StoreParams {
   float* kscale;
   float* vscale;
   int n_blocks, bs, n_rows, nh, nkv, d;
-  int seg;  // lanes of a head: d / 8, rounded up to a power of two
+  int seg_shift;  // log2 of a head's lanes: d / 8, rounded up to a power of two
   int* err;
 };
 
@@ -64,112 +66,131 @@ __device__ __forceinline__ uint32_t codes4(const float (&v)[4], float inv) {
   return w;
 }
 
-// A group of `seg` lanes takes one head of one row; a lane has values 4 l .. 4 l + 3 of each half of the head, which are the
-// rotation's pairs where the whole head is rotated in halves (VEC: 8- or 16-byte accesses). Else (part of the head rotated,
-// neighbours as pairs, rows that are not aligned) the same values are fetched one by one with their partners. A head stays
-// within a warp, and everything is read before anything is written: q_out may be the rows themselves.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(STORE_THREADS) rope_store_q8_kernel(const StoreParams p) {
+// A group of lanes takes one head of a row, of ROWS rows in turn whose loads go out together; a lane has values 4 l .. 4 l + 3 of
+// each half of the head, which are the rotation's pairs where the whole head is rotated in halves (VEC: 8- or 16-byte accesses).
+// Else (part of the head rotated, neighbours as pairs, rows that are not aligned) the same values are fetched one by one with
+// their partners. A head stays within a warp, and everything is read before anything is written: q_out may be the rows
+// themselves.
+template <typename T, bool VEC, int ROWS>
+__global__ void __launch_bounds__(STORE_THREADS, ROWS > 1 ? 4 : 1) rope_store_q8_kernel(const StoreParams p) {
   pdl_trigger();
   pdl_wait();
   const int heads = p.nh + 2 * p.nkv;
-  const long long unit = ((long long)blockIdx.x * STORE_THREADS + threadIdx.x) / p.seg;
-  const int l = threadIdx.x & (p.seg - 1);
-  const int row = (int)(unit / heads), head = (int)(unit % heads);
+  const int head = (int)((blockIdx.x * STORE_THREADS + threadIdx.x) >> p.seg_shift);
+  const int l = threadIdx.x & ((1 << p.seg_shift) - 1);
   const int half = p.d / 2;
-  const bool lane_ok = row < p.n_rows && 4 * l < half;
-  const int seq = row < p.n_rows ? p.seq_of_row[row] : -1;
-  const int pos = seq >= 0 ? p.positions[row] : 0;
+  const bool lane_ok = head < heads && 4 * l < half;
   const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
   const bool rotate = !is_v && p.rot > 0;
-  const bool in_table = pos >= 0 && pos < p.table_rows;
-  const bool live = lane_ok && seq >= 0;
-  float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-  if (live) {
-    if (rotate && !in_table && l == 0 && p.err) atomicExch(p.err, CUCA_ERR_TOKEN_RANGE);
-    const T* src = (const T*)p.qkv + (size_t)row * p.row_stride + (size_t)head * p.d;
-    const float* cr = p.cos_t + (size_t)(in_table ? pos : 0) * (p.rot / 2);
-    const float* sr = p.sin_t + (size_t)(in_table ? pos : 0) * (p.rot / 2);
-    if (VEC) {
-      load4(src + 4 * l, a);
-      load4(src + half + 4 * l, b);
-      if (rotate && in_table) {
-        float c[4], s[4];
-        load4(cr + 4 * l, c);
-        load4(sr + 4 * l, s);
+  const int row0 = blockIdx.y * ROWS;
+  int seq[ROWS], pos[ROWS];
+  bool live[ROWS];
+  float a[ROWS][4], b[ROWS][4], c[VEC ? ROWS : 1][4], s[VEC ? ROWS : 1][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = a[i], y = b[i];
-          a[i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
-          b[i] = __fadd_rn(__fmul_rn(x, s[i]), __fmul_rn(y, c[i]));
-        }
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = row0 + r;
+    seq[r] = row < p.n_rows ? p.seq_of_row[row] : -1;
+    pos[r] = row < p.n_rows ? p.positions[row] : 0;
+    live[r] = lane_ok && seq[r] >= 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[r][i] = b[r][i] = 0.f;
+    if (VEC && lane_ok && row < p.n_rows) {  // (whoever's the row is: its numbers need not be known first)
+      const T* src = (const T*)p.qkv + (size_t)row * p.row_stride + (size_t)head * p.d;
+      load4(src + 4 * l, a[r]);
+      load4(src + half + 4 * l, b[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const bool in_table = pos[r] >= 0 && pos[r] < p.table_rows;
+    const float* cr = p.cos_t + (size_t)(in_table ? pos[r] : 0) * (p.rot / 2);
+    const float* sr = p.sin_t + (size_t)(in_table ? pos[r] : 0) * (p.rot / 2);
+    if (VEC) {
+      if (rotate && lane_ok) {
+        load4(cr + 4 * l, c[VEC ? r : 0]);
+        load4(sr + 4 * l, s[VEC ? r : 0]);
       }
-    } else {
+    } else if (live[r]) {
+      const T* src = (const T*)p.qkv + (size_t)(row0 + r) * p.row_stride + (size_t)head * p.d;
       auto value = [&](int e) {
         const float x = to_f32(src[e]);
         if (!rotate || !in_table || e >= p.rot) return x;
         const int hr = p.rot / 2;
         const int i = p.adjacent ? e / 2 : (e < hr ? e : e - hr);
         const bool first = p.adjacent ? (e & 1) == 0 : e < hr;
-        const float c = cr[i], s = sr[i];
+        const float cs = cr[i], sn = sr[i];
         const float y = to_f32(src[p.adjacent ? e ^ 1 : (first ? e + hr : i)]);
-        return first ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)) : __fadd_rn(__fmul_rn(y, s), __fmul_rn(x, c));
+        return first ? __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn)) : __fadd_rn(__fmul_rn(y, sn), __fmul_rn(x, cs));
       };
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { a[i] = value(4 * l + i); b[i] = value(half + 4 * l + i); }
+      for (int i = 0; i < 4; ++i) { a[r][i] = value(4 * l + i); b[r][i] = value(half + 4 * l + i); }
     }
   }
-  // the largest magnitude of the head, as bits: anything not finite compares above every number
-  uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    top = max(top, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
-  for (int o = p.seg >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));  // (also: all has been read)
-  if (!live) return;
-  if (is_q) {
-    T* dst = (T*)p.q_out + (size_t)row * p.q_stride + (size_t)head * p.d;
-    if (VEC) {
-      store4(dst + 4 * l, a);
-      store4(dst + half + 4 * l, b);
+  for (int r = 0; r < ROWS; ++r) {
+    const bool in_table = pos[r] >= 0 && pos[r] < p.table_rows;
+    if (rotate && live[r] && !in_table && l == 0 && p.err) atomicExch(p.err, CUCA_ERR_TOKEN_RANGE);
+    if (VEC && rotate && in_table) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = a[r][i], y = b[r][i], cs = c[VEC ? r : 0][i], sn = s[VEC ? r : 0][i];
+        a[r][i] = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
+        b[r][i] = __fadd_rn(__fmul_rn(x, sn), __fmul_rn(y, cs));
+      }
+    }
+    // the largest magnitude of the head, as bits: anything not finite compares above every number
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      top = max(top, max(__float_as_uint(a[r][i]) & 0x7fffffffu, __float_as_uint(b[r][i]) & 0x7fffffffu));
+    for (int o = (1 << p.seg_shift) >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));  // (and all has been read)
+    if (!live[r]) continue;
+    const int row = row0 + r;
+    if (is_q) {
+      T* dst = (T*)p.q_out + (size_t)row * p.q_stride + (size_t)head * p.d;
+      if (VEC) {
+        store4(dst + 4 * l, a[r]);
+        store4(dst + half + 4 * l, b[r]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { dst[4 * l + i] = from_f32<T>(a[r][i]); dst[half + 4 * l + i] = from_f32<T>(b[r][i]); }
+      }
+      continue;
+    }
+    const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
+    const int entry = pos[r] / p.bs;
+    const int blk = pos[r] >= 0 && entry < p.table_stride ? p.tables[(size_t)seq[r] * p.table_stride + entry] : -1;
+    if (blk < 0 || blk >= p.n_blocks) {
+      if (l == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+      continue;
+    }
+    const size_t at = ((size_t)blk * p.nkv + kvh) * p.bs + pos[r] % p.bs;
+    const float most = __uint_as_float(top);
+    float scale, inv;
+    if (top >= 0x7f800000u) {
+      scale = __uint_as_float(0x7fc00000u);
+      inv = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[r][i] = b[r][i] = 0.f;
+    } else if (most < CUCA_Q8_TINY) {
+      scale = inv = 0.f;
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { dst[4 * l + i] = from_f32<T>(a[i]); dst[half + 4 * l + i] = from_f32<T>(b[i]); }
+      scale = __fdiv_rn(most, 127.f);
+      inv = __fdiv_rn(127.f, most);
     }
-    return;
+    int8_t* dst = (is_v ? p.vpool : p.kpool) + at * p.d;
+    *reinterpret_cast<uint32_t*>(dst + 4 * l) = codes4(a[r], inv);
+    *reinterpret_cast<uint32_t*>(dst + half + 4 * l) = codes4(b[r], inv);
+    if (l == 0) (is_v ? p.vscale : p.kscale)[at] = scale;
   }
-  const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
-  const int entry = pos / p.bs;
-  const int blk = pos >= 0 && entry < p.table_stride ? p.tables[(size_t)seq * p.table_stride + entry] : -1;
-  if (blk < 0 || blk >= p.n_blocks) {
-    if (l == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
-    return;
-  }
-  const size_t at = ((size_t)blk * p.nkv + kvh) * p.bs + pos % p.bs;
-  const float most = __uint_as_float(top);
-  float scale, inv;
-  if (top >= 0x7f800000u) {
-    scale = __uint_as_float(0x7fc00000u);
-    inv = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = b[i] = 0.f;
-  } else if (most < CUCA_Q8_TINY) {
-    scale = inv = 0.f;
-  } else {
-    scale = __fdiv_rn(most, 127.f);
-    inv = __fdiv_rn(127.f, most);
-  }
-  int8_t* dst = (is_v ? p.vpool : p.kpool) + at * p.d;
-  *reinterpret_cast<uint32_t*>(dst + 4 * l) = codes4(a, inv);
-  *reinterpret_cast<uint32_t*>(dst + half + 4 * l) = codes4(b, inv);
-  if (l == 0) (is_v ? p.vscale : p.kscale)[at] = scale;
 }
 
 // ------------------------------------------------------------------ reading back
-constexpr int READ_THREADS = 256, READ_UNROLL = 4;
+constexpr int READ_WARPS = 8, READ_ROWS = 4, READ_PIECES = 4;
 
 template <typename T> struct Piece;  // what a thread writes at once: 16 bytes
-template <> struct Piece<float> { static constexpr int N = 4; };
-template <> struct Piece<__nv_bfloat16> { static constexpr int N = 8; };
+template <> struct Piece<float> { static constexpr int N = 4; using Codes = uint32_t; };
+template <> struct Piece<__nv_bfloat16> { static constexpr int N = 8; using Codes = uint2; };
 
 struct ReadParams {
   const int8_t* pool[2];
@@ -179,68 +200,86 @@ struct ReadParams {
   const int* positions;
   const int* seq_of_row;
   const int* tables;
-  int table_stride, n_blocks, bs, n_rows, nkv, d, rows_per_block;
+  int table_stride, n_blocks, bs, n_rows, nkv, d;
   int* err;
 };
 
-// A block takes `rows_per_block` rows of one tensor; a thread writes 16 bytes at a time, four of them requested together.
+__device__ __forceinline__ uint32_t word_of(uint32_t w, int) { return w; }
+__device__ __forceinline__ uint32_t word_of(const uint2& w, int i) { return i == 0 ? w.x : w.y; }
+
+// A warp brings READ_PIECES x 32 pieces of a row, of one tensor, for READ_ROWS rows whose loads go out together: a lane's places in
+// the page and in the row are the same for all of them. gridDim: rows, pieces, tensors.
 template <typename T>
-__global__ void __launch_bounds__(READ_THREADS) read_q8_kernel(const ReadParams p) {
+__global__ void __launch_bounds__(READ_WARPS * 32) read_q8_kernel(const __grid_constant__ ReadParams p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int N = Piece<T>::N;
-  const int which = blockIdx.y;
-  T* out = (T*)p.out[which];
+  using P = Piece<T>;
+  constexpr int N = P::N;
+  const bool values = blockIdx.z != 0;
+  T* out = (T*)(values ? p.out[1] : p.out[0]);
   if (!out) return;
-  const int8_t* pool = p.pool[which];
-  const float* scales = p.scale[which];
-  const int row0 = blockIdx.x * p.rows_per_block;
-  const unsigned per_head = p.d / N, per_row = per_head * p.nkv;
-  const unsigned total = per_row * (unsigned)min(p.rows_per_block, p.n_rows - row0);
-  for (unsigned first = threadIdx.x; first < total; first += READ_THREADS * READ_UNROLL) {
-    uint2 w[READ_UNROLL];
-    float s[READ_UNROLL];
-    T* dst[READ_UNROLL];
+  const int8_t* pool = values ? p.pool[1] : p.pool[0];
+  const float* scales = values ? p.scale[1] : p.scale[0];
+  const int stride = values ? p.out_stride[1] : p.out_stride[0];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_head = p.d / N, per_row = per_head * p.nkv;
+  int head[READ_PIECES], e[READ_PIECES];  // of the lane's pieces: key head (-1: none), first value
 #pragma unroll
-    for (int u = 0; u < READ_UNROLL; ++u) {
-      const unsigned idx = first + u * READ_THREADS;
-      dst[u] = nullptr;
-      if (idx >= total) continue;
-      const int row = row0 + (int)(idx / per_row);
-      const unsigned rest = idx % per_row;
-      const int kvh = (int)(rest / per_head), e = (int)(rest % per_head) * N;
-      dst[u] = out + (size_t)row * p.out_stride[which] + (size_t)kvh * p.d + e;
-      w[u] = make_uint2(0u, 0u);
-      s[u] = 0.f;
-      const int seq = p.seq_of_row[row];
-      if (seq < 0) continue;  // a row of no request: zeros
-      const int pos = p.positions[row], entry = pos / p.bs;
-      const int blk = pos >= 0 && entry < p.table_stride ? p.tables[(size_t)seq * p.table_stride + entry] : -1;
-      if (blk < 0 || blk >= p.n_blocks) {
-        if (p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
-        continue;
+  for (int i = 0; i < READ_PIECES; ++i) {
+    const int piece = (blockIdx.y * READ_PIECES + i) * 32 + lane;
+    head[i] = piece < per_row ? piece / per_head : -1;
+    e[i] = (piece - max(head[i], 0) * per_head) * N;
+  }
+  const int row0 = (blockIdx.x * READ_WARPS + warp) * READ_ROWS;
+  int seq[READ_ROWS], pos[READ_ROWS], blk[READ_ROWS];
+#pragma unroll
+  for (int r = 0; r < READ_ROWS; ++r) {
+    seq[r] = row0 + r < p.n_rows ? p.seq_of_row[row0 + r] : -1;
+    pos[r] = row0 + r < p.n_rows ? p.positions[row0 + r] : 0;
+  }
+#pragma unroll
+  for (int r = 0; r < READ_ROWS; ++r) {
+    const int entry = pos[r] / p.bs;
+    blk[r] = seq[r] >= 0 && pos[r] >= 0 && entry < p.table_stride ? p.tables[(size_t)seq[r] * p.table_stride + entry] : -1;
+  }
+  typename P::Codes w[READ_ROWS][READ_PIECES];
+  float s[READ_ROWS][READ_PIECES];
+#pragma unroll
+  for (int r = 0; r < READ_ROWS; ++r) {
+    const bool there = blk[r] >= 0 && blk[r] < p.n_blocks;
+    if (!there && seq[r] >= 0 && lane == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+    const size_t at = (size_t)(there ? blk[r] : 0) * p.nkv * p.bs + (there ? pos[r] % p.bs : 0);
+#pragma unroll
+    for (int i = 0; i < READ_PIECES; ++i) {
+      w[r][i] = typename P::Codes{};
+      s[r][i] = 0.f;  // (a row of no request, or without a page: zeros)
+      if (there && head[i] >= 0) {
+        const size_t row = at + (size_t)head[i] * p.bs;
+        s[r][i] = __ldg(scales + row);
+        w[r][i] = __ldg(reinterpret_cast<const typename P::Codes*>(pool + row * p.d + e[i]));
       }
-      const size_t at = ((size_t)blk * p.nkv + kvh) * p.bs + pos % p.bs;
-      s[u] = scales[at];
-      if (N == 8) w[u] = *reinterpret_cast<const uint2*>(pool + at * p.d + e);
-      else w[u].x = *reinterpret_cast<const uint32_t*>(pool + at * p.d + e);
     }
+  }
 #pragma unroll
-    for (int u = 0; u < READ_UNROLL; ++u) {
-      if (!dst[u]) continue;
+  for (int r = 0; r < READ_ROWS; ++r) {
+    if (row0 + r >= p.n_rows) break;
+#pragma unroll
+    for (int i = 0; i < READ_PIECES; ++i) {
+      if (head[i] < 0) continue;
       float v[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = (float)(int8_t)((i < 4 ? w[u].x : w[u].y) >> (8 * (i & 3))) * s[u];
+      for (int n = 0; n < N; ++n) v[n] = (float)(int8_t)(word_of(w[r][i], n / 4) >> (8 * (n & 3))) * s[r][i];
+      T* dst = out + (size_t)(row0 + r) * stride + (size_t)head[i] * p.d + e[i];
       if constexpr (N == 4) {
-        *reinterpret_cast<float4*>(dst[u]) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
         uint32_t o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-          o[i] = *reinterpret_cast<uint32_t*>(&t);
+        for (int n = 0; n < 4; ++n) {
+          __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * n], v[2 * n + 1]);
+          o[n] = *reinterpret_cast<uint32_t*>(&t);
         }
-        *reinterpret_cast<uint4*>(dst[u]) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
   }
@@ -262,17 +301,21 @@ CUCA_API int cuca_rope_store_q8(const void* qkv, int row_stride, void* q_out, in
   CUCA_REQUIRE(((uintptr_t)kpool & 3) == 0 && ((uintptr_t)vpool & 3) == 0, "rope_store_q8: pools must be 4-byte aligned");
   if (n_rows == 0) return 0;
   StoreParams p{qkv, row_stride, q_out, q_stride, positions, seq_of_row, tables, table_stride, cos_t, sin_t, table_rows, rot,
-                adjacent, (int8_t*)kpool, (int8_t*)vpool, kscale, vscale, n_blocks, bs, n_rows, nh, nkv, d, 1, err};
-  while (p.seg * 8 < d) p.seg *= 2;
-  const long long threads = (long long)n_rows * (nh + 2 * nkv) * p.seg;
-  const long long blocks = (threads + STORE_THREADS - 1) / STORE_THREADS;
-  CUCA_REQUIRE(blocks < (1ll << 31), "rope_store_q8: too many rows");
+                adjacent, (int8_t*)kpool, (int8_t*)vpool, kscale, vscale, n_blocks, bs, n_rows, nh, nkv, d, 0, err};
+  while ((8 << p.seg_shift) < d) ++p.seg_shift;
   const uintptr_t align = dtype == CUCA_F32 ? 15 : 7;
-  const bool vec = (rot == d || rot == 0) && !adjacent && d % 8 == 0 && row_stride % 4 == 0 && q_stride % 4 == 0 &&
+  const bool vec = (rot == d || rot == 0) && !adjacent && row_stride % 4 == 0 && q_stride % 4 == 0 &&
                    (((uintptr_t)qkv | (uintptr_t)q_out) & align) == 0 && (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15) == 0;
-  auto kernel = dtype == CUCA_F32 ? (vec ? rope_store_q8_kernel<float, true> : rope_store_q8_kernel<float, false>)
-                                  : (vec ? rope_store_q8_kernel<__nv_bfloat16, true> : rope_store_q8_kernel<__nv_bfloat16, false>);
-  cuca_launch(kernel, dim3((unsigned)blocks), dim3(STORE_THREADS), 0, stream, true, p);
+  const unsigned blocks = (unsigned)((((long long)(nh + 2 * nkv) << p.seg_shift) + STORE_THREADS - 1) / STORE_THREADS);
+  // two rows a thread where that still fills the GPU with threads
+  const bool many = vec && (long long)blocks * n_rows >= 8ll * 2 * cuca_device_sms();
+  const int per = many ? 2 : 1;
+  CUCA_REQUIRE((n_rows + per - 1) / per <= 65535, "rope_store_q8: too many rows");
+  auto kernel = dtype == CUCA_F32
+      ? (many ? rope_store_q8_kernel<float, true, 2> : vec ? rope_store_q8_kernel<float, true, 1> : rope_store_q8_kernel<float, false, 1>)
+      : (many ? rope_store_q8_kernel<__nv_bfloat16, true, 2> : vec ? rope_store_q8_kernel<__nv_bfloat16, true, 1>
+                                                                  : rope_store_q8_kernel<__nv_bfloat16, false, 1>);
+  cuca_launch(kernel, dim3(blocks, (n_rows + per - 1) / per), dim3(STORE_THREADS), 0, stream, true, p);
   CUCA_CHECK_LAUNCH("rope_store_q8");
   return 0;
 }
@@ -291,12 +334,12 @@ CUCA_API int cuca_read_q8(const void* kpool, const void* vpool, const float* ksc
                (((uintptr_t)kpool | (uintptr_t)vpool) & 7) == 0, "read_q8: rows must start on 16 bytes, pools on 8");
   if (n_rows == 0 || (!k_out && !v_out)) return 0;
   ReadParams p{{(const int8_t*)kpool, (const int8_t*)vpool}, {kscale, vscale}, {k_out, v_out}, {k_stride, v_stride}, positions,
-               seq_of_row, tables, table_stride, n_blocks, bs, n_rows, nkv, d, 1, err};
+               seq_of_row, tables, table_stride, n_blocks, bs, n_rows, nkv, d, err};
   const int pieces = nkv * d / n;  // of a row
-  p.rows_per_block = READ_THREADS * READ_UNROLL / pieces > 1 ? READ_THREADS * READ_UNROLL / pieces : 1;
-  const int blocks = (n_rows + p.rows_per_block - 1) / p.rows_per_block;
+  const dim3 grid((n_rows + READ_WARPS * READ_ROWS - 1) / (READ_WARPS * READ_ROWS), (pieces + 32 * READ_PIECES - 1) / (32 * READ_PIECES), 2);
+  CUCA_REQUIRE(grid.y <= 65535, "read_q8: too many heads");
   auto kernel = dtype == CUCA_F32 ? read_q8_kernel<float> : read_q8_kernel<__nv_bfloat16>;
-  cuca_launch(kernel, dim3(blocks, 2), dim3(READ_THREADS), 0, stream, true, p);
+  cuca_launch(kernel, grid, dim3(READ_WARPS * 32), 0, stream, true, p);
   CUCA_CHECK_LAUNCH("read_q8");
   return 0;
 }
