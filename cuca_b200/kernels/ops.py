@@ -1558,17 +1558,22 @@ class QuantizedPages:
         return cls(*(torch.zeros(shape, dtype=torch.int8, device=device) for _ in range(2)),
                    *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
 
-    def check(self, n_kv_heads: int, head_dim: int) -> None:
-        shape = self.k.shape
-        if len(shape) != 4 or shape[1] != n_kv_heads or shape[3] != head_dim or self.v.shape != shape \
-                or self.k_scale.shape != shape[:3] or self.v_scale.shape != shape[:3]:
+    def check(self, n_kv_heads: int, head_dim: int) -> tuple:
+        """Refuses pages of another shape, type or layout; (codes of keys, of values, their scales' addresses, pages, positions of
+        a page)."""
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        shape = k.shape
+        if len(shape) != 4 or shape[1] != n_kv_heads or shape[3] != head_dim or v.shape != shape or ks.shape != shape[:3] \
+                or vs.shape != ks.shape:
             raise library.KernelError(f"8-bit pages of {n_kv_heads} heads of {head_dim}: codes are [pages, heads, positions, head "
-                                      f"size], scales the same without the last; given {tuple(shape)}, {tuple(self.v.shape)}, "
-                                      f"{tuple(self.k_scale.shape)}, {tuple(self.v_scale.shape)}")
-        for t, dtype in ((self.k, torch.int8), (self.v, torch.int8), (self.k_scale, torch.float32), (self.v_scale, torch.float32)):
-            if t.dtype != dtype or not t.is_contiguous():
-                raise library.KernelError("8-bit pages are contiguous int8 codes and contiguous float32 scales")
-        _cuda(self.k, self.v, self.k_scale, self.v_scale)
+                                      f"size], scales the same without the last; given {tuple(shape)}, {tuple(v.shape)}, "
+                                      f"{tuple(ks.shape)}, {tuple(vs.shape)}")
+        if not (k.dtype == v.dtype == torch.int8 and ks.dtype == vs.dtype == torch.float32 and k.is_contiguous()
+                and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+            raise library.KernelError("8-bit pages are contiguous int8 codes and contiguous float32 scales")
+        if not (k.is_cuda and v.is_cuda and ks.is_cuda and vs.is_cuda):
+            _cuda(k, v, ks, vs)
+        return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), shape[0], shape[2]
 
 
 Q8_MAX_HEAD_DIM = 256
@@ -1584,17 +1589,23 @@ def _q8_head_dim(head_dim: int) -> None:
         raise library.KernelError(f"8-bit pages take head sizes that are multiples of 16 up to {Q8_MAX_HEAD_DIM}, not {head_dim}")
 
 
-def _ints(n, *tensors) -> None:
-    """32-bit whole numbers on the device, `n` of them at least (None: of any number), without gaps."""
-    for t in tensors:
+def _ints(t, n: int = 0) -> int:
+    """The address of 32-bit whole numbers on the device, `n` of them at least, without gaps."""
+    if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
+        raise library.KernelError("positions, slots and page tables are contiguous int32 tensors, one number per row")
+    if not t.is_cuda:
         _cuda(t)
-        if t.dtype != torch.int32 or not t.is_contiguous() or (n is not None and t.numel() < n):
-            raise library.KernelError("positions, slots and page tables are contiguous int32 tensors, one number per row")
+    return t.data_ptr()
 
 
-def _rows(t, n_rows: int, width: int, what: str) -> None:
-    if t.dim() != 2 or t.shape[0] != n_rows or t.shape[1] < width or (t.stride(1) != 1 and width > 1):
-        raise library.KernelError(f"{what} are [{n_rows}, {width} or more] with contiguous rows, not {tuple(t.shape)}")
+def _rows(t, n_rows: int, width: int, what: str) -> int:
+    """The address of `n_rows` rows of `width` values, with any stride between them."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != n_rows or shape[1] < width or t.stride(1) != 1:
+        raise library.KernelError(f"{what} are [{n_rows}, {width} or more] with contiguous rows, not {tuple(shape)}")
+    if not t.is_cuda:
+        _cuda(t)
+    return t.data_ptr()
 
 
 def rope_store_q8(qkv, q_out, positions, seq_of_row, tables, cos, sin, rotary_dim, pages: QuantizedPages, n_heads, n_kv_heads,
@@ -1602,26 +1613,25 @@ def rope_store_q8(qkv, q_out, positions, seq_of_row, tables, cos, sin, rotary_di
     """Rows q | k | v: q, rotated, into `q_out` (which may be the rows themselves), k, rotated, and v quantised into their
     pages. The first `rotary_dim` values of a head are rotated (cos None: none), in halves or as neighbouring pairs. A row that is
     not finite reads back as NaN. Rows with seq_of_row < 0 are left out."""
-    _cuda(qkv, q_out, cos, sin)
     code, n = dtype_code(qkv.dtype), qkv.shape[0]
     _q8_head_dim(head_dim)
-    pages.check(n_kv_heads, head_dim)
-    _rows(qkv, n, (n_heads + 2 * n_kv_heads) * head_dim, "projected rows")
-    _rows(q_out, n, n_heads * head_dim, "rotated queries")
+    k, v, ks, vs, n_pages, bs = pages.check(n_kv_heads, head_dim)
+    src = _rows(qkv, n, (n_heads + 2 * n_kv_heads) * head_dim, "projected rows")
+    dst = _rows(q_out, n, n_heads * head_dim, "rotated queries")
     if q_out.dtype != qkv.dtype:
         raise library.KernelError(f"rotated queries have the rows' dtype {qkv.dtype}, not {q_out.dtype}")
-    _ints(n, positions, seq_of_row)
-    _ints(None, tables)
-    rot = int(rotary_dim) if cos is not None else 0
+    rot = table_rows = 0
     if cos is not None:
-        for x in (cos, sin):
-            if x is None or x.dtype != torch.float32 or not x.is_contiguous() or x.shape != cos.shape or x.shape[1] * 2 != rot:
-                raise library.KernelError(f"cosines and sines are contiguous float32 [positions, {rot // 2}]")
+        rot = int(rotary_dim)
+        if sin is None or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2 \
+                or cos.shape[1] * 2 != rot or not cos.is_contiguous() or not sin.is_contiguous():
+            raise library.KernelError(f"cosines and sines are contiguous float32 [positions, {rot // 2}]")
+        _cuda(cos, sin)
+        table_rows = cos.shape[0]
     library.check(library.load().cuca_rope_store_q8(
-        _p(qkv), qkv.stride(0), _p(q_out), q_out.stride(0), code, _p(positions), _p(seq_of_row), _p(tables), tables.shape[1],
-        _p(cos), _p(sin), cos.shape[0] if cos is not None else 0, rot, int(bool(adjacent)), _p(pages.k), _p(pages.v),
-        _p(pages.k_scale), _p(pages.v_scale), pages.k.shape[0], pages.k.shape[2], n, n_heads, n_kv_heads, head_dim, _p(err),
-        _stream()), "rope_store_q8")
+        src, qkv.stride(0), dst, q_out.stride(0), code, _ints(positions, n), _ints(seq_of_row, n), _ints(tables), tables.shape[1],
+        _p(cos), _p(sin), table_rows, rot, 1 if adjacent else 0, k, v, ks, vs, n_pages, bs, n, n_heads, n_kv_heads, head_dim,
+        _p(err), _stream()), "rope_store_q8")
 
 
 def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, err) -> None:
@@ -1629,23 +1639,26 @@ def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, 
     position positions[r] of the request with page table seq_of_row[r]; zeros where seq_of_row < 0."""
     nkv, d, n = pages.k.shape[1], pages.k.shape[3], positions.shape[0]
     _q8_head_dim(d)
-    pages.check(nkv, d)
-    outs = [t for t in (k_out, v_out) if t is not None]
-    if not outs:
+    k, v, ks, vs, n_pages, bs = pages.check(nkv, d)
+    some = k_out if k_out is not None else v_out
+    if some is None:
         return
-    _cuda(*outs)
-    for t in outs:
-        if t.shape != (n, nkv, d) or t.dtype != outs[0].dtype or t.stride(2) != 1 or t.stride(1) != d:
+    dtype, at = some.dtype, []
+    for t in (k_out, v_out):
+        if t is None:
+            at += (None, 0)
+            continue
+        strides = t.stride()
+        if t.shape != (n, nkv, d) or t.dtype != dtype or strides[2] != 1 or strides[1] != d:
             raise library.KernelError(f"rows read back are [{n}, {nkv}, {d}], contiguous but for the rows' stride and of one dtype")
-    _ints(n, positions, seq_of_row)
-    _ints(None, tables)
-    library.check(library.load().cuca_read_q8(
-        _p(pages.k), _p(pages.v), _p(pages.k_scale), _p(pages.v_scale), pages.k.shape[0], pages.k.shape[2], _p(positions),
-        _p(seq_of_row), _p(tables), tables.shape[1], _p(k_out), 0 if k_out is None else k_out.stride(0), _p(v_out),
-        0 if v_out is None else v_out.stride(0), dtype_code(outs[0].dtype), n, nkv, d, _p(err), _stream()), "read_q8")
+        if not t.is_cuda:
+            _cuda(t)
+        at += (t.data_ptr(), strides[0])
+    library.check(library.load().cuca_read_q8(k, v, ks, vs, n_pages, bs, _ints(positions, n), _ints(seq_of_row, n), _ints(tables),
+                                              tables.shape[1], *at, dtype_code(dtype), n, nkv, d, _p(err), _stream()), "read_q8")
 
 
-Q8_FEW_ROWS = 32  # query rows of a key head that the form for few rows takes of a portion
+Q8_FEW_ROWS = 16  # query rows of a key head that the form for few rows takes of a portion
 
 
 class QuantizedPlan:
@@ -1661,7 +1674,30 @@ class QuantizedPlan:
             self.lengths = [int(s) + c for s, c in zip(step.host["starts"], self.counts)]
         self.all_single = all(c == 1 for c in self.counts)
         self.longest = max(self.counts, default=0)
+        self._arrays = self._addresses = None
         self._launches: dict = {}
+        self._options: dict = {}
+
+    def arrays(self, step) -> tuple:
+        """The addresses of the step's positions, slots, first rows and counts, checked once per step."""
+        a = self._arrays
+        if a is None or a[0] is not step.positions or a[1] is not step.seq_of_row or a[2] is not step.req_row0 \
+                or a[3] is not step.req_count:
+            n, m = step.n_rows, step.n_seqs
+            self._addresses = (_ints(step.positions, n), _ints(step.seq_of_row, n)), \
+                (_ints(step.req_row0, m), None if self.all_single else _ints(step.req_count, m), m)
+            self._arrays = step.positions, step.seq_of_row, step.req_row0, step.req_count
+        return self._addresses
+
+    def options(self, n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes) -> AttentionOptions:
+        """`attention_options`, kept for the other layers of the step where they point to nothing."""
+        if sink_values is not None or slopes is not None:
+            return attention_options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
+        key = (scale, window, softcap, sink, keep_first)
+        opt = self._options.get(key)
+        if opt is None:
+            opt = self._options[key] = attention_options(n_heads, scale, window, softcap, sink, None, keep_first)
+        return opt
 
     def launches(self, n_heads, n_kv_heads, head_dim, dtype, window, keep):
         """[(form, least count, most count, rows of a tile, tiles, heads of a block, column tiles, keys of a share, shares)];
@@ -1673,8 +1709,9 @@ class QuantizedPlan:
                 few = Q8_FEW_ROWS // group
             if 1 in self.counts:
                 out.append(self._few(1, 1, *key))
-            if any(1 < c <= few for c in self.counts):
-                out.append(self._few(2, few, *key))
+            most = max((c for c in self.counts if c <= few), default=0)
+            if most > 1:
+                out.append(self._few(2, most, *key))
             if self.longest > max(few, 1):
                 out.append(self._many(max(few, 1) + 1, self.longest, *key))
             self._launches[key] = out
@@ -1752,27 +1789,24 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
     [rows, heads * head_dim] in q's dtype (bfloat16 or float32). `step` describes the rows (`StepBatch`: positions, seq_of_row,
     req_row0, req_count, counts and starts on the host). Rows of no request (seq_of_row < 0) get zeros. The other options: see
     `attention_options`."""
-    _cuda(q, out, tables)
     code, n = dtype_code(q.dtype), step.n_rows
     _q8_head_dim(head_dim)
     if n_kv_heads < 1 or n_heads % n_kv_heads:
         raise library.KernelError(f"{n_kv_heads} key heads must divide {n_heads} query heads")
-    pages.check(n_kv_heads, head_dim)
-    _rows(q, n, n_heads * head_dim, "queries")
-    _rows(out, n, n_heads * head_dim, "results")
+    pool = pages.check(n_kv_heads, head_dim)
+    src, dst = _rows(q, n, n_heads * head_dim, "queries"), _rows(out, n, n_heads * head_dim, "results")
     if out.dtype != q.dtype:
         raise library.KernelError(f"results have the queries' dtype {q.dtype}, not {out.dtype}")
-    _ints(n, step.positions, step.seq_of_row)
-    _ints(step.n_seqs, step.req_row0)
-    _ints(None, tables)
     if window is not None and window < 0 or keep_first < 0 or softcap < 0:
         raise library.KernelError("a window, kept first keys and a score cap are not negative")
     plan = attention_q8_plan(step)
-    opt = attention_options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
-    lib = library.load()
-    rows = (_p(pages.k), _p(pages.v), _p(pages.k_scale), _p(pages.v_scale), pages.k.shape[0], pages.k.shape[2], _p(step.positions),
-            _p(step.seq_of_row), _p(tables), tables.shape[1], _p(step.req_row0), None if plan.all_single else _p(step.req_count),
-            step.n_seqs)
+    opt = plan.options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
+    at = ctypes.addressof(opt)
+    lib, stream, e = library.load(), _stream(), _p(err)
+    of_rows, of_requests = plan.arrays(step)
+    rows = (*pool, *of_rows, _ints(tables), tables.shape[1], *of_requests)
+    qs, os_ = q.stride(0), out.stride(0)
+    group = n_heads // n_kv_heads
     for form, lo, hi, tokens, tiles, heads, nt, share, shares in plan.launches(n_heads, n_kv_heads, head_dim, q.dtype, window or None,
                                                                                opt.keep):
         part = None
@@ -1780,14 +1814,12 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
             if shares > 1:
                 part = torch.empty(tiles * n_kv_heads * shares * (256 * (64 if head_dim <= 64 else 128) + 512), dtype=torch.float32,
                                    device=q.device)
-            library.check(lib.cuca_attention_q8_tc(_p(q), q.stride(0), _p(out), out.stride(0), *rows, lo, hi, nt, tiles, n_heads,
-                                                   n_kv_heads, head_dim, ctypes.addressof(opt), share, shares, _p(part), _p(err),
-                                                   _stream()), "attention_q8")
+            library.check(lib.cuca_attention_q8_tc(src, qs, dst, os_, *rows, lo, hi, nt, tiles, n_heads, n_kv_heads, head_dim, at, share,
+                                                   shares, _p(part), e, stream), "attention_q8")
             continue
         if shares > 1:
             cols = 8 * nt // (2 if code == F32 else 1)
-            part = torch.empty(tiles * n_kv_heads * -(-(n_heads // n_kv_heads) // heads) * shares * cols * (head_dim + 2),
-                               dtype=torch.float32, device=q.device)
-        library.check(lib.cuca_attention_q8(_p(q), q.stride(0), _p(out), out.stride(0), code, *rows, lo, hi, tokens, tiles, n_heads,
-                                            n_kv_heads, head_dim, ctypes.addressof(opt), heads, nt, share, shares, _p(part), _p(err),
-                                            _stream()), "attention_q8")
+            part = torch.empty(tiles * n_kv_heads * -(-group // heads) * shares * cols * (head_dim + 2), dtype=torch.float32,
+                               device=q.device)
+        library.check(lib.cuca_attention_q8(src, qs, dst, os_, code, *rows, lo, hi, tokens, tiles, n_heads, n_kv_heads, head_dim, at,
+                                            heads, nt, share, shares, _p(part), e, stream), "attention_q8")
