@@ -8,7 +8,7 @@ configuration file (here JSON with `LocalModelConfig`'s field names), the reques
 Flags of the reference: --config, --prompt (token ids; text when the model folder brings a tokenizer.json and
 the prompt is not a list of numbers), --max-tokens (default 1024), --temperature (0 is greedy; default: the
 model's own). `--thinking` is accepted and ignored: chat templates are outside this engine. Ours: --model-dir,
---model-config, --random-weights SEED, --dtype, --top-k, --top-p, --seed, --prompt-len, --stop (a stop string,
+--model-config, --random-weights SEED, --dtype, --kv-cache-dtype, --top-k, --top-p, --seed, --prompt-len, --stop (a stop string,
 may be given several times; needs the tokenizer).
 It prints `load:`, `loaded on`, the generated ids (the text, with a tokenizer), and the reference's `timing:` line
 on standard error.
@@ -37,6 +37,7 @@ def main(argv=None) -> int:
     ap.add_argument("--model-config", help="a config.json to run with random weights")
     ap.add_argument("--random-weights", type=int, metavar="SEED", help="draw the weights from this seed")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default=None)
+    ap.add_argument("--kv-cache-dtype", choices=["int8"], default=None, help="keep keys and values in 8 bits")
     args = ap.parse_args(argv)
 
     from .config.engine_config import LocalModelConfig, RandomWeights
@@ -52,6 +53,8 @@ def main(argv=None) -> int:
         config.random_weights = RandomWeights(seed=args.random_weights)
     if args.dtype:
         config.dtype = args.dtype
+    if args.kv_cache_dtype:
+        config.kv_cache_dtype = args.kv_cache_dtype
 
     started = time.perf_counter()
     model = LocalModel.load(config)

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(STORE_THREADS, ROWS > 1 ? 4 : 1) rope_store_q8
   for (int r = 0; r < ROWS; ++r) {
     const bool in_table = pos[r] >= 0 && pos[r] < p.table_rows;
     if (rotate && live[r] && !in_table && l == 0 && p.err) atomicExch(p.err, CUCA_ERR_TOKEN_RANGE);
-    if (VEC && rotate && in_table) {
+    if (VEC && rotate && in_table && lane_ok) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float x = a[r][i], y = b[r][i], cs = c[VEC ? r : 0][i], sn = s[VEC ? r : 0][i];

@@ -38,10 +38,14 @@ class EngineCore:
     def __init__(self, spec, source: Optional[WeightSource], dtype=torch.bfloat16, device="cuda:0",
                  context_length: Optional[int] = None, kv_tokens: Optional[int] = None, max_sequences: int = 4,
                  block_size: int = 16, max_step_tokens: Optional[int] = None, window_pools: str = "sized",
-                 random_seed: Optional[int] = None, random_std: float = 0.02):
+                 random_seed: Optional[int] = None, random_std: float = 0.02, kv_cache_dtype: Optional[str] = None):
+        if kv_cache_dtype not in (None, "int8"):
+            raise ValueError(f"keys and values are kept in the compute dtype or in int8, not {kv_cache_dtype}")
         self.spec = spec
         self.rt = Runtime(device, parse_dtype(dtype))
         self.model = Model(spec, self.rt)
+        if kv_cache_dtype is not None:
+            self.model.check_quantized_cache()
         if source is None:
             if random_seed is None:
                 raise ValueError("neither a weight source nor a seed for random weights was given")
@@ -62,7 +66,8 @@ class EngineCore:
         self.pools = KvPools(self.groups, block_size)
         self.pools.stateful = any(n.state is not None for n in needs.values())
         self.slots = StateSlots(max_sequences)
-        self.cache = DeviceCache(self.rt, self.groups, block_size, needs, max_sequences, self.context_length)
+        self.cache = DeviceCache(self.rt, self.groups, block_size, needs, max_sequences, self.context_length,
+                                 quantized=kv_cache_dtype is not None)
         self.stepper = Stepper(self.model, self.pools, self.cache, self.context_length)
 
     @classmethod

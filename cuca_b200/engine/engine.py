@@ -216,7 +216,8 @@ class LocalModel:
         sizes = config.resolve(spec.max_positions)
         kw = dict(dtype=config.dtype, device=config.device, context_length=sizes["context_length"],
                   kv_tokens=sizes["kv_tokens"], max_sequences=config.batching.max_sequences,
-                  block_size=config.kv_block_size, max_step_tokens=sizes["max_step_tokens"])
+                  block_size=config.kv_block_size, max_step_tokens=sizes["max_step_tokens"],
+                  kv_cache_dtype=config.kv_cache_dtype)
         if model_dir is not None:
             core = EngineCore(spec, FolderSource(model_dir), **kw)
         else:

@@ -60,6 +60,12 @@ class Model:
                 out[run.cache] = self.blocks[run.layer].cache_needs()
         return out
 
+    def check_quantized_cache(self) -> None:
+        """Refuses keys and values in 8 bits where a layer keeps or reads rows that its kernels take in full only."""
+        for i, block in enumerate(self.blocks):
+            if block.mixer.cache_needs().kv is not None and not block.mixer.takes_quantized_cache:
+                raise ValueError(f"layer {i}: its mixer (`{block.mixer.spec.kind}`) does not take keys and values in 8 bits")
+
     def graph_safe(self) -> bool:
         return all(b.graph_safe for b in self.blocks)
 

@@ -124,6 +124,7 @@ class PagedAttention(Mixer):
             raise ValueError("attention: a layer that reads another layer's pages takes neither a value size of its "
                              "own, an output gate, head norms, a score cap, a sink, a distance bias, kept first keys nor "
                              "adjacent rotation pairs")
+        self.takes_quantized_cache = not self.general and ops.q8_supported(self.head_dim)
         # what the decode kernel that makes its own queries and keys takes
         self.fusable = (self.norm_unit and self.position is None and self.q_temp is None and not self.v_norm
                         and not self.head_gate and self.v_head_dim == self.head_dim and self.head_dim in (16, 32, 64, 128)
@@ -295,8 +296,29 @@ class PagedAttention(Mixer):
             ops.head_gate_(attn, proj[:, g_col:g_col + nh], nh, dv)
         stream.add_linear(attn, self.w_o, bias=self.b_o)
 
+    def forward_quantized(self, h, stream, step, cache) -> None:
+        """Over pages in 8 bits: one projection; q rotated where it stands, k rotated, k and v quantised into their pages;
+        attention over the codes."""
+        nh, nkv, d = self.n_heads, self.n_kv_heads, self.head_dim
+        proj = self.rt.linear(h, self.w_qkv, bias=self.b_qkv)
+        fused = self.position.fused_tables() if self.position is not None else None
+        if fused is None and self.position is not None:
+            self.position.apply(proj, nh, 0 if self.shares_cache else nkv, d, step.positions)
+        cos, sin, rot = fused if fused is not None else (None, None, 0)
+        if not self.shares_cache:
+            ops.rope_store_q8(proj, proj, step.positions, step.seq_of_row, cache.tables, cos, sin, rot, cache.quantized, nh, nkv,
+                              d, self.rt.err)
+        elif fused is not None:
+            ops.rope_store(proj, step.positions, step.seq_of_row, cache.tables, cos, sin, rot, None, None, cache.block_size, nh,
+                           0, d, self.rt.err)
+        attn = self.rt.empty(h.shape[0], nh * d)
+        ops.attention_q8(proj, attn, cache.quantized, cache.tables, step, nh, nkv, d, self.scale, self.window, self.rt.err)
+        stream.add_linear(attn, self.w_o, bias=self.b_o)
+
     def forward(self, h, stream, step, cache) -> None:
         stream = self.rt.stream(stream)
+        if cache.quantized is not None:
+            return self.forward_quantized(h, stream, step, cache)
         if self.general:
             return self.forward_general(h, stream, step, cache)
         nh, d = self.n_heads, self.head_dim

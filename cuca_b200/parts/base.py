@@ -113,6 +113,7 @@ class PositionEncoding(Part):
 
 class Mixer(Part):
     graph_safe = False  # True when forward() only launches kernels on static buffers
+    takes_quantized_cache = False  # True when forward() works on a view whose pages are `quantized`
 
     def cache_needs(self) -> CacheNeeds:
         return CacheNeeds()
