@@ -479,9 +479,8 @@ attention_q8_kernel(const Q8Params p) {
   }
 }
 
-// Joins the shares of a tile's keys, in their order: a warp per query row. Its lanes take two shares' maxima and sums each, then
+// Joins the shares of a tile's keys, in their order: a warp per query row. Its lanes take two shares' maxima and sums each (there are 64 at most), then
 // four dimensions (of each 128).
-constexpr int MOST_SHARES = 64;
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32) join_q8_kernel(const Q8Params p, int cols) {
   pdl_trigger();
@@ -574,47 +573,24 @@ int launch_q8_nt(const Q8Params& p, int nt, int n_tiles, cudaStream_t stream) {
 }  // namespace
 
 
-// Requests that bring count_lo .. count_hi rows (req_count null: every request one), tile_tokens rows of a request and
-// heads_per_cta query heads to a block of `nt` column tiles; keys in shares of `chunk`, n_splits of them at most (the last has
-// the rest). part: [n_tiles][nkv * pieces of a group][n_splits][8 nt / parts][d + 2] floats where n_splits > 1.
-CUCA_API int cuca_attention_q8(const void* q, int q_stride, void* out, int out_stride, int dtype, const void* kpool,
-                               const void* vpool, const float* kscale, const float* vscale, int n_blocks, int bs,
-                               const int* positions, const int* seq_of_row, const int* tables, int table_stride,
-                               const int* req_row0, const int* req_count, int n_seqs, int count_lo, int count_hi, int tile_tokens,
-                               int n_tiles, int nh, int nkv, int d, const CucaAttnOptions* opt, int heads_per_cta, int nt,
-                               int chunk, int n_splits, float* part, int* err, cudaStream_t stream) {
-  if (n_tiles == 0) return 0;
-  CUCA_REQUIRE(dtype == CUCA_F32 || dtype == CUCA_BF16, "attention_q8: unknown dtype %d", dtype);
-  CUCA_REQUIRE(opt != nullptr && opt->window >= 0 && opt->keep >= 0, "attention_q8: bad options");
-  CUCA_REQUIRE(opt->gate == nullptr && opt->key_scale == nullptr, "attention_q8: no output gate and no shared rows over 8-bit pages");
-  CUCA_REQUIRE(nkv > 0 && nh > 0 && nh % nkv == 0 && d >= 16 && d <= 256 && d % 16 == 0,
-               "attention_q8: unsupported shape (heads %d/%d, head size %d)", nh, nkv, d);
-  CUCA_REQUIRE(bs > 0 && n_blocks > 0 && table_stride > 0, "attention_q8: empty pages or tables");
-  CUCA_REQUIRE((((uintptr_t)kpool | (uintptr_t)vpool) & 15) == 0, "attention_q8: pools must be 16-byte aligned");
-  CUCA_REQUIRE(nt == 1 || nt == 2 || (nt == 4 && d <= 128), "attention_q8: %d column tiles", nt);
-  const int parts = dtype == CUCA_F32 ? 2 : 1, group = nh / nkv;
-  CUCA_REQUIRE(heads_per_cta > 0 && heads_per_cta <= group && tile_tokens > 0 && (long long)tile_tokens * heads_per_cta * parts <= 8 * nt,
-               "attention_q8: %d rows of %d heads do not fit %d columns", tile_tokens, heads_per_cta, 8 * nt / parts);
-  CUCA_REQUIRE(chunk >= 0 && chunk % 64 == 0 && n_splits >= 1 && n_splits <= MOST_SHARES &&
-               (n_splits == 1 || (chunk > 0 && part && ((uintptr_t)part & 15) == 0)), "attention_q8: bad shares of the keys");
-  const int head_parts = (group + heads_per_cta - 1) / heads_per_cta;
-  CUCA_REQUIRE(n_tiles <= 65535 && (long long)nkv * head_parts <= 65535, "attention_q8: too many tiles or heads");
+// bfloat16 or 32-bit rows; tile_tokens rows of a request and heads_per_cta query heads to a block of `width` (1, 2, 4; not 4 beyond
+// 128 dimensions) column tiles. part: [n_tiles][nkv * pieces of a group][n_splits][8 width / parts][d + 2] floats where
+// n_splits > 1 (parts: 2 for 32-bit rows, else 1).
+CUCA_API int cuca_attention_q8(const CucaQ8Attention* c) {
+  if (c->n_tiles == 0) return 0;
   Q8Params p;
-  p.q = q; p.q_stride = q_stride; p.out = out; p.out_stride = out_stride;
-  p.kpool = (const int8_t*)kpool; p.vpool = (const int8_t*)vpool; p.kscale = kscale; p.vscale = vscale;
-  p.n_blocks = n_blocks; p.bs = bs; p.tables = tables; p.table_stride = table_stride; p.positions = positions;
-  p.seq_of_row = seq_of_row; p.req_row0 = req_row0; p.req_count = req_count; p.n_seqs = n_seqs; p.count_lo = count_lo;
-  p.count_hi = count_hi; p.tile_tokens = tile_tokens; p.nh = nh; p.nkv = nkv; p.d = d;
-  p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E; p.cap = opt->softcap; p.cap_arg = opt->softcap > 0.f ? 2.f * CUCA_LOG2E / opt->softcap : 0.f; p.sink = opt->sink ? 1 : 0;
-  p.sink_val = opt->sink ? opt->sink_val : nullptr; p.window = opt->window; p.keep = opt->window > 0 ? opt->keep : 0;
-  p.slopes = opt->slopes; p.heads_per_cta = heads_per_cta; p.head_parts = head_parts; p.chunk = n_splits > 1 ? chunk : 0;
-  p.n_splits = n_splits; p.part = part; p.err = err; p.run_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
+  if (const int code = q8_params(*c, "attention_q8", 256, p)) return code;
+  const int nt = (int)c->width, parts = c->dtype == CUCA_F32 ? 2 : 1, n_tiles = (int)c->n_tiles, d = p.d;
+  CUCA_REQUIRE(nt == 1 || nt == 2 || (nt == 4 && d <= 128), "attention_q8: %d column tiles", nt);
+  CUCA_REQUIRE((long long)p.tile_tokens * p.heads_per_cta * parts <= 8 * nt, "attention_q8: %d rows of %d heads do not fit %d columns",
+               p.tile_tokens, p.heads_per_cta, 8 * nt / parts);
+  CUCA_REQUIRE((long long)p.nkv * p.head_parts <= 65535, "attention_q8: too many heads");
   if (parts == 2) {
-    if (d <= 64) return launch_q8_nt<64, 2>(p, nt, n_tiles, stream);
-    if (d <= 128) return launch_q8_nt<128, 2>(p, nt, n_tiles, stream);
-    return launch_q8_nt<256, 2>(p, nt, n_tiles, stream);
+    if (d <= 64) return launch_q8_nt<64, 2>(p, nt, n_tiles, c->stream);
+    if (d <= 128) return launch_q8_nt<128, 2>(p, nt, n_tiles, c->stream);
+    return launch_q8_nt<256, 2>(p, nt, n_tiles, c->stream);
   }
-  if (d <= 64) return launch_q8_nt<64, 1>(p, nt, n_tiles, stream);
-  if (d <= 128) return launch_q8_nt<128, 1>(p, nt, n_tiles, stream);
-  return launch_q8_nt<256, 1>(p, nt, n_tiles, stream);
+  if (d <= 64) return launch_q8_nt<64, 1>(p, nt, n_tiles, c->stream);
+  if (d <= 128) return launch_q8_nt<128, 1>(p, nt, n_tiles, c->stream);
+  return launch_q8_nt<256, 1>(p, nt, n_tiles, c->stream);
 }

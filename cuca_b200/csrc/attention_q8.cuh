@@ -23,6 +23,41 @@ namespace {
 // (rescaling is rare then), and LIFT puts the weights' 29 binades of full precision below 2^15.
 constexpr float Q8_LIFT = 7.f, Q8_LAG = 7.f;
 
+}  // namespace
+
+// A launch, as Python packs it: one 64-bit word each, in this order (kernels/ops.py:attention_q8; 33 arguments one by one cost
+// the caller 3.7 us, packed 0.9).
+struct CucaQ8Attention {
+  const void* q;
+  int64_t q_stride;  // values between rows
+  void* out;
+  int64_t out_stride, dtype;
+  const int8_t* kpool;
+  const int8_t* vpool;
+  const float* kscale;
+  const float* vscale;
+  int64_t n_blocks, bs;
+  const int* positions;
+  const int* seq_of_row;
+  const int* tables;
+  int64_t table_stride;
+  const int* req_row0;
+  const int* req_count;  // null: every request brings one row
+  int64_t n_seqs, count_lo, count_hi;  // requests with so many rows are this launch's
+  int64_t tile_tokens, n_tiles;        // rows of a request that a tile takes
+  int64_t nh, nkv, d;
+  const CucaAttnOptions* opt;
+  int64_t heads_per_cta;  // query heads of a key head that a block takes
+  int64_t width;          // of a block: column tiles, or query tiles
+  int64_t chunk, n_splits;  // keys of a share (the last has the rest) and how many
+  float* part;
+  int* err;
+  cudaStream_t stream;
+};
+static_assert(sizeof(CucaQ8Attention) == 33 * 8, "one 64-bit word each");
+
+namespace {
+
 struct Q8Params {
   const void* q;
   int q_stride;  // values between rows
@@ -192,6 +227,39 @@ __device__ __forceinline__ float q8_capped(float s, const Q8Params& p) {
 // What a sink adds to a denominator that is relative to the reference m.
 __device__ __forceinline__ float q8_sink_term(const Q8Params& p, int head, float m) {
   return q8_exp2((p.sink_val ? p.sink_val[head] * CUCA_LOG2E : 0.f) - m + Q8_LIFT);
+}
+
+// What both entry points check, and the kernels' parameters.
+inline int q8_params(const CucaQ8Attention& c, const char* name, int most_d, Q8Params& p) {
+  CUCA_REQUIRE(c.dtype == CUCA_F32 || c.dtype == CUCA_BF16, "%s: unknown dtype %lld", name, (long long)c.dtype);
+  const CucaAttnOptions* opt = c.opt;
+  CUCA_REQUIRE(opt != nullptr && opt->window >= 0 && opt->keep >= 0, "%s: bad options", name);
+  CUCA_REQUIRE(opt->gate == nullptr && opt->key_scale == nullptr, "%s: no output gate and no shared rows over 8-bit pages", name);
+  CUCA_REQUIRE(c.nkv > 0 && c.nkv <= 65535 && c.nh > 0 && c.nh <= (1 << 20) && c.nh % c.nkv == 0 && c.d >= 16 && c.d <= most_d && c.d % 16 == 0,
+               "%s: unsupported shape (heads %lld/%lld, head size %lld)", name, (long long)c.nh, (long long)c.nkv, (long long)c.d);
+  CUCA_REQUIRE(c.bs > 0 && c.bs < (1 << 30) && c.n_blocks > 0 && c.n_blocks < (1ll << 31) && c.table_stride > 0 && c.table_stride < (1ll << 31),
+               "%s: empty or endless pages or tables", name);
+  CUCA_REQUIRE((((uintptr_t)c.kpool | (uintptr_t)c.vpool) & 15) == 0, "%s: pools must be 16-byte aligned", name);
+  CUCA_REQUIRE(c.q_stride < (1ll << 31) && c.out_stride < (1ll << 31), "%s: rows too far apart", name);
+  CUCA_REQUIRE(c.n_tiles > 0 && c.n_tiles <= 65535, "%s: %lld tiles", name, (long long)c.n_tiles);
+  CUCA_REQUIRE(c.chunk >= 0 && c.chunk % 64 == 0 && c.n_splits >= 1 && c.n_splits <= 64 &&
+               (c.n_splits == 1 || (c.chunk > 0 && c.part && ((uintptr_t)c.part & 15) == 0)), "%s: bad shares of the keys", name);
+  const int group = (int)(c.nh / c.nkv);
+  CUCA_REQUIRE(c.heads_per_cta > 0 && c.heads_per_cta <= group && c.tile_tokens > 0 && c.tile_tokens <= 65536, "%s: bad tiles", name);
+  p.q = c.q; p.q_stride = (int)c.q_stride; p.out = c.out; p.out_stride = (int)c.out_stride;
+  p.kpool = c.kpool; p.vpool = c.vpool; p.kscale = c.kscale; p.vscale = c.vscale;
+  p.n_blocks = (int)c.n_blocks; p.bs = (int)c.bs; p.run_shift = (c.bs & (c.bs - 1)) == 0 ? __builtin_ctzll(c.bs) : -1;
+  p.tables = c.tables; p.table_stride = (int)c.table_stride; p.positions = c.positions; p.seq_of_row = c.seq_of_row;
+  p.req_row0 = c.req_row0; p.req_count = c.req_count; p.n_seqs = (int)c.n_seqs;
+  p.count_lo = (int)c.count_lo; p.count_hi = (int)c.count_hi; p.tile_tokens = (int)c.tile_tokens;
+  p.nh = (int)c.nh; p.nkv = (int)c.nkv; p.d = (int)c.d;
+  p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E;
+  p.cap = opt->softcap; p.cap_arg = opt->softcap > 0.f ? 2.f * CUCA_LOG2E / opt->softcap : 0.f;
+  p.sink = opt->sink ? 1 : 0; p.sink_val = opt->sink ? opt->sink_val : nullptr;
+  p.window = opt->window; p.keep = opt->window > 0 ? opt->keep : 0; p.slopes = opt->slopes;
+  p.heads_per_cta = (int)c.heads_per_cta; p.head_parts = (group + p.heads_per_cta - 1) / p.heads_per_cta;
+  p.n_splits = (int)c.n_splits; p.chunk = c.n_splits > 1 ? (int)c.chunk : 0; p.part = c.part; p.err = c.err;
+  return 0;
 }
 
 }  // namespace

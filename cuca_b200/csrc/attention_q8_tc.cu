@@ -697,38 +697,19 @@ int launch_q8_tc(const Q8Params& p, int n_tiles, cudaStream_t stream) {
 
 }  // namespace
 
-// As cuca_attention_q8 for bfloat16 rows and head sizes up to 128, whole groups of at most 128 heads: tile_tokens is
-// query_tiles (1 or 2) times the tokens whose rows fit 128. part: [n_tiles][nkv][n_splits][256 (d rounded up to 64 or 128) + 512]
-// floats where n_splits > 1.
-CUCA_API int cuca_attention_q8_tc(const void* q, int q_stride, void* out, int out_stride, const void* kpool, const void* vpool,
-                                  const float* kscale, const float* vscale, int n_blocks, int bs, const int* positions,
-                                  const int* seq_of_row, const int* tables, int table_stride, const int* req_row0,
-                                  const int* req_count, int n_seqs, int count_lo, int count_hi, int query_tiles, int n_tiles,
-                                  int nh, int nkv, int d, const CucaAttnOptions* opt, int chunk, int n_splits, float* part,
-                                  int* err, cudaStream_t stream) {
-  if (n_tiles == 0) return 0;
-  CUCA_REQUIRE(opt != nullptr && opt->window >= 0 && opt->keep >= 0, "attention_q8_tc: bad options");
-  CUCA_REQUIRE(opt->gate == nullptr && opt->key_scale == nullptr, "attention_q8_tc: no output gate and no shared rows over 8-bit pages");
-  CUCA_REQUIRE(nkv > 0 && nh > 0 && nh % nkv == 0 && nh / nkv <= ROWS && d >= 16 && d <= 128 && d % 16 == 0,
-               "attention_q8_tc: unsupported shape (heads %d/%d, head size %d)", nh, nkv, d);
-  CUCA_REQUIRE(bs > 0 && n_blocks > 0 && table_stride > 0, "attention_q8_tc: empty pages or tables");
-  CUCA_REQUIRE((((uintptr_t)kpool | (uintptr_t)vpool) & 15) == 0, "attention_q8_tc: pools must be 16-byte aligned");
-  CUCA_REQUIRE((long long)n_blocks * nkv * bs < 0xffffffffll, "attention_q8_tc: more than 2^32 rows in the pools");
-  CUCA_REQUIRE(query_tiles == 1 || query_tiles == NQ, "attention_q8_tc: %d query tiles", query_tiles);
-  CUCA_REQUIRE(chunk >= 0 && chunk % KEYS == 0 && n_splits >= 1 && (n_splits == 1 || (chunk > 0 && part && ((uintptr_t)part & 15) == 0)),
-               "attention_q8_tc: bad shares of the keys");
-  CUCA_REQUIRE(n_tiles <= 65535 && nkv <= 65535, "attention_q8_tc: too many tiles or heads");
+// bfloat16 rows of head sizes up to 128, groups of at most 128 heads whole; `width` (1 or 2) query tiles to a block: tile_tokens is
+// that times the tokens whose rows fit 128. part: [n_tiles][nkv][n_splits][256 (d rounded up to 64 or 128) + 512] floats where
+// n_splits > 1.
+CUCA_API int cuca_attention_q8_tc(const CucaQ8Attention* c) {
+  if (c->n_tiles == 0) return 0;
   Q8Params p;
-  p.q = q; p.q_stride = q_stride; p.out = out; p.out_stride = out_stride;
-  p.kpool = (const int8_t*)kpool; p.vpool = (const int8_t*)vpool; p.kscale = kscale; p.vscale = vscale;
-  p.n_blocks = n_blocks; p.bs = bs; p.tables = tables; p.table_stride = table_stride; p.positions = positions;
-  p.seq_of_row = seq_of_row; p.req_row0 = req_row0; p.req_count = req_count; p.n_seqs = n_seqs; p.count_lo = count_lo;
-  p.count_hi = count_hi; p.tile_tokens = query_tiles * (ROWS / (nh / nkv)); p.nh = nh; p.nkv = nkv; p.d = d;
-  p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E; p.cap = opt->softcap; p.cap_arg = opt->softcap > 0.f ? 2.f * CUCA_LOG2E / opt->softcap : 0.f; p.sink = opt->sink ? 1 : 0;
-  p.sink_val = opt->sink ? opt->sink_val : nullptr; p.window = opt->window; p.keep = opt->window > 0 ? opt->keep : 0;
-  p.slopes = opt->slopes; p.heads_per_cta = nh / nkv; p.head_parts = 1; p.chunk = n_splits > 1 ? chunk : 0;
-  p.n_splits = n_splits; p.part = part; p.err = err; p.run_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
+  if (const int code = q8_params(*c, "attention_q8_tc", 128, p)) return code;
+  const int group = p.nh / p.nkv;
+  CUCA_REQUIRE(c->dtype == CUCA_BF16 && group <= ROWS && p.heads_per_cta == group, "attention_q8_tc: bfloat16 rows and groups of at most %d heads", ROWS);
+  CUCA_REQUIRE((long long)p.n_blocks * p.nkv * p.bs < 0xffffffffll, "attention_q8_tc: more than 2^32 rows in the pools");
+  CUCA_REQUIRE((c->width == 1 || c->width == NQ) && p.tile_tokens == (int)c->width * (ROWS / group), "attention_q8_tc: %d rows to %lld query tiles",
+               p.tile_tokens, (long long)c->width);
   const bool extra = p.cap > 0.f || p.sink || p.slopes;
-  if (d <= 64) return extra ? launch_q8_tc<64, true>(p, n_tiles, stream) : launch_q8_tc<64, false>(p, n_tiles, stream);
-  return extra ? launch_q8_tc<128, true>(p, n_tiles, stream) : launch_q8_tc<128, false>(p, n_tiles, stream);
+  if (p.d <= 64) return extra ? launch_q8_tc<64, true>(p, (int)c->n_tiles, c->stream) : launch_q8_tc<64, false>(p, (int)c->n_tiles, c->stream);
+  return extra ? launch_q8_tc<128, true>(p, (int)c->n_tiles, c->stream) : launch_q8_tc<128, false>(p, (int)c->n_tiles, c->stream);
 }

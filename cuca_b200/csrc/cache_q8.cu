@@ -15,6 +15,46 @@
 
 int cuca_device_sms();
 
+// A launch of either, as Python packs it: one 64-bit word each, in this order (kernels/ops.py:rope_store_q8, read_q8).
+struct CucaQ8Store {
+  const void* qkv;
+  int64_t row_stride;
+  void* q_out;
+  int64_t q_stride, dtype;
+  const int* positions;
+  const int* seq_of_row;
+  const int* tables;
+  int64_t table_stride;
+  const float* cos_t;
+  const float* sin_t;
+  int64_t table_rows, rot, adjacent;
+  void* kpool;
+  void* vpool;
+  float* kscale;
+  float* vscale;
+  int64_t n_blocks, bs, n_rows, nh, nkv, d;
+  int* err;
+  cudaStream_t stream;
+};
+struct CucaQ8Read {
+  const void* kpool;
+  const void* vpool;
+  const float* kscale;
+  const float* vscale;
+  int64_t n_blocks, bs;
+  const int* positions;
+  const int* seq_of_row;
+  const int* tables;
+  int64_t table_stride;
+  void* k_out;
+  int64_t k_stride;
+  void* v_out;
+  int64_t v_stride, dtype, n_rows, nkv, d;
+  int* err;
+  cudaStream_t stream;
+};
+static_assert(sizeof(CucaQ8Store) == 26 * 8 && sizeof(CucaQ8Read) == 20 * 8, "one 64-bit word each");
+
 namespace {
 
 constexpr float CUCA_Q8_TINY = 7.888609052210118e-31f;  // 2^-100
@@ -289,19 +329,24 @@ __global__ void __launch_bounds__(READ_WARPS * 32) read_q8_kernel(const __grid_c
 
 // Rotates q (into q_out, which may be the rows themselves) and k, quantises k and v and writes them to their pages.
 // `adjacent`: neighbouring values are the rotation's pairs instead of the halves of the first `rot`.
-CUCA_API int cuca_rope_store_q8(const void* qkv, int row_stride, void* q_out, int q_stride, int dtype, const int* positions,
-                                const int* seq_of_row, const int* tables, int table_stride, const float* cos_t,
-                                const float* sin_t, int table_rows, int rot, int adjacent, void* kpool, void* vpool,
-                                float* kscale, float* vscale, int n_blocks, int bs, int n_rows, int nh, int nkv, int d,
-                                int* err, cudaStream_t stream) {
+CUCA_API int cuca_rope_store_q8(const CucaQ8Store* c) {
+  const void* qkv = c->qkv;
+  void *q_out = c->q_out, *kpool = c->kpool, *vpool = c->vpool;
+  const float *cos_t = c->cos_t, *sin_t = c->sin_t;
+  const int dtype = (int)c->dtype, n_rows = (int)c->n_rows, nh = (int)c->nh, nkv = (int)c->nkv, d = (int)c->d, bs = (int)c->bs;
+  const int n_blocks = (int)c->n_blocks, table_stride = (int)c->table_stride, rot = (int)c->rot, table_rows = (int)c->table_rows;
+  const int row_stride = (int)c->row_stride, q_stride = (int)c->q_stride, adjacent = c->adjacent != 0;
+  const cudaStream_t stream = c->stream;
+  CUCA_REQUIRE(c->row_stride < (1ll << 31) && c->q_stride < (1ll << 31) && c->n_blocks < (1ll << 31) && c->n_rows < (1ll << 31) &&
+               c->table_stride < (1ll << 31) && c->table_rows < (1ll << 31), "rope_store_q8: a size beyond 32 bits");
   CUCA_REQUIRE(dtype == CUCA_F32 || dtype == CUCA_BF16, "rope_store_q8: unknown dtype %d", dtype);
   CUCA_REQUIRE(nh > 0 && nkv > 0 && bs > 0 && n_blocks > 0 && table_stride > 0, "rope_store_q8: empty heads, pages or tables");
   CUCA_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "rope_store_q8: head size %d is not a multiple of 16 up to 256", d);
   CUCA_REQUIRE(rot >= 0 && rot <= d && rot % 2 == 0 && (rot == 0 || (cos_t && sin_t)), "rope_store_q8: %d rotated values of %d", rot, d);
   CUCA_REQUIRE(((uintptr_t)kpool & 3) == 0 && ((uintptr_t)vpool & 3) == 0, "rope_store_q8: pools must be 4-byte aligned");
   if (n_rows == 0) return 0;
-  StoreParams p{qkv, row_stride, q_out, q_stride, positions, seq_of_row, tables, table_stride, cos_t, sin_t, table_rows, rot,
-                adjacent, (int8_t*)kpool, (int8_t*)vpool, kscale, vscale, n_blocks, bs, n_rows, nh, nkv, d, 0, err};
+  StoreParams p{qkv, row_stride, q_out, q_stride, c->positions, c->seq_of_row, c->tables, table_stride, cos_t, sin_t, table_rows, rot,
+                adjacent, (int8_t*)kpool, (int8_t*)vpool, c->kscale, c->vscale, n_blocks, bs, n_rows, nh, nkv, d, 0, c->err};
   while ((8 << p.seg_shift) < d) ++p.seg_shift;
   const uintptr_t align = dtype == CUCA_F32 ? 15 : 7;
   const bool vec = (rot == d || rot == 0) && !adjacent && row_stride % 4 == 0 && q_stride % 4 == 0 &&
@@ -322,10 +367,14 @@ CUCA_API int cuca_rope_store_q8(const void* qkv, int row_stride, void* q_out, in
 
 // Rows of k_out / v_out (either may be null): the values that the codes of (seq_of_row, positions) stand for; zeros for a row
 // of no request (seq < 0).
-CUCA_API int cuca_read_q8(const void* kpool, const void* vpool, const float* kscale, const float* vscale, int n_blocks, int bs,
-                          const int* positions, const int* seq_of_row, const int* tables, int table_stride, void* k_out,
-                          int k_stride, void* v_out, int v_stride, int dtype, int n_rows, int nkv, int d, int* err,
-                          cudaStream_t stream) {
+CUCA_API int cuca_read_q8(const CucaQ8Read* c) {
+  const int dtype = (int)c->dtype, n_rows = (int)c->n_rows, nkv = (int)c->nkv, d = (int)c->d, bs = (int)c->bs;
+  const int n_blocks = (int)c->n_blocks, table_stride = (int)c->table_stride, k_stride = (int)c->k_stride, v_stride = (int)c->v_stride;
+  const void *kpool = c->kpool, *vpool = c->vpool;
+  void *k_out = c->k_out, *v_out = c->v_out;
+  const cudaStream_t stream = c->stream;
+  CUCA_REQUIRE(c->k_stride < (1ll << 31) && c->v_stride < (1ll << 31) && c->n_blocks < (1ll << 31) && c->n_rows < (1ll << 31) &&
+               c->table_stride < (1ll << 31), "read_q8: a size beyond 32 bits");
   CUCA_REQUIRE(dtype == CUCA_F32 || dtype == CUCA_BF16, "read_q8: unknown dtype %d", dtype);
   CUCA_REQUIRE(nkv > 0 && bs > 0 && n_blocks > 0 && table_stride > 0, "read_q8: empty heads, pages or tables");
   CUCA_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "read_q8: head size %d is not a multiple of 16 up to 256", d);
@@ -333,8 +382,8 @@ CUCA_API int cuca_read_q8(const void* kpool, const void* vpool, const float* ksc
   CUCA_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0 && (!k_out || k_stride % n == 0) && (!v_out || v_stride % n == 0) &&
                (((uintptr_t)kpool | (uintptr_t)vpool) & 7) == 0, "read_q8: rows must start on 16 bytes, pools on 8");
   if (n_rows == 0 || (!k_out && !v_out)) return 0;
-  ReadParams p{{(const int8_t*)kpool, (const int8_t*)vpool}, {kscale, vscale}, {k_out, v_out}, {k_stride, v_stride}, positions,
-               seq_of_row, tables, table_stride, n_blocks, bs, n_rows, nkv, d, err};
+  ReadParams p{{(const int8_t*)kpool, (const int8_t*)vpool}, {c->kscale, c->vscale}, {k_out, v_out}, {k_stride, v_stride},
+               c->positions, c->seq_of_row, c->tables, table_stride, n_blocks, bs, n_rows, nkv, d, c->err};
   const int pieces = nkv * d / n;  // of a row
   const dim3 grid((n_rows + READ_WARPS * READ_ROWS - 1) / (READ_WARPS * READ_ROWS), (pieces + 32 * READ_PIECES - 1) / (32 * READ_PIECES), 2);
   CUCA_REQUIRE(grid.y <= 65535, "read_q8: too many heads");

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -1577,6 +1578,13 @@ class QuantizedPages:
 
 
 Q8_MAX_HEAD_DIM = 256
+# a call's arguments as 64-bit words (`CucaQ8Store` and `CucaQ8Read` in csrc/cache_q8.cu, `CucaQ8Attention` in csrc/attention_q8.cuh)
+_Q8_STORE, _Q8_READ, _Q8_ATTENTION = struct.Struct("26q"), struct.Struct("20q"), struct.Struct("33q")
+
+
+def _at(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
 
 
 def q8_supported(head_dim: int) -> bool:
@@ -1628,10 +1636,10 @@ def rope_store_q8(qkv, q_out, positions, seq_of_row, tables, cos, sin, rotary_di
             raise library.KernelError(f"cosines and sines are contiguous float32 [positions, {rot // 2}]")
         _cuda(cos, sin)
         table_rows = cos.shape[0]
-    library.check(library.load().cuca_rope_store_q8(
+    library.check(library.load().cuca_rope_store_q8(_Q8_STORE.pack(
         src, qkv.stride(0), dst, q_out.stride(0), code, _ints(positions, n), _ints(seq_of_row, n), _ints(tables), tables.shape[1],
-        _p(cos), _p(sin), table_rows, rot, 1 if adjacent else 0, k, v, ks, vs, n_pages, bs, n, n_heads, n_kv_heads, head_dim,
-        _p(err), _stream()), "rope_store_q8")
+        _at(cos), _at(sin), table_rows, rot, 1 if adjacent else 0, k, v, ks, vs, n_pages, bs, n, n_heads, n_kv_heads, head_dim,
+        _at(err), _stream())), "rope_store_q8")
 
 
 def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, err) -> None:
@@ -1646,7 +1654,7 @@ def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, 
     dtype, at = some.dtype, []
     for t in (k_out, v_out):
         if t is None:
-            at += (None, 0)
+            at += (0, 0)
             continue
         strides = t.stride()
         if t.shape != (n, nkv, d) or t.dtype != dtype or strides[2] != 1 or strides[1] != d:
@@ -1654,8 +1662,9 @@ def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, 
         if not t.is_cuda:
             _cuda(t)
         at += (t.data_ptr(), strides[0])
-    library.check(library.load().cuca_read_q8(k, v, ks, vs, n_pages, bs, _ints(positions, n), _ints(seq_of_row, n), _ints(tables),
-                                              tables.shape[1], *at, dtype_code(dtype), n, nkv, d, _p(err), _stream()), "read_q8")
+    library.check(library.load().cuca_read_q8(_Q8_READ.pack(
+        k, v, ks, vs, n_pages, bs, _ints(positions, n), _ints(seq_of_row, n), _ints(tables), tables.shape[1], *at, dtype_code(dtype),
+        n, nkv, d, _at(err), _stream())), "read_q8")
 
 
 Q8_FEW_ROWS = 16  # query rows of a key head that the form for few rows takes of a portion
@@ -1685,7 +1694,7 @@ class QuantizedPlan:
                 or a[3] is not step.req_count:
             n, m = step.n_rows, step.n_seqs
             self._addresses = (_ints(step.positions, n), _ints(step.seq_of_row, n)), \
-                (_ints(step.req_row0, m), None if self.all_single else _ints(step.req_count, m), m)
+                (_ints(step.req_row0, m), 0 if self.all_single else _ints(step.req_count, m), m)
             self._arrays = step.positions, step.seq_of_row, step.req_row0, step.req_count
         return self._addresses
 
@@ -1700,8 +1709,8 @@ class QuantizedPlan:
         return opt
 
     def launches(self, n_heads, n_kv_heads, head_dim, dtype, window, keep):
-        """[(form, least count, most count, rows of a tile, tiles, heads of a block, column tiles, keys of a share, shares)];
-        form 0: few rows a block, 1: tcgen05 (there `column tiles` are query tiles of 128)"""
+        """[(form, least count, most count, rows of a tile, tiles, heads of a block, width, keys of a share, shares)]; form 0: few
+        rows a block, `width` column tiles of 8; 1: tcgen05, `width` query tiles of 128"""
         key = (n_heads, n_kv_heads, head_dim, dtype, window, keep)
         if key not in self._launches:
             group, out, few = n_heads // n_kv_heads, [], self.longest
@@ -1736,7 +1745,7 @@ class QuantizedPlan:
                 if best is None or cost < best[0]:
                     best = cost, query_tiles, len(tiles), share, -(-longest // share)
         _, query_tiles, n_tiles, share, shares = best
-        return 1, lo, hi, tokens * query_tiles, n_tiles, 0, query_tiles, share * 64, shares
+        return 1, lo, hi, tokens * query_tiles, n_tiles, n_heads // n_kv_heads, query_tiles, share * 64, shares
 
     def _few(self, lo, hi, n_heads, n_kv_heads, head_dim, dtype, window, keep):
         parts, group = (2 if dtype == torch.float32 else 1), n_heads // n_kv_heads
@@ -1801,25 +1810,20 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
         raise library.KernelError("a window, kept first keys and a score cap are not negative")
     plan = attention_q8_plan(step)
     opt = plan.options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
-    at = ctypes.addressof(opt)
-    lib, stream, e = library.load(), _stream(), _p(err)
+    lib, stream, e = library.load(), _stream(), _at(err)
     of_rows, of_requests = plan.arrays(step)
-    rows = (*pool, *of_rows, _ints(tables), tables.shape[1], *of_requests)
-    qs, os_ = q.stride(0), out.stride(0)
+    rows = (src, q.stride(0), dst, out.stride(0), code, *pool, *of_rows, _ints(tables), tables.shape[1], *of_requests)
+    shape = n_heads, n_kv_heads, head_dim, ctypes.addressof(opt)
     group = n_heads // n_kv_heads
-    for form, lo, hi, tokens, tiles, heads, nt, share, shares in plan.launches(n_heads, n_kv_heads, head_dim, q.dtype, window or None,
-                                                                               opt.keep):
-        part = None
-        if form == 1:
-            if shares > 1:
-                part = torch.empty(tiles * n_kv_heads * shares * (256 * (64 if head_dim <= 64 else 128) + 512), dtype=torch.float32,
-                                   device=q.device)
-            library.check(lib.cuca_attention_q8_tc(src, qs, dst, os_, *rows, lo, hi, nt, tiles, n_heads, n_kv_heads, head_dim, at, share,
-                                                   shares, _p(part), e, stream), "attention_q8")
-            continue
-        if shares > 1:
-            cols = 8 * nt // (2 if code == F32 else 1)
-            part = torch.empty(tiles * n_kv_heads * -(-group // heads) * shares * cols * (head_dim + 2), dtype=torch.float32,
+    for form, lo, hi, tokens, tiles, heads, width, share, shares in plan.launches(n_heads, n_kv_heads, head_dim, q.dtype,
+                                                                                  window or None, opt.keep):
+        part, at = None, 0
+        if shares > 1:  # the shares' results, joined by a second launch
+            cols = 8 * width // (2 if code == F32 else 1)
+            part = torch.empty(tiles * n_kv_heads * shares * (256 * (64 if head_dim <= 64 else 128) + 512) if form == 1 else
+                               tiles * n_kv_heads * -(-group // heads) * shares * cols * (head_dim + 2), dtype=torch.float32,
                                device=q.device)
-        library.check(lib.cuca_attention_q8(src, qs, dst, os_, code, *rows, lo, hi, tokens, tiles, n_heads, n_kv_heads, head_dim, at,
-                                            heads, nt, share, shares, _p(part), e, stream), "attention_q8")
+            at = part.data_ptr()
+        entry = lib.cuca_attention_q8_tc if form == 1 else lib.cuca_attention_q8
+        library.check(entry(_Q8_ATTENTION.pack(*rows, lo, hi, tokens, tiles, *shape, heads, width, share, shares, at, e, stream)),
+                      "attention_q8")
