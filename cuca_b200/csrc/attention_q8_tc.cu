@@ -7,7 +7,7 @@
 //   S[128 rows, 64 keys]  = Q K^T      Q and K as 16-bit floats in shared memory (K-major, 128-byte swizzle)
 //   O[128 rows, d]       += W V        W from tensor memory, where S was; V as 16-bit floats in shared memory (MN-major)
 //
-// Four warps fetch the codes (into registers, a tile ahead), turn them into 16-bit floats and store them as operand tiles, with
+// Two warps copy codes from the pages, three tiles ahead; four turn them into 16-bit floats and store them as operand tiles, with
 // each key's factors beside them; four warps per query tile own a row per thread (a lane of tensor memory) and turn scores into
 // weights; a warp per query tile issues its products. Where the two query tiles share a converted tile, the conversion is a
 // seventh of the block's instructions.
@@ -30,12 +30,14 @@ constexpr int ROWS = 128;  // query rows of a tile = lanes of tensor memory
 constexpr int KEYS = 64;   // keys of a tile
 constexpr int NQ = 2;      // query tiles of a block
 constexpr int SOFT_WARPS = 4 * NQ, CONV_WARPS = 4;  // (8 that convert, with 144 registers for the softmax: a prompt of 2,048 76 us, not 70)
-constexpr int CONV = CONV_WARPS * 32;
-constexpr int NTHREADS = (SOFT_WARPS + CONV_WARPS + 4) * 32;  // softmax, conversion, issue (two warps of four)
+constexpr int LOAD_WARPS = 2;
+constexpr int NTHREADS = (SOFT_WARPS + CONV_WARPS + NQ + LOAD_WARPS) * 32;  // softmax, conversion, issue, copies
 // Registers a thread: 128 at launch, then by role; the sum, 2 x 176 + 88 + 64 over groups of 128 threads, is within the 4 x 128
 // of the launch.
 constexpr int SOFT_REGS = 176, CONV_REGS = 88, ISSUE_REGS = 64;
-constexpr int STAGES = 3;         // of operand tiles
+// Operand tiles of keys are free again when their scores are there, those of values only after the weights' product: with three
+// of both, a tile's way round (conversion, scores, softmax, product: some 6,000 clocks) set the pace and not any unit.
+constexpr int K_STAGES = 2, V_STAGES = 4;
 constexpr int RAW = 3;            // tiles of codes on their way
 constexpr float V_LIFT = 7.f;     // values are 2^7 larger in the operand tile: 127 2^7 2 is the most that fits
 constexpr int WIDE = 20;
@@ -54,11 +56,9 @@ struct Shape {
   static constexpr int KV_HALF = KEYS * 128, KV_TILE = HALVES * KV_HALF;
   static constexpr int FACTORS = (3 * KEYS + 4) * 4;  // of a stage: the keys' factors; the value scales' exponents less E and their
                                                       // inverse (of a wide tile); E, its inverse, and whether the tile is wide
-  static constexpr int STAGE = 2 * KV_TILE;
-  static constexpr int PER = KEYS * (DP / 16) / CONV;  // 16-byte pieces of keys, and of values, that a thread converts
-  static constexpr int RAW_STAGE = CONV * (2 * PER * 16 + 16);  // codes of a tile and four scales a thread, each thread's its own
-  static constexpr int TILES = NQ * Q_BYTES + STAGES * (STAGE + FACTORS) + RAW * RAW_STAGE;
-  static constexpr int SMEM = TILES + 256 + 1024;  // + barriers, + alignment
+  static constexpr int RAW_STAGE = 2 * KEYS * DP + 2 * KEYS * 4;  // codes of a tile's keys and values, their scales
+  static constexpr int TILES = NQ * Q_BYTES + (K_STAGES + V_STAGES) * KV_TILE + V_STAGES * FACTORS + RAW * RAW_STAGE;
+  static constexpr int SMEM = TILES + 384 + 1024;  // + barriers, + alignment
 };
 
 // f16 x f16 -> f32, M = 128, N = n; b_mn: the second operand is MN-major
@@ -109,14 +109,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   // (by an offset, so that the compiler still knows it for shared memory)
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* q_s = smem;
-  uint8_t* kv_s = q_s + NQ * SH::Q_BYTES;
-  float* factor_s = (float*)(kv_s + STAGES * SH::STAGE);
-  uint8_t* raw_s = (uint8_t*)factor_s + STAGES * SH::FACTORS;
+  uint8_t* k_s = q_s + NQ * SH::Q_BYTES;
+  uint8_t* v_s = k_s + K_STAGES * SH::KV_TILE;
+  float* factor_s = (float*)(v_s + V_STAGES * SH::KV_TILE);  // [V_STAGES]
+  uint8_t* raw_s = (uint8_t*)factor_s + V_STAGES * SH::FACTORS;
   uint64_t* bars = (uint64_t*)(raw_s + RAW * SH::RAW_STAGE);
-  uint64_t* q_full = bars;                   // [NQ]
-  uint64_t* kv_full = q_full + NQ;           // [STAGES]
-  uint64_t* kv_empty = kv_full + STAGES;     // [STAGES]
-  uint64_t* s_full = kv_empty + STAGES;      // [NQ][2]
+  uint64_t* q_full = bars;                     // [NQ]
+  uint64_t* k_full = q_full + NQ;              // [K_STAGES]
+  uint64_t* k_empty = k_full + K_STAGES;       // [K_STAGES]
+  uint64_t* v_full = k_empty + K_STAGES;       // [V_STAGES]
+  uint64_t* v_empty = v_full + V_STAGES;       // [V_STAGES]
+  uint64_t* factor_full = v_empty + V_STAGES;  // [V_STAGES]
+  uint64_t* raw_full = factor_full + V_STAGES;   // [RAW]
+  uint64_t* raw_empty = raw_full + RAW;          // [RAW]
+  uint64_t* s_full = raw_empty + RAW;      // [NQ][2]
   // (a warp can be a tile ahead of the others, so even and odd tiles have a barrier each: its two arrivals must not count for one)
   uint64_t* p_full = s_full + 2 * NQ;        // [NQ][2]
   uint64_t* pv_done = p_full + 2 * NQ;       // [NQ][2]
@@ -168,9 +174,18 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       mbar_init(&pv_done[2 * x], 1);
       mbar_init(&pv_done[2 * x + 1], 1);
     }
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&kv_full[s], CONV_WARPS);
-      mbar_init(&kv_empty[s], nq);
+    for (int s = 0; s < K_STAGES; ++s) {
+      mbar_init(&k_full[s], CONV_WARPS);
+      mbar_init(&k_empty[s], nq);
+    }
+    for (int s = 0; s < V_STAGES; ++s) {
+      mbar_init(&v_full[s], CONV_WARPS);
+      mbar_init(&v_empty[s], nq);
+      mbar_init(&factor_full[s], 1);
+    }
+    for (int s = 0; s < RAW; ++s) {
+      mbar_init(&raw_full[s], LOAD_WARPS * 32);
+      mbar_init(&raw_empty[s], CONV_WARPS);
     }
     mbar_init(ahead, 4);
     *abort_flag = 0;
@@ -183,6 +198,45 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   const uint32_t tmem_base = *tmem_slot;
   auto tmem_s = [&](int x, int t) { return tmem_base + (uint32_t)((2 * x + (t & 1)) * KEYS); };
   auto tmem_o = [&](int x) { return tmem_base + (uint32_t)(2 * NQ * KEYS + x * DP); };
+
+  // ------------------------------------------------ copies: two warps, 32 keys of a tile each, a lane a key for pages and scales
+  auto load_codes = [&](int lw) {
+    constexpr int CHUNKS = DP / 16, AT_ONCE = 32 / CHUNKS;  // 16-byte pieces of a row; rows of an instruction
+    constexpr uint32_t NOWHERE = 0xffffffffu;
+    const int c = lane % CHUNKS, key = lw * 32 + lane;
+    const int* table = p.tables + (size_t)seq * p.table_stride;
+    const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
+    auto look = [&](int j) {  // the page of the lane's key: a tile before it is needed
+      const int kp = min(keys.at(first + min(j, n_tiles - 1)) * KEYS + key, keys.hi - 1);
+      return __ldg(table + min(p.run_shift >= 0 ? kp >> p.run_shift : kp / p.bs, p.table_stride - 1));
+    };
+    int page = look(0);
+    for (int j = 0; j < n_tiles; ++j) {
+      const int kp = keys.at(first + j) * KEYS + key, off = p.run_shift >= 0 ? kp & (p.bs - 1) : kp % p.bs;
+      const bool mine = kp < keys.hi, paged = page >= 0 && page < p.n_blocks;
+      if (mine && !paged && (kp >= lo || kp < p.keep) && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);  // (pages behind a window may have gone back)
+      const uint32_t row = mine && paged ? ((uint32_t)page * p.nkv + kvh) * p.bs + off : NOWHERE;
+      page = look(j + 1);
+      if (j >= RAW && !warp_wait(&raw_empty[j % RAW], ((j / RAW) & 1) ^ 1, p.err, abort_flag)) break;
+      const uint32_t to = q8_shared(raw_s) + (j % RAW) * SH::RAW_STAGE, scales = to + 2 * KEYS * DP;
+      const bool ok = row != NOWHERE;
+      copy4(scales + key * 4, p.kscale + (ok ? row : 0u), ok);
+      copy4(scales + (KEYS + key) * 4, p.vscale + (ok ? row : 0u), ok);
+#pragma unroll
+      for (int i = 0; i < 32 / AT_ONCE; ++i) {
+        const int at = i * AT_ONCE + lane / CHUNKS;
+        const uint32_t its = __shfl_sync(0xffffffffu, row, at);
+        if (c * 16 < p.d) {  // (beyond the head's size anything will do: the queries are zeros there, and the results not stored)
+          const size_t src = (size_t)(its == NOWHERE ? 0u : its) * p.d + c * 16;  // (a key that is not there: zeros, masked)
+          const uint32_t dst = to + (lw * 32 + at) * DP + c * 16;
+          copy16(dst, p.kpool + src, its != NOWHERE);
+          copy16(dst + KEYS * DP, p.vpool + src, its != NOWHERE);
+        }
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&raw_full[j % RAW])) : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  };
 
   if (warp < SOFT_WARPS) {
     // ------------------------------------------------ a query row per thread
@@ -288,11 +342,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       return warp_wait(&pv_done[2 * x + ((j - 1) & 1)], ((j - 1) >> 1) & 1, p.err, abort_flag);
     };
     for (int j = 0; ok && j < n_tiles; ++j) {
-      const int st = j % STAGES;
+      const int st = j % V_STAGES;
       if (!warp_wait(&s_full[2 * x + (j & 1)], (j >> 1) & 1, p.err, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      // (long complete: the scores were made from the tile; for the factors that came with it)
-      if (!warp_wait(&kv_full[st], (j / STAGES) & 1, p.err, abort_flag)) { ok = false; break; }
+      // (long complete: they were written with the keys)
+      if (!warp_wait(&factor_full[st], (j / V_STAGES) & 1, p.err, abort_flag)) { ok = false; break; }
       const float* factor = factor_s + st * (SH::FACTORS / 4);
       const float4* kf4 = reinterpret_cast<const float4*>(factor);
       const float4 tile_e = kf4[3 * KEYS / 4];  // E, 2^-E, wide
@@ -447,77 +501,41 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   } else if (warp < SOFT_WARPS + CONV_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONV_REGS));
     // ------------------------------------------------ codes to operand tiles
-    // Every warp works for itself. Its lanes stand for the tile's keys lane and lane + 32 (pages, scales, the tile's exponent) and
-    // hand rows and factors round; it converts every fourth set of rows. A page is looked up a tile before its rows are asked for,
-    // and they three tiles before they are used, by asynchronous copies into places that are each thread's own: a load takes
-    // 1,700 to 2,700 clocks here, and with one tile on its way in registers a tile took as long.
+    // Every warp works for itself: its lanes stand for the tile's keys lane and lane + 32 (scales, the tile's exponent) and hand
+    // factors round; it converts every fourth set of rows. It asks for nothing from memory itself: what a thread has on its way
+    // would have to arrive before its fence between the two proxies is over, 1,700 to 2,700 clocks a tile.
     const int cw = warp - SOFT_WARPS;
     constexpr int ROWS_AT_ONCE = DP == 128 ? 4 : 8;         // of a warp: 16-byte pieces of keys or values
     constexpr int STEP = CONV_WARPS * ROWS_AT_ONCE, PER = KEYS / STEP;
     // (a warp's rows of a set are all among the tile's first 32 keys or all among its last)
-    // Eight lanes that store together have two rows of four pieces, and find eight places.
-    const int half = DP == 128 ? lane >> 4 : 0, quad = lane & 3, r0 = cw * ROWS_AT_ONCE + ((lane >> 2) & (ROWS_AT_ONCE - 1));
-    const int c = half * 4 + quad;
-    const int c_at = c * 16 < p.d ? c * 16 : 0;  // (beyond the head's size anything will do: the queries are zeros there, and
-                                                 // the results are not stored)
+    // Eight lanes that read and store together have four pieces each of two neighbouring rows, of different halves: eight places
+    // of 128 bytes where the codes are and eight where they go.
+    const int half = DP == 128 ? (lane >> 4) ^ ((lane >> 2) & 1) : 0, quad = lane & 3;
+    const int r0 = cw * ROWS_AT_ONCE + ((lane >> 2) & (ROWS_AT_ONCE - 1));
     const int place0 = half * SH::KV_HALF + r0 * 128 + (((2 * quad) ^ (r0 & 7)) << 4);
     const int place1 = half * SH::KV_HALF + r0 * 128 + (((2 * quad + 1) ^ (r0 & 7)) << 4);
-    const int* table = p.tables + (size_t)seq * p.table_stride;
-    const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
-    constexpr uint32_t NOWHERE = 0xffffffffu;
-    int page[2];                // of the tile that is asked for next
-    const uint32_t raw = q8_shared(raw_s) + (threadIdx.x - SOFT_WARPS * 32) * 16;
-    auto look = [&](int j) {
-      const int key0 = keys.at(first + min(j, n_tiles - 1)) * KEYS;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int kp = min(key0 + lane + 32 * h, keys.hi - 1);
-        page[h] = __ldg(table + min(p.run_shift >= 0 ? kp >> p.run_shift : kp / p.bs, p.table_stride - 1));
-      }
-    };
-    auto fetch = [&](int j) {
-      if (j < n_tiles) {
-        const int key0 = keys.at(first + j) * KEYS;
-        const uint32_t to = raw + (j % RAW) * SH::RAW_STAGE;
-        bool wrong = false;
-        uint32_t key_row[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int kp = key0 + lane + 32 * h, off = p.run_shift >= 0 ? kp & (p.bs - 1) : kp % p.bs;
-          const bool mine = kp < keys.hi, paged = page[h] >= 0 && page[h] < p.n_blocks;
-          wrong |= mine && !paged && (kp >= lo || kp < p.keep);  // (pages behind a window may have gone back)
-          key_row[h] = mine && paged ? ((uint32_t)page[h] * p.nkv + kvh) * p.bs + off : NOWHERE;
-          const bool ok = key_row[h] != NOWHERE;
-          copy4(to + 2 * PER * CONV * 16 + 8 * h, p.vscale + (ok ? key_row[h] : 0u), ok);
-          copy4(to + 2 * PER * CONV * 16 + 8 * h + 4, p.kscale + (ok ? key_row[h] : 0u), ok);
-        }
-        if (wrong && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const uint32_t row = __shfl_sync(0xffffffffu, r0 + i * STEP < 32 ? key_row[0] : key_row[1], (r0 + i * STEP) & 31);
-          const size_t at = (size_t)(row == NOWHERE ? 0u : row) * p.d + c_at;  // (a key that is not there: zeros, scales 0, masked)
-          copy16(to + 2 * i * CONV * 16, p.kpool + at, row != NOWHERE);
-          copy16(to + (2 * i + 1) * CONV * 16, p.vpool + at, row != NOWHERE);
-        }
-      }
-      copies_commit();
-    };
-    look(0);
-#pragma unroll
-    for (int j = 0; j < RAW; ++j) {
-      fetch(j);
-      look(j + 1);
-    }
+    const uint32_t raw = q8_shared(raw_s);
     asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
     float up, down;
     q8_query_scale(*q_top, up, down);
     const float key_factor = down * (OPT && p.cap > 0.f ? p.scale : p.scale_log2e);
     for (int j = 0; j < n_tiles; ++j) {
-      const int st = j % STAGES;
-      copies_wait<RAW - 1>();  // the thread's own copies of the tile
-      const uint32_t from = raw + (j % RAW) * SH::RAW_STAGE;
-      const uint4 scales = shared_16(from + 2 * PER * CONV * 16);
-      const float vs[2] = {__uint_as_float(scales.x), __uint_as_float(scales.z)}, ks[2] = {__uint_as_float(scales.y), __uint_as_float(scales.w)};
+      const int ks_at = j % K_STAGES, st = j % V_STAGES, from = j % RAW;
+      if (!warp_wait(&raw_full[from], (j / RAW) & 1, p.err, abort_flag)) break;
+      const uint32_t codes = raw + from * SH::RAW_STAGE, scales = codes + 2 * KEYS * DP;
+      float ks[2], vs[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ks[h] = shared_f(scales + (lane + 32 * h) * 4);
+        vs[h] = shared_f(scales + (KEYS + lane + 32 * h) * 4);
+      }
+      uint4 k[PER], v[PER];  // (all asked for before any is used)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t at = codes + (r0 + i * STEP) * DP + (half * 4 + quad) * 16;
+        k[i] = shared_16(at);
+        v[i] = shared_16(at + KEYS * DP);
+      }
       // the tile's exponent: the largest of its finite scales other than 0
       float e[2], f, inv;
       bool fine[2];
@@ -537,8 +555,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         const float x = fine[h] ? vs[h] * q8_pow2(V_LIFT - (wide ? e[h] : (float)hi)) : 0.f;
         factor2[h] = q8_pack(x, x);
       }
-      if (j >= STAGES && !warp_wait(&kv_empty[st], ((j / STAGES) & 1) ^ 1, p.err, abort_flag)) break;
-      uint8_t* kt = kv_s + st * SH::STAGE;
+      if (j >= V_STAGES && !warp_wait(&v_empty[st], ((j / V_STAGES) & 1) ^ 1, p.err, abort_flag)) break;
+      if (j >= K_STAGES && !warp_wait(&k_empty[ks_at], ((j / K_STAGES) & 1) ^ 1, p.err, abort_flag)) break;
+      uint8_t* kt = k_s + ks_at * SH::KV_TILE;
       if (cw == j % CONV_WARPS) {
         float* factor = factor_s + st * (SH::FACTORS / 4);
 #pragma unroll
@@ -552,20 +571,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
           }
         }
         if (lane == 0) *reinterpret_cast<float4*>(factor + 3 * KEYS) = make_float4((float)hi, q8_pow2(-(float)hi), wide ? 1.f : 0.f, 0.f);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&factor_full[st]);
       }
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const uint4 k = shared_16(from + 2 * i * CONV * 16);
-        const uint32_t w[4] = {k.x ^ 0x80808080u, k.y ^ 0x80808080u, k.z ^ 0x80808080u, k.w ^ 0x80808080u};
+        const uint32_t w[4] = {k[i].x ^ 0x80808080u, k[i].y ^ 0x80808080u, k[i].z ^ 0x80808080u, k[i].w ^ 0x80808080u};
         *reinterpret_cast<uint4*>(kt + place0 + i * STEP * 128) = make_uint4(q8_pair_lo(w[0]), q8_pair_hi(w[0]), q8_pair_lo(w[1]), q8_pair_hi(w[1]));
         *reinterpret_cast<uint4*>(kt + place1 + i * STEP * 128) = make_uint4(q8_pair_lo(w[2]), q8_pair_hi(w[2]), q8_pair_lo(w[3]), q8_pair_hi(w[3]));
       }
-      uint8_t* vt = kt + SH::KV_TILE;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[ks_at]);
+      uint8_t* vt = v_s + st * SH::KV_TILE;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const uint32_t times = __shfl_sync(0xffffffffu, r0 + i * STEP < 32 ? factor2[0] : factor2[1], (r0 + i * STEP) & 31);
-        const uint4 v = shared_16(from + (2 * i + 1) * CONV * 16);
-        const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+        const uint32_t w[4] = {v[i].x ^ 0x80808080u, v[i].y ^ 0x80808080u, v[i].z ^ 0x80808080u, v[i].w ^ 0x80808080u};
         uint32_t h[8];
 #pragma unroll
         for (int n = 0; n < 4; ++n) { h[2 * n] = q8_times(q8_pair_lo(w[n]), times); h[2 * n + 1] = q8_times(q8_pair_hi(w[n]), times); }
@@ -574,51 +596,57 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&kv_full[st]);
-      fetch(j + RAW);  // where the codes were that have just been converted
-      look(j + RAW + 1);
+      if (lane == 0) {
+        mbar_arrive(&v_full[st]);
+        mbar_arrive(&raw_empty[from]);
+      }
     }
-    copies_wait<0>();
   } else {
     // ------------------------------------------------ products: a warp per query tile; scores run a tile ahead
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ISSUE_REGS));
+    if (warp >= SOFT_WARPS + CONV_WARPS + NQ) {
+      load_codes(warp - SOFT_WARPS - CONV_WARPS - NQ);
+    } else {
     const int x = warp - SOFT_WARPS - CONV_WARPS;
     constexpr uint32_t idesc_qk = desc_f16(false, KEYS), idesc_pv = desc_f16(true, DP);
     bool ok = x < nq && warp_wait(&q_full[x], 0, p.err, abort_flag);
     // The second query tile starts half a tile behind the first, so that one's exponents run beside the other's maxima and sums.
     if (ok && x == 1) ok = warp_wait(ahead, 0, p.err, abort_flag);
     const uint64_t q_desc = smem_desc(smem_u32(q_s + x * SH::Q_BYTES));
-    const uint32_t kv_at = smem_u32(kv_s);
+    const uint32_t k_at = smem_u32(k_s), v_at = smem_u32(v_s);
     auto scores = [&](int t) {
-      const int st = t % STAGES;
-      if (!warp_wait(&kv_full[st], (t / STAGES) & 1, p.err, abort_flag)) return false;
+      const int st = t % K_STAGES;
+      if (!warp_wait(&k_full[st], (t / K_STAGES) & 1, p.err, abort_flag)) return false;
       tc_fence_after();
-      const uint64_t kd = smem_desc(kv_at + st * SH::STAGE);
+      const uint64_t kd = smem_desc(k_at + st * SH::KV_TILE);
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
           umma_bf16(tmem_s(x, t), q_desc + (uint64_t)(((k / 4) * SH::Q_HALF + (k % 4) * 32) >> 4),
                     kd + (uint64_t)(((k / 4) * SH::KV_HALF + (k % 4) * 32) >> 4), idesc_qk, k > 0);
         umma_commit(&s_full[2 * x + (t & 1)]);
+        umma_commit(&k_empty[st]);
       }
       __syncwarp();
       return true;
     };
     ok = ok && scores(0) && (n_tiles < 2 || scores(1));
     for (int j = 0; ok && j < n_tiles; ++j) {
-      const int st = j % STAGES;
-      if (!warp_wait(&p_full[2 * x + (j & 1)], (j >> 1) & 1, p.err, abort_flag)) break;
+      const int st = j % V_STAGES;
+      if (!warp_wait(&p_full[2 * x + (j & 1)], (j >> 1) & 1, p.err, abort_flag) ||
+          !warp_wait(&v_full[st], (j / V_STAGES) & 1, p.err, abort_flag)) break;
       tc_fence_after();
-      const uint64_t vd = desc_mnmajor(kv_at + st * SH::STAGE + SH::KV_TILE, SH::KV_HALF, 1024);
+      const uint64_t vd = desc_mnmajor(v_at + st * SH::KV_TILE, SH::KV_HALF, 1024);
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < KEYS / 16; ++k)
           umma_bf16_tmem_a(tmem_o(x), tmem_s(x, j) + k * 8, vd + (uint64_t)((k * 2048) >> 4), idesc_pv, j > 0 || k > 0);
-        umma_commit(&kv_empty[st]);
+        umma_commit(&v_empty[st]);
         umma_commit(&pv_done[2 * x + (j & 1)]);
       }
       __syncwarp();
       if (j + 2 < n_tiles && !scores(j + 2)) break;
+    }
     }
   }
   __syncwarp();
