@@ -7,7 +7,7 @@
 //   S[128 rows, 64 keys]  = Q K^T      Q and K as 16-bit floats in shared memory (K-major, 128-byte swizzle)
 //   O[128 rows, d]       += W V        W from tensor memory, where S was; V as 16-bit floats in shared memory (MN-major)
 //
-// Two warps copy codes from the pages, three tiles ahead; four turn them into 16-bit floats and store them as operand tiles, with
+// A warp or two copy codes from the pages, three tiles ahead; four turn them into 16-bit floats and store them as operand tiles, with
 // each key's factors beside them; four warps per query tile own a row per thread (a lane of tensor memory) and turn scores into
 // weights; a warp per query tile issues its products. Where the two query tiles share a converted tile, the conversion is a
 // seventh of the block's instructions.
@@ -160,6 +160,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   const uint32_t per_head = (65536u + G - 1) / G;  // a row of a query tile over G: right for up to 128 of both
   auto token_of = [&](int row) { return (int)(((uint32_t)row * per_head) >> 16); };
 
+  // Pages of a power of two of positions, four at least: a page's part of a tile is a run of bytes in each of the four pools.
+  const bool runs = p.run_shift >= 2 && (((uintptr_t)p.kscale | (uintptr_t)p.vscale) & 15) == 0;
   if (warp == SOFT_WARPS + CONV_WARPS) {
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       mbar_init(&factor_full[s], 1);
     }
     for (int s = 0; s < RAW; ++s) {
-      mbar_init(&raw_full[s], LOAD_WARPS * 32);
+      mbar_init(&raw_full[s], runs ? 1 : LOAD_WARPS * 32);
       mbar_init(&raw_empty[s], CONV_WARPS);
     }
     mbar_init(ahead, 4);
@@ -199,13 +201,48 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   auto tmem_s = [&](int x, int t) { return tmem_base + (uint32_t)((2 * x + (t & 1)) * KEYS); };
   auto tmem_o = [&](int x) { return tmem_base + (uint32_t)(2 * NQ * KEYS + x * DP); };
 
-  // ------------------------------------------------ copies: two warps, 32 keys of a tile each, a lane a key for pages and scales
+  // ------------------------------------------------ copies, RAW tiles ahead
   auto load_codes = [&](int lw) {
+    const int* table = p.tables + (size_t)seq * p.table_stride;
+    const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
+    if (runs) {
+      // One warp, a lane a page: four bulk copies each. Positions from keys.hi on come along where their page does; what converts
+      // them takes their scales for 0. (A page behind a window may have gone back, another that is not there is an error: page 0
+      // comes instead; its keys are masked, or the step is lost.)
+      if (lw > 0) return;
+      const int run = min(p.bs, KEYS), n = KEYS / run;
+      auto look = [&](int j) {
+        const int kp = min(keys.at(first + min(j, n_tiles - 1)) * KEYS + lane * run, keys.hi - 1);
+        return __ldg(table + min(kp >> p.run_shift, p.table_stride - 1));
+      };
+      int page[2] = {look(0), look(1)};  // (two tiles ahead: the next use does not wait for them)
+      for (int j = 0; j < n_tiles; ++j) {
+        const int kp = keys.at(first + j) * KEYS + lane * run;
+        const bool mine = lane < n && kp < keys.hi, paged = page[0] >= 0 && page[0] < p.n_blocks;
+        if (mine && !paged && (kp + run > lo || kp < p.keep) && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+        const uint32_t row = ((uint32_t)(paged ? page[0] : 0) * p.nkv + kvh) * p.bs + (kp & (p.bs - 1));
+        page[0] = page[1];
+        page[1] = look(j + 2);
+        if (j >= RAW && !warp_wait(&raw_empty[j % RAW], ((j / RAW) & 1) ^ 1, p.err, abort_flag)) break;
+        uint8_t* to = raw_s + (j % RAW) * SH::RAW_STAGE;
+        uint64_t* bar = &raw_full[j % RAW];
+        const int pages = __popc(__ballot_sync(0xffffffffu, mine));
+        if (lane == 0) mbar_expect_tx(bar, pages * run * (2 * p.d + 8));
+        __syncwarp();
+        if (mine) {
+          const size_t at = (size_t)row * p.d;
+          bulk_load(to + lane * run * p.d, p.kpool + at, bar, run * p.d);
+          bulk_load(to + KEYS * DP + lane * run * p.d, p.vpool + at, bar, run * p.d);
+          bulk_load(to + 2 * KEYS * DP + lane * run * 4, p.kscale + row, bar, run * 4);
+          bulk_load(to + 2 * KEYS * DP + (KEYS + lane * run) * 4, p.vscale + row, bar, run * 4);
+        }
+      }
+      return;
+    }
+    // Two warps, 32 keys of a tile each, a lane a key for pages and scales.
     constexpr int CHUNKS = DP / 16, AT_ONCE = 32 / CHUNKS;  // 16-byte pieces of a row; rows of an instruction
     constexpr uint32_t NOWHERE = 0xffffffffu;
     const int c = lane % CHUNKS, key = lw * 32 + lane;
-    const int* table = p.tables + (size_t)seq * p.table_stride;
-    const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
     auto look = [&](int j) {  // the page of the lane's key: a tile before it is needed
       const int kp = min(keys.at(first + min(j, n_tiles - 1)) * KEYS + key, keys.hi - 1);
       return __ldg(table + min(p.run_shift >= 0 ? kp >> p.run_shift : kp / p.bs, p.table_stride - 1));
@@ -226,9 +263,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       for (int i = 0; i < 32 / AT_ONCE; ++i) {
         const int at = i * AT_ONCE + lane / CHUNKS;
         const uint32_t its = __shfl_sync(0xffffffffu, row, at);
-        if (c * 16 < p.d) {  // (beyond the head's size anything will do: the queries are zeros there, and the results not stored)
+        if (c * 16 < p.d) {
           const size_t src = (size_t)(its == NOWHERE ? 0u : its) * p.d + c * 16;  // (a key that is not there: zeros, masked)
-          const uint32_t dst = to + (lw * 32 + at) * DP + c * 16;
+          const uint32_t dst = to + (lw * 32 + at) * p.d + c * 16;
           copy16(dst, p.kpool + src, its != NOWHERE);
           copy16(dst + KEYS * DP, p.vpool + src, its != NOWHERE);
         }
@@ -515,6 +552,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const int place0 = half * SH::KV_HALF + r0 * 128 + (((2 * quad) ^ (r0 & 7)) << 4);
     const int place1 = half * SH::KV_HALF + r0 * 128 + (((2 * quad + 1) ^ (r0 & 7)) << 4);
     const uint32_t raw = q8_shared(raw_s);
+    // (beyond the head's size anything will do: the queries are zeros there, and the results are not stored)
+    const int piece = (half * 4 + quad) * 16 < p.d ? (half * 4 + quad) * 16 : 0;
     asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
     float up, down;
     q8_query_scale(*q_top, up, down);
@@ -526,13 +565,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       float ks[2], vs[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        ks[h] = shared_f(scales + (lane + 32 * h) * 4);
-        vs[h] = shared_f(scales + (KEYS + lane + 32 * h) * 4);
+        const bool seen = keys.at(first + j) * KEYS + lane + 32 * h < keys.hi;  // (by some row)
+        ks[h] = seen ? shared_f(scales + (lane + 32 * h) * 4) : 0.f;
+        vs[h] = seen ? shared_f(scales + (KEYS + lane + 32 * h) * 4) : 0.f;
       }
       uint4 k[PER], v[PER];  // (all asked for before any is used)
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const uint32_t at = codes + (r0 + i * STEP) * DP + (half * 4 + quad) * 16;
+        const uint32_t at = codes + (r0 + i * STEP) * p.d + piece;
         k[i] = shared_16(at);
         v[i] = shared_16(at + KEYS * DP);
       }
