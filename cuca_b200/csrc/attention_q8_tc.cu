@@ -37,7 +37,7 @@ constexpr int NTHREADS = (SOFT_WARPS + CONV_WARPS + NQ + LOAD_WARPS) * 32;  // s
 constexpr int SOFT_REGS = 176, CONV_REGS = 88, ISSUE_REGS = 64;
 // Operand tiles of keys are free again when their scores are there, those of values only after the weights' product: with three
 // of both, a tile's way round (conversion, scores, softmax, product: some 6,000 clocks) set the pace and not any unit.
-constexpr int K_STAGES = 2, V_STAGES = 4;
+constexpr int K_STAGES = 3, V_STAGES = 3;
 constexpr int RAW = 3;            // tiles of codes on their way
 constexpr float V_LIFT = 7.f;     // values are 2^7 larger in the operand tile: 127 2^7 2 is the most that fits
 constexpr int WIDE = 20;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       mbar_init(&factor_full[s], 1);
     }
     for (int s = 0; s < RAW; ++s) {
-      mbar_init(&raw_full[s], runs ? 1 : LOAD_WARPS * 32);
+      mbar_init(&raw_full[s], LOAD_WARPS * (runs ? 1 : 32));
       mbar_init(&raw_empty[s], CONV_WARPS);
     }
     mbar_init(ahead, 4);
@@ -206,10 +206,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const int* table = p.tables + (size_t)seq * p.table_stride;
     const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
     if (runs) {
-      // One warp, a lane a page: four bulk copies each. Positions from keys.hi on come along where their page does; what converts
-      // them takes their scales for 0. (A page behind a window may have gone back, another that is not there is an error: page 0
-      // comes instead; its keys are masked, or the step is lost.)
-      if (lw > 0) return;
+      // A warp for the keys, one for the values (a copy takes its thread some 100 clocks), a lane a page: codes and scales.
+      // Positions from keys.hi on come along where their page does; what converts them takes their scales for 0. (A page behind a
+      // window may have gone back, another that is not there is an error: page 0 comes instead; its keys are masked, or the step
+      // is lost.)
+      const int8_t* pool = lw == 0 ? p.kpool : p.vpool;
+      const float* scales = lw == 0 ? p.kscale : p.vscale;
       const int run = min(p.bs, KEYS), n = KEYS / run;
       auto look = [&](int j) {
         const int kp = min(keys.at(first + min(j, n_tiles - 1)) * KEYS + lane * run, keys.hi - 1);
@@ -227,14 +229,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         uint8_t* to = raw_s + (j % RAW) * SH::RAW_STAGE;
         uint64_t* bar = &raw_full[j % RAW];
         const int pages = __popc(__ballot_sync(0xffffffffu, mine));
-        if (lane == 0) mbar_expect_tx(bar, pages * run * (2 * p.d + 8));
+        if (lane == 0) mbar_expect_tx(bar, pages * run * (p.d + 4));
         __syncwarp();
         if (mine) {
-          const size_t at = (size_t)row * p.d;
-          bulk_load(to + lane * run * p.d, p.kpool + at, bar, run * p.d);
-          bulk_load(to + KEYS * DP + lane * run * p.d, p.vpool + at, bar, run * p.d);
-          bulk_load(to + 2 * KEYS * DP + lane * run * 4, p.kscale + row, bar, run * 4);
-          bulk_load(to + 2 * KEYS * DP + (KEYS + lane * run) * 4, p.vscale + row, bar, run * 4);
+          bulk_load(to + lw * KEYS * DP + lane * run * p.d, pool + (size_t)row * p.d, bar, run * p.d);
+          bulk_load(to + 2 * KEYS * DP + (lw * KEYS + lane * run) * 4, scales + row, bar, run * 4);
         }
       }
       return;
