@@ -1667,7 +1667,8 @@ def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, 
         n, nkv, d, _at(err), _stream())), "read_q8")
 
 
-Q8_FEW_ROWS = 16  # query rows of a key head that the form for few rows takes of a portion
+Q8_FEW_ROWS = 24  # query rows of a key head that the form for few rows takes of a portion
+Q8_SINGLES_ALONG = 0.25  # single tokens for each portion of a step that go with the portions through tcgen05
 
 
 class QuantizedPlan:
@@ -1713,16 +1714,18 @@ class QuantizedPlan:
         rows a block, `width` column tiles of 8; 1: tcgen05, `width` query tiles of 128"""
         key = (n_heads, n_kv_heads, head_dim, dtype, window, keep)
         if key not in self._launches:
-            group, out, few = n_heads // n_kv_heads, [], self.longest
-            if dtype == torch.bfloat16 and head_dim <= 128 and group <= 128:
-                few = Q8_FEW_ROWS // group
-            if 1 in self.counts:
+            group, out = n_heads // n_kv_heads, []
+            singles = self.counts.count(1)
+            portions = len(self.counts) - singles
+            # Portions go together: where the longest has few rows a block of few rows each, else all through tcgen05 (twelve
+            # requests of up to 9 tokens: those of up to four apart from the rest 56 us, together 46).
+            many = (portions and dtype == torch.bfloat16 and head_dim <= 128 and group <= 128
+                    and self.longest * group > Q8_FEW_ROWS)
+            least = 1 if many and singles <= portions * Q8_SINGLES_ALONG else 2
+            if singles and least == 2:
                 out.append(self._few(1, 1, *key))
-            most = max((c for c in self.counts if c <= few), default=0)
-            if most > 1:
-                out.append(self._few(2, most, *key))
-            if self.longest > max(few, 1):
-                out.append(self._many(max(few, 1) + 1, self.longest, *key))
+            if portions:
+                out.append((self._many if many else self._few)(least, self.longest, *key))
             self._launches[key] = out
         return self._launches[key]
 
