@@ -8,7 +8,8 @@
 //
 // A block (4 warps) takes one tile of rows, one key head and a share of the keys; its warps take the groups of 16 keys in
 // turn, each through a ring of its own (16-byte asynchronous copies straight from the pages, no barrier in the loop), and are
-// joined at the end; shares of a tile's keys are joined by a second small launch. A thread's values sit in shared memory so
+// joined at the end; shares of a tile's keys are joined through distributed shared memory, their blocks being a cluster, where
+// there are 2, 4 or 8 of them and all blocks are resident at once, else by a second small launch. A thread's values sit in shared memory so
 // that it reads its fragments 16 bytes at a time without bank conflicts (`place`), and the order of dimensions and keys
 // within an instruction is chosen to match: a contraction may be summed in any order.
 //
@@ -31,6 +32,27 @@ __device__ __forceinline__ uint32_t turned_8x8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
+}
+
+// A barrier over every thread of the cluster, and loads from the shared memory of one of its blocks.
+constexpr int MOST_CLUSTER = 8;
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_at(uint32_t at, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 cluster_2(uint32_t at, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_at(at, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_4(uint32_t at, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_at(at, rank)) : "memory");
+  return v;
 }
 
 // DP: the head size rounded up to 64, 128 or 256 (what is beyond d stays zero).
@@ -91,8 +113,15 @@ attention_q8_kernel(const Q8Params p) {
   const int share = p.chunk > 0 ? p.chunk / GROUP : keys.groups;
   const int first = blockIdx.x * share;
   const int last = (int)blockIdx.x == p.n_splits - 1 ? keys.groups : min(keys.groups, first + share);
-  if (first >= last) return;  // a share that this tile does not have
   const bool alone = share >= keys.groups || p.n_splits == 1;
+  const bool as_cluster = !alone && p.part == nullptr;  // the shares' blocks are a cluster
+  if (first >= last) {  // a share that this tile does not have
+    if (as_cluster) {
+      cluster_sync();
+      cluster_sync();
+    }
+    return;
+  }
   const int* table = p.tables + (size_t)seq * p.table_stride;
 
   // ---------------------------------------------------------------- queries: the second operand's fragments
@@ -429,6 +458,7 @@ attention_q8_kernel(const Q8Params p) {
   constexpr int OS = DP + 4;  // floats between columns
   float* o_s = reinterpret_cast<float*>(smem);             // [WARPS][COLS][OS]
   float* ml_s = o_s + WARPS * COLS * OS;                   // [WARPS][COLS][2]
+  float* ml_all = ml_s + WARPS * COLS * 2;                 // [COLS][2]: of the block
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -471,16 +501,56 @@ attention_q8_kernel(const Q8Params p) {
       T* dst = (T*)p.out + (size_t)(row0 + col / heads) * p.out_stride + (size_t)head * p.d + e;
 #pragma unroll
       for (int k = 0; k < 4; ++k) dst[k] = from_f32<T>(o[k] * inv);
+    } else if (as_cluster) {  // (the first warp's place: nobody else reads it)
+      *reinterpret_cast<float4*>(o_s + col * OS + e) = make_float4(o[0], o[1], o[2], o[3]);
+      if (e == 0) *reinterpret_cast<float2*>(ml_all + 2 * col) = make_float2(top, den);
     } else {
       float* part = p.part + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.n_splits + blockIdx.x) * (COLS * (p.d + 2));
       *reinterpret_cast<float4*>(part + col * p.d + e) = make_float4(o[0], o[1], o[2], o[3]);
       if (e == 0) *reinterpret_cast<float2*>(part + COLS * p.d + 2 * col) = make_float2(top, den);
     }
   }
+  if (!as_cluster) return;
+
+  // ---------------------------------------------------------------- the shares joined, in their order, out of one another's
+  // shared memory; each block of the cluster writes a part of the rows
+  cluster_sync();
+  const int used = min(p.n_splits, (keys.groups + share - 1) / share);
+  const uint32_t o_at = q8_shared(o_s), ml_at = q8_shared(ml_all);
+  for (int i = blockIdx.x * WARPS * 32 + threadIdx.x; i < n_cols * per_col; i += used * WARPS * 32) {
+    const int col = i / per_col, e = (i % per_col) * 4;
+    float2 ml[MOST_CLUSTER];
+    float4 v[MOST_CLUSTER];
+    float top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < MOST_CLUSTER; ++s) {
+      ml[s] = make_float2(-INFINITY, 0.f);
+      v[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s < used) {
+        ml[s] = cluster_2(ml_at + col * 8, s);
+        v[s] = cluster_4(o_at + (col * OS + e) * 4, s);
+      }
+      top = fmaxf(top, ml[s].x);
+    }
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+    for (int s = 0; s < MOST_CLUSTER; ++s) {
+      const float f = ml[s].x == top ? 1.f : q8_exp2(ml[s].x - top);
+      o[0] += f * v[s].x; o[1] += f * v[s].y; o[2] += f * v[s].z; o[3] += f * v[s].w;
+      den += f * ml[s].y;
+    }
+    const int head = head0 + col % heads;
+    if (OPT && p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    T* dst = (T*)p.out + (size_t)(row0 + col / heads) * p.out_stride + (size_t)head * p.d + e;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) dst[k] = from_f32<T>(o[k] * inv);
+  }
+  cluster_sync();  // nobody leaves while another reads its memory
 }
 
-// Joins the shares of a tile's keys, in their order: a warp per query row. Its lanes take two shares' maxima and sums each (there are 64 at most), then
-// four dimensions (of each 128).
+// Joins the shares of a tile's keys, in their order: a warp per query row. Its lanes take two shares' maxima and sums each (there
+// are 64 at most), then four dimensions (of each 128).
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32) join_q8_kernel(const Q8Params p, int cols) {
   pdl_trigger();
@@ -537,7 +607,7 @@ template <int DP, int NT, int PARTS>
 constexpr int smem_bytes() {
   const int ring = WARPS * Ring<DP>::WARP + (NT * DP > 256 ? (DP / 16) * NT * 32 * 8 : 0);
   const int cols = NT * 8 / PARTS;
-  const int join = WARPS * cols * (DP + 4 + 2) * 4;
+  const int join = (WARPS * cols * (DP + 4 + 2) + cols * 2) * 4;
   return ring > join ? ring : join;
 }
 
@@ -547,7 +617,14 @@ int launch_q8(const Q8Params& p, int n_tiles, cudaStream_t stream) {
   auto kernel = attention_q8_kernel<DP, NT, PARTS, OPT>;
   static cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   CUCA_REQUIRE(configured == cudaSuccess, "attention_q8: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(configured));
-  cuca_launch(kernel, dim3(p.n_splits, p.nkv * p.head_parts, n_tiles), dim3(WARPS * 32), smem, stream, true, p);
+  const dim3 grid(p.n_splits, p.nkv * p.head_parts, n_tiles);
+  if (p.n_splits > 1 && p.part == nullptr) {
+    CUCA_REQUIRE(p.n_splits <= MOST_CLUSTER, "attention_q8: %d shares do not join as a cluster", p.n_splits);
+    cuca_launch_cluster(kernel, grid, dim3(WARPS * 32), smem, stream, true, p.n_splits, p);
+    CUCA_CHECK_LAUNCH("attention_q8");
+    return 0;
+  }
+  cuca_launch(kernel, grid, dim3(WARPS * 32), smem, stream, true, p);
   CUCA_CHECK_LAUNCH("attention_q8");
   if (p.n_splits > 1) {
     auto join = join_q8_kernel<typename std::conditional<PARTS == 2, float, __nv_bfloat16>::type>;
@@ -575,7 +652,7 @@ int launch_q8_nt(const Q8Params& p, int nt, int n_tiles, cudaStream_t stream) {
 
 // bfloat16 or 32-bit rows; tile_tokens rows of a request and heads_per_cta query heads to a block of `width` (1, 2, 4; not 4 beyond
 // 128 dimensions) column tiles. part: [n_tiles][nkv * pieces of a group][n_splits][8 width / parts][d + 2] floats where
-// n_splits > 1 (parts: 2 for 32-bit rows, else 1).
+// n_splits > 1 (parts: 2 for 32-bit rows, else 1), or null: the shares (8 at most) join as a cluster.
 CUCA_API int cuca_attention_q8(const CucaQ8Attention* c) {
   if (c->n_tiles == 0) return 0;
   Q8Params p;

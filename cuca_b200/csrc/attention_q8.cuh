@@ -243,7 +243,7 @@ inline int q8_params(const CucaQ8Attention& c, const char* name, int most_d, Q8P
   CUCA_REQUIRE(c.q_stride < (1ll << 31) && c.out_stride < (1ll << 31), "%s: rows too far apart", name);
   CUCA_REQUIRE(c.n_tiles > 0 && c.n_tiles <= 65535, "%s: %lld tiles", name, (long long)c.n_tiles);
   CUCA_REQUIRE(c.chunk >= 0 && c.chunk % 64 == 0 && c.n_splits >= 1 && c.n_splits <= 64 &&
-               (c.n_splits == 1 || (c.chunk > 0 && c.part && ((uintptr_t)c.part & 15) == 0)), "%s: bad shares of the keys", name);
+               (c.n_splits == 1 || c.chunk > 0) && ((uintptr_t)c.part & 15) == 0, "%s: bad shares of the keys", name);
   const int group = (int)(c.nh / c.nkv);
   CUCA_REQUIRE(c.heads_per_cta > 0 && c.heads_per_cta <= group && c.tile_tokens > 0 && c.tile_tokens <= 65536, "%s: bad tiles", name);
   p.q = c.q; p.q_stride = (int)c.q_stride; p.out = c.out; p.out_stride = (int)c.out_stride;

@@ -773,6 +773,7 @@ CUCA_API int cuca_attention_q8_tc(const CucaQ8Attention* c) {
   if (const int code = q8_params(*c, "attention_q8_tc", 128, p)) return code;
   const int group = p.nh / p.nkv;
   CUCA_REQUIRE(c->dtype == CUCA_BF16 && group <= ROWS && p.heads_per_cta == group, "attention_q8_tc: bfloat16 rows and groups of at most %d heads", ROWS);
+  CUCA_REQUIRE(p.n_splits == 1 || p.part, "attention_q8_tc: no place for the shares' results");
   CUCA_REQUIRE((long long)p.n_blocks * p.nkv * p.bs < 0xffffffffll, "attention_q8_tc: more than 2^32 rows in the pools");
   CUCA_REQUIRE((c->width == 1 || c->width == NQ) && p.tile_tokens == (int)c->width * (ROWS / group), "attention_q8_tc: %d rows to %lld query tiles",
                p.tile_tokens, (long long)c->width);

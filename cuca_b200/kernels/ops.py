@@ -1780,12 +1780,25 @@ def _q8_shares(blocks: int, keys: int, longest: int, head_dim: int, nt: int, sms
     11.6 us, 256 10.5, 512 12.7)."""
     if sms is None:
         sms = sm_count()
-    resident = sms * max(1, 3 * 128 // (max(64, head_dim) * nt))
+    resident = _q8_resident(sms, head_dim, nt)
     share = max(Q8_LEAST_SHARE, -(-keys // max(1, Q8_UNITS * resident) // 64) * 64)
     share = max(share, -(-longest // 64 // 64) * 64)  # at most 64 shares
     if blocks == 0 or share >= longest:
         return 0, 1
-    return share, min(64, -(-(longest + 32) // share))
+    shares = min(64, -(-(longest + 32) // share))
+    for n in (8, 4, 2):  # few of them: as many as join as a cluster
+        if n >= shares > n // 2 or (n < shares <= 10 and n == 8):
+            while n > 1 and not _merge_as_cluster(blocks, n, resident):
+                n //= 2
+            if n > 1:
+                return -(-(longest + 32) // (64 * n)) * 64, n
+            break
+    return share, shares
+
+
+def _q8_resident(sms: int, head_dim: int, nt: int) -> int:
+    """Blocks of the form for few rows that the GPU holds at once: three an SM with one column tile of 128 dimensions."""
+    return sms * max(1, 3 * 128 // (max(64, head_dim) * nt))
 
 
 def attention_q8_plan(step) -> QuantizedPlan:
@@ -1821,7 +1834,9 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
     for form, lo, hi, tokens, tiles, heads, width, share, shares in plan.launches(n_heads, n_kv_heads, head_dim, q.dtype,
                                                                                   window or None, opt.keep):
         part, at = None, 0
-        if shares > 1:  # the shares' results, joined by a second launch
+        if shares > 1 and (form == 1 or not _merge_as_cluster(tiles * n_kv_heads * -(-group // heads), shares,
+                                                              _q8_resident(sm_count(), head_dim, width))):
+            # the shares' results, joined by a second launch
             cols = 8 * width // (2 if code == F32 else 1)
             part = torch.empty(tiles * n_kv_heads * shares * (256 * (64 if head_dim <= 64 else 128) + 512) if form == 1 else
                                tiles * n_kv_heads * -(-group // heads) * shares * cols * (head_dim + 2), dtype=torch.float32,
