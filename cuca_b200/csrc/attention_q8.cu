@@ -16,11 +16,12 @@
 // Decoding is bound by the pages' bytes: 16 keys of 128 are 4.2 KB and some 270 warp instructions (176 of them turn codes into
 // 16-bit floats).
 #include "attention_q8.cuh"
+#include <type_traits>
 
 namespace {
 
 constexpr int GROUP = 16;     // keys of a step
-constexpr int STAGES = 4;     // of a warp's ring
+constexpr int STAGES = 3;     // of a warp's ring (four, with three blocks an SM: 64 ragged requests 118 us, not 114; five 134)
 constexpr int WARPS = 4;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -34,6 +35,18 @@ __device__ __forceinline__ uint32_t turned_8x8(uint32_t a) {
   return d;
 }
 
+// 16 bytes (none, and zeros: bytes 0) with constant offsets on both sides
+template <int DST, int SRC>
+__device__ __forceinline__ void copy16_at(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16, %4;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC), "r"(bytes) : "memory");
+}
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void for_each(F f) {  // f(0), .. f(N - 1), each a constant
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    for_each<N, I + 1>(f);
+  }
+}
 // A barrier over every thread of the cluster, and loads from the shared memory of one of its blocks.
 constexpr int MOST_CLUSTER = 8;
 __device__ __forceinline__ void cluster_sync() {
@@ -214,6 +227,8 @@ attention_q8_kernel(const Q8Params p) {
   // runs of bytes a group. `find` gives the page, `fetch` checks it and asks for the rows; the look goes out a step before.
   const bool in_page = p.run_shift >= 4 && p.d == DP;
   constexpr int KEYS_AT_ONCE = 32 / CHUNKS;
+  const uint32_t place_even = R::place(lane / CHUNKS, lane % CHUNKS);
+  const uint32_t place_odd = R::place(4 + lane / CHUNKS, lane % CHUNKS) - 4 * DP;
   const int lo = p.window > 0 ? pos0 - (p.window - 1) : 0;
   // Else lane k of 16: the page of key k of the group.
   auto find = [&](int j) -> int {
@@ -236,12 +251,16 @@ attention_q8_kernel(const Q8Params p) {
       const size_t row = ((size_t)(paged ? blk : 0) * p.nkv + kvh) * p.bs + (key0 & (p.bs - 1));
       const int8_t* kr = p.kpool + row * DP + lane * 16;
       const int8_t* vr = p.vpool + row * DP + lane * 16;
-#pragma unroll
-      for (int i = 0; i < GROUP / KEYS_AT_ONCE; ++i) {
-        const int k = i * KEYS_AT_ONCE + lane / CHUNKS;
-        copy16(at + R::place(k, c), kr + i * 512, paged);
-        copy16(at + R::TENSOR + R::place(k, c), vr + i * 512, paged);
-      }
+      const uint32_t bytes = paged ? 16u : 0u;
+      for_each<GROUP / KEYS_AT_ONCE>([&](auto n) {
+        constexpr int i = decltype(n)::value;
+        // Where the lane's piece of row i * KEYS_AT_ONCE + lane / CHUNKS goes, less i * 512: the place turns with the row's lowest
+        // three bits, of which the lane gives all but the highest (all, with half rows; the lowest, with rows of 256).
+        const uint32_t to = at + (DP == 256 ? R::place(i * KEYS_AT_ONCE + lane / CHUNKS, c) - i * 512 :
+                                  (i * KEYS_AT_ONCE) & 4 ? place_odd : place_even);
+        copy16_at<i * 512, i * 512>(to, kr, bytes);
+        copy16_at<R::TENSOR + i * 512, i * 512>(to, vr, bytes);
+      });
       copy4(at + 2 * R::TENSOR + lane * 4, (lane < 16 ? p.kscale : p.vscale) + row + (lane & 15), paged);
       return;
     }

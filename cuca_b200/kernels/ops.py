@@ -1781,7 +1781,7 @@ def _q8_shares(blocks: int, keys: int, longest: int, head_dim: int, nt: int, sms
     if sms is None:
         sms = sm_count()
     resident = _q8_resident(sms, head_dim, nt)
-    share = max(Q8_LEAST_SHARE, -(-keys // max(1, Q8_UNITS * resident) // 64) * 64)
+    share = max(Q8_LEAST_SHARE, -(-keys // max(1, int(Q8_UNITS * resident)) // 64) * 64)
     share = max(share, -(-longest // 64 // 64) * 64)  # at most 64 shares
     if blocks == 0 or share >= longest:
         return 0, 1
@@ -1797,8 +1797,8 @@ def _q8_shares(blocks: int, keys: int, longest: int, head_dim: int, nt: int, sms
 
 
 def _q8_resident(sms: int, head_dim: int, nt: int) -> int:
-    """Blocks of the form for few rows that the GPU holds at once: three an SM with one column tile of 128 dimensions."""
-    return sms * max(1, 3 * 128 // (max(64, head_dim) * nt))
+    """Blocks of the form for few rows that the GPU holds at once: four an SM with one column tile of 128 dimensions."""
+    return sms * max(1, 4 * 128 // (max(64, head_dim) * nt))
 
 
 def attention_q8_plan(step) -> QuantizedPlan:
