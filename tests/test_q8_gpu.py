@@ -381,3 +381,36 @@ def test_portions_give_the_same_bits_in_every_run(heads, kv, dim, counts, starts
     first = _check(c)
     for _ in range(60):
         assert torch.equal(first, _attend(c))
+
+
+def test_no_rows_attend_to_nothing():
+    c = Case(4, 2, 64, 16, [], [], torch.bfloat16)
+    assert _attend(c).numel() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cluster", [True, False])
+@pytest.mark.parametrize("starts", [[600], [700, 3], [1500, 0, 40], [2500]])
+def test_shares_join_through_a_cluster_and_through_memory(monkeypatch, starts, cluster, dtype):
+    from cuca_b200.kernels import ops
+    monkeypatch.setattr(ops, "CLUSTER_MERGE", cluster)
+    c = Case(8, 2, 128, 16, [1] * len(starts), starts, dtype, seed=len(starts))
+    *_, share, shares = ops.attention_q8_plan(c.step).launches(8, 2, 128, dtype, None, 0)[0]
+    assert shares > 1
+    if cluster:
+        assert shares in (2, 4, 8)
+    got = _check(c, sink=True)
+    assert torch.equal(got, _attend(c, sink=True))
+    _check(c, window=300, keep_first=5, softcap=20.0)
+
+
+@pytest.mark.parametrize("few,along", [(0, 0.0), (0, 10.0), (24, 0.0), (10 ** 6, 0.0)])
+def test_a_mixed_step_in_every_form(monkeypatch, few, along):
+    """Portions through blocks of few rows or through tcgen05, single tokens apart or with them."""
+    from cuca_b200.kernels import ops
+    monkeypatch.setattr(ops, "Q8_FEW_ROWS", few)
+    monkeypatch.setattr(ops, "Q8_SINGLES_ALONG", along)
+    for heads, kv, dim in ((8, 2, 64), (5, 1, 112)):
+        c = Case(heads, kv, dim, 16, *BATCHES["mixed"], torch.bfloat16, seed=few % 7)
+        _check(c)
+        _check(c, window=33, keep_first=2, sink=True)
