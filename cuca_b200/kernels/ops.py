@@ -1686,7 +1686,7 @@ class QuantizedPlan:
         self.longest = max(self.counts, default=0)
         self._arrays = self._addresses = None
         self._launches: dict = {}
-        self._options: dict = {}
+        self._calls: dict = {}
 
     def arrays(self, step) -> tuple:
         """The addresses of the step's positions, slots, first rows and counts, checked once per step."""
@@ -1699,19 +1699,25 @@ class QuantizedPlan:
             self._arrays = step.positions, step.seq_of_row, step.req_row0, step.req_count
         return self._addresses
 
-    def options(self, n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes) -> AttentionOptions:
-        """`attention_options`, kept for the other layers of the step where they point to nothing."""
-        if sink_values is not None or slopes is not None:
-            return attention_options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
-        key = (scale, window, softcap, sink, keep_first)
-        opt = self._options.get(key)
-        if opt is None:
-            opt = self._options[key] = attention_options(n_heads, scale, window, softcap, sink, None, keep_first)
-        return opt
+    def call(self, dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first):
+        """(dtype code, options, launches) of a layer's attention: what its numbers ask for, checked once per step."""
+        key = (dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first)
+        entry = self._calls.get(key)
+        if entry is None:
+            code = dtype_code(dtype)
+            _q8_head_dim(head_dim)
+            if n_kv_heads < 1 or n_heads % n_kv_heads:
+                raise library.KernelError(f"{n_kv_heads} key heads must divide {n_heads} query heads")
+            if window is not None and window < 0 or keep_first < 0 or softcap < 0:
+                raise library.KernelError("a window, kept first keys and a score cap are not negative")
+            opt = attention_options(n_heads, scale, window, softcap, sink, None, keep_first)
+            entry = code, opt, self.launches(n_heads, n_kv_heads, head_dim, dtype, window or None, opt.keep)
+            self._calls[key] = entry
+        return entry
 
     def launches(self, n_heads, n_kv_heads, head_dim, dtype, window, keep):
-        """[(form, least count, most count, rows of a tile, tiles, heads of a block, width, keys of a share, shares)]; form 0: few
-        rows a block, `width` column tiles of 8; 1: tcgen05, `width` query tiles of 128"""
+        """[(form, least count, most count, rows of a tile, tiles, heads of a block, width, keys of a share, shares, whether those
+        are joined through memory)]; form 0: few rows a block, `width` column tiles of 8; 1: tcgen05, `width` query tiles of 128"""
         key = (n_heads, n_kv_heads, head_dim, dtype, window, keep)
         if key not in self._launches:
             group, out = n_heads // n_kv_heads, []
@@ -1726,7 +1732,9 @@ class QuantizedPlan:
                 out.append(self._few(1, 1, *key))
             if portions:
                 out.append((self._many if many else self._few)(least, self.longest, *key))
-            self._launches[key] = out
+            # (last: whether the shares' results go through memory)
+            self._launches[key] = [(*n, n[-1] > 1 and (n[0] == 1 or not _merge_as_cluster(
+                n[4] * n_kv_heads * -(-group // n[5]), n[-1], _q8_resident(sm_count(), head_dim, n[6])))) for n in out]
         return self._launches[key]
 
     def _many(self, lo, hi, n_heads, n_kv_heads, head_dim, dtype, window, keep):
@@ -1814,29 +1822,25 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
     [rows, heads * head_dim] in q's dtype (bfloat16 or float32). `step` describes the rows (`StepBatch`: positions, seq_of_row,
     req_row0, req_count, counts and starts on the host). Rows of no request (seq_of_row < 0) get zeros. The other options: see
     `attention_options`."""
-    code, n = dtype_code(q.dtype), step.n_rows
-    _q8_head_dim(head_dim)
-    if n_kv_heads < 1 or n_heads % n_kv_heads:
-        raise library.KernelError(f"{n_kv_heads} key heads must divide {n_heads} query heads")
+    n, width, dtype = step.n_rows, n_heads * head_dim, q.dtype
+    plan = step.plans.get("paged_attention_q8")
+    if plan is None:
+        plan = attention_q8_plan(step)
+    code, opt, launches = plan.call(dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first)
+    if sink_values is not None or slopes is not None:
+        opt = attention_options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
     pool = pages.check(n_kv_heads, head_dim)
-    src, dst = _rows(q, n, n_heads * head_dim, "queries"), _rows(out, n, n_heads * head_dim, "results")
-    if out.dtype != q.dtype:
-        raise library.KernelError(f"results have the queries' dtype {q.dtype}, not {out.dtype}")
-    if window is not None and window < 0 or keep_first < 0 or softcap < 0:
-        raise library.KernelError("a window, kept first keys and a score cap are not negative")
-    plan = attention_q8_plan(step)
-    opt = plan.options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
+    src, dst = _rows(q, n, width, "queries"), _rows(out, n, width, "results")
+    if out.dtype != dtype:
+        raise library.KernelError(f"results have the queries' dtype {dtype}, not {out.dtype}")
     lib, stream, e = library.load(), _stream(), _at(err)
     of_rows, of_requests = plan.arrays(step)
     rows = (src, q.stride(0), dst, out.stride(0), code, *pool, *of_rows, _ints(tables), tables.shape[1], *of_requests)
     shape = n_heads, n_kv_heads, head_dim, ctypes.addressof(opt)
     group = n_heads // n_kv_heads
-    for form, lo, hi, tokens, tiles, heads, width, share, shares in plan.launches(n_heads, n_kv_heads, head_dim, q.dtype,
-                                                                                  window or None, opt.keep):
+    for form, lo, hi, tokens, tiles, heads, width, share, shares, through_memory in launches:
         part, at = None, 0
-        if shares > 1 and (form == 1 or not _merge_as_cluster(tiles * n_kv_heads * -(-group // heads), shares,
-                                                              _q8_resident(sm_count(), head_dim, width))):
-            # the shares' results, joined by a second launch
+        if through_memory:  # the shares' results, joined by a second launch
             cols = 8 * width // (2 if code == F32 else 1)
             part = torch.empty(tiles * n_kv_heads * shares * (256 * (64 if head_dim <= 64 else 128) + 512) if form == 1 else
                                tiles * n_kv_heads * -(-group // heads) * shares * cols * (head_dim + 2), dtype=torch.float32,

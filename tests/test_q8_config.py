@@ -40,7 +40,7 @@ def test_every_request_of_a_step_is_in_one_launch_exactly():
                     plan = ops.QuantizedPlan(step).launches(heads, kv, dim, dtype, None, 0)
                     for c in counts:
                         assert sum(lo <= c <= hi for _, lo, hi, *_ in plan) == 1
-                    for form, lo, hi, tokens, tiles, group, nt, share, shares in plan:
+                    for form, lo, hi, tokens, tiles, group, nt, share, shares, _ in plan:
                         assert tiles == sum(-(-c // tokens) for c in counts if lo <= c <= hi)
                         if form == 0:
                             assert tokens * group * (2 if dtype == torch.float32 else 1) <= 8 * nt

@@ -395,10 +395,9 @@ def test_shares_join_through_a_cluster_and_through_memory(monkeypatch, starts, c
     from cuca_b200.kernels import ops
     monkeypatch.setattr(ops, "CLUSTER_MERGE", cluster)
     c = Case(8, 2, 128, 16, [1] * len(starts), starts, dtype, seed=len(starts))
-    *_, share, shares = ops.attention_q8_plan(c.step).launches(8, 2, 128, dtype, None, 0)[0]
+    *_, share, shares, memory = ops.attention_q8_plan(c.step).launches(8, 2, 128, dtype, None, 0)[0]
     assert shares > 1
-    if cluster:
-        assert shares in (2, 4, 8)
+    assert memory == (not cluster) and (memory or shares in (2, 4, 8))
     got = _check(c, sink=True)
     assert torch.equal(got, _attend(c, sink=True))
     _check(c, window=300, keep_first=5, softcap=20.0)
