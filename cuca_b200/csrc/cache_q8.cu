@@ -33,6 +33,8 @@ struct CucaQ8Store {
   float* kscale;
   float* vscale;
   int64_t n_blocks, bs, n_rows, nh, nkv, d;
+  int64_t slices, slice_stride;  // > 0: qkv is so many K slices of the rows, 32-bit, to be added (and `bias` to their sum)
+  const void* bias;              // of q_out's type, or null
   int* err;
   cudaStream_t stream;
 };
@@ -53,7 +55,7 @@ struct CucaQ8Read {
   int* err;
   cudaStream_t stream;
 };
-static_assert(sizeof(CucaQ8Store) == 26 * 8 && sizeof(CucaQ8Read) == 20 * 8, "one 64-bit word each");
+static_assert(sizeof(CucaQ8Store) == 29 * 8 && sizeof(CucaQ8Read) == 20 * 8, "one 64-bit word each");
 
 namespace {
 
@@ -78,6 +80,9 @@ struct StoreParams {
   float* vscale;
   int n_blocks, bs, n_rows, nh, nkv, d;
   int seg_shift;  // log2 of a head's lanes: d / 8, rounded up to a power of two
+  int slices;
+  size_t slice_stride;
+  const void* bias;
   int* err;
 };
 
@@ -110,8 +115,38 @@ __device__ __forceinline__ uint32_t codes4(const float (&v)[4], float inv) {
 // each half of the head, which are the rotation's pairs where the whole head is rotated in halves (VEC: 8- or 16-byte accesses).
 // Else (part of the head rotated, neighbours as pairs, rows that are not aligned) the same values are fetched one by one with
 // their partners. A head stays within a warp, and everything is read before anything is written: q_out may be the rows
-// themselves.
-template <typename T, bool VEC, int ROWS>
+// themselves. SLICES: the rows are a contraction's K slices, added in their order in 32 bits (and the bias to the sum), and not
+// rounded before they are rotated and quantised.
+template <typename T, bool SLICES>
+__device__ __forceinline__ float row_value(const StoreParams& p, size_t at, int column) {
+  if constexpr (!SLICES) {
+    return to_f32(((const T*)p.qkv)[at]);
+  } else {
+    float x = 0.f;
+    for (int s = 0; s < p.slices; ++s) x += ((const float*)p.qkv)[s * p.slice_stride + at];
+    return p.bias ? x + to_f32(((const T*)p.bias)[column]) : x;
+  }
+}
+template <typename T, bool SLICES>
+__device__ __forceinline__ void row_values(const StoreParams& p, size_t at, int column, float (&v)[4]) {
+  if constexpr (!SLICES) {
+    load4((const T*)p.qkv + at, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < p.slices; ++s) {
+      float x[4];
+      load4((const float*)p.qkv + s * p.slice_stride + at, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += x[i];
+    }
+    if (p.bias)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += to_f32(((const T*)p.bias)[column + i]);
+  }
+}
+template <typename T, bool VEC, int ROWS, bool SLICES>
 __global__ void __launch_bounds__(STORE_THREADS, ROWS > 1 ? 4 : 1) rope_store_q8_kernel(const StoreParams p) {
   pdl_trigger();
   pdl_wait();
@@ -135,9 +170,9 @@ __global__ void __launch_bounds__(STORE_THREADS, ROWS > 1 ? 4 : 1) rope_store_q8
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[r][i] = b[r][i] = 0.f;
     if (VEC && lane_ok && row < p.n_rows) {  // (whoever's the row is: its numbers need not be known first)
-      const T* src = (const T*)p.qkv + (size_t)row * p.row_stride + (size_t)head * p.d;
-      load4(src + 4 * l, a[r]);
-      load4(src + half + 4 * l, b[r]);
+      const size_t at = (size_t)row * p.row_stride + (size_t)head * p.d;
+      row_values<T, SLICES>(p, at + 4 * l, head * p.d + 4 * l, a[r]);
+      row_values<T, SLICES>(p, at + half + 4 * l, head * p.d + half + 4 * l, b[r]);
     }
   }
 #pragma unroll
@@ -151,15 +186,16 @@ __global__ void __launch_bounds__(STORE_THREADS, ROWS > 1 ? 4 : 1) rope_store_q8
         load4(sr + 4 * l, s[VEC ? r : 0]);
       }
     } else if (live[r]) {
-      const T* src = (const T*)p.qkv + (size_t)(row0 + r) * p.row_stride + (size_t)head * p.d;
+      const size_t at = (size_t)(row0 + r) * p.row_stride + (size_t)head * p.d;
+      auto src = [&](int e) { return row_value<T, SLICES>(p, at + e, head * p.d + e); };
       auto value = [&](int e) {
-        const float x = to_f32(src[e]);
+        const float x = src(e);
         if (!rotate || !in_table || e >= p.rot) return x;
         const int hr = p.rot / 2;
         const int i = p.adjacent ? e / 2 : (e < hr ? e : e - hr);
         const bool first = p.adjacent ? (e & 1) == 0 : e < hr;
         const float cs = cr[i], sn = sr[i];
-        const float y = to_f32(src[p.adjacent ? e ^ 1 : (first ? e + hr : i)]);
+        const float y = src(p.adjacent ? e ^ 1 : (first ? e + hr : i));
         return first ? __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn)) : __fadd_rn(__fmul_rn(y, sn), __fmul_rn(x, cs));
       };
 #pragma unroll
@@ -346,20 +382,24 @@ CUCA_API int cuca_rope_store_q8(const CucaQ8Store* c) {
   CUCA_REQUIRE(((uintptr_t)kpool & 3) == 0 && ((uintptr_t)vpool & 3) == 0, "rope_store_q8: pools must be 4-byte aligned");
   if (n_rows == 0) return 0;
   StoreParams p{qkv, row_stride, q_out, q_stride, c->positions, c->seq_of_row, c->tables, table_stride, cos_t, sin_t, table_rows, rot,
-                adjacent, (int8_t*)kpool, (int8_t*)vpool, c->kscale, c->vscale, n_blocks, bs, n_rows, nh, nkv, d, 0, c->err};
+                adjacent, (int8_t*)kpool, (int8_t*)vpool, c->kscale, c->vscale, n_blocks, bs, n_rows, nh, nkv, d, 0, (int)c->slices,
+                (size_t)c->slice_stride, c->bias, c->err};
   while ((8 << p.seg_shift) < d) ++p.seg_shift;
-  const uintptr_t align = dtype == CUCA_F32 ? 15 : 7;
+  const bool slices = c->slices > 0;
+  CUCA_REQUIRE(!slices || (dtype == CUCA_BF16 && c->slices <= 64 && c->slice_stride >= 0), "rope_store_q8: K slices give bfloat16 queries");
+  const uintptr_t align = dtype == CUCA_F32 ? 15 : 7, from = slices ? 15 : align;
   const bool vec = (rot == d || rot == 0) && !adjacent && row_stride % 4 == 0 && q_stride % 4 == 0 &&
-                   (((uintptr_t)qkv | (uintptr_t)q_out) & align) == 0 && (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15) == 0;
+                   ((uintptr_t)qkv & from) == 0 && (!slices || c->slice_stride % 4 == 0) && ((uintptr_t)q_out & align) == 0 && (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15) == 0;
   const unsigned blocks = (unsigned)((((long long)(nh + 2 * nkv) << p.seg_shift) + STORE_THREADS - 1) / STORE_THREADS);
   // two rows a thread where that still fills the GPU with threads
-  const bool many = vec && (long long)blocks * n_rows >= 8ll * 2 * cuca_device_sms();
+  const bool many = vec && !slices && (long long)blocks * n_rows >= 8ll * 2 * cuca_device_sms();
   const int per = many ? 2 : 1;
   CUCA_REQUIRE((n_rows + per - 1) / per <= 65535, "rope_store_q8: too many rows");
-  auto kernel = dtype == CUCA_F32
-      ? (many ? rope_store_q8_kernel<float, true, 2> : vec ? rope_store_q8_kernel<float, true, 1> : rope_store_q8_kernel<float, false, 1>)
-      : (many ? rope_store_q8_kernel<__nv_bfloat16, true, 2> : vec ? rope_store_q8_kernel<__nv_bfloat16, true, 1>
-                                                                  : rope_store_q8_kernel<__nv_bfloat16, false, 1>);
+  auto kernel = slices ? (vec ? rope_store_q8_kernel<__nv_bfloat16, true, 1, true> : rope_store_q8_kernel<__nv_bfloat16, false, 1, true>)
+      : dtype == CUCA_F32
+      ? (many ? rope_store_q8_kernel<float, true, 2, false> : vec ? rope_store_q8_kernel<float, true, 1, false> : rope_store_q8_kernel<float, false, 1, false>)
+      : (many ? rope_store_q8_kernel<__nv_bfloat16, true, 2, false> : vec ? rope_store_q8_kernel<__nv_bfloat16, true, 1, false>
+                                                                         : rope_store_q8_kernel<__nv_bfloat16, false, 1, false>);
   cuca_launch(kernel, dim3(blocks, (n_rows + per - 1) / per), dim3(STORE_THREADS), 0, stream, true, p);
   CUCA_CHECK_LAUNCH("rope_store_q8");
   return 0;

@@ -1579,7 +1579,7 @@ class QuantizedPages:
 
 Q8_MAX_HEAD_DIM = 256
 # a call's arguments as 64-bit words (`CucaQ8Store` and `CucaQ8Read` in csrc/cache_q8.cu, `CucaQ8Attention` in csrc/attention_q8.cuh)
-_Q8_STORE, _Q8_READ, _Q8_ATTENTION = struct.Struct("26q"), struct.Struct("20q"), struct.Struct("33q")
+_Q8_STORE, _Q8_READ, _Q8_ATTENTION = struct.Struct("29q"), struct.Struct("20q"), struct.Struct("33q")
 
 
 def _at(t) -> int:
@@ -1617,17 +1617,30 @@ def _rows(t, n_rows: int, width: int, what: str) -> int:
 
 
 def rope_store_q8(qkv, q_out, positions, seq_of_row, tables, cos, sin, rotary_dim, pages: QuantizedPages, n_heads, n_kv_heads,
-                  head_dim, err, adjacent: bool = False) -> None:
-    """Rows q | k | v: q, rotated, into `q_out` (which may be the rows themselves), k, rotated, and v quantised into their
+                  head_dim, err, adjacent: bool = False, bias=None) -> None:
+    """Rows q | k | v, or a projection's unadded K slices of them (`PartialSums`; then `bias` or None, and bfloat16 queries): q,
+    rotated, into `q_out` (which may be the rows themselves), k, rotated, and v quantised into their
     pages. The first `rotary_dim` values of a head are rotated (cos None: none), in halves or as neighbouring pairs. A row that is
     not finite reads back as NaN. Rows with seq_of_row < 0 are left out."""
-    code, n = dtype_code(qkv.dtype), qkv.shape[0]
+    width, n = (n_heads + 2 * n_kv_heads) * head_dim, q_out.shape[0]
+    code = dtype_code(q_out.dtype)
     _q8_head_dim(head_dim)
     k, v, ks, vs, n_pages, bs = pages.check(n_kv_heads, head_dim)
-    src = _rows(qkv, n, (n_heads + 2 * n_kv_heads) * head_dim, "projected rows")
+    slices = slice_stride = 0
+    if isinstance(qkv, PartialSums):
+        slices, slice_stride, rows = qkv.slices, qkv.slice_stride, qkv.data[0]
+        if rows.dtype != torch.float32 or q_out.dtype != torch.bfloat16:
+            raise library.KernelError("K slices are 32-bit, queries made of them bfloat16")
+        if bias is not None and (bias.dtype != q_out.dtype or bias.shape != (width,) or not bias.is_contiguous() or not bias.is_cuda):
+            raise library.KernelError(f"a bias is {width} contiguous numbers of the queries' dtype, on the device")
+    elif bias is not None:
+        raise library.KernelError("a bias goes with K slices; rows have it already")
+    else:
+        rows = qkv
+        if q_out.dtype != rows.dtype:
+            raise library.KernelError(f"rotated queries have the rows' dtype {rows.dtype}, not {q_out.dtype}")
+    src = _rows(rows, n, width, "projected rows")
     dst = _rows(q_out, n, n_heads * head_dim, "rotated queries")
-    if q_out.dtype != qkv.dtype:
-        raise library.KernelError(f"rotated queries have the rows' dtype {qkv.dtype}, not {q_out.dtype}")
     rot = table_rows = 0
     if cos is not None:
         rot = int(rotary_dim)
@@ -1637,9 +1650,9 @@ def rope_store_q8(qkv, q_out, positions, seq_of_row, tables, cos, sin, rotary_di
         _cuda(cos, sin)
         table_rows = cos.shape[0]
     library.check(library.load().cuca_rope_store_q8(_Q8_STORE.pack(
-        src, qkv.stride(0), dst, q_out.stride(0), code, _ints(positions, n), _ints(seq_of_row, n), _ints(tables), tables.shape[1],
+        src, rows.stride(0), dst, q_out.stride(0), code, _ints(positions, n), _ints(seq_of_row, n), _ints(tables), tables.shape[1],
         _at(cos), _at(sin), table_rows, rot, 1 if adjacent else 0, k, v, ks, vs, n_pages, bs, n, n_heads, n_kv_heads, head_dim,
-        _at(err), _stream())), "rope_store_q8")
+        slices, slice_stride, _at(bias), _at(err), _stream())), "rope_store_q8")
 
 
 def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, err) -> None:

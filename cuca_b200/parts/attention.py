@@ -297,20 +297,27 @@ class PagedAttention(Mixer):
         stream.add_linear(attn, self.w_o, bias=self.b_o)
 
     def forward_quantized(self, h, stream, step, cache) -> None:
-        """Over pages in 8 bits: one projection; q rotated where it stands, k rotated, k and v quantised into their pages;
-        attention over the codes."""
+        """Over pages in 8 bits: one projection; q rotated, k rotated, k and v quantised into their pages; attention over the
+        codes."""
         nh, nkv, d = self.n_heads, self.n_kv_heads, self.head_dim
-        proj = self.rt.linear(h, self.w_qkv, bias=self.b_qkv)
         fused = self.position.fused_tables() if self.position is not None else None
-        if fused is None and self.position is not None:
-            self.position.apply(proj, nh, 0 if self.shares_cache else nkv, d, step.positions)
         cos, sin, rot = fused if fused is not None else (None, None, 0)
-        if not self.shares_cache:
-            ops.rope_store_q8(proj, proj, step.positions, step.seq_of_row, cache.tables, cos, sin, rot, cache.quantized, nh, nkv,
-                              d, self.rt.err)
-        elif fused is not None:
-            ops.rope_store(proj, step.positions, step.seq_of_row, cache.tables, cos, sin, rot, None, None, cache.block_size, nh,
-                           0, d, self.rt.err)
+        if (not self.shares_cache and (fused is not None or self.position is None) and self.rt.use_partials
+                and h.shape[0] <= ops.ROPE_PARTIAL_MAX_ROWS and ops.gemm_partial_supported(h, self.w_qkv)):
+            # few tokens: the projection leaves its K slices unadded, what writes the pages adds them
+            proj = self.rt.empty(h.shape[0], nh * d)
+            ops.rope_store_q8(ops.gemm_partial(h, self.w_qkv, self.rt.err), proj, step.positions, step.seq_of_row, cache.tables, cos,
+                              sin, rot, cache.quantized, nh, nkv, d, self.rt.err, bias=self.b_qkv)
+        else:
+            proj = self.rt.linear(h, self.w_qkv, bias=self.b_qkv)
+            if fused is None and self.position is not None:
+                self.position.apply(proj, nh, 0 if self.shares_cache else nkv, d, step.positions)
+            if not self.shares_cache:
+                ops.rope_store_q8(proj, proj, step.positions, step.seq_of_row, cache.tables, cos, sin, rot, cache.quantized, nh, nkv,
+                                  d, self.rt.err)
+            elif fused is not None:
+                ops.rope_store(proj, step.positions, step.seq_of_row, cache.tables, cos, sin, rot, None, None, cache.block_size,
+                               nh, 0, d, self.rt.err)
         attn = self.rt.empty(h.shape[0], nh * d)
         ops.attention_q8(proj, attn, cache.quantized, cache.tables, step, nh, nkv, d, self.scale, self.window, self.rt.err)
         stream.add_linear(attn, self.w_o, bias=self.b_o)

@@ -107,6 +107,32 @@ def test_codes_of_the_vectorised_and_the_plain_form_are_the_same():
     assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("slices,dim,rot,rows", [(1, 128, 128, 3), (5, 64, 64, 40), (16, 80, 80, 1), (3, 96, 32, 9), (2, 32, 0, 7)])
+def test_k_slices_are_added_before_they_are_rotated_and_quantised(slices, dim, rot, rows, with_bias):
+    """The same codes, bit for bit, as from the 32-bit rows that the slices, added in order, make; the same queries, rounded."""
+    from cuca_b200.kernels import ops
+    heads, kv = 4, 2
+    c = Case(heads, kv, dim, 16, [rows], [5], torch.bfloat16, seed=slices, fill=False, padding=1)
+    n, width = rows + 1, (heads + 2 * kv) * dim
+    data = torch.randn(slices, n + 3, width, device=c.device, generator=c.g)[:, :n]
+    bias = torch.randn(width, device=c.device, generator=c.g).to(torch.bfloat16) if with_bias else None
+    total = torch.zeros(n, width, device=c.device)
+    for s in range(slices):
+        total = total + data[s]
+    if with_bias:
+        total = total + bias.float()
+    cos, sin = _tables(64, rot, c.device) if rot else (None, None)
+    results = []
+    for source, dtype in ((ops.PartialSums(data, slices), torch.bfloat16), (total, torch.float32)):
+        c.k.zero_(), c.v.zero_(), c.k_scale.zero_(), c.v_scale.zero_()
+        q = torch.zeros(n, heads * dim, dtype=dtype, device=c.device)
+        ops.rope_store_q8(source, q, c.step.positions, c.step.seq_of_row, c.tables, cos, sin, rot, c.pages(), heads, kv, dim, c.err,
+                          bias=bias if dtype == torch.bfloat16 else None)
+        results.append([t.clone() for t in (q.to(torch.bfloat16), c.k, c.v, c.k_scale, c.v_scale)])
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and int(c.err) == 0
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rows_of_zeros_of_tiny_values_and_rows_that_are_not_finite(dtype):
     c = Case(2, 1, 32, 16, [8], [3], dtype, seed=9, fill=False)
@@ -348,7 +374,9 @@ def test_refusals():
                              sin=sin, rotary_dim=64, pages=c.pages(), n_heads=4, n_kv_heads=2, head_dim=64, err=c.err) | k
     before = c.k.clone()
     for bad in (dict(qkv=qkv[:, :400]), dict(q_out=out.float()), dict(rotary_dim=32), dict(sin=None), dict(cos=cos.double()),
-                dict(positions=c.step.positions.long()), dict(positions=c.step.positions[:2]), dict(n_kv_heads=1), dict(qkv=qkv.cpu())):
+                dict(positions=c.step.positions.long()), dict(positions=c.step.positions[:2]), dict(n_kv_heads=1), dict(qkv=qkv.cpu()),
+                dict(bias=qkv[0]), dict(qkv=ops.PartialSums(qkv[None], 1)),
+                dict(qkv=ops.PartialSums(qkv[None].float(), 1), bias=qkv[0].float())):
         with pytest.raises(library.KernelError):
             ops.rope_store_q8(**store(**bad))
     assert torch.equal(before, c.k)
