@@ -7,16 +7,22 @@
 //   S[128 rows, 64 keys]  = Q K^T      Q and K as 16-bit floats in shared memory (K-major, 128-byte swizzle)
 //   O[128 rows, d]       += W V        W from tensor memory, where S was; V as 16-bit floats in shared memory (MN-major)
 //
-// A warp or two copy codes from the pages, three tiles ahead; four turn them into 16-bit floats and store them as operand tiles, with
+// Two warps copy codes from the pages, three tiles ahead; four turn them into 16-bit floats and store them as operand tiles, with
 // each key's factors beside them; four warps per query tile own a row per thread (a lane of tensor memory) and turn scores into
 // weights; a warp per query tile issues its products. Where the two query tiles share a converted tile, the conversion is a
-// seventh of the block's instructions.
+// sixth of the block's instructions.
 //
 // A value scale goes into the operand tile here: V = code vs 2^(7 - E) with E the largest exponent of the tile's scales, rounded
 // to 11 bits, factor and product, so that z = s + E for every key of the tile and one multiplication a tile brings the sum of
 // the weights to the denominator's unit. Per-key factors in the softmax would each cost 16 loads of 512 bytes a warp and tile:
-// with three of them a tile of 64 keys took 3,900 clocks, 2,048 of them of shared memory's bandwidth. Where a tile's scales are
-// more than 2^20 apart the exponents stay with the keys (`wide`). The keys' scales multiply the scores, so codes of keys are exact.
+// one, the keys' scales, is left of four. Where a tile's scales are more than 2^20 apart the exponents stay with the keys
+// (`wide`). The keys' scales multiply the scores, so codes of keys are exact.
+//
+// Measured, 32 heads of 128 over 8: a prompt of 2,048 58 us (590 TFLOP/s), a portion of 512 on 8,192 107 us (664 TFLOP/s; over
+// bfloat16 pages, attention_tc.cu, 56 and 138). A tile of 64 keys takes two query tiles some 2,450 clocks, of which the tensor
+// pipe and the exponent unit need 1,024 each. No unit sets the pace: without seven eighths of the softmax's arithmetic the portion
+// took 20 % less, without most products 9 %, without all three roles' work still 72 us. What is left is the way round: a score
+// tile, its weights, their product, and the hand-overs between (barriers, tensor memory's loads and stores), two deep.
 //
 // Every wait is bounded; when one runs out the kernel records CUCA_ERR_WAIT_TIMEOUT, all roles stop, tensor memory is freed and
 // the kernel returns.
@@ -35,10 +41,10 @@ constexpr int NTHREADS = (SOFT_WARPS + CONV_WARPS + NQ + LOAD_WARPS) * 32;  // s
 // Registers a thread: 128 at launch, then by role; the sum, 2 x 176 + 88 + 64 over groups of 128 threads, is within the 4 x 128
 // of the launch.
 constexpr int SOFT_REGS = 176, CONV_REGS = 88, ISSUE_REGS = 64;
-// Operand tiles of keys are free again when their scores are there, those of values only after the weights' product: with three
-// of both, a tile's way round (conversion, scores, softmax, product: some 6,000 clocks) set the pace and not any unit.
+// Operand tiles: those of keys are free again when their scores are there, those of values after the weights' product. (Two and
+// four, three and four with two tiles of codes on their way, four and three: within 2 %.)
 constexpr int K_STAGES = 3, V_STAGES = 3;
-constexpr int RAW = 3;            // tiles of codes on their way
+constexpr int RAW = 3;  // tiles of codes on their way
 constexpr float V_LIFT = 7.f;     // values are 2^7 larger in the operand tile: 127 2^7 2 is the most that fits
 constexpr int WIDE = 20;
 constexpr int TMEM_COLS = 512;  // two score buffers per query tile (4 x 64 columns), results of both (2 x DP)
@@ -206,7 +212,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const int* table = p.tables + (size_t)seq * p.table_stride;
     const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
     if (runs) {
-      // A warp for the keys, one for the values (a copy takes its thread some 100 clocks), a lane a page: codes and scales.
+      // A warp for the keys, one for the values (one for both was busy for 1,770 clocks a tile), a lane a page: codes and scales.
       // Positions from keys.hi on come along where their page does; what converts them takes their scales for 0. (A page behind a
       // window may have gone back, another that is not there is an error: page 0 comes instead; its keys are masked, or the step
       // is lost.)
@@ -538,8 +544,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONV_REGS));
     // ------------------------------------------------ codes to operand tiles
     // Every warp works for itself: its lanes stand for the tile's keys lane and lane + 32 (scales, the tile's exponent) and hand
-    // factors round; it converts every fourth set of rows. It asks for nothing from memory itself: what a thread has on its way
-    // would have to arrive before its fence between the two proxies is over, 1,700 to 2,700 clocks a tile.
+    // factors round; it converts every fourth set of rows. It asks for nothing from memory itself: its fence between the two
+    // proxies would wait for what is on its way (a prompt of 2,048 62 us so, 60 with copies in warps of their own).
     const int cw = warp - SOFT_WARPS;
     constexpr int ROWS_AT_ONCE = DP == 128 ? 4 : 8;         // of a warp: 16-byte pieces of keys or values
     constexpr int STEP = CONV_WARPS * ROWS_AT_ONCE, PER = KEYS / STEP;

@@ -10,7 +10,9 @@
 // depend on the form that made them. Rounding to 8 bits here is the cache's own choice: against bfloat16 pages it halves the
 // bytes a decode step reads; the error of a value is at most half a 127th of its row's largest.
 //
-// Both kernels do a few operations per byte and are bound by memory, or by latency when there are few rows.
+// Both kernels do a few operations per byte and are bound by memory, or by latency when there are few rows. Measured, 32 heads of
+// 128 over 8: writing 2,048 rows 14.5 us (torch's copy of the queries' part alone: 13.1), reading 34,000 positions back 51 us
+// (5.3 TB/s, 0.81 of a copy's rate).
 #include "common.cuh"
 
 int cuca_device_sms();
@@ -101,14 +103,14 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
 }
 
+// Four codes. 1.5 2^23 more, a number is rounded to a whole one, ties to even, and its low byte is the code; no product exceeds
+// 127 by so much that it would be 128. Without `inv` (a row of zeros, or one that is not finite, whose products may be NaN): 0.
 __device__ __forceinline__ uint32_t codes4(const float (&v)[4], float inv) {
-  uint32_t w = 0;
+  uint32_t r[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = max(-127, min(127, __float2int_rn(__fmul_rn(v[i], inv))));
-    w |= (uint32_t)(c & 0xff) << (8 * i);
-  }
-  return w;
+  for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], inv), 12582912.f));
+  const uint32_t codes = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+  return inv > 0.f ? codes : 0;
 }
 
 // A group of lanes takes one head of a row, of ROWS rows in turn whose loads go out together; a lane has values 4 l .. 4 l + 3 of
@@ -282,6 +284,9 @@ struct ReadParams {
 
 __device__ __forceinline__ uint32_t word_of(uint32_t w, int) { return w; }
 __device__ __forceinline__ uint32_t word_of(const uint2& w, int i) { return i == 0 ? w.x : w.y; }
+// What uses the value stays behind this point, and so behind the other loads (34,000 positions: 51 us, left to the compiler 80).
+__device__ __forceinline__ void stay(uint32_t& w) { asm volatile("" : "+r"(w)); }
+__device__ __forceinline__ void stay(uint2& w) { asm volatile("" : "+r"(w.x), "+r"(w.y)); }
 
 // A warp brings READ_PIECES x 32 pieces of a row, of one tensor, for READ_ROWS rows whose loads go out together: a lane's places in
 // the page and in the row are the same for all of them. gridDim: rows, pieces, tensors.
@@ -337,6 +342,10 @@ __global__ void __launch_bounds__(READ_WARPS * 32) read_q8_kernel(const __grid_c
     }
   }
 #pragma unroll
+  for (int r = 0; r < READ_ROWS; ++r)
+#pragma unroll
+    for (int i = 0; i < READ_PIECES; ++i) stay(w[r][i]);
+#pragma unroll
   for (int r = 0; r < READ_ROWS; ++r) {
     if (row0 + r >= p.n_rows) break;
 #pragma unroll
@@ -344,7 +353,10 @@ __global__ void __launch_bounds__(READ_WARPS * 32) read_q8_kernel(const __grid_c
       if (head[i] < 0) continue;
       float v[N];
 #pragma unroll
-      for (int n = 0; n < N; ++n) v[n] = (float)(int8_t)(word_of(w[r][i], n / 4) >> (8 * (n & 3))) * s[r][i];
+      for (int n = 0; n < N; ++n) {  // x + 128 in the low bits of 2^23, less those (a conversion instruction is four times slower)
+        const uint32_t biased = word_of(w[r][i], n / 4) ^ 0x80808080u;
+        v[n] = (__uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7650 | (n & 3))) - 8388736.f) * s[r][i];
+      }
       T* dst = out + (size_t)(row0 + r) * stride + (size_t)head[i] * p.d + e[i];
       if constexpr (N == 4) {
         *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);

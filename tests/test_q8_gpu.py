@@ -155,6 +155,20 @@ def test_rows_of_zeros_of_tiny_values_and_rows_that_are_not_finite(dtype):
     assert gk[4].isfinite().all() and gv[6].isfinite().all()
 
 
+@pytest.mark.parametrize("what", [0.0, TINY / 4, math.inf, -math.inf, math.nan])
+def test_a_row_that_keeps_nothing_has_codes_of_zero(what):
+    c = Case(2, 1, 32, 16, [8], [0], torch.float32, seed=2, fill=False)
+    qkv = torch.randn(8, 4 * 32, device=c.device, generator=c.g)
+    qkv[:, 64:] *= 0 if abs(what) < 1 else 1
+    qkv[:, 64::7] = what
+    c.k.fill_(5), c.v.fill_(5)
+    _write(c, qkv, torch.empty(8, 64, device=c.device), None, None, 0)
+    page = c.tables[c.slots[0], 0].long()
+    assert (c.k[page, :, :8] == 0).all() and (c.v[page, :, :8] == 0).all() and (c.k[page, :, 8:] == 5).all()
+    scales = torch.cat([c.k_scale[page, :, :8], c.v_scale[page, :, :8]])
+    assert (scales == 0).all() if abs(what) < 1 else scales.isnan().all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("kv,dim,page,totals", [(8, 128, 16, [300, 1, 77]), (1, 16, 8, [9]), (3, 80, 24, [50, 49]), (2, 256, 1, [5])])
 def test_reading_back_is_exact(dtype, kv, dim, page, totals):
