@@ -87,7 +87,7 @@ struct Ring {
   }
 };
 
-// NT: tiles of 8 columns. PARTS: 1: bfloat16 rows, a column each; 2: 32-bit rows, two columns each. OPT: score cap, sink and
+// NT: tiles of 8 columns. PARTS: 1: bfloat16 rows, a column each; 2: 32-bit rows, two columns each. OPT: score cap and
 // distance bias.
 template <int DP, int NT, int PARTS, bool OPT>
 __global__ void __launch_bounds__(WARPS * 32)
@@ -517,7 +517,7 @@ attention_q8_kernel(const Q8Params p) {
     }
     const int head = head0 + col % heads;
     if (alone) {
-      if (OPT && p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
+      if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
       const float inv = den == 0.f ? 0.f : 1.f / den;  // (a column that saw nothing has zeros)
       T* dst = (T*)p.out + (size_t)(row0 + col / heads) * p.out_stride + (size_t)head * p.d + e;
 #pragma unroll
@@ -561,7 +561,7 @@ attention_q8_kernel(const Q8Params p) {
       den += f * ml[s].y;
     }
     const int head = head0 + col % heads;
-    if (OPT && p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
+    if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
     const float inv = den == 0.f ? 0.f : 1.f / den;
     T* dst = (T*)p.out + (size_t)(row0 + col / heads) * p.out_stride + (size_t)head * p.d + e;
 #pragma unroll
@@ -656,7 +656,7 @@ int launch_q8(const Q8Params& p, int n_tiles, cudaStream_t stream) {
 }
 template <int DP, int NT, int PARTS>
 int launch_q8_opt(const Q8Params& p, int n_tiles, cudaStream_t stream) {
-  return p.cap > 0.f || p.sink || p.slopes ? launch_q8<DP, NT, PARTS, true>(p, n_tiles, stream)
+  return p.cap > 0.f || p.slopes ? launch_q8<DP, NT, PARTS, true>(p, n_tiles, stream)
                                            : launch_q8<DP, NT, PARTS, false>(p, n_tiles, stream);
 }
 template <int DP, int PARTS>

@@ -224,6 +224,20 @@ __device__ __forceinline__ float q8_capped(float s, const Q8Params& p) {
   if (EXACT) return p.cap * CUCA_LOG2E * tanhf(s / p.cap);
   return p.cap * CUCA_LOG2E * (1.f - __fdividef(2.f, q8_exp2(s * p.cap_arg) + 1.f));
 }
+// Two of them through one reciprocal: 1/a = b / (a b). Beyond 2^60 a summand e^2y makes no difference, and the product stays finite.
+// (A score that is no number stays none.)
+__device__ __forceinline__ float q8_at_most_60(float x) {
+  float r;
+  asm("min.NaN.f32 %0, %1, 0f42700000;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 q8_capped_pair(float2 s, const Q8Params& p) {
+  const float2 y = __fmul2_rn(s, make_float2(p.cap_arg, p.cap_arg));
+  const float a = q8_exp2(q8_at_most_60(y.x)) + 1.f, b = q8_exp2(q8_at_most_60(y.y)) + 1.f;
+  const float r = __fdividef(-2.f * CUCA_LOG2E * p.cap, a * b);
+  const float top = p.cap * CUCA_LOG2E;
+  return __ffma2_rn(make_float2(r, r), make_float2(b, a), make_float2(top, top));
+}
 // What a sink adds to a denominator that is relative to the reference m.
 __device__ __forceinline__ float q8_sink_term(const Q8Params& p, int head, float m) {
   return q8_exp2((p.sink_val ? p.sink_val[head] * CUCA_LOG2E : 0.f) - m + Q8_LIFT);

@@ -108,7 +108,9 @@ __device__ __forceinline__ void tmem_ld32_done(uint32_t taddr, float (&v)[32]) {
       : "r"(taddr) : "memory");
 }
 
-template <int DP, bool OPT>
+// EXTRA: what a score goes through beside its factor: 1: a distance bias, 2: a cap (and a bias). Constants, as a branch a pair of
+// scores keeps their instructions from overlapping (a portion with either took twice the time without).
+template <int DP, int EXTRA>
 __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Params p) {
   using SH = Shape<DP>;
   extern __shared__ uint8_t smem_raw[];
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const int row_lo = p.window > 0 ? row_pos - (p.window - 1) : 0;
     const int least_pos = pos0 + x * tile_tok;  // of the query tile's rows
     const int most_lo = p.window > 0 ? pos0 + min(n_tok, (x + 1) * tile_tok) - 1 - (p.window - 1) : 0;
-    const float slope2 = OPT && p.slopes ? p.slopes[head] * CUCA_LOG2E : 0.f;
+    const float slope2 = EXTRA && p.slopes ? p.slopes[head] * CUCA_LOG2E : 0.f;
     float m = -INFINITY, l = 0.f;
     bool ok = x < nq;
     // The product of tile j - 1. Not every one is waited for and two can be on their way, so even and odd tiles have a barrier
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       const float4 tile_e = kf4[3 * KEYS / 4];  // E, 2^-E, wide
       const int key0 = keys.at(first + j) * KEYS;
       const bool whole = key0 + KEYS - 1 <= least_pos && (p.window <= 0 || key0 >= most_lo || key0 + KEYS <= p.keep);
-      const float bias0 = OPT ? slope2 * (float)(key0 - row_pos) : 0.f;
+      const float bias0 = EXTRA ? slope2 * (float)(key0 - row_pos) : 0.f;
       // Weights relative to the maximum of the tiles before, with this tile's maximum beside them, so that the exponents need not
       // wait for it; only where a row exceeds the reference by more than 2^LAG is the tile's row read and worked out again.
       float corr = 1.f;
@@ -419,9 +421,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
               const int k = 4 * i + 2 * h;
               float2 x2 = make_float2(__uint_as_float(raw[k / 32][k % 32]), __uint_as_float(raw[k / 32][k % 32 + 1]));
               const float2 f2 = make_float2(f[2 * h], f[2 * h + 1]);
-              if (OPT) {
+              if (EXTRA) {
                 x2 = __fmul2_rn(x2, f2);
-                if (p.cap > 0.f) x2 = make_float2(q8_capped<false>(x2.x, p), q8_capped<false>(x2.y, p));
+                if (EXTRA == 2) x2 = q8_capped_pair(x2, p);
                 x2 = __fadd2_rn(x2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
                 x2 = __fadd2_rn(x2, neg2);
               } else {
@@ -483,7 +485,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     if (ok && product_done(n_tiles)) {
       tc_fence_after();
       if (alone) {
-        if (OPT && p.sink && m != -INFINITY) l += q8_sink_term(p, head, m);
+        if (p.sink && m != -INFINITY) l += q8_sink_term(p, head, m);
         const float inv = bad ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : q8_pow2(-V_LIFT) / l;
         // Through shared memory, where the queries were (every product that read them is done), so that what is stored is whole
         // lines; a row's pieces are turned round by its number, as in the operand tiles.
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
     float up, down;
     q8_query_scale(*q_top, up, down);
-    const float key_factor = down * (OPT && p.cap > 0.f ? p.scale : p.scale_log2e);
+    const float key_factor = down * (EXTRA == 2 ? p.scale : p.scale_log2e);
     for (int j = 0; j < n_tiles; ++j) {
       const int ks_at = j % K_STAGES, st = j % V_STAGES, from = j % RAW;
       if (!warp_wait(&raw_full[from], (j / RAW) & 1, p.err, abort_flag)) break;
@@ -753,10 +755,10 @@ __global__ void __launch_bounds__(ROWS) join_q8_tc_kernel(const Q8Params p) {
   }
 }
 
-template <int DP, bool OPT>
+template <int DP, int EXTRA>
 int launch_q8_tc(const Q8Params& p, int n_tiles, cudaStream_t stream) {
   constexpr int smem = Shape<DP>::SMEM;
-  auto kernel = attention_q8_tc_kernel<DP, OPT>;
+  auto kernel = attention_q8_tc_kernel<DP, EXTRA>;
   static cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   CUCA_REQUIRE(configured == cudaSuccess, "attention_q8_tc: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(configured));
   cuca_launch(kernel, dim3(p.nkv * p.n_splits, n_tiles), dim3(NTHREADS), smem, stream, true, p);
@@ -766,6 +768,11 @@ int launch_q8_tc(const Q8Params& p, int n_tiles, cudaStream_t stream) {
     CUCA_CHECK_LAUNCH("attention_q8_tc (join)");
   }
   return 0;
+}
+template <int DP>
+int launch_q8_tc_extra(const Q8Params& p, int n_tiles, cudaStream_t stream) {
+  if (p.cap > 0.f) return launch_q8_tc<DP, 2>(p, n_tiles, stream);
+  return p.slopes ? launch_q8_tc<DP, 1>(p, n_tiles, stream) : launch_q8_tc<DP, 0>(p, n_tiles, stream);
 }
 
 }  // namespace
@@ -783,7 +790,5 @@ CUCA_API int cuca_attention_q8_tc(const CucaQ8Attention* c) {
   CUCA_REQUIRE((long long)p.n_blocks * p.nkv * p.bs < 0xffffffffll, "attention_q8_tc: more than 2^32 rows in the pools");
   CUCA_REQUIRE((c->width == 1 || c->width == NQ) && p.tile_tokens == (int)c->width * (ROWS / group), "attention_q8_tc: %d rows to %lld query tiles",
                p.tile_tokens, (long long)c->width);
-  const bool extra = p.cap > 0.f || p.sink || p.slopes;
-  if (p.d <= 64) return extra ? launch_q8_tc<64, true>(p, (int)c->n_tiles, c->stream) : launch_q8_tc<64, false>(p, (int)c->n_tiles, c->stream);
-  return extra ? launch_q8_tc<128, true>(p, (int)c->n_tiles, c->stream) : launch_q8_tc<128, false>(p, (int)c->n_tiles, c->stream);
+  return p.d <= 64 ? launch_q8_tc_extra<64>(p, (int)c->n_tiles, c->stream) : launch_q8_tc_extra<128>(p, (int)c->n_tiles, c->stream);
 }
