@@ -738,7 +738,7 @@ __global__ void __launch_bounds__(ROWS) join_q8_tc_kernel(const Q8Params p) {
     o[0] += f * lo.x; o[1] += f * lo.y; o[2] += f * lo.z; o[3] += f * lo.w;
     o[4] += f * hi.x; o[5] += f * hi.y; o[6] += f * hi.z; o[7] += f * hi.w;
   }
-  if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top);
+  if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top) * q8_pow2(V_LIFT);  // (sums come lifted as results do)
   const float inv = den == 0.f ? 0.f : 1.f / den;
   __nv_bfloat16* dst = (__nv_bfloat16*)p.out + (size_t)(row0 + tok) * p.out_stride + (size_t)head * p.d + c8 * 8;
   if (((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0) {

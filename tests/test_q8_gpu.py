@@ -258,6 +258,14 @@ def test_attention_options(number, heads, kv, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,dim,counts,starts", [(8, 2, 128, [64, 1, 20], [3000, 5000, 2]), (4, 4, 64, [1, 300], [40, 2500]),
+                                                         (8, 2, 128, [1], [4000]), (8, 2, 64, [2, 1], [4000, 700])])
+def test_sinks_that_weigh_as_much_as_the_keys_where_keys_are_shared_out(heads, kv, dim, counts, starts, dtype):
+    c = Case(heads, kv, dim, 16, counts, starts, dtype, seed=5)
+    _check(c, sink=True, sink_values=8 + torch.randn(heads, device=c.device, generator=c.g))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("heads,kv,dim,counts,starts", [
     (8, 2, 128, [1, 1], [9000, 30]), (2, 1, 64, [3], [20000]), (32, 8, 128, [300], [2000]), (4, 4, 128, [1], [40000])])
 def test_attention_over_many_keys(heads, kv, dim, counts, starts, dtype):
