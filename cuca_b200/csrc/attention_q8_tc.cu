@@ -55,13 +55,14 @@ __device__ __forceinline__ uint32_t q8_times(uint32_t a, uint32_t b) {
   return r;
 }
 
-template <int DP>
+template <int DP, bool F32>
 struct Shape {
   static constexpr int HALVES = DP / 64;
   static constexpr int Q_HALF = ROWS * 128, Q_BYTES = HALVES * Q_HALF;
   static constexpr int KV_HALF = KEYS * 128, KV_TILE = HALVES * KV_HALF;
-  static constexpr int FACTORS = (3 * KEYS + 4) * 4;  // of a stage: the keys' factors; the value scales' exponents less E and their
-                                                      // inverse (of a wide tile); E, its inverse, and whether the tile is wide
+  // Of a stage: the keys' factors; the value scales' exponents less E and their inverse (of a wide tile, and in 32-bit mode); (there)
+  // their fractions; E, its inverse, and whether the tile is wide.
+  static constexpr int TILE_E = (F32 ? 4 : 3) * KEYS, FACTORS = (TILE_E + 4) * 4;
   static constexpr int RAW_STAGE = 2 * KEYS * DP + 2 * KEYS * 4;  // codes of a tile's keys and values, their scales
   static constexpr int TILES = NQ * Q_BYTES + (K_STAGES + V_STAGES) * KV_TILE + V_STAGES * FACTORS + RAW * RAW_STAGE;
   static constexpr int SMEM = TILES + 384 + 1024;  // + barriers, + alignment
@@ -110,9 +111,14 @@ __device__ __forceinline__ void tmem_ld32_done(uint32_t taddr, float (&v)[32]) {
 
 // EXTRA: what a score goes through beside its factor: 1: a distance bias, 2: a cap (and a bias). Constants, as a branch a pair of
 // scores keeps their instructions from overlapping (a portion with either took twice the time without).
-template <int DP, int EXTRA>
+// F32: 32-bit rows, one query tile a block. A query goes in as two 16-bit parts, in two operand tiles, and so does a weight; the lower
+// parts have the second query tile's places in shared and tensor memory. (Sums of their own, as the tensor cores cut off what a
+// larger sum has no bits for.) The value scales stay out of the operand tile: their exponents go to the scores and their fractions
+// to the weights, so that codes are exact there too.
+template <int DP, int EXTRA, bool F32>
 __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Params p) {
-  using SH = Shape<DP>;
+  using SH = Shape<DP, F32>;
+  using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
   extern __shared__ uint8_t smem_raw[];
   // (by an offset, so that the compiler still knows it for shared memory)
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -149,11 +155,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   const int G = p.nh / p.nkv, head0 = kvh * G;
   const int seq = p.seq_of_row[row0];
   const int pos0 = p.positions[row0];
-  __nv_bfloat16* out = (__nv_bfloat16*)p.out;
+  T* out = (T*)p.out;
   if (seq < 0 || pos0 < 0) {  // rows of no request
     if (split == 0)
       for (int i = threadIdx.x; i < n_tok * G * p.d; i += NTHREADS)
-        out[(size_t)(row0 + i / (G * p.d)) * p.out_stride + (size_t)head0 * p.d + i % (G * p.d)] = __float2bfloat16_rn(0.f);
+        out[(size_t)(row0 + i / (G * p.d)) * p.out_stride + (size_t)head0 * p.d + i % (G * p.d)] = from_f32<T>(0.f);
     return;
   }
   const Q8Keys keys = q8_keys<KEYS>(p, pos0, n_tok);
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   const bool alone = share >= keys.groups || p.n_splits == 1;
   const int n_tiles = last - first;
   const int tile_tok = ROWS / G;             // tokens of a query tile
-  const int nq = n_tok > tile_tok ? 2 : 1;
+  const int nq = !F32 && n_tok > tile_tok ? 2 : 1;
   const uint32_t per_head = (65536u + G - 1) / G;  // a row of a query tile over G: right for up to 128 of both
   auto token_of = [&](int row) { return (int)(((uint32_t)row * per_head) >> 16); };
 
@@ -176,7 +182,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   }
   if (threadIdx.x == 0) {
     for (int x = 0; x < NQ; ++x) {
-      mbar_init(&q_full[x], 4);
+      mbar_init(&q_full[x], F32 ? SOFT_WARPS : 4);
       mbar_init(&s_full[2 * x], 1);
       mbar_init(&s_full[2 * x + 1], 1);
       mbar_init(&p_full[2 * x], 4);
@@ -293,7 +299,55 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     constexpr int LANES = DP / 8, AT_ONCE = 32 / LANES, SETS = 32 / AT_ONCE;
     const int c = lane % LANES;  // 16 bytes of a row
     uint32_t* bad_s = q_top + 1;  // [8]: rows that are not finite, a bit each
-    {
+    float row_down = 1.f;         // of the thread's row, in 32-bit mode
+    bool bad = false;
+    if constexpr (F32) {
+      // The warps of both query tiles read the same rows, the first four for the upper parts, the others for the lower. Each row has
+      // a power of two of its own.
+      const bool aligned = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 4 == 0;
+#pragma unroll 4
+      for (int i = 0; i < SETS; ++i) {
+        const int row = quarter * 32 + i * AT_ONCE + lane / LANES, t0 = token_of(row);
+        const bool there = row < tile_tok * G && t0 < n_tok && c * 8 < p.d;
+        const float* src = (const float*)p.q + (size_t)(row0 + (there ? t0 : 0)) * p.q_stride + (size_t)(head0 + (there ? row - t0 * G : 0)) * p.d + (there ? c * 8 : 0);
+        float v[8];
+        if (aligned) {
+          const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = src[k];
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, there ? __float_as_uint(v[k]) & 0x7fffffffu : 0u);
+#pragma unroll
+        for (int o = 1; o < LANES; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool none = !there || top >= 0x7f800000u;  // a row that is not finite goes in as zeros and comes out as NaN
+        float up, down;
+        q8_query_scale(top, up, down);
+        const float mine = __shfl_sync(0xffffffffu, down, (lane % AT_ONCE) * LANES);  // (NaN of a row that is not finite)
+        if (lane / AT_ONCE == i) row_down = mine;
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float lo = none ? 0.f : v[2 * k] * up, hi = none ? 0.f : v[2 * k + 1] * up;
+          if (x == 1) {
+            lo -= __half2float(__float2half_rn(lo));
+            hi -= __half2float(__float2half_rn(hi));
+          }
+          h[k] = q8_pack(lo, hi);
+        }
+        *reinterpret_cast<uint4*>(q_s + x * SH::Q_BYTES + (c / 8) * SH::Q_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      bad = !(row_down == row_down);
+      if (bad) row_down = 1.f;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[0]);
+      asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
+    } else {
       uint4 raw_q[SETS];
       uint32_t top = 0, bad_rows = 0;
       const bool aligned = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 8 == 0;
@@ -371,7 +425,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         if (lane == 0) mbar_arrive(&q_full[x]);
       }
     }
-    const bool bad = (bad_s[warp] >> lane) & 1u;
+    if (!F32) bad = (bad_s[warp] >> lane) & 1u;
 
     const int row_pos = pos0 + tok;
     const int row_lo = p.window > 0 ? row_pos - (p.window - 1) : 0;
@@ -393,7 +447,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       if (!warp_wait(&factor_full[st], (j / V_STAGES) & 1, p.err, abort_flag)) { ok = false; break; }
       const float* factor = factor_s + st * (SH::FACTORS / 4);
       const float4* kf4 = reinterpret_cast<const float4*>(factor);
-      const float4 tile_e = kf4[3 * KEYS / 4];  // E, 2^-E, wide
+      const float4 tile_e = kf4[SH::TILE_E / 4];  // E, 2^-E, wide
       const int key0 = keys.at(first + j) * KEYS;
       const bool whole = key0 + KEYS - 1 <= least_pos && (p.window <= 0 || key0 >= most_lo || key0 + KEYS <= p.keep);
       const float bias0 = EXTRA ? slope2 * (float)(key0 - row_pos) : 0.f;
@@ -402,11 +456,22 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       float corr = 1.f;
       bool moved = false;
       float2 sum2[2];
-      uint32_t pw[KEYS / 2];
+      uint32_t pw[KEYS / 2], pw_lo[F32 ? KEYS / 2 : 1];
 #pragma unroll 1
       for (;;) {
         uint32_t raw[2][32];
-        tmem_ld64(tmem_s(x, j) + lane_bits, raw);
+        if constexpr (F32) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float a[32], b[32];
+            tmem_ld32_done(tmem_s(0, j) + lane_bits + h * 32, a);
+            tmem_ld32_done(tmem_s(1, j) + lane_bits + h * 32, b);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) raw[h][i] = __float_as_uint(a[i] + b[i]);
+          }
+        } else {
+          tmem_ld64(tmem_s(x, j) + lane_bits, raw);
+        }
         const float ref = m == -INFINITY ? 0.f : m - Q8_LIFT;  // the exponents are z - ref
         const float2 neg2 = make_float2(tile_e.x - ref, tile_e.x - ref);
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -420,7 +485,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
             for (int h = 0; h < 2; ++h) {
               const int k = 4 * i + 2 * h;
               float2 x2 = make_float2(__uint_as_float(raw[k / 32][k % 32]), __uint_as_float(raw[k / 32][k % 32 + 1]));
-              const float2 f2 = make_float2(f[2 * h], f[2 * h + 1]);
+              float2 f2 = make_float2(f[2 * h], f[2 * h + 1]);
+              if (F32) f2 = __fmul2_rn(f2, make_float2(row_down, row_down));
               if (EXTRA) {
                 x2 = __fmul2_rn(x2, f2);
                 if (EXTRA == 2) x2 = q8_capped_pair(x2, p);
@@ -441,11 +507,21 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
                 sum2[h] = __ffma2_rn(u2, *reinterpret_cast<const float2*>(factor + 2 * KEYS + k), sum2[h]);
               else
                 sum2[h] = __fadd2_rn(sum2[h], u2);
-              pw[k / 2] = q8_pack(u2.x, u2.y);
+              if (F32) {
+                const float2 w2 = __fmul2_rn(u2, *reinterpret_cast<const float2*>(factor + 3 * KEYS + k));
+                pw[k / 2] = q8_pack(w2.x, w2.y);
+                const float2 upper = __half22float2(*reinterpret_cast<const __half2*>(&pw[k / 2]));
+                pw_lo[F32 ? k / 2 : 0] = q8_pack(w2.x - upper.x, w2.y - upper.y);
+              } else {
+                pw[k / 2] = q8_pack(u2.x, u2.y);
+              }
             }
           }
         };
-        if (tile_e.z != 0.f) row(std::true_type{}, std::true_type{});
+        if (F32) {  // (every tile is wide, and E is 0)
+          if (!whole) row(std::true_type{}, std::true_type{});
+          else row(std::false_type{}, std::true_type{});
+        } else if (tile_e.z != 0.f) row(std::true_type{}, std::true_type{});
         else if (!whole) row(std::true_type{}, std::false_type{});
         else row(std::false_type{}, std::false_type{});
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) + ref;
@@ -460,13 +536,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       static_assert(KEYS == 64, "one 32-column store holds a row's weights of a tile");
       __syncwarp();
       tmem_st32_raw(tmem_s(x, j) + lane_bits, pw);
+      if constexpr (F32) tmem_st32_raw(tmem_s(1, j) + lane_bits, pw_lo);
       l = fmaf((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y), tile_e.y, l * corr);
       // O is made smaller where a row's maximum moved; only then must the product before have finished
       if (j > 0 && moved) {
         if (!product_done(j)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
+        for (int c = 0; c < (F32 ? 2 : 1) * DP / 32; ++c) {  // (the lower parts' results follow the upper's)
           float o[32];
           tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);
 #pragma unroll
@@ -482,11 +559,41 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         if (j == 0 && x == 0) mbar_arrive(ahead);
       }
     }
+    auto both = [&](int c, float (&o)[32]) {  // 32 dimensions of the results, in 32-bit mode the sum of both parts'
+      tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);
+      if constexpr (F32) {
+        float lower[32];
+        tmem_ld32_done(tmem_o(1) + lane_bits + c * 32, lower);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] += lower[i];
+      }
+    };
     if (ok && product_done(n_tiles)) {
       tc_fence_after();
       if (alone) {
         if (p.sink && m != -INFINITY) l += q8_sink_term(p, head, m);
         const float inv = bad ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : q8_pow2(-V_LIFT) / l;
+        if constexpr (F32) {
+          const bool mine = r < tile_tok * G && tok < n_tok;
+          float* dst = out + (size_t)(row0 + (mine ? tok : 0)) * p.out_stride + (size_t)head * p.d;
+          const bool aligned = ((uintptr_t)p.out & 15) == 0 && p.out_stride % 4 == 0;
+#pragma unroll
+          for (int c0 = 0; c0 < DP / 32; ++c0) {
+            float o[32];
+            both(c0, o);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const int e = c0 * 32 + q * 4;
+              if (!mine || e >= p.d) continue;
+              if (aligned) {
+                *reinterpret_cast<float4*>(dst + e) = make_float4(o[4 * q] * inv, o[4 * q + 1] * inv, o[4 * q + 2] * inv, o[4 * q + 3] * inv);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) dst[e + k] = o[4 * q + k] * inv;
+              }
+            }
+          }
+        } else {
         // Through shared memory, where the queries were (every product that read them is done), so that what is stored is whole
         // lines; a row's pieces are turned round by its number, as in the operand tiles.
         uint8_t* mine = q_s + x * SH::Q_BYTES + quarter * 32 * (DP * 2);
@@ -526,6 +633,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         };
         if (aligned) store(std::true_type{});
         else store(std::false_type{});
+        }
       } else {
         // [NQ][DP / 4][ROWS][4], then m and l [NQ][2][ROWS]: rows side by side
         float* part = p.part + (((size_t)blockIdx.y * p.nkv + kvh) * p.n_splits + split) * (size_t)(NQ * ROWS * (DP + 2));
@@ -533,7 +641,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
           float o[32];
-          tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);
+          both(c, o);
 #pragma unroll
           for (int q = 0; q < 8; ++q) dst[(c * 8 + q) * ROWS] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
         }
@@ -564,7 +672,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
     float up, down;
     q8_query_scale(*q_top, up, down);
-    const float key_factor = down * (EXTRA == 2 ? p.scale : p.scale_log2e);
+    const float key_factor = (F32 ? 1.f : down) * (EXTRA == 2 ? p.scale : p.scale_log2e);
     for (int j = 0; j < n_tiles; ++j) {
       const int ks_at = j % K_STAGES, st = j % V_STAGES, from = j % RAW;
       if (!warp_wait(&raw_full[from], (j / RAW) & 1, p.err, abort_flag)) break;
@@ -593,13 +701,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         fine[h] = e[h] == e[h];
         if (fine[h] && vs[h] != 0.f) { hi = max(hi, (int)e[h]); least = min(least, (int)e[h]); }
       }
-      hi = __reduce_max_sync(0xffffffffu, hi);
+      hi = F32 ? 0 : __reduce_max_sync(0xffffffffu, hi);
       least = __reduce_min_sync(0xffffffffu, least);
-      const bool wide = hi - least > WIDE;
+      const bool wide = F32 || hi - least > WIDE;
       uint32_t factor2[2];  // what a key's value codes are multiplied by, twice
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float x = fine[h] ? vs[h] * q8_pow2(V_LIFT - (wide ? e[h] : (float)hi)) : 0.f;
+        const float x = F32 ? q8_pow2(V_LIFT) : fine[h] ? vs[h] * q8_pow2(V_LIFT - (wide ? e[h] : (float)hi)) : 0.f;
         factor2[h] = q8_pack(x, x);
       }
       if (j >= V_STAGES && !warp_wait(&v_empty[st], ((j / V_STAGES) & 1) ^ 1, p.err, abort_flag)) break;
@@ -612,12 +720,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
           const int key = lane + 32 * h;
           // (a value row that is not finite: its scores are NaN for those who see it)
           factor[key] = fine[h] ? ks[h] * key_factor : __uint_as_float(0x7fc00000u);
+          if (F32) factor[3 * KEYS + key] = fine[h] ? vs[h] * q8_pow2(-e[h]) : 0.f;
           if (wide) {
             factor[KEYS + key] = fine[h] ? e[h] - (float)hi : 0.f;
             factor[2 * KEYS + key] = fine[h] ? q8_pow2(fmaxf(-126.f, fminf(127.f, (float)hi - e[h]))) : 1.f;
           }
         }
-        if (lane == 0) *reinterpret_cast<float4*>(factor + 3 * KEYS) = make_float4((float)hi, q8_pow2(-(float)hi), wide ? 1.f : 0.f, 0.f);
+        if (lane == 0) *reinterpret_cast<float4*>(factor + SH::TILE_E) = make_float4((float)hi, q8_pow2(-(float)hi), wide ? 1.f : 0.f, 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&factor_full[st]);
       }
@@ -669,8 +778,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
-          umma_bf16(tmem_s(x, t), q_desc + (uint64_t)(((k / 4) * SH::Q_HALF + (k % 4) * 32) >> 4),
-                    kd + (uint64_t)(((k / 4) * SH::KV_HALF + (k % 4) * 32) >> 4), idesc_qk, k > 0);
+#pragma unroll
+          for (int part = 0; part < (F32 ? 2 : 1); ++part)
+            umma_bf16(tmem_s(x + part, t), q_desc + (uint64_t)((part * SH::Q_BYTES + (k / 4) * SH::Q_HALF + (k % 4) * 32) >> 4),
+                      kd + (uint64_t)(((k / 4) * SH::KV_HALF + (k % 4) * 32) >> 4), idesc_qk, k > 0);
         umma_commit(&s_full[2 * x + (t & 1)]);
         umma_commit(&k_empty[st]);
       }
@@ -687,7 +798,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < KEYS / 16; ++k)
-          umma_bf16_tmem_a(tmem_o(x), tmem_s(x, j) + k * 8, vd + (uint64_t)((k * 2048) >> 4), idesc_pv, j > 0 || k > 0);
+#pragma unroll
+          for (int part = 0; part < (F32 ? 2 : 1); ++part)
+            umma_bf16_tmem_a(tmem_o(x + part), tmem_s(x + part, j) + k * 8, vd + (uint64_t)((k * 2048) >> 4), idesc_pv, j > 0 || k > 0);
         umma_commit(&v_empty[st]);
         umma_commit(&pv_done[2 * x + (j & 1)]);
       }
@@ -709,7 +822,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 }
 
 // Joins the shares of a tile's keys, in their order: a thread per query row and eight dimensions.
-template <int DP>
+template <int DP, bool F32>
 __global__ void __launch_bounds__(ROWS) join_q8_tc_kernel(const Q8Params p) {
   pdl_trigger();
   pdl_wait();
@@ -740,7 +853,19 @@ __global__ void __launch_bounds__(ROWS) join_q8_tc_kernel(const Q8Params p) {
   }
   if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top) * q8_pow2(V_LIFT);  // (sums come lifted as results do)
   const float inv = den == 0.f ? 0.f : 1.f / den;
-  __nv_bfloat16* dst = (__nv_bfloat16*)p.out + (size_t)(row0 + tok) * p.out_stride + (size_t)head * p.d + c8 * 8;
+  const size_t to = (size_t)(row0 + tok) * p.out_stride + (size_t)head * p.d + c8 * 8;
+  if constexpr (F32) {
+    float* dst = (float*)p.out + to;
+    if (((uintptr_t)p.out & 15) == 0 && p.out_stride % 4 == 0) {
+      *reinterpret_cast<float4*>(dst) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dst[i] = o[i] * inv;
+    }
+    return;
+  }
+  __nv_bfloat16* dst = (__nv_bfloat16*)p.out + to;
   if (((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0) {
     uint32_t w[4];
 #pragma unroll
@@ -755,29 +880,30 @@ __global__ void __launch_bounds__(ROWS) join_q8_tc_kernel(const Q8Params p) {
   }
 }
 
-template <int DP, int EXTRA>
+template <int DP, int EXTRA, bool F32>
 int launch_q8_tc(const Q8Params& p, int n_tiles, cudaStream_t stream) {
-  constexpr int smem = Shape<DP>::SMEM;
-  auto kernel = attention_q8_tc_kernel<DP, EXTRA>;
+  constexpr int smem = Shape<DP, F32>::SMEM;
+  auto kernel = attention_q8_tc_kernel<DP, EXTRA, F32>;
   static cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   CUCA_REQUIRE(configured == cudaSuccess, "attention_q8_tc: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(configured));
   cuca_launch(kernel, dim3(p.nkv * p.n_splits, n_tiles), dim3(NTHREADS), smem, stream, true, p);
   CUCA_CHECK_LAUNCH("attention_q8_tc");
   if (p.n_splits > 1) {
-    cuca_launch(join_q8_tc_kernel<DP>, dim3(NQ * DP / 8, p.nkv, n_tiles), dim3(ROWS), 0, stream, true, p);
+    cuca_launch(join_q8_tc_kernel<DP, F32>, dim3(NQ * DP / 8, p.nkv, n_tiles), dim3(ROWS), 0, stream, true, p);
     CUCA_CHECK_LAUNCH("attention_q8_tc (join)");
   }
   return 0;
 }
 template <int DP>
-int launch_q8_tc_extra(const Q8Params& p, int n_tiles, cudaStream_t stream) {
-  if (p.cap > 0.f) return launch_q8_tc<DP, 2>(p, n_tiles, stream);
-  return p.slopes ? launch_q8_tc<DP, 1>(p, n_tiles, stream) : launch_q8_tc<DP, 0>(p, n_tiles, stream);
+int launch_q8_tc_extra(const Q8Params& p, bool f32, int n_tiles, cudaStream_t stream) {
+  if (f32) return launch_q8_tc<DP, 0, true>(p, n_tiles, stream);
+  if (p.cap > 0.f) return launch_q8_tc<DP, 2, false>(p, n_tiles, stream);
+  return p.slopes ? launch_q8_tc<DP, 1, false>(p, n_tiles, stream) : launch_q8_tc<DP, 0, false>(p, n_tiles, stream);
 }
 
 }  // namespace
 
-// bfloat16 rows of head sizes up to 128, groups of at most 128 heads whole; `width` (1 or 2) query tiles to a block: tile_tokens is
+// bfloat16 rows, or 32-bit rows (one query tile, neither cap nor bias), of head sizes up to 128, groups of at most 128 heads whole; `width` (1 or 2) query tiles to a block: tile_tokens is
 // that times the tokens whose rows fit 128. part: [n_tiles][nkv][n_splits][256 (d rounded up to 64 or 128) + 512] floats where
 // n_splits > 1.
 CUCA_API int cuca_attention_q8_tc(const CucaQ8Attention* c) {
@@ -785,10 +911,12 @@ CUCA_API int cuca_attention_q8_tc(const CucaQ8Attention* c) {
   Q8Params p;
   if (const int code = q8_params(*c, "attention_q8_tc", 128, p)) return code;
   const int group = p.nh / p.nkv;
-  CUCA_REQUIRE(c->dtype == CUCA_BF16 && group <= ROWS && p.heads_per_cta == group, "attention_q8_tc: bfloat16 rows and groups of at most %d heads", ROWS);
+  const bool f32 = c->dtype == CUCA_F32;
+  CUCA_REQUIRE(group <= ROWS && p.heads_per_cta == group, "attention_q8_tc: groups of at most %d heads, whole", ROWS);
+  CUCA_REQUIRE(!f32 || (c->width == 1 && p.cap == 0.f && !p.slopes), "attention_q8_tc: 32-bit rows one query tile a block, without cap or bias");
   CUCA_REQUIRE(p.n_splits == 1 || p.part, "attention_q8_tc: no place for the shares' results");
   CUCA_REQUIRE((long long)p.n_blocks * p.nkv * p.bs < 0xffffffffll, "attention_q8_tc: more than 2^32 rows in the pools");
   CUCA_REQUIRE((c->width == 1 || c->width == NQ) && p.tile_tokens == (int)c->width * (ROWS / group), "attention_q8_tc: %d rows to %lld query tiles",
                p.tile_tokens, (long long)c->width);
-  return p.d <= 64 ? launch_q8_tc_extra<64>(p, (int)c->n_tiles, c->stream) : launch_q8_tc_extra<128>(p, (int)c->n_tiles, c->stream);
+  return p.d <= 64 ? launch_q8_tc_extra<64>(p, f32, (int)c->n_tiles, c->stream) : launch_q8_tc_extra<128>(p, f32, (int)c->n_tiles, c->stream);
 }

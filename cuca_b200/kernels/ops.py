@@ -1681,6 +1681,11 @@ def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, 
 
 
 Q8_FEW_ROWS = 24  # query rows of a key head that the form for few rows takes of a portion
+# 32-bit rows through tcgen05. The tensor cores cut off what a sum has no bits for: 512 keys in a row at most, then results are
+# joined (values of one sign, 544 keys: 1.2e-6 off as one sum, 3e-7 as two; a prompt of 2,048 228 us, with 1,024 keys in a row 205).
+# And 700,000 pairs of a query row and a key at least: of 45 steps those with more took 0.4 to 1.0 of the other form's time but for
+# seven (up to 1.4 of it), those with fewer 0.9 to 1.6 but for five.
+Q8_SUMS_F32, Q8_LEAST_F32 = 512, 700_000
 Q8_SINGLES_ALONG = 0.25  # single tokens for each portion of a step that go with the portions through tcgen05
 
 
@@ -1712,9 +1717,9 @@ class QuantizedPlan:
             self._arrays = step.positions, step.seq_of_row, step.req_row0, step.req_count
         return self._addresses
 
-    def call(self, dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first):
+    def call(self, dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first, biased=False):
         """(dtype code, options, launches) of a layer's attention: what its numbers ask for, checked once per step."""
-        key = (dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first)
+        key = (dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first, biased)
         entry = self._calls.get(key)
         if entry is None:
             code = dtype_code(dtype)
@@ -1724,31 +1729,37 @@ class QuantizedPlan:
             if window is not None and window < 0 or keep_first < 0 or softcap < 0:
                 raise library.KernelError("a window, kept first keys and a score cap are not negative")
             opt = attention_options(n_heads, scale, window, softcap, sink, None, keep_first)
-            entry = code, opt, self.launches(n_heads, n_kv_heads, head_dim, dtype, window or None, opt.keep)
+            entry = code, opt, self.launches(n_heads, n_kv_heads, head_dim, dtype, window or None, opt.keep, softcap > 0 or biased)
             self._calls[key] = entry
         return entry
 
-    def launches(self, n_heads, n_kv_heads, head_dim, dtype, window, keep):
+    def launches(self, n_heads, n_kv_heads, head_dim, dtype, window, keep, extra=False):
         """[(form, least count, most count, rows of a tile, tiles, heads of a block, width, keys of a share, shares, whether those
         are joined through memory)]; form 0: few rows a block, `width` column tiles of 8; 1: tcgen05, `width` query tiles of 128"""
         key = (n_heads, n_kv_heads, head_dim, dtype, window, keep)
-        if key not in self._launches:
+        extra = extra and dtype == torch.float32  # a cap or a bias, which 32-bit rows do not take through tcgen05
+        if (*key, extra) not in self._launches:
             group, out = n_heads // n_kv_heads, []
             singles = self.counts.count(1)
             portions = len(self.counts) - singles
             # Portions go together: where the longest has few rows a block of few rows each, else all through tcgen05 (twelve
             # requests of up to 9 tokens: those of up to four apart from the rest 56 us, together 46).
-            many = (portions and dtype == torch.bfloat16 and head_dim <= 128 and group <= 128
-                    and self.longest * group > Q8_FEW_ROWS)
+            many = (portions and head_dim <= 128 and group <= 128 and self.longest * group > Q8_FEW_ROWS
+                    and (dtype == torch.bfloat16 or not extra and self._fits_f32(n_heads, window, keep)))
             least = 1 if many and singles <= portions * Q8_SINGLES_ALONG else 2
             if singles and least == 2:
                 out.append(self._few(1, 1, *key))
             if portions:
                 out.append((self._many if many else self._few)(least, self.longest, *key))
             # (last: whether the shares' results go through memory)
-            self._launches[key] = [(*n, n[-1] > 1 and (n[0] == 1 or not _merge_as_cluster(
+            self._launches[*key, extra] = [(*n, n[-1] > 1 and (n[0] == 1 or not _merge_as_cluster(
                 n[4] * n_kv_heads * -(-group // n[5]), n[-1], _q8_resident(sm_count(), head_dim, n[6])))) for n in out]
-        return self._launches[key]
+        return self._launches[*key, extra]
+
+    def _fits_f32(self, n_heads, window, keep) -> bool:
+        pairs = sum(c * (length if window is None else min(length, window + c + keep)) for c, length in zip(self.counts, self.lengths)
+                    if c > 1)
+        return max(self.lengths) <= 64 * Q8_SUMS_F32 and pairs * n_heads >= Q8_LEAST_F32
 
     def _many(self, lo, hi, n_heads, n_kv_heads, head_dim, dtype, window, keep):
         """One or two query tiles a block and how many shares of the keys, by an estimate in key tiles of two query tiles (1.3 us): one
@@ -1760,10 +1771,12 @@ class QuantizedPlan:
         def lengths(n):  # key tiles of 64 of every tile of n rows
             return [-(-(e if window is None else min(e, window + n + keep)) // 64) for c, length in zip(self.counts, self.lengths)
                     if lo <= c <= hi for e in range(length, length - c, -n)]
-        for query_tiles, tile_cost in ((1, 0.7), (2, 1.0)):
+        f32 = dtype == torch.float32
+        for query_tiles, tile_cost in ((1, 0.7),) if f32 else ((1, 0.7), (2, 1.0)):
             tiles = lengths(tokens * query_tiles)
             longest, total = max(tiles), sum(tiles) * n_kv_heads
-            for shares in range(1, min(16, -(-longest // 4)) + 1):
+            least = -(-64 * longest // Q8_SUMS_F32) if f32 else 1
+            for shares in range(least, max(least, min(16, -(-longest // 4))) + 1):
                 share = -(-longest // shares)
                 blocks = sum(-(-t // share) for t in tiles) * n_kv_heads
                 rounds = -(-blocks // sms)
@@ -1842,7 +1855,7 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
     plan = step.plans.get("paged_attention_q8")
     if plan is None:
         plan = attention_q8_plan(step)
-    code, opt, launches = plan.call(dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first)
+    code, opt, launches = plan.call(dtype, n_heads, n_kv_heads, head_dim, scale, window, softcap, sink, keep_first, slopes is not None)
     if sink_values is not None or slopes is not None:
         opt = attention_options(n_heads, scale, window, softcap, sink, sink_values, keep_first, slopes)
     pool = pages.check(n_kv_heads, head_dim)

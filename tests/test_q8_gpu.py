@@ -463,3 +463,58 @@ def test_a_mixed_step_in_every_form(monkeypatch, few, along):
         c = Case(heads, kv, dim, 16, *BATCHES["mixed"], torch.bfloat16, seed=few % 7)
         _check(c)
         _check(c, window=33, keep_first=2, sink=True)
+
+
+@pytest.fixture
+def through_tcgen05(monkeypatch):
+    """32-bit portions of any size through tcgen05, and that they went there."""
+    from cuca_b200.kernels import ops
+    monkeypatch.setattr(ops, "Q8_FEW_ROWS", 0)
+    monkeypatch.setattr(ops, "Q8_LEAST_F32", 0)
+    seen, launches = [], ops.QuantizedPlan.launches
+
+    def watched(self, *a, **k):
+        plan = launches(self, *a, **k)
+        seen.extend(n[0] for n in plan if n[2] > 1)
+        return plan
+    monkeypatch.setattr(ops.QuantizedPlan, "launches", watched)
+    return seen
+
+
+@pytest.mark.parametrize("heads,kv,dim", [s for s in SHAPES if s[2] <= 128])
+def test_32_bit_portions_of_every_shape_through_tcgen05(through_tcgen05, heads, kv, dim):
+    c = Case(heads, kv, dim, 16, *BATCHES["mixed"], torch.float32, seed=dim)
+    _check(c)
+    _check(c, window=33, keep_first=2, sink=True, sink_values=4 * torch.randn(heads, device=c.device, generator=c.g))
+    _check(Case(heads, kv, dim, 24, [3, 2, 130], [0, 1000, 600], torch.float32, seed=dim + 1), scale=0.4)
+    assert set(through_tcgen05) == {1}
+    _check(c, softcap=9.0)  # (this form does not take it)
+    assert set(through_tcgen05) == {0, 1}
+
+
+def test_32_bit_portions_through_tcgen05_where_it_can_go_wrong(through_tcgen05):
+    f32 = torch.float32
+    for page in (1, 8, 24, 128):
+        _check(Case(8, 2, 64, page, *BATCHES["mixed"], f32, seed=page))
+    test_value_scales_far_apart_and_large_scores([200], f32)
+    test_value_scales_far_apart_and_large_scores([40, 1], f32)
+    test_queries_of_any_magnitude(f32)
+    test_what_is_not_finite_reaches_those_who_see_it_alone([30, 150], [50, 20], f32)
+    test_rows_of_no_request_get_zeros([1, 40], f32)
+    test_sinks_that_weigh_as_much_as_the_keys_where_keys_are_shared_out(8, 2, 128, [64, 1, 20], [3000, 5000, 2], f32)
+    assert 1 in through_tcgen05
+
+
+@pytest.mark.parametrize("skew", [0, 1, 2])
+def test_32_bit_portions_through_tcgen05_anywhere_in_memory(through_tcgen05, skew):
+    """Rows that do not begin on 16 bytes, further apart than they are long; the same bits from each, and in every run."""
+    from cuca_b200.kernels import ops
+    c = Case(6, 2, 80, 16, [33, 70], [700, 0], torch.float32, seed=3)
+    want = _attend(c).flatten(1)
+    wide = torch.zeros(c.step.n_rows, 480 + 16 + skew, device=c.device)
+    q, out = wide[:, skew:skew + 480], torch.full_like(wide, 3.0)
+    q.copy_(c.q)
+    for _ in range(3):
+        ops.attention_q8(q, out[:, skew:skew + 480], c.pages(), c.tables, c.step, 6, 2, 80, 80 ** -0.5, None, c.err)
+        assert torch.equal(out[:, skew:skew + 480], want) and int(c.err) == 0
+    assert (out[:, :skew] == 3).all() and (out[:, skew + 480:] == 3).all() and set(through_tcgen05) == {1}
