@@ -1,4 +1,5 @@
-// Causal grouped-query attention over 8-bit pages for few query rows: single tokens, short portions, and the 32-bit mode.
+// Causal grouped-query attention over 8-bit pages for few query rows: single tokens and short portions; and portions that
+// attention_q8_tc.cu does not take (heads beyond 128, 32-bit rows with a score cap or a distance bias).
 // (Scales, weights and their exactness: attention_q8.cuh.)
 //
 // Both products run turned round on mma.sync.m16n8k16 (16-bit floats, 32-bit sums): the 16 rows are keys (then dimensions of

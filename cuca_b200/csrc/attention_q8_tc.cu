@@ -1,5 +1,5 @@
-// Causal grouped-query attention over 8-bit pages for portions of tokens, on the 5th-generation tensor cores (bfloat16 rows,
-// head sizes up to 128). (Scales, weights and their exactness: attention_q8.cuh.)
+// Causal grouped-query attention over 8-bit pages for portions of tokens, on the 5th-generation tensor cores (bfloat16 or 32-bit
+// rows, head sizes up to 128). (Scales, weights and their exactness: attention_q8.cuh.)
 //
 // A block takes up to 2 x 128 query rows of one request and key head, a row being a (token, head) pair, so that every head of
 // the group shares the block's keys and values, and walks the keys in tiles of 64:
@@ -18,7 +18,7 @@
 // one, the keys' scales, is left of four. Where a tile's scales are more than 2^20 apart the exponents stay with the keys
 // (`wide`). The keys' scales multiply the scores, so codes of keys are exact.
 //
-// Measured, 32 heads of 128 over 8: a prompt of 2,048 58 us (590 TFLOP/s), a portion of 512 on 8,192 107 us (664 TFLOP/s; over
+// Measured, 32 heads of 128 over 8: a prompt of 2,048 58 us (590 TFLOP/s), a portion of 512 on 8,192 106 us (668 TFLOP/s; over
 // bfloat16 pages, attention_tc.cu, 56 and 138). A tile of 64 keys takes two query tiles some 2,450 clocks, of which the tensor
 // pipe and the exponent unit need 1,024 each. No unit sets the pace: without seven eighths of the softmax's arithmetic the portion
 // took 20 % less, without most products 9 %, without all three roles' work still 72 us. What is left is the way round: a score
@@ -113,8 +113,9 @@ __device__ __forceinline__ void tmem_ld32_done(uint32_t taddr, float (&v)[32]) {
 // scores keeps their instructions from overlapping (a portion with either took twice the time without).
 // F32: 32-bit rows, one query tile a block. A query goes in as two 16-bit parts, in two operand tiles, and so does a weight; the lower
 // parts have the second query tile's places in shared and tensor memory. (Sums of their own, as the tensor cores cut off what a
-// larger sum has no bits for.) The value scales stay out of the operand tile: their exponents go to the scores and their fractions
-// to the weights, so that codes are exact there too.
+// larger sum has no bits for; the errors are half of those of one sum.) The value scales stay out of the operand tile: their exponents go to the scores and their fractions
+// to the weights, so that codes are exact there too. 32 heads of 128 over 8: a prompt of 2,048 228 us, a portion of 512 on 8,192 368
+// (attention_q8.cu: 418 and 706), bound by a start and a join every 512 keys, which the errors ask for, and four factors a key.
 template <int DP, int EXTRA, bool F32>
 __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Params p) {
   using SH = Shape<DP, F32>;
