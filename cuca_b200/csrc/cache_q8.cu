@@ -11,11 +11,9 @@
 // bytes a decode step reads; the error of a value is at most half a 127th of its row's largest.
 //
 // Both kernels do a few operations per byte and are bound by memory, or by latency when there are few rows. Measured, 32 heads of
-// 128 over 8: writing 2,048 rows 14.5 us (torch's copy of the queries' part alone: 13.1), reading 34,000 positions back 51 us
-// (5.3 TB/s, 0.81 of a copy's rate).
+// 128 over 8: writing 2,048 rows and reading them back 16.4 us (10.5 and 6.4 by themselves; torch's copy of the queries' part alone
+// takes 13.1), reading 34,000 positions back 51 us (5.3 TB/s, 0.81 of a copy's rate).
 #include "common.cuh"
-
-int cuca_device_sms();
 
 // A launch of either, as Python packs it: one 64-bit word each, in this order (kernels/ops.py:rope_store_q8, read_q8).
 struct CucaQ8Store {
@@ -92,12 +90,6 @@ __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
   const float4 x = *reinterpret_cast<const float4*>(p);
   v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
 }
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&v)[4]) {
-  const uint2 x = *reinterpret_cast<const uint2*>(p);
-  v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
-  v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
-}
-__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
   __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
@@ -113,8 +105,20 @@ __device__ __forceinline__ uint32_t codes4(const float (&v)[4], float inv) {
   return inv > 0.f ? codes : 0;
 }
 
-// A group of lanes takes one head of a row, of ROWS rows in turn whose loads go out together; a lane has values 4 l .. 4 l + 3 of
-// each half of the head, which are the rotation's pairs where the whole head is rotated in halves (VEC: 8- or 16-byte accesses).
+// A row's scale from its largest magnitude, and what its values are multiplied by (0: the codes are).
+__device__ __forceinline__ void row_scale(uint32_t top, float& scale, float& inv) {
+  const float most = __uint_as_float(top);
+  scale = inv = 0.f;
+  if (top >= 0x7f800000u) {
+    scale = __uint_as_float(0x7fc00000u);
+  } else if (most >= CUCA_Q8_TINY) {
+    scale = __fdiv_rn(most, 127.f);
+    inv = __fdiv_rn(127.f, most);
+  }
+}
+
+// A group of lanes takes one head of a row; a lane has values 4 l .. 4 l + 3 of each half of the head, which are the rotation's
+// pairs where the whole head is rotated in halves (VEC, of K slices: 16-byte accesses).
 // Else (part of the head rotated, neighbours as pairs, rows that are not aligned) the same values are fetched one by one with
 // their partners. A head stays within a warp, and everything is read before anything is written: q_out may be the rows
 // themselves. SLICES: the rows are a contraction's K slices, added in their order in 32 bits (and the bias to the sum), and not
@@ -129,138 +133,202 @@ __device__ __forceinline__ float row_value(const StoreParams& p, size_t at, int 
     return p.bias ? x + to_f32(((const T*)p.bias)[column]) : x;
   }
 }
-template <typename T, bool SLICES>
-__device__ __forceinline__ void row_values(const StoreParams& p, size_t at, int column, float (&v)[4]) {
-  if constexpr (!SLICES) {
-    load4((const T*)p.qkv + at, v);
-  } else {
+template <typename T>
+__device__ __forceinline__ void sliced_values(const StoreParams& p, size_t at, int column, float (&v)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = 0.f;
+  for (int i = 0; i < 4; ++i) v[i] = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < p.slices; ++s) {
-      float x[4];
-      load4((const float*)p.qkv + s * p.slice_stride + at, x);
+  for (int s = 0; s < p.slices; ++s) {
+    float x[4];
+    load4((const float*)p.qkv + s * p.slice_stride + at, x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += x[i];
-    }
-    if (p.bias)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += to_f32(((const T*)p.bias)[column + i]);
+    for (int i = 0; i < 4; ++i) v[i] += x[i];
   }
+  if (p.bias)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += to_f32(((const T*)p.bias)[column + i]);
 }
-template <typename T, bool VEC, int ROWS, bool SLICES>
-__global__ void __launch_bounds__(STORE_THREADS, ROWS > 1 ? 4 : 1) rope_store_q8_kernel(const StoreParams p) {
+template <typename T, bool VEC, bool SLICES>
+__global__ void __launch_bounds__(STORE_THREADS) rope_store_q8_kernel(const StoreParams p) {
   pdl_trigger();
   pdl_wait();
   const int heads = p.nh + 2 * p.nkv;
   const int head = (int)((blockIdx.x * STORE_THREADS + threadIdx.x) >> p.seg_shift);
   const int l = threadIdx.x & ((1 << p.seg_shift) - 1);
-  const int half = p.d / 2;
+  const int half = p.d / 2, row = blockIdx.y;
   const bool lane_ok = head < heads && 4 * l < half;
   const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
   const bool rotate = !is_v && p.rot > 0;
-  const int row0 = blockIdx.y * ROWS;
-  int seq[ROWS], pos[ROWS];
-  bool live[ROWS];
-  float a[ROWS][4], b[ROWS][4], c[VEC ? ROWS : 1][4], s[VEC ? ROWS : 1][4];
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int row = row0 + r;
-    seq[r] = row < p.n_rows ? p.seq_of_row[row] : -1;
-    pos[r] = row < p.n_rows ? p.positions[row] : 0;
-    live[r] = lane_ok && seq[r] >= 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[r][i] = b[r][i] = 0.f;
-    if (VEC && lane_ok && row < p.n_rows) {  // (whoever's the row is: its numbers need not be known first)
-      const size_t at = (size_t)row * p.row_stride + (size_t)head * p.d;
-      row_values<T, SLICES>(p, at + 4 * l, head * p.d + 4 * l, a[r]);
-      row_values<T, SLICES>(p, at + half + 4 * l, head * p.d + half + 4 * l, b[r]);
-    }
+  const int seq = p.seq_of_row[row], pos = p.positions[row];
+  const bool live = lane_ok && seq >= 0;
+  const size_t from = (size_t)row * p.row_stride + (size_t)head * p.d;
+  float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
+  if (VEC && lane_ok) {  // (whoever's the row is: its numbers need not be known first)
+    sliced_values<T>(p, from + 4 * l, head * p.d + 4 * l, a);
+    sliced_values<T>(p, from + half + 4 * l, head * p.d + half + 4 * l, b);
   }
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const bool in_table = pos[r] >= 0 && pos[r] < p.table_rows;
-    const float* cr = p.cos_t + (size_t)(in_table ? pos[r] : 0) * (p.rot / 2);
-    const float* sr = p.sin_t + (size_t)(in_table ? pos[r] : 0) * (p.rot / 2);
-    if (VEC) {
-      if (rotate && lane_ok) {
-        load4(cr + 4 * l, c[VEC ? r : 0]);
-        load4(sr + 4 * l, s[VEC ? r : 0]);
-      }
-    } else if (live[r]) {
-      const size_t at = (size_t)(row0 + r) * p.row_stride + (size_t)head * p.d;
-      auto src = [&](int e) { return row_value<T, SLICES>(p, at + e, head * p.d + e); };
-      auto value = [&](int e) {
-        const float x = src(e);
-        if (!rotate || !in_table || e >= p.rot) return x;
-        const int hr = p.rot / 2;
-        const int i = p.adjacent ? e / 2 : (e < hr ? e : e - hr);
-        const bool first = p.adjacent ? (e & 1) == 0 : e < hr;
-        const float cs = cr[i], sn = sr[i];
-        const float y = src(p.adjacent ? e ^ 1 : (first ? e + hr : i));
-        return first ? __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn)) : __fadd_rn(__fmul_rn(y, sn), __fmul_rn(x, cs));
-      };
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { a[r][i] = value(4 * l + i); b[r][i] = value(half + 4 * l + i); }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const bool in_table = pos[r] >= 0 && pos[r] < p.table_rows;
-    if (rotate && live[r] && !in_table && l == 0 && p.err) atomicExch(p.err, CUCA_ERR_TOKEN_RANGE);
-    if (VEC && rotate && in_table && lane_ok) {
+  const bool in_table = pos >= 0 && pos < p.table_rows;
+  if (rotate && live && !in_table && l == 0 && p.err) atomicExch(p.err, CUCA_ERR_TOKEN_RANGE);
+  const float* cr = p.cos_t + (size_t)(in_table ? pos : 0) * (p.rot / 2);
+  const float* sr = p.sin_t + (size_t)(in_table ? pos : 0) * (p.rot / 2);
+  if (VEC) {
+    if (rotate && in_table && lane_ok) {
+      float c[4], s[4];
+      load4(cr + 4 * l, c);
+      load4(sr + 4 * l, s);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float x = a[r][i], y = b[r][i], cs = c[VEC ? r : 0][i], sn = s[VEC ? r : 0][i];
-        a[r][i] = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
-        b[r][i] = __fadd_rn(__fmul_rn(x, sn), __fmul_rn(y, cs));
+        const float x = a[i], y = b[i];
+        a[i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
+        b[i] = __fadd_rn(__fmul_rn(x, s[i]), __fmul_rn(y, c[i]));
       }
     }
-    // the largest magnitude of the head, as bits: anything not finite compares above every number
-    uint32_t top = 0;
+  } else if (live) {
+    auto src = [&](int e) { return row_value<T, SLICES>(p, from + e, head * p.d + e); };
+    auto value = [&](int e) {
+      const float x = src(e);
+      if (!rotate || !in_table || e >= p.rot) return x;
+      const int hr = p.rot / 2;
+      const int i = p.adjacent ? e / 2 : (e < hr ? e : e - hr);
+      const bool first = p.adjacent ? (e & 1) == 0 : e < hr;
+      const float cs = cr[i], sn = sr[i];
+      const float y = src(p.adjacent ? e ^ 1 : (first ? e + hr : i));
+      return first ? __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn)) : __fadd_rn(__fmul_rn(y, sn), __fmul_rn(x, cs));
+    };
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      top = max(top, max(__float_as_uint(a[r][i]) & 0x7fffffffu, __float_as_uint(b[r][i]) & 0x7fffffffu));
-    for (int o = (1 << p.seg_shift) >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));  // (and all has been read)
-    if (!live[r]) continue;
-    const int row = row0 + r;
-    if (is_q) {
-      T* dst = (T*)p.q_out + (size_t)row * p.q_stride + (size_t)head * p.d;
-      if (VEC) {
-        store4(dst + 4 * l, a[r]);
-        store4(dst + half + 4 * l, b[r]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { dst[4 * l + i] = from_f32<T>(a[r][i]); dst[half + 4 * l + i] = from_f32<T>(b[r][i]); }
-      }
-      continue;
-    }
-    const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
-    const int entry = pos[r] / p.bs;
-    const int blk = pos[r] >= 0 && entry < p.table_stride ? p.tables[(size_t)seq[r] * p.table_stride + entry] : -1;
-    if (blk < 0 || blk >= p.n_blocks) {
-      if (l == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
-      continue;
-    }
-    const size_t at = ((size_t)blk * p.nkv + kvh) * p.bs + pos[r] % p.bs;
-    const float most = __uint_as_float(top);
-    float scale, inv;
-    if (top >= 0x7f800000u) {
-      scale = __uint_as_float(0x7fc00000u);
-      inv = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[r][i] = b[r][i] = 0.f;
-    } else if (most < CUCA_Q8_TINY) {
-      scale = inv = 0.f;
-    } else {
-      scale = __fdiv_rn(most, 127.f);
-      inv = __fdiv_rn(127.f, most);
-    }
-    int8_t* dst = (is_v ? p.vpool : p.kpool) + at * p.d;
-    *reinterpret_cast<uint32_t*>(dst + 4 * l) = codes4(a[r], inv);
-    *reinterpret_cast<uint32_t*>(dst + half + 4 * l) = codes4(b[r], inv);
-    if (l == 0) (is_v ? p.vscale : p.kscale)[at] = scale;
+    for (int i = 0; i < 4; ++i) { a[i] = value(4 * l + i); b[i] = value(half + 4 * l + i); }
   }
+  // the largest magnitude of the head, as bits: anything not finite compares above every number
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
+  for (int o = (1 << p.seg_shift) >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));  // (and all has been read)
+  if (!live) return;
+  if (is_q) {
+    T* dst = (T*)p.q_out + (size_t)row * p.q_stride + (size_t)head * p.d;
+    if constexpr (VEC) {
+      store4(dst + 4 * l, a);
+      store4(dst + half + 4 * l, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { dst[4 * l + i] = from_f32<T>(a[i]); dst[half + 4 * l + i] = from_f32<T>(b[i]); }
+    }
+    return;
+  }
+  const int entry = pos / p.bs;
+  const int blk = pos >= 0 && entry < p.table_stride ? p.tables[(size_t)seq * p.table_stride + entry] : -1;
+  if (blk < 0 || blk >= p.n_blocks) {
+    if (l == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+    return;
+  }
+  float scale, inv;
+  row_scale(top, scale, inv);
+  const size_t at = ((size_t)blk * p.nkv + (is_v ? head - p.nh - p.nkv : head - p.nh)) * p.bs + (pos - entry * p.bs);
+  int8_t* dst = (is_v ? p.vpool : p.kpool) + at * p.d;
+  *reinterpret_cast<uint32_t*>(dst + 4 * l) = codes4(a, inv);
+  *reinterpret_cast<uint32_t*>(dst + half + 4 * l) = codes4(b, inv);
+  if (l == 0) (is_v ? p.vscale : p.kscale)[at] = scale;
+}
+
+// The same for rows on 16 bytes that are rotated whole, in halves, or not at all: a lane has eight values of either half of a head.
+// gridDim: rows, heads.
+// (Blocks of 96 threads: 2,048 rows written and read back 16.4 us; 64 17.8, 128 17.1, 256 20.3; two heads a thread 2 more.)
+constexpr int LINE = 8, LINE_THREADS = 96;
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p + i);
+    v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+  }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 x = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&x);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_codes8(int8_t* p, const float (&v)[8], float inv) {
+  const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+  *reinterpret_cast<uint2*>(p) = make_uint2(codes4(lo, inv), codes4(hi, inv));
+}
+template <typename T>
+__global__ void __launch_bounds__(LINE_THREADS, 16) rope_store_q8_lines_kernel(const StoreParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int heads = p.nh + 2 * p.nkv, half = p.d / 2, row = blockIdx.x;
+  const int head = (int)((blockIdx.y * LINE_THREADS + threadIdx.x) >> p.seg_shift);
+  const int l = threadIdx.x & ((1 << p.seg_shift) - 1);
+  const bool lane_ok = head < heads && LINE * l < half;
+  const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+  const int seq = p.seq_of_row[row], pos = p.positions[row];
+  float a[LINE], b[LINE];
+#pragma unroll
+  for (int i = 0; i < LINE; ++i) a[i] = b[i] = 0.f;
+  if (lane_ok) {  // (whoever's the row is: its numbers need not be known first)
+    const T* src = (const T*)p.qkv + (size_t)row * p.row_stride + (size_t)head * p.d + LINE * l;
+    load8(src, a);
+    load8(src + half, b);
+  }
+  if (seq < 0) return;
+  int blk = -1, entry = 0;
+  if (lane_ok && !is_q) {
+    entry = pos / p.bs;
+    if (pos >= 0 && entry < p.table_stride) blk = p.tables[(size_t)seq * p.table_stride + entry];
+  }
+  const bool in_table = pos >= 0 && pos < p.table_rows;
+  if (p.rot > 0 && !in_table && threadIdx.x == 0 && blockIdx.y == 0 && p.err) atomicExch(p.err, CUCA_ERR_TOKEN_RANGE);
+  if (p.rot > 0 && in_table && lane_ok && !is_v) {
+    const float *cr = p.cos_t + (size_t)pos * half + LINE * l, *sr = p.sin_t + (size_t)pos * half + LINE * l;
+#pragma unroll
+    for (int j = 0; j < LINE; j += 4) {
+      float c[4], s[4];
+      load4(cr + j, c);
+      load4(sr + j, s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = a[j + i], y = b[j + i];
+        a[j + i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
+        b[j + i] = __fadd_rn(__fmul_rn(x, s[i]), __fmul_rn(y, c[i]));
+      }
+    }
+  }
+  if (lane_ok && is_q) {
+    T* dst = (T*)p.q_out + (size_t)row * p.q_stride + (size_t)head * p.d + LINE * l;
+    store8(dst, a);
+    store8(dst + half, b);
+  }
+  if (!__any_sync(0xffffffffu, lane_ok && !is_q)) return;  // (a warp of queries)
+  // the largest magnitude of the head, as bits: anything not finite compares above every number
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < LINE; ++i)
+    top = max(top, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
+  for (int o = (1 << p.seg_shift) >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (!lane_ok || is_q) return;
+  if (blk < 0 || blk >= p.n_blocks) {
+    if (l == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
+    return;
+  }
+  float scale, inv;
+  row_scale(top, scale, inv);
+  const size_t at = ((size_t)blk * p.nkv + (is_v ? head - p.nh - p.nkv : head - p.nh)) * p.bs + (pos - entry * p.bs);
+  int8_t* dst = (is_v ? p.vpool : p.kpool) + at * p.d + LINE * l;
+  store_codes8(dst, a, inv);
+  store_codes8(dst + half, b, inv);
+  if (l == 0) (is_v ? p.vscale : p.kscale)[at] = scale;
 }
 
 // ------------------------------------------------------------------ reading back
@@ -396,23 +464,28 @@ CUCA_API int cuca_rope_store_q8(const CucaQ8Store* c) {
   StoreParams p{qkv, row_stride, q_out, q_stride, c->positions, c->seq_of_row, c->tables, table_stride, cos_t, sin_t, table_rows, rot,
                 adjacent, (int8_t*)kpool, (int8_t*)vpool, c->kscale, c->vscale, n_blocks, bs, n_rows, nh, nkv, d, 0, (int)c->slices,
                 (size_t)c->slice_stride, c->bias, c->err};
-  while ((8 << p.seg_shift) < d) ++p.seg_shift;
-  const bool slices = c->slices > 0;
+  const bool slices = c->slices > 0, whole = (rot == d || rot == 0) && !adjacent;
+  const uintptr_t tables = (uintptr_t)cos_t | (uintptr_t)sin_t;
   CUCA_REQUIRE(!slices || (dtype == CUCA_BF16 && c->slices <= 64 && c->slice_stride >= 0), "rope_store_q8: K slices give bfloat16 queries");
-  const uintptr_t align = dtype == CUCA_F32 ? 15 : 7, from = slices ? 15 : align;
-  const bool vec = (rot == d || rot == 0) && !adjacent && row_stride % 4 == 0 && q_stride % 4 == 0 &&
-                   ((uintptr_t)qkv & from) == 0 && (!slices || c->slice_stride % 4 == 0) && ((uintptr_t)q_out & align) == 0 && (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15) == 0;
-  const unsigned blocks = (unsigned)((((long long)(nh + 2 * nkv) << p.seg_shift) + STORE_THREADS - 1) / STORE_THREADS);
-  // two rows a thread where that still fills the GPU with threads
-  const bool many = vec && !slices && (long long)blocks * n_rows >= 8ll * 2 * cuca_device_sms();
-  const int per = many ? 2 : 1;
-  CUCA_REQUIRE((n_rows + per - 1) / per <= 65535, "rope_store_q8: too many rows");
-  auto kernel = slices ? (vec ? rope_store_q8_kernel<__nv_bfloat16, true, 1, true> : rope_store_q8_kernel<__nv_bfloat16, false, 1, true>)
-      : dtype == CUCA_F32
-      ? (many ? rope_store_q8_kernel<float, true, 2, false> : vec ? rope_store_q8_kernel<float, true, 1, false> : rope_store_q8_kernel<float, false, 1, false>)
-      : (many ? rope_store_q8_kernel<__nv_bfloat16, true, 2, false> : vec ? rope_store_q8_kernel<__nv_bfloat16, true, 1, false>
-                                                                         : rope_store_q8_kernel<__nv_bfloat16, false, 1, false>);
-  cuca_launch(kernel, dim3(blocks, (n_rows + per - 1) / per), dim3(STORE_THREADS), 0, stream, true, p);
+  const int heads = nh + 2 * nkv, line = dtype == CUCA_F32 ? 4 : 8;  // values of 16 bytes
+  if (!slices && whole && row_stride % line == 0 && q_stride % line == 0 &&
+      (((uintptr_t)qkv | (uintptr_t)q_out | tables) & 15) == 0 && (((uintptr_t)kpool | (uintptr_t)vpool) & 7) == 0) {
+    while ((2 * LINE << p.seg_shift) < d) ++p.seg_shift;
+    const unsigned blocks = (unsigned)((((long long)heads << p.seg_shift) + LINE_THREADS - 1) / LINE_THREADS);
+    auto kernel = dtype == CUCA_F32 ? rope_store_q8_lines_kernel<float> : rope_store_q8_lines_kernel<__nv_bfloat16>;
+    CUCA_REQUIRE(blocks <= 65535, "rope_store_q8: too many heads");
+    cuca_launch(kernel, dim3(n_rows, blocks), dim3(LINE_THREADS), 0, stream, true, p);
+    CUCA_CHECK_LAUNCH("rope_store_q8");
+    return 0;
+  }
+  while ((8 << p.seg_shift) < d) ++p.seg_shift;
+  const bool vec = slices && whole && row_stride % 4 == 0 && q_stride % 4 == 0 && (((uintptr_t)qkv | tables) & 15) == 0 &&
+                   c->slice_stride % 4 == 0 && ((uintptr_t)q_out & 7) == 0;
+  const unsigned blocks = (unsigned)((((long long)heads << p.seg_shift) + STORE_THREADS - 1) / STORE_THREADS);
+  CUCA_REQUIRE(n_rows <= 65535, "rope_store_q8: too many rows");
+  auto kernel = vec ? rope_store_q8_kernel<__nv_bfloat16, true, true> : slices ? rope_store_q8_kernel<__nv_bfloat16, false, true>
+      : dtype == CUCA_F32 ? rope_store_q8_kernel<float, false, false> : rope_store_q8_kernel<__nv_bfloat16, false, false>;
+  cuca_launch(kernel, dim3(blocks, n_rows), dim3(STORE_THREADS), 0, stream, true, p);
   CUCA_CHECK_LAUNCH("rope_store_q8");
   return 0;
 }
