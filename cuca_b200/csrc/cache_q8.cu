@@ -11,9 +11,11 @@
 // bytes a decode step reads; the error of a value is at most half a 127th of its row's largest.
 //
 // Both kernels do a few operations per byte and are bound by memory, or by latency when there are few rows. Measured, 32 heads of
-// 128 over 8: writing 2,048 rows and reading them back 16.4 us (10.5 and 6.4 by themselves; torch's copy of the queries' part alone
-// takes 13.1), reading 34,000 positions back 51 us (5.3 TB/s, 0.81 of a copy's rate).
+// 128 over 8: writing 2,048 rows and reading them back 16.4 us (10.5 and 5.1 by themselves; torch's copy of the queries' part alone
+// takes 13.1), reading 34,000 positions back 47 us (5.8 TB/s, 0.89 of a copy's rate).
 #include "common.cuh"
+
+int cuca_device_sms();
 
 // A launch of either, as Python packs it: one 64-bit word each, in this order (kernels/ops.py:rope_store_q8, read_q8).
 struct CucaQ8Store {
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(LINE_THREADS, 16) rope_store_q8_lines_kernel(c
 }
 
 // ------------------------------------------------------------------ reading back
-constexpr int READ_WARPS = 8, READ_ROWS = 4, READ_PIECES = 4;
+constexpr int READ_WARPS = 2, READ_PIECES = 4;
 
 template <typename T> struct Piece;  // what a thread writes at once: 16 bytes
 template <> struct Piece<float> { static constexpr int N = 4; using Codes = uint32_t; };
@@ -352,13 +354,13 @@ struct ReadParams {
 
 __device__ __forceinline__ uint32_t word_of(uint32_t w, int) { return w; }
 __device__ __forceinline__ uint32_t word_of(const uint2& w, int i) { return i == 0 ? w.x : w.y; }
-// What uses the value stays behind this point, and so behind the other loads (34,000 positions: 51 us, left to the compiler 80).
+// What uses the value stays behind this point, and so behind the other loads (34,000 positions: 47 us, left to the compiler 80).
 __device__ __forceinline__ void stay(uint32_t& w) { asm volatile("" : "+r"(w)); }
 __device__ __forceinline__ void stay(uint2& w) { asm volatile("" : "+r"(w.x), "+r"(w.y)); }
 
-// A warp brings READ_PIECES x 32 pieces of a row, of one tensor, for READ_ROWS rows whose loads go out together: a lane's places in
+// A warp brings READ_PIECES x 32 pieces of a row, of one tensor, for ROWS rows whose loads go out together: a lane's places in
 // the page and in the row are the same for all of them. gridDim: rows, pieces, tensors.
-template <typename T>
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(READ_WARPS * 32) read_q8_kernel(const __grid_constant__ ReadParams p) {
   pdl_trigger();
   pdl_wait();
@@ -379,22 +381,22 @@ __global__ void __launch_bounds__(READ_WARPS * 32) read_q8_kernel(const __grid_c
     head[i] = piece < per_row ? piece / per_head : -1;
     e[i] = (piece - max(head[i], 0) * per_head) * N;
   }
-  const int row0 = (blockIdx.x * READ_WARPS + warp) * READ_ROWS;
-  int seq[READ_ROWS], pos[READ_ROWS], blk[READ_ROWS];
+  const int row0 = (blockIdx.x * READ_WARPS + warp) * ROWS;
+  int seq[ROWS], pos[ROWS], blk[ROWS];
 #pragma unroll
-  for (int r = 0; r < READ_ROWS; ++r) {
+  for (int r = 0; r < ROWS; ++r) {
     seq[r] = row0 + r < p.n_rows ? p.seq_of_row[row0 + r] : -1;
     pos[r] = row0 + r < p.n_rows ? p.positions[row0 + r] : 0;
   }
 #pragma unroll
-  for (int r = 0; r < READ_ROWS; ++r) {
+  for (int r = 0; r < ROWS; ++r) {
     const int entry = pos[r] / p.bs;
     blk[r] = seq[r] >= 0 && pos[r] >= 0 && entry < p.table_stride ? p.tables[(size_t)seq[r] * p.table_stride + entry] : -1;
   }
-  typename P::Codes w[READ_ROWS][READ_PIECES];
-  float s[READ_ROWS][READ_PIECES];
+  typename P::Codes w[ROWS][READ_PIECES];
+  float s[ROWS][READ_PIECES];
 #pragma unroll
-  for (int r = 0; r < READ_ROWS; ++r) {
+  for (int r = 0; r < ROWS; ++r) {
     const bool there = blk[r] >= 0 && blk[r] < p.n_blocks;
     if (!there && seq[r] >= 0 && lane == 0 && p.err) atomicExch(p.err, CUCA_ERR_BLOCK_RANGE);
     const size_t at = (size_t)(there ? blk[r] : 0) * p.nkv * p.bs + (there ? pos[r] % p.bs : 0);
@@ -410,11 +412,11 @@ __global__ void __launch_bounds__(READ_WARPS * 32) read_q8_kernel(const __grid_c
     }
   }
 #pragma unroll
-  for (int r = 0; r < READ_ROWS; ++r)
+  for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int i = 0; i < READ_PIECES; ++i) stay(w[r][i]);
 #pragma unroll
-  for (int r = 0; r < READ_ROWS; ++r) {
+  for (int r = 0; r < ROWS; ++r) {
     if (row0 + r >= p.n_rows) break;
 #pragma unroll
     for (int i = 0; i < READ_PIECES; ++i) {
@@ -510,9 +512,14 @@ CUCA_API int cuca_read_q8(const CucaQ8Read* c) {
   ReadParams p{{(const int8_t*)kpool, (const int8_t*)vpool}, {c->kscale, c->vscale}, {k_out, v_out}, {k_stride, v_stride},
                c->positions, c->seq_of_row, c->tables, table_stride, n_blocks, bs, n_rows, nkv, d, c->err};
   const int pieces = nkv * d / n;  // of a row
-  const dim3 grid((n_rows + READ_WARPS * READ_ROWS - 1) / (READ_WARPS * READ_ROWS), (pieces + 32 * READ_PIECES - 1) / (32 * READ_PIECES), 2);
+  // Four rows a warp where that leaves 16 warps an SM (34,000 rows of 8 heads of 128: 47 us, with one row 54), else one (2,048 rows:
+  // 5.1 us, with four 6.3).
+  const unsigned across = (unsigned)((pieces + 32 * READ_PIECES - 1) / (32 * READ_PIECES));
+  const int rows = (long long)n_rows / 4 * across * 2 >= 16ll * cuca_device_sms() ? 4 : 1;
+  const dim3 grid((n_rows + READ_WARPS * rows - 1) / (READ_WARPS * rows), across, 2);
   CUCA_REQUIRE(grid.y <= 65535, "read_q8: too many heads");
-  auto kernel = dtype == CUCA_F32 ? read_q8_kernel<float> : read_q8_kernel<__nv_bfloat16>;
+  auto kernel = dtype == CUCA_F32 ? (rows == 4 ? read_q8_kernel<float, 4> : read_q8_kernel<float, 1>)
+                                  : (rows == 4 ? read_q8_kernel<__nv_bfloat16, 4> : read_q8_kernel<__nv_bfloat16, 1>);
   cuca_launch(kernel, grid, dim3(READ_WARPS * 32), 0, stream, true, p);
   CUCA_CHECK_LAUNCH("read_q8");
   return 0;

@@ -187,6 +187,12 @@ def test_reading_back_is_exact(dtype, kv, dim, page, totals):
     assert torch.equal(only, v) and int(c.err) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kv,dim,page,totals", [(2, 64, 16, [4003, 1500, 1]), (9, 256, 24, [2051, 333]), (1, 16, 64, [9001])])
+def test_reading_many_rows_back_is_exact(kv, dim, page, totals, dtype):
+    test_reading_back_is_exact(dtype=dtype, kv=kv, dim=dim, page=page, totals=totals)
+
+
 def test_no_rows_write_and_read_nothing():
     c = Case(2, 1, 32, 16, [4], [0], torch.float32, fill=False)
     empty = torch.empty(0, dtype=torch.int32, device=c.device)
