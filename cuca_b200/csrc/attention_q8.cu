@@ -427,10 +427,10 @@ attention_q8_kernel(const Q8Params p) {
         }
         uint32_t packed;
         if (PARTS == 2) {
-          const float hi = __half2float(__float2half_rn(w[0]));
-          packed = q8_pack(hi, w[0] - hi);
+          const uint32_t upper = q8_pack_weights(w[0], 0.f);
+          packed = (upper & 0xffffu) | q8_pack_weights(0.f, w[0] - __half22float2(*reinterpret_cast<const __half2*>(&upper)).x);
         } else {
-          packed = q8_pack(w[0], w[LC - 1]);
+          packed = q8_pack_weights(w[0], w[LC - 1]);
         }
         wb[j][r] = turned_8x8(packed);
       }

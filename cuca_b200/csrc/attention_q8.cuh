@@ -20,7 +20,10 @@
 namespace {
 
 // Weights are less than 2^(LIFT + LAG + 1): the running maximum follows a larger one only when it is exceeded by more than LAG
-// (rescaling is rare then), and LIFT puts the weights' 29 binades of full precision below 2^15.
+// (rescaling is rare then), and LIFT puts the weights' 29 binades of full precision below 2^15. Of scores from some 2^20 on 32-bit
+// numbers have no steps that small: a score is rounded before the reference is taken off, as the maximum was, so that the largest
+// has its exponent to within a step, and a weight that a rounded reference makes too large for a 16-bit float becomes the largest
+// one. (Keys that close to the largest share the weight in no certain proportion then: their scores' own steps are larger.)
 constexpr float Q8_LIFT = 7.f, Q8_LAG = 7.f;
 
 }  // namespace
@@ -190,6 +193,11 @@ __device__ __forceinline__ float q8_exp2(float x) {  // 2^x; 0 at -infinity
 __device__ __forceinline__ uint32_t q8_pack(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t q8_pack_weights(float lo, float hi) {  // finite, but for what is no number
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 __device__ __forceinline__ float q8_pow2(float e) {  // 2^e, e a whole number of -126 .. 127
   return __uint_as_float((uint32_t)((int)e + 127) << 23);

@@ -488,14 +488,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
               float2 x2 = make_float2(__uint_as_float(raw[k / 32][k % 32]), __uint_as_float(raw[k / 32][k % 32 + 1]));
               float2 f2 = make_float2(f[2 * h], f[2 * h + 1]);
               if (F32) f2 = __fmul2_rn(f2, make_float2(row_down, row_down));
-              if (EXTRA) {
-                x2 = __fmul2_rn(x2, f2);
-                if (EXTRA == 2) x2 = q8_capped_pair(x2, p);
-                x2 = __fadd2_rn(x2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
-                x2 = __fadd2_rn(x2, neg2);
-              } else {
-                x2 = __ffma2_rn(x2, f2, neg2);
-              }
+              x2 = __fmul2_rn(x2, f2);
+              if (EXTRA == 2) x2 = q8_capped_pair(x2, p);
+              if (EXTRA) x2 = __fadd2_rn(x2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
+              x2 = __fadd2_rn(x2, neg2);
               if (decltype(wide)::value) x2 = __fadd2_rn(x2, *reinterpret_cast<const float2*>(factor + KEYS + k));
               if (decltype(masked)::value) {
                 const int kp = key0 + k;
@@ -510,11 +506,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
                 sum2[h] = __fadd2_rn(sum2[h], u2);
               if (F32) {
                 const float2 w2 = __fmul2_rn(u2, *reinterpret_cast<const float2*>(factor + 3 * KEYS + k));
-                pw[k / 2] = q8_pack(w2.x, w2.y);
+                pw[k / 2] = q8_pack_weights(w2.x, w2.y);
                 const float2 upper = __half22float2(*reinterpret_cast<const __half2*>(&pw[k / 2]));
-                pw_lo[F32 ? k / 2 : 0] = q8_pack(w2.x - upper.x, w2.y - upper.y);
+                pw_lo[F32 ? k / 2 : 0] = q8_pack_weights(w2.x - upper.x, w2.y - upper.y);
               } else {
-                pw[k / 2] = q8_pack(u2.x, u2.y);
+                pw[k / 2] = q8_pack_weights(u2.x, u2.y);
               }
             }
           }

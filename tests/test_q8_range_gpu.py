@@ -1,0 +1,89 @@
+"""The attention over 8-bit pages where magnitudes, masks, page tables and sizes lie far apart, against its formulas in 64 bits
+(`q8_util`); writing many rows; what a call leaves behind."""
+import itertools
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from q8_util import Case
+
+pytestmark = pytest.mark.gpu
+DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+
+
+@pytest.fixture(scope="module", autouse=True)
+def lib():
+    from cuca_b200.kernels import library
+    return library.load()
+
+
+@pytest.fixture
+def through_tcgen05(monkeypatch):
+    """Portions of any size through tcgen05."""
+    from cuca_b200.kernels import ops
+    monkeypatch.setattr(ops, "Q8_FEW_ROWS", 0)
+    monkeypatch.setattr(ops, "Q8_LEAST_F32", 0)
+
+
+def _call(c, window=None, scale=None, **options):
+    from cuca_b200.kernels import ops
+    out = torch.full((c.step.n_rows, c.heads * c.dim), 5.0, dtype=c.dtype, device=c.device)
+    ops.attention_q8(c.q, out, c.pages(), c.tables, c.step, c.heads, c.kv, c.dim, scale or c.dim ** -0.5, window, c.err, **options)
+    return out.view(-1, c.heads, c.dim)
+
+
+def _check(c, scale=None, most_work=math.inf, **options):
+    got = _call(c, scale=scale, **options)
+    assert int(c.err) == 0
+    want, size, work, most = c.attend(scale or c.dim ** -0.5, **options)
+    off = (got.double() - want).abs() - c.bound(want, size, work.clamp_max(most_work), most)
+    assert (off <= 0).all(), (float(off.max()), float((got.double() - want).abs().max()))
+    return got
+
+
+def _at(c, positions, request=0):
+    """Where positions of a request stand in the pools, for all key heads."""
+    p = torch.as_tensor(positions, device=c.device)
+    return c.tables[c.slots[request]].long()[p // c.page], slice(None), p % c.page
+
+
+# ------------------------------------------------------------------ magnitudes
+def _one_axis(counts, starts, dtype, positions, scores, values, value_scales):
+    """The first request's queries are 1 along the first dimension alone: its scores (in log2 units, with a scale of ln 2, whose
+    product with log2 e is 1 in 32 bits) are what its keys say, and `values` codes times `value_scales` its values."""
+    c = Case(8, 2, 64, 16, counts, starts, dtype, seed=1)
+    c.q.zero_()
+    c.q.view(-1, 8, 64)[..., 0] = 1
+    where = _at(c, positions)
+    k = torch.zeros(len(positions), 64, dtype=torch.int8, device=c.device)
+    k[:, 0] = -1
+    c.k[where] = k[:, None].expand(-1, 2, -1)
+    c.k_scale[where] = -torch.as_tensor(scores, device=c.device).float()[:, None].expand(-1, 2)
+    c.v[where] = torch.as_tensor(values, device=c.device).to(torch.int8)[:, None, None].expand(-1, 2, 64)
+    c.v_scale[where] = torch.as_tensor(value_scales, device=c.device).float()[:, None].expand(-1, 2)
+    return c
+
+
+@DTYPES
+@pytest.mark.parametrize("count", [1, 2, 40])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [3, 16, 20, 23, 24, 25, 26, 27, 28, 30, 40, 60, 90])
+def test_scores_with_steps_of_one_and_more(through_tcgen05, power, sign, count, dtype):
+    """Scores of 2^power and the next few 32-bit numbers above, over all the rest: the larger comes 64 keys later each time. Where
+    steps are smaller than one the weights are the formula's; else results lie between the values of the largest three."""
+    n = 400
+    for odd in (0, 1):
+        step = max(1.0, 2.0 ** (power - 23))
+        scores = np.full(n, min(0.0, 2 * sign * 2.0 ** power) - 1000.0)
+        largest = [3, 67, 131]
+        scores[largest] = sign * 2.0 ** power + step * (odd + np.array([1, 2, 4]))
+        codes = np.arange(n) % 100 + 20
+        c = _one_axis([count], [n - count], dtype, range(n), scores, codes, np.full(n, 2.0 ** -3))
+        if power <= 23:  # (the scores are exact: what a form's 32-bit sums cost shows between keys less than some 2^8 apart)
+            _check(c, scale=math.log(2), most_work=2.0 ** 8)
+            continue
+        got, near = _call(c, scale=math.log(2)), 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -19
+        assert int(c.err) == 0
+        assert (got >= codes[largest].min() / 8 * (1 - near)).all() and (got <= codes[largest].max() / 8 * (1 + near)).all()
