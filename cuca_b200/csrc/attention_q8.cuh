@@ -1,8 +1,9 @@
 // What the attention kernels over 8-bit pages share: their parameters, which rows a block takes, scores and codes.
 //
 // A cached row is d signed codes and a 32-bit scale (csrc/cache_q8.cu). Codes are whole numbers of at most 127, exact in
-// 16-bit floats, and a query times a power of two is too where it came in bfloat16 (in 32-bit mode it goes in two 16-bit
-// parts), so the raw score q . codes is as exact as a 32-bit sum of exact products. The scales never touch the codes:
+// 16-bit floats, and a query times a power of two is too where it came in bfloat16, down to some 2^-20 of its row's largest (in
+// 32-bit mode it goes in two 16-bit parts), so the raw score q . codes is as exact as a 32-bit sum of exact products. A row's power
+// of two never depends on other rows. The scales never touch the codes:
 //
 //   s_j = raw_j ks_j (scale log2 e)                 the key's scale multiplies its score (log2 units)
 //   vs_j = f_j 2^e_j, 1 <= f_j < 2                  the value's scale goes into the weight: its exponent into the softmax's,

@@ -47,6 +47,12 @@ constexpr int K_STAGES = 3, V_STAGES = 3;
 constexpr int RAW = 3;  // tiles of codes on their way
 constexpr float V_LIFT = 7.f;     // values are 2^7 larger in the operand tile: 127 2^7 2 is the most that fits
 constexpr int WIDE = 20;
+// bfloat16 queries whose row's largest magnitude is 2^-6 to 2^9, as good as all, go in times 2^6, whatever rows are beside them: what
+// 16-bit floats have no steps for is 2^-25 of that magnitude and less. Another row has a power of two of its own, and its warp
+// walks the keys in a way of its own, which multiplies by the inverse (a portion of 512 on 8,192 136 us if all do, 107 if none).
+constexpr float Q_UNIT = 64.f;
+// Scores of such size have steps of an eighth: they are walked in that way too, which rounds a score before the reference is taken off.
+constexpr float FAR = 1048576.f;
 constexpr int TMEM_COLS = 512;  // two score buffers per query tile (4 x 64 columns), results of both (2 x DP)
 
 __device__ __forceinline__ uint32_t q8_times(uint32_t a, uint32_t b) {
@@ -144,7 +150,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   uint64_t* ahead = pv_done + 2 * NQ;        // the first query tile has handed over its first weights
   uint32_t* tmem_slot = (uint32_t*)(ahead + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  uint32_t* q_top = tmem_slot + 2;           // the largest magnitude of the block's queries, as bits
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
@@ -206,7 +211,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     }
     mbar_init(ahead, 4);
     *abort_flag = 0;
-    *q_top = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tc_fence_before();
@@ -299,134 +303,117 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     // The warp's 32 rows of queries: DP / 8 lanes a row, so that a request for them is whole lines.
     constexpr int LANES = DP / 8, AT_ONCE = 32 / LANES, SETS = 32 / AT_ONCE;
     const int c = lane % LANES;  // 16 bytes of a row
-    uint32_t* bad_s = q_top + 1;  // [8]: rows that are not finite, a bit each
-    float row_down = 1.f;         // of the thread's row, in 32-bit mode
-    bool bad = false;
-    if constexpr (F32) {
-      // The warps of both query tiles read the same rows, the first four for the upper parts, the others for the lower. Each row has
-      // a power of two of its own.
-      const bool aligned = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 4 == 0;
-#pragma unroll 4
-      for (int i = 0; i < SETS; ++i) {
-        const int row = quarter * 32 + i * AT_ONCE + lane / LANES, t0 = token_of(row);
-        const bool there = row < tile_tok * G && t0 < n_tok && c * 8 < p.d;
-        const float* src = (const float*)p.q + (size_t)(row0 + (there ? t0 : 0)) * p.q_stride + (size_t)(head0 + (there ? row - t0 * G : 0)) * p.d + (there ? c * 8 : 0);
-        float v[8];
+    // In 32-bit mode both halves of the warps read the same rows, the first for the upper parts, the second for the lower.
+    float row_down = 1.f;  // of the thread's row
+    {
+      constexpr int PIECES = F32 ? 2 : 1;                                         // of 16 bytes
+      constexpr int AHEAD = F32 ? 4 : SETS, LOG_AHEAD = AHEAD == 4 ? 2 : AHEAD == 8 ? 3 : 4;  // sets whose loads are out together
+      const bool aligned = ((uintptr_t)p.q & 15) == 0 && p.q_stride % (16 / (int)sizeof(T)) == 0;
+#pragma unroll
+      for (int i0 = 0; i0 < SETS; i0 += AHEAD) {
+        uint4 raw_q[AHEAD][PIECES];
+        uint32_t there = 0;  // a bit a set
+        auto piece = [&](int i) {  // where the lane's piece of set i stands (of rows that are not there: another's)
+          const int row = quarter * 32 + (i0 + i) * AT_ONCE + lane / LANES, t0 = token_of(row), its_tok = (F32 ? 0 : x * tile_tok) + t0;
+          const bool ok = (F32 || x < nq) && row < tile_tok * G && its_tok < n_tok && c * 8 < p.d;
+          if (ok) there |= 1u << i;
+          return (const T*)p.q + (size_t)(row0 + (ok ? its_tok : 0)) * p.q_stride + (size_t)(head0 + (ok ? row - t0 * G : 0)) * p.d + (ok ? c * 8 : 0);
+        };
         if (aligned) {
-          const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
-          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+#pragma unroll
+          for (int i = 0; i < AHEAD; ++i) {
+            const uint4* src = reinterpret_cast<const uint4*>(piece(i));
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n) raw_q[i][n] = src[n];
+          }
         } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = src[k];
-        }
-        uint32_t top = 0;
+          for (int i = 0; i < AHEAD; ++i) {
+            const T* src = piece(i);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = max(top, there ? __float_as_uint(v[k]) & 0x7fffffffu : 0u);
-#pragma unroll
-        for (int o = 1; o < LANES; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const bool none = !there || top >= 0x7f800000u;  // a row that is not finite goes in as zeros and comes out as NaN
-        float up, down;
-        q8_query_scale(top, up, down);
-        const float mine = __shfl_sync(0xffffffffu, down, (lane % AT_ONCE) * LANES);  // (NaN of a row that is not finite)
-        if (lane / AT_ONCE == i) row_down = mine;
-        uint32_t h[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float lo = none ? 0.f : v[2 * k] * up, hi = none ? 0.f : v[2 * k + 1] * up;
-          if (x == 1) {
-            lo -= __half2float(__float2half_rn(lo));
-            hi -= __half2float(__float2half_rn(hi));
+            for (int n = 0; n < PIECES; ++n) {
+              if constexpr (F32) {
+                const uint32_t* h = reinterpret_cast<const uint32_t*>(src) + 4 * n;
+                raw_q[i][n] = make_uint4(h[0], h[1], h[2], h[3]);
+              } else {
+                const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
+                raw_q[i][n] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+              }
+            }
           }
-          h[k] = q8_pack(lo, hi);
         }
-        *reinterpret_cast<uint4*>(q_s + x * SH::Q_BYTES + (c / 8) * SH::Q_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-            make_uint4(h[0], h[1], h[2], h[3]);
-      }
-      bad = !(row_down == row_down);
-      if (bad) row_down = 1.f;
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[0]);
-      asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
-    } else {
-      uint4 raw_q[SETS];
-      uint32_t top = 0, bad_rows = 0;
-      const bool aligned = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 8 == 0;
-      auto at = [&](int i, bool& ok) {  // where the lane's piece of set i stands (of rows that are not there: another's)
-        const int row = quarter * 32 + i * AT_ONCE + lane / LANES, t0 = token_of(row), its_tok = x * tile_tok + t0;
-        ok = x < nq && row < tile_tok * G && its_tok < n_tok && c * 8 < p.d;
-        return (const __nv_bfloat16*)p.q + (size_t)(row0 + (ok ? its_tok : 0)) * p.q_stride + (size_t)(head0 + (ok ? row - t0 * G : 0)) * p.d + (ok ? c * 8 : 0);
-      };
-      if (aligned) {
+        // The rows' largest magnitudes, as bits: of half the sets at each step, so that lane i of a row ends with one set's.
+        uint32_t top[AHEAD];
 #pragma unroll
-        for (int i = 0; i < SETS; ++i) {
-          bool ok;
-          const uint4 w = *reinterpret_cast<const uint4*>(at(i, ok));
-          raw_q[i] = ok ? w : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < AHEAD; ++i) {
+          top[i] = 0;
+#pragma unroll
+          for (int n = 0; n < PIECES; ++n) {
+            uint4& w = raw_q[i][n];
+            if (!((there >> i) & 1u)) w = make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              top[i] = max(top[i], F32 ? words[k] & 0x7fffffffu : max((words[k] << 16) & 0x7fffffffu, words[k] & 0x7fff0000u));
+          }
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < SETS; ++i) {
-          bool ok;
-          const unsigned short* h = reinterpret_cast<const unsigned short*>(at(i, ok));
-          raw_q[i] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
-          if (!ok) raw_q[i] = make_uint4(0u, 0u, 0u, 0u);
-        }
-      }
-      auto top_of = [&](const uint4& q) {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        uint32_t m = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) m = max(m, max((w[k] << 16) & 0x7fffffffu, w[k] & 0x7fff0000u));
-        return m;
-      };
-#pragma unroll
-      for (int i = 0; i < SETS; ++i) top = max(top, top_of(raw_q[i]));
-      if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {
-        // a row that is not finite goes in as zeros and comes out as NaN
-        top = 0;
-#pragma unroll
-        for (int i = 0; i < SETS; ++i) {
-          const uint32_t its = top_of(raw_q[i]);
-          const uint32_t hit = __ballot_sync(0xffffffffu, its >= 0x7f800000u);
-          const uint32_t mates = (LANES == 32 ? 0xffffffffu : (1u << (LANES & 31)) - 1) << (lane / LANES * LANES);
-          if (hit & mates) {
-            bad_rows |= 1u << (i * AT_ONCE + lane / LANES);
-            raw_q[i] = make_uint4(0u, 0u, 0u, 0u);
+        auto halve = [&](auto size, int o) {  // n sets a lane become n / 2 (one stays one)
+          constexpr int n = decltype(size)::value;
+          const bool upper = lane & o;
+          if constexpr (n == 1) {
+            top[0] = max(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
           } else {
-            top = max(top, its);
-          }
-        }
-        bad_rows = __reduce_or_sync(0xffffffffu, bad_rows);
-      }
-      // One power of two for the block's rows: what it costs rows much smaller than the largest is far below what a score can
-      // show.
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) {
-        atomicMax(q_top, top);
-        bad_s[warp] = bad_rows;
-      }
-      asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
-      float up, down;
-      q8_query_scale(*q_top, up, down);
-      if (x < nq) {
 #pragma unroll
-        for (int i = 0; i < SETS; ++i) {
-          const int row = quarter * 32 + i * AT_ONCE + lane / LANES;
-          const uint32_t w[4] = {raw_q[i].x, raw_q[i].y, raw_q[i].z, raw_q[i].w};
+            for (int i = 0; i < n / 2; ++i) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? top[i] : top[i + n / 2], o);
+              top[i] = max(upper ? top[i + n / 2] : top[i], other);
+            }
+          }
+        };
+        halve(std::integral_constant<int, AHEAD>{}, 1);
+        halve(std::integral_constant<int, AHEAD / 2>{}, 2);
+        halve(std::integral_constant<int, (AHEAD > 4 ? AHEAD / 4 : 1)>{}, 4);
+        if (LANES == 16) halve(std::integral_constant<int, (AHEAD > 8 ? AHEAD / 8 : 1)>{}, 8);
+        auto holder = [&](int i) { return (int)(__brev((uint32_t)i) >> (32 - LOG_AHEAD)); };  // the lane of a row that has set i's
+        float its_up, its_down;  // (not finite: 0 and NaN; such a row goes in as zeros and comes out as NaN)
+        q8_query_scale(top[0], its_up, its_down);
+        if (!F32) {
+          const float most = __uint_as_float(top[0]);
+          const bool usual = (most >= 1.f / 64.f && most < 512.f) || top[0] == 0;
+          its_up = usual ? Q_UNIT : its_up;
+          its_down = usual ? 1.f : its_down * Q_UNIT;
+        }
+        const float mine = __shfl_sync(0xffffffffu, its_down, (lane % AT_ONCE) * LANES + holder((lane / AT_ONCE) % AHEAD));
+        if (lane / AT_ONCE / AHEAD == i0 / AHEAD) row_down = mine;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const int row = quarter * 32 + (i0 + i) * AT_ONCE + lane / LANES;
+          const float up = __shfl_sync(0xffffffffu, its_up, lane / LANES * LANES + holder(i));
           uint32_t h[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            h[k] = q8_pack(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xffff0000u) * up);
+          for (int k = 0; k < 4; ++k) {
+            const uint4& w = raw_q[i][F32 ? k / 2 : 0];
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            float lo = F32 ? __uint_as_float(words[2 * k % 4]) : __uint_as_float(words[k] << 16);
+            float hi = F32 ? __uint_as_float(words[(2 * k + 1) % 4]) : __uint_as_float(words[k] & 0xffff0000u);
+            lo = up == 0.f ? 0.f : lo * up;
+            hi = up == 0.f ? 0.f : hi * up;
+            if (F32 && x == 1) {
+              lo -= __half2float(__float2half_rn(lo));
+              hi -= __half2float(__float2half_rn(hi));
+            }
+            h[k] = q8_pack(lo, hi);
+          }
           *reinterpret_cast<uint4*>(q_s + x * SH::Q_BYTES + (c / 8) * SH::Q_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
               make_uint4(h[0], h[1], h[2], h[3]);
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[x]);
       }
     }
-    if (!F32) bad = (bad_s[warp] >> lane) & 1u;
+    const bool bad = !(row_down == row_down);
+    if (bad) row_down = 1.f;
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_full[F32 ? 0 : x]);
 
     const int row_pos = pos0 + tok;
     const int row_lo = p.window > 0 ? row_pos - (p.window - 1) : 0;
@@ -440,122 +427,136 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     auto product_done = [&](int j) {
       return warp_wait(&pv_done[2 * x + ((j - 1) & 1)], ((j - 1) >> 1) & 1, p.err, abort_flag);
     };
-    for (int j = 0; ok && j < n_tiles; ++j) {
-      const int st = j % V_STAGES;
-      if (!warp_wait(&s_full[2 * x + (j & 1)], (j >> 1) & 1, p.err, abort_flag)) { ok = false; break; }
-      tc_fence_after();
-      // (long complete: they were written with the keys)
-      if (!warp_wait(&factor_full[st], (j / V_STAGES) & 1, p.err, abort_flag)) { ok = false; break; }
-      const float* factor = factor_s + st * (SH::FACTORS / 4);
-      const float4* kf4 = reinterpret_cast<const float4*>(factor);
-      const float4 tile_e = kf4[SH::TILE_E / 4];  // E, 2^-E, wide
-      const int key0 = keys.at(first + j) * KEYS;
-      const bool whole = key0 + KEYS - 1 <= least_pos && (p.window <= 0 || key0 >= most_lo || key0 + KEYS <= p.keep);
-      const float bias0 = EXTRA ? slope2 * (float)(key0 - row_pos) : 0.f;
-      // Weights relative to the maximum of the tiles before, with this tile's maximum beside them, so that the exponents need not
-      // wait for it; only where a row exceeds the reference by more than 2^LAG is the tile's row read and worked out again.
-      float corr = 1.f;
-      bool moved = false;
-      float2 sum2[2];
-      uint32_t pw[KEYS / 2], pw_lo[F32 ? KEYS / 2 : 1];
+    // The tiles from j0 on; returns the one where scores became too large for it. own: for rows with powers of two of their own and
+    // scores of any size.
+    auto walk = [&](auto own, int j0) {
+      for (int j = j0; ok && j < n_tiles; ++j) {
+        const int st = j % V_STAGES;
+        if (!warp_wait(&s_full[2 * x + (j & 1)], (j >> 1) & 1, p.err, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        // (long complete: they were written with the keys)
+        if (!warp_wait(&factor_full[st], (j / V_STAGES) & 1, p.err, abort_flag)) { ok = false; break; }
+        const float* factor = factor_s + st * (SH::FACTORS / 4);
+        const float4* kf4 = reinterpret_cast<const float4*>(factor);
+        const float4 tile_e = kf4[SH::TILE_E / 4];  // E, 2^-E, wide
+        const int key0 = keys.at(first + j) * KEYS;
+        const bool whole = key0 + KEYS - 1 <= least_pos && (p.window <= 0 || key0 >= most_lo || key0 + KEYS <= p.keep);
+        const float bias0 = EXTRA ? slope2 * (float)(key0 - row_pos) : 0.f;
+        // Weights relative to the maximum of the tiles before, with this tile's maximum beside them, so that the exponents need not
+        // wait for it; only where a row exceeds the reference by more than 2^LAG is the tile's row read and worked out again.
+        float corr = 1.f;
+        bool moved = false;
+        float2 sum2[2];
+        uint32_t pw[KEYS / 2], pw_lo[F32 ? KEYS / 2 : 1];
 #pragma unroll 1
-      for (;;) {
-        uint32_t raw[2][32];
-        if constexpr (F32) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float a[32], b[32];
-            tmem_ld32_done(tmem_s(0, j) + lane_bits + h * 32, a);
-            tmem_ld32_done(tmem_s(1, j) + lane_bits + h * 32, b);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) raw[h][i] = __float_as_uint(a[i] + b[i]);
-          }
-        } else {
-          tmem_ld64(tmem_s(x, j) + lane_bits, raw);
-        }
-        const float ref = m == -INFINITY ? 0.f : m - Q8_LIFT;  // the exponents are z - ref
-        const float2 neg2 = make_float2(tile_e.x - ref, tile_e.x - ref);
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        sum2[0] = sum2[1] = make_float2(0.f, 0.f);
-        auto row = [&](auto masked, auto wide) {
-#pragma unroll
-          for (int i = 0; i < KEYS / 4; ++i) {
-            const float4 kf = kf4[i];
-            const float f[4] = {kf.x, kf.y, kf.z, kf.w};
+        for (;;) {
+          uint32_t raw[2][32];
+          if constexpr (F32) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int k = 4 * i + 2 * h;
-              float2 x2 = make_float2(__uint_as_float(raw[k / 32][k % 32]), __uint_as_float(raw[k / 32][k % 32 + 1]));
-              float2 f2 = make_float2(f[2 * h], f[2 * h + 1]);
-              if (F32) f2 = __fmul2_rn(f2, make_float2(row_down, row_down));
-              x2 = __fmul2_rn(x2, f2);
-              if (EXTRA == 2) x2 = q8_capped_pair(x2, p);
-              if (EXTRA) x2 = __fadd2_rn(x2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
-              x2 = __fadd2_rn(x2, neg2);
-              if (decltype(wide)::value) x2 = __fadd2_rn(x2, *reinterpret_cast<const float2*>(factor + KEYS + k));
-              if (decltype(masked)::value) {
-                const int kp = key0 + k;
-                if (!(kp <= row_pos && (kp >= row_lo || kp < p.keep))) x2.x = -INFINITY;
-                if (!(kp + 1 <= row_pos && (kp + 1 >= row_lo || kp + 1 < p.keep))) x2.y = -INFINITY;
-              }
-              const float2 u2 = make_float2(q8_exp2(x2.x), q8_exp2(x2.y));
-              mx4[k / 2 & 3] = fmaxf(fmaxf(mx4[k / 2 & 3], x2.x), x2.y);
-              if (decltype(wide)::value)
-                sum2[h] = __ffma2_rn(u2, *reinterpret_cast<const float2*>(factor + 2 * KEYS + k), sum2[h]);
-              else
-                sum2[h] = __fadd2_rn(sum2[h], u2);
-              if (F32) {
-                const float2 w2 = __fmul2_rn(u2, *reinterpret_cast<const float2*>(factor + 3 * KEYS + k));
-                pw[k / 2] = q8_pack_weights(w2.x, w2.y);
-                const float2 upper = __half22float2(*reinterpret_cast<const __half2*>(&pw[k / 2]));
-                pw_lo[F32 ? k / 2 : 0] = q8_pack_weights(w2.x - upper.x, w2.y - upper.y);
-              } else {
-                pw[k / 2] = q8_pack_weights(u2.x, u2.y);
+              float a[32], b[32];
+              tmem_ld32_done(tmem_s(0, j) + lane_bits + h * 32, a);
+              tmem_ld32_done(tmem_s(1, j) + lane_bits + h * 32, b);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) raw[h][i] = __float_as_uint(a[i] + b[i]);
+            }
+          } else {
+            tmem_ld64(tmem_s(x, j) + lane_bits, raw);
+          }
+          const float ref = m == -INFINITY ? 0.f : m - Q8_LIFT;  // the exponents are z - ref
+          const float2 neg2 = make_float2(tile_e.x - ref, tile_e.x - ref);
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          sum2[0] = sum2[1] = make_float2(0.f, 0.f);
+          auto row = [&](auto masked, auto wide) {
+#pragma unroll
+            for (int i = 0; i < KEYS / 4; ++i) {
+              const float4 kf = kf4[i];
+              const float f[4] = {kf.x, kf.y, kf.z, kf.w};
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int k = 4 * i + 2 * h;
+                float2 x2 = make_float2(__uint_as_float(raw[k / 32][k % 32]), __uint_as_float(raw[k / 32][k % 32 + 1]));
+                float2 f2 = make_float2(f[2 * h], f[2 * h + 1]);
+                if (decltype(own)::value) {
+                  f2 = __fmul2_rn(f2, make_float2(row_down, row_down));
+                  x2 = make_float2(__fmul_rn(x2.x, f2.x), __fmul_rn(x2.y, f2.y));  // (a product of two and a sum become one instruction)
+                } else if (EXTRA) {
+                  x2 = __fmul2_rn(x2, f2);
+                }
+                if (EXTRA) {
+                  if (EXTRA == 2) x2 = q8_capped_pair(x2, p);
+                  x2 = __fadd2_rn(x2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
+                }
+                x2 = EXTRA || decltype(own)::value ? __fadd2_rn(x2, neg2) : __ffma2_rn(x2, f2, neg2);
+                if (decltype(wide)::value) x2 = __fadd2_rn(x2, *reinterpret_cast<const float2*>(factor + KEYS + k));
+                if (decltype(masked)::value) {
+                  const int kp = key0 + k;
+                  if (!(kp <= row_pos && (kp >= row_lo || kp < p.keep))) x2.x = -INFINITY;
+                  if (!(kp + 1 <= row_pos && (kp + 1 >= row_lo || kp + 1 < p.keep))) x2.y = -INFINITY;
+                }
+                const float2 u2 = make_float2(q8_exp2(x2.x), q8_exp2(x2.y));
+                mx4[k / 2 & 3] = fmaxf(fmaxf(mx4[k / 2 & 3], x2.x), x2.y);
+                if (decltype(wide)::value)
+                  sum2[h] = __ffma2_rn(u2, *reinterpret_cast<const float2*>(factor + 2 * KEYS + k), sum2[h]);
+                else
+                  sum2[h] = __fadd2_rn(sum2[h], u2);
+                if (F32) {
+                  const float2 w2 = __fmul2_rn(u2, *reinterpret_cast<const float2*>(factor + 3 * KEYS + k));
+                  pw[k / 2] = q8_pack_weights(w2.x, w2.y);
+                  const float2 upper = __half22float2(*reinterpret_cast<const __half2*>(&pw[k / 2]));
+                  pw_lo[F32 ? k / 2 : 0] = q8_pack_weights(w2.x - upper.x, w2.y - upper.y);
+                } else {
+                  pw[k / 2] = q8_pack_weights(u2.x, u2.y);
+                }
               }
             }
+          };
+          if (F32) {  // (every tile is wide, and E is 0)
+            if (!whole) row(std::true_type{}, std::true_type{});
+            else row(std::false_type{}, std::true_type{});
+          } else if (tile_e.z != 0.f) row(std::true_type{}, std::true_type{});
+          else if (decltype(own)::value || !whole) row(std::true_type{}, std::false_type{});
+          else row(std::false_type{}, std::false_type{});
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) + ref;
+          const bool moves = mx > m + Q8_LAG;
+          if (!__any_sync(0xffffffffu, moves)) break;
+          if (!decltype(own)::value && !moved && __any_sync(0xffffffffu, moves && fabsf(mx) >= FAR)) return j;
+          if (moves) {
+            corr = q8_exp2(m - mx);
+            m = mx;
           }
-        };
-        if (F32) {  // (every tile is wide, and E is 0)
-          if (!whole) row(std::true_type{}, std::true_type{});
-          else row(std::false_type{}, std::true_type{});
-        } else if (tile_e.z != 0.f) row(std::true_type{}, std::true_type{});
-        else if (!whole) row(std::true_type{}, std::false_type{});
-        else row(std::false_type{}, std::false_type{});
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) + ref;
-        const bool moves = mx > m + Q8_LAG;
-        if (!__any_sync(0xffffffffu, moves)) break;
-        if (moves) {
-          corr = q8_exp2(m - mx);
-          m = mx;
+          moved = true;
         }
-        moved = true;
-      }
-      static_assert(KEYS == 64, "one 32-column store holds a row's weights of a tile");
-      __syncwarp();
-      tmem_st32_raw(tmem_s(x, j) + lane_bits, pw);
-      if constexpr (F32) tmem_st32_raw(tmem_s(1, j) + lane_bits, pw_lo);
-      l = fmaf((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y), tile_e.y, l * corr);
-      // O is made smaller where a row's maximum moved; only then must the product before have finished
-      if (j > 0 && moved) {
-        if (!product_done(j)) { ok = false; break; }
-        tc_fence_after();
+        static_assert(KEYS == 64, "one 32-column store holds a row's weights of a tile");
+        __syncwarp();
+        tmem_st32_raw(tmem_s(x, j) + lane_bits, pw);
+        if constexpr (F32) tmem_st32_raw(tmem_s(1, j) + lane_bits, pw_lo);
+        l = fmaf((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y), tile_e.y, l * corr);
+        // O is made smaller where a row's maximum moved; only then must the product before have finished
+        if (j > 0 && moved) {
+          if (!product_done(j)) { ok = false; break; }
+          tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < (F32 ? 2 : 1) * DP / 32; ++c) {  // (the lower parts' results follow the upper's)
-          float o[32];
-          tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);
+          for (int c = 0; c < (F32 ? 2 : 1) * DP / 32; ++c) {  // (the lower parts' results follow the upper's)
+            float o[32];
+            tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] *= corr;
-          tmem_st32(tmem_o(x) + lane_bits + c * 32, o);
+            for (int i = 0; i < 32; ++i) o[i] *= corr;
+            tmem_st32(tmem_o(x) + lane_bits + c * 32, o);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&p_full[2 * x + (j & 1)]);
+          if (j == 0 && x == 0) mbar_arrive(ahead);
         }
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&p_full[2 * x + (j & 1)]);
-        if (j == 0 && x == 0) mbar_arrive(ahead);
-      }
-    }
+      return n_tiles;
+    };
+    const int rest = F32 || __any_sync(0xffffffffu, row_down != 1.f) ? 0 : walk(std::false_type{}, 0);
+    if (rest < n_tiles) walk(std::true_type{}, rest);
     auto both = [&](int c, float (&o)[32]) {  // 32 dimensions of the results, in 32-bit mode the sum of both parts'
       tmem_ld32_done(tmem_o(x) + lane_bits + c * 32, o);
       if constexpr (F32) {
@@ -666,10 +667,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const uint32_t raw = q8_shared(raw_s);
     // (beyond the head's size anything will do: the queries are zeros there, and the results are not stored)
     const int piece = (half * 4 + quad) * 16 < p.d ? (half * 4 + quad) * 16 : 0;
-    asm volatile("bar.sync 1, %0;" ::"n"((SOFT_WARPS + CONV_WARPS) * 32) : "memory");
-    float up, down;
-    q8_query_scale(*q_top, up, down);
-    const float key_factor = (F32 ? 1.f : down) * (EXTRA == 2 ? p.scale : p.scale_log2e);
+    const float key_factor = (F32 ? 1.f : 1.f / Q_UNIT) * (EXTRA == 2 ? p.scale : p.scale_log2e);
     for (int j = 0; j < n_tiles; ++j) {
       const int ks_at = j % K_STAGES, st = j % V_STAGES, from = j % RAW;
       if (!warp_wait(&raw_full[from], (j / RAW) & 1, p.err, abort_flag)) break;

@@ -87,3 +87,18 @@ def test_scores_with_steps_of_one_and_more(through_tcgen05, power, sign, count, 
         got, near = _call(c, scale=math.log(2)), 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -19
         assert int(c.err) == 0
         assert (got >= codes[largest].min() / 8 * (1 - near)).all() and (got <= codes[largest].max() / 8 * (1 + near)).all()
+
+
+@DTYPES
+@pytest.mark.parametrize("counts", [[40, 1], [3, 1]])
+@pytest.mark.parametrize("power", [8, 16, 24, 30, 40, 60])
+def test_rows_beside_much_larger_queries(through_tcgen05, power, counts, dtype):
+    """Other tokens' and other heads' queries are 2^power larger, or as much smaller."""
+    c = Case(8, 2, 64, 16, counts, [200, 100], dtype, seed=power)
+    q = c.q.view(-1, 8, 64)
+    q[1, 1] *= 2.0 ** power
+    q[-1, 6] *= 2.0 ** power
+    q[2, :4] *= 2.0 ** -power
+    q[0] *= 2.0 ** power
+    _check(c)
+    _check(c, window=50, keep_first=3, sink=True)
