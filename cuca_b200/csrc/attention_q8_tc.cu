@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   if (first >= last) return;
   const bool alone = share >= keys.groups || p.n_splits == 1;
   const int n_tiles = last - first;
+  const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;  // no row sees positions from p.keep to here
   const int tile_tok = ROWS / G;             // tokens of a query tile
   const int nq = !F32 && n_tok > tile_tok ? 2 : 1;
   const uint32_t per_head = (65536u + G - 1) / G;  // a row of a query tile over G: right for up to 128 of both
@@ -223,10 +224,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
   // ------------------------------------------------ copies, RAW tiles ahead
   auto load_codes = [&](int lw) {
     const int* table = p.tables + (size_t)seq * p.table_stride;
-    const int lo = p.window > 0 ? max(0, pos0 - (p.window - 1)) : 0;
     if (runs) {
       // A warp for the keys, one for the values (one for both was busy for 1,770 clocks a tile), a lane a page: codes and scales.
-      // Positions from keys.hi on come along where their page does; what converts them takes their scales for 0. (A page behind a
+      // Positions that no row sees come along where their page does; what converts them takes their scales for 0. (A page behind a
       // window may have gone back, another that is not there is an error: page 0 comes instead; its keys are masked, or the step
       // is lost.)
       const int8_t* pool = lw == 0 ? p.kpool : p.vpool;
@@ -675,7 +675,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       float ks[2], vs[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const bool seen = keys.at(first + j) * KEYS + lane + 32 * h < keys.hi;  // (by some row)
+        // (by some row: neither the exponent of the tile nor its bits depend on another, nor on what came for a page that is gone)
+        const int kp = keys.at(first + j) * KEYS + lane + 32 * h;
+        const bool seen = kp < keys.hi && (kp >= lo || kp < p.keep);
         ks[h] = seen ? shared_f(scales + (lane + 32 * h) * 4) : 0.f;
         vs[h] = seen ? shared_f(scales + (KEYS + lane + 32 * h) * 4) : 0.f;
       }

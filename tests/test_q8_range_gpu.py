@@ -102,3 +102,26 @@ def test_rows_beside_much_larger_queries(through_tcgen05, power, counts, dtype):
     q[0] *= 2.0 ** power
     _check(c)
     _check(c, window=50, keep_first=3, sink=True)
+
+
+# ------------------------------------------------------------------ masks and tables
+@DTYPES
+@pytest.mark.parametrize("keep", [0, 20])
+@pytest.mark.parametrize("page", [4, 16, 24])
+def test_pages_behind_a_window_may_be_gone(through_tcgen05, page, keep, dtype):
+    """Without them, and whatever the pool's first page holds, the same bits."""
+    c = Case(8, 2, 64, page, [50, 1, 2], [400, 300, 155], dtype, seed=page)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        x = getattr(c, name)
+        first = torch.randint(-127, 128, x[:1].shape, device=c.device, generator=c.g).to(x.dtype) if x.dtype == torch.int8 else \
+            torch.full_like(x[:1], 3.0)
+        setattr(c, name, torch.cat([first, x]))
+    c.tables = torch.where(c.tables >= 0, c.tables + 1, -1)
+    whole = _check(c, window=100, keep_first=keep)
+    for slot, start in zip(c.slots, c.starts):
+        behind = [p for p in range((start - 99) // page) if p * page >= keep]
+        assert behind
+        c.tables[slot, behind] = -1
+    for scale in (3.0, 1e9, 0.0):
+        c.k_scale[0], c.v_scale[0] = scale, scale
+        assert torch.equal(whole, _call(c, window=100, keep_first=keep)) and int(c.err) == 0
