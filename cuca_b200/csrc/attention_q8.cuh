@@ -248,8 +248,8 @@ __device__ __forceinline__ float2 q8_capped_pair(float2 s, const Q8Params& p) {
   return __ffma2_rn(make_float2(r, r), make_float2(b, a), make_float2(top, top));
 }
 // What a sink adds to a denominator that is relative to the reference m.
-__device__ __forceinline__ float q8_sink_term(const Q8Params& p, int head, float m) {
-  return q8_exp2((p.sink_val ? p.sink_val[head] * CUCA_LOG2E : 0.f) - m + Q8_LIFT);
+__device__ __forceinline__ float q8_sink_term(const Q8Params& p, int head, float m, float lift = Q8_LIFT) {
+  return q8_exp2((p.sink_val ? p.sink_val[head] * CUCA_LOG2E : 0.f) - m + lift);
 }
 
 // What both entry points check, and the kernels' parameters.

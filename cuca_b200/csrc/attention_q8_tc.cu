@@ -15,7 +15,7 @@
 // A value scale goes into the operand tile here: V = code vs 2^(7 - E) with E the largest exponent of the tile's scales, rounded
 // to 11 bits, factor and product, so that z = s + E for every key of the tile and one multiplication a tile brings the sum of
 // the weights to the denominator's unit. Per-key factors in the softmax would each cost 16 loads of 512 bytes a warp and tile:
-// one, the keys' scales, is left of four. Where a tile's scales are more than 2^20 apart the exponents stay with the keys
+// one, the keys' scales, is left of four. Where a tile's scales are more than 2^4 apart the exponents stay with the keys
 // (`wide`). The keys' scales multiply the scores, so codes of keys are exact.
 //
 // Measured, 32 heads of 128 over 8: a prompt of 2,048 58 us (590 TFLOP/s), a portion of 512 on 8,192 106 us (668 TFLOP/s; over
@@ -46,7 +46,13 @@ constexpr int SOFT_REGS = 176, CONV_REGS = 88, ISSUE_REGS = 64;
 constexpr int K_STAGES = 3, V_STAGES = 3;
 constexpr int RAW = 3;  // tiles of codes on their way
 constexpr float V_LIFT = 7.f;     // values are 2^7 larger in the operand tile: 127 2^7 2 is the most that fits
-constexpr int WIDE = 20;
+// A tile's keys take weights relative to the tile's exponent E where their value scales are within 2^WIDE: the reference may be as
+// much above a key's own, so a key's weight is good to 2^(WIDE - LIFT - 24) = 2^-28 of the largest weight times value, and what a
+// hundred thousand keys lose is under a rounding of the result. (Within 2^20 four thousand keys of 2^-14 of the largest weight lost
+// a seventh of theirs beside a key of none with a value 2^18 larger.) Weights are at most 2^(LIFT + LAG). A LAG of 5 and a LIFT of 10
+// cost 1 %, 3 and 12 14 %. In 32-bit mode a value scale's fraction goes into the weight, and E is 0.
+constexpr int WIDE = 4;
+template <bool F32> constexpr float LIFT = F32 ? Q8_LIFT : 8.f;
 // bfloat16 queries whose row's largest magnitude is 2^-6 to 2^9, as good as all, go in times 2^6, whatever rows are beside them: what
 // 16-bit floats have no steps for is 2^-25 of that magnitude and less. Another row has a power of two of its own, and its warp
 // walks the keys in a way of its own, which multiplies by the inverse (a portion of 512 on 8,192 136 us if all do, 107 if none).
@@ -463,7 +469,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
           } else {
             tmem_ld64(tmem_s(x, j) + lane_bits, raw);
           }
-          const float ref = m == -INFINITY ? 0.f : m - Q8_LIFT;  // the exponents are z - ref
+          const float ref = m == -INFINITY ? 0.f : m - LIFT<F32>;  // the exponents are z - ref
           const float2 neg2 = make_float2(tile_e.x - ref, tile_e.x - ref);
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           sum2[0] = sum2[1] = make_float2(0.f, 0.f);
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     if (ok && product_done(n_tiles)) {
       tc_fence_after();
       if (alone) {
-        if (p.sink && m != -INFINITY) l += q8_sink_term(p, head, m);
+        if (p.sink && m != -INFINITY) l += q8_sink_term(p, head, m, LIFT<F32>);
         const float inv = bad ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : q8_pow2(-V_LIFT) / l;
         if constexpr (F32) {
           const bool mine = r < tile_tok * G && tok < n_tok;
@@ -848,7 +854,7 @@ __global__ void __launch_bounds__(ROWS) join_q8_tc_kernel(const Q8Params p) {
     o[0] += f * lo.x; o[1] += f * lo.y; o[2] += f * lo.z; o[3] += f * lo.w;
     o[4] += f * hi.x; o[5] += f * hi.y; o[6] += f * hi.z; o[7] += f * hi.w;
   }
-  if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top) * q8_pow2(V_LIFT);  // (sums come lifted as results do)
+  if (p.sink && top != -INFINITY) den += q8_sink_term(p, head, top, LIFT<F32>) * q8_pow2(V_LIFT);  // (sums come lifted as results do)
   const float inv = den == 0.f ? 0.f : 1.f / den;
   const size_t to = (size_t)(row0 + tok) * p.out_stride + (size_t)head * p.d + c8 * 8;
   if constexpr (F32) {

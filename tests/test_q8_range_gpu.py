@@ -104,6 +104,19 @@ def test_rows_beside_much_larger_queries(through_tcgen05, power, counts, dtype):
     _check(c, window=50, keep_first=3, sink=True)
 
 
+@DTYPES
+@pytest.mark.parametrize("power", [3, 5, 8, 12, 16, 18, 20, 21, 30])
+@pytest.mark.parametrize("where", [1, 100, 3000])
+def test_a_large_value_without_weight_leaves_a_flat_tail_its_weight(through_tcgen05, where, power, dtype):
+    """One key of weight 2^-14.5 of the first for each of four thousand: together they weigh six times what the first does.
+    A key of no weight has a value scale 2^power above the others."""
+    n = 4140
+    scores, scales = np.full(n, -14.5), np.full(n, 2.0 ** -6)
+    scores[0], scores[where], scales[where] = 0.0, -60.0, 2.0 ** (power - 6)
+    got = _check(_one_axis([40], [n - 40], dtype, range(n), scores, np.full(n, 64), scales), scale=math.log(2))
+    assert (got.float() - 1).abs().max() < 2.0 ** -7
+
+
 # ------------------------------------------------------------------ masks and tables
 @DTYPES
 @pytest.mark.parametrize("keep", [0, 20])
