@@ -13,7 +13,7 @@
 // sixth of the block's instructions.
 //
 // A value scale goes into the operand tile here: V = code vs 2^(7 - E) with E the largest exponent of the tile's scales, rounded
-// to 11 bits, factor and product, so that z = s + E for every key of the tile and one multiplication a tile brings the sum of
+// to 11 bits, so that z = s + E for every key of the tile and one multiplication a tile brings the sum of
 // the weights to the denominator's unit. Per-key factors in the softmax would each cost 16 loads of 512 bytes a warp and tile:
 // one, the keys' scales, is left of four. Where a tile's scales are more than 2^4 apart the exponents stay with the keys
 // (`wide`). The keys' scales multiply the scores, so codes of keys are exact.
@@ -61,9 +61,9 @@ constexpr float Q_UNIT = 64.f;
 constexpr float FAR = 1048576.f;
 constexpr int TMEM_COLS = 512;  // two score buffers per query tile (4 x 64 columns), results of both (2 x DP)
 
-__device__ __forceinline__ uint32_t q8_times(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t q8_times(uint32_t a, uint32_t hi, uint32_t lo) {  // a (hi + lo), rounded once but for a lo
   uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("{\n.reg .b32 t;\nmul.rn.f16x2 t, %1, %3;\nfma.rn.f16x2 %0, %1, %2, t;\n}" : "=r"(r) : "r"(a), "r"(hi), "r"(lo));
   return r;
 }
 
@@ -707,11 +707,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       hi = F32 ? 0 : __reduce_max_sync(0xffffffffu, hi);
       least = __reduce_min_sync(0xffffffffu, least);
       const bool wide = F32 || hi - least > WIDE;
-      uint32_t factor2[2];  // what a key's value codes are multiplied by, twice
+      // What a key's value codes are multiplied by, twice, and what its rounding left: so a value in the operand tile is rounded once.
+      uint32_t factor2[2], left2[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float x = F32 ? q8_pow2(V_LIFT) : fine[h] ? vs[h] * q8_pow2(V_LIFT - (wide ? e[h] : (float)hi)) : 0.f;
         factor2[h] = q8_pack(x, x);
+        const float left = x - __half22float2(*reinterpret_cast<const __half2*>(&factor2[h])).x;
+        left2[h] = q8_pack(left, left);
       }
       if (j >= V_STAGES && !warp_wait(&v_empty[st], ((j / V_STAGES) & 1) ^ 1, p.err, abort_flag)) break;
       if (j >= K_STAGES && !warp_wait(&k_empty[ks_at], ((j / K_STAGES) & 1) ^ 1, p.err, abort_flag)) break;
@@ -746,10 +749,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const uint32_t times = __shfl_sync(0xffffffffu, r0 + i * STEP < 32 ? factor2[0] : factor2[1], (r0 + i * STEP) & 31);
+        const uint32_t left = F32 ? 0u : __shfl_sync(0xffffffffu, r0 + i * STEP < 32 ? left2[0] : left2[1], (r0 + i * STEP) & 31);
         const uint32_t w[4] = {v[i].x ^ 0x80808080u, v[i].y ^ 0x80808080u, v[i].z ^ 0x80808080u, v[i].w ^ 0x80808080u};
         uint32_t h[8];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) { h[2 * n] = q8_times(q8_pair_lo(w[n]), times); h[2 * n + 1] = q8_times(q8_pair_hi(w[n]), times); }
+        for (int n = 0; n < 4; ++n) { h[2 * n] = q8_times(q8_pair_lo(w[n]), times, left); h[2 * n + 1] = q8_times(q8_pair_hi(w[n]), times, left); }
         *reinterpret_cast<uint4*>(vt + place0 + i * STEP * 128) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(vt + place1 + i * STEP * 128) = make_uint4(h[4], h[5], h[6], h[7]);
       }

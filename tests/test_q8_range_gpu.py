@@ -117,6 +117,30 @@ def test_a_large_value_without_weight_leaves_a_flat_tail_its_weight(through_tcge
     assert (got.float() - 1).abs().max() < 2.0 ** -7
 
 
+def _rounded_twice(up):
+    """(scale, code) whose product, the scale rounded to 11 bits and then the product, is furthest up or down in units of 2^-11."""
+    best = None
+    for a, code in itertools.product(range(64), range(64, 80)):
+        x = 1 + (a + (0.51 if up else 0.49)) * 2.0 ** -10
+        off = (float(np.float16(code * float(np.float16(x)))) / (code * x) - 1) * 2048
+        if best is None or (off > best[0] if up else off < best[0]):
+            best = off, x, code
+    return best
+
+
+@DTYPES
+def test_results_that_rest_on_two_keys_of_opposite_sign(through_tcgen05, dtype):
+    """Weights and values that lie between two 16-bit floats, so that what is rounded away of the one is not made up by the other."""
+    (far, x, cx), (near, y, cy) = _rounded_twice(True), _rounded_twice(False)
+    assert far > 1.8 and near < -1.8
+    n = 140
+    scores, scales, codes = np.full(n, -200.0), np.full(n, 2.0 ** -3), np.full(n, 64)
+    scores[:3] = 0.0, np.log2(1 + 1.02 * 2.0 ** -11) - 1, np.log2(1 + 0.98 * 2.0 ** -11) - 1
+    scales[:3], codes[:3] = (0.0, x, y), (0, cx, -cy)
+    c = _one_axis([40], [n - 40], dtype, range(n), scores, codes, scales)
+    _check(c, scale=math.log(2))
+
+
 # ------------------------------------------------------------------ masks and tables
 @DTYPES
 @pytest.mark.parametrize("keep", [0, 20])
