@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       const int run = min(p.bs, KEYS), n = KEYS / run;
       auto look = [&](int j) {
         const int kp = min(keys.at(first + min(j, n_tiles - 1)) * KEYS + lane * run, keys.hi - 1);
-        return __ldg(table + min(kp >> p.run_shift, p.table_stride - 1));
+        return (kp >> p.run_shift) < p.table_stride ? __ldg(table + (kp >> p.run_shift)) : -1;
       };
       int page[2] = {look(0), look(1)};  // (two tiles ahead: the next use does not wait for them)
       for (int j = 0; j < n_tiles; ++j) {
@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
     const int c = lane % CHUNKS, key = lw * 32 + lane;
     auto look = [&](int j) {  // the page of the lane's key: a tile before it is needed
       const int kp = min(keys.at(first + min(j, n_tiles - 1)) * KEYS + key, keys.hi - 1);
-      return __ldg(table + min(p.run_shift >= 0 ? kp >> p.run_shift : kp / p.bs, p.table_stride - 1));
+      const int entry = p.run_shift >= 0 ? kp >> p.run_shift : kp / p.bs;
+      return entry < p.table_stride ? __ldg(table + entry) : -1;
     };
     int page = look(0);
     for (int j = 0; j < n_tiles; ++j) {

@@ -162,3 +162,22 @@ def test_pages_behind_a_window_may_be_gone(through_tcgen05, page, keep, dtype):
     for scale in (3.0, 1e9, 0.0):
         c.k_scale[0], c.v_scale[0] = scale, scale
         assert torch.equal(whole, _call(c, window=100, keep_first=keep)) and int(c.err) == 0
+
+
+@DTYPES
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("counts", [[40], [1], [3, 1]])
+def test_positions_without_a_page_are_recorded(through_tcgen05, counts, page, dtype):
+    """In every form: entries that are no page, and tables that end before the positions do."""
+    c = Case(8, 2, 64, page, counts, [100] * len(counts), dtype, seed=1)
+    whole = c.tables.clone()
+    for entry, bad in itertools.product((0, 3), (-1, c.k.shape[0], 1 << 30)):
+        c.tables[c.slots[0], entry] = bad
+        _call(c)
+        assert int(c.err) == 2
+        c.err.zero_()
+        c.tables.copy_(whole)
+    _check(c)
+    c.tables = whole[:, :3].contiguous()
+    _call(c)
+    assert int(c.err) == 2
