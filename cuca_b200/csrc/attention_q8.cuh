@@ -279,7 +279,8 @@ inline int q8_params(const CucaQ8Attention& c, const char* name, int most_d, Q8P
   p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E;
   p.cap = opt->softcap; p.cap_arg = opt->softcap > 0.f ? 2.f * CUCA_LOG2E / opt->softcap : 0.f;
   p.sink = opt->sink ? 1 : 0; p.sink_val = opt->sink ? opt->sink_val : nullptr;
-  p.window = opt->window; p.keep = opt->window > 0 ? opt->keep : 0; p.slopes = opt->slopes;
+  p.window = opt->window; p.slopes = opt->slopes;
+  p.keep = opt->window > 0 ? (opt->keep < 1 << 30 ? opt->keep : 1 << 30) : 0;  // (so that it can be rounded up)
   p.heads_per_cta = (int)c.heads_per_cta; p.head_parts = (group + p.heads_per_cta - 1) / p.heads_per_cta;
   p.n_splits = (int)c.n_splits; p.chunk = c.n_splits > 1 ? (int)c.chunk : 0; p.part = c.part; p.err = c.err;
   return 0;

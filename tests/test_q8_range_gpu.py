@@ -181,3 +181,11 @@ def test_positions_without_a_page_are_recorded(through_tcgen05, counts, page, dt
     c.tables = whole[:, :3].contiguous()
     _call(c)
     assert int(c.err) == 2
+
+
+@DTYPES
+@pytest.mark.parametrize("counts", [[40], [1], [3, 1]])
+def test_first_keys_that_stay_without_end(through_tcgen05, counts, dtype):
+    """As many as a 32-bit number holds: every key is seen."""
+    c = Case(8, 2, 64, 16, counts, [300] * len(counts), dtype, seed=2)
+    assert torch.equal(_call(c, window=5, keep_first=2 ** 31 - 1), _check(c)) and int(c.err) == 0
