@@ -48,7 +48,7 @@ struct CucaQ8Attention {
   const int* req_row0;
   const int* req_count;  // null: every request brings one row
   int64_t n_seqs, count_lo, count_hi;  // requests with so many rows are this launch's
-  int64_t tile_tokens, n_tiles;        // rows of a request that a tile takes
+  int64_t tile_tokens, n_tiles, tile0;  // rows of a request that a tile takes; how many tiles from which on
   int64_t nh, nkv, d;
   const CucaAttnOptions* opt;
   int64_t heads_per_cta;  // query heads of a key head that a block takes
@@ -58,7 +58,7 @@ struct CucaQ8Attention {
   int* err;
   cudaStream_t stream;
 };
-static_assert(sizeof(CucaQ8Attention) == 33 * 8, "one 64-bit word each");
+static_assert(sizeof(CucaQ8Attention) == 34 * 8, "one 64-bit word each");
 
 namespace {
 
@@ -82,6 +82,8 @@ struct Q8Params {
   int n_seqs;
   int count_lo, count_hi;  // requests with so many rows are this launch's
   int tile_tokens;         // rows of a request that a tile takes
+  int tile0;               // the launch's first tile
+  int width;               // of a block: column tiles, or query tiles
   int nh, nkv, d;
   float scale_log2e;
   float cap;       // > 0: a score s becomes cap tanh(s / cap) ...
@@ -98,9 +100,10 @@ struct Q8Params {
   int* err;
 };
 
-// Which rows tile number `tile` of a launch takes: those of the requests that are the launch's, tile_tokens at a time, a
+// Which rows tile number `tile` of a launch takes (counted from tile0 on): those of the requests that are the launch's, tile_tokens at a time, a
 // request's last ones (which see most keys) first. By every warp for itself.
 __device__ __forceinline__ bool q8_rows_of_tile(const Q8Params& p, int tile, int& row0, int& n) {
+  tile += p.tile0;
   if (p.req_count == nullptr) {
     row0 = p.req_row0[tile];
     n = 1;
@@ -264,7 +267,8 @@ inline int q8_params(const CucaQ8Attention& c, const char* name, int most_d, Q8P
                "%s: empty or endless pages or tables", name);
   CUCA_REQUIRE((((uintptr_t)c.kpool | (uintptr_t)c.vpool) & 15) == 0, "%s: pools must be 16-byte aligned", name);
   CUCA_REQUIRE(c.q_stride < (1ll << 31) && c.out_stride < (1ll << 31), "%s: rows too far apart", name);
-  CUCA_REQUIRE(c.n_tiles > 0 && c.n_tiles <= 65535, "%s: %lld tiles", name, (long long)c.n_tiles);
+  CUCA_REQUIRE(c.n_tiles > 0 && c.n_tiles <= 65535 && c.tile0 >= 0 && c.tile0 < (1ll << 30), "%s: %lld tiles from %lld on", name,
+               (long long)c.n_tiles, (long long)c.tile0);
   CUCA_REQUIRE(c.chunk >= 0 && c.chunk % 64 == 0 && c.n_splits >= 1 && c.n_splits <= 64 &&
                (c.n_splits == 1 || c.chunk > 0) && ((uintptr_t)c.part & 15) == 0, "%s: bad shares of the keys", name);
   const int group = (int)(c.nh / c.nkv);
@@ -275,6 +279,7 @@ inline int q8_params(const CucaQ8Attention& c, const char* name, int most_d, Q8P
   p.tables = c.tables; p.table_stride = (int)c.table_stride; p.positions = c.positions; p.seq_of_row = c.seq_of_row;
   p.req_row0 = c.req_row0; p.req_count = c.req_count; p.n_seqs = (int)c.n_seqs;
   p.count_lo = (int)c.count_lo; p.count_hi = (int)c.count_hi; p.tile_tokens = (int)c.tile_tokens;
+  p.tile0 = (int)c.tile0; p.width = (int)c.width;
   p.nh = (int)c.nh; p.nkv = (int)c.nkv; p.d = (int)c.d;
   p.scale = opt->scale; p.scale_log2e = opt->scale * CUCA_LOG2E;
   p.cap = opt->softcap; p.cap_arg = opt->softcap > 0.f ? 2.f * CUCA_LOG2E / opt->softcap : 0.f;

@@ -640,8 +640,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         else store(std::false_type{});
         }
       } else {
-        // [NQ][DP / 4][ROWS][4], then m and l [NQ][2][ROWS]: rows side by side
-        float* part = p.part + (((size_t)blockIdx.y * p.nkv + kvh) * p.n_splits + split) * (size_t)(NQ * ROWS * (DP + 2));
+        // [width][DP / 4][ROWS][4], then m and l [width][2][ROWS]: rows side by side
+        float* part = p.part + (((size_t)blockIdx.y * p.nkv + kvh) * p.n_splits + split) * (size_t)(p.width * ROWS * (DP + 2));
         float4* dst = reinterpret_cast<float4*>(part) + (size_t)x * (DP / 4) * ROWS + r;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
 #pragma unroll
           for (int q = 0; q < 8; ++q) dst[(c * 8 + q) * ROWS] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
         }
-        float* ml = part + NQ * ROWS * DP + x * 2 * ROWS;
+        float* ml = part + p.width * ROWS * DP + x * 2 * ROWS;
         ml[r] = m;
         ml[ROWS + r] = bad ? __uint_as_float(0x7fc00000u) : l * q8_pow2(V_LIFT);
       }
@@ -842,12 +842,12 @@ __global__ void __launch_bounds__(ROWS) join_q8_tc_kernel(const Q8Params p) {
   const Q8Keys keys = q8_keys<KEYS>(p, pos0, n_tok);
   const int share = p.chunk / KEYS, used = min(p.n_splits, (keys.groups + share - 1) / share);
   if (used <= 1) return;  // written already
-  const int x = blockIdx.x % NQ, c8 = blockIdx.x / NQ, r = threadIdx.x;
+  const int x = blockIdx.x % p.width, c8 = blockIdx.x / p.width, r = threadIdx.x;
   const int tile_tok = ROWS / G, tok = x * tile_tok + r / G, head = kvh * G + r % G;
   if (r >= tile_tok * G || tok >= n_tok || c8 * 8 >= p.d) return;
-  const size_t step = (size_t)NQ * ROWS * (DP + 2);
+  const size_t step = (size_t)p.width * ROWS * (DP + 2);
   const float* part = p.part + ((size_t)blockIdx.z * p.nkv + kvh) * p.n_splits * step;
-  const float* ml = part + NQ * ROWS * DP + x * 2 * ROWS + r;
+  const float* ml = part + p.width * ROWS * DP + x * 2 * ROWS + r;
   float top = -INFINITY;
   for (int s = 0; s < used; ++s) top = fmaxf(top, ml[s * step]);
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, den = 0.f;
@@ -897,7 +897,7 @@ int launch_q8_tc(const Q8Params& p, int n_tiles, cudaStream_t stream) {
   cuca_launch(kernel, dim3(p.nkv * p.n_splits, n_tiles), dim3(NTHREADS), smem, stream, true, p);
   CUCA_CHECK_LAUNCH("attention_q8_tc");
   if (p.n_splits > 1) {
-    cuca_launch(join_q8_tc_kernel<DP, F32>, dim3(NQ * DP / 8, p.nkv, n_tiles), dim3(ROWS), 0, stream, true, p);
+    cuca_launch(join_q8_tc_kernel<DP, F32>, dim3(p.width * DP / 8, p.nkv, n_tiles), dim3(ROWS), 0, stream, true, p);
     CUCA_CHECK_LAUNCH("attention_q8_tc (join)");
   }
   return 0;
@@ -912,7 +912,7 @@ int launch_q8_tc_extra(const Q8Params& p, bool f32, int n_tiles, cudaStream_t st
 }  // namespace
 
 // bfloat16 rows, or 32-bit rows (one query tile, neither cap nor bias), of head sizes up to 128, groups of at most 128 heads whole; `width` (1 or 2) query tiles to a block: tile_tokens is
-// that times the tokens whose rows fit 128. part: [n_tiles][nkv][n_splits][256 (d rounded up to 64 or 128) + 512] floats where
+// that times the tokens whose rows fit 128. part: [n_tiles][nkv][n_splits][width][128 (d rounded up to 64 or 128) + 256] floats where
 // n_splits > 1.
 CUCA_API int cuca_attention_q8_tc(const CucaQ8Attention* c) {
   if (c->n_tiles == 0) return 0;

@@ -1579,7 +1579,7 @@ class QuantizedPages:
 
 Q8_MAX_HEAD_DIM = 256
 # a call's arguments as 64-bit words (`CucaQ8Store` and `CucaQ8Read` in csrc/cache_q8.cu, `CucaQ8Attention` in csrc/attention_q8.cuh)
-_Q8_STORE, _Q8_READ, _Q8_ATTENTION = struct.Struct("29q"), struct.Struct("20q"), struct.Struct("33q")
+_Q8_STORE, _Q8_READ, _Q8_ATTENTION = struct.Struct("29q"), struct.Struct("20q"), struct.Struct("34q")
 
 
 def _at(t) -> int:
@@ -1687,6 +1687,10 @@ Q8_FEW_ROWS = 24  # query rows of a key head that the form for few rows takes of
 # seven (up to 1.4 of it), those with fewer 0.9 to 1.6 but for five.
 Q8_SUMS_F32, Q8_LEAST_F32 = 512, 700_000
 Q8_SINGLES_ALONG = 0.25  # single tokens for each portion of a step that go with the portions through tcgen05
+# Bytes of shares' results that one launch may leave for its join: a launch that would leave more goes in parts, one after the other
+# through the same memory. (Shares of a long 32-bit prompt grow with tokens times context: 8,192 tokens of 32 heads of 128 over 8
+# would leave 2.2 GB. A part of this size is some 4,000 blocks.)
+Q8_SCRATCH = 256 << 20
 
 
 class QuantizedPlan:
@@ -1838,6 +1842,13 @@ def _q8_resident(sms: int, head_dim: int, nt: int) -> int:
     return sms * max(1, 4 * 128 // (max(64, head_dim) * nt))
 
 
+def _q8_part(form, n_kv_heads, group, heads, head_dim, code, width, shares) -> int:
+    """Floats that the shares of one tile of rows leave for their join, over all key heads."""
+    if form == 1:
+        return n_kv_heads * shares * width * 128 * ((64 if head_dim <= 64 else 128) + 2)
+    return n_kv_heads * -(-group // heads) * shares * (8 * width // (2 if code == F32 else 1)) * (head_dim + 2)
+
+
 def attention_q8_plan(step) -> QuantizedPlan:
     plan = step.plans.get("paged_attention_q8")
     if plan is None:
@@ -1868,13 +1879,13 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
     shape = n_heads, n_kv_heads, head_dim, ctypes.addressof(opt)
     group = n_heads // n_kv_heads
     for form, lo, hi, tokens, tiles, heads, width, share, shares, through_memory in launches:
-        part, at = None, 0
+        at, once = 0, 65535  # tiles of a launch
         if through_memory:  # the shares' results, joined by a second launch
-            cols = 8 * width // (2 if code == F32 else 1)
-            part = torch.empty(tiles * n_kv_heads * shares * (256 * (64 if head_dim <= 64 else 128) + 512) if form == 1 else
-                               tiles * n_kv_heads * -(-group // heads) * shares * cols * (head_dim + 2), dtype=torch.float32,
-                               device=q.device)
+            floats = _q8_part(form, n_kv_heads, group, heads, head_dim, code, width, shares)  # of a tile
+            once = max(1, min(once, tiles, Q8_SCRATCH // (4 * floats)))
+            part = torch.empty(once * floats, dtype=torch.float32, device=q.device)
             at = part.data_ptr()
         entry = lib.cuca_attention_q8_tc if form == 1 else lib.cuca_attention_q8
-        library.check(entry(_Q8_ATTENTION.pack(*rows, lo, hi, tokens, tiles, *shape, heads, width, share, shares, at, e, stream)),
-                      "attention_q8")
+        for tile0 in range(0, tiles, once):
+            library.check(entry(_Q8_ATTENTION.pack(*rows, lo, hi, tokens, min(once, tiles - tile0), tile0, *shape, heads, width, share,
+                                                   shares, at, e, stream)), "attention_q8")

@@ -189,3 +189,32 @@ def test_first_keys_that_stay_without_end(through_tcgen05, counts, dtype):
     """As many as a 32-bit number holds: every key is seen."""
     c = Case(8, 2, 64, 16, counts, [300] * len(counts), dtype, seed=2)
     assert torch.equal(_call(c, window=5, keep_first=2 ** 31 - 1), _check(c)) and int(c.err) == 0
+
+
+# ------------------------------------------------------------------ memory
+@pytest.mark.parametrize("counts,starts,dtype", [([8192], [0], torch.float32), ([512, 64], [30000, 100], torch.float32),
+                                                 ([1] * 256, [60000] + [50] * 255, torch.bfloat16)])
+def test_what_a_call_needs_of_memory_is_bounded(counts, starts, dtype):
+    c = Case(32, 8, 128, 64, counts, starts, dtype, seed=1, fill=False)
+    c.k_scale.fill_(0.01), c.v_scale.fill_(0.01)
+    out = torch.empty_like(c.q)
+    from cuca_b200.kernels import ops
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.attention_q8(c.q, out, c.pages(), c.tables, c.step, 32, 8, 128, 0.01, None, c.err)
+    torch.cuda.synchronize()
+    assert int(c.err) == 0 and out.isfinite().all()
+    assert torch.cuda.max_memory_allocated() - before <= 300 * 2 ** 20
+
+
+@DTYPES
+@pytest.mark.parametrize("counts,starts", [([300, 40], [2000, 1500]), ([1, 1, 1], [4000, 3, 2500]), ([5, 2], [3000, 2000])])
+def test_launches_in_parts_give_the_same_bits(monkeypatch, counts, starts, dtype):
+    from cuca_b200.kernels import ops
+    monkeypatch.setattr(ops, "CLUSTER_MERGE", False)
+    c = Case(8, 2, 128, 16, counts, starts, dtype, seed=4)
+    want = _check(c, sink=True)
+    for limit in (0, 1 << 21):
+        monkeypatch.setattr(ops, "Q8_SCRATCH", limit)
+        assert torch.equal(want, _call(c, sink=True))
