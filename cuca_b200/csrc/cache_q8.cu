@@ -155,9 +155,9 @@ __global__ void __launch_bounds__(STORE_THREADS) rope_store_q8_kernel(const Stor
   pdl_trigger();
   pdl_wait();
   const int heads = p.nh + 2 * p.nkv;
-  const int head = (int)((blockIdx.x * STORE_THREADS + threadIdx.x) >> p.seg_shift);
+  const int head = (int)((blockIdx.y * STORE_THREADS + threadIdx.x) >> p.seg_shift);  // gridDim: rows, heads
   const int l = threadIdx.x & ((1 << p.seg_shift) - 1);
-  const int half = p.d / 2, row = blockIdx.y;
+  const int half = p.d / 2, row = blockIdx.x;
   const bool lane_ok = head < heads && 4 * l < half;
   const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
   const bool rotate = !is_v && p.rot > 0;
@@ -484,10 +484,10 @@ CUCA_API int cuca_rope_store_q8(const CucaQ8Store* c) {
   const bool vec = slices && whole && row_stride % 4 == 0 && q_stride % 4 == 0 && (((uintptr_t)qkv | tables) & 15) == 0 &&
                    c->slice_stride % 4 == 0 && ((uintptr_t)q_out & 7) == 0;
   const unsigned blocks = (unsigned)((((long long)heads << p.seg_shift) + STORE_THREADS - 1) / STORE_THREADS);
-  CUCA_REQUIRE(n_rows <= 65535, "rope_store_q8: too many rows");
+  CUCA_REQUIRE(blocks <= 65535, "rope_store_q8: too many heads");
   auto kernel = vec ? rope_store_q8_kernel<__nv_bfloat16, true, true> : slices ? rope_store_q8_kernel<__nv_bfloat16, false, true>
       : dtype == CUCA_F32 ? rope_store_q8_kernel<float, false, false> : rope_store_q8_kernel<__nv_bfloat16, false, false>;
-  cuca_launch(kernel, dim3(blocks, n_rows), dim3(STORE_THREADS), 0, stream, true, p);
+  cuca_launch(kernel, dim3(n_rows, blocks), dim3(STORE_THREADS), 0, stream, true, p);
   CUCA_CHECK_LAUNCH("rope_store_q8");
   return 0;
 }

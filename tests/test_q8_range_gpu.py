@@ -218,3 +218,33 @@ def test_launches_in_parts_give_the_same_bits(monkeypatch, counts, starts, dtype
     for limit in (0, 1 << 21):
         monkeypatch.setattr(ops, "Q8_SCRATCH", limit)
         assert torch.equal(want, _call(c, sink=True))
+
+
+# ------------------------------------------------------------------ many rows
+@DTYPES
+@pytest.mark.parametrize("adjacent,rot,slices", [(True, 16, 0), (False, 8, 0), (False, 16, 2), (True, 16, 2)])
+def test_more_rows_than_a_grid_has_along_its_second_axis(adjacent, rot, slices, dtype):
+    """As in two calls of fewer rows."""
+    from cuca_b200.kernels import ops
+    if slices and dtype == torch.float32:
+        pytest.skip("K slices give bfloat16 queries")
+    n, cut = 70_000, 40_000
+    c = Case(2, 1, 16, 64, [n], [0], dtype, seed=1, fill=False)
+    angle = torch.arange(n, device=c.device, dtype=torch.float64)[:, None] * 0.1 ** torch.arange(rot // 2, device=c.device)
+    cos, sin = angle.cos().float(), angle.sin().float()
+    x = torch.randn(max(slices, 1), n, 64, device=c.device, generator=c.g)
+
+    def write(lo, hi, q):
+        rows = ops.PartialSums(x[:, lo:hi], slices) if slices else x[0, lo:hi].to(dtype)
+        ops.rope_store_q8(rows, q[lo:hi], c.step.positions[lo:hi], c.step.seq_of_row[lo:hi], c.tables, cos, sin, rot, c.pages(), 2, 1,
+                          16, c.err, adjacent=adjacent)
+        assert int(c.err) == 0
+    results = []
+    for parts in ([(0, n)], [(0, cut), (cut, n)]):
+        for t in (c.k, c.v, c.k_scale, c.v_scale):
+            t.zero_()
+        q = torch.zeros(n, 32, dtype=dtype, device=c.device)
+        for lo, hi in parts:
+            write(lo, hi, q)
+        results.append([t.clone() for t in (q, c.k, c.v, c.k_scale, c.v_scale)])
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and (results[0][3][c.tables[c.slots[0], :n // 64].long()] > 0).all()
