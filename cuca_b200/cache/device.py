@@ -160,8 +160,9 @@ class DeviceCache:
 
     def read(self, cache_id: int, slot: int, positions: int, dtype=None):
         """(keys, values), [positions, kv heads, head size] each: what a cache kept in 8 bits holds for the first positions of
-        the request in this slot, in the compute dtype unless told otherwise. Positions whose pages have gone back (behind a
-        window) are refused by the error word, as in a step."""
+        the request in this slot, which is alive (a slot goes to another request when its own ends), in the compute dtype unless
+        told otherwise. Waits for the GPU; positions without a page, never written or gone back from behind a window, are an
+        `IndexError`, and the steps' error word knows nothing of it."""
         if not self.quantized:
             raise ValueError("only a cache that is kept in 8 bits is read back")
         pages, tables = self.pages(cache_id), self.tables[self._where[cache_id][0]]
@@ -170,5 +171,8 @@ class DeviceCache:
         at = torch.arange(positions, dtype=torch.int32, device=self.rt.device)
         k = torch.empty(positions, pages.k.shape[1], pages.k.shape[3], dtype=dtype or self.rt.dtype, device=self.rt.device)
         v = torch.empty_like(k)
-        ops.read_q8(pages, at, torch.full_like(at, slot), tables, k, v, self.rt.err)
+        err = torch.zeros(1, dtype=torch.int32, device=self.rt.device)
+        ops.read_q8(pages, at, torch.full_like(at, slot), tables, k, v, err)
+        if int(err):
+            raise IndexError(f"slot {slot} has no page for some of its first {positions} positions")
         return k, v
