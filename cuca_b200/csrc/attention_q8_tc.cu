@@ -680,13 +680,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       if (!warp_wait(&raw_full[from], (j / RAW) & 1, p.err, abort_flag)) break;
       const uint32_t codes = raw + from * SH::RAW_STAGE, scales = codes + 2 * KEYS * DP;
       float ks[2], vs[2];
+      bool seen[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         // (by some row: neither the exponent of the tile nor its bits depend on another, nor on what came for a page that is gone)
         const int kp = keys.at(first + j) * KEYS + lane + 32 * h;
-        const bool seen = kp < keys.hi && (kp >= lo || kp < p.keep);
-        ks[h] = seen ? shared_f(scales + (lane + 32 * h) * 4) : 0.f;
-        vs[h] = seen ? shared_f(scales + (KEYS + lane + 32 * h) * 4) : 0.f;
+        seen[h] = kp < keys.hi && (kp >= lo || kp < p.keep);
+        ks[h] = seen[h] ? shared_f(scales + (lane + 32 * h) * 4) : 0.f;
+        vs[h] = seen[h] ? shared_f(scales + (KEYS + lane + 32 * h) * 4) : 0.f;
       }
       uint4 k[PER], v[PER];  // (all asked for before any is used)
 #pragma unroll
@@ -695,7 +696,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
         k[i] = shared_16(at);
         v[i] = shared_16(at + KEYS * DP);
       }
-      // the tile's exponent: the largest of its finite scales other than 0
+      // the tile's exponent: the largest of its finite scales other than 0; the least of those that some row sees
       float e[2], f, inv;
       bool fine[2];
       int hi = -60, least = 1000;
@@ -703,7 +704,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
       for (int h = 0; h < 2; ++h) {
         q8_value_scale(vs[h], e[h], f, inv);
         fine[h] = e[h] == e[h];
-        if (fine[h] && vs[h] != 0.f) { hi = max(hi, (int)e[h]); least = min(least, (int)e[h]); }
+        if (fine[h] && vs[h] != 0.f) hi = max(hi, (int)e[h]);
+        if (fine[h] && seen[h]) least = min(least, (int)e[h]);  // (a row of zeros by its -60: it must not raise the reference)
       }
       hi = F32 ? 0 : __reduce_max_sync(0xffffffffu, hi);
       least = __reduce_min_sync(0xffffffffu, least);

@@ -141,6 +141,16 @@ def test_results_that_rest_on_two_keys_of_opposite_sign(through_tcgen05, dtype):
     _check(c, scale=math.log(2))
 
 
+@DTYPES
+@pytest.mark.parametrize("depth", [10, 20, 30, 60])
+def test_what_is_left_beside_a_value_of_zeros(through_tcgen05, depth, dtype):
+    """The key that has nearly all the weight has a value of zeros: the result is what the others' 2^-depth make, to its own bits."""
+    n = 340
+    scores, scales = np.full(n, -float(depth)), np.full(n, 2.0 ** -6)
+    scores[5], scales[5] = 0.0, 0.0
+    _check(_one_axis([40], [n - 40], dtype, range(n), scores, np.arange(n) % 50 + 50, scales), scale=math.log(2))
+
+
 # ------------------------------------------------------------------ masks and tables
 @DTYPES
 @pytest.mark.parametrize("keep", [0, 20])
