@@ -363,7 +363,7 @@ attention_q8_kernel(const Q8Params p) {
       q8_value_scale(shared_f(at + 2 * R::TENSOR + GROUP * 4 + (g + 8 * r) * 4), ve[r], vf[r], vi[r]);
     }
     const bool whole = key0 + GROUP - 1 <= least_pos && (p.window <= 0 || key0 >= most_lo || key0 + GROUP <= p.keep);
-    float z[NT][LC][2];
+    float z[NT][LC][2], zs[NT][LC][2];  // (in 32-bit mode the scores without the values' exponents too)
     bool higher = false;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -378,7 +378,11 @@ attention_q8_kernel(const Q8Params p) {
             x = raw * f;
             if (p.cap > 0.f) x = q8_capped<PARTS == 2>(x, p);
             if (p.slopes) x -= p.slopes[col_head[j][c]] * CUCA_LOG2E * (float)(col_pos[j][c] - (key0 + g + 8 * r));
+            if (PARTS == 2) zs[j][c][r] = x;
             x += ve[r];
+          } else if (PARTS == 2) {
+            zs[j][c][r] = raw * f;
+            x = zs[j][c][r] + ve[r];
           } else {
             x = fmaf(raw, f, ve[r]);
           }
@@ -421,7 +425,9 @@ attention_q8_kernel(const Q8Params p) {
         float w[LC];
 #pragma unroll
         for (int c = 0; c < LC; ++c) {
-          w[c] = q8_exp2(z[j][c][r] - (m[j][c] == -INFINITY ? 0.f : m[j][c] - Q8_LIFT));
+          const float ref = m[j][c] == -INFINITY ? 0.f : m[j][c] - Q8_LIFT;
+          // In 32-bit mode an exponent meets the reference first: their difference is exact where values are large, and z is not.
+          w[c] = PARTS == 2 && z[j][c][r] != -INFINITY ? q8_exp2(zs[j][c][r] + (ve[r] - ref)) : q8_exp2(z[j][c][r] - ref);
           l[j][c] = fmaf(w[c], vi[r], l[j][c]);
           w[c] *= vf[r];
         }

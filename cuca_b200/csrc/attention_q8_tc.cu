@@ -490,12 +490,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Pa
                 } else if (EXTRA) {
                   x2 = __fmul2_rn(x2, f2);
                 }
+                // (the key's exponent meets the reference first: their difference is exact where they are large)
+                const float2 at2 = decltype(wide)::value ? __fadd2_rn(neg2, *reinterpret_cast<const float2*>(factor + KEYS + k)) : neg2;
                 if (EXTRA) {
                   if (EXTRA == 2) x2 = q8_capped_pair(x2, p);
                   x2 = __fadd2_rn(x2, make_float2(fmaf(slope2, (float)k, bias0), fmaf(slope2, (float)(k + 1), bias0)));
                 }
-                x2 = EXTRA || decltype(own)::value ? __fadd2_rn(x2, neg2) : __ffma2_rn(x2, f2, neg2);
-                if (decltype(wide)::value) x2 = __fadd2_rn(x2, *reinterpret_cast<const float2*>(factor + KEYS + k));
+                x2 = EXTRA || decltype(own)::value ? __fadd2_rn(x2, at2) : __ffma2_rn(x2, f2, at2);
                 if (decltype(masked)::value) {
                   const int kp = key0 + k;
                   if (!(kp <= row_pos && (kp >= row_lo || kp < p.keep))) x2.x = -INFINITY;

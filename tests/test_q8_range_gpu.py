@@ -151,6 +151,19 @@ def test_what_is_left_beside_a_value_of_zeros(through_tcgen05, depth, dtype):
     _check(_one_axis([40], [n - 40], dtype, range(n), scores, np.arange(n) % 50 + 50, scales), scale=math.log(2))
 
 
+@DTYPES
+@pytest.mark.parametrize("few", [10 ** 6, 0])
+def test_weights_of_values_of_any_size(monkeypatch, few, dtype):
+    """Rows that see five keys of about the same weight, whose values are up to 2^70 apart."""
+    from cuca_b200.kernels import ops
+    monkeypatch.setattr(ops, "Q8_FEW_ROWS", few)
+    monkeypatch.setattr(ops, "Q8_LEAST_F32", 0)
+    for seed in range(6):
+        c = Case(12, 12, 96, 32, [322], [12], dtype, seed=seed, level=1e-3)
+        c.v_scale *= 2.0 ** torch.randint(0, 71, c.v_scale.shape, device=c.device, generator=c.g).float()
+        _check(c, window=1, keep_first=4)
+
+
 # ------------------------------------------------------------------ masks and tables
 @DTYPES
 @pytest.mark.parametrize("keep", [0, 20])
