@@ -214,6 +214,25 @@ def test_first_keys_that_stay_without_end(through_tcgen05, counts, dtype):
     assert torch.equal(_call(c, window=5, keep_first=2 ** 31 - 1), _check(c)) and int(c.err) == 0
 
 
+@DTYPES
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (6, 1, 96)])
+def test_every_option_with_every_other(through_tcgen05, heads, kv, dim, dtype):
+    c = Case(heads, kv, dim, 16, [1, 37, 2], [150, 70, 0], dtype, seed=dim)
+    sinks = 3 * torch.randn(heads, device=c.device, generator=c.g)
+    slopes = 0.1 * torch.rand(heads, device=c.device, generator=c.g)
+    for window, keep, cap, sink, slope in itertools.product((None, 40), (0, 5), (0.0, 8.0), (None, True, sinks), (None, slopes)):
+        _check(c, window=window, keep_first=keep, softcap=cap, sink=sink is not None, sink_values=sink if sink is sinks else None,
+               slopes=slope)
+
+
+@DTYPES
+def test_a_request_alone_first_and_last(dtype):
+    """Within the bound of the formula whatever else the step brings."""
+    mine, others = (37, 100), [(1, 900), (150, 30), (5, 2000)]
+    for order in ([mine], [mine] + others, others + [mine], others[:1] + [mine] + others[1:]):
+        _check(Case(8, 2, 64, 16, [n for n, _ in order], [s for _, s in order], dtype, seed=3))
+
+
 # ------------------------------------------------------------------ memory
 @pytest.mark.parametrize("counts,starts,dtype", [([8192], [0], torch.float32), ([512, 64], [30000, 100], torch.float32),
                                                  ([1] * 256, [60000] + [50] * 255, torch.bfloat16)])
