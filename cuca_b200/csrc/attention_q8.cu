@@ -17,7 +17,7 @@
 // Decoding would be bound by the pages' bytes (16 keys of 128 are 4.2 KB, 183 clocks of an SM's share of memory) but for the
 // instructions that turn codes into 16-bit floats: some 320 a warp and group, 176 of them conversion. Measured, 32 heads of 128 over 8,
 // pages of 16: 64 requests of up to 8,192 positions 111 us (5.1 TB/s, 0.78 of a copy's rate; with nothing fetched 98), 8 of 1,152
-// 12.3 us (latency: three groups a warp), one of 77 4.7 us; over bfloat16 pages 190, 12.9 and 6.9 us.
+// 12.7 us (latency: three groups a warp), one of 77 4.7 us; over bfloat16 pages 190, 12.9 and 6.9 us.
 #include "attention_q8.cuh"
 #include <type_traits>
 

@@ -20,17 +20,18 @@
 
 namespace {
 
-// Weights are less than 2^(LIFT + LAG + 1): the running maximum follows a larger one only when it is exceeded by more than LAG
-// (rescaling is rare then), and LIFT puts the weights' 29 binades of full precision below 2^15. Of scores from some 2^20 on 32-bit
-// numbers have no steps that small: a score is rounded before the reference is taken off, as the maximum was, so that the largest
-// has its exponent to within a step, and a weight that a rounded reference makes too large for a 16-bit float becomes the largest
-// one. (Keys that close to the largest share the weight in no certain proportion then: their scores' own steps are larger.)
+// Weights are less than 2^(LIFT + LAG + 1), below 2^15: the running maximum follows a larger one only when it is exceeded by more than
+// LAG (rescaling is rare then), and LIFT leaves the largest weight 31 binades above a 16-bit float's least step. Of scores from
+// some 2^20 on 32-bit numbers have no steps that small: a score is rounded before the reference is taken off, as the maximum was,
+// so that the largest has its exponent to within a step, and a weight that a rounded reference makes too large for a 16-bit float
+// becomes the largest one. (Keys that close to the largest share the weight in no certain proportion then: their scores' own steps
+// are larger.)
 constexpr float Q8_LIFT = 7.f, Q8_LAG = 7.f;
 
 }  // namespace
 
-// A launch, as Python packs it: one 64-bit word each, in this order (kernels/ops.py:attention_q8; 33 arguments one by one cost
-// the caller 3.7 us, packed 0.9).
+// A launch, as Python packs it: one 64-bit word each, in this order (kernels/ops.py:attention_q8; so many arguments one by one cost
+// the caller 3.6 us, packed 1.1).
 struct CucaQ8Attention {
   const void* q;
   int64_t q_stride;  // values between rows
@@ -207,7 +208,8 @@ __device__ __forceinline__ float q8_pow2(float e) {  // 2^e, e a whole number of
   return __uint_as_float((uint32_t)((int)e + 127) << 23);
 }
 // A value scale as f 2^e (e as a float), and 2^-e for the denominator. e is -60 at least, so that u 2^-e does not leave 32 bits
-// where scales are far apart; f is smaller than 1 then, 0 for a row of zeros. A scale that is not finite (2^123 and more, which
+// where scales are far apart; f is smaller than 1 then, 0 for a row of zeros. (Such a row keeps its part of the denominator beside
+// values of up to some 2^80; in 32-bit mode to 20 bits or so, as its exponent in the softmax is that much larger.) A scale that is not finite (2^123 and more, which
 // no row has, count as that) makes e, so the weight, NaN where the key is seen; the factors are numbers, so that a masked key's
 // weight of zero stays zero.
 __device__ __forceinline__ void q8_value_scale(float vs, float& e, float& f, float& inv) {

@@ -13,12 +13,12 @@
 // sixth of the block's instructions.
 //
 // A value scale goes into the operand tile here: V = code vs 2^(7 - E) with E the largest exponent of the tile's scales, rounded
-// to 11 bits, so that z = s + E for every key of the tile and one multiplication a tile brings the sum of
-// the weights to the denominator's unit. Per-key factors in the softmax would each cost 16 loads of 512 bytes a warp and tile:
-// one, the keys' scales, is left of four. Where a tile's scales are more than 2^4 apart the exponents stay with the keys
-// (`wide`). The keys' scales multiply the scores, so codes of keys are exact.
+// to 11 bits, so that z = s + E for every key of the tile and one multiplication a tile brings the sum of the weights to the
+// denominator's unit. Per-key factors in the softmax would each cost 16 loads of 512 bytes a warp and tile: one, the keys' scales,
+// is left of four. Where a tile's scales are more than 2^4 apart, or a row is zeros, the exponents stay with the keys (`wide`: the
+// portion below 147 us if all tiles are). The keys' scales multiply the scores, so codes of keys are exact.
 //
-// Measured, 32 heads of 128 over 8: a prompt of 2,048 58 us (590 TFLOP/s), a portion of 512 on 8,192 106 us (668 TFLOP/s; over
+// Measured, 32 heads of 128 over 8: a prompt of 2,048 60 us (576 TFLOP/s), a portion of 512 on 8,192 106 us (668 TFLOP/s; over
 // bfloat16 pages, attention_tc.cu, 56 and 138). A tile of 64 keys takes two query tiles some 2,450 clocks, of which the tensor
 // pipe and the exponent unit need 1,024 each. No unit sets the pace: without seven eighths of the softmax's arithmetic the portion
 // took 20 % less, without most products 9 %, without all three roles' work still 72 us. What is left is the way round: a score
@@ -55,7 +55,7 @@ constexpr int WIDE = 4;
 template <bool F32> constexpr float LIFT = F32 ? Q8_LIFT : 8.f;
 // bfloat16 queries whose row's largest magnitude is 2^-6 to 2^9, as good as all, go in times 2^6, whatever rows are beside them: what
 // 16-bit floats have no steps for is 2^-25 of that magnitude and less. Another row has a power of two of its own, and its warp
-// walks the keys in a way of its own, which multiplies by the inverse (a portion of 512 on 8,192 136 us if all do, 107 if none).
+// walks the keys in a way of its own, which multiplies by the inverse (a portion of 512 on 8,192 141 us if all do, 106 if none).
 constexpr float Q_UNIT = 64.f;
 // Scores of such size have steps of an eighth: they are walked in that way too, which rounds a score before the reference is taken off.
 constexpr float FAR = 1048576.f;
@@ -126,8 +126,8 @@ __device__ __forceinline__ void tmem_ld32_done(uint32_t taddr, float (&v)[32]) {
 // F32: 32-bit rows, one query tile a block. A query goes in as two 16-bit parts, in two operand tiles, and so does a weight; the lower
 // parts have the second query tile's places in shared and tensor memory. (Sums of their own, as the tensor cores cut off what a
 // larger sum has no bits for; the errors are half of those of one sum.) The value scales stay out of the operand tile: their exponents go to the scores and their fractions
-// to the weights, so that codes are exact there too. 32 heads of 128 over 8: a prompt of 2,048 228 us, a portion of 512 on 8,192 368
-// (attention_q8.cu: 418 and 706), bound by a start and a join every 512 keys, which the errors ask for, and four factors a key.
+// to the weights, so that codes are exact there too. 32 heads of 128 over 8: a prompt of 2,048 237 us, a portion of 512 on 8,192 379
+// (attention_q8.cu: 429 and 736), bound by a start and a join every 512 keys, which the errors ask for, and four factors a key.
 template <int DP, int EXTRA, bool F32>
 __global__ void __launch_bounds__(NTHREADS, 1) attention_q8_tc_kernel(const Q8Params p) {
   using SH = Shape<DP, F32>;

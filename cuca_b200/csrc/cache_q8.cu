@@ -11,7 +11,7 @@
 // bytes a decode step reads; the error of a value is at most half a 127th of its row's largest.
 //
 // Both kernels do a few operations per byte and are bound by memory, or by latency when there are few rows. Measured, 32 heads of
-// 128 over 8: writing 2,048 rows and reading them back 16.4 us (10.5 and 5.1 by themselves; torch's copy of the queries' part alone
+// 128 over 8: writing 2,048 rows and reading them back 16.2 us (10.6 and 5.0 by themselves; torch's copy of the queries' part alone
 // takes 13.1), reading 34,000 positions back 47 us (5.8 TB/s, 0.89 of a copy's rate).
 #include "common.cuh"
 

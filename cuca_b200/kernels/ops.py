@@ -1682,7 +1682,7 @@ def read_q8(pages: QuantizedPages, positions, seq_of_row, tables, k_out, v_out, 
 
 Q8_FEW_ROWS = 24  # query rows of a key head that the form for few rows takes of a portion
 # 32-bit rows through tcgen05. The tensor cores cut off what a sum has no bits for: 512 keys in a row at most, then results are
-# joined (values of one sign, 544 keys: 1.2e-6 off as one sum, 3e-7 as two; a prompt of 2,048 228 us, with 1,024 keys in a row 205).
+# joined (values of one sign, 544 keys: 1.2e-6 off as one sum, 3e-7 as two; a prompt of 2,048 237 us, with 1,024 keys in a row 214).
 # And 700,000 pairs of a query row and a key at least: of 45 steps those with more took 0.4 to 1.0 of the other form's time but for
 # seven (up to 1.4 of it), those with fewer 0.9 to 1.6 but for five.
 Q8_SUMS_F32, Q8_LEAST_F32 = 512, 700_000
