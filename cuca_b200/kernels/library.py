@@ -190,10 +190,13 @@ _SIGNATURES = {
     "cuca_sum_norm_shift": [_P, _P, _P, _P, _F, _F, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P],
     "cuca_shift_rows": [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P],
     "cuca_moe_glu_capped_dense": [_P, _P, _I, _P, _I, _I, _I, _I, _I, _F, _F, _F, _P],
-    "cuca_rope_store_q8": [ctypes.c_char_p],  # (these four: a call's arguments packed as 64-bit words)
+    "cuca_rope_store_q8": [ctypes.c_char_p],  # (these: a call's arguments packed as 64-bit words)
     "cuca_read_q8": [ctypes.c_char_p],
     "cuca_attention_q8": [ctypes.c_char_p],
     "cuca_attention_q8_tc": [ctypes.c_char_p],
+    "cuca_mx4_quantise": [ctypes.c_char_p],
+    "cuca_mx4_values": [ctypes.c_char_p],
+    "cuca_gemm_mx4": [ctypes.c_char_p],
 }
 
 _lock = threading.Lock()

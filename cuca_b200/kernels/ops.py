@@ -1889,3 +1889,123 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
         for tile0 in range(0, tiles, once):
             library.check(entry(_Q8_ATTENTION.pack(*rows, lo, hi, tokens, min(once, tiles - tile0), tile0, *shape, heads, width, share,
                                                    shares, at, e, stream)), "attention_q8")
+
+
+# ------------------------------------------------------------------ matrices in 4 bits
+MX4_BLOCK, MX4_STEP, MX4_TILE = 32, 128, 128  # values of a scale; values and rows of 512 bytes of scales (`csrc/mx4.cuh`)
+# a call's arguments as 64-bit words (`CucaMx4Rows` and `CucaMx4Gemm` in csrc/mx4.cuh)
+_MX4_ROWS, _MX4_GEMM = struct.Struct("8q"), struct.Struct("17q")
+
+
+class Mx4Matrix:
+    """Rows in microscaled 4-bit floating point: every 32 values of a row are codes of 4 bits (a sign and one of 0, 1/2, 1, 3/2,
+    2, 3, 4, 6) and a byte for a power of two (`csrc/mx4.cuh`). Made by `mx4_quantise`; `shape` is that of the values."""
+
+    __slots__ = ("shape", "codes", "scales", "_at")
+
+    def __init__(self, rows: int, cols: int, codes: torch.Tensor, scales: torch.Tensor):
+        steps = -(-cols // MX4_STEP)
+        want = (rows, steps * MX4_STEP // 2), (-(-rows // MX4_TILE), steps, 32, 4, 4)
+        if cols < 1 or codes.shape != want[0] or scales.shape != want[1]:
+            raise library.KernelError(f"{rows} rows of {cols} values in 4 bits are codes {want[0]} and scales {want[1]}, not "
+                                      f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_contiguous() or not scales.is_contiguous():
+            raise library.KernelError("codes and scales in 4 bits are contiguous bytes")
+        if codes.device != scales.device:
+            raise library.KernelError(f"codes on {codes.device}, scales on {scales.device}")
+        self.shape, self.codes, self.scales = torch.Size((rows, cols)), codes, scales
+        self._at = codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, device) -> "Mx4Matrix":
+        """Memory for so many rows."""
+        steps = -(-cols // MX4_STEP)
+        return cls(rows, cols, torch.empty(rows, steps * MX4_STEP // 2, dtype=torch.uint8, device=device),
+                   torch.empty(-(-rows // MX4_TILE), steps, 32, 4, 4, dtype=torch.uint8, device=device))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+def _here(*tensors) -> None:
+    """Refuses tensors that are not on the current device: a launch goes to its stream."""
+    _cuda(*tensors)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise library.KernelError(f"kernel arguments on {t.device}, but the current device is cuda:{here}")
+
+
+def _rows(t, what: str) -> int:
+    """The stride of a tensor's rows, whose values lie next to each other."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise library.KernelError(f"{what} are a matrix whose rows have no gaps, not {tuple(t.shape)} with strides {t.stride()}")
+    if t.shape[0] <= 1:
+        return max(t.shape[1], 1)
+    if t.stride(0) < t.shape[1]:
+        raise library.KernelError(f"{what} overlap: strides {t.stride()}")
+    return t.stride(0)
+
+
+def mx4_quantise(x, out: Mx4Matrix | None = None) -> Mx4Matrix:
+    """Rows of 32 or 16 bits in 4 bits: of every 32 values, with a = max |x|, e = max(floor(log2 a) - 2, -127), codes are x / 2^e
+    rounded to the nearest, ties to the even code, at most 6. A block that is not finite reads back as NaN. `out`: memory to
+    use (of rows of the same shape)."""
+    ld = _rows(x, "rows to be quantised")
+    if x.shape[1] < 1:
+        raise library.KernelError("rows to be quantised hold no values")
+    if out is None:
+        out = Mx4Matrix.empty(*x.shape, x.device)
+    elif out.shape != x.shape:
+        raise library.KernelError(f"rows {tuple(x.shape)} do not fit memory for {tuple(out.shape)}")
+    _here(x, out.codes, out.scales)
+    library.check(library.load().cuca_mx4_quantise(_MX4_ROWS.pack(
+        x.data_ptr(), ld, dtype_code(x.dtype), *out._at, *x.shape, _stream())), "mx4_quantise")
+    return out
+
+
+def mx4_values(a: Mx4Matrix, out) -> None:
+    """out (32 or 16 bits) = the values that rows in 4 bits stand for, exactly."""
+    ld = _rows(out, "values")
+    if out.shape != a.shape:
+        raise library.KernelError(f"values of {tuple(a.shape)} rows in 4 bits do not fit {tuple(out.shape)}")
+    _here(out, a.codes, a.scales)
+    library.check(library.load().cuca_mx4_values(_MX4_ROWS.pack(
+        out.data_ptr(), ld, dtype_code(out.dtype), *a._at, *a.shape, _stream())), "mx4_values")
+
+
+def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> None:
+    """out = epilogue(a @ w.T) with a weight in 4 bits; `a`: [M, K] rows of 16 or 32 bits (of any stride and alignment) as they are, or
+    rows in 4 bits. Products are exact and summed in 32 bits. `epilogue`: EPI_STORE (plus `bias`; `out` 32-bit, or bfloat16 where
+    `a` is not 32-bit), EPI_RESIDUAL (added to a 32-bit `out`, with `bias`), EPI_SWIGLU (silu(g) u of the stacked gate and up rows
+    of `w`). `bias` is 32-bit with 32-bit rows, else bfloat16."""
+    M, K = a.shape
+    N = w.shape[0]
+    if epilogue == EPI_SWIGLU:
+        if N % 2 or bias is not None:
+            raise library.KernelError("a gated unit takes as many gate rows as up rows, and no bias")
+        N //= 2
+    if w.shape[1] != K or out.dim() != 2 or out.shape[0] != M or out.shape[1] != N:
+        raise library.KernelError(f"rows {tuple(a.shape)} times a weight {tuple(w.shape)} do not make {tuple(out.shape)}")
+    ldo = _rows(out, "results")
+    if isinstance(a, Mx4Matrix):
+        a_at, a_scales = a._at
+        kind, lda, f32 = 2, 0, False
+        _here(a.codes, w.codes, out, bias, err)
+    else:
+        a_at, a_scales, kind, lda = a.data_ptr(), 0, dtype_code(a.dtype), _rows(a, "rows")
+        f32 = kind == F32
+        _here(a, w.codes, out, bias, err)
+    out_f32 = out.dtype == torch.float32
+    if not out_f32 and (f32 or epilogue == EPI_RESIDUAL or out.dtype != torch.bfloat16):
+        raise library.KernelError(f"gemm_mx4: results in {out.dtype}")
+    if bias is not None and (bias.dtype != (torch.float32 if f32 else torch.bfloat16) or bias.shape != (N,)
+                             or not bias.is_contiguous()):
+        raise library.KernelError(f"gemm_mx4: a bias is {N} numbers of the compute type without gaps, not {tuple(bias.shape)} in {bias.dtype}")
+    library.check(library.load().cuca_gemm_mx4(_MX4_GEMM.pack(
+        a_at, a_scales, lda, kind, *w._at, _at(bias), out.data_ptr(), ldo, out_f32, M, N, K, epilogue, 0, _at(err), _stream())),
+        "gemm_mx4")
