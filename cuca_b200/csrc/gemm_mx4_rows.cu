@@ -10,10 +10,8 @@
 // scale per row; the rows of A lie in shared memory in the order in which the conversion leaves the codes. Few tiles: a
 // cluster of up to eight blocks shares K, and adds its sums in order out of each other's shared memory: no workspace, and
 // equal bits in every run.
-#include "mx4.cuh"
+#include "mx4_mma.cuh"
 #include <type_traits>
-
-int cuca_device_sms();
 
 namespace {
 
@@ -42,21 +40,6 @@ struct Params {
   int share;  // blocks of a cluster
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float peer_f32(const float* p, uint32_t rank) {  // the same place in a peer's shared memory
-  uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
-}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -139,7 +122,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_rows_kernel(const Params 
   constexpr int TOKENS = ROWS / PARTS;  // rows of A that a block takes
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int set = warp >> 2;
-  const int rank = p.share > 1 ? (int)cluster_rank() : 0;
+  const int rank = p.share > 1 ? (int)mx4_cluster_rank() : 0;
   const int tile = (int)blockIdx.x / p.share;
   const bool dual = p.epilogue == EPI_SWIGLU;
   const int m0 = (int)blockIdx.y * TOKENS;
@@ -247,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_rows_kernel(const Params 
     *reinterpret_cast<float2*>(at + 8 * SUM_STRIDE) = make_float2(acc[j][2], acc[j][3]);
   }
   __syncthreads();
-  if (p.share > 1) cluster_sync();
+  if (p.share > 1) mx4_cluster_sync();
   const int cols = dual ? TILE / 2 : TILE;  // output columns of a tile; this block finishes `mine` of them
   const int mine = cols / p.share, c0 = rank * mine;
   auto total = [&](int row, int v) {
@@ -255,7 +238,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_rows_kernel(const Params 
     for (int part = PARTS - 1; part >= 0; --part) {  // (small parts first)
       const float* at = sums + (row + part) * SUM_STRIDE + v;
       for (int r = 0; r < p.share; ++r) {
-        if (p.share > 1) y += peer_f32(at, r), y += peer_f32(at + ROWS * SUM_STRIDE, r);
+        if (p.share > 1) y += mx4_peer_f32(at, r), y += mx4_peer_f32(at + ROWS * SUM_STRIDE, r);
         else y += at[0], y += at[ROWS * SUM_STRIDE];
       }
     }
@@ -276,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_rows_kernel(const Params 
     else if (p.out_f32) ((float*)p.out)[o] = y;
     else ((__nv_bfloat16*)p.out)[o] = __float2bfloat16_rn(y);
   }
-  if (p.share > 1) cluster_sync();  // until nobody reads these sums any more
+  if (p.share > 1) mx4_cluster_sync();  // until nobody reads these sums any more
 }
 
 template <int KIND>
@@ -301,16 +284,4 @@ int launch(const CucaMx4Gemm* c) {
 
 int cuca_gemm_mx4_rows(const CucaMx4Gemm* c) {
   return c->a_kind == MX4_CODES ? launch<MX4_CODES>(c) : c->a_kind == CUCA_F32 ? launch<CUCA_F32>(c) : launch<CUCA_BF16>(c);
-}
-
-CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
-  CUCA_REQUIRE(c->a_kind == CUCA_F32 || c->a_kind == CUCA_BF16 || c->a_kind == MX4_CODES, "gemm_mx4: unknown rows %d", (int)c->a_kind);
-  CUCA_REQUIRE(c->epilogue >= EPI_STORE && c->epilogue <= EPI_SWIGLU, "gemm_mx4: unknown epilogue %d", (int)c->epilogue);
-  CUCA_REQUIRE(c->m >= 0 && c->n >= 0 && c->k > 0 && c->m < (1ll << 30) && c->n < (1ll << 29) && c->k < (1ll << 30),
-               "gemm_mx4: %lld x %lld x %lld", (long long)c->m, (long long)c->n, (long long)c->k);
-  CUCA_REQUIRE(c->epilogue != EPI_RESIDUAL || c->out_f32, "gemm_mx4: only a 32-bit stream is added to");
-  CUCA_REQUIRE(c->epilogue != EPI_SWIGLU || !c->bias, "gemm_mx4: a gated unit takes no bias");
-  CUCA_REQUIRE((((uintptr_t)c->w | (uintptr_t)c->w_scales) & 15) == 0, "gemm_mx4: codes and scales must start on 16 bytes");
-  if (c->m == 0 || c->n == 0) return 0;
-  return cuca_gemm_mx4_rows(c);
 }

@@ -1,0 +1,75 @@
+// What the tensor-core products with 4-bit weights share: block-scaled contractions, clusters, results.
+#pragma once
+#include "mx4.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+
+__device__ __forceinline__ uint32_t mx4_cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void mx4_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float mx4_peer_f32(const float* p, uint32_t rank) {  // the same place in a peer's shared memory
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void mx4_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
+}
+// After a wait gave up: copies in flight land before the shared memory is handed on.
+__device__ __forceinline__ void mx4_let_copies_land() {
+  const unsigned long long t0 = global_ns();
+  while (global_ns() - t0 < 2000000ull) { }
+}
+
+// ---- kind::mxf4: both operands e2m1, a power of two for 32 values
+// M rows by n columns, both K-major.
+__host__ __device__ constexpr uint32_t mx4_instr_desc(int n, int m) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24);
+}
+// which two of a column's four bytes the 64 values of an instruction go by, in both operands
+__host__ __device__ constexpr uint32_t mx4_scale_half(int half) { return half ? (2u << 4) | (2u << 29) : 0u; }
+__device__ __forceinline__ void mx4_umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t scale_a, uint32_t scale_b,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate) : "memory");
+}
+// 512 bytes of scales: 32 rows of 16 bytes, eight rows to 128 bytes, not swizzled
+__device__ __forceinline__ uint64_t mx4_scale_desc(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(128 >> 4) << 32;  // between groups of eight rows
+  d |= (uint64_t)1 << 46;
+  return d;
+}
+// ... into four columns of tensor memory, the same in each quarter of the lanes
+__device__ __forceinline__ void mx4_scales_to_tmem(uint32_t col, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(col), "l"(desc) : "memory");
+}
+
+// ---- results
+struct Mx4Out {
+  void* out;
+  const void* bias;  // bfloat16
+  int64_t ldo;
+  int m, n, out_f32, epilogue;
+};
+__device__ __forceinline__ float mx4_gate(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+__device__ __forceinline__ void mx4_put(const Mx4Out& o, int m, int n, float y) {
+  if (o.bias) y += __bfloat162float(((const __nv_bfloat16*)o.bias)[n]);
+  const int64_t at = m * o.ldo + n;
+  if (o.epilogue == EPI_RESIDUAL) ((float*)o.out)[at] += y;
+  else if (o.out_f32) ((float*)o.out)[at] = y;
+  else ((__nv_bfloat16*)o.out)[at] = __float2bfloat16_rn(y);
+}
+
+}  // namespace
