@@ -3,6 +3,7 @@
 
 int cuca_gemm_mx4_rows(const CucaMx4Gemm* c);
 int cuca_gemm_mx4_codes(const CucaMx4Gemm* c);
+int cuca_gemm_mx4_wide(const CucaMx4Gemm* c);
 
 CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
   CUCA_REQUIRE(c->a_kind == CUCA_F32 || c->a_kind == CUCA_BF16 || c->a_kind == MX4_CODES, "gemm_mx4: unknown rows %d", (int)c->a_kind);
@@ -16,7 +17,10 @@ CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
                "gemm_mx4: codes and scales must start on 16 bytes");
   if (c->m == 0 || c->n == 0) return 0;
   try {
-    return c->a_kind == MX4_CODES ? cuca_gemm_mx4_codes(c) : cuca_gemm_mx4_rows(c);
+    if (c->a_kind == MX4_CODES) return cuca_gemm_mx4_codes(c);
+    const bool copied = ((uintptr_t)c->a & 15) == 0 && (c->lda % 8 == 0 || c->m == 1);  // rows that the copy engine takes
+    if (c->a_kind == CUCA_BF16 && copied) return cuca_gemm_mx4_wide(c);
+    return cuca_gemm_mx4_rows(c);
   } catch (...) {  // the cache of tensor maps may find no memory
     cuca_set_error("gemm_mx4: out of host memory");
     return 3;

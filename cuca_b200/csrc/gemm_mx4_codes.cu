@@ -161,28 +161,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
       tc_fence_after();
       const int row = (warp & 3) * 32 + lane;
       const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
-      const int m_here = min(p.nt, p.o.m - m0);
-      if (p.share == 1) {
-        for (int c = 0; c < m_here; c += 16) {
-          float v[16], u[16];
-          tmem_ld16(at + c, v);
-          if (DUAL) tmem_ld16(at + p.nt + c, u);
-          if (n0 + row < p.o.n) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c + j < m_here) mx4_put(p.o, m0 + c + j, n0 + row, DUAL ? mx4_gate(v[j], u[j]) : v[j]);
-          }
-        }
-      } else {  // [accumulator][column][feature], where the stages lay: every copy into them has been waited for
-        float* sums = reinterpret_cast<float*>(smem) + row;
-        for (int b = 0; b < BLOCKS; ++b)
-          for (int c = 0; c < m_here; c += 16) {
-            float v[16];
-            tmem_ld16(at + b * p.nt + c, v);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sums[(b * p.nt + c + j) * TILE_A] = v[j];
-          }
-      }
+      mx4_leave<DUAL>(p.o, at, p.nt, m0, min(p.nt, p.o.m - m0), n0, row, p.share == 1, reinterpret_cast<float*>(smem));
       if (row == 0) *ok_flag = 1;
     }
   }
@@ -191,30 +170,14 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(acc, p.tmem_cols);
-  if (p.share > 1) {
-    mx4_cluster_sync();
-    const int mine = TILE_A / p.share, r0 = rank * mine, m_here = min(p.nt, p.o.m - m0);
-    const float* sums = reinterpret_cast<const float*>(smem);
-    if (*ok_flag) {
-      for (int i = threadIdx.x; i < m_here * mine; i += THREADS) {
-        const int c = i / mine, row = r0 + i - c * mine;
-        float v = 0.f, u = 0.f;
-        for (int r = 0; r < p.share; ++r) {
-          v += mx4_peer_f32(sums + c * TILE_A + row, r);
-          if (DUAL) u += mx4_peer_f32(sums + (p.nt + c) * TILE_A + row, r);
-        }
-        if (n0 + row < p.o.n) mx4_put(p.o, m0 + c, n0 + row, DUAL ? mx4_gate(v, u) : v);
-      }
-    }
-    mx4_cluster_sync();  // until nobody reads these sums any more
-  }
+  if (p.share > 1) mx4_join<DUAL>(p.o, reinterpret_cast<const float*>(smem), p.nt, m0, min(p.nt, p.o.m - m0), n0, rank, p.share, *ok_flag != 0);
 }
 
 template <bool DUAL>
 int launch(const CucaMx4Gemm* c) {
   Params p;
   p.a_scales = c->a_scales; p.w_scales = c->w_scales;
-  p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue};
+  p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, 0};
   p.k_steps = (int)mx4_steps(c->k);
   p.k_stages = (p.k_steps + STAGE_STEPS - 1) / STAGE_STEPS;
   p.err = c->err;

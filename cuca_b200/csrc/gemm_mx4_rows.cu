@@ -7,8 +7,7 @@
 //
 // A block has eight warps: four take 32 weight rows each of a tile of 128, and two sets of four take the steps of 128 values in turn.
 // A lane's 16 bytes are one block of 32 codes of one weight row, so a warp reads 64 bytes of 32 rows at a time and every lane has one
-// scale per row; the rows of A lie in shared memory in the order in which the conversion leaves the codes. Few tiles: a
-// cluster of up to eight blocks shares K, and adds its sums in order out of each other's shared memory: no workspace, and
+// scale per row. Few tiles: a cluster of up to eight blocks shares K, and adds its sums in order out of each other's shared memory: no workspace, and
 // equal bits in every run.
 #include "mx4_mma.cuh"
 #include <type_traits>
@@ -49,12 +48,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&t);
 }
-// pairs (0,1) (2,3) (4,5) (6,7) -> (0,4) (1,5) (2,6) (3,7): the order of mx4_to_bf16
-__device__ __forceinline__ uint4 in_code_order(const uint32_t (&w)[4]) {
-  return make_uint4(__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410),
-                    __byte_perm(w[1], w[3], 0x7632));
-}
-
 // Values c .. c + 7 of row m into the rows of shared memory that belong to it, one for each of its parts.
 template <int KIND>
 __device__ __forceinline__ void fill8(const Params& p, uint8_t* smem, int row, int m, int c, int at) {
@@ -81,7 +74,7 @@ __device__ __forceinline__ void fill8(const Params& p, uint8_t* smem, int row, i
           if (c + j < p.k) w[j >> 1] |= (uint32_t)__ldcg(reinterpret_cast<const unsigned short*>(src) + j) << (16 * (j & 1));
       }
     }
-    *reinterpret_cast<uint4*>(smem + row * A_STRIDE + at) = in_code_order(w);
+    *reinterpret_cast<uint4*>(smem + row * A_STRIDE + at) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
     float v[8];
 #pragma unroll
@@ -105,7 +98,7 @@ __device__ __forceinline__ void fill8(const Params& p, uint8_t* smem, int row, i
         v[2 * j] -= __uint_as_float(w[j] << 16);
         v[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
       }
-      *reinterpret_cast<uint4*>(smem + (row + part) * A_STRIDE + at) = in_code_order(w);
+      *reinterpret_cast<uint4*>(smem + (row + part) * A_STRIDE + at) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }

@@ -91,7 +91,10 @@ __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams 
   uint32_t word = 0;
   if (finite) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) word |= code_pair(e.v[2 * j] * inv, e.v[2 * j + 1] * inv) << (8 * j);
+    for (int j = 0; j < 4; ++j) {  // bytes hold codes 0 and 2, 4 and 6, 1 and 3, 5 and 7
+      const int i = (j & 1) * 4 + (j >> 1);
+      word |= code_pair(e.v[i] * inv, e.v[i + 2] * inv) << (8 * j);
+    }
   }
   // the four blocks' bytes, lowest first, by the step's first thread
   const uint32_t s1 = __shfl_down_sync(0xffffffffu, byte, 4), s2 = __shfl_down_sync(0xffffffffu, byte, 8),
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(THREADS) mx4_values_kernel(const RowsParams p)
   const float power = mx4_power(byte);
 #pragma unroll
   for (int j = 0; j < RUN; ++j) {
-    const uint32_t code = word >> (4 * j);
+    const uint32_t code = word >> (4 * ((j >> 1) + (j & 1) * 4));
     // the code's bits as a 32-bit number times 2^-126, brought up exactly
     const float x = __uint_as_float((code & 8) << 28 | (code & 7) << 22) * 8.507059173023462e+37f;  // 2^126
     v[j] = from_f32<T>(x * power);

@@ -3,8 +3,10 @@
 // A row is cut into blocks of 32 values. A block is a byte e, which stands for 2^(e - 127) (255: NaN), and 32 codes of 4 bits: a
 // sign and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6, so that the low three bits are two of exponent and one of mantissa.
 //
-//   codes   [rows, steps * 64] bytes, two codes to a byte, the first in the low half; a step is 128 values, and what a row's last
-//           step has beyond the row is zeros;
+//   codes   [rows, steps * 64] bytes; a step is 128 values, and what a row's last step has beyond the row is zeros. Eight codes are a
+//           32-bit word, in the order 0, 2, 4, 6, 1, 3, 5, 7 from its lowest bits up: the codes sixteen bits apart are next to
+//           each other, so masks and multiplications that work on both halves of a word at once leave pairs in their order. To a
+//           product of rows in 4 bits the order is nothing, both operands having it;
 //   scales  [tiles of 128 rows, steps, 32, 4, 4] bytes: row r, block b of it at [r / 128, b / 4, r % 32, r % 128 / 32, b % 4].
 //           512 bytes are the scales of 128 rows and 128 values as the tensor cores take them (four blocks of a row to a 32-bit
 //           column of tensor memory), so they go there without being moved about.
@@ -68,7 +70,7 @@ __device__ __forceinline__ float mx4_power(uint32_t e) {
   return __uint_as_float(e == 255 ? 0x7fffffffu : e ? e << 23 : 1u << 22);
 }
 
-// Eight codes as bfloat16 numbers times the power of two that a byte stands for, exactly: pair i holds codes i and i + 4.
+// Eight codes as bfloat16 numbers times the power of two that a byte stands for, exactly, in their order.
 // A code's sign goes to the sign, its other bits to the lowest exponent bits and the highest mantissa bit, which reads as the
 // magnitude times 2^-126 (1/2 as a number below the normal ones); the factor brings it up and applies the scale at once. Both
 // moves of a code are one multiplication: by 2^6 + 2^12 its copies do not meet, since 15 (2^6 + 2^12) < 2^16. The integer pipe is

@@ -59,17 +59,58 @@ __device__ __forceinline__ void mx4_scales_to_tmem(uint32_t col, uint64_t desc) 
 // ---- results
 struct Mx4Out {
   void* out;
-  const void* bias;  // bfloat16
+  const void* bias;  // 32-bit where `bias_f32`, else bfloat16
   int64_t ldo;
-  int m, n, out_f32, epilogue;
+  int m, n, out_f32, epilogue, bias_f32;
 };
 __device__ __forceinline__ float mx4_gate(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 __device__ __forceinline__ void mx4_put(const Mx4Out& o, int m, int n, float y) {
-  if (o.bias) y += __bfloat162float(((const __nv_bfloat16*)o.bias)[n]);
+  if (o.bias) y += o.bias_f32 ? ((const float*)o.bias)[n] : __bfloat162float(((const __nv_bfloat16*)o.bias)[n]);
   const int64_t at = m * o.ldo + n;
   if (o.epilogue == EPI_RESIDUAL) ((float*)o.out)[at] += y;
   else if (o.out_f32) ((float*)o.out)[at] = y;
   else ((__nv_bfloat16*)o.out)[at] = __float2bfloat16_rn(y);
+}
+
+// A finished tile: lane `row` (0..127) of tensor memory holds feature n0 + row, columns `at`.. the rows of A from m0 on (of a gated unit
+// the up part's `nt` further on). Alone, they are results; with shares of K in a cluster they go to shared memory, [accumulator][column]
+// [feature], from where every block of the cluster finishes its part of the features (mx4_join).
+template <bool DUAL>
+__device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int nt, int m0, int m_here, int n0, int row, bool alone, float* sums) {
+  for (int c = 0; c < m_here; c += 16) {
+    float v[16], u[16];
+    tmem_ld16(at + c, v);
+    if (DUAL) tmem_ld16(at + nt + c, u);
+    if (!alone) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        sums[(c + j) * TILE_A + row] = v[j];
+        if (DUAL) sums[(nt + c + j) * TILE_A + row] = u[j];
+      }
+    } else if (n0 + row < o.n) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, DUAL ? mx4_gate(v[j], u[j]) : v[j]);
+    }
+  }
+}
+// The shares' sums in order; all threads of all blocks of the cluster come here.
+template <bool DUAL>
+__device__ __forceinline__ void mx4_join(const Mx4Out& o, const float* sums, int nt, int m0, int m_here, int n0, int rank, int share, bool ok) {
+  mx4_cluster_sync();
+  const int mine = TILE_A / share, r0 = rank * mine;
+  if (ok) {
+    for (int i = threadIdx.x; i < m_here * mine; i += blockDim.x) {
+      const int c = i / mine, row = r0 + i - c * mine;
+      float v = 0.f, u = 0.f;
+      for (int r = 0; r < share; ++r) {
+        v += mx4_peer_f32(sums + c * TILE_A + row, r);
+        if (DUAL) u += mx4_peer_f32(sums + (nt + c) * TILE_A + row, r);
+      }
+      if (n0 + row < o.n) mx4_put(o, m0 + c, n0 + row, DUAL ? mx4_gate(v, u) : v);
+    }
+  }
+  mx4_cluster_sync();  // until nobody reads these sums any more
 }
 
 }  // namespace

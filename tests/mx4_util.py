@@ -37,7 +37,7 @@ def unpack(matrix):
     rows, cols = matrix.shape
     blocks = -(-cols // 32)
     c = matrix.codes.long()
-    code = torch.stack((c & 15, c >> 4), -1).view(rows, -1, 32)
+    code = torch.stack((c & 15, c >> 4), -1).view(rows, -1, 2, 4).transpose(2, 3).reshape(rows, -1, 32)  # 0 2 4 6 1 3 5 7
     tail = code[:, blocks:]
     assert not tail.any(), "what lies beyond a row in its last step is zeros"
     s = matrix.scales.long()  # [tiles, steps, 32, 4, 4]

@@ -13,7 +13,8 @@ def test_layout_of_codes_and_scales():
     q.codes.zero_()
     code, byte = torch.randint(0, 16, (300, 7, 32)), torch.randint(0, 256, (300, 7))
     flat = code.flatten(1)
-    q.codes[:, :112] = (flat[:, ::2] + 16 * flat[:, 1::2]).to(torch.uint8)
+    for i, (low, high) in enumerate(((0, 2), (4, 6), (1, 3), (5, 7))):
+        q.codes[:, i:112:4] = (flat[:, low::8] + 16 * flat[:, high::8]).to(torch.uint8)
     for r in range(300):
         for b in range(7):
             q.scales[r // 128, b // 4, r % 32, r % 128 // 32, b % 4] = byte[r, b]
