@@ -1,13 +1,16 @@
 // Rows in 4 bits times a weight in 4 bits: out = epilogue(A W^T) on tcgen05.mma.kind::mxf4, which takes the codes and the powers of two
 // of both operands as they are and sums in 32 bits.
 //
-// The weight is the 128-row operand, the rows of A the columns: D[feature, row], a lane of tensor memory per output feature (of a gated
-// unit two accumulators side by side, gate and up). Codes come by TMA in stages of 256 values of a row, 128 bytes, with 128-byte
-// swizzle; the scales of 128 rows and 128 values are 512 bytes that go into shared memory as one bulk copy and from there by
-// tcgen05.cp into four columns of tensor memory, in columns of their own for each stage, which are free when the stage is. Nothing is
-// converted, so few rows are bound by the weight's bytes; a block an SM has up to eight stages in flight, or two blocks five each.
-// Few tiles: a cluster of up to eight blocks shares K; each leaves its sums in shared memory and adds an eighth of the features up in
-// order out of the others': no workspace, equal bits in every run.
+// The weight is the 128-row operand, the rows of A the columns: D[feature, row], a lane of tensor memory per output feature. A tile has
+// one block of 128 features, or two that share the rows' tile: gate and up of a gated unit, or 256 features over many rows, where a
+// block alone would be bound by what it loads (96 bytes a clock at the tensor cores' rate, two blocks 72). Codes come by TMA in
+// stages of 256 values of a row, 128 bytes, with 128-byte swizzle; the scales of 128 rows and 128 values are 512 bytes that go into
+// shared memory as one bulk copy and from there by tcgen05.cp into four columns of tensor memory, columns of their own for each
+// stage, which are free when the stage is. A tile of A's rows may start at any multiple of 64: scales are taken
+// from the 128 rows that it starts in, two columns further on.
+// Nothing is converted, so few rows are bound by the weight's bytes. Few tiles: a cluster of up to eight blocks shares K; each
+// leaves its sums in shared memory and adds an eighth of the features up in order out of the others': no workspace, equal bits in
+// every run.
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
 
@@ -16,10 +19,13 @@ namespace {
 constexpr int STAGE_BYTES_K = 128;          // bytes of a row in a stage
 constexpr int STAGE_STEPS = 2;              // of 128 values
 constexpr int MAX_STAGES = 8;
-constexpr int A_BYTES = TILE_A * STAGE_BYTES_K;
+constexpr int W_BYTES = TILE_A * STAGE_BYTES_K;
 constexpr int SCALE_BYTES = 512;            // of 128 rows and a step
 constexpr int MAX_CLUSTER = 8;
-constexpr int THREADS = 192;                // a warp that loads, one that multiplies, four that read tensor memory
+constexpr int MANY_ROWS = 256;              // more rows than these: two blocks of features
+constexpr int MANY_TILE = 192;              // ... and tiles of so many rows: two accumulators leave 128 columns for scales
+constexpr int READ_WARP = 2, READ_WARPS = 8, ROW_WARP = READ_WARP + READ_WARPS;
+constexpr int THREADS = 32 * (ROW_WARP + 1);  // a warp that loads weights, one that multiplies, eight that read results, one that loads rows
 constexpr int BARRIERS = 512;
 
 struct Params {
@@ -27,17 +33,17 @@ struct Params {
   const uint8_t* w_scales;
   Mx4Out o;
   int k_steps, k_stages;
-  int nt;          // columns of a tile: rows of A, a multiple of 16
+  int nt;          // rows of A of a whole tile, a multiple of 16
   int a_tiles;     // tiles of 128 rows that A's scales have
   int tiles_n, share;
   int stages, stage_bytes, tmem_cols;
   int* err;
 };
 
-template <bool DUAL>
+template <int BLOCKS, bool DUAL, int SPANS>
 __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
                                                                  const Params p) {
-  constexpr int BLOCKS = DUAL ? 2 : 1;
+  static_assert(!DUAL || BLOCKS == 2, "gate and up");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = (uint64_t*)(smem + p.stages * p.stage_bytes);
@@ -49,18 +55,20 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.share > 1 ? (int)mx4_cluster_rank() : 0;
   const int tile = (int)blockIdx.x / p.share;
-  const int n0 = (tile % p.tiles_n) * TILE_A, m0 = (tile / p.tiles_n) * p.nt;
+  const int n0 = (tile % p.tiles_n) * (DUAL ? TILE_A : BLOCKS * TILE_A), m0 = (tile / p.tiles_n) * p.nt;
+  const int m_here = min(p.nt, p.o.m - m0), nt = (m_here + 15) & ~15;  // (the last tile multiplies no more columns than it has)
   const int ks0 = (int)((int64_t)p.k_stages * rank / p.share), ks1 = (int)((int64_t)p.k_stages * (rank + 1) / p.share);
-  const int up0 = p.o.n + n0;                     // the first up row
-  const bool up_apart = DUAL && (p.o.n & 127);    // the up rows' scales do not start where 128 rows' do
-  const int scale_tiles = min((p.nt + 127) >> 7, p.a_tiles - (m0 >> 7));
-  const int b_bytes = p.nt * STAGE_BYTES_K;
-  // scales of a stage: [block of weight rows][step][512], then [tile of 128 rows of A][step][512]
-  const int sc_w = BLOCKS * A_BYTES + b_bytes, sc_a = sc_w + BLOCKS * STAGE_STEPS * SCALE_BYTES;
+  const int second = DUAL ? p.o.n + n0 : n0 + TILE_A;  // the second block's first weight row
+  const bool up_apart = DUAL && (p.o.n & 127);         // the up rows' scales do not start where 128 rows' do
+  const bool scaled = DUAL || second < p.o.n;          // the second block has features (else it multiplies zeros)
+  const int span0 = m0 >> 7, spans = min(SPANS, p.a_tiles - span0);
+  const int a_bytes = p.nt * STAGE_BYTES_K;
+  // scales of a stage: [block of features][step][512], then [128 rows of A][step][512]
+  const int sc_w = BLOCKS * W_BYTES + a_bytes, sc_a = sc_w + BLOCKS * STAGE_STEPS * SCALE_BYTES;
   pdl_trigger();
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full[s], up_apart ? 2 : 1);
+      mbar_init(&full[s], up_apart ? 3 : 2);
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
@@ -76,93 +84,126 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t acc = *tmem_slot;
-  // columns: the accumulators, then a stage's scales in turn
-  const int b_cols = 4 * ((p.nt + 127) >> 7);  // of a step
-  const int stage_cols = STAGE_STEPS * (4 * BLOCKS + b_cols);
-  const uint32_t scale_cols = acc + BLOCKS * p.nt;
+  const uint32_t scale_cols = acc + BLOCKS * p.nt;  // of each stage and step [block of features][4], [128 rows of A][4]
 
   if (warp == 0) {
-    if (lane == 0) {  // the first weights into L2: that needs no wait for the kernel before, whatever it writes
+    // ------------------------------------------------ weights
+    if (lane == 0) {  // the first ones into L2: that needs no wait for the kernel before, whatever it writes
       for (int ks = ks0; ks < ks1 && ks < ks0 + p.stages; ++ks) {
         mx4_prefetch_2d(&tm_w, ks * 64, n0);
-        if (DUAL) mx4_prefetch_2d(&tm_w, ks * 64, up0);
+        if (BLOCKS == 2) mx4_prefetch_2d(&tm_w, ks * 64, second);
       }
     }
     __syncwarp();
     pdl_wait();
-    for (int ks = ks0, it = 0; ks < ks1; ++ks, ++it) {
-      const int st = it % p.stages;
-      uint8_t* sp = smem + st * p.stage_bytes;
-      if (it >= p.stages && !warp_wait(&empty[st], ((it / p.stages) & 1) ^ 1, p.err, abort_flag)) break;
+    Mx4Ring ring;
+    for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
+      uint8_t* sp = smem + ring.at * p.stage_bytes;
+      uint64_t* bar = &full[ring.at];
+      if (!warp_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) break;
       const int s0 = ks * STAGE_STEPS, steps = min(STAGE_STEPS, p.k_steps - s0);
       if (lane == 0) {
         const uint32_t sc = steps * SCALE_BYTES;
-        mbar_expect_tx(&full[st], BLOCKS * A_BYTES + b_bytes + sc * ((up_apart ? 1 : BLOCKS) + scale_tiles));
-        tma_load_2d(sp, &tm_w, &full[st], ks * 64, n0);
-        if (DUAL) tma_load_2d(sp + A_BYTES, &tm_w, &full[st], ks * 64, up0);
-        tma_load_2d(sp + BLOCKS * A_BYTES, &tm_a, &full[st], ks * 64, m0);
-        bulk_load(sp + sc_w, p.w_scales + mx4_scale_at(n0, s0, p.k_steps), &full[st], sc);
-        if (DUAL && !up_apart)
-          bulk_load(sp + sc_w + STAGE_STEPS * SCALE_BYTES, p.w_scales + mx4_scale_at(up0, s0, p.k_steps), &full[st], sc);
-        for (int t = 0; t < scale_tiles; ++t)
-          bulk_load(sp + sc_a + t * STAGE_STEPS * SCALE_BYTES, p.a_scales + mx4_scale_at(m0 + 128 * t, s0, p.k_steps), &full[st], sc);
+        mbar_expect_tx(bar, BLOCKS * W_BYTES + sc * (up_apart || !scaled ? 1 : BLOCKS));
+        tma_load_2d(sp, &tm_w, bar, ks * 64, n0);
+        if (BLOCKS == 2) tma_load_2d(sp + W_BYTES, &tm_w, bar, ks * 64, second);
+        bulk_load(sp + sc_w, p.w_scales + mx4_scale_at(n0, s0, p.k_steps), bar, sc);
+        if (BLOCKS == 2 && !up_apart && scaled)
+          bulk_load(sp + sc_w + STAGE_STEPS * SCALE_BYTES, p.w_scales + mx4_scale_at(second, s0, p.k_steps), bar, sc);
       }
       if (up_apart) {  // word by word: a lane's sixteen bytes are the scales of rows 32 apart
         for (int s = 0; s < steps; ++s) {
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = min(up0 + 32 * i + lane, 2 * p.o.n - 1);
+            const int r = min(second + 32 * i + lane, 2 * p.o.n - 1);
             w[i] = __ldcg(reinterpret_cast<const uint32_t*>(p.w_scales + mx4_scale_at(r, s0 + s, p.k_steps)));
           }
           *reinterpret_cast<uint4*>(sp + sc_w + (STAGE_STEPS + s) * SCALE_BYTES + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[st]);
+        if (lane == 0) mbar_arrive(bar);
       }
       __syncwarp();
     }
+  } else if (warp == ROW_WARP) {
+    // ------------------------------------------------ rows of A
+    if (lane == 0) {
+      pdl_wait();
+      Mx4Ring ring;
+      for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
+        uint8_t* sp = smem + ring.at * p.stage_bytes;
+        uint64_t* bar = &full[ring.at];
+        if (!mbar_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) break;
+        const int s0 = ks * STAGE_STEPS;
+        const uint32_t sc = min(STAGE_STEPS, p.k_steps - s0) * SCALE_BYTES;
+        mbar_expect_tx(bar, a_bytes + sc * spans);
+        tma_load_2d(sp + BLOCKS * W_BYTES, &tm_a, bar, ks * 64, m0);
+        for (int t = 0; t < spans; ++t)
+          bulk_load(sp + sc_a + t * STAGE_STEPS * SCALE_BYTES, p.a_scales + mx4_scale_at((span0 + t) * 128, s0, p.k_steps), bar, sc);
+      }
+    }
   } else if (warp == 1) {
+    // ------------------------------------------------ products. What a stage issues stands unrolled, its descriptors one addition from
+    // the first stage's: an instruction whose operands are worked out beside it takes twice as long to issue, and a stage has seventeen
     pdl_wait();
-    const uint32_t idesc = mx4_instr_desc(p.nt, TILE_A);
+    const uint32_t idesc = mx4_instr_desc(nt, TILE_A);
+    const uint32_t sa = smem_u32(smem);
+    const uint64_t w0 = smem_desc(sa), a0 = smem_desc(sa + BLOCKS * W_BYTES), sw0 = mx4_scale_desc(sa + sc_w), sr0 = mx4_scale_desc(sa + sc_a);
+    const uint32_t shift = (m0 & 127) >> 5;  // columns of scales before this tile's first row
+    const uint64_t stride = p.stage_bytes >> 4;
+    constexpr int STEP_COLS = 4 * (BLOCKS + SPANS);
+    Mx4Ring ring;
     bool ok = true;
-    for (int ks = ks0, it = 0; ks < ks1; ++ks, ++it) {
-      const int st = it % p.stages;
-      if (!warp_wait(&full[st], (it / p.stages) & 1, p.err, abort_flag)) { ok = false; break; }
+    for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
+      if (!warp_wait(&full[ring.at], ring.parity, p.err, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      const uint32_t sa = smem_u32(smem + st * p.stage_bytes);
-      const uint64_t adesc = smem_desc(sa), adesc2 = smem_desc(sa + A_BYTES), bdesc = smem_desc(sa + BLOCKS * A_BYTES);
-      const uint32_t cols = scale_cols + st * stage_cols, cols_b = cols + STAGE_STEPS * 4 * BLOCKS;
-      const int steps = min(STAGE_STEPS, p.k_steps - ks * STAGE_STEPS);
+      const uint64_t at = ring.at * stride;
+      const uint32_t cols = scale_cols + ring.at * (STAGE_STEPS * STEP_COLS);
+      const bool whole = (ks + 1) * STAGE_STEPS <= p.k_steps;
       if (elect_one()) {
-        for (int s = 0; s < steps; ++s) {
-          for (int b = 0; b < BLOCKS; ++b)
-            mx4_scales_to_tmem(cols + (b * STAGE_STEPS + s) * 4, mx4_scale_desc(sa + sc_w + (b * STAGE_STEPS + s) * SCALE_BYTES));
-          for (int t = 0; t < scale_tiles; ++t)
-            mx4_scales_to_tmem(cols_b + s * b_cols + 4 * t, mx4_scale_desc(sa + sc_a + (t * STAGE_STEPS + s) * SCALE_BYTES));
+#pragma unroll
+        for (int s = 0; s < STAGE_STEPS; ++s) {
+          if (s == 0 || whole) {
+            const uint32_t cols_w = cols + s * STEP_COLS, cols_a = cols_w + 4 * BLOCKS;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+              mx4_scales_to_tmem(cols_w + 4 * b, sw0 + at + (uint64_t)((b * STAGE_STEPS + s) * SCALE_BYTES >> 4));
+#pragma unroll
+            for (int t = 0; t < SPANS; ++t)
+              mx4_scales_to_tmem(cols_a + 4 * t, sr0 + at + (uint64_t)((t * STAGE_STEPS + s) * SCALE_BYTES >> 4));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // 64 values each
+              const uint64_t off = at + (uint64_t)((s * 64 + h * 32) >> 4);
+              const uint32_t id = idesc | mx4_scale_half(h), accumulate = s + h > 0 ? 1u : ks > ks0;
+#pragma unroll
+              for (int b = 0; b < BLOCKS; ++b)
+                mx4_umma(acc + b * p.nt, w0 + off + (uint64_t)(b * W_BYTES >> 4), a0 + off, id, cols_w + 4 * b, cols_a + shift, accumulate);
+            }
+          }
         }
-        for (int j = 0; j < 2 * steps; ++j) {  // 64 values each
-          const uint64_t off = (uint64_t)(j * 32 >> 4);
-          const uint32_t id = idesc | mx4_scale_half(j & 1), sb = cols_b + (j >> 1) * b_cols;
-          const uint32_t accumulate = it > 0 || j > 0;
-          mx4_umma(acc, adesc + off, bdesc + off, id, cols + (j >> 1) * 4, sb, accumulate);
-          if (DUAL) mx4_umma(acc + p.nt, adesc2 + off, bdesc + off, id, cols + (STAGE_STEPS + (j >> 1)) * 4, sb, accumulate);
-        }
-        umma_commit(&empty[st]);
+        umma_commit(&empty[ring.at]);
       }
       __syncwarp();
     }
     if (ok && elect_one()) umma_commit(done);
     __syncwarp();
   } else {
+    // ------------------------------------------------ results: of two blocks of features a set of four warps takes each, else halves of the columns
     pdl_wait();
     if (warp_wait(done, 0, p.err, abort_flag)) {
       tc_fence_after();
-      const int row = (warp & 3) * 32 + lane;
+      const int set = (warp - READ_WARP) >> 2, row = (warp & 3) * 32 + lane;
       const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
-      mx4_leave<DUAL>(p.o, at, p.nt, m0, min(p.nt, p.o.m - m0), n0, row, p.share == 1, reinterpret_cast<float*>(smem));
-      if (row == 0) *ok_flag = 1;
+      float* sums = reinterpret_cast<float*>(smem);  // (every copy into the stages has been waited for)
+      if (BLOCKS == 2 && !DUAL) {
+        if (set == 0 || scaled) mx4_leave<false>(p.o, at + set * p.nt, p.nt, m0, m_here, n0 + set * TILE_A, row, p.share == 1, sums + set * p.nt * TILE_A);
+      } else {
+        const int half = (nt / 2 + 15) & ~15, first = set * half, last = set ? m_here : min(half, m_here);
+        if (last > first) mx4_leave<DUAL>(p.o, at + first, p.nt, m0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A);
+      }
+      if (threadIdx.x == READ_WARP * 32) *ok_flag = 1;
     }
   }
   __syncwarp();
@@ -170,45 +211,47 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(acc, p.tmem_cols);
-  if (p.share > 1) mx4_join<DUAL>(p.o, reinterpret_cast<const float*>(smem), p.nt, m0, min(p.nt, p.o.m - m0), n0, rank, p.share, *ok_flag != 0);
+  if (p.share > 1) {
+    const float* sums = reinterpret_cast<const float*>(smem);
+    mx4_join<DUAL>(p.o, sums, p.nt, m0, m_here, n0, rank, p.share, *ok_flag != 0);
+    if (BLOCKS == 2 && !DUAL) mx4_join<false>(p.o, sums + p.nt * TILE_A, p.nt, m0, m_here, n0 + TILE_A, rank, p.share, *ok_flag != 0 && scaled);
+  }
 }
 
-template <bool DUAL>
-int launch(const CucaMx4Gemm* c) {
+template <int BLOCKS, bool DUAL, int SPANS>
+int launch_spans(const CucaMx4Gemm* c) {
   Params p;
   p.a_scales = c->a_scales; p.w_scales = c->w_scales;
   p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, 0};
   p.k_steps = (int)mx4_steps(c->k);
   p.k_stages = (p.k_steps + STAGE_STEPS - 1) / STAGE_STEPS;
   p.err = c->err;
-  const int most = DUAL ? 128 : 256;
+  const int most = BLOCKS == 2 ? MANY_TILE : MANY_ROWS;
   p.nt = c->m >= most ? most : ((int)c->m + 15) / 16 * 16;
   p.a_tiles = (int)((c->m + 127) / 128);
-  p.tiles_n = (int)((c->n + TILE_A - 1) / TILE_A);
+  const int features = DUAL ? TILE_A : BLOCKS * TILE_A;
+  p.tiles_n = (int)((c->n + features - 1) / features);
   const int64_t tiles = (int64_t)p.tiles_n * ((c->m + p.nt - 1) / p.nt);
   CUCA_REQUIRE(tiles * MAX_CLUSTER < (1ll << 31), "gemm_mx4: %lld rows by %lld features are too many", (long long)c->m, (long long)c->n);
-  const int blocks = DUAL ? 2 : 1, scale_tiles = (p.nt + 127) / 128;
-  p.stage_bytes = blocks * (A_BYTES + STAGE_STEPS * SCALE_BYTES) + p.nt * STAGE_BYTES_K + scale_tiles * STAGE_STEPS * SCALE_BYTES;
-  // two blocks an SM where tiles are small
-  const bool two = p.nt * blocks <= 64;
-  const int budget = (two ? 108 : 210) * 1024;
-  p.stages = budget / p.stage_bytes < MAX_STAGES ? budget / p.stage_bytes : MAX_STAGES;
+  p.stage_bytes = BLOCKS * (W_BYTES + STAGE_STEPS * SCALE_BYTES) + p.nt * STAGE_BYTES_K + SPANS * STAGE_STEPS * SCALE_BYTES;
+  const bool two = p.nt * BLOCKS <= 64;  // blocks an SM
+  const int budget = (two ? 108 : 222) * 1024, room = (two ? 256 : 512) - BLOCKS * p.nt, stage_cols = STAGE_STEPS * 4 * (BLOCKS + SPANS);
+  p.stages = budget / p.stage_bytes;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  if (p.stages > room / stage_cols) p.stages = room / stage_cols;
   if (p.stages > p.k_stages) p.stages = p.k_stages;
-  const int need = blocks * p.nt + p.stages * STAGE_STEPS * 4 * (blocks + scale_tiles);
   p.tmem_cols = 32;
-  while (p.tmem_cols < need) p.tmem_cols *= 2;
+  while (p.tmem_cols < BLOCKS * p.nt + p.stages * stage_cols) p.tmem_cols *= 2;
   CUCA_REQUIRE(p.stages >= 1 && p.tmem_cols <= (two ? 256 : 512), "gemm_mx4: no room for a tile");
-  const int slots = cuca_device_sms() * (two ? 2 : 1);
+  const int slots = cuca_device_sms() * (two ? 2 : 1), sums = BLOCKS * p.nt * TILE_A * 4;
   p.share = 1;
-  while (p.share < MAX_CLUSTER && tiles * p.share * 2 <= slots && p.k_stages >= p.share * 4) p.share *= 2;
-  // (shares are cut from four stages on, so a block has that many, or two of a gated unit: sums fit)
-  CUCA_REQUIRE(p.share == 1 || p.stages * p.stage_bytes >= blocks * p.nt * TILE_A * 4, "gemm_mx4: sums do not fit");
+  while (p.share < MAX_CLUSTER && tiles * p.share * 2 <= slots && p.k_stages >= p.share * 4 && sums <= p.stages * p.stage_bytes) p.share *= 2;
   const int smem = p.stages * p.stage_bytes + 1024 + BARRIERS;
   CUtensorMap tm_w, tm_a;
   const uint64_t cols = (uint64_t)p.k_steps * 32;  // the codes as 16-bit elements
-  CUCA_REQUIRE(cuca_tensor_map_2d(c->w, 2, (uint64_t)c->n * blocks, cols, cols, TILE_A, &tm_w) &&
+  CUCA_REQUIRE(cuca_tensor_map_2d(c->w, 2, (uint64_t)c->n * (DUAL ? 2 : 1), cols, cols, TILE_A, &tm_w) &&
                cuca_tensor_map_2d(c->a, 2, (uint64_t)c->m, cols, cols, p.nt, &tm_a), "gemm_mx4: tensor map failed");
-  constexpr auto kernel = gemm_mx4_codes_kernel<DUAL>;
+  constexpr auto kernel = gemm_mx4_codes_kernel<BLOCKS, DUAL, SPANS>;
   if (int e = mx4_configure<kernel>(227 * 1024)) return e;
   const dim3 grid((unsigned)(tiles * p.share));
   if (p.share > 1) cuca_launch_cluster(kernel, grid, dim3(THREADS), smem, c->stream, true, p.share, tm_w, tm_a, p);
@@ -217,6 +260,15 @@ int launch(const CucaMx4Gemm* c) {
   return 0;
 }
 
+// a tile of more than 128 rows, or one that starts in the middle of 128, touches the scales of two runs of 128 rows
+template <int BLOCKS, bool DUAL>
+int launch(const CucaMx4Gemm* c) {
+  return c->m > 128 ? launch_spans<BLOCKS, DUAL, 2>(c) : launch_spans<BLOCKS, DUAL, 1>(c);
+}
+
 }  // namespace
 
-int cuca_gemm_mx4_codes(const CucaMx4Gemm* c) { return c->epilogue == EPI_SWIGLU ? launch<true>(c) : launch<false>(c); }
+int cuca_gemm_mx4_codes(const CucaMx4Gemm* c) {
+  if (c->epilogue == EPI_SWIGLU) return launch<2, true>(c);
+  return c->m > MANY_ROWS ? launch_spans<2, false, 2>(c) : launch<1, false>(c);
+}

@@ -100,10 +100,11 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_con
         if (DUAL) mx4_prefetch_2d(&tm_w, ks * 64, up0);
       }
       pdl_wait();
-      for (int ks = ks0, it = 0; ks < ks1; ++ks, ++it) {
-        const int st = it % p.codes;
+      Mx4Ring ring;
+      for (int ks = ks0; ks < ks1; ++ks, ring.next(p.codes)) {
+        const int st = ring.at;
         uint8_t* sp = smem + st * CODE_STAGE;
-        if (it >= p.codes && !mbar_wait(&code_empty[st], ((it / p.codes) & 1) ^ 1, p.err, abort_flag)) break;
+        if (!mbar_wait(&code_empty[st], ring.parity ^ 1, p.err, abort_flag)) break;
         const int s0 = ks * STAGE_STEPS;
         const uint32_t sc = min(STAGE_STEPS, p.k_steps - s0) * SCALE_BYTES;
         mbar_expect_tx(&code_full[st], BLOCKS * CODE_BYTES + sc * (up_apart ? 1 : BLOCKS));
@@ -118,11 +119,11 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_con
     // ------------------------------------------------ rows of X
     if (lane == 0) {
       pdl_wait();
-      for (int c = c0, it = 0; c < c1; ++c, ++it) {
-        const int st = it % p.xs;
-        if (it >= p.xs && !mbar_wait(&x_empty[st], ((it / p.xs) & 1) ^ 1, p.err, abort_flag)) break;
-        mbar_expect_tx(&x_full[st], x_bytes);
-        tma_load_2d(x_smem + st * x_bytes, &tm_x, &x_full[st], c * CHUNK, m0);
+      Mx4Ring ring;
+      for (int c = c0; c < c1; ++c, ring.next(p.xs)) {
+        if (!mbar_wait(&x_empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) break;
+        mbar_expect_tx(&x_full[ring.at], x_bytes);
+        tma_load_2d(x_smem + ring.at * x_bytes, &tm_x, &x_full[ring.at], c * CHUNK, m0);
       }
     }
   } else if (warp == 1) {
@@ -130,10 +131,11 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_con
     pdl_wait();
     const uint32_t idesc = instr_desc(p.nt);
     bool ok = true;
-    for (int c = c0, it = 0; c < c1; ++c, ++it) {
-      const int xs = it % p.xs, buf = it % p.bufs;
-      if (!warp_wait(&x_full[xs], (it / p.xs) & 1, p.err, abort_flag)) { ok = false; break; }
-      if (!warp_wait(&a_full[buf], (it / p.bufs) & 1, p.err, abort_flag)) { ok = false; break; }
+    Mx4Ring x_ring, a_ring;
+    for (int c = c0; c < c1; ++c, x_ring.next(p.xs), a_ring.next(p.bufs)) {
+      const int xs = x_ring.at, buf = a_ring.at;
+      if (!warp_wait(&x_full[xs], x_ring.parity, p.err, abort_flag)) { ok = false; break; }
+      if (!warp_wait(&a_full[buf], a_ring.parity, p.err, abort_flag)) { ok = false; break; }
       tc_fence_after();
       const uint64_t bdesc = smem_desc(smem_u32(x_smem + xs * x_bytes));
       const uint32_t a = a_cols + buf * BLOCKS * CHUNK_COLS;
@@ -141,8 +143,8 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_con
 #pragma unroll
         for (int k = 0; k < CHUNK / UMMA_K; ++k) {
           const uint64_t off = (uint64_t)(k * UMMA_K * 2 >> 4);
-          umma_bf16_tmem_a(acc, a + k * 8, bdesc + off, idesc, it > 0 || k > 0);
-          if (DUAL) umma_bf16_tmem_a(acc + p.nt, a + CHUNK_COLS + k * 8, bdesc + off, idesc, it > 0 || k > 0);
+          umma_bf16_tmem_a(acc, a + k * 8, bdesc + off, idesc, c > c0 || k > 0);
+          if (DUAL) umma_bf16_tmem_a(acc + p.nt, a + CHUNK_COLS + k * 8, bdesc + off, idesc, c > c0 || k > 0);
         }
         umma_commit(&x_empty[xs]);
         umma_commit(&a_empty[buf]);
@@ -161,18 +163,20 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_con
     const uint8_t* scales_of_row = p.w_scales + mx4_scale_at(min(up0 + row, 2 * p.o.n - 1), 0, p.k_steps);
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     bool ok = true;
-    for (int ks = ks0, it = 0; ok && ks < ks1; ++ks, ++it) {
-      const int st = it % p.codes;
+    Mx4Ring ring, a_ring;
+    if (!DUAL) a_ring.next(p.bufs, set);
+    for (int ks = ks0; ok && ks < ks1; ++ks, ring.next(p.codes)) {
+      const int st = ring.at;
       const uint8_t* sp = smem + st * CODE_STAGE;
       const uint8_t* codes = sp + block * CODE_BYTES + row * STAGE_BYTES_K;
       const int steps = min(STAGE_STEPS, p.k_steps - ks * STAGE_STEPS);
-      if (!warp_wait(&code_full[st], (it / p.codes) & 1, p.err, abort_flag)) { ok = false; break; }
+      if (!warp_wait(&code_full[st], ring.parity, p.err, abort_flag)) { ok = false; break; }
       for (int s = 0; s < steps; ++s) {
         const uint32_t bytes = apart ? __ldcg(reinterpret_cast<const uint32_t*>(scales_of_row + (ks * STAGE_STEPS + s) * 512ll))
                                      : *reinterpret_cast<const uint32_t*>(sp + BLOCKS * CODE_BYTES + (block * STAGE_STEPS + s) * SCALE_BYTES +
                                                                           lane * 16 + quarter * 4);
-        for (int h = DUAL ? 0 : set; h < (DUAL ? 2 : set + 1); ++h) {  // halves of a step: chunks
-          const int chunk = s * 2 + h, c = it * STAGE_CHUNKS + chunk, buf = c % p.bufs;
+        for (int h = DUAL ? 0 : set; h < (DUAL ? 2 : set + 1); ++h, a_ring.next(p.bufs, DUAL ? 1 : 2)) {  // halves of a step: chunks
+          const int chunk = s * 2 + h, buf = a_ring.at;
           uint32_t r[32];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
@@ -198,7 +202,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_con
               }
             }
           }
-          if (c >= p.bufs && !warp_wait(&a_empty[buf], ((c / p.bufs) & 1) ^ 1, p.err, abort_flag)) { ok = false; break; }
+          if (!warp_wait(&a_empty[buf], a_ring.parity ^ 1, p.err, abort_flag)) { ok = false; break; }
           tc_fence_after();
           tmem_st32_raw(a_cols + (buf * BLOCKS + block) * CHUNK_COLS + lanes, r);
           tmem_st_wait();

@@ -29,6 +29,18 @@ __device__ __forceinline__ void mx4_let_copies_land() {
   while (global_ns() - t0 < 2000000ull) { }
 }
 
+// A place in a ring of n, and the parity of the phase that is being filled (a remainder costs some 100 clocks a turn). Those who
+// wait for a place to be full wait for `parity`, those who wait for it to be free for its opposite, which a new barrier grants.
+struct Mx4Ring {
+  int at;
+  uint32_t parity;
+  __device__ Mx4Ring() : at(0), parity(0) {}
+  __device__ void next(int n, int by = 1) {
+    at += by;
+    if (at >= n) { at -= n; parity ^= 1; }
+  }
+};
+
 // ---- kind::mxf4: both operands e2m1, a power of two for 32 values
 // M rows by n columns, both K-major.
 __host__ __device__ constexpr uint32_t mx4_instr_desc(int n, int m) {
