@@ -198,10 +198,11 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
       const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
       float* sums = reinterpret_cast<float*>(smem);  // (every copy into the stages has been waited for)
       if (BLOCKS == 2 && !DUAL) {
-        if (set == 0 || scaled) mx4_leave<false>(p.o, at + set * p.nt, p.nt, m0, m_here, n0 + set * TILE_A, row, p.share == 1, sums + set * p.nt * TILE_A);
+        if (set == 0 || scaled) mx4_leave(p.o, at + set * p.nt, m0, m_here, n0 + set * TILE_A, row, p.share == 1, sums + set * p.nt * TILE_A);
       } else {
         const int half = (nt / 2 + 15) & ~15, first = set * half, last = set ? m_here : min(half, m_here);
-        if (last > first) mx4_leave<DUAL>(p.o, at + first, p.nt, m0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A);
+        if (last > first && DUAL) mx4_leave_gated(p.o, at + first, p.nt, m0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A);
+        else if (last > first) mx4_leave(p.o, at + first, m0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A);
       }
       if (threadIdx.x == READ_WARP * 32) *ok_flag = 1;
     }
@@ -213,8 +214,8 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   if (warp == 1) tmem_dealloc(acc, p.tmem_cols);
   if (p.share > 1) {
     const float* sums = reinterpret_cast<const float*>(smem);
-    mx4_join<DUAL>(p.o, sums, p.nt, m0, m_here, n0, rank, p.share, *ok_flag != 0);
-    if (BLOCKS == 2 && !DUAL) mx4_join<false>(p.o, sums + p.nt * TILE_A, p.nt, m0, m_here, n0 + TILE_A, rank, p.share, *ok_flag != 0 && scaled);
+    mx4_join<false>(p.o, sums, m0, m_here, n0, rank, p.share, *ok_flag != 0, DUAL ? p.nt : 0);
+    if (BLOCKS == 2 && !DUAL) mx4_join<false>(p.o, sums + p.nt * TILE_A, m0, m_here, n0 + TILE_A, rank, p.share, *ok_flag != 0 && scaled);
   }
 }
 

@@ -84,45 +84,67 @@ __device__ __forceinline__ void mx4_put(const Mx4Out& o, int m, int n, float y) 
   else ((__nv_bfloat16*)o.out)[at] = __float2bfloat16_rn(y);
 }
 
-// A finished tile: lane `row` (0..127) of tensor memory holds feature n0 + row, columns `at`.. the rows of A from m0 on (of a gated unit
-// the up part's `nt` further on). Alone, they are results; with shares of K in a cluster they go to shared memory, [accumulator][column]
-// [feature], from where every block of the cluster finishes its part of the features (mx4_join).
-template <bool DUAL>
-__device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int nt, int m0, int m_here, int n0, int row, bool alone, float* sums) {
+// A finished tile: lane `row` (0..127) of tensor memory holds weight row `row` of the tile, columns `at`.. the rows of A from m0 on.
+// Alone they are results, features from n0 on; else they go to shared memory, [column][128], for mx4_join.
+__device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, int m_here, int n0, int row, bool alone, float* sums) {
+  for (int c = 0; c < m_here; c += 16) {
+    float v[16];
+    tmem_ld16(at + c, v);
+    if (!alone) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sums[(c + j) * TILE_A + row] = v[j];
+    } else if (n0 + row < o.n) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, v[j]);
+    }
+  }
+}
+// ... with gate and up accumulators `up` columns apart
+__device__ __forceinline__ void mx4_leave_gated(const Mx4Out& o, uint32_t at, int up, int m0, int m_here, int n0, int row, bool alone, float* sums) {
   for (int c = 0; c < m_here; c += 16) {
     float v[16], u[16];
     tmem_ld16(at + c, v);
-    if (DUAL) tmem_ld16(at + nt + c, u);
+    tmem_ld16(at + up + c, u);
     if (!alone) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         sums[(c + j) * TILE_A + row] = v[j];
-        if (DUAL) sums[(nt + c + j) * TILE_A + row] = u[j];
+        sums[(up + c + j) * TILE_A + row] = u[j];
       }
     } else if (n0 + row < o.n) {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, DUAL ? mx4_gate(v[j], u[j]) : v[j]);
+        if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, mx4_gate(v[j], u[j]));
     }
   }
 }
-// The shares' sums in order; all threads of all blocks of the cluster come here.
-template <bool DUAL>
-__device__ __forceinline__ void mx4_join(const Mx4Out& o, const float* sums, int nt, int m0, int m_here, int n0, int rank, int share, bool ok) {
-  mx4_cluster_sync();
-  const int mine = TILE_A / share, r0 = rank * mine;
+// The sums that the blocks of a cluster left, added up in order, each block for its part of the features; a block alone finishes its own.
+// All threads of all blocks of the cluster come here. HALVES: weight rows 64.. of the tile are the up part of rows 0..63; with `up` the
+// up part stands so many columns further on.
+template <bool HALVES>
+__device__ __forceinline__ void mx4_join(const Mx4Out& o, const float* sums, int m0, int m_here, int n0, int rank, int share, bool ok, int up = 0) {
+  if (share > 1) mx4_cluster_sync();
+  const int mine = (HALVES ? TILE_A / 2 : TILE_A) / share, r0 = rank * mine;
+  const int second = HALVES ? TILE_A / 2 : up * TILE_A;
   if (ok) {
     for (int i = threadIdx.x; i < m_here * mine; i += blockDim.x) {
       const int c = i / mine, row = r0 + i - c * mine;
+      const float* at = sums + c * TILE_A + row;
       float v = 0.f, u = 0.f;
-      for (int r = 0; r < share; ++r) {
-        v += mx4_peer_f32(sums + c * TILE_A + row, r);
-        if (DUAL) u += mx4_peer_f32(sums + (nt + c) * TILE_A + row, r);
+      if (share == 1) {
+        v = at[0];
+        if (second) u = at[second];
+      } else {
+        for (int r = 0; r < share; ++r) {
+          v += mx4_peer_f32(at, r);
+          if (second) u += mx4_peer_f32(at + second, r);
+        }
       }
-      if (n0 + row < o.n) mx4_put(o, m0 + c, n0 + row, DUAL ? mx4_gate(v, u) : v);
+      if (n0 + row < o.n) mx4_put(o, m0 + c, n0 + row, second ? mx4_gate(v, u) : v);
     }
   }
-  mx4_cluster_sync();  // until nobody reads these sums any more
+  if (share > 1) mx4_cluster_sync();  // until nobody reads these sums any more
 }
 
 }  // namespace
