@@ -1,5 +1,6 @@
 // The product with a weight in 4 bits: checks of a call, and which form takes it.
 #include "mx4.cuh"
+#include <stdlib.h>
 
 int cuca_gemm_mx4_rows(const CucaMx4Gemm* c);
 int cuca_gemm_mx4_codes(const CucaMx4Gemm* c);
@@ -19,7 +20,7 @@ CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
   try {
     if (c->a_kind == MX4_CODES) return cuca_gemm_mx4_codes(c);
     const bool copied = ((uintptr_t)c->a & 15) == 0 && (c->lda % 8 == 0 || c->m == 1);  // rows that the copy engine takes
-    if (c->a_kind == CUCA_BF16 && copied) return cuca_gemm_mx4_wide(c);
+    if (c->a_kind == CUCA_BF16 && copied && (c->m > 16 || getenv("MXW"))) return cuca_gemm_mx4_wide(c);
     return cuca_gemm_mx4_rows(c);
   } catch (...) {  // the cache of tensor maps may find no memory
     cuca_set_error("gemm_mx4: out of host memory");

@@ -179,16 +179,16 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_con
                                     : *reinterpret_cast<const uint32_t*>(sp + scale_at + s * SCALE_BYTES)) >> (16 * set);
         const uint4 q[2] = {*reinterpret_cast<const uint4*>(codes + (((s * 4 + set * 2) ^ (row & 7)) << 4)),
                             *reinterpret_cast<const uint4*>(codes + (((s * 4 + set * 2 + 1) ^ (row & 7)) << 4))};
-        const Mx4Factor f[2] = {mx4_factor(bytes & 255), mx4_factor((bytes >> 8) & 255)};
         uint32_t r[32];
         auto convert = [&](auto large) {
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
+            const Mx4Factor f = mx4_factor<decltype(large)::value>((bytes >> (8 * b)) & 255);
             const uint32_t words[4] = {q[b].x, q[b].y, q[b].z, q[b].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t t[4];
-              mx4_to_bf16<decltype(large)::value>(words[i], f[b], t);
+              mx4_to_bf16<decltype(large)::value>(words[i], f, t);
 #pragma unroll
               for (int j = 0; j < 4; ++j) r[b * 16 + i * 4 + j] = t[j];
             }

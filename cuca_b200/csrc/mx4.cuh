@@ -81,8 +81,10 @@ __device__ __forceinline__ uint32_t mx4_mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// 2^(e - 1) = `first` for e up to 128; above, times `second`
+// 2^(e - 1) for e below 128, as `first`; LARGE: any byte, 2^127 and the rest as `second`
+template <bool LARGE>
 __device__ __forceinline__ Mx4Factor mx4_factor(uint32_t e) {
+  if (!LARGE) return {e * 0x00800080u + 126u * 0x00800080u, 0u};
   const uint32_t f = e == 255 ? 0x7fffu : (min(e, 128u) + 126u) << 7;
   const uint32_t s = e > 128 && e < 255 ? (e - 1u) << 7 : 0x3f80u;  // 2^(e - 128)
   return {f | f << 16, s | s << 16};

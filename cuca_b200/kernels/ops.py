@@ -7,6 +7,7 @@ back to torch operators.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 from dataclasses import dataclass
@@ -1897,11 +1898,19 @@ MX4_BLOCK, MX4_STEP, MX4_TILE = 32, 128, 128  # values of a scale; values and ro
 _MX4_ROWS, _MX4_GEMM = struct.Struct("8q"), struct.Struct("17q")
 
 
+@functools.lru_cache(maxsize=4096)
+def _mx4_layout(rows: int, cols: int) -> tuple:
+    """(bytes of a row of codes, steps of a row, bytes of all codes, rounded up to 256, bytes of all)."""
+    steps = -(-cols // MX4_STEP)
+    codes = -(-rows * steps * 64 // 256) * 256
+    return steps * 64, steps, codes, codes + -(-rows // MX4_TILE) * steps * 512
+
+
 class Mx4Matrix:
     """Rows in microscaled 4-bit floating point: every 32 values of a row are codes of 4 bits (a sign and one of 0, 1/2, 1, 3/2,
     2, 3, 4, 6) and a byte for a power of two (`csrc/mx4.cuh`). Made by `mx4_quantise`; `shape` is that of the values."""
 
-    __slots__ = ("shape", "codes", "scales", "_at")
+    __slots__ = ("shape", "device_index", "_memory", "_codes", "_scales", "_at")
 
     def __init__(self, rows: int, cols: int, codes: torch.Tensor, scales: torch.Tensor):
         steps = -(-cols // MX4_STEP)
@@ -1913,42 +1922,74 @@ class Mx4Matrix:
             raise library.KernelError("codes and scales in 4 bits are contiguous bytes")
         if codes.device != scales.device:
             raise library.KernelError(f"codes on {codes.device}, scales on {scales.device}")
-        self.shape, self.codes, self.scales = torch.Size((rows, cols)), codes, scales
+        self.shape, self._memory, self._codes, self._scales = (rows, cols), None, codes, scales
+        self.device_index = codes.get_device()
         self._at = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Mx4Matrix":
-        """Memory for so many rows."""
-        steps = -(-cols // MX4_STEP)
-        return cls(rows, cols, torch.empty(rows, steps * MX4_STEP // 2, dtype=torch.uint8, device=device),
-                   torch.empty(-(-rows // MX4_TILE), steps, 32, 4, 4, dtype=torch.uint8, device=device))
+        """Memory for so many rows, in one piece."""
+        if cols < 1:
+            raise library.KernelError("rows in 4 bits hold one value at least")
+        self = cls.__new__(cls)
+        _, _, codes, total = _mx4_layout(rows, cols)
+        memory = torch.empty(total, dtype=torch.uint8, device=device)
+        at = memory.data_ptr()
+        self.shape, self._memory, self._codes, self._scales = (rows, cols), memory, None, None
+        self.device_index, self._at = memory.get_device(), (at, at + codes)
+        return self
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """uint8 [rows, steps of 128 values * 64]."""
+        if self._codes is None:
+            row, _, _, _ = _mx4_layout(*self.shape)
+            self._codes = self._memory[:self.shape[0] * row].view(self.shape[0], row)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """uint8 [tiles of 128 rows, steps, 32, 4, 4]."""
+        if self._scales is None:
+            _, steps, codes, _ = _mx4_layout(*self.shape)
+            self._scales = self._memory[codes:].view(-(-self.shape[0] // MX4_TILE), steps, 32, 4, 4)
+        return self._scales
 
     @property
     def device(self):
-        return self.codes.device
+        return (self._codes if self._memory is None else self._memory).device
 
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
 
 
-def _here(*tensors) -> None:
-    """Refuses tensors that are not on the current device: a launch goes to its stream."""
-    _cuda(*tensors)
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise library.KernelError(f"kernel arguments on {t.device}, but the current device is cuda:{here}")
+def _here(*devices) -> int:
+    """The current device, which all of the given device numbers have to be: a launch goes to its stream."""
+    here = torch.cuda.current_device() if devices[0] >= 0 else -1
+    for d in devices:
+        if d != here or d < 0:
+            if d < 0:
+                raise library.KernelError("kernel arguments must live on the CUDA device (there is no CPU path)")
+            raise library.KernelError(f"kernel arguments on cuda:{d}, but the current device is cuda:{here}")
+    return here
+
+
+def _stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _rows(t, what: str) -> int:
     """The stride of a tensor's rows, whose values lie next to each other."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise library.KernelError(f"{what} are a matrix whose rows have no gaps, not {tuple(t.shape)} with strides {t.stride()}")
-    if t.shape[0] <= 1:
-        return max(t.shape[1], 1)
-    if t.stride(0) < t.shape[1]:
-        raise library.KernelError(f"{what} overlap: strides {t.stride()}")
-    return t.stride(0)
+    shape = t.shape
+    if len(shape) == 2:
+        rows, cols = shape
+        ld, one = t.stride()
+        if one == 1 or cols <= 1:
+            if rows <= 1:
+                return cols or 1
+            if ld >= cols:
+                return ld
+    raise library.KernelError(f"{what} are a matrix whose rows have no gaps and do not overlap, not {tuple(shape)} with strides {t.stride()}")
 
 
 def mx4_quantise(x, out: Mx4Matrix | None = None) -> Mx4Matrix:
@@ -1956,56 +1997,66 @@ def mx4_quantise(x, out: Mx4Matrix | None = None) -> Mx4Matrix:
     rounded to the nearest, ties to the even code, at most 6. A block that is not finite reads back as NaN. `out`: memory to
     use (of rows of the same shape)."""
     ld = _rows(x, "rows to be quantised")
-    if x.shape[1] < 1:
-        raise library.KernelError("rows to be quantised hold no values")
+    rows, cols = x.shape
+    device = x.get_device()
     if out is None:
-        out = Mx4Matrix.empty(*x.shape, x.device)
-    elif out.shape != x.shape:
-        raise library.KernelError(f"rows {tuple(x.shape)} do not fit memory for {tuple(out.shape)}")
-    _here(x, out.codes, out.scales)
+        _here(device)
+        out = Mx4Matrix.empty(rows, cols, x.device)
+    elif out.shape != (rows, cols):
+        raise library.KernelError(f"rows {tuple(x.shape)} do not fit memory for {out.shape}")
+    else:
+        _here(device, out.device_index)
+    at = out._at
     library.check(library.load().cuca_mx4_quantise(_MX4_ROWS.pack(
-        x.data_ptr(), ld, dtype_code(x.dtype), *out._at, *x.shape, _stream())), "mx4_quantise")
+        x.data_ptr(), ld, dtype_code(x.dtype), at[0], at[1], rows, cols, _stream_of(device))), "mx4_quantise")
     return out
 
 
 def mx4_values(a: Mx4Matrix, out) -> None:
     """out (32 or 16 bits) = the values that rows in 4 bits stand for, exactly."""
     ld = _rows(out, "values")
-    if out.shape != a.shape:
-        raise library.KernelError(f"values of {tuple(a.shape)} rows in 4 bits do not fit {tuple(out.shape)}")
-    _here(out, a.codes, a.scales)
+    if tuple(out.shape) != a.shape:
+        raise library.KernelError(f"values of {a.shape} rows in 4 bits do not fit {tuple(out.shape)}")
+    device = _here(out.get_device(), a.device_index)
     library.check(library.load().cuca_mx4_values(_MX4_ROWS.pack(
-        out.data_ptr(), ld, dtype_code(out.dtype), *a._at, *a.shape, _stream())), "mx4_values")
+        out.data_ptr(), ld, dtype_code(out.dtype), *a._at, *a.shape, _stream_of(device))), "mx4_values")
 
 
 def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> None:
     """out = epilogue(a @ w.T) with a weight in 4 bits; `a`: [M, K] rows of 16 or 32 bits (of any stride and alignment) as they are, or
     rows in 4 bits. Products are exact and summed in 32 bits. `epilogue`: EPI_STORE (plus `bias`; `out` 32-bit, or bfloat16 where
     `a` is not 32-bit), EPI_RESIDUAL (added to a 32-bit `out`, with `bias`), EPI_SWIGLU (silu(g) u of the stacked gate and up rows
-    of `w`). `bias` is 32-bit with 32-bit rows, else bfloat16."""
+    of `w`). `bias` is 32-bit with 32-bit rows, else bfloat16. `out` must not overlap what is read."""
     M, K = a.shape
-    N = w.shape[0]
+    N, wk = w.shape
     if epilogue == EPI_SWIGLU:
         if N % 2 or bias is not None:
             raise library.KernelError("a gated unit takes as many gate rows as up rows, and no bias")
         N //= 2
-    if w.shape[1] != K or out.dim() != 2 or out.shape[0] != M or out.shape[1] != N:
-        raise library.KernelError(f"rows {tuple(a.shape)} times a weight {tuple(w.shape)} do not make {tuple(out.shape)}")
+    if wk != K or tuple(out.shape) != (M, N):
+        raise library.KernelError(f"rows {tuple(a.shape)} times a weight {w.shape} do not make {tuple(out.shape)}")
     ldo = _rows(out, "results")
-    if isinstance(a, Mx4Matrix):
+    if type(a) is Mx4Matrix:
         a_at, a_scales = a._at
-        kind, lda, f32 = 2, 0, False
-        _here(a.codes, w.codes, out, bias, err)
+        kind, lda, device = 2, 0, a.device_index
     else:
-        a_at, a_scales, kind, lda = a.data_ptr(), 0, dtype_code(a.dtype), _rows(a, "rows")
-        f32 = kind == F32
-        _here(a, w.codes, out, bias, err)
-    out_f32 = out.dtype == torch.float32
-    if not out_f32 and (f32 or epilogue == EPI_RESIDUAL or out.dtype != torch.bfloat16):
-        raise library.KernelError(f"gemm_mx4: results in {out.dtype}")
-    if bias is not None and (bias.dtype != (torch.float32 if f32 else torch.bfloat16) or bias.shape != (N,)
-                             or not bias.is_contiguous()):
-        raise library.KernelError(f"gemm_mx4: a bias is {N} numbers of the compute type without gaps, not {tuple(bias.shape)} in {bias.dtype}")
+        a_at, a_scales, kind, lda, device = a.data_ptr(), 0, dtype_code(a.dtype), _rows(a, "rows"), a.get_device()
+    _here(device, w.device_index, out.get_device())
+    f32, out_dtype = kind == F32, out.dtype
+    out_f32 = out_dtype is torch.float32
+    if not out_f32 and (f32 or epilogue == EPI_RESIDUAL or out_dtype is not torch.bfloat16):
+        raise library.KernelError(f"gemm_mx4: results in {out_dtype}")
+    bias_at = err_at = 0
+    if bias is not None:
+        if bias.dtype != (torch.float32 if f32 else torch.bfloat16) or bias.shape != (N,) or not bias.is_contiguous():
+            raise library.KernelError(f"gemm_mx4: a bias is {N} numbers of the compute type without gaps, not {tuple(bias.shape)} in "
+                                      f"{bias.dtype}")
+        _here(bias.get_device())
+        bias_at = bias.data_ptr()
+    if err is not None:
+        err_at = err.data_ptr()
+        if err.get_device() != device or err.dtype is not torch.int32:
+            raise library.KernelError("gemm_mx4: the error word is 32 bits on the device of the rest")
     library.check(library.load().cuca_gemm_mx4(_MX4_GEMM.pack(
-        a_at, a_scales, lda, kind, *w._at, _at(bias), out.data_ptr(), ldo, out_f32, M, N, K, epilogue, 0, _at(err), _stream())),
+        a_at, a_scales, lda, kind, *w._at, bias_at, out.data_ptr(), ldo, out_f32, M, N, K, epilogue, 0, err_at, _stream_of(device))),
         "gemm_mx4")
