@@ -2,14 +2,44 @@
 #include "mx4.cuh"
 #include <stdlib.h>
 
-int cuca_gemm_mx4_rows(const CucaMx4Gemm* c);
-int cuca_gemm_mx4_codes(const CucaMx4Gemm* c);
+int cuca_mx4_digits(const CucaMx4Rows* c);
+int cuca_mx4_align(const void* x, int64_t ldx, void* out, int ldo, int rows, int cols, cudaStream_t stream);
+int cuca_gemm_mx4_codes(const CucaMx4Gemm* c, bool digits);
 int cuca_gemm_mx4_wide(const CucaMx4Gemm* c);
+
+namespace {
+
+// Most bfloat16 rows that go as digits, eight rows in 4 bits each
+int most_digits() { const char* e = getenv("MXD"); return e ? atoi(e) : 32; }
+
+enum Form { CODES, DIGITS, ALIGNED, WIDE };
+
+Form form_of(const CucaMx4Gemm* c) {
+  if (c->a_kind == MX4_CODES) return CODES;
+  if (c->a_kind == CUCA_F32 || c->m <= most_digits()) return DIGITS;
+  return ((uintptr_t)c->a & 15) == 0 && c->lda % 8 == 0 ? WIDE : ALIGNED;  // rows that the copy engine takes
+}
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+int64_t digit_codes(const CucaMx4Gemm* c) { return round256(c->m * MX4_DIGITS * mx4_steps(c->k) * 64); }
+
+int64_t scratch_of(const CucaMx4Gemm* c) {
+  if (c->m <= 0 || c->n <= 0 || c->k <= 0) return 0;
+  switch (form_of(c)) {
+    case DIGITS: return digit_codes(c) + (c->m * MX4_DIGITS + 127) / 128 * mx4_steps(c->k) * 512;
+    case ALIGNED: return c->m * ((c->k + 7) / 8 * 16);
+    default: return 0;
+  }
+}
+
+}  // namespace
+
+// Bytes of scratch that a call needs, by its rows' kind, address and stride and its sizes.
+CUCA_API long long cuca_gemm_mx4_scratch(const CucaMx4Gemm* c) { return scratch_of(c); }
 
 CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
   CUCA_REQUIRE(c->a_kind == CUCA_F32 || c->a_kind == CUCA_BF16 || c->a_kind == MX4_CODES, "gemm_mx4: unknown rows %d", (int)c->a_kind);
   CUCA_REQUIRE(c->epilogue >= EPI_STORE && c->epilogue <= EPI_SWIGLU, "gemm_mx4: unknown epilogue %d", (int)c->epilogue);
-  CUCA_REQUIRE(c->m >= 0 && c->n >= 0 && c->k > 0 && c->m < (1ll << 30) && c->n < (1ll << 29) && c->k < (1ll << 30),
+  CUCA_REQUIRE(c->m >= 0 && c->n >= 0 && c->k > 0 && c->m < (1ll << 27) && c->n < (1ll << 29) && c->k < (1ll << 30),
                "gemm_mx4: %lld x %lld x %lld", (long long)c->m, (long long)c->n, (long long)c->k);
   CUCA_REQUIRE(c->epilogue != EPI_RESIDUAL || c->out_f32, "gemm_mx4: only a 32-bit stream is added to");
   CUCA_REQUIRE(c->epilogue != EPI_SWIGLU || !c->bias, "gemm_mx4: a gated unit takes no bias");
@@ -17,11 +47,24 @@ CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
                (c->a_kind != MX4_CODES || (((uintptr_t)c->a | (uintptr_t)c->a_scales) & 15) == 0),
                "gemm_mx4: codes and scales must start on 16 bytes");
   if (c->m == 0 || c->n == 0) return 0;
+  const Form form = form_of(c);
+  CUCA_REQUIRE((form != DIGITS && form != ALIGNED) || (c->scratch && ((uintptr_t)c->scratch & 255) == 0),
+               "gemm_mx4: these rows need scratch on 256 bytes");
   try {
-    if (c->a_kind == MX4_CODES) return cuca_gemm_mx4_codes(c);
-    const bool copied = ((uintptr_t)c->a & 15) == 0 && (c->lda % 8 == 0 || c->m == 1);  // rows that the copy engine takes
-    if (c->a_kind == CUCA_BF16 && copied && (c->m > 16 || getenv("MXW"))) return cuca_gemm_mx4_wide(c);
-    return cuca_gemm_mx4_rows(c);
+    CucaMx4Gemm d = *c;
+    if (form == DIGITS) {
+      d.a = c->scratch;
+      d.a_scales = (uint8_t*)c->scratch + digit_codes(c);
+      CucaMx4Rows r{const_cast<void*>(c->a), c->lda, c->a_kind, (uint8_t*)c->scratch, const_cast<uint8_t*>(d.a_scales), c->m, c->k, c->stream};
+      if (int e = cuca_mx4_digits(&r)) return e;
+      return cuca_gemm_mx4_codes(&d, true);
+    }
+    if (form == ALIGNED) {
+      d.a = c->scratch;
+      d.lda = (c->k + 7) / 8 * 8;
+      if (int e = cuca_mx4_align(c->a, c->lda, c->scratch, (int)d.lda, (int)c->m, (int)c->k, c->stream)) return e;
+    }
+    return form == CODES ? cuca_gemm_mx4_codes(c, false) : cuca_gemm_mx4_wide(&d);
   } catch (...) {  // the cache of tensor maps may find no memory
     cuca_set_error("gemm_mx4: out of host memory");
     return 3;

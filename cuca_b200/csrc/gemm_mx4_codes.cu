@@ -40,7 +40,7 @@ struct Params {
   int* err;
 };
 
-template <int BLOCKS, bool DUAL, int SPANS>
+template <int BLOCKS, bool DUAL, int SPANS, int G>
 __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
                                                                  const Params p) {
   static_assert(!DUAL || BLOCKS == 2, "gate and up");
@@ -56,7 +56,8 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   const int rank = p.share > 1 ? (int)mx4_cluster_rank() : 0;
   const int tile = (int)blockIdx.x / p.share;
   const int n0 = (tile % p.tiles_n) * (DUAL ? TILE_A : BLOCKS * TILE_A), m0 = (tile / p.tiles_n) * p.nt;
-  const int m_here = min(p.nt, p.o.m - m0), nt = (m_here + 15) & ~15;  // (the last tile multiplies no more columns than it has)
+  const int rows_here = min(p.nt, p.o.m * G - m0), nt = (rows_here + 15) & ~15;  // (the last tile multiplies no more columns than it has)
+  const int t0 = m0 / G, m_here = rows_here / G;  // G rows in 4 bits make one of the result
   const int ks0 = (int)((int64_t)p.k_stages * rank / p.share), ks1 = (int)((int64_t)p.k_stages * (rank + 1) / p.share);
   const int second = DUAL ? p.o.n + n0 : n0 + TILE_A;  // the second block's first weight row
   const bool up_apart = DUAL && (p.o.n & 127);         // the up rows' scales do not start where 128 rows' do
@@ -198,11 +199,14 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
       const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
       float* sums = reinterpret_cast<float*>(smem);  // (every copy into the stages has been waited for)
       if (BLOCKS == 2 && !DUAL) {
-        if (set == 0 || scaled) mx4_leave(p.o, at + set * p.nt, m0, m_here, n0 + set * TILE_A, row, p.share == 1, sums + set * p.nt * TILE_A);
+        if (set == 0 || scaled)
+          mx4_leave<G>(p.o, at + set * p.nt, t0, m_here, n0 + set * TILE_A, row, p.share == 1, sums + set * (p.nt / G) * TILE_A);
       } else {
-        const int half = (nt / 2 + 15) & ~15, first = set * half, last = set ? m_here : min(half, m_here);
-        if (last > first && DUAL) mx4_leave_gated(p.o, at + first, p.nt, m0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A);
-        else if (last > first) mx4_leave(p.o, at + first, m0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A);
+        const int half = ((nt / 2 + 15) & ~15) / G, first = set * half, last = set ? m_here : min(half, m_here);
+        if (last > first && DUAL)
+          mx4_leave_gated<G>(p.o, at + first * G, p.nt, t0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A, p.nt / G);
+        else if (last > first)
+          mx4_leave<G>(p.o, at + first * G, t0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A);
       }
       if (threadIdx.x == READ_WARP * 32) *ok_flag = 1;
     }
@@ -214,25 +218,26 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   if (warp == 1) tmem_dealloc(acc, p.tmem_cols);
   if (p.share > 1) {
     const float* sums = reinterpret_cast<const float*>(smem);
-    mx4_join<false>(p.o, sums, m0, m_here, n0, rank, p.share, *ok_flag != 0, DUAL ? p.nt : 0);
-    if (BLOCKS == 2 && !DUAL) mx4_join<false>(p.o, sums + p.nt * TILE_A, m0, m_here, n0 + TILE_A, rank, p.share, *ok_flag != 0 && scaled);
+    mx4_join<false>(p.o, sums, t0, m_here, n0, rank, p.share, *ok_flag != 0, DUAL ? p.nt / G : 0);
+    if (BLOCKS == 2 && !DUAL) mx4_join<false>(p.o, sums + (p.nt / G) * TILE_A, t0, m_here, n0 + TILE_A, rank, p.share, *ok_flag != 0 && scaled);
   }
 }
 
-template <int BLOCKS, bool DUAL, int SPANS>
+template <int BLOCKS, bool DUAL, int SPANS, int G>
 int launch_spans(const CucaMx4Gemm* c) {
+  const int64_t m = c->m * G;  // rows in 4 bits
   Params p;
   p.a_scales = c->a_scales; p.w_scales = c->w_scales;
-  p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, 0};
+  p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, G > 1 && c->a_kind == CUCA_F32};
   p.k_steps = (int)mx4_steps(c->k);
   p.k_stages = (p.k_steps + STAGE_STEPS - 1) / STAGE_STEPS;
   p.err = c->err;
   const int most = BLOCKS == 2 ? MANY_TILE : MANY_ROWS;
-  p.nt = c->m >= most ? most : ((int)c->m + 15) / 16 * 16;
-  p.a_tiles = (int)((c->m + 127) / 128);
+  p.nt = m >= most ? most : ((int)m + 15) / 16 * 16;
+  p.a_tiles = (int)((m + 127) / 128);
   const int features = DUAL ? TILE_A : BLOCKS * TILE_A;
   p.tiles_n = (int)((c->n + features - 1) / features);
-  const int64_t tiles = (int64_t)p.tiles_n * ((c->m + p.nt - 1) / p.nt);
+  const int64_t tiles = (int64_t)p.tiles_n * ((m + p.nt - 1) / p.nt);
   CUCA_REQUIRE(tiles * MAX_CLUSTER < (1ll << 31), "gemm_mx4: %lld rows by %lld features are too many", (long long)c->m, (long long)c->n);
   p.stage_bytes = BLOCKS * (W_BYTES + STAGE_STEPS * SCALE_BYTES) + p.nt * STAGE_BYTES_K + SPANS * STAGE_STEPS * SCALE_BYTES;
   const bool two = p.nt * BLOCKS <= 64;  // blocks an SM
@@ -244,15 +249,15 @@ int launch_spans(const CucaMx4Gemm* c) {
   p.tmem_cols = 32;
   while (p.tmem_cols < BLOCKS * p.nt + p.stages * stage_cols) p.tmem_cols *= 2;
   CUCA_REQUIRE(p.stages >= 1 && p.tmem_cols <= (two ? 256 : 512), "gemm_mx4: no room for a tile");
-  const int slots = cuca_device_sms() * (two ? 2 : 1), sums = BLOCKS * p.nt * TILE_A * 4;
+  const int slots = cuca_device_sms() * (two ? 2 : 1), sums = BLOCKS * p.nt / G * TILE_A * 4;
   p.share = 1;
   while (p.share < MAX_CLUSTER && tiles * p.share * 2 <= slots && p.k_stages >= p.share * 4 && sums <= p.stages * p.stage_bytes) p.share *= 2;
   const int smem = p.stages * p.stage_bytes + 1024 + BARRIERS;
   CUtensorMap tm_w, tm_a;
   const uint64_t cols = (uint64_t)p.k_steps * 32;  // the codes as 16-bit elements
   CUCA_REQUIRE(cuca_tensor_map_2d(c->w, 2, (uint64_t)c->n * (DUAL ? 2 : 1), cols, cols, TILE_A, &tm_w) &&
-               cuca_tensor_map_2d(c->a, 2, (uint64_t)c->m, cols, cols, p.nt, &tm_a), "gemm_mx4: tensor map failed");
-  constexpr auto kernel = gemm_mx4_codes_kernel<BLOCKS, DUAL, SPANS>;
+               cuca_tensor_map_2d(c->a, 2, (uint64_t)m, cols, cols, p.nt, &tm_a), "gemm_mx4: tensor map failed");
+  constexpr auto kernel = gemm_mx4_codes_kernel<BLOCKS, DUAL, SPANS, G>;
   if (int e = mx4_configure<kernel>(227 * 1024)) return e;
   const dim3 grid((unsigned)(tiles * p.share));
   if (p.share > 1) cuca_launch_cluster(kernel, grid, dim3(THREADS), smem, c->stream, true, p.share, tm_w, tm_a, p);
@@ -261,15 +266,16 @@ int launch_spans(const CucaMx4Gemm* c) {
   return 0;
 }
 
-// a tile of more than 128 rows, or one that starts in the middle of 128, touches the scales of two runs of 128 rows
-template <int BLOCKS, bool DUAL>
+template <int G>
 int launch(const CucaMx4Gemm* c) {
-  return c->m > 128 ? launch_spans<BLOCKS, DUAL, 2>(c) : launch_spans<BLOCKS, DUAL, 1>(c);
+  const int64_t m = c->m * G;
+  // a tile of more than 128 rows, or one that starts in the middle of 128, touches the scales of two runs of 128 rows
+  if (c->epilogue == EPI_SWIGLU) return m > 128 ? launch_spans<2, true, 2, G>(c) : launch_spans<2, true, 1, G>(c);
+  if (m > MANY_ROWS) return launch_spans<2, false, 2, G>(c);
+  return m > 128 ? launch_spans<1, false, 2, G>(c) : launch_spans<1, false, 1, G>(c);
 }
 
 }  // namespace
 
-int cuca_gemm_mx4_codes(const CucaMx4Gemm* c) {
-  if (c->epilogue == EPI_SWIGLU) return launch<2, true>(c);
-  return c->m > MANY_ROWS ? launch_spans<2, false, 2>(c) : launch<1, false>(c);
-}
+// `digits`: A holds MX4_DIGITS rows for each of c->m
+int cuca_gemm_mx4_codes(const CucaMx4Gemm* c, bool digits) { return digits ? launch<MX4_DIGITS>(c) : launch<1>(c); }

@@ -105,6 +105,77 @@ __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams 
     *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(row, run >> 4, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
 }
 
+// Rows of 16 or 32 bits as eight rows in 4 bits each, whose values add up to theirs: digits of three bits. With a = max |r| of what is
+// left of a block (first the block itself),
+//
+//   e = max(ceil(log2 a) - 1, -126),   d = r / 2^e rounded to a multiple of 1/2 (at most 2 in magnitude),   r <- r - d 2^e,
+//
+// every step exact. What is left after a digit is at most 2^(e-2), so e falls by three or more a digit, and after eight what is left of a
+// value is at most 2^-23 of its block's largest: of bfloat16 numbers nothing, where they are within 2^14 of it, and where some are
+// much larger than the rest the digits that these do not need go to the others. A block that is not finite becomes NaN whole.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int runs = p.steps * (MX4_STEP / RUN);
+  const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+  const int64_t in = (uint32_t)i / (uint32_t)runs;
+  const int run = (int)((uint32_t)i - (uint32_t)in * (uint32_t)runs);
+  const bool live = in < p.rows;
+  const int64_t row = p.first + (live ? in : 0);
+  Eight<T> e;
+#pragma unroll
+  for (int j = 0; j < RUN; ++j) e.v[j] = 0.f;
+  if (live) e = load8<T>(p, row, run * RUN);
+#pragma unroll
+  for (int t = 0; t < MX4_DIGITS; ++t) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) most = max(most, magnitude(e.v[j]));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    uint32_t byte = 255, word = 0;
+    if (most < 0x7f800000u) {
+      const int up = (int)(most >> 23) - ((most & 0x7fffffu) ? 0 : 1);
+      byte = max(up, 1);
+      const float by = __uint_as_float((255u - byte) << 23), back = mx4_power(byte) * 0.5f;  // 2^(1-e), 2^(e-1)
+#pragma unroll
+      for (int j = 0; j < RUN; ++j) {
+        const float d = rintf(e.v[j] * by);  // halves: -4 .. 4, whose magnitudes are their codes
+        const uint32_t code = (uint32_t)fabsf(d) | (d < 0.f ? 8u : 0u);
+        word |= code << (4 * ((j >> 1) + (j & 1) * 4));
+        e.v[j] = fmaf(-d, back, e.v[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < RUN; ++j) e.v[j] = 0.f;
+    }
+    const uint32_t s1 = __shfl_down_sync(0xffffffffu, byte, 4), s2 = __shfl_down_sync(0xffffffffu, byte, 8),
+                   s3 = __shfl_down_sync(0xffffffffu, byte, 12);
+    if (live) {
+      const int64_t r = row * MX4_DIGITS + t;
+      *reinterpret_cast<uint32_t*>(p.codes + r * (p.steps * 64ll) + run * 4) = word;
+      if ((run & 15) == 0)
+        *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(r, run >> 4, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
+    }
+  }
+}
+
+// bfloat16 rows of any stride and alignment into rows that start on 16 bytes, the rest of a row zeros (for the copy engine)
+__global__ void __launch_bounds__(THREADS) mx4_align_kernel(const __nv_bfloat16* x, int64_t ldx, __nv_bfloat16* out, int ldo, int cols) {
+  pdl_trigger();
+  pdl_wait();
+  const __nv_bfloat16* src = x + blockIdx.x * ldx;
+  __nv_bfloat16* dst = out + (int64_t)blockIdx.x * ldo;
+  for (int c = threadIdx.x * RUN; c < ldo; c += THREADS * RUN) {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < RUN; ++j)
+      if (c + j < cols) w[j >> 1] |= (uint32_t)__ldcg(reinterpret_cast<const unsigned short*>(src) + c + j) << (16 * (j & 1));
+    *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS) mx4_values_kernel(const RowsParams p) {
   pdl_trigger();
@@ -141,23 +212,27 @@ __global__ void __launch_bounds__(THREADS) mx4_values_kernel(const RowsParams p)
   }
 }
 
-int launch_rows(const CucaMx4Rows* c, bool quantise) {
-  const char* what = quantise ? "mx4_quantise" : "mx4_values";
+enum Form { QUANTISE, VALUES, DIGITS };
+
+int launch_rows(const CucaMx4Rows* c, Form form) {
+  const char* what = form == QUANTISE ? "mx4_quantise" : form == VALUES ? "mx4_values" : "gemm_mx4";
   CUCA_REQUIRE(c->dtype == CUCA_F32 || c->dtype == CUCA_BF16, "%s: unknown dtype %d", what, (int)c->dtype);
   CUCA_REQUIRE(c->rows >= 0 && c->cols > 0 && c->cols < (1ll << 30), "%s: %lld rows of %lld values", what, (long long)c->rows, (long long)c->cols);
   CUCA_REQUIRE(c->ldx >= c->cols || c->rows <= 1, "%s: rows overlap", what);
   CUCA_REQUIRE((((uintptr_t)c->codes | (uintptr_t)c->scales) & 15) == 0, "%s: codes and scales must start on 16 bytes", what);
   const int64_t elem = c->dtype == CUCA_F32 ? 4 : 2, steps = mx4_steps(c->cols);
-  const int64_t runs = quantise ? steps * (MX4_STEP / RUN) : (c->cols + RUN - 1) / RUN;
+  const int64_t runs = form == VALUES ? (c->cols + RUN - 1) / RUN : steps * (MX4_STEP / RUN);
   RowsParams p{c->x, c->x, c->codes, c->scales, c->ldx, 0, 0, (int)c->cols, (int)steps, false};
   p.wide = ((uintptr_t)c->x & 15) == 0 && (c->ldx * elem % 16 == 0 || c->rows == 1);
+  const bool f32 = c->dtype == CUCA_F32;
+  auto kernel = form == QUANTISE ? (f32 ? mx4_quantise_kernel<float> : mx4_quantise_kernel<__nv_bfloat16>)
+                : form == VALUES ? (f32 ? mx4_values_kernel<float> : mx4_values_kernel<__nv_bfloat16>)
+                                 : (f32 ? mx4_digits_kernel<float> : mx4_digits_kernel<__nv_bfloat16>);
   const int64_t most = (1ll << 31) / runs;  // rows of a launch
   for (int64_t at = 0; at < c->rows; at += most) {
     p.first = at;
     p.rows = c->rows - at < most ? c->rows - at : most;
     const dim3 grid((unsigned)((p.rows * runs + THREADS - 1) / THREADS));
-    auto kernel = quantise ? (c->dtype == CUCA_F32 ? mx4_quantise_kernel<float> : mx4_quantise_kernel<__nv_bfloat16>)
-                           : (c->dtype == CUCA_F32 ? mx4_values_kernel<float> : mx4_values_kernel<__nv_bfloat16>);
     cuca_launch(kernel, grid, dim3(THREADS), 0, c->stream, true, p);
     CUCA_CHECK_LAUNCH(what);
   }
@@ -166,5 +241,11 @@ int launch_rows(const CucaMx4Rows* c, bool quantise) {
 
 }  // namespace
 
-CUCA_API int cuca_mx4_quantise(const CucaMx4Rows* c) { return launch_rows(c, true); }
-CUCA_API int cuca_mx4_values(const CucaMx4Rows* c) { return launch_rows(c, false); }
+CUCA_API int cuca_mx4_quantise(const CucaMx4Rows* c) { return launch_rows(c, QUANTISE); }
+CUCA_API int cuca_mx4_values(const CucaMx4Rows* c) { return launch_rows(c, VALUES); }
+int cuca_mx4_digits(const CucaMx4Rows* c) { return launch_rows(c, DIGITS); }
+int cuca_mx4_align(const void* x, int64_t ldx, void* out, int ldo, int rows, int cols, cudaStream_t stream) {
+  cuca_launch(mx4_align_kernel, dim3(rows), dim3(THREADS), 0, stream, true, (const __nv_bfloat16*)x, ldx, (__nv_bfloat16*)out, ldo, cols);
+  CUCA_CHECK_LAUNCH("gemm_mx4");
+  return 0;
+}

@@ -76,6 +76,8 @@ struct Mx4Out {
   int m, n, out_f32, epilogue, bias_f32;
 };
 __device__ __forceinline__ float mx4_gate(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// silu(g) u: for bfloat16 results the approximate quotient and exponential, good to 2^-20
+__device__ __forceinline__ float mx4_gate(const Mx4Out& o, float g, float u) { return o.out_f32 ? g / (1.f + expf(-g)) * u : mx4_gate(g, u); }
 __device__ __forceinline__ void mx4_put(const Mx4Out& o, int m, int n, float y) {
   if (o.bias) y += o.bias_f32 ? ((const float*)o.bias)[n] : __bfloat162float(((const __nv_bfloat16*)o.bias)[n]);
   const int64_t at = m * o.ldo + n;
@@ -84,44 +86,59 @@ __device__ __forceinline__ void mx4_put(const Mx4Out& o, int m, int n, float y) 
   else ((__nv_bfloat16*)o.out)[at] = __float2bfloat16_rn(y);
 }
 
-// A finished tile: lane `row` (0..127) of tensor memory holds weight row `row` of the tile, columns `at`.. the rows of A from m0 on.
-// Alone they are results, features from n0 on; else they go to shared memory, [column][128], for mx4_join.
+// Sixteen columns of this thread's lane as 16 / G results: G columns are one row of A (its digits, the smallest added first).
+template <int G>
+__device__ __forceinline__ void mx4_take16(uint32_t at, float (&y)[16 / G]) {
+  float v[16];
+  tmem_ld16(at, v);
+#pragma unroll
+  for (int i = 0; i < 16 / G; ++i) {
+    y[i] = v[i * G + G - 1];
+#pragma unroll
+    for (int j = G - 2; j >= 0; --j) y[i] += v[i * G + j];
+  }
+}
+// A finished tile: lane `row` (0..127) of tensor memory holds weight row `row` of the tile, G columns `at`.. each of the m_here rows of A
+// from m0 on. Alone they are results, features from n0 on; else they go to shared memory, [row of A][128], for mx4_join.
+template <int G>
 __device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, int m_here, int n0, int row, bool alone, float* sums) {
-  for (int c = 0; c < m_here; c += 16) {
-    float v[16];
-    tmem_ld16(at + c, v);
+  for (int c = 0; c < m_here; c += 16 / G) {
+    float v[16 / G];
+    mx4_take16<G>(at + c * G, v);
     if (!alone) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sums[(c + j) * TILE_A + row] = v[j];
+      for (int j = 0; j < 16 / G; ++j) sums[(c + j) * TILE_A + row] = v[j];
     } else if (n0 + row < o.n) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
+      for (int j = 0; j < 16 / G; ++j)
         if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, v[j]);
     }
   }
 }
-// ... with gate and up accumulators `up` columns apart
-__device__ __forceinline__ void mx4_leave_gated(const Mx4Out& o, uint32_t at, int up, int m0, int m_here, int n0, int row, bool alone, float* sums) {
-  for (int c = 0; c < m_here; c += 16) {
-    float v[16], u[16];
-    tmem_ld16(at + c, v);
-    tmem_ld16(at + up + c, u);
+// ... with gate and up accumulators `apart` columns apart, in shared memory `up` rows
+template <int G>
+__device__ __forceinline__ void mx4_leave_gated(const Mx4Out& o, uint32_t at, int apart, int m0, int m_here, int n0, int row, bool alone, float* sums,
+                                                int up) {
+  for (int c = 0; c < m_here; c += 16 / G) {
+    float v[16 / G], u[16 / G];
+    mx4_take16<G>(at + c * G, v);
+    mx4_take16<G>(at + apart + c * G, u);
     if (!alone) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < 16 / G; ++j) {
         sums[(c + j) * TILE_A + row] = v[j];
         sums[(up + c + j) * TILE_A + row] = u[j];
       }
     } else if (n0 + row < o.n) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, mx4_gate(v[j], u[j]));
+      for (int j = 0; j < 16 / G; ++j)
+        if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, mx4_gate(o, v[j], u[j]));
     }
   }
 }
 // The sums that the blocks of a cluster left, added up in order, each block for its part of the features; a block alone finishes its own.
 // All threads of all blocks of the cluster come here. HALVES: weight rows 64.. of the tile are the up part of rows 0..63; with `up` the
-// up part stands so many columns further on.
+// up part stands so many rows of A further on.
 template <bool HALVES>
 __device__ __forceinline__ void mx4_join(const Mx4Out& o, const float* sums, int m0, int m_here, int n0, int rank, int share, bool ok, int up = 0) {
   if (share > 1) mx4_cluster_sync();
@@ -141,7 +158,7 @@ __device__ __forceinline__ void mx4_join(const Mx4Out& o, const float* sums, int
           if (second) u += mx4_peer_f32(at + second, r);
         }
       }
-      if (n0 + row < o.n) mx4_put(o, m0 + c, n0 + row, second ? mx4_gate(v, u) : v);
+      if (n0 + row < o.n) mx4_put(o, m0 + c, n0 + row, second ? mx4_gate(o, v, u) : v);
     }
   }
   if (share > 1) mx4_cluster_sync();  // until nobody reads these sums any more

@@ -197,6 +197,7 @@ _SIGNATURES = {
     "cuca_mx4_quantise": [ctypes.c_char_p],
     "cuca_mx4_values": [ctypes.c_char_p],
     "cuca_gemm_mx4": [ctypes.c_char_p],
+    "cuca_gemm_mx4_scratch": [ctypes.c_char_p],
 }
 
 _lock = threading.Lock()
@@ -228,6 +229,7 @@ def load(verbose: bool = True):
                 raise KernelLibraryError(f"{path} lacks `{name}`: stale build? remove {path.parent}") from e
             fn.restype = c_int
             fn.argtypes = args
+        lib.cuca_gemm_mx4_scratch.restype = ctypes.c_longlong
         _lib = lib
         return lib
 

@@ -2022,6 +2022,9 @@ def mx4_values(a: Mx4Matrix, out) -> None:
         out.data_ptr(), ld, dtype_code(out.dtype), *a._at, *a.shape, _stream_of(device))), "mx4_values")
 
 
+_mx4_scratch: dict = {}
+
+
 def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> None:
     """out = epilogue(a @ w.T) with a weight in 4 bits; `a`: [M, K] rows of 16 or 32 bits (of any stride and alignment) as they are, or
     rows in 4 bits. Products are exact and summed in 32 bits. `epilogue`: EPI_STORE (plus `bias`; `out` 32-bit, or bfloat16 where
@@ -2057,6 +2060,19 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
         err_at = err.data_ptr()
         if err.get_device() != device or err.dtype is not torch.int32:
             raise library.KernelError("gemm_mx4: the error word is 32 bits on the device of the rest")
-    library.check(library.load().cuca_gemm_mx4(_MX4_GEMM.pack(
-        a_at, a_scales, lda, kind, *w._at, bias_at, out.data_ptr(), ldo, out_f32, M, N, K, epilogue, 0, err_at, _stream_of(device))),
-        "gemm_mx4")
+    lib, w_at, w_scales = library.load(), *w._at
+    scratch = None
+    if kind != 2:
+        # what the library makes of the rows first; the answer depends on the address only by where its 16 bytes start
+        key = kind, a_at & 15, lda & 7, M, N > 0, K
+        need = _mx4_scratch.get(key)
+        if need is None:
+            if len(_mx4_scratch) >= 4096:
+                _mx4_scratch.clear()
+            need = _mx4_scratch[key] = lib.cuca_gemm_mx4_scratch(_MX4_GEMM.pack(
+                a_at, 0, lda, kind, w_at, w_scales, 0, 0, ldo, out_f32, M, N, K, epilogue, 0, 0, 0))
+        if need:
+            scratch = torch.empty(need, dtype=torch.uint8, device=a.device)
+    library.check(lib.cuca_gemm_mx4(_MX4_GEMM.pack(
+        a_at, a_scales, lda, kind, w_at, w_scales, bias_at, out.data_ptr(), ldo, out_f32, M, N, K, epilogue, _at(scratch), err_at,
+        _stream_of(device))), "gemm_mx4")

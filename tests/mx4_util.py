@@ -56,9 +56,22 @@ def chain_bound(x, w, additions):
     return additions * 2.0 ** -23 * (x.abs() @ w.abs().T)
 
 
-def product(x, w, epilogue, out_dtype, additions, bias=None, stream=None):
-    """(result, bound on the error) of epilogue(x w^T) over 64-bit rows."""
+def digits_bound(x, w):
+    """How far a product may be off whose rows go as eight digits in 4 bits: what is left of a value is at most 2^-23 of the largest
+    magnitude among its 32."""
+    m, k = x.shape
+    most = torch.zeros(m, -(-k // 32) * 32, dtype=torch.float64, device=x.device)
+    most[:, :k] = x.abs()
+    most = most.view(m, -1, 32).amax(-1, keepdim=True).expand(-1, -1, 32).flatten(1)[:, :k]
+    return 2.0 ** -23 * (most @ w.abs().T)
+
+
+def product(x, w, epilogue, out_dtype, additions, bias=None, stream=None, digits=False):
+    """(result, bound on the error) of epilogue(x w^T) over 64-bit rows. `digits`: the rows go as digits in 4 bits; a value's digits, the
+    first of which may be twice it and the others an eighth of it in all, come to 2.5 of its magnitude at most."""
     y, b = x @ w.T, chain_bound(x, w, additions)
+    if digits:
+        b = 2.5 * b + digits_bound(x, w)
     if epilogue == "swiglu":
         n = y.shape[1] // 2
         g, u, bg, bu = y[:, :n], y[:, n:], b[:, :n], b[:, n:]

@@ -117,10 +117,14 @@ def _operands(kind, m, k, n, seed, x=None, w=None):
     return x, x.double(), q, mx.held(w)
 
 
-def _additions(kind, k):
-    """Additions in a row of one output: the matrix instructions of 16 products, then shares and parts. 32-bit rows: sums of 128
-    products meet the others with rounding."""
-    return (8 + k / 128 if kind == "f32" else k / 16) + 24
+def _additions(k):
+    """Additions in a row of one output: the matrix instructions of 16 products and more, then shares and digits."""
+    return k / 16 + 24
+
+
+def _product(kind, x, w, epilogue, out_dtype, bias=None, stream=None):
+    """(result, bound): rows that are not in 4 bits may go as digits."""
+    return mx.product(x, w, epilogue, out_dtype, _additions(x.shape[1]), bias, stream, digits=kind != "codes")
 
 
 def _check(out, want, bound):
@@ -143,15 +147,15 @@ def test_products(kind, m, k, n):
     for out_dtype in ((F32,) if kind == "f32" else (BF16, F32)):
         out = torch.full((m, n), 7.0, dtype=out_dtype, device="cuda")
         ops.gemm_mx4(a, q, out, err=err)
-        _check(out, *mx.product(x, w, "store", out_dtype, _additions(kind, k)))
+        _check(out, *_product(kind, x, w, "store", out_dtype))
     bias = _rows(1, n, F32 if kind == "f32" else BF16, 5)[0].contiguous()
     out = torch.full((m, n), 7.0, dtype=bias.dtype, device="cuda")
     ops.gemm_mx4(a, q, out, bias=bias, err=err)
-    _check(out, *mx.product(x, w, "store", out.dtype, _additions(kind, k), bias=bias))
+    _check(out, *_product(kind, x, w, "store", out.dtype, bias=bias))
     stream = _rows(m, n, F32, 6)
     out = stream.clone()
     ops.gemm_mx4(a, q, out, ops.EPI_RESIDUAL, bias, err)
-    want, bound = mx.product(x, w, "store", F32, _additions(kind, k), bias=bias, stream=stream)
+    want, bound = _product(kind, x, w, "store", F32, bias=bias, stream=stream)
     _check(out, want, bound)
     assert err.item() == 0
 
@@ -165,7 +169,7 @@ def test_gated_unit(kind, m, k, n):
     err = torch.zeros(1, dtype=torch.int32, device="cuda")
     out = torch.full((m, n), 7.0, dtype=F32 if kind == "f32" else BF16, device="cuda")
     ops.gemm_mx4(a, q, out, ops.EPI_SWIGLU, err=err)
-    _check(out, *mx.product(x, w, "swiglu", out.dtype, _additions(kind, k)))
+    _check(out, *_product(kind, x, w, "swiglu", out.dtype))
     assert err.item() == 0
 
 
@@ -182,7 +186,7 @@ def test_strides(kind, m):
         wide = torch.full((m, n + gap + 9), 7.0, device="cuda")
         out = wide[:, 3 + shift:3 + shift + n]
         ops.gemm_mx4(a, q, out)
-        _check(out, *mx.product(x, w, "store", F32, _additions(kind, k)))
+        _check(out, *_product(kind, x, w, "store", F32))
         assert (wide[:, :3 + shift] == 7).all() and (wide[:, 3 + shift + n:] == 7).all()
 
 
@@ -199,7 +203,26 @@ def test_powers_far_apart(kind, m):
     from cuca_b200.kernels import ops
     out = torch.empty(m, n, device="cuda")
     ops.gemm_mx4(a, q, out)
-    _check(out, *mx.product(x, w, "store", F32, _additions(kind, k)))
+    _check(out, *_product(kind, x, w, "store", F32))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_a_large_value_of_no_weight_beside_small_ones(kind):
+    """Few rows go as eight digits: a value of 2^30 that meets weights of zero leaves the others digits of their own. It has eight
+    significant bits, which three digits hold, four where a digit carries; four are left, and after a digit at most an eighth is."""
+    from cuca_b200.kernels import ops
+    m, k, n = 4, 256, 64
+    x, w = _rows(m, k, BF16, 1, 0.0).float(), _rows(n, k, F32, 2, 0.0)
+    x[:, ::32] = (x[:, ::32] * 2.0 ** 30).to(BF16).float()
+    w[:, ::32] = 0
+    a, xv, q, wv = _operands(kind, m, k, n, 1, x.to(F32 if kind == "f32" else BF16), w)
+    out = torch.empty(m, n, device="cuda")
+    ops.gemm_mx4(a, q, out)
+    rest = xv.clone()
+    rest[:, ::32] = 0
+    most = rest.view(m, -1, 32).abs().amax(-1, keepdim=True).expand(-1, -1, 32).flatten(1)
+    bound = 2.0 ** -11 * (most @ wv.abs().T) + mx.chain_bound(rest, wv, 2.5 * _additions(k))
+    _check(out, xv @ wv.T, bound)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -223,7 +246,7 @@ def test_weights_of_no_size_and_not_finite(kind, m):
     assert torch.equal(out.isnan(), bad)
     good_n = [i for i in range(n) if i not in (7, 140)]
     good_m = [i for i in range(m) if i != 1]
-    want, bound = mx.product(xv[good_m], wv[good_n], "store", F32, _additions(kind, k))
+    want, bound = _product(kind, xv[good_m], wv[good_n], "store", F32)
     _check(out[good_m][:, good_n], want, bound)
 
 
@@ -277,10 +300,10 @@ def test_a_chain_in_a_graph(m):
         graph.replay()
         torch.cuda.synchronize()
         v1, v2 = mx.held(w1), mx.held(w2)
-        _check(act, *mx.product(mx.held(x), v1, "swiglu", BF16, _additions("codes", e)))
-        _check(wide, *mx.product(x.double(), v1, "swiglu", BF16, _additions("bf16", e)))
-        y1, b1 = mx.product(mx.held(act), v2, "store", F32, _additions("codes", f), stream=kept)
-        y2, b2 = mx.product(wide.double(), v2, "store", F32, _additions("bf16", f), stream=y1)
+        _check(act, *_product("codes", mx.held(x), v1, "swiglu", BF16))
+        _check(wide, *_product("bf16", x.double(), v1, "swiglu", BF16))
+        y1, b1 = _product("codes", mx.held(act), v2, "store", F32, stream=kept)
+        y2, b2 = _product("bf16", wide.double(), v2, "store", F32, stream=y1)
         _check(stream, y2, b1 + b2)
 
 
