@@ -1,6 +1,5 @@
 // The product with a weight in 4 bits: checks of a call, and which form takes it.
 #include "mx4.cuh"
-#include <stdlib.h>
 
 int cuca_mx4_digits(const CucaMx4Rows* c);
 int cuca_mx4_align(const void* x, int64_t ldx, void* out, int ldo, int rows, int cols, cudaStream_t stream);
@@ -9,14 +8,16 @@ int cuca_gemm_mx4_wide(const CucaMx4Gemm* c);
 
 namespace {
 
-// Most bfloat16 rows that go as digits, eight rows in 4 bits each
-int most_digits() { const char* e = getenv("MXD"); return e ? atoi(e) : 32; }
+// Most bfloat16 rows that go as digits, eight rows in 4 bits each, where converting the weight takes longer. Measured, K x features, us, digits
+// and converted weight: 4096 x 14336 gated 16 rows 17.3 and 29.2, 24 rows 20.1 and 30.4, 32 rows 28.2 and 30.6; 14336 x 4096 16 rows 15.2
+// and 16.4, 24 rows 16.0 and 17.1, 32 rows 17.9 and 17.4; 4096 x 4096 24 rows 11.3 and 9.3.
+int most_digits(const CucaMx4Gemm* c) { return c->epilogue == EPI_SWIGLU ? 24 : 16; }
 
 enum Form { CODES, DIGITS, ALIGNED, WIDE };
 
 Form form_of(const CucaMx4Gemm* c) {
   if (c->a_kind == MX4_CODES) return CODES;
-  if (c->a_kind == CUCA_F32 || c->m <= most_digits()) return DIGITS;
+  if (c->a_kind == CUCA_F32 || c->m <= most_digits(c)) return DIGITS;
   return ((uintptr_t)c->a & 15) == 0 && c->lda % 8 == 0 ? WIDE : ALIGNED;  // rows that the copy engine takes
 }
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }

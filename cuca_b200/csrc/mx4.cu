@@ -59,12 +59,6 @@ __device__ __forceinline__ Eight<T> load8(const RowsParams& p, int64_t row, int 
   return e;
 }
 
-__device__ __forceinline__ uint32_t code_pair(float lo, float hi) {  // nearest, ties to even, at most 6
-  uint32_t d;
-  asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\ncvt.u32.u8 %0, b;\n}\n" : "=r"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams p) {
   pdl_trigger();
@@ -91,9 +85,9 @@ __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams 
   uint32_t word = 0;
   if (finite) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // bytes hold codes 0 and 2, 4 and 6, 1 and 3, 5 and 7
-      const int i = (j & 1) * 4 + (j >> 1);
-      word |= code_pair(e.v[i] * inv, e.v[i + 2] * inv) << (8 * j);
+    for (int j = 0; j < 4; ++j) {
+      const int i = mx4_first_of(j);
+      word |= mx4_code_pair(e.v[i] * inv, e.v[i + 2] * inv) << (8 * j);
     }
   }
   // the four blocks' bytes, lowest first, by the step's first thread
@@ -105,14 +99,9 @@ __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams 
     *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(row, run >> 4, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
 }
 
-// Rows of 16 or 32 bits as eight rows in 4 bits each, whose values add up to theirs: digits of three bits. With a = max |r| of what is
-// left of a block (first the block itself),
-//
-//   e = max(ceil(log2 a) - 1, -126),   d = r / 2^e rounded to a multiple of 1/2 (at most 2 in magnitude),   r <- r - d 2^e,
-//
-// every step exact. What is left after a digit is at most 2^(e-2), so e falls by three or more a digit, and after eight what is left of a
-// value is at most 2^-23 of its block's largest: of bfloat16 numbers nothing, where they are within 2^14 of it, and where some are
-// much larger than the rest the digits that these do not need go to the others. A block that is not finite becomes NaN whole.
+// Rows of 16 or 32 bits as eight rows in 4 bits each, whose values add up to theirs: digits of three bits (mx4_digit). After eight what is
+// left of a value is at most 2^-23 of its block's largest: of bfloat16 numbers nothing, where they are within 2^14 of it, and where
+// some are much larger than the rest the digits that these do not need go to the others.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p) {
   pdl_trigger();
@@ -129,27 +118,8 @@ __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p)
   if (live) e = load8<T>(p, row, run * RUN);
 #pragma unroll
   for (int t = 0; t < MX4_DIGITS; ++t) {
-    uint32_t most = 0;
-#pragma unroll
-    for (int j = 0; j < RUN; ++j) most = max(most, magnitude(e.v[j]));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    uint32_t byte = 255, word = 0;
-    if (most < 0x7f800000u) {
-      const int up = (int)(most >> 23) - ((most & 0x7fffffu) ? 0 : 1);
-      byte = max(up, 1);
-      const float by = __uint_as_float((255u - byte) << 23), back = mx4_power(byte) * 0.5f;  // 2^(1-e), 2^(e-1)
-#pragma unroll
-      for (int j = 0; j < RUN; ++j) {
-        const float d = rintf(e.v[j] * by);  // halves: -4 .. 4, whose magnitudes are their codes
-        const uint32_t code = (uint32_t)fabsf(d) | (d < 0.f ? 8u : 0u);
-        word |= code << (4 * ((j >> 1) + (j & 1) * 4));
-        e.v[j] = fmaf(-d, back, e.v[j]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < RUN; ++j) e.v[j] = 0.f;
-    }
+    uint32_t byte, word;
+    mx4_digit(e.v, byte, word);
     const uint32_t s1 = __shfl_down_sync(0xffffffffu, byte, 4), s2 = __shfl_down_sync(0xffffffffu, byte, 8),
                    s3 = __shfl_down_sync(0xffffffffu, byte, 12);
     if (live) {

@@ -71,6 +71,50 @@ __device__ __forceinline__ float mx4_power(uint32_t e) {
   return __uint_as_float(e == 255 ? 0x7fffffffu : e ? e << 23 : 1u << 22);
 }
 
+// Two values' codes: to the nearest, ties to even, at most 6; the first in the low half.
+__device__ __forceinline__ uint32_t mx4_code_pair(float lo, float hi) {
+  uint32_t d;
+  asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\ncvt.u32.u8 %0, b;\n}\n" : "=r"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+// The bytes of a word of codes hold values 0 and 2, 4 and 6, 1 and 3, 5 and 7: the first value of byte j
+__host__ __device__ constexpr int mx4_first_of(int j) { return (j & 1) * 4 + (j >> 1); }
+
+// A digit of eight values, a quarter of a block whose other quarters the three neighbouring lanes have. With a = max |v| of the block,
+//
+//   e = max(ceil(log2 a) - 1, -126),   d = v / 2^e rounded to a multiple of 1/2 (at most 2 in magnitude),   v <- v - d 2^e,
+//
+// every step exact. What is left is at most 2^(e-2), so e falls by three or more a digit. A block that is not finite becomes NaN whole.
+__device__ __forceinline__ void mx4_digit(float (&v)[8], uint32_t& byte, uint32_t& word) {
+  float a = 0.f;
+  bool finite = true;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    a = fmaxf(a, fabsf(v[j]));  // (a NaN is passed over)
+    finite = finite && fabsf(v[j]) <= 3.402823466e38f;
+  }
+  uint32_t most = finite ? __float_as_uint(a) : 0x7f800000u;
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+  word = 0;
+  if (most < 0x7f800000u) {
+    byte = max((int)(most >> 23) - ((most & 0x7fffffu) ? 0 : 1), 1);
+    const float down = mx4_power(254 - byte), up = mx4_power(byte);  // 2^-e, 2^e
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      d[j] = __fadd_rn(__fmul_rn(v[j], down), 6291456.f) - 6291456.f;  // 1.5 * 2^22, whose last place is 1/2
+      v[j] = fmaf(-d[j], up, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) word |= mx4_code_pair(d[mx4_first_of(j)], d[mx4_first_of(j) + 2]) << (8 * j);
+  } else {
+    byte = 255;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  }
+}
+
 // Eight codes as bfloat16 numbers times the power of two that a byte stands for, exactly, in their order.
 // A code's sign goes to the sign, its other bits to the lowest exponent bits and the highest mantissa bit, which reads as the
 // magnitude times 2^-126 (1/2 as a number below the normal ones); the factor brings it up and applies the scale at once. Both
