@@ -38,6 +38,9 @@ def main(argv=None) -> int:
     ap.add_argument("--random-weights", type=int, metavar="SEED", help="draw the weights from this seed")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default=None)
     ap.add_argument("--kv-cache-dtype", choices=["int8"], default=None, help="keep keys and values in 8 bits")
+    ap.add_argument("--weight-dtype", choices=["mxfp4"], default=None, help="keep the projections' weights in 4 bits")
+    ap.add_argument("--activation-dtype", choices=["mxfp4"], default=None,
+                    help="bring what enters the projections to 4 bits too (with --weight-dtype)")
     args = ap.parse_args(argv)
 
     from .config.engine_config import LocalModelConfig, RandomWeights
@@ -55,6 +58,10 @@ def main(argv=None) -> int:
         config.dtype = args.dtype
     if args.kv_cache_dtype:
         config.kv_cache_dtype = args.kv_cache_dtype
+    if args.weight_dtype:
+        config.weight_dtype = args.weight_dtype
+    if args.activation_dtype:
+        config.activation_dtype = args.activation_dtype
 
     started = time.perf_counter()
     model = LocalModel.load(config)

@@ -4,7 +4,7 @@
 on one GPU needs (src/provider/local/mod.rs:1762-1915): `source`,
 `context_length`, `sampling` (`SamplingConfig`, :1018-1039) and `batching`
 (`BatchingConfig`, :2234-2277), validated as there (:2587-2608,2741-2757).
-Ours: `dtype`, `kv_block_size`, `kv_cache_dtype` and `random_weights`.
+Ours: `dtype`, `kv_block_size`, `kv_cache_dtype`, `weight_dtype`, `activation_dtype` and `random_weights`.
 """
 from __future__ import annotations
 
@@ -59,6 +59,8 @@ class LocalModelConfig:
     dtype: str = "bfloat16"
     kv_block_size: int = 16
     kv_cache_dtype: Optional[str] = None  # None: keys and values in `dtype`; "int8": in 8 bits, a 32-bit scale per row
+    weight_dtype: Optional[str] = None  # None: projections in `dtype`; "mxfp4": in 4 bits, a power of two per 32 values
+    activation_dtype: Optional[str] = None  # with weights in 4 bits; "mxfp4": what enters the projections is brought to 4 bits too
     random_weights: Optional[RandomWeights] = None  # with `model_config`: weights drawn on the device
     model_config: Optional[dict] = None  # a config.json given inline (random weights only)
     device: str = "cuda:0"
@@ -83,6 +85,12 @@ class LocalModelConfig:
             raise EngineConfigError(f"dtype must be bfloat16 or float32, found {self.dtype}")
         if self.kv_cache_dtype not in (None, "int8"):
             raise EngineConfigError(f"kv_cache_dtype must be int8 or absent, found {self.kv_cache_dtype}")
+        if self.weight_dtype not in (None, "mxfp4"):
+            raise EngineConfigError(f"weight_dtype must be mxfp4 or absent, found {self.weight_dtype}")
+        if self.activation_dtype not in (None, "mxfp4"):
+            raise EngineConfigError(f"activation_dtype must be mxfp4 or absent, found {self.activation_dtype}")
+        if self.activation_dtype is not None and self.weight_dtype is None:
+            raise EngineConfigError("activation_dtype mxfp4 wants weight_dtype mxfp4")
         if self.kv_block_size < 1 or self.kv_block_size & (self.kv_block_size - 1):
             raise EngineConfigError("kv_block_size must be a power of two")
         if (self.source is None) == (self.model_config is None):

@@ -228,7 +228,7 @@ int launch_spans(const CucaMx4Gemm* c) {
   const int64_t m = c->m * G;  // rows in 4 bits
   Params p;
   p.a_scales = c->a_scales; p.w_scales = c->w_scales;
-  p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, G > 1 && c->a_kind == CUCA_F32};
+  p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, (int)c->bias_f32};
   p.k_steps = (int)mx4_steps(c->k);
   p.k_stages = (p.k_steps + STAGE_STEPS - 1) / STAGE_STEPS;
   p.err = c->err;

@@ -230,7 +230,7 @@ int launch(const CucaMx4Gemm* c, int nt) {
   constexpr int CODE_STAGE = CODE_BYTES + (DUAL ? 2 : 1) * STAGE_STEPS * SCALE_BYTES;
   Params p;
   p.w_scales = c->w_scales;
-  p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, 0};
+  p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, (int)c->bias_f32};
   p.k_steps = (int)mx4_steps(c->k);
   p.k_stages = (p.k_steps + STAGE_STEPS - 1) / STAGE_STEPS;
   p.err = c->err;

@@ -33,14 +33,14 @@ struct CucaMx4Gemm {
   int64_t lda, a_kind;
   const uint8_t* w;
   const uint8_t* w_scales;
-  const void* bias;  // of the compute type: 32-bit with 32-bit rows, else bfloat16; or null
+  const void* bias;  // 32-bit where `bias_f32`, else bfloat16; or null
   void* out;
-  int64_t ldo, out_f32, m, n, k, epilogue;
+  int64_t ldo, out_f32, bias_f32, m, n, k, epilogue;
   void* scratch;  // what cuca_gemm_mx4_scratch asked for
   int* err;
   cudaStream_t stream;
 };
-static_assert(sizeof(CucaMx4Rows) == 8 * 8 && sizeof(CucaMx4Gemm) == 17 * 8, "one 64-bit word each");
+static_assert(sizeof(CucaMx4Rows) == 8 * 8 && sizeof(CucaMx4Gemm) == 18 * 8, "one 64-bit word each");
 
 #define MX4_CODES 2
 #define EPI_STORE 0

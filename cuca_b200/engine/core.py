@@ -38,12 +38,19 @@ class EngineCore:
     def __init__(self, spec, source: Optional[WeightSource], dtype=torch.bfloat16, device="cuda:0",
                  context_length: Optional[int] = None, kv_tokens: Optional[int] = None, max_sequences: int = 4,
                  block_size: int = 16, max_step_tokens: Optional[int] = None, window_pools: str = "sized",
-                 random_seed: Optional[int] = None, random_std: float = 0.02, kv_cache_dtype: Optional[str] = None):
+                 random_seed: Optional[int] = None, random_std: float = 0.02, kv_cache_dtype: Optional[str] = None,
+                 weight_dtype: Optional[str] = None, activation_dtype: Optional[str] = None):
+        if weight_dtype not in (None, "mxfp4") or activation_dtype not in (None, "mxfp4"):
+            raise ValueError(f"weights and activations are kept in the compute dtype or in mxfp4, not {weight_dtype}, {activation_dtype}")
+        if activation_dtype is not None and weight_dtype is None:
+            raise ValueError("activations in mxfp4 want weights in mxfp4")
         if kv_cache_dtype not in (None, "int8"):
             raise ValueError(f"keys and values are kept in the compute dtype or in int8, not {kv_cache_dtype}")
         self.spec = spec
-        self.rt = Runtime(device, parse_dtype(dtype))
+        self.rt = Runtime(device, parse_dtype(dtype), weight_dtype is not None, activation_dtype is not None)
         self.model = Model(spec, self.rt)
+        if weight_dtype is not None:
+            self.model.check_small_weights()
         if kv_cache_dtype is not None:
             self.model.check_quantized_cache()
         if source is None:

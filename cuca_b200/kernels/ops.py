@@ -344,8 +344,11 @@ def gemm_pair_mode(mode: int) -> None:
 
 def gemm(a, w, out, epilogue=EPI_STORE, bias=None, err=None) -> None:
     """out = epilogue(a @ w.T), on the kernel that fits dtype and shape: `gemm_tc` for bfloat16 (rows of 16-byte
-    multiples), `gemm_simt` for the 32-bit path and for shapes the former refuses. `w` as in those."""
-    if a.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and (bias is None or bias.dtype == torch.bfloat16) \
+    multiples), `gemm_simt` for the 32-bit path and for shapes the former refuses, `gemm_mx4` for a weight in 4 bits. `w` as in
+    those."""
+    if type(w) is Mx4Matrix:
+        gemm_mx4(a, w, out, epilogue, bias, err)
+    elif a.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and (bias is None or bias.dtype == torch.bfloat16) \
             and gemm_tc_supported(a, w):
         gemm_tc(a, w, out, epilogue, bias, err)
     else:
@@ -796,6 +799,8 @@ def _partial_plan(M: int, N: int, K: int, max_slices: int):
 
 
 def gemm_partial_supported(a, w) -> bool:
+    if type(w) is Mx4Matrix:  # one slice: its kernels add up what they share
+        return (type(a) is Mx4Matrix or a.dtype == torch.bfloat16) and a.shape[0] <= partial_max_tokens()
     return (a.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and a.shape[0] <= partial_max_tokens()
             and gemm_tc_supported(a, w) and _partial_plan(a.shape[0], w.shape[0], a.shape[1], 16)[0] > 0)
 
@@ -806,7 +811,12 @@ _SLICES_WRITTEN_AT = ctypes.addressof(_slices_written)
 
 
 def gemm_partial(a, w, err=None, max_slices=16) -> PartialSums:
-    """a @ w.T for few rows (`partial_max_tokens`), as partial sums over K slices (see `PartialSums`); `w` as in `gemm_tc`."""
+    """a @ w.T for few rows (`partial_max_tokens`), as partial sums over K slices (see `PartialSums`); `w` as in `gemm_tc`, or in 4
+    bits."""
+    if type(w) is Mx4Matrix:
+        data = torch.empty(1, a.shape[0], w.shape[0], dtype=torch.float32, device=w.device)
+        gemm_mx4(a, w, data[0], err=err)
+        return PartialSums(data, 1)
     _cuda(a, w)
     lib = library.load()
     M, K = a.shape
@@ -1895,7 +1905,7 @@ def attention_q8(q, out, pages: QuantizedPages, tables, step, n_heads, n_kv_head
 # ------------------------------------------------------------------ matrices in 4 bits
 MX4_BLOCK, MX4_STEP, MX4_TILE = 32, 128, 128  # values of a scale; values and rows of 512 bytes of scales (`csrc/mx4.cuh`)
 # a call's arguments as 64-bit words (`CucaMx4Rows` and `CucaMx4Gemm` in csrc/mx4.cuh)
-_MX4_ROWS, _MX4_GEMM = struct.Struct("8q"), struct.Struct("17q")
+_MX4_ROWS, _MX4_GEMM = struct.Struct("8q"), struct.Struct("18q")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1959,6 +1969,7 @@ class Mx4Matrix:
     def device(self):
         return (self._codes if self._memory is None else self._memory).device
 
+    @property
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
 
@@ -1978,7 +1989,7 @@ def _stream_of(device: int) -> int:
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _rows(t, what: str) -> int:
+def _mx4_rows(t, what: str) -> int:
     """The stride of a tensor's rows, whose values lie next to each other."""
     shape = t.shape
     if len(shape) == 2:
@@ -1996,7 +2007,7 @@ def mx4_quantise(x, out: Mx4Matrix | None = None) -> Mx4Matrix:
     """Rows of 32 or 16 bits in 4 bits: of every 32 values, with a = max |x|, e = max(floor(log2 a) - 2, -127), codes are x / 2^e
     rounded to the nearest, ties to the even code, at most 6. A block that is not finite reads back as NaN. `out`: memory to
     use (of rows of the same shape)."""
-    ld = _rows(x, "rows to be quantised")
+    ld = _mx4_rows(x, "rows to be quantised")
     rows, cols = x.shape
     device = x.get_device()
     if out is None:
@@ -2014,7 +2025,7 @@ def mx4_quantise(x, out: Mx4Matrix | None = None) -> Mx4Matrix:
 
 def mx4_values(a: Mx4Matrix, out) -> None:
     """out (32 or 16 bits) = the values that rows in 4 bits stand for, exactly."""
-    ld = _rows(out, "values")
+    ld = _mx4_rows(out, "values")
     if tuple(out.shape) != a.shape:
         raise library.KernelError(f"values of {a.shape} rows in 4 bits do not fit {tuple(out.shape)}")
     device = _here(out.get_device(), a.device_index)
@@ -2029,7 +2040,8 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
     """out = epilogue(a @ w.T) with a weight in 4 bits; `a`: [M, K] rows of 16 or 32 bits (of any stride and alignment) as they are, or
     rows in 4 bits. Products are exact and summed in 32 bits. `epilogue`: EPI_STORE (plus `bias`; `out` 32-bit, or bfloat16 where
     `a` is not 32-bit), EPI_RESIDUAL (added to a 32-bit `out`, with `bias`), EPI_SWIGLU (silu(g) u of the stacked gate and up rows
-    of `w`). `bias` is 32-bit with 32-bit rows, else bfloat16. `out` must not overlap what is read."""
+    of `w`). `bias`: 32 or 16 bits. `out` must not overlap what is read. bfloat16 rows are multiplied as they are or, where there are few,
+    as digits that add up to them (`csrc/mx4.cu`), like 32-bit ones; a row that is not finite gives no finite results."""
     M, K = a.shape
     N, wk = w.shape
     if epilogue == EPI_SWIGLU:
@@ -2038,22 +2050,22 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
         N //= 2
     if wk != K or tuple(out.shape) != (M, N):
         raise library.KernelError(f"rows {tuple(a.shape)} times a weight {w.shape} do not make {tuple(out.shape)}")
-    ldo = _rows(out, "results")
+    ldo = _mx4_rows(out, "results")
     if type(a) is Mx4Matrix:
         a_at, a_scales = a._at
         kind, lda, device = 2, 0, a.device_index
     else:
-        a_at, a_scales, kind, lda, device = a.data_ptr(), 0, dtype_code(a.dtype), _rows(a, "rows"), a.get_device()
+        a_at, a_scales, kind, lda, device = a.data_ptr(), 0, dtype_code(a.dtype), _mx4_rows(a, "rows"), a.get_device()
     _here(device, w.device_index, out.get_device())
     f32, out_dtype = kind == F32, out.dtype
     out_f32 = out_dtype is torch.float32
     if not out_f32 and (f32 or epilogue == EPI_RESIDUAL or out_dtype is not torch.bfloat16):
         raise library.KernelError(f"gemm_mx4: results in {out_dtype}")
-    bias_at = err_at = 0
+    bias_at = err_at = bias_f32 = 0
     if bias is not None:
-        if bias.dtype != (torch.float32 if f32 else torch.bfloat16) or bias.shape != (N,) or not bias.is_contiguous():
-            raise library.KernelError(f"gemm_mx4: a bias is {N} numbers of the compute type without gaps, not {tuple(bias.shape)} in "
-                                      f"{bias.dtype}")
+        bias_f32 = dtype_code(bias.dtype) == F32
+        if tuple(bias.shape) != (N,) or not bias.is_contiguous():
+            raise library.KernelError(f"gemm_mx4: a bias is {N} numbers without gaps, not {tuple(bias.shape)}")
         _here(bias.get_device())
         bias_at = bias.data_ptr()
     if err is not None:
@@ -2064,15 +2076,15 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
     scratch = None
     if kind != 2:
         # what the library makes of the rows first; the answer depends on the address only by where its 16 bytes start
-        key = kind, a_at & 15, lda & 7, M, N > 0, K
+        key = kind, a_at & 15, lda & 7, M, N > 0, K, epilogue
         need = _mx4_scratch.get(key)
         if need is None:
             if len(_mx4_scratch) >= 4096:
                 _mx4_scratch.clear()
             need = _mx4_scratch[key] = lib.cuca_gemm_mx4_scratch(_MX4_GEMM.pack(
-                a_at, 0, lda, kind, w_at, w_scales, 0, 0, ldo, out_f32, M, N, K, epilogue, 0, 0, 0))
+                a_at, 0, lda, kind, w_at, w_scales, 0, 0, ldo, out_f32, 0, M, N, K, epilogue, 0, 0, 0))
         if need:
             scratch = torch.empty(need, dtype=torch.uint8, device=a.device)
     library.check(lib.cuca_gemm_mx4(_MX4_GEMM.pack(
-        a_at, a_scales, lda, kind, w_at, w_scales, bias_at, out.data_ptr(), ldo, out_f32, M, N, K, epilogue, _at(scratch), err_at,
+        a_at, a_scales, lda, kind, w_at, w_scales, bias_at, out.data_ptr(), ldo, out_f32, bias_f32, M, N, K, epilogue, _at(scratch), err_at,
         _stream_of(device))), "gemm_mx4")

@@ -1,6 +1,8 @@
 """The generic model: parts built from a `ModelSpec`, run in the order its schedule gives."""
 from __future__ import annotations
 
+from collections import Counter
+
 import torch
 
 from ..kernels import ops
@@ -66,6 +68,13 @@ class Model:
             if block.mixer.cache_needs().kv is not None and not block.mixer.takes_quantized_cache:
                 raise ValueError(f"layer {i}: its mixer (`{block.mixer.spec.kind}`) does not take keys and values in 8 bits")
 
+    def check_small_weights(self) -> None:
+        """Refuses weights in 4 bits where a layer's parts do not take them."""
+        for i, block in enumerate(self.blocks):
+            for what, part in (("mixer", block.mixer), ("feed-forward", block.feed_forward)):
+                if part is not None and not part.takes_small_weights:
+                    raise ValueError(f"layer {i}: its {what} (`{part.spec.kind}`) does not take weights in 4 bits")
+
     def graph_safe(self) -> bool:
         return all(b.graph_safe for b in self.blocks)
 
@@ -80,11 +89,18 @@ class Model:
         self.check_weights(source)
         raw = loader.binder(needs, source, self.rt.device, self.rt.dtype)
         seen: dict = {}
+        # with weights in 4 bits, a tensor that no further part asks for is not kept beside what was made of it
+        users = Counter(name for part in self.parts() for name in part.tensors()) if self.rt.small_weights else None
 
         def get(name):
-            if name not in seen:
-                seen[name] = raw(name)
-            return seen[name]
+            t = seen[name] if name in seen else raw(name)
+            if users is not None:
+                users[name] -= 1
+            if users is None or users[name] > 0:
+                seen[name] = t
+            else:
+                seen.pop(name, None)
+            return t
 
         for part in self.parts():
             part.load(get)

@@ -125,6 +125,7 @@ class PagedAttention(Mixer):
                              "own, an output gate, head norms, a score cap, a sink, a distance bias, kept first keys nor "
                              "adjacent rotation pairs")
         self.takes_quantized_cache = not self.general and ops.q8_supported(self.head_dim)
+        self.takes_small_weights = not self.general
         # what the decode kernel that makes its own queries and keys takes
         self.fusable = (self.norm_unit and self.position is None and self.q_temp is None and not self.v_norm
                         and not self.head_gate and self.v_head_dim == self.head_dim and self.head_dim in (16, 32, 64, 128)
@@ -182,7 +183,7 @@ class PagedAttention(Mixer):
         if self.head_gate and rows % 8:  # rows of no weight, so that a projected row stays a multiple of 16 bytes
             stacked.append(stacked[0].new_zeros(8 - rows % 8, self.width))
             biases.append(None)
-        self.w_qkv = torch.cat(stacked, dim=0).contiguous()
+        self.w_qkv = self.rt.projection(torch.cat(stacked, dim=0).contiguous())
         if any(b is not None for b in biases):
             if any(b is None for r, b in zip(roles, biases) if r in ("q", "k", "v")):
                 raise ValueError("attention biases must be given for q, k and v together")
@@ -194,6 +195,7 @@ class PagedAttention(Mixer):
             wide = w.new_zeros(self.width, self.n_heads, self.v_pool_dim)
             wide[:, :, :self.v_head_dim] = w
             self.w_o = wide.view(self.width, self.n_heads * self.v_pool_dim).contiguous()
+        self.w_o = self.rt.projection(self.w_o)
         self.b_o = get(t["o_bias"]) if "o_bias" in t else None
         if self.slope_list is not None:
             self.slopes = torch.tensor(self.slope_list, dtype=torch.float32, device=self.rt.device)
@@ -205,7 +207,7 @@ class PagedAttention(Mixer):
             self.sink_values = get(t["sink"]).contiguous()
 
     def weight_bytes(self):
-        return sum(w.numel() * w.element_size() for w in (self.w_qkv, self.w_o, self.b_qkv, self.b_o, self.w_qn, self.w_kn,
+        return sum(w.nbytes for w in (self.w_qkv, self.w_o, self.b_qkv, self.b_o, self.w_qn, self.w_kn,
                                                           self.sink_values, self.q_mul) if w is not None)
 
     def prepare(self, context_length: int) -> None:
@@ -306,7 +308,7 @@ class PagedAttention(Mixer):
                 and h.shape[0] <= ops.ROPE_PARTIAL_MAX_ROWS and ops.gemm_partial_supported(h, self.w_qkv)):
             # few tokens: the projection leaves its K slices unadded, what writes the pages adds them
             proj = self.rt.empty(h.shape[0], nh * d)
-            ops.rope_store_q8(ops.gemm_partial(h, self.w_qkv, self.rt.err), proj, step.positions, step.seq_of_row, cache.tables, cos,
+            ops.rope_store_q8(ops.gemm_partial(self.rt.rows(h, self.w_qkv), self.w_qkv, self.rt.err), proj, step.positions, step.seq_of_row, cache.tables, cos,
                               sin, rot, cache.quantized, nh, nkv, d, self.rt.err, bias=self.b_qkv)
         else:
             proj = self.rt.linear(h, self.w_qkv, bias=self.b_qkv)
@@ -337,7 +339,7 @@ class PagedAttention(Mixer):
                 and ops.gemm_partial_supported(h, self.w_qkv)):
             # few tokens: the projection leaves its K slices unadded; rotate-and-store adds them in 32-bit
             cos, sin, rot = fused
-            parts = ops.gemm_partial(h, self.w_qkv, self.rt.err)
+            parts = ops.gemm_partial(self.rt.rows(h, self.w_qkv), self.w_qkv, self.rt.err)
             if ops.attention_decode_fused_supported(plan, cache, h.dtype, h.shape[0], nh, self.n_kv_heads, d):
                 # single tokens only: adding the slices, rotation, the page write and attention are one launch
                 attn = self.rt.empty(h.shape[0], nh * d)

@@ -114,6 +114,7 @@ class PositionEncoding(Part):
 class Mixer(Part):
     graph_safe = False  # True when forward() only launches kernels on static buffers
     takes_quantized_cache = False  # True when forward() works on a view whose pages are `quantized`
+    takes_small_weights = False  # True when load() keeps projections as `runtime.projection` makes them and forward() takes those
 
     def cache_needs(self) -> CacheNeeds:
         return CacheNeeds()
@@ -127,6 +128,7 @@ class Mixer(Part):
 
 class FeedForward(Part):
     graph_safe = False
+    takes_small_weights = False  # as a mixer's
 
     def forward(self, h, stream, step) -> None:  # pragma: no cover - interface
         raise NotImplementedError

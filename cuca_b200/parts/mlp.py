@@ -15,6 +15,7 @@ class SwiGLU(FeedForward):
     """params: width, inner. tensors: gate [inner, width], up [inner, width], down [width, inner]."""
 
     graph_safe = True
+    takes_small_weights = True
 
     def __init__(self, spec, runtime):
         super().__init__(spec, runtime)
@@ -29,11 +30,11 @@ class SwiGLU(FeedForward):
 
     def load(self, get):
         t = self.spec.tensors
-        self.w_gate_up = torch.cat([get(t["gate"]), get(t["up"])], dim=0).contiguous()
-        self.w_down = get(t["down"])
+        self.w_gate_up = self.rt.projection(torch.cat([get(t["gate"]), get(t["up"])], dim=0).contiguous())
+        self.w_down = self.rt.projection(get(t["down"]))
 
     def weight_bytes(self):
-        return sum(w.numel() * w.element_size() for w in (self.w_gate_up, self.w_down))
+        return sum(w.nbytes for w in (self.w_gate_up, self.w_down))
 
     def forward(self, h, stream, step) -> None:
         act = self.rt.linear(h, self.w_gate_up, epilogue=ops.EPI_SWIGLU)

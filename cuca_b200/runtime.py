@@ -21,7 +21,8 @@ _ERR_TEXT = {
 class Runtime:
     """Device, compute dtype (float32: true 32-bit everywhere; bfloat16: serving precision) and shared helpers."""
 
-    def __init__(self, device="cuda:0", dtype: torch.dtype = torch.bfloat16):
+    def __init__(self, device="cuda:0", dtype: torch.dtype = torch.bfloat16, small_weights: bool = False, small_rows: bool = False):
+        """`small_weights`: projections keep their weights in 4 bits; `small_rows`: what enters them is brought to 4 bits too."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype must be float32 or bfloat16, not {dtype}")
         self.device = torch.device(device)
@@ -34,18 +35,27 @@ class Runtime:
         library.load()
         torch.cuda.set_device(self.device)
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.small_weights, self.small_rows = bool(small_weights), bool(small_rows)
         self.use_partials = True  # few-token contractions may leave their K slices unadded for the next reader
 
     # ---------------------------------------------------------------- helpers
     def empty(self, *shape, dtype=None) -> torch.Tensor:
         return torch.empty(*shape, dtype=dtype or self.dtype, device=self.device)
 
+    def projection(self, w):
+        """A projection's weight as it is kept: as given, or in 4 bits."""
+        return ops.mx4_quantise(w) if self.small_weights else w
+
+    def rows(self, a, w):
+        """`a` as it enters a product with `w`: as given, or in 4 bits."""
+        return ops.mx4_quantise(a) if self.small_rows and type(w) is ops.Mx4Matrix else a
+
     def linear(self, a, w, out=None, epilogue=ops.EPI_STORE, bias=None, out_dtype=None):
         """out = epilogue(a @ w.T): store, add to the 32-bit stream, or SwiGLU over stacked [gate; up]."""
         n = w.shape[0] // 2 if epilogue == ops.EPI_SWIGLU else w.shape[0]
         if out is None:
             out = self.empty(a.shape[0], n, dtype=out_dtype or self.dtype)
-        ops.gemm(a, w, out, epilogue, bias, self.err)
+        ops.gemm(self.rows(a, w), w, out, epilogue, bias, self.err)
         return out
 
     def stream(self, x) -> "ResidualStream":
@@ -140,6 +150,7 @@ class ResidualStream:
     def add_linear(self, a, w, bias=None) -> None:
         """stream += a @ w.T (+ bias). Over few tokens the slices may stay pending until the next reader."""
         rt = self.rt
+        a = rt.rows(a, w)
         self._rounded = None
         if self._unwritten:
             self._unwritten = False
@@ -275,6 +286,7 @@ class SublayerOutput(ResidualStream):
 
     def add_linear(self, a, w, bias=None) -> None:
         rt = self.rt
+        a = rt.rows(a, w)
         if (rt.use_partials and bias is None and len(self.terms) < ops.MAX_TERMS - 1
                 and ops.gemm_partial_supported(a, w)):
             self.terms.append((ops.gemm_partial(a, w, rt.err), self.factor))

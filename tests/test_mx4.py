@@ -9,7 +9,7 @@ def test_layout_of_codes_and_scales():
     from cuca_b200.kernels import ops
     q = ops.Mx4Matrix.empty(300, 200, "cpu")
     assert q.shape == (300, 200) and q.codes.shape == (300, 128) and q.scales.shape == (3, 2, 32, 4, 4)
-    assert q.nbytes() == 300 * 128 + 3 * 2 * 512 and q.device.type == "cpu"
+    assert q.nbytes == 300 * 128 + 3 * 2 * 512 and q.device.type == "cpu"
     q.codes.zero_()
     code, byte = torch.randint(0, 16, (300, 7, 32)), torch.randint(0, 256, (300, 7))
     flat = code.flatten(1)

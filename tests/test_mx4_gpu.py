@@ -148,8 +148,8 @@ def test_products(kind, m, k, n):
         out = torch.full((m, n), 7.0, dtype=out_dtype, device="cuda")
         ops.gemm_mx4(a, q, out, err=err)
         _check(out, *_product(kind, x, w, "store", out_dtype))
-    bias = _rows(1, n, F32 if kind == "f32" else BF16, 5)[0].contiguous()
-    out = torch.full((m, n), 7.0, dtype=bias.dtype, device="cuda")
+    bias = _rows(1, n, F32 if (kind == "f32") == (n % 2 == 0) else BF16, 5)[0].contiguous()
+    out = torch.full((m, n), 7.0, dtype=F32 if kind == "f32" else BF16, device="cuda")
     ops.gemm_mx4(a, q, out, bias=bias, err=err)
     _check(out, *_product(kind, x, w, "store", out.dtype, bias=bias))
     stream = _rows(m, n, F32, 6)
@@ -322,7 +322,8 @@ def test_refusals():
     refuse(x.float(), w, out)
     refuse(x, w, out, ops.EPI_RESIDUAL)
     refuse(x, w, torch.empty(4, 5, dtype=BF16, device="cuda"), ops.EPI_SWIGLU, torch.zeros(5, dtype=BF16, device="cuda"))
-    refuse(x, w, out, bias=torch.zeros(10, device="cuda"))
+    refuse(x, w, out, bias=torch.zeros(10, dtype=torch.half, device="cuda"))
+    refuse(x, w, out, bias=torch.zeros(10, device="cuda").cpu())
     refuse(x, w, out, bias=torch.zeros(9, dtype=BF16, device="cuda"))
     refuse(x, w, out, 7)
     refuse(x.cpu(), w, out)
