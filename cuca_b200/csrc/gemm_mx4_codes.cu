@@ -200,13 +200,11 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
       float* sums = reinterpret_cast<float*>(smem);  // (every copy into the stages has been waited for)
       if (BLOCKS == 2 && !DUAL) {
         if (set == 0 || scaled)
-          mx4_leave<G>(p.o, at + set * p.nt, t0, m_here, n0 + set * TILE_A, row, p.share == 1, sums + set * (p.nt / G) * TILE_A);
+          mx4_leave<G, false>(p.o, at + set * p.nt, t0, m_here, n0 + set * TILE_A, row, p.share == 1, sums + set * (p.nt / G) * TILE_A);
       } else {
         const int half = ((nt / 2 + 15) & ~15) / G, first = set * half, last = set ? m_here : min(half, m_here);
-        if (last > first && DUAL)
-          mx4_leave_gated<G>(p.o, at + first * G, p.nt, t0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A, p.nt / G);
-        else if (last > first)
-          mx4_leave<G>(p.o, at + first * G, t0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A);
+        if (last > first)
+          mx4_leave<G, DUAL>(p.o, at + first * G, t0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A, p.nt, p.nt / G);
       }
       if (threadIdx.x == READ_WARP * 32) *ok_flag = 1;
     }

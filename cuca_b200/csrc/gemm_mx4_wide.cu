@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_con
       tc_fence_after();
       const int half = ((m_here + 1) / 2 + 15) & ~15, first = set * half, last = set ? m_here : min(half, m_here);
       if (last > first)
-        mx4_leave<1>(p.o, acc + first + lanes, m0 + first, last - first, n0, row, !DUAL && p.share == 1, reinterpret_cast<float*>(smem) + first * TILE_A);
+        mx4_leave<1, false>(p.o, acc + first + lanes, m0 + first, last - first, n0, row, !DUAL && p.share == 1, reinterpret_cast<float*>(smem) + first * TILE_A);
       if (threadIdx.x == CONVERT_WARP * 32) *ok_flag = 1;
     }
   }

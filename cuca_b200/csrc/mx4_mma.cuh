@@ -13,9 +13,7 @@ __device__ __forceinline__ uint32_t mx4_cluster_rank() {
 __device__ __forceinline__ void mx4_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float mx4_peer_f32(const float* p, uint32_t rank) {  // the same place in a peer's shared memory
-  uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+__device__ __forceinline__ float mx4_peer_f32(uint32_t at) {  // an address that mapa made
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
   return v;
@@ -75,16 +73,32 @@ struct Mx4Out {
   int64_t ldo;
   int m, n, out_f32, epilogue, bias_f32;
 };
-__device__ __forceinline__ float mx4_gate(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 // silu(g) u: for bfloat16 results the approximate quotient and exponential, good to 2^-20
-__device__ __forceinline__ float mx4_gate(const Mx4Out& o, float g, float u) { return o.out_f32 ? g / (1.f + expf(-g)) * u : mx4_gate(g, u); }
-__device__ __forceinline__ void mx4_put(const Mx4Out& o, int m, int n, float y) {
-  if (o.bias) y += o.bias_f32 ? ((const float*)o.bias)[n] : __bfloat162float(((const __nv_bfloat16*)o.bias)[n]);
-  const int64_t at = m * o.ldo + n;
-  if (o.epilogue == EPI_RESIDUAL) ((float*)o.out)[at] += y;
-  else if (o.out_f32) ((float*)o.out)[at] = y;
-  else ((__nv_bfloat16*)o.out)[at] = __float2bfloat16_rn(y);
+__device__ __forceinline__ float mx4_gate(bool exact, float g, float u) {
+  return exact ? g / (1.f + expf(-g)) * u : __fdividef(g, 1.f + __expf(-g)) * u;
 }
+// Where a feature's results go, one row of A after the other. What does not change from row to row is settled once: with the checks at
+// each result a tile's results took longer than its products (14 us of 26 for 192 x 256).
+struct Mx4Column {
+  char* at;
+  int64_t step;  // bytes from row to row
+  float bias;
+  bool f32, add;
+  __device__ Mx4Column(const Mx4Out& o, int m, int n) {
+    const int size = o.out_f32 ? 4 : 2;
+    at = (char*)o.out + (m * o.ldo + n) * size;
+    step = o.ldo * size;
+    bias = !o.bias ? 0.f : o.bias_f32 ? ((const float*)o.bias)[n] : __bfloat162float(((const __nv_bfloat16*)o.bias)[n]);
+    f32 = o.out_f32;
+    add = o.epilogue == EPI_RESIDUAL;
+  }
+  __device__ void put(float y) const {
+    y += bias;
+    if (!f32) *(__nv_bfloat16*)at = __float2bfloat16_rn(y);
+    else if (add) *(float*)at += y;
+    else *(float*)at = y;
+  }
+};
 
 // Sixteen columns of this thread's lane as 16 / G results: G columns are one row of A (its digits, the smallest added first).
 template <int G>
@@ -99,40 +113,30 @@ __device__ __forceinline__ void mx4_take16(uint32_t at, float (&y)[16 / G]) {
   }
 }
 // A finished tile: lane `row` (0..127) of tensor memory holds weight row `row` of the tile, G columns `at`.. each of the m_here rows of A
-// from m0 on. Alone they are results, features from n0 on; else they go to shared memory, [row of A][128], for mx4_join.
-template <int G>
-__device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, int m_here, int n0, int row, bool alone, float* sums) {
-  for (int c = 0; c < m_here; c += 16 / G) {
-    float v[16 / G];
+// from m0 on. Alone they are results, features from n0 on; else they go to shared memory, [row of A][128], for mx4_join. GATED: the up
+// part's accumulator lies `apart` columns further on, in shared memory `up` rows.
+template <int G, bool GATED>
+__device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, int m_here, int n0, int row, bool alone, float* sums, int apart = 0,
+                                          int up = 0) {
+  constexpr int N = 16 / G;
+  const bool live = n0 + row < o.n;
+  Mx4Column out(o, m0, live ? n0 + row : 0);
+  for (int c = 0; c < m_here; c += N) {
+    float v[N], u[N];
     mx4_take16<G>(at + c * G, v);
+    if (GATED) mx4_take16<G>(at + apart + c * G, u);
     if (!alone) {
 #pragma unroll
-      for (int j = 0; j < 16 / G; ++j) sums[(c + j) * TILE_A + row] = v[j];
-    } else if (n0 + row < o.n) {
-#pragma unroll
-      for (int j = 0; j < 16 / G; ++j)
-        if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, v[j]);
-    }
-  }
-}
-// ... with gate and up accumulators `apart` columns apart, in shared memory `up` rows
-template <int G>
-__device__ __forceinline__ void mx4_leave_gated(const Mx4Out& o, uint32_t at, int apart, int m0, int m_here, int n0, int row, bool alone, float* sums,
-                                                int up) {
-  for (int c = 0; c < m_here; c += 16 / G) {
-    float v[16 / G], u[16 / G];
-    mx4_take16<G>(at + c * G, v);
-    mx4_take16<G>(at + apart + c * G, u);
-    if (!alone) {
-#pragma unroll
-      for (int j = 0; j < 16 / G; ++j) {
+      for (int j = 0; j < N; ++j) {
         sums[(c + j) * TILE_A + row] = v[j];
-        sums[(up + c + j) * TILE_A + row] = u[j];
+        if (GATED) sums[(up + c + j) * TILE_A + row] = u[j];
       }
-    } else if (n0 + row < o.n) {
+    } else if (live) {
 #pragma unroll
-      for (int j = 0; j < 16 / G; ++j)
-        if (c + j < m_here) mx4_put(o, m0 + c + j, n0 + row, mx4_gate(o, v[j], u[j]));
+      for (int j = 0; j < N; ++j) {
+        if (c + j < m_here) out.put(GATED ? mx4_gate(out.f32, v[j], u[j]) : v[j]);
+        out.at += out.step;
+      }
     }
   }
 }
@@ -141,24 +145,39 @@ __device__ __forceinline__ void mx4_leave_gated(const Mx4Out& o, uint32_t at, in
 // up part stands so many rows of A further on.
 template <bool HALVES>
 __device__ __forceinline__ void mx4_join(const Mx4Out& o, const float* sums, int m0, int m_here, int n0, int rank, int share, bool ok, int up = 0) {
+  constexpr int THREADS = 256, MOST = 8;
   if (share > 1) mx4_cluster_sync();
-  const int mine = (HALVES ? TILE_A / 2 : TILE_A) / share, r0 = rank * mine;
+  // a thread has a feature, and rows of A in turn with the other threads that have it
+  const int mine = (HALVES ? TILE_A / 2 : TILE_A) / share, shift = 31 - __clz(mine);
+  const int row = rank * mine + (threadIdx.x & (mine - 1)), turn = THREADS >> shift;
   const int second = HALVES ? TILE_A / 2 : up * TILE_A;
-  if (ok) {
-    for (int i = threadIdx.x; i < m_here * mine; i += blockDim.x) {
-      const int c = i / mine, row = r0 + i - c * mine;
-      const float* at = sums + c * TILE_A + row;
+  int c = threadIdx.x >> shift;
+  if (ok && threadIdx.x < THREADS && n0 + row < o.n && c < m_here) {
+    Mx4Column out(o, m0 + c, n0 + row);
+    const float* at = sums + c * TILE_A + row;
+    uint32_t peer[MOST];
+#pragma unroll
+    for (int r = 0; r < MOST; ++r)
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[r]) : "r"(smem_u32(at)), "r"(r < share ? r : 0));
+    const uint32_t apart = second * 4;
+    for (; c < m_here; c += turn) {
       float v = 0.f, u = 0.f;
       if (share == 1) {
         v = at[0];
         if (second) u = at[second];
+        at += turn * TILE_A;
       } else {
-        for (int r = 0; r < share; ++r) {
-          v += mx4_peer_f32(at, r);
-          if (second) u += mx4_peer_f32(at + second, r);
+#pragma unroll
+        for (int r = 0; r < MOST; ++r) {
+          if (r < share) {
+            v += mx4_peer_f32(peer[r]);
+            if (second) u += mx4_peer_f32(peer[r] + apart);
+            peer[r] += turn * TILE_A * 4;
+          }
         }
       }
-      if (n0 + row < o.n) mx4_put(o, m0 + c, n0 + row, second ? mx4_gate(o, v, u) : v);
+      out.put(second ? mx4_gate(out.f32, v, u) : v);
+      out.at += turn * out.step;
     }
   }
   if (share > 1) mx4_cluster_sync();  // until nobody reads these sums any more
