@@ -13,9 +13,9 @@ __device__ __forceinline__ uint32_t mx4_cluster_rank() {
 __device__ __forceinline__ void mx4_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float mx4_peer_f32(uint32_t at) {  // an address that mapa made
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+__device__ __forceinline__ float2 mx4_peer_f32x2(uint32_t at) {  // an address that mapa made
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
   return v;
 }
 __device__ __forceinline__ void mx4_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
@@ -98,6 +98,19 @@ struct Mx4Column {
     else if (add) *(float*)at += y;
     else *(float*)at = y;
   }
+  __device__ void put2(float y, float z) const {  // z: of the next feature, its bias added; for places on two results' size
+    y += bias;
+    if (!f32) {
+      *(__nv_bfloat162*)at = __floats2bfloat162_rn(y, z);
+    } else {
+      if (add) {
+        const float2 old = *(const float2*)at;
+        y += old.x;
+        z += old.y;
+      }
+      *(float2*)at = make_float2(y, z);
+    }
+  }
 };
 
 // Sixteen columns of this thread's lane as 16 / G results: G columns are one row of A (its digits, the smallest added first).
@@ -147,37 +160,53 @@ template <bool HALVES>
 __device__ __forceinline__ void mx4_join(const Mx4Out& o, const float* sums, int m0, int m_here, int n0, int rank, int share, bool ok, int up = 0) {
   constexpr int THREADS = 256, MOST = 8;
   if (share > 1) mx4_cluster_sync();
-  // a thread has a feature, and rows of A in turn with the other threads that have it
-  const int mine = (HALVES ? TILE_A / 2 : TILE_A) / share, shift = 31 - __clz(mine);
-  const int row = rank * mine + (threadIdx.x & (mine - 1)), turn = THREADS >> shift;
+  // a thread has two features, and rows of A in turn with the other threads that have them
+  const int mine = (HALVES ? TILE_A / 2 : TILE_A) / share, shift = 30 - __clz(mine);
+  const int row = rank * mine + 2 * (threadIdx.x & (mine / 2 - 1)), turn = THREADS >> shift;
   const int second = HALVES ? TILE_A / 2 : up * TILE_A;
   int c = threadIdx.x >> shift;
   if (ok && threadIdx.x < THREADS && n0 + row < o.n && c < m_here) {
-    Mx4Column out(o, m0 + c, n0 + row);
-    const float* at = sums + c * TILE_A + row;
+    Mx4Column out(o, m0 + c, n0 + row), next(o, m0 + c, min(n0 + row + 1, o.n - 1));
+    const bool both = n0 + row + 1 < o.n, wide = both && !(((uintptr_t)out.at | out.step) & (out.f32 ? 7 : 3));
+    const uint32_t at = smem_u32(sums + c * TILE_A + row), apart = second * 4;
     uint32_t peer[MOST];
 #pragma unroll
-    for (int r = 0; r < MOST; ++r)
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[r]) : "r"(smem_u32(at)), "r"(r < share ? r : 0));
-    const uint32_t apart = second * 4;
+    for (int r = 0; r < MOST; ++r) {
+      peer[r] = at;
+      if (share > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[r]) : "r"(at), "r"(r < share ? r : 0));
+    }
+    const float* here = sums + c * TILE_A + row;
     for (; c < m_here; c += turn) {
-      float v = 0.f, u = 0.f;
+      float2 v = make_float2(0.f, 0.f), u = v;
       if (share == 1) {
-        v = at[0];
-        if (second) u = at[second];
-        at += turn * TILE_A;
+        v = *reinterpret_cast<const float2*>(here);
+        if (second) u = *reinterpret_cast<const float2*>(here + second);
+        here += turn * TILE_A;
       } else {
 #pragma unroll
         for (int r = 0; r < MOST; ++r) {
           if (r < share) {
-            v += mx4_peer_f32(peer[r]);
-            if (second) u += mx4_peer_f32(peer[r] + apart);
+            const float2 a = mx4_peer_f32x2(peer[r]);
+            v.x += a.x;
+            v.y += a.y;
+            if (second) {
+              const float2 b = mx4_peer_f32x2(peer[r] + apart);
+              u.x += b.x;
+              u.y += b.y;
+            }
             peer[r] += turn * TILE_A * 4;
           }
         }
       }
-      out.put(second ? mx4_gate(out.f32, v, u) : v);
+      if (second) v = make_float2(mx4_gate(out.f32, v.x, u.x), mx4_gate(out.f32, v.y, u.y));
+      if (wide) {
+        out.put2(v.x, v.y + next.bias);
+      } else {
+        out.put(v.x);
+        if (both) next.put(v.y);
+      }
       out.at += turn * out.step;
+      next.at += turn * out.step;
     }
   }
   if (share > 1) mx4_cluster_sync();  // until nobody reads these sums any more
