@@ -35,7 +35,7 @@ struct Params {
   int k_steps, k_stages;
   int nt;          // rows of A of a whole tile, a multiple of 16
   int a_tiles;     // tiles of 128 rows that A's scales have
-  int tiles_n, share;
+  int tiles, tiles_n, share;
   int stages, stage_bytes, tmem_cols;
   int* err;
 };
@@ -49,20 +49,36 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   uint64_t* full = (uint64_t*)(smem + p.stages * p.stage_bytes);
   uint64_t* empty = full + MAX_STAGES;
   uint64_t* done = empty + MAX_STAGES;
-  uint32_t* tmem_slot = (uint32_t*)(done + 1);
+  uint64_t* acc_free = done + 1;
+  uint32_t* tmem_slot = (uint32_t*)(acc_free + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* ok_flag = (volatile int*)(tmem_slot + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.share > 1 ? (int)mx4_cluster_rank() : 0;
-  const int tile = (int)blockIdx.x / p.share;
-  const int n0 = (tile % p.tiles_n) * (DUAL ? TILE_A : BLOCKS * TILE_A), m0 = (tile / p.tiles_n) * p.nt;
-  const int rows_here = min(p.nt, p.o.m * G - m0), nt = (rows_here + 15) & ~15;  // (the last tile multiplies no more columns than it has)
-  const int t0 = m0 / G, m_here = rows_here / G;  // G rows in 4 bits make one of the result
+  const int first_tile = (int)blockIdx.x / p.share, tile_step = (int)gridDim.x / p.share;  // (of a cluster one tile)
+  struct Tile {
+    int n0, m0, nt;       // first feature, first row of A, columns that are multiplied (the last tile has no more than it needs)
+    int t0, m_here;       // rows of the result: G rows in 4 bits make one
+    int second;           // the second block's first weight row
+    bool scaled;          // it has features (else it multiplies zeros)
+    int span0, spans;     // A's runs of 128 scales
+  };
+  auto tile_at = [&](int tile) {
+    Tile t;
+    t.n0 = (tile % p.tiles_n) * (DUAL ? TILE_A : BLOCKS * TILE_A);
+    t.m0 = (tile / p.tiles_n) * p.nt;
+    const int rows = min(p.nt, p.o.m * G - t.m0);
+    t.nt = (rows + 15) & ~15;
+    t.t0 = t.m0 / G;
+    t.m_here = rows / G;
+    t.second = DUAL ? p.o.n + t.n0 : t.n0 + TILE_A;
+    t.scaled = DUAL || t.second < p.o.n;
+    t.span0 = t.m0 >> 7;
+    t.spans = min(SPANS, p.a_tiles - t.span0);
+    return t;
+  };
   const int ks0 = (int)((int64_t)p.k_stages * rank / p.share), ks1 = (int)((int64_t)p.k_stages * (rank + 1) / p.share);
-  const int second = DUAL ? p.o.n + n0 : n0 + TILE_A;  // the second block's first weight row
   const bool up_apart = DUAL && (p.o.n & 127);         // the up rows' scales do not start where 128 rows' do
-  const bool scaled = DUAL || second < p.o.n;          // the second block has features (else it multiplies zeros)
-  const int span0 = m0 >> 7, spans = min(SPANS, p.a_tiles - span0);
   const int a_bytes = p.nt * STAGE_BYTES_K;
   // scales of a stage: [block of features][step][512], then [128 rows of A][step][512]
   const int sc_w = BLOCKS * W_BYTES + a_bytes, sc_a = sc_w + BLOCKS * STAGE_STEPS * SCALE_BYTES;
@@ -73,6 +89,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
+    mbar_init(acc_free, READ_WARPS);
     *abort_flag = 0;
     *ok_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -90,122 +107,142 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   if (warp == 0) {
     // ------------------------------------------------ weights
     if (lane == 0) {  // the first ones into L2: that needs no wait for the kernel before, whatever it writes
+      const Tile t = tile_at(first_tile);
       for (int ks = ks0; ks < ks1 && ks < ks0 + p.stages; ++ks) {
-        mx4_prefetch_2d(&tm_w, ks * 64, n0);
-        if (BLOCKS == 2) mx4_prefetch_2d(&tm_w, ks * 64, second);
+        mx4_prefetch_2d(&tm_w, ks * 64, t.n0);
+        if (BLOCKS == 2) mx4_prefetch_2d(&tm_w, ks * 64, t.second);
       }
     }
     __syncwarp();
     pdl_wait();
     Mx4Ring ring;
-    for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
-      uint8_t* sp = smem + ring.at * p.stage_bytes;
-      uint64_t* bar = &full[ring.at];
-      if (!warp_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) break;
-      const int s0 = ks * STAGE_STEPS, steps = min(STAGE_STEPS, p.k_steps - s0);
-      if (lane == 0) {
-        const uint32_t sc = steps * SCALE_BYTES;
-        mbar_expect_tx(bar, BLOCKS * W_BYTES + sc * (up_apart || !scaled ? 1 : BLOCKS));
-        tma_load_2d(sp, &tm_w, bar, ks * 64, n0);
-        if (BLOCKS == 2) tma_load_2d(sp + W_BYTES, &tm_w, bar, ks * 64, second);
-        bulk_load(sp + sc_w, p.w_scales + mx4_scale_at(n0, s0, p.k_steps), bar, sc);
-        if (BLOCKS == 2 && !up_apart && scaled)
-          bulk_load(sp + sc_w + STAGE_STEPS * SCALE_BYTES, p.w_scales + mx4_scale_at(second, s0, p.k_steps), bar, sc);
-      }
-      if (up_apart) {  // word by word: a lane's sixteen bytes are the scales of rows 32 apart
-        for (int s = 0; s < steps; ++s) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = min(second + 32 * i + lane, 2 * p.o.n - 1);
-            w[i] = __ldcg(reinterpret_cast<const uint32_t*>(p.w_scales + mx4_scale_at(r, s0 + s, p.k_steps)));
-          }
-          *reinterpret_cast<uint4*>(sp + sc_w + (STAGE_STEPS + s) * SCALE_BYTES + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step) {
+      const Tile t = tile_at(tile);
+      for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
+        uint8_t* sp = smem + ring.at * p.stage_bytes;
+        uint64_t* bar = &full[ring.at];
+        if (!warp_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) { ok = false; break; }
+        const int s0 = ks * STAGE_STEPS, steps = min(STAGE_STEPS, p.k_steps - s0);
+        if (lane == 0) {
+          const uint32_t sc = steps * SCALE_BYTES;
+          mbar_expect_tx(bar, BLOCKS * W_BYTES + sc * (up_apart || !t.scaled ? 1 : BLOCKS));
+          tma_load_2d(sp, &tm_w, bar, ks * 64, t.n0);
+          if (BLOCKS == 2) tma_load_2d(sp + W_BYTES, &tm_w, bar, ks * 64, t.second);
+          bulk_load(sp + sc_w, p.w_scales + mx4_scale_at(t.n0, s0, p.k_steps), bar, sc);
+          if (BLOCKS == 2 && !up_apart && t.scaled)
+            bulk_load(sp + sc_w + STAGE_STEPS * SCALE_BYTES, p.w_scales + mx4_scale_at(t.second, s0, p.k_steps), bar, sc);
         }
-        fence_proxy_async();
+        if (up_apart) {  // word by word: a lane's sixteen bytes are the scales of rows 32 apart
+          for (int s = 0; s < steps; ++s) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = min(t.second + 32 * i + lane, 2 * p.o.n - 1);
+              w[i] = __ldcg(reinterpret_cast<const uint32_t*>(p.w_scales + mx4_scale_at(r, s0 + s, p.k_steps)));
+            }
+            *reinterpret_cast<uint4*>(sp + sc_w + (STAGE_STEPS + s) * SCALE_BYTES + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar);
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
       }
-      __syncwarp();
     }
   } else if (warp == ROW_WARP) {
     // ------------------------------------------------ rows of A
     if (lane == 0) {
       pdl_wait();
       Mx4Ring ring;
-      for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
-        uint8_t* sp = smem + ring.at * p.stage_bytes;
-        uint64_t* bar = &full[ring.at];
-        if (!mbar_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) break;
-        const int s0 = ks * STAGE_STEPS;
-        const uint32_t sc = min(STAGE_STEPS, p.k_steps - s0) * SCALE_BYTES;
-        mbar_expect_tx(bar, a_bytes + sc * spans);
-        tma_load_2d(sp + BLOCKS * W_BYTES, &tm_a, bar, ks * 64, m0);
-        for (int t = 0; t < spans; ++t)
-          bulk_load(sp + sc_a + t * STAGE_STEPS * SCALE_BYTES, p.a_scales + mx4_scale_at((span0 + t) * 128, s0, p.k_steps), bar, sc);
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step) {
+        const Tile t = tile_at(tile);
+        for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
+          uint8_t* sp = smem + ring.at * p.stage_bytes;
+          uint64_t* bar = &full[ring.at];
+          if (!mbar_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) { ok = false; break; }
+          const int s0 = ks * STAGE_STEPS;
+          const uint32_t sc = min(STAGE_STEPS, p.k_steps - s0) * SCALE_BYTES;
+          mbar_expect_tx(bar, a_bytes + sc * t.spans);
+          tma_load_2d(sp + BLOCKS * W_BYTES, &tm_a, bar, ks * 64, t.m0);
+          for (int i = 0; i < t.spans; ++i)
+            bulk_load(sp + sc_a + i * STAGE_STEPS * SCALE_BYTES, p.a_scales + mx4_scale_at((t.span0 + i) * 128, s0, p.k_steps), bar, sc);
+        }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------ products. What a stage issues stands unrolled, its descriptors one addition from
     // the first stage's: an instruction whose operands are worked out beside it takes twice as long to issue, and a stage has seventeen
     pdl_wait();
-    const uint32_t idesc = mx4_instr_desc(nt, TILE_A);
     const uint32_t sa = smem_u32(smem);
     const uint64_t w0 = smem_desc(sa), a0 = smem_desc(sa + BLOCKS * W_BYTES), sw0 = mx4_scale_desc(sa + sc_w), sr0 = mx4_scale_desc(sa + sc_a);
-    const uint32_t shift = (m0 & 127) >> 5;  // columns of scales before this tile's first row
     const uint64_t stride = p.stage_bytes >> 4;
     constexpr int STEP_COLS = 4 * (BLOCKS + SPANS);
-    Mx4Ring ring;
+    Mx4Ring ring, acc_ring;
     bool ok = true;
-    for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
-      if (!warp_wait(&full[ring.at], ring.parity, p.err, abort_flag)) { ok = false; break; }
+    for (int tile = first_tile; ok && tile < p.tiles; tile += tile_step, acc_ring.next(1)) {
+      const Tile t = tile_at(tile);
+      const uint32_t idesc = mx4_instr_desc(t.nt, TILE_A);
+      const uint32_t shift = (t.m0 & 127) >> 5;  // columns of scales before this tile's first row
+      if (!warp_wait(acc_free, acc_ring.parity ^ 1, p.err, abort_flag)) break;
       tc_fence_after();
-      const uint64_t at = ring.at * stride;
-      const uint32_t cols = scale_cols + ring.at * (STAGE_STEPS * STEP_COLS);
-      const bool whole = (ks + 1) * STAGE_STEPS <= p.k_steps;
-      if (elect_one()) {
+      for (int ks = ks0; ks < ks1; ++ks, ring.next(p.stages)) {
+        if (!warp_wait(&full[ring.at], ring.parity, p.err, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t at = ring.at * stride;
+        const uint32_t cols = scale_cols + ring.at * (STAGE_STEPS * STEP_COLS);
+        const bool whole = (ks + 1) * STAGE_STEPS <= p.k_steps;
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < STAGE_STEPS; ++s) {
-          if (s == 0 || whole) {
-            const uint32_t cols_w = cols + s * STEP_COLS, cols_a = cols_w + 4 * BLOCKS;
-#pragma unroll
-            for (int b = 0; b < BLOCKS; ++b)
-              mx4_scales_to_tmem(cols_w + 4 * b, sw0 + at + (uint64_t)((b * STAGE_STEPS + s) * SCALE_BYTES >> 4));
-#pragma unroll
-            for (int t = 0; t < SPANS; ++t)
-              mx4_scales_to_tmem(cols_a + 4 * t, sr0 + at + (uint64_t)((t * STAGE_STEPS + s) * SCALE_BYTES >> 4));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {  // 64 values each
-              const uint64_t off = at + (uint64_t)((s * 64 + h * 32) >> 4);
-              const uint32_t id = idesc | mx4_scale_half(h), accumulate = s + h > 0 ? 1u : ks > ks0;
+          for (int s = 0; s < STAGE_STEPS; ++s) {
+            if (s == 0 || whole) {
+              const uint32_t cols_w = cols + s * STEP_COLS, cols_a = cols_w + 4 * BLOCKS;
 #pragma unroll
               for (int b = 0; b < BLOCKS; ++b)
-                mx4_umma(acc + b * p.nt, w0 + off + (uint64_t)(b * W_BYTES >> 4), a0 + off, id, cols_w + 4 * b, cols_a + shift, accumulate);
+                mx4_scales_to_tmem(cols_w + 4 * b, sw0 + at + (uint64_t)((b * STAGE_STEPS + s) * SCALE_BYTES >> 4));
+#pragma unroll
+              for (int i = 0; i < SPANS; ++i)
+                mx4_scales_to_tmem(cols_a + 4 * i, sr0 + at + (uint64_t)((i * STAGE_STEPS + s) * SCALE_BYTES >> 4));
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {  // 64 values each
+                const uint64_t off = at + (uint64_t)((s * 64 + h * 32) >> 4);
+                const uint32_t id = idesc | mx4_scale_half(h), accumulate = s + h > 0 ? 1u : ks > ks0;
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b)
+                  mx4_umma(acc + b * p.nt, w0 + off + (uint64_t)(b * W_BYTES >> 4), a0 + off, id, cols_w + 4 * b, cols_a + shift, accumulate);
+              }
             }
           }
+          umma_commit(&empty[ring.at]);
         }
-        umma_commit(&empty[ring.at]);
+        __syncwarp();
       }
+      if (ok && elect_one()) umma_commit(done);
       __syncwarp();
     }
-    if (ok && elect_one()) umma_commit(done);
-    __syncwarp();
   } else {
     // ------------------------------------------------ results: of two blocks of features a set of four warps takes each, else halves of the columns
     pdl_wait();
-    if (warp_wait(done, 0, p.err, abort_flag)) {
+    const int set = (warp - READ_WARP) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
+    float* sums = reinterpret_cast<float*>(smem);  // (of a cluster: every copy into the stages has been waited for)
+    Mx4Ring acc_ring;
+    for (int tile = first_tile; tile < p.tiles; tile += tile_step, acc_ring.next(1)) {
+      const Tile t = tile_at(tile);
+      if (!warp_wait(done, acc_ring.parity, p.err, abort_flag)) break;
       tc_fence_after();
-      const int set = (warp - READ_WARP) >> 2, row = (warp & 3) * 32 + lane;
-      const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
-      float* sums = reinterpret_cast<float*>(smem);  // (every copy into the stages has been waited for)
       if (BLOCKS == 2 && !DUAL) {
-        if (set == 0 || scaled)
-          mx4_leave<G, false>(p.o, at + set * p.nt, t0, m_here, n0 + set * TILE_A, row, p.share == 1, sums + set * (p.nt / G) * TILE_A);
+        if (set == 0 || t.scaled)
+          mx4_leave<G, false>(p.o, at + set * p.nt, t.t0, t.m_here, t.n0 + set * TILE_A, row, p.share == 1, sums + set * (p.nt / G) * TILE_A);
       } else {
-        const int half = ((nt / 2 + 15) & ~15) / G, first = set * half, last = set ? m_here : min(half, m_here);
+        const int half = ((t.nt / 2 + 15) & ~15) / G, first = set * half, last = set ? t.m_here : min(half, t.m_here);
         if (last > first)
-          mx4_leave<G, DUAL>(p.o, at + first * G, t0 + first, last - first, n0, row, p.share == 1, sums + first * TILE_A, p.nt, p.nt / G);
+          mx4_leave<G, DUAL>(p.o, at + first * G, t.t0 + first, last - first, t.n0, row, p.share == 1, sums + first * TILE_A, p.nt, p.nt / G);
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_free);
       if (threadIdx.x == READ_WARP * 32) *ok_flag = 1;
     }
   }
@@ -216,8 +253,9 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   if (warp == 1) tmem_dealloc(acc, p.tmem_cols);
   if (p.share > 1) {
     const float* sums = reinterpret_cast<const float*>(smem);
-    mx4_join<false>(p.o, sums, t0, m_here, n0, rank, p.share, *ok_flag != 0, DUAL ? p.nt / G : 0);
-    if (BLOCKS == 2 && !DUAL) mx4_join<false>(p.o, sums + (p.nt / G) * TILE_A, t0, m_here, n0 + TILE_A, rank, p.share, *ok_flag != 0 && scaled);
+    const Tile t = tile_at(first_tile);
+    mx4_join<false>(p.o, sums, t.t0, t.m_here, t.n0, rank, p.share, *ok_flag != 0, DUAL ? p.nt / G : 0);
+    if (BLOCKS == 2 && !DUAL) mx4_join<false>(p.o, sums + (p.nt / G) * TILE_A, t.t0, t.m_here, t.n0 + TILE_A, rank, p.share, *ok_flag != 0 && t.scaled);
   }
 }
 
@@ -257,7 +295,8 @@ int launch_spans(const CucaMx4Gemm* c) {
                cuca_tensor_map_2d(c->a, 2, (uint64_t)m, cols, cols, p.nt, &tm_a), "gemm_mx4: tensor map failed");
   constexpr auto kernel = gemm_mx4_codes_kernel<BLOCKS, DUAL, SPANS, G>;
   if (int e = mx4_configure<kernel>(227 * 1024)) return e;
-  const dim3 grid((unsigned)(tiles * p.share));
+  p.tiles = (int)tiles;
+  const dim3 grid(p.share > 1 || tiles < slots ? (unsigned)(tiles * p.share) : (unsigned)slots);
   if (p.share > 1) cuca_launch_cluster(kernel, grid, dim3(THREADS), smem, c->stream, true, p.share, tm_w, tm_a, p);
   else cuca_launch(kernel, grid, dim3(THREADS), smem, c->stream, true, tm_w, tm_a, p);
   CUCA_CHECK_LAUNCH("gemm_mx4");
