@@ -24,8 +24,11 @@ constexpr int SCALE_BYTES = 512;            // of 128 rows and a step
 constexpr int MAX_CLUSTER = 8;
 constexpr int MANY_ROWS = 256;              // more rows than these: two blocks of features
 constexpr int MANY_TILE = 192;              // ... and tiles of so many rows: two accumulators leave 128 columns for scales
-constexpr int READ_WARP = 2, READ_WARPS = 8, ROW_WARP = READ_WARP + READ_WARPS;
-constexpr int THREADS = 32 * (ROW_WARP + 1);  // a warp that loads weights, one that multiplies, eight that read results, one that loads rows
+// A warp that loads weights, one that loads rows, one that multiplies, and the others read results: sixteen of tiles of many rows, whose
+// reading nothing hides, eight of small ones, of which an SM takes two.
+constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 2, READ_WARP = 4;
+constexpr int read_warps(int spans) { return spans == 2 ? 16 : 8; }
+constexpr int threads(int spans) { return 32 * (READ_WARP + read_warps(spans)); }
 constexpr int BARRIERS = 512;
 
 struct Params {
@@ -41,9 +44,10 @@ struct Params {
 };
 
 template <int BLOCKS, bool DUAL, int SPANS, int G>
-__global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
+__global__ void __launch_bounds__(threads(SPANS), SPANS == 2 ? 1 : 2) gemm_mx4_codes_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
                                                                  const Params p) {
   static_assert(!DUAL || BLOCKS == 2, "gate and up");
+  constexpr int READ_WARPS = read_warps(SPANS), SETS = READ_WARPS / 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = (uint64_t*)(smem + p.stages * p.stage_bytes);
@@ -94,7 +98,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
     *ok_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
+  if (warp == MMA_WARP) {
     tmem_alloc(tmem_slot, p.tmem_cols);
     tmem_relinquish();
   }
@@ -104,7 +108,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   const uint32_t acc = *tmem_slot;
   const uint32_t scale_cols = acc + BLOCKS * p.nt;  // of each stage and step [block of features][4], [128 rows of A][4]
 
-  if (warp == 0) {
+  if (warp == WEIGHT_WARP) {
     // ------------------------------------------------ weights
     if (lane == 0) {  // the first ones into L2: that needs no wait for the kernel before, whatever it writes
       const Tile t = tile_at(first_tile);
@@ -171,7 +175,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == MMA_WARP) {
     // ------------------------------------------------ products. What a stage issues stands unrolled, its descriptors one addition from
     // the first stage's: an instruction whose operands are worked out beside it takes twice as long to issue, and a stage has seventeen
     pdl_wait();
@@ -221,25 +225,23 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
       if (ok && elect_one()) umma_commit(done);
       __syncwarp();
     }
-  } else {
-    // ------------------------------------------------ results: of two blocks of features a set of four warps takes each, else halves of the columns
+  } else if (warp >= READ_WARP) {
+    // ------------------------------------------------ results: sets of four warps take a part of the columns each, of one of two blocks of
+    // features or of both accumulators of a gated unit
     pdl_wait();
-    const int set = (warp - READ_WARP) >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
-    float* sums = reinterpret_cast<float*>(smem);  // (of a cluster: every copy into the stages has been waited for)
+    constexpr int PARTS = BLOCKS == 2 && !DUAL ? SETS / 2 : SETS;
+    const int set = (warp - READ_WARP) >> 2, part = set % PARTS, block = set / PARTS, row = (warp & 3) * 32 + lane;
+    const uint32_t at = acc + block * p.nt + ((uint32_t)((warp & 3) * 32) << 16);
+    float* sums = reinterpret_cast<float*>(smem) + block * (p.nt / G) * TILE_A;  // (of a cluster: every copy into the stages has been waited for)
     Mx4Ring acc_ring;
     for (int tile = first_tile; tile < p.tiles; tile += tile_step, acc_ring.next(1)) {
       const Tile t = tile_at(tile);
       if (!warp_wait(done, acc_ring.parity, p.err, abort_flag)) break;
       tc_fence_after();
-      if (BLOCKS == 2 && !DUAL) {
-        if (set == 0 || t.scaled)
-          mx4_leave<G, false>(p.o, at + set * p.nt, t.t0, t.m_here, t.n0 + set * TILE_A, row, p.share == 1, sums + set * (p.nt / G) * TILE_A);
-      } else {
-        const int half = ((t.nt / 2 + 15) & ~15) / G, first = set * half, last = set ? t.m_here : min(half, t.m_here);
-        if (last > first)
-          mx4_leave<G, DUAL>(p.o, at + first * G, t.t0 + first, last - first, t.n0, row, p.share == 1, sums + first * TILE_A, p.nt, p.nt / G);
-      }
+      const int each = (((t.nt + PARTS - 1) / PARTS + 15) & ~15) / G, first = part * each, last = min(first + each, t.m_here);
+      if (last > first && (block == 0 || t.scaled))
+        mx4_leave<G, DUAL>(p.o, at + first * G, t.t0 + first, last - first, t.n0 + block * TILE_A, row, p.share == 1, sums + first * TILE_A,
+                           p.nt, p.nt / G);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_free);
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mx4_codes_kernel(const __grid_co
   if (*abort_flag) mx4_let_copies_land();
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(acc, p.tmem_cols);
+  if (warp == MMA_WARP) tmem_dealloc(acc, p.tmem_cols);
   if (p.share > 1) {
     const float* sums = reinterpret_cast<const float*>(smem);
     const Tile t = tile_at(first_tile);
@@ -297,8 +299,8 @@ int launch_spans(const CucaMx4Gemm* c) {
   if (int e = mx4_configure<kernel>(227 * 1024)) return e;
   p.tiles = (int)tiles;
   const dim3 grid(p.share > 1 || tiles < slots ? (unsigned)(tiles * p.share) : (unsigned)slots);
-  if (p.share > 1) cuca_launch_cluster(kernel, grid, dim3(THREADS), smem, c->stream, true, p.share, tm_w, tm_a, p);
-  else cuca_launch(kernel, grid, dim3(THREADS), smem, c->stream, true, tm_w, tm_a, p);
+  if (p.share > 1) cuca_launch_cluster(kernel, grid, dim3(threads(SPANS)), smem, c->stream, true, p.share, tm_w, tm_a, p);
+  else cuca_launch(kernel, grid, dim3(threads(SPANS)), smem, c->stream, true, tm_w, tm_a, p);
   CUCA_CHECK_LAUNCH("gemm_mx4");
   return 0;
 }

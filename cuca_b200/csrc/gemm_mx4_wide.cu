@@ -43,7 +43,7 @@ struct Params {
 };
 
 template <bool DUAL, int KC>
-__global__ void __launch_bounds__(THREADS) gemm_mx4_wide_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+__global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                                                                 const Params p) {
   constexpr int BLOCKS = DUAL ? 2 : 1;  // runs of weight rows, each with its scales
   constexpr int CODE_STAGE = CODE_BYTES + BLOCKS * STAGE_STEPS * SCALE_BYTES;

@@ -115,15 +115,21 @@ struct Mx4Column {
 
 // Sixteen columns of this thread's lane as 16 / G results: G columns are one row of A (its digits, the smallest added first).
 template <int G>
-__device__ __forceinline__ void mx4_take16(uint32_t at, float (&y)[16 / G]) {
-  float v[16];
-  tmem_ld16(at, v);
+__device__ __forceinline__ void mx4_sum16(const uint32_t (&r)[16], float (&y)[16 / G]) {
 #pragma unroll
   for (int i = 0; i < 16 / G; ++i) {
-    y[i] = v[i * G + G - 1];
+    y[i] = __uint_as_float(r[i * G + G - 1]);
 #pragma unroll
-    for (int j = G - 2; j >= 0; --j) y[i] += v[i * G + j];
+    for (int j = G - 2; j >= 0; --j) y[i] += __uint_as_float(r[i * G + j]);
   }
+}
+__device__ __forceinline__ void mx4_ask16(uint32_t at, uint32_t (&r)[16]) {  // to be waited for
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at) : "memory");
 }
 // A finished tile: lane `row` (0..127) of tensor memory holds weight row `row` of the tile, G columns `at`.. each of the m_here rows of A
 // from m0 on. Alone they are results, features from n0 on; else they go to shared memory, [row of A][128], for mx4_join. GATED: the up
@@ -135,9 +141,13 @@ __device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, 
   const bool live = n0 + row < o.n;
   Mx4Column out(o, m0, live ? n0 + row : 0);
   for (int c = 0; c < m_here; c += N) {
+    uint32_t r[16], q[16];
+    mx4_ask16(at + c * G, r);
+    if (GATED) mx4_ask16(at + apart + c * G, q);
+    tmem_ld_wait();
     float v[N], u[N];
-    mx4_take16<G>(at + c * G, v);
-    if (GATED) mx4_take16<G>(at + apart + c * G, u);
+    mx4_sum16<G>(r, v);
+    if (GATED) mx4_sum16<G>(q, u);
     if (!alone) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
