@@ -8,95 +8,143 @@
 // equal rows make equal bytes whatever their type, alignment or place. A block of zeros has byte 0. A block that is not finite has
 // byte 255 and codes 0 and reads back as NaN whole: codes have no infinity and no NaN of their own.
 //
-// Both kernels do a few operations per byte: bound by memory, by the launch where rows are few. A thread takes eight values, four
-// threads a block, and sixteen write the four bytes of their step's scales as one word.
+// Both are bound by memory, by the launch where rows are few. A thread takes sixteen values, two threads a block, and eight write the four
+// bytes of their step's scales as one word: with eight values a thread what is done once a thread bound them (2,048 x 14,336
+// bfloat16 numbers to 4 bits and back 43 us).
 #include "mx4.cuh"
 
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int RUN = 8;  // values of a thread
+constexpr int RUN = 16;         // values of a thread
+constexpr int DIGIT_RUN = 8;    // ... that makes digits
 
 struct RowsParams {
   const void* x;
   void* out;
   uint8_t* codes;
   uint8_t* scales;
-  int64_t ldx, first, rows;  // rows of this launch start at `first`
+  int64_t ldx, first;
+  uint32_t rows;    // of this launch, from `first` on
+  uint32_t runs;    // of a row
+  uint32_t magic, shift;  // i / runs = (i * magic >> 32) >> shift, for i below 2^31
   int cols, steps;
-  bool wide;  // rows start on 16 bytes
+  int align;  // rows start on so many bytes: 32, 16 or less
 };
 
-template <typename T> struct Eight { float v[RUN]; uint32_t most; };  // eight values and the bits of the largest magnitude
+// Row of the launch and run of it that thread i has.
+__device__ __forceinline__ uint32_t split(const RowsParams& p, uint32_t i, uint32_t& run) {
+  const uint32_t row = __umulhi(i, p.magic) >> p.shift;
+  run = i - row * p.runs;
+  return row;
+}
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-template <typename T>
-__device__ __forceinline__ Eight<T> load8(const RowsParams& p, int64_t row, int c) {
-  Eight<T> e;
+// 32 bytes, past L1.
+__device__ __forceinline__ void load32(const void* src, int align, uint32_t (&w)[8]) {
+  if (align == 32) {
+    asm volatile("ld.relaxed.gpu.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(src) : "memory");
+  } else {
+    const uint4 a = __ldcg((const uint4*)src), b = __ldcg((const uint4*)src + 1);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  }
+}
+__device__ __forceinline__ void store32(void* dst, int align, const uint32_t (&w)[8]) {
+  if (align == 32) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+  } else {
+    *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
+    *((uint4*)dst + 1) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// N values of a row from c on; zeros past its end.
+template <typename T, int N>
+__device__ __forceinline__ void load(const RowsParams& p, int64_t row, int c, float (&v)[N]) {
   const T* src = (const T*)p.x + row * p.ldx + c;
-  if (p.wide && c + RUN <= p.cols) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 q = __ldcg(reinterpret_cast<const uint4*>(src));
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if (p.align >= 16 && c + N <= p.cols) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e.v[2 * i] = __uint_as_float(w[i] << 16);
-        e.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < N; i += 8) {
+        uint32_t w[8];
+        load32(src + i, p.align, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i + j] = __uint_as_float(w[j]);
       }
     } else {
-      const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
-      e.v[0] = a.x; e.v[1] = a.y; e.v[2] = a.z; e.v[3] = a.w;
-      e.v[4] = b.x; e.v[5] = b.y; e.v[6] = b.z; e.v[7] = b.w;
+      uint32_t w[8];
+      if constexpr (N == 16) {
+        load32(src, p.align, w);
+      } else {
+        const uint4 q = __ldcg((const uint4*)src);
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+      }
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < RUN; ++i) e.v[i] = c + i < p.cols ? to_f32(src[i]) : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = c + i < p.cols ? to_f32(src[i]) : 0.f;
   }
-  e.most = 0;
-#pragma unroll
-  for (int i = 0; i < RUN; ++i) e.most = max(e.most, magnitude(e.v[i]));
-  return e;
 }
+
+// Rows off 16 bytes go through shared memory: the eight threads of a step ask for values next to each other, each eighth of a step at a
+// time, and then take their sixteen. (Each asking for its own sixteen, 1,003 x 2,050 32-bit numbers took 25 us to 4 bits and back, 14 so.)
+__device__ __forceinline__ int staged(int value) {  // of a step's 128; sixteen of a thread lie a bank apart from the next thread's
+  return (threadIdx.x >> 3) * (MX4_STEP + 8) + value + (value >> 4);
+}
+constexpr int STAGED = THREADS / 8 * (MX4_STEP + 8);
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams p) {
   pdl_trigger();
   pdl_wait();
-  const int runs = p.steps * (MX4_STEP / RUN);  // of a row, a multiple of 16
-  const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-  // (32 bits: a launch has at most 2^31 runs)
-  const int64_t in = (uint32_t)i / (uint32_t)runs;
-  const int run = (int)((uint32_t)i - (uint32_t)in * (uint32_t)runs);
-  const bool live = in < p.rows;  // the sixteen threads of a step alike
-  const int64_t row = p.first + (live ? in : 0);
-  Eight<T> e;
-  e.most = 0;
+  uint32_t run;
+  const uint32_t in = split(p, blockIdx.x * THREADS + threadIdx.x, run);
+  const bool live = in < p.rows;  // the eight threads of a step alike
+  const int64_t row = p.first + in;
+  float v[RUN];
+  if (p.align < 16) {
+    __shared__ float stage[STAGED];
+    const int c = (int)(run & ~7u) * RUN + (threadIdx.x & 7);
+    const T* src = (const T*)p.x + row * p.ldx + c;
 #pragma unroll
-  for (int j = 0; j < RUN; ++j) e.v[j] = 0.f;
-  if (live) e = load8<T>(p, row, run * RUN);
-  uint32_t most = e.most;
+    for (int j = 0; j < RUN; ++j) stage[staged(j * 8 + (threadIdx.x & 7))] = live && c + j * 8 < p.cols ? to_f32(src[j * 8]) : 0.f;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) v[j] = stage[staged((threadIdx.x & 7) * RUN + j)];
+  } else if (live) {
+    load<T, RUN>(p, row, run * RUN, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) v[j] = 0.f;
+  }
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < RUN; ++j) most = max(most, magnitude(v[j]));  // (of a NaN above all others)
   most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-  most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
   const bool finite = most < 0x7f800000u;
   const uint32_t field = most >> 23;
   const uint32_t byte = finite ? (field > 2 ? field - 2 : 0) : 255u;
-  const float inv = __uint_as_float((254u - min(byte, 252u)) << 23);  // 2^-e
-  uint32_t word = 0;
-  if (finite) {
+  const float inv = finite ? __uint_as_float((254u - min(byte, 252u)) << 23) : 0.f;  // 2^-e
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = mx4_first_of(j);
-      word |= mx4_code_pair(e.v[i] * inv, e.v[i + 2] * inv) << (8 * j);
-    }
-  }
+  for (int j = 0; j < RUN; ++j) v[j] *= inv;
+  uint2 words = make_uint2(mx4_codes(v), mx4_codes(v + 8));
+  if (!finite) words = make_uint2(0, 0);
   // the four blocks' bytes, lowest first, by the step's first thread
-  const uint32_t s1 = __shfl_down_sync(0xffffffffu, byte, 4), s2 = __shfl_down_sync(0xffffffffu, byte, 8),
-                 s3 = __shfl_down_sync(0xffffffffu, byte, 12);
+  const uint32_t s1 = __shfl_down_sync(0xffffffffu, byte, 2), s2 = __shfl_down_sync(0xffffffffu, byte, 4),
+                 s3 = __shfl_down_sync(0xffffffffu, byte, 6);
   if (!live) return;
-  *reinterpret_cast<uint32_t*>(p.codes + row * (p.steps * 64ll) + run * 4) = word;
-  if ((run & 15) == 0)
-    *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(row, run >> 4, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
+  *reinterpret_cast<uint2*>(p.codes + row * (p.steps * 64ll) + run * 8) = words;
+  if ((run & 7) == 0)
+    *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(row, run >> 3, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
 }
 
 // Rows of 16 or 32 bits as eight rows in 4 bits each, whose values add up to theirs: digits of three bits (mx4_digit). After eight what is
@@ -106,20 +154,18 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p) {
   pdl_trigger();
   pdl_wait();
-  const int runs = p.steps * (MX4_STEP / RUN);
-  const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-  const int64_t in = (uint32_t)i / (uint32_t)runs;
-  const int run = (int)((uint32_t)i - (uint32_t)in * (uint32_t)runs);
+  uint32_t run;
+  const uint32_t in = split(p, blockIdx.x * THREADS + threadIdx.x, run);
   const bool live = in < p.rows;
-  const int64_t row = p.first + (live ? in : 0);
-  Eight<T> e;
+  const int64_t row = p.first + in;
+  float v[DIGIT_RUN];
 #pragma unroll
-  for (int j = 0; j < RUN; ++j) e.v[j] = 0.f;
-  if (live) e = load8<T>(p, row, run * RUN);
+  for (int j = 0; j < DIGIT_RUN; ++j) v[j] = 0.f;
+  if (live) load<T, DIGIT_RUN>(p, row, run * DIGIT_RUN, v);
 #pragma unroll
   for (int t = 0; t < MX4_DIGITS; ++t) {
     uint32_t byte, word;
-    mx4_digit(e.v, byte, word);
+    mx4_digit(v, byte, word);
     const uint32_t s1 = __shfl_down_sync(0xffffffffu, byte, 4), s2 = __shfl_down_sync(0xffffffffu, byte, 8),
                    s3 = __shfl_down_sync(0xffffffffu, byte, 12);
     if (live) {
@@ -137,10 +183,10 @@ __global__ void __launch_bounds__(THREADS) mx4_align_kernel(const __nv_bfloat16*
   pdl_wait();
   const __nv_bfloat16* src = x + blockIdx.x * ldx;
   __nv_bfloat16* dst = out + (int64_t)blockIdx.x * ldo;
-  for (int c = threadIdx.x * RUN; c < ldo; c += THREADS * RUN) {
+  for (int c = threadIdx.x * DIGIT_RUN; c < ldo; c += THREADS * DIGIT_RUN) {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < RUN; ++j)
+    for (int j = 0; j < DIGIT_RUN; ++j)
       if (c + j < cols) w[j >> 1] |= (uint32_t)__ldcg(reinterpret_cast<const unsigned short*>(src) + c + j) << (16 * (j & 1));
     *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -150,35 +196,53 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) mx4_values_kernel(const RowsParams p) {
   pdl_trigger();
   pdl_wait();
-  const int runs = (p.cols + RUN - 1) / RUN;
-  const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-  const int64_t in = (uint32_t)i / (uint32_t)runs;
-  if (in >= p.rows) return;
-  const int c = (int)((uint32_t)i - (uint32_t)in * (uint32_t)runs) * RUN;
-  const int64_t row = p.first + in;
-  const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(p.codes + row * (p.steps * 64ll) + c / 2));
-  const uint32_t byte = __ldcg(p.scales + mx4_scale_at(row, c >> 7, p.steps) + ((c >> 5) & 3));
-  T* dst = (T*)p.out + row * p.ldx + c;
-  T v[RUN];
-  const float power = mx4_power(byte);
+  uint32_t run;
+  const uint32_t in = split(p, blockIdx.x * THREADS + threadIdx.x, run);
+  const bool live = in < p.rows;
+  if (!live && p.align >= 16) return;
+  const int64_t row = live ? p.first + in : p.first;
+  const int c = (int)run * RUN;
+  const uint2 words = __ldcg(reinterpret_cast<const uint2*>(p.codes + row * (p.steps * 64ll) + c / 2));
+  const Mx4Factor f = mx4_factor<true>(__ldcg(p.scales + mx4_scale_at(row, c >> 7, p.steps) + ((c >> 5) & 3)));
+  uint32_t r[8];  // as bfloat16 numbers, which the values are exactly
+  uint32_t t[4];
+  mx4_to_bf16<true>(words.x, f, t);
 #pragma unroll
-  for (int j = 0; j < RUN; ++j) {
-    const uint32_t code = word >> (4 * ((j >> 1) + (j & 1) * 4));
-    // the code's bits as a 32-bit number times 2^-126, brought up exactly
-    const float x = __uint_as_float((code & 8) << 28 | (code & 7) << 22) * 8.507059173023462e+37f;  // 2^126
-    v[j] = from_f32<T>(x * power);
-  }
-  if (p.wide && c + RUN <= p.cols) {
+  for (int i = 0; i < 4; ++i) r[i] = t[i];
+  mx4_to_bf16<true>(words.y, f, t);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[4 + i] = t[i];
+  T* dst = (T*)p.out + row * p.ldx + c;
+  if (p.align >= 16 && c + RUN <= p.cols) {
     if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+      store32(dst, p.align, r);
     } else {
-      *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(v);
-      *reinterpret_cast<float4*>(dst + 4) = *reinterpret_cast<const float4*>(v + 4);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[2 * i] = r[4 * h + i] << 16;
+          w[2 * i + 1] = r[4 * h + i] & 0xffff0000u;
+        }
+        store32(dst + 8 * h, p.align, w);
+      }
     }
+  } else if (p.align < 16) {  // as rows come in
+    __shared__ float stage[STAGED];
+#pragma unroll
+    for (int j = 0; j < RUN; ++j)
+      stage[staged((threadIdx.x & 7) * RUN + j)] = __uint_as_float(j & 1 ? r[j / 2] & 0xffff0000u : r[j / 2] << 16);
+    __syncwarp();
+    const int c0 = (int)(run & ~7u) * RUN + (threadIdx.x & 7);
+    dst = (T*)p.out + row * p.ldx + c0;
+#pragma unroll
+    for (int j = 0; j < RUN; ++j)
+      if (live && c0 + j * 8 < p.cols) dst[j * 8] = from_f32<T>(stage[staged(j * 8 + (threadIdx.x & 7))]);
   } else {
 #pragma unroll
     for (int j = 0; j < RUN; ++j)
-      if (c + j < p.cols) dst[j] = v[j];
+      if (c + j < p.cols) dst[j] = from_f32<T>(__uint_as_float(j & 1 ? r[j / 2] & 0xffff0000u : r[j / 2] << 16));
   }
 }
 
@@ -191,18 +255,22 @@ int launch_rows(const CucaMx4Rows* c, Form form) {
   CUCA_REQUIRE(c->ldx >= c->cols || c->rows <= 1, "%s: rows overlap", what);
   CUCA_REQUIRE((((uintptr_t)c->codes | (uintptr_t)c->scales) & 15) == 0, "%s: codes and scales must start on 16 bytes", what);
   const int64_t elem = c->dtype == CUCA_F32 ? 4 : 2, steps = mx4_steps(c->cols);
-  const int64_t runs = form == VALUES ? (c->cols + RUN - 1) / RUN : steps * (MX4_STEP / RUN);
-  RowsParams p{c->x, c->x, c->codes, c->scales, c->ldx, 0, 0, (int)c->cols, (int)steps, false};
-  p.wide = ((uintptr_t)c->x & 15) == 0 && (c->ldx * elem % 16 == 0 || c->rows == 1);
+  const int64_t runs = steps * (MX4_STEP / (form == DIGITS ? DIGIT_RUN : RUN));
+  RowsParams p{c->x, c->x, c->codes, c->scales, c->ldx, 0, 0, (uint32_t)runs, 0, 0, (int)c->cols, (int)steps, 1};
+  for (int align = 32; align >= 16 && p.align == 1; align /= 2)
+    if ((uintptr_t)c->x % align == 0 && (c->ldx * elem % align == 0 || c->rows == 1)) p.align = align;
+  // magic = ceil(2^(32 + shift) / runs) with 2^shift < runs <= 2^(shift + 1) is below 2^32 and off by less than one: exact below 2^31
+  while ((2ll << p.shift) < runs) ++p.shift;
+  p.magic = (uint32_t)(((1ull << (32 + p.shift)) + runs - 1) / runs);
   const bool f32 = c->dtype == CUCA_F32;
   auto kernel = form == QUANTISE ? (f32 ? mx4_quantise_kernel<float> : mx4_quantise_kernel<__nv_bfloat16>)
                 : form == VALUES ? (f32 ? mx4_values_kernel<float> : mx4_values_kernel<__nv_bfloat16>)
                                  : (f32 ? mx4_digits_kernel<float> : mx4_digits_kernel<__nv_bfloat16>);
-  const int64_t most = (1ll << 31) / runs;  // rows of a launch
+  const int64_t most = ((1ll << 31) - THREADS) / runs;  // rows of a launch
   for (int64_t at = 0; at < c->rows; at += most) {
     p.first = at;
-    p.rows = c->rows - at < most ? c->rows - at : most;
-    const dim3 grid((unsigned)((p.rows * runs + THREADS - 1) / THREADS));
+    p.rows = (uint32_t)(c->rows - at < most ? c->rows - at : most);
+    const dim3 grid((unsigned)((p.rows * (uint64_t)runs + THREADS - 1) / THREADS));
     cuca_launch(kernel, grid, dim3(THREADS), 0, c->stream, true, p);
     CUCA_CHECK_LAUNCH(what);
   }

@@ -71,14 +71,16 @@ __device__ __forceinline__ float mx4_power(uint32_t e) {
   return __uint_as_float(e == 255 ? 0x7fffffffu : e ? e << 23 : 1u << 22);
 }
 
-// Two values' codes: to the nearest, ties to even, at most 6; the first in the low half.
-__device__ __forceinline__ uint32_t mx4_code_pair(float lo, float hi) {
-  uint32_t d;
-  asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\ncvt.u32.u8 %0, b;\n}\n" : "=r"(d) : "f"(lo), "f"(hi));
-  return d;
+// Eight values' codes as a word: to the nearest, ties to even, at most 6.
+__device__ __forceinline__ uint32_t mx4_codes(const float* v) {
+  uint32_t w;
+  asm("{\n.reg .b8 a, b, c, d;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %3, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %7, %5;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %4, %2;\ncvt.rn.satfinite.e2m1x2.f32 d, %8, %6;\n"
+      "mov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(w) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return w;
 }
-// The bytes of a word of codes hold values 0 and 2, 4 and 6, 1 and 3, 5 and 7: the first value of byte j
-__host__ __device__ constexpr int mx4_first_of(int j) { return (j & 1) * 4 + (j >> 1); }
 
 // A digit of eight values, a quarter of a block whose other quarters the three neighbouring lanes have. With a = max |v| of the block,
 //
@@ -106,8 +108,7 @@ __device__ __forceinline__ void mx4_digit(float (&v)[8], uint32_t& byte, uint32_
       d[j] = __fadd_rn(__fmul_rn(v[j], down), 6291456.f) - 6291456.f;  // 1.5 * 2^22, whose last place is 1/2
       v[j] = fmaf(-d[j], up, v[j]);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) word |= mx4_code_pair(d[mx4_first_of(j)], d[mx4_first_of(j) + 2]) << (8 * j);
+    word = mx4_codes(d);
   } else {
     byte = 255;
 #pragma unroll

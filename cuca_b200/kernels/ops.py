@@ -1974,9 +1974,12 @@ class Mx4Matrix:
         return self.codes.numel() + self.scales.numel()
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (what the latter calls, without its Python)
+
+
 def _here(*devices) -> int:
     """The current device, which all of the given device numbers have to be: a launch goes to its stream."""
-    here = torch.cuda.current_device() if devices[0] >= 0 else -1
+    here = _current_device() if devices[0] >= 0 else -1
     for d in devices:
         if d != here or d < 0:
             if d < 0:
@@ -2026,7 +2029,7 @@ def mx4_quantise(x, out: Mx4Matrix | None = None) -> Mx4Matrix:
 def mx4_values(a: Mx4Matrix, out) -> None:
     """out (32 or 16 bits) = the values that rows in 4 bits stand for, exactly."""
     ld = _mx4_rows(out, "values")
-    if tuple(out.shape) != a.shape:
+    if out.shape != a.shape:
         raise library.KernelError(f"values of {a.shape} rows in 4 bits do not fit {tuple(out.shape)}")
     device = _here(out.get_device(), a.device_index)
     library.check(library.load().cuca_mx4_values(_MX4_ROWS.pack(
@@ -2048,7 +2051,7 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
         if N % 2 or bias is not None:
             raise library.KernelError("a gated unit takes as many gate rows as up rows, and no bias")
         N //= 2
-    if wk != K or tuple(out.shape) != (M, N):
+    if wk != K or out.shape != (M, N):
         raise library.KernelError(f"rows {tuple(a.shape)} times a weight {w.shape} do not make {tuple(out.shape)}")
     ldo = _mx4_rows(out, "results")
     if type(a) is Mx4Matrix:
@@ -2064,7 +2067,7 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
     bias_at = err_at = bias_f32 = 0
     if bias is not None:
         bias_f32 = dtype_code(bias.dtype) == F32
-        if tuple(bias.shape) != (N,) or not bias.is_contiguous():
+        if bias.shape != (N,) or not bias.is_contiguous():
             raise library.KernelError(f"gemm_mx4: a bias is {N} numbers without gaps, not {tuple(bias.shape)}")
         _here(bias.get_device())
         bias_at = bias.data_ptr()
