@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
       mbar_init(&code_empty[s], CONVERT_WARPS);
     }
     for (int s = 0; s < p.ring; ++s) {
-      mbar_init(&full[s], 1 + (KC == MX4_STEP ? CONVERT_WARPS : CONVERT_WARPS / 2));
+      mbar_init(&full[s], 1 + CONVERT_WARPS / 2);
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
     if (ok && elect_one()) umma_commit(done);
     __syncwarp();
   } else {
-    // ------------------------------------------------ conversion: of each 128 values a set of four warps takes 64, a row a lane
+    // ------------------------------------------------ conversion, a row a lane: two sets of four warps take steps in turn
     pdl_wait();
     const int quarter = warp & 3, set = (warp - CONVERT_WARP) >> 2, row = quarter * 32 + lane;
     const int block = DUAL && row >= HALF;
@@ -175,35 +175,47 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
 #pragma unroll
       for (int s = 0; s < STAGE_STEPS; ++s) {
         if (ks * STAGE_STEPS + s >= p.k_steps) break;
-        const uint32_t bytes = (far ? __ldcg(reinterpret_cast<const uint32_t*>(far_scales + (ks * STAGE_STEPS + s) * 512ll))
-                                    : *reinterpret_cast<const uint32_t*>(sp + scale_at + s * SCALE_BYTES)) >> (16 * set);
-        const uint4 q[2] = {*reinterpret_cast<const uint4*>(codes + (((s * 4 + set * 2) ^ (row & 7)) << 4)),
-                            *reinterpret_cast<const uint4*>(codes + (((s * 4 + set * 2 + 1) ^ (row & 7)) << 4))};
-        uint32_t r[32];
-        auto convert = [&](auto large) {
+        if (KC == MX4_STEP && s != set) {
+          ring.next(p.ring);
+          continue;
+        }
+        const uint32_t bytes = far ? __ldcg(reinterpret_cast<const uint32_t*>(far_scales + (ks * STAGE_STEPS + s) * 512ll))
+                                   : *reinterpret_cast<const uint32_t*>(sp + scale_at + s * SCALE_BYTES);
+        const bool large = __any_sync(0xffffffffu, bytes & 0x80808080u);
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const Mx4Factor f = mx4_factor<decltype(large)::value>((bytes >> (8 * b)) & 255);
-            const uint32_t words[4] = {q[b].x, q[b].y, q[b].z, q[b].w};
+        for (int i = 0; i < KC / BOX_K; ++i) {
+          const int h = KC == MX4_STEP ? i : set;  // 64 of the 128 values
+          const uint4 q[2] = {*reinterpret_cast<const uint4*>(codes + (((s * 4 + h * 2) ^ (row & 7)) << 4)),
+                              *reinterpret_cast<const uint4*>(codes + (((s * 4 + h * 2 + 1) ^ (row & 7)) << 4))};
+          uint32_t r[32];
+          auto convert = [&](auto is_large) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t t[4];
-              mx4_to_bf16<decltype(large)::value>(words[i], f, t);
+            for (int b = 0; b < 2; ++b) {
+              const Mx4Factor f = mx4_factor<decltype(is_large)::value>((bytes >> (16 * h + 8 * b)) & 255);
+              const uint32_t words[4] = {q[b].x, q[b].y, q[b].z, q[b].w};
 #pragma unroll
-              for (int j = 0; j < 4; ++j) r[b * 16 + i * 4 + j] = t[j];
+              for (int k = 0; k < 4; ++k) {
+                uint32_t t[4];
+                mx4_to_bf16<decltype(is_large)::value>(words[k], f, t);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[b * 16 + k * 4 + j] = t[j];
+              }
             }
+          };
+          if (large) convert(std::true_type{});
+          else convert(std::false_type{});
+          if (i == 0) {
+            if (!warp_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) { ok = false; break; }
+            tc_fence_after();
           }
-        };
-        if (__any_sync(0xffffffffu, bytes & 0x8080u)) convert(std::true_type{});
-        else convert(std::false_type{});
-        if (!warp_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) { ok = false; break; }
-        tc_fence_after();
-        tmem_st32_raw(w_cols + ring.at * COLS + (KC < MX4_STEP ? 0 : set * 32) + lanes, r);
+          tmem_st32_raw(w_cols + ring.at * COLS + i * (BOX_K / 2) + lanes, r);
+        }
+        if (!ok) break;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[ring.at]);
-        ring.next(p.ring, MX4_STEP / KC);
+        ring.next(p.ring, KC == MX4_STEP ? 1 : 2);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&code_empty[codes_ring.at]);
