@@ -8,8 +8,8 @@
 // shared memory as one bulk copy and from there by tcgen05.cp into four columns of tensor memory, columns of their own for each
 // stage, which are free when the stage is. A tile of A's rows may start at any multiple of 64: scales are taken
 // from the 128 rows that it starts in, two columns further on.
-// Nothing is converted, so few rows are bound by the weight's bytes. Few tiles: a cluster of up to eight blocks shares K; each
-// leaves its sums in shared memory and adds an eighth of the features up in order out of the others': no workspace, equal bits in
+// Nothing is converted, so few rows are bound by the weight's bytes. Few tiles: a cluster of up to four blocks shares K; each
+// leaves its sums in shared memory and adds its part of the features up in order out of the others': no workspace, equal bits in
 // every run.
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
@@ -21,7 +21,7 @@ constexpr int STAGE_STEPS = 2;              // of 128 values
 constexpr int MAX_STAGES = 8;
 constexpr int W_BYTES = TILE_A * STAGE_BYTES_K;
 constexpr int SCALE_BYTES = 512;            // of 128 rows and a step
-constexpr int MAX_CLUSTER = 8;
+constexpr int MAX_CLUSTER = 4;              // (shares of K; eight took as long or longer: 14336 x 4096, 8 rows as digits 15.0 us, four 13.5)
 constexpr int MANY_ROWS = 256;              // more rows than these: two blocks of features
 constexpr int MANY_TILE = 192;              // ... and tiles of so many rows: two accumulators leave 128 columns for scales
 // A warp that loads weights, one that loads rows, one that multiplies, and the others read results: sixteen of tiles of many rows, whose
