@@ -95,7 +95,7 @@ struct Mx4Column {
   __device__ void put(float y) const {
     y += bias;
     if (!f32) *(__nv_bfloat16*)at = __float2bfloat16_rn(y);
-    else if (add) *(float*)at += y;
+    else if (add) atomicAdd((float*)at, y);  // one thread owns the place: its result is not waited for, as that of a load would be
     else *(float*)at = y;
   }
   __device__ void put2(float y, float z) const {  // z: of the next feature, its bias added; for places on two results' size
@@ -104,9 +104,9 @@ struct Mx4Column {
       *(__nv_bfloat162*)at = __floats2bfloat162_rn(y, z);
     } else {
       if (add) {
-        const float2 old = *(const float2*)at;
-        y += old.x;
-        z += old.y;
+        atomicAdd((float*)at, y);
+        atomicAdd((float*)at + 1, z);
+        return;
       }
       *(float2*)at = make_float2(y, z);
     }
