@@ -173,6 +173,31 @@ def test_gated_unit(kind, m, k, n):
     assert err.item() == 0
 
 
+@pytest.mark.parametrize("kind", ["bf16", "codes"])
+@pytest.mark.parametrize("m,k,n", [(4, 300, 100), (40, 300, 192), (300, 700, 130)])
+def test_gated_unit_in_32_bits(kind, m, k, n):
+    from cuca_b200.kernels import ops
+    a, x, q, w = _operands(kind, m, k, 2 * n, m)
+    out = torch.full((m, n), 7.0, device="cuda")
+    ops.gemm_mx4(a, q, out, ops.EPI_SWIGLU)
+    _check(out, *_product(kind, x, w, "swiglu", F32))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_one_shape_with_every_epilogue_in_turn(kind):
+    """What a call needs of memory depends on its epilogue too: the same rows and sizes, one after the other, from a fresh memory of it."""
+    from cuca_b200.kernels import ops
+    m, k, n = 20, 128, 64
+    a, x, q, w = _operands(kind, m, k, n, 1)
+    for order in ((ops.EPI_STORE, ops.EPI_SWIGLU, ops.EPI_RESIDUAL), (ops.EPI_SWIGLU, ops.EPI_STORE)):
+        ops._mx4_scratch.clear()
+        for epilogue in order:
+            gated = epilogue == ops.EPI_SWIGLU
+            out = torch.zeros(m, n // 2 if gated else n, device="cuda")
+            ops.gemm_mx4(a, q, out, epilogue)
+            _check(out, *_product(kind, x, w, "swiglu" if gated else "store", F32))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("m", [2, 40, 300])
 def test_strides(kind, m):
@@ -307,6 +332,60 @@ def test_a_chain_in_a_graph(m):
         _check(stream, y2, b1 + b2)
 
 
+@pytest.mark.parametrize("m", [2, 20, 90])
+def test_two_graphs_at_once(m):
+    """Two captured graphs replayed on two streams at once keep what they make for themselves apart."""
+    from cuca_b200.kernels import ops
+    k, n = 2048, 512
+    cases, graphs = [_operands("bf16", m, k, n, s) for s in (1, 2)], []
+    outs = [torch.zeros(m, n, device="cuda") for _ in cases]
+    for (a, _, q, _), out in zip(cases, outs):
+        ops.gemm_mx4(a, q, out)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(20):
+                ops.gemm_mx4(a, q, out)
+        graphs.append(g)
+        out.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, x, _, w), out in zip(cases, outs):
+        _check(out, *_product("bf16", x, w, "store", F32))
+
+
+def test_codes_past_2_to_the_31_bytes():
+    """A weight and rows whose codes reach past 2^31 bytes: their ends are where they should be."""
+    from cuca_b200.kernels import ops
+    n, k = 140_001, 32_768
+    w = _rows(2048, k, BF16, 1, 0.0)
+    big = torch.empty(n, k, dtype=BF16, device="cuda")
+    for at in range(0, n, 2048):
+        big[at:at + 2048] = w[:min(2048, n - at)]
+    big[-3:] = _rows(3, k, BF16, 2, 0.0)
+    q = ops.mx4_quantise(big)
+    assert q.codes.numel() > 2 ** 31
+    tail = mx.held(big[-200:])
+    back = torch.empty(n, k, dtype=BF16, device="cuda")
+    ops.mx4_values(q, back)
+    assert torch.equal(back[-200:].double(), tail)
+    del back
+    for m in (2, 33):
+        x = _rows(m, k, BF16, 3, 0.0)
+        out = torch.empty(m, n, dtype=BF16, device="cuda")
+        ops.gemm_mx4(x, q, out)
+        _check(out[:, -200:], *_product("bf16", x.double(), tail, "store", BF16))
+    few = ops.mx4_quantise(big[:70].contiguous())
+    out = torch.empty(n, 70, dtype=BF16, device="cuda")
+    ops.gemm_mx4(q, few, out)
+    _check(out[-200:], *_product("codes", tail, mx.held(big[:70]), "store", BF16))
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     from cuca_b200.kernels import library, ops
@@ -326,6 +405,11 @@ def test_refusals():
     refuse(x, w, out, bias=torch.zeros(10, device="cuda").cpu())
     refuse(x, w, out, bias=torch.zeros(9, dtype=BF16, device="cuda"))
     refuse(x, w, out, 7)
+    refuse(x, w, out, err=torch.zeros(1, device="cuda"))
+    refuse(x, w, out, err=torch.zeros(1, dtype=torch.int32))
+    off = ops.Mx4Matrix(10, 64, torch.zeros(10 * 64 + 8, dtype=torch.uint8, device="cuda")[8:].view(10, 64), w.scales)
+    refuse(x, off, out)  # codes off 16 bytes
+    refuse(ops.mx4_quantise(x), off, out)
     refuse(x.cpu(), w, out)
     refuse(x, ops.mx4_quantise(_rows(9, 64, F32, 2)), torch.empty(4, 4, dtype=BF16, device="cuda"), ops.EPI_SWIGLU)
     refuse(x, w, torch.empty(1, 10, dtype=BF16, device="cuda").expand(4, 10))
