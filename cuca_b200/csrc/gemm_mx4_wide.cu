@@ -13,6 +13,8 @@
 // what it waits for is one barrier a step, on which the converted weights and the rows arrive, and a step is 128 values of a row
 // but for the largest tiles, whose rows' tiles would leave two steps in shared memory.
 // Few tiles: a cluster of up to eight blocks shares K and adds its sums in order out of each other's shared memory.
+// The tensor cores cut off what a sum has no bits for (14,336 values in a row: 1.7e-6 off, of one sign 1.6e-5), so 32-bit results leave
+// after 8,192 values at most and what follows is added to them with rounding (6e-7; leaving costs a tenth of that).
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
 #include <type_traits>
@@ -27,16 +29,18 @@ constexpr int SCALE_BYTES = 512;            // of 128 rows and a step
 constexpr int BOX_K = 64;                   // values of a row in a box of X
 constexpr int MAX_CODES = 5, MAX_RING = 4, MAX_CLUSTER = 8;
 constexpr int MOST_ROWS = 256;              // of X in a tile
+constexpr int SUM_STAGES = 32;              // of codes that one 32-bit sum runs over at most
 constexpr int CONVERT_WARP = 2, CONVERT_WARPS = 8, X_WARP = CONVERT_WARP + CONVERT_WARPS;
 constexpr int THREADS = 32 * (X_WARP + 1);  // a warp that loads codes, one that multiplies, eight that convert, one that loads rows
 constexpr int BARRIERS = 512;
 
 struct Params {
   const uint8_t* w_scales;
-  Mx4Out o;
+  Mx4Out o, more;   // where results go; what is added to them later
   int k_steps, k_stages;
   int nt;  // rows of X of a whole tile, a multiple of 16
   int tiles_n, share;
+  int sum_stages;   // stages of codes after which results leave
   int codes, ring;  // stages of codes; steps in shared (rows) and tensor memory (weights)
   int tmem_cols;
   int* err;
@@ -58,7 +62,8 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
   uint64_t* full = code_empty + MAX_CODES;
   uint64_t* empty = full + MAX_RING;
   uint64_t* done = empty + MAX_RING;
-  uint32_t* tmem_slot = (uint32_t*)(done + 1);
+  uint64_t* acc_free = done + 1;
+  uint32_t* tmem_slot = (uint32_t*)(acc_free + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* ok_flag = (volatile int*)(tmem_slot + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -81,6 +86,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
+    mbar_init(acc_free, CONVERT_WARPS);
     *abort_flag = 0;
     *ok_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -138,23 +144,29 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
     const uint32_t idesc = instr_desc((m_here + 15) & ~15);
     const uint64_t x0 = smem_desc(smem_u32(smem));
     const uint32_t x_stride = x_bytes >> 4, box_stride = box_bytes >> 4;
-    Mx4Ring ring;
+    Mx4Ring ring, acc_ring;
     bool ok = true;
-    for (int c = 0; c < steps; ++c, ring.next(p.ring)) {
-      if (!warp_wait(&full[ring.at], ring.parity, p.err, abort_flag)) { ok = false; break; }
+    const int run = p.sum_stages * (STAGE_STEPS * MX4_STEP / KC);
+    for (int from = 0; ok && from < steps; from += run, acc_ring.next(1)) {
+      const int to = min(from + run, steps);
+      if (!warp_wait(acc_free, acc_ring.parity ^ 1, p.err, abort_flag)) break;
       tc_fence_after();
-      const uint64_t x = x0 + ring.at * x_stride;
-      const uint32_t w = w_cols + ring.at * COLS;
-      if (elect_one()) {
+      for (int c = from; c < to; ++c, ring.next(p.ring)) {
+        if (!warp_wait(&full[ring.at], ring.parity, p.err, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t x = x0 + ring.at * x_stride;
+        const uint32_t w = w_cols + ring.at * COLS;
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < KC / UMMA_K; ++k)
-          umma_bf16_tmem_a(acc, w + k * 8, x + (k >> 2) * box_stride + (uint64_t)((k & 3) * UMMA_K * 2 >> 4), idesc, k > 0 ? 1u : c > 0);
-        umma_commit(&empty[ring.at]);
+          for (int k = 0; k < KC / UMMA_K; ++k)
+            umma_bf16_tmem_a(acc, w + k * 8, x + (k >> 2) * box_stride + (uint64_t)((k & 3) * UMMA_K * 2 >> 4), idesc, k > 0 ? 1u : c > from);
+          umma_commit(&empty[ring.at]);
+        }
+        __syncwarp();
       }
+      if (ok && elect_one()) umma_commit(done);
       __syncwarp();
     }
-    if (ok && elect_one()) umma_commit(done);
-    __syncwarp();
   } else {
     // ------------------------------------------------ conversion, a row a lane: two sets of four warps take steps in turn
     pdl_wait();
@@ -165,67 +177,75 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
     const uint8_t* far_scales = p.w_scales + mx4_scale_at(w_row, 0, p.k_steps);
     const int scale_at = CODE_BYTES + block * STAGE_STEPS * SCALE_BYTES + (w_row & 31) * 16 + ((w_row >> 5) & 3) * 4;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    Mx4Ring codes_ring, ring;
+    Mx4Ring codes_ring, ring, acc_ring;
     if (KC < MX4_STEP) ring.next(p.ring, set);
     bool ok = true;
-    for (int ks = ks0; ok && ks < ks1; ++ks, codes_ring.next(p.codes)) {
-      const uint8_t* sp = code_smem + codes_ring.at * CODE_STAGE;
-      const uint8_t* codes = sp + row * STAGE_BYTES_K;
-      if (!warp_wait(&code_full[codes_ring.at], codes_ring.parity, p.err, abort_flag)) { ok = false; break; }
+    for (int from = ks0; ok && from < ks1; from += p.sum_stages, acc_ring.next(1)) {
+      const int to = min(from + p.sum_stages, ks1);
+      for (int ks = from; ok && ks < to; ++ks, codes_ring.next(p.codes)) {
+        const uint8_t* sp = code_smem + codes_ring.at * CODE_STAGE;
+        const uint8_t* codes = sp + row * STAGE_BYTES_K;
+        if (!warp_wait(&code_full[codes_ring.at], codes_ring.parity, p.err, abort_flag)) { ok = false; break; }
 #pragma unroll
-      for (int s = 0; s < STAGE_STEPS; ++s) {
-        if (ks * STAGE_STEPS + s >= p.k_steps) break;
-        if (KC == MX4_STEP && s != set) {
-          ring.next(p.ring);
-          continue;
-        }
-        const uint32_t bytes = far ? __ldcg(reinterpret_cast<const uint32_t*>(far_scales + (ks * STAGE_STEPS + s) * 512ll))
-                                   : *reinterpret_cast<const uint32_t*>(sp + scale_at + s * SCALE_BYTES);
-        const bool large = __any_sync(0xffffffffu, bytes & 0x80808080u);
-#pragma unroll
-        for (int i = 0; i < KC / BOX_K; ++i) {
-          const int h = KC == MX4_STEP ? i : set;  // 64 of the 128 values
-          const uint4 q[2] = {*reinterpret_cast<const uint4*>(codes + (((s * 4 + h * 2) ^ (row & 7)) << 4)),
-                              *reinterpret_cast<const uint4*>(codes + (((s * 4 + h * 2 + 1) ^ (row & 7)) << 4))};
-          uint32_t r[32];
-          auto convert = [&](auto is_large) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const Mx4Factor f = mx4_factor<decltype(is_large)::value>((bytes >> (16 * h + 8 * b)) & 255);
-              const uint32_t words[4] = {q[b].x, q[b].y, q[b].z, q[b].w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                uint32_t t[4];
-                mx4_to_bf16<decltype(is_large)::value>(words[k], f, t);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) r[b * 16 + k * 4 + j] = t[j];
-              }
-            }
-          };
-          if (large) convert(std::true_type{});
-          else convert(std::false_type{});
-          if (i == 0) {
-            if (!warp_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) { ok = false; break; }
-            tc_fence_after();
+        for (int s = 0; s < STAGE_STEPS; ++s) {
+          if (ks * STAGE_STEPS + s >= p.k_steps) break;
+          if (KC == MX4_STEP && s != set) {
+            ring.next(p.ring);
+            continue;
           }
-          tmem_st32_raw(w_cols + ring.at * COLS + i * (BOX_K / 2) + lanes, r);
+          const uint32_t bytes = far ? __ldcg(reinterpret_cast<const uint32_t*>(far_scales + (ks * STAGE_STEPS + s) * 512ll))
+                                     : *reinterpret_cast<const uint32_t*>(sp + scale_at + s * SCALE_BYTES);
+          const bool large = __any_sync(0xffffffffu, bytes & 0x80808080u);
+#pragma unroll
+          for (int i = 0; i < KC / BOX_K; ++i) {
+            const int h = KC == MX4_STEP ? i : set;  // 64 of the 128 values
+            const uint4 q[2] = {*reinterpret_cast<const uint4*>(codes + (((s * 4 + h * 2) ^ (row & 7)) << 4)),
+                                *reinterpret_cast<const uint4*>(codes + (((s * 4 + h * 2 + 1) ^ (row & 7)) << 4))};
+            uint32_t r[32];
+            auto convert = [&](auto is_large) {
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                const Mx4Factor f = mx4_factor<decltype(is_large)::value>((bytes >> (16 * h + 8 * b)) & 255);
+                const uint32_t words[4] = {q[b].x, q[b].y, q[b].z, q[b].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  uint32_t t[4];
+                  mx4_to_bf16<decltype(is_large)::value>(words[k], f, t);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) r[b * 16 + k * 4 + j] = t[j];
+                }
+              }
+            };
+            if (large) convert(std::true_type{});
+            else convert(std::false_type{});
+            if (i == 0) {
+              if (!warp_wait(&empty[ring.at], ring.parity ^ 1, p.err, abort_flag)) { ok = false; break; }
+              tc_fence_after();
+            }
+            tmem_st32_raw(w_cols + ring.at * COLS + i * (BOX_K / 2) + lanes, r);
+          }
+          if (!ok) break;
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[ring.at]);
+          ring.next(p.ring, KC == MX4_STEP ? 1 : 2);
         }
-        if (!ok) break;
-        tmem_st_wait();
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[ring.at]);
-        ring.next(p.ring, KC == MX4_STEP ? 1 : 2);
+        if (lane == 0) mbar_arrive(&code_empty[codes_ring.at]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&code_empty[codes_ring.at]);
-    }
-    // ------------------------------------------------ results: the sets take halves of the columns
-    if (ok && warp_wait(done, 0, p.err, abort_flag)) {
+      // ---------------------------------------------- results: the sets take halves of the columns
+      if (!ok || !warp_wait(done, acc_ring.parity, p.err, abort_flag)) break;
       tc_fence_after();
       const int half = ((m_here + 1) / 2 + 15) & ~15, first = set * half, last = set ? m_here : min(half, m_here);
-      if (last > first)
-        mx4_leave<1, false>(p.o, acc + first + lanes, m0 + first, last - first, n0, row, !DUAL && p.share == 1, reinterpret_cast<float*>(smem) + first * TILE_A);
+      float* const sums = reinterpret_cast<float*>(smem) + first * TILE_A;
+      if (last > first) {
+        if (DUAL || from == ks0) mx4_leave<1, false>(p.o, acc + first + lanes, m0 + first, last - first, n0, row, !DUAL && p.share == 1, sums);
+        else mx4_leave<1, false>(p.more, acc + first + lanes, m0 + first, last - first, n0, row, true, sums);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_free);
       if (threadIdx.x == CONVERT_WARP * 32) *ok_flag = 1;
     }
   }
@@ -262,6 +282,12 @@ int launch(const CucaMx4Gemm* c, int nt) {
   const int slots = cuca_device_sms() * (two ? 2 : 1);
   p.share = 1;
   while (p.share < MAX_CLUSTER && tiles * p.share * 2 <= slots && p.k_stages >= p.share * 4) p.share *= 2;
+  // (a gated unit's sums, and those that a cluster adds up, run over all of a block's stages)
+  const int sums = !DUAL && p.share == 1 && c->out_f32 ? (p.k_stages + SUM_STAGES - 1) / SUM_STAGES : 1;
+  p.sum_stages = (p.k_stages + sums - 1) / sums;
+  p.more = p.o;
+  p.more.bias = nullptr;
+  p.more.epilogue = EPI_RESIDUAL;
   const int data = p.codes * CODE_STAGE + p.ring * x_bytes;
   CUCA_REQUIRE(p.codes >= 2 && p.ring >= 2 && p.tmem_cols <= (two ? 256 : 512) && data >= nt * TILE_A * 4, "gemm_mx4: no room for a tile");
   const uint64_t lda = c->m == 1 ? (c->k + 7) / 8 * 8 : c->lda;  // (of one row there is no stride)

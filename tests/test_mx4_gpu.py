@@ -359,6 +359,24 @@ def test_two_graphs_at_once(m):
         _check(out, *_product("bf16", x, w, "store", F32))
 
 
+@pytest.mark.parametrize("sign", [False, True])
+def test_long_sums_in_32_bits(sign):
+    """Of 17,000 values 32-bit sums run over 8,192 at most: 512 contractions in a row cut off at most 2^-23 of the sum each, in the mean
+    a quarter of that over a sum that grows from nothing."""
+    from cuca_b200.kernels import ops
+    m, k, n = 300, 17_000, 19_200
+    x, w = _rows(m, k, BF16, 1, 0.0), _rows(n, k, BF16, 2, 0.0)
+    if sign:
+        x, w = x.abs(), w.abs()
+    q = ops.mx4_quantise(w)
+    bias, stream = _rows(1, n, F32, 3)[0].contiguous(), _rows(m, n, F32, 4)
+    out = stream.clone()
+    ops.gemm_mx4(x, q, out, ops.EPI_RESIDUAL, bias)
+    some = torch.arange(0, n, 257, device="cuda")
+    want = x.double() @ mx.held(w[some]).T + bias[some].double() + stream[:, some].double()
+    assert (out[:, some].double() - want).norm() < 512 * 2.0 ** -25 * want.norm()
+
+
 def test_codes_past_2_to_the_31_bytes():
     """A weight and rows whose codes reach past 2^31 bytes: their ends are where they should be."""
     from cuca_b200.kernels import ops
