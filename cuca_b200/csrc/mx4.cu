@@ -9,8 +9,8 @@
 // byte 255 and codes 0 and reads back as NaN whole: codes have no infinity and no NaN of their own.
 //
 // Both are bound by memory, by the launch where rows are few. A thread takes sixteen values, two threads a block, and eight write the four
-// bytes of their step's scales as one word: with eight values a thread what is done once a thread bound them (2,048 x 14,336
-// bfloat16 numbers to 4 bits and back 43 us).
+// bytes of their step's scales as one word. 2,048 x 14,336 bfloat16 numbers to 4 bits and back take 26.5 us, 5.6 TB/s of what is read and
+// written; with eight values a thread, what is done once a thread bound them (43 us).
 #include "mx4.cuh"
 
 namespace {
@@ -96,7 +96,7 @@ __device__ __forceinline__ void load(const RowsParams& p, int64_t row, int c, fl
 }
 
 // Rows off 16 bytes go through shared memory: the eight threads of a step ask for values next to each other, each eighth of a step at a
-// time, and then take their sixteen. (Each asking for its own sixteen, 1,003 x 2,050 32-bit numbers took 25 us to 4 bits and back, 14 so.)
+// time, and then take their sixteen. (Each asking for its own sixteen, 1,003 x 2,050 32-bit numbers took 25 us to 4 bits and back; so 11.7, the host's pace.)
 __device__ __forceinline__ int staged(int value) {  // of a step's 128; sixteen of a thread lie a bank apart from the next thread's
   return (threadIdx.x >> 3) * (MX4_STEP + 8) + value + (value >> 4);
 }
