@@ -105,6 +105,13 @@ __global__ void __launch_bounds__(threads(SPANS), SPANS == 2 ? 1 : 2) gemm_mx4_c
     *ok_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == ROW_WARP && lane == 0) {  // the first weights into L2: that needs no wait for the kernel before, whatever it writes
+    const Tile t = tile_at(first_tile);
+    for (int ks = ks0; ks < ks1 && ks < ks0 + p.stages; ++ks) {
+      mx4_prefetch_2d(&tm_w, ks * 64, t.n0);
+      if (BLOCKS == 2) mx4_prefetch_2d(&tm_w, ks * 64, t.second);
+    }
+  }
   if (warp == MMA_WARP) {
     tmem_alloc(tmem_slot, p.tmem_cols);
     tmem_relinquish();
@@ -117,14 +124,6 @@ __global__ void __launch_bounds__(threads(SPANS), SPANS == 2 ? 1 : 2) gemm_mx4_c
 
   if (warp == WEIGHT_WARP) {
     // ------------------------------------------------ weights
-    if (lane == 0) {  // the first ones into L2: that needs no wait for the kernel before, whatever it writes
-      const Tile t = tile_at(first_tile);
-      for (int ks = ks0; ks < ks1 && ks < ks0 + p.stages; ++ks) {
-        mx4_prefetch_2d(&tm_w, ks * 64, t.n0);
-        if (BLOCKS == 2) mx4_prefetch_2d(&tm_w, ks * 64, t.second);
-      }
-    }
-    __syncwarp();
     pdl_wait();
     Mx4Ring ring;
     bool ok = true;

@@ -93,6 +93,12 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
     *ok_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == X_WARP && lane == 0) {  // the first weights into L2: that needs no wait for the kernel before, whatever it writes
+    for (int ks = ks0; ks < ks1 && ks < ks0 + p.codes; ++ks) {
+      mx4_prefetch_2d(&tm_w, ks * 64, n0);
+      mx4_prefetch_2d(&tm_w, ks * 64, second);
+    }
+  }
   if (warp == 1) {
     tmem_alloc(tmem_slot, p.tmem_cols);
     tmem_relinquish();
@@ -106,11 +112,6 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
   if (warp == 0) {
     // ------------------------------------------------ codes and scales
     if (lane == 0) {
-      // the first weights into L2: that needs no wait for the kernel before, whatever it writes
-      for (int ks = ks0; ks < ks1 && ks < ks0 + p.codes; ++ks) {
-        mx4_prefetch_2d(&tm_w, ks * 64, n0);
-        mx4_prefetch_2d(&tm_w, ks * 64, second);
-      }
       pdl_wait();
       Mx4Ring ring;
       for (int ks = ks0; ks < ks1; ++ks, ring.next(p.codes)) {
