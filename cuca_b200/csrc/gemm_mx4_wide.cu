@@ -16,7 +16,8 @@
 // but for the largest tiles, whose rows' tiles would leave two steps in shared memory.
 // Few tiles: a cluster of up to eight blocks shares K and adds its sums in order out of each other's shared memory.
 // The tensor cores cut off what a sum has no bits for (14,336 values in a row: 1.7e-6 off, of one sign 1.6e-5), so 32-bit results leave
-// after 8,192 values at most and what follows is added to them with rounding (6e-7; leaving costs a tenth of that).
+// after 8,192 values at most and what follows is added to them with rounding (6e-7; leaving costs a tenth of that). A result, and the
+// stream or bias in it, is so rounded once for each 8,192 values begun.
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
 #include <type_traits>
@@ -293,11 +294,10 @@ int launch(const CucaMx4Gemm* c, int nt) {
   p.more.epilogue = EPI_RESIDUAL;
   const int data = p.codes * CODE_STAGE + p.ring * x_bytes;
   CUCA_REQUIRE(p.codes >= 2 && p.ring >= 2 && p.tmem_cols <= (two ? 256 : 512) && data >= nt * TILE_A * 4, "gemm_mx4: no room for a tile");
-  const uint64_t lda = c->m == 1 ? (c->k + 7) / 8 * 8 : c->lda;  // (of one row there is no stride)
   CUtensorMap tm_w, tm_x;
   const uint64_t cols = (uint64_t)p.k_steps * 32;  // the codes as 16-bit elements
   CUCA_REQUIRE(cuca_tensor_map_2d(c->w, 2, (uint64_t)c->n * (DUAL ? 2 : 1), cols, cols, HALF, &tm_w) &&
-               cuca_tensor_map_2d(c->a, 2, (uint64_t)c->m, (uint64_t)c->k, lda, nt, &tm_x), "gemm_mx4: tensor map failed");
+               cuca_tensor_map_2d(c->a, 2, (uint64_t)c->m, (uint64_t)c->k, (uint64_t)c->lda, nt, &tm_x), "gemm_mx4: tensor map failed");
   constexpr auto kernel = gemm_mx4_wide_kernel<DUAL, KC>;
   if (int e = mx4_configure<kernel>(227 * 1024)) return e;
   const dim3 grid((unsigned)(tiles * p.share));

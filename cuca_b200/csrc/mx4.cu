@@ -91,7 +91,7 @@ __device__ __forceinline__ void load(const RowsParams& p, int64_t row, int c, fl
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = c + i < p.cols ? to_f32(src[i]) : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = c + i < p.cols ? mx4_read(src + i) : 0.f;
   }
 }
 
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams 
     const int c = (int)(run & ~7u) * RUN + (threadIdx.x & 7);
     const T* src = (const T*)p.x + row * p.ldx + c;
 #pragma unroll
-    for (int j = 0; j < RUN; ++j) stage[staged(j * 8 + (threadIdx.x & 7))] = live && c + j * 8 < p.cols ? to_f32(src[j * 8]) : 0.f;
+    for (int j = 0; j < RUN; ++j) stage[staged(j * 8 + (threadIdx.x & 7))] = live && c + j * 8 < p.cols ? mx4_read(src + j * 8) : 0.f;
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < RUN; ++j) v[j] = stage[staged((threadIdx.x & 7) * RUN + j)];

@@ -65,7 +65,14 @@ int mx4_configure(int smem) {
   if (device < 64) done.fetch_or(1ull << device, std::memory_order_relaxed);
   return 0;
 }
-// Reads go past L1 in all of these kernels: a launch that started before the one ahead had ended does not find L1 invalidated.
+
+// What an earlier kernel may have written is read past L1 in all of these kernels: a launch that started before the one ahead had ended
+// does not find L1 invalidated.
+__device__ __forceinline__ float mx4_read(const float* at) { return __ldcg(at); }
+__device__ __forceinline__ float mx4_read(const __nv_bfloat16* at) {
+  return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short*>(at)) << 16);
+}
+
 // 2^(e - 127); NaN for 255
 __device__ __forceinline__ float mx4_power(uint32_t e) {
   return __uint_as_float(e == 255 ? 0x7fffffffu : e ? e << 23 : 1u << 22);

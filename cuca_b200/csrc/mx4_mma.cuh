@@ -91,10 +91,11 @@ struct Mx4Column {
     const int size = o.out_f32 ? 4 : 2;
     at = (char*)o.out + (m * o.ldo + n) * size;
     step = o.ldo * size;
-    bias = !o.bias ? 0.f : o.bias_f32 ? ((const float*)o.bias)[n] : __bfloat162float(((const __nv_bfloat16*)o.bias)[n]);
+    bias = !o.bias ? 0.f : o.bias_f32 ? mx4_read((const float*)o.bias + n) : mx4_read((const __nv_bfloat16*)o.bias + n);
     f32 = o.out_f32;
     add = o.epilogue == EPI_RESIDUAL;
   }
+  // (an atomic takes and leaves numbers below 2^-126 as zeros)
   __device__ void put(float y) const {
     y += bias;
     if (!f32) *(__nv_bfloat16*)at = __float2bfloat16_rn(y);
