@@ -47,6 +47,7 @@ CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
   CUCA_REQUIRE((((uintptr_t)c->w | (uintptr_t)c->w_scales) & 15) == 0 &&
                (c->a_kind != MX4_CODES || (((uintptr_t)c->a | (uintptr_t)c->a_scales) & 15) == 0),
                "gemm_mx4: codes and scales must start on 16 bytes");
+  CUCA_REQUIRE(c->m <= 1 || (c->ldo >= c->n && (c->a_kind == MX4_CODES || c->lda >= c->k)), "gemm_mx4: rows overlap");
   if (c->m == 0 || c->n == 0) return 0;
   const Form form = form_of(c);
   CUCA_REQUIRE((form != DIGITS && form != ALIGNED) || (c->scratch && ((uintptr_t)c->scratch & 255) == 0),

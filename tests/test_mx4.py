@@ -50,6 +50,19 @@ def test_there_is_no_cpu_path():
             call()
 
 
+def test_rows_that_overlap_are_refused_at_the_c_entry():
+    """The host's checks come before any launch: no kernel runs here."""
+    from cuca_b200.kernels import library, ops
+    lib = library.load()
+    at = 1 << 20
+    for kind, lda, ldo in ((1, 63, 10), (0, 63, 10), (1, 64, 9), (2, 0, 9)):
+        call = ops._MX4_GEMM.pack(at, at, lda, kind, at, at, 0, at, ldo, 1, 0, 20, 10, 64, 0, at, 0, 0)
+        assert lib.cuca_gemm_mx4(call) != 0 and b"overlap" in lib.cuca_last_error()
+    call = ops._MX4_ROWS.pack(at, 63, 0, at, at, 2, 64, 0)
+    for entry in (lib.cuca_mx4_quantise, lib.cuca_mx4_values):
+        assert entry(call) != 0 and b"overlap" in lib.cuca_last_error()
+
+
 def test_the_formula_against_a_search():
     """The nearest of the sixteen values for every block, found by trying all of them."""
     g = torch.Generator().manual_seed(1)

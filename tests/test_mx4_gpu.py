@@ -377,6 +377,24 @@ def test_long_sums_in_32_bits(sign):
     assert (out[:, some].double() - want).norm() < 512 * 2.0 ** -25 * want.norm()
 
 
+@pytest.mark.parametrize("epilogue", [0, 1])
+def test_parts_of_a_long_sum_beside_a_large_stream(epilogue):
+    """Of 17,000 values three parts are added to the bias and the stream, each with one rounding, at most 2^-24 of what has been added;
+    a bias is added to the first part with one more."""
+    from cuca_b200.kernels import ops
+    m, k, n = 300, 17_000, 19_200
+    x, w = _rows(m, k, BF16, 1, 0.0) / 4096, _rows(n, k, BF16, 2, 0.0)
+    q = ops.mx4_quantise(w)
+    bias, out = _rows(1, n, F32, 3)[0].contiguous(), _rows(m, n, F32, 4)
+    some = torch.arange(0, n, 257, device="cuda")
+    rows, held = x.double(), mx.held(w[some])
+    want = rows @ held.T + bias[some].double() + epilogue * out[:, some].double()
+    most = rows.abs() @ held.abs().T + bias[some].double().abs() + epilogue * out[:, some].double().abs()
+    bound = 4 * 2.0 ** -24 * most + mx.chain_bound(rows, held, 512)
+    ops.gemm_mx4(x, q, out, epilogue, bias)
+    assert ((out[:, some].double() - want).abs() <= bound).all()
+
+
 def test_codes_past_2_to_the_31_bytes():
     """A weight and rows whose codes reach past 2^31 bytes: their ends are where they should be."""
     from cuca_b200.kernels import ops
