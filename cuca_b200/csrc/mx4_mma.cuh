@@ -10,7 +10,9 @@ __device__ __forceinline__ uint32_t mx4_cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// (.aligned: a warp's lanes come here together, whatever they did before)
 __device__ __forceinline__ void mx4_cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float2 mx4_peer_f32x2(uint32_t at) {  // an address that mapa made
@@ -165,6 +167,7 @@ __device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, 
         out.at += out.step;
       }
     }
+    __syncwarp();  // what is asked of tensor memory next is asked by all lanes together
   }
 }
 // The sums that the blocks of a cluster left, added up in order, each block for its part of the features; a block alone finishes its own.
