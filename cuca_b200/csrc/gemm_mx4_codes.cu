@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(threads(SPANS), SPANS == 2 ? 1 : 2) gemm_mx4_c
       const int each = (((t.nt + PARTS - 1) / PARTS + 15) & ~15) / G, first = part * each, last = min(first + each, t.m_here);
       if (last > first && (block == 0 || t.scaled))
         mx4_leave<G, DUAL>(p.o, at + first * G, t.t0 + first, last - first, t.n0 + block * TILE_A, row, p.share == 1, sums + first * TILE_A,
-                           p.nt, p.nt / G);
+                           false, p.nt, p.nt / G);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_free);

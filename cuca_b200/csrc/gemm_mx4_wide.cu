@@ -16,8 +16,9 @@
 // but for the largest tiles, whose rows' tiles would leave two steps in shared memory.
 // Few tiles: a cluster of up to eight blocks shares K and adds its sums in order out of each other's shared memory.
 // The tensor cores cut off what a sum has no bits for (14,336 values in a row: 1.7e-6 off, of one sign 1.6e-5), so 32-bit results leave
-// after 8,192 values at most and what follows is added to them with rounding (6e-7; leaving costs a tenth of that). A result, and the
-// stream or bias in it, is so rounded once for each 8,192 values begun.
+// after 8,192 values at most and what follows is added to them with rounding (6e-7; leaving costs a tenth of that), to results in
+// memory, or in shared memory where a cluster or a gated unit joins them later. A result, and the stream or bias in it, is so
+// rounded once for each 8,192 values begun.
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
 #include <type_traits>
@@ -32,6 +33,7 @@ constexpr int SCALE_BYTES = 512;            // of 128 rows and a step
 constexpr int BOX_K = 64;                   // values of a row in a box of X
 constexpr int MAX_CODES = 5, MAX_RING = 4, MAX_CLUSTER = 8;
 constexpr int MOST_ROWS = 256;              // of X in a tile
+constexpr int MOST_WAITING = 240;           // ... whose sums wait in shared memory of their own
 constexpr int SUM_STAGES = 32;              // of codes that one 32-bit sum runs over at most
 constexpr int CONVERT_WARP = 2, CONVERT_WARPS = 8, X_WARP = CONVERT_WARP + CONVERT_WARPS;
 constexpr int THREADS = 32 * (X_WARP + 1);  // a warp that loads codes, one that multiplies, eight that convert, one that loads rows
@@ -43,7 +45,9 @@ struct Params {
   int k_steps, k_stages;
   int nt;  // rows of X of a whole tile, a multiple of 16
   int tiles_n, share;
-  int sum_stages;   // stages of codes after which results leave
+  int sum_stages;   // stages of codes after which sums leave
+  int sums_at;      // bytes into shared memory where sums that leave and are not results yet go: over the stages, where a block leaves once,
+  int sums_bytes;   // else so many behind them
   int codes, ring;  // stages of codes; steps in shared (rows) and tensor memory (weights)
   int tmem_cols;
   int* err;
@@ -60,7 +64,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int box_bytes = p.nt * BOX_K * 2, x_bytes = BOXES * box_bytes;
   uint8_t* const code_smem = smem + p.ring * x_bytes;
-  uint64_t* code_full = (uint64_t*)(code_smem + p.codes * CODE_STAGE);
+  uint64_t* code_full = (uint64_t*)(code_smem + p.codes * CODE_STAGE + p.sums_bytes);
   uint64_t* code_empty = code_full + MAX_CODES;
   uint64_t* full = code_empty + MAX_CODES;
   uint64_t* empty = full + MAX_RING;
@@ -242,9 +246,10 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
       if (!ok || !warp_wait(done, acc_ring.parity, p.err, abort_flag)) break;
       tc_fence_after();
       const int half = ((m_here + 1) / 2 + 15) & ~15, first = set * half, last = set ? m_here : min(half, m_here);
-      float* const sums = reinterpret_cast<float*>(smem) + first * TILE_A;
+      float* const sums = reinterpret_cast<float*>(smem + p.sums_at) + first * TILE_A;
       if (last > first) {
-        if (DUAL || from == ks0) mx4_leave<1, false>(p.o, acc + first + lanes, m0 + first, last - first, n0, row, !DUAL && p.share == 1, sums);
+        const bool alone = !DUAL && p.share == 1;
+        if (!alone || from == ks0) mx4_leave<1, false>(p.o, acc + first + lanes, m0 + first, last - first, n0, row, alone, sums, from > ks0);
         else mx4_leave<1, false>(p.more, acc + first + lanes, m0 + first, last - first, n0, row, true, sums);
       }
       tc_fence_before();
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(acc, p.tmem_cols);
-  if (DUAL || p.share > 1) mx4_join<DUAL>(p.o, reinterpret_cast<const float*>(smem), m0, m_here, n0, rank, p.share, *ok_flag != 0);
+  if (DUAL || p.share > 1) mx4_join<DUAL>(p.o, reinterpret_cast<const float*>(smem + p.sums_at), m0, m_here, n0, rank, p.share, *ok_flag != 0);
 }
 
 template <bool DUAL, int KC>
@@ -277,23 +282,27 @@ int launch(const CucaMx4Gemm* c, int nt) {
   CUCA_REQUIRE(tiles * MAX_CLUSTER < (1ll << 31), "gemm_mx4: %lld rows by %lld features are too many", (long long)c->m, (long long)c->n);
   const bool two = nt <= 64;  // blocks an SM
   const int x_bytes = nt * KC * 2, budget = (two ? 108 : 222) * 1024;
-  p.ring = ((two ? 256 : 512) - nt) / (KC / 2);
-  if (p.ring > MAX_RING) p.ring = MAX_RING;
-  p.codes = (budget - p.ring * x_bytes) / CODE_STAGE;
-  if (p.codes > MAX_CODES) p.codes = MAX_CODES;
-  p.tmem_cols = 32;
-  while (p.tmem_cols < nt + p.ring * (KC / 2)) p.tmem_cols *= 2;
   const int slots = cuca_device_sms() * (two ? 2 : 1);
   p.share = 1;
   while (p.share < MAX_CLUSTER && tiles * p.share * 2 <= slots && p.k_stages >= p.share * 4) p.share *= 2;
-  // (a gated unit's sums, and those that a cluster adds up, run over all of a block's stages)
-  const int sums = !DUAL && p.share == 1 && c->out_f32 ? (p.k_stages + SUM_STAGES - 1) / SUM_STAGES : 1;
-  p.sum_stages = (p.k_stages + sums - 1) / sums;
+  const int stages = (p.k_stages + p.share - 1) / p.share;  // of a block, at most
+  const int sums = c->out_f32 ? (stages + SUM_STAGES - 1) / SUM_STAGES : 1;
+  p.sum_stages = (stages + sums - 1) / sums;
   p.more = p.o;
   p.more.bias = nullptr;
   p.more.epilogue = EPI_RESIDUAL;
-  const int data = p.codes * CODE_STAGE + p.ring * x_bytes;
-  CUCA_REQUIRE(p.codes >= 2 && p.ring >= 2 && p.tmem_cols <= (two ? 256 : 512) && data >= nt * TILE_A * 4, "gemm_mx4: no room for a tile");
+  const bool joined = DUAL || p.share > 1;  // what leaves goes to shared memory
+  p.sums_bytes = joined && sums > 1 ? nt * TILE_A * 4 : 0;
+  p.ring = ((two ? 256 : 512) - nt) / (KC / 2);
+  if (p.ring > MAX_RING) p.ring = MAX_RING;
+  while (p.ring > 2 && budget - p.sums_bytes - p.ring * x_bytes < 2 * CODE_STAGE) --p.ring;
+  p.codes = (budget - p.sums_bytes - p.ring * x_bytes) / CODE_STAGE;
+  if (p.codes > MAX_CODES) p.codes = MAX_CODES;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < nt + p.ring * (KC / 2)) p.tmem_cols *= 2;
+  const int stage_bytes = p.codes * CODE_STAGE + p.ring * x_bytes, data = stage_bytes + p.sums_bytes;
+  p.sums_at = p.sums_bytes ? stage_bytes : 0;
+  CUCA_REQUIRE(p.codes >= 2 && p.ring >= 2 && p.tmem_cols <= (two ? 256 : 512) && data - p.sums_at >= nt * TILE_A * 4, "gemm_mx4: no room for a tile");
   CUtensorMap tm_w, tm_x;
   const uint64_t cols = (uint64_t)p.k_steps * 32;  // the codes as 16-bit elements
   CUCA_REQUIRE(cuca_tensor_map_2d(c->w, 2, (uint64_t)c->n * (DUAL ? 2 : 1), cols, cols, HALF, &tm_w) &&
@@ -310,7 +319,12 @@ int launch(const CucaMx4Gemm* c, int nt) {
 
 template <bool DUAL>
 int launch_tiles(const CucaMx4Gemm* c) {
-  const int64_t tiles = (c->m + MOST_ROWS - 1) / MOST_ROWS, rows = (c->m + tiles - 1) / tiles;  // tiles of equal height
+  // 32-bit sums of many values that wait beside the stages leave room for fewer rows
+  const int64_t features = (c->n + (DUAL ? HALF : TILE_A) - 1) / (DUAL ? HALF : TILE_A);
+  const bool waits = c->out_f32 && c->k > SUM_STAGES * STAGE_STEPS * MX4_STEP &&
+                     (DUAL || features * ((c->m + MOST_ROWS - 1) / MOST_ROWS) * 2 <= cuca_device_sms());
+  const int64_t most = waits ? MOST_WAITING : MOST_ROWS;
+  const int64_t tiles = (c->m + most - 1) / most, rows = (c->m + tiles - 1) / tiles;  // tiles of equal height
   const int nt = (int)(rows + 15) / 16 * 16;
   return nt > 128 ? launch<DUAL, 64>(c, nt) : launch<DUAL, 128>(c, nt);
 }

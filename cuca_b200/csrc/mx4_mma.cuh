@@ -138,11 +138,11 @@ __device__ __forceinline__ void mx4_ask16(uint32_t at, uint32_t (&r)[16]) {  // 
       : "r"(at) : "memory");
 }
 // A finished tile: lane `row` (0..127) of tensor memory holds weight row `row` of the tile, G columns `at`.. each of the m_here rows of A
-// from m0 on. Alone they are results, features from n0 on; else they go to shared memory, [row of A][128], for mx4_join. GATED: the up
-// part's accumulator lies `apart` columns further on, in shared memory `up` rows.
+// from m0 on. Alone they are results, features from n0 on; else they go to shared memory, [row of A][128], for mx4_join (`again`: are added
+// to what this thread left there). GATED: the up part's accumulator lies `apart` columns further on, in shared memory `up` rows.
 template <int G, bool GATED>
-__device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, int m_here, int n0, int row, bool alone, float* sums, int apart = 0,
-                                          int up = 0) {
+__device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, int m_here, int n0, int row, bool alone, float* sums,
+                                          bool again = false, int apart = 0, int up = 0) {
   constexpr int N = 16 / G;
   const bool live = n0 + row < o.n;
   Mx4Column out(o, m0, live ? n0 + row : 0);
@@ -157,8 +157,11 @@ __device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, 
     if (!alone) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        sums[(c + j) * TILE_A + row] = v[j];
-        if (GATED) sums[(up + c + j) * TILE_A + row] = u[j];
+        if (c + j < m_here) {
+          float* const sum = sums + (c + j) * TILE_A + row;
+          *sum = again ? *sum + v[j] : v[j];
+          if (GATED) sum[up * TILE_A] = u[j];
+        }
       }
     } else if (live) {
 #pragma unroll

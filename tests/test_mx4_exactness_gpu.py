@@ -50,3 +50,40 @@ def test_ragged_tiles_that_share_a_long_sum(kind, m, n):
     for epilogue in ("store", "swiglu"):
         out, xv, wv = _multiply(kind, x, w, epilogue)
         _within(out, *mx.product(xv, wv, epilogue, F32, k / 16 + 24, digits=kind != "codes"))
+
+
+def _drift(values, one_sign=False):
+    """How far (2-norm over that of the result) a 32-bit sum of so many exact products may be off. The tensor cores take 16 at a time and cut
+    off at most 2^-23 of what has been summed. Cut off evenly up to that, with signs that vary over sums that grow as a square root,
+    n times come to sqrt(n / 6) of it; where everything has one sign half of it each time, over sums that are half the last in
+    the mean. One more for the rounding of what is left and joined."""
+    n = values / 16
+    return 2.0 ** -23 * ((n / 4 if one_sign else math.sqrt(n / 6)) + 1)
+
+
+@pytest.mark.parametrize("one_sign", [False, True])
+@pytest.mark.parametrize("m,k,n,epilogue", [
+    (200, 40_000, 8192, "store"), (20, 40_000, 9000, "residual"), (250, 36_000, 8192, "store"),
+    (200, 20_000, 9500, "swiglu"), (300, 20_000, 2050, "swiglu"), (40, 36_000, 4600, "swiglu"), (300, 17_000, 19_200, "store")])
+def test_long_sums_in_32_bits_leave_after_8192_values(m, k, n, epilogue, one_sign):
+    """Alone, in a cluster's shares and in a gated unit alike."""
+    gated = epilogue == "swiglu"
+    x, w = _normal(m, k, BF16, 1), _normal(2 * n if gated else n, k, BF16, 2) / math.sqrt(k)
+    if one_sign:
+        x, w = x.abs(), w.abs()
+    stream = _normal(m, n, F32, 3) if epilogue == "residual" else None
+    from cuca_b200.kernels import ops
+    some = torch.arange(0, n, 257, device="cuda")
+    held = mx.held(w[torch.cat((some, n + some)) if gated else some])
+    q = ops.mx4_quantise(w)
+    del w
+    out = torch.empty(m, n, device="cuda") if stream is None else stream.clone()
+    ops.gemm_mx4(x, q, out, {"store": ops.EPI_STORE, "swiglu": ops.EPI_SWIGLU, "residual": ops.EPI_RESIDUAL}[epilogue])
+    want = x.double() @ held.T
+    limit = _drift(8192, one_sign)
+    if gated:  # silu's slope is below 1.1, both factors are off
+        g, u = want.chunk(2, 1)
+        want, limit = g * torch.sigmoid(g) * u, 2.1 * limit
+    elif stream is not None:
+        want = want + stream[:, some].double()
+    assert (out[:, some].double() - want).norm() < limit * want.norm()
