@@ -2,9 +2,9 @@
 #include "mx4.cuh"
 
 int cuca_mx4_digits(const CucaMx4Rows* c);
-int cuca_mx4_align(const void* x, int64_t ldx, void* out, int ldo, int rows, int cols, cudaStream_t stream);
+int cuca_mx4_spread(const void* x, int64_t ldx, bool f32, void* out, int ldo, int rows, int cols, cudaStream_t stream);
 int cuca_gemm_mx4_codes(const CucaMx4Gemm* c, bool digits);
-int cuca_gemm_mx4_wide(const CucaMx4Gemm* c);
+int cuca_gemm_mx4_wide(const CucaMx4Gemm* c, bool parts);
 
 namespace {
 
@@ -13,11 +13,14 @@ namespace {
 // and 16.4, 24 rows 16.0 and 17.1, 32 rows 17.9 and 17.4; 4096 x 4096 24 rows 11.3 and 9.3.
 int most_digits(const CucaMx4Gemm* c) { return c->epilogue == EPI_SWIGLU ? 24 : 16; }
 
-enum Form { CODES, DIGITS, ALIGNED, WIDE };
+enum Form { CODES, DIGITS, PARTS, ALIGNED, WIDE };
 
 Form form_of(const CucaMx4Gemm* c) {
   if (c->a_kind == MX4_CODES) return CODES;
-  if (c->a_kind == CUCA_F32 || c->m <= most_digits(c)) return DIGITS;
+  // 32-bit rows are three bfloat16 rows each: digits, which share a power of two, would lose bits beside larger values. What that costs, us,
+  // with eight digits in brackets: 4096 x 4096 8 rows 10.8 (8.3), 256 rows 32 (34); 4096 x 14336 gated 8 rows 38 (16), 256 rows 203 (105).
+  if (c->a_kind == CUCA_F32) return PARTS;
+  if (c->m <= most_digits(c)) return DIGITS;
   return ((uintptr_t)c->a & 15) == 0 && c->lda % 8 == 0 ? WIDE : ALIGNED;  // rows that the copy engine takes
 }
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -27,6 +30,7 @@ int64_t scratch_of(const CucaMx4Gemm* c) {
   if (c->m <= 0 || c->n <= 0 || c->k <= 0) return 0;
   switch (form_of(c)) {
     case DIGITS: return digit_codes(c) + (c->m * MX4_DIGITS + 127) / 128 * mx4_steps(c->k) * 512;
+    case PARTS: return 3 * c->m * ((c->k + 7) / 8 * 16);
     case ALIGNED: return c->m * ((c->k + 7) / 8 * 16);
     default: return 0;
   }
@@ -50,7 +54,7 @@ CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
   CUCA_REQUIRE(c->m <= 1 || (c->ldo >= c->n && (c->a_kind == MX4_CODES || c->lda >= c->k)), "gemm_mx4: rows overlap");
   if (c->m == 0 || c->n == 0) return 0;
   const Form form = form_of(c);
-  CUCA_REQUIRE((form != DIGITS && form != ALIGNED) || (c->scratch && ((uintptr_t)c->scratch & 255) == 0),
+  CUCA_REQUIRE(form == CODES || form == WIDE || (c->scratch && ((uintptr_t)c->scratch & 255) == 0),
                "gemm_mx4: these rows need scratch on 256 bytes");
   try {
     CucaMx4Gemm d = *c;
@@ -61,12 +65,13 @@ CUCA_API int cuca_gemm_mx4(const CucaMx4Gemm* c) {
       if (int e = cuca_mx4_digits(&r)) return e;
       return cuca_gemm_mx4_codes(&d, true);
     }
-    if (form == ALIGNED) {
+    if (form == CODES) return cuca_gemm_mx4_codes(c, false);
+    if (form != WIDE) {
       d.a = c->scratch;
       d.lda = (c->k + 7) / 8 * 8;
-      if (int e = cuca_mx4_align(c->a, c->lda, c->scratch, (int)d.lda, (int)c->m, (int)c->k, c->stream)) return e;
+      if (int e = cuca_mx4_spread(c->a, c->lda, form == PARTS, c->scratch, (int)d.lda, (int)c->m, (int)c->k, c->stream)) return e;
     }
-    return form == CODES ? cuca_gemm_mx4_codes(c, false) : cuca_gemm_mx4_wide(&d);
+    return cuca_gemm_mx4_wide(&d, form == PARTS);
   } catch (...) {  // the cache of tensor maps may find no memory
     cuca_set_error("gemm_mx4: out of host memory");
     return 3;

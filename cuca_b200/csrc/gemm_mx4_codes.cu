@@ -13,7 +13,7 @@
 // its part of the features up in order out of the others': no workspace, equal bits in every run. Many tiles: a block takes tiles in turn,
 // the next one's loads under this one's results.
 //
-// Rows of 16 or 32 bits come here too where they are few, or of 32 bits, as eight digits each (mx4.cu): G columns make one row of the result.
+// Few bfloat16 rows come here too, as eight digits each (mx4.cu): G columns make one row of the result.
 //
 // Measured, K x features: 2,048 rows 4096 x 14336 gated 120 us (4.0 PFLOP/s; the tensor pipe busy for half of it: a stage takes 1,190
 // clocks of which its contractions need 768, and a tile's results are not hidden), 14336 x 4096 66 us (3.6); 8 rows 4096 x 6144 5.9 us;

@@ -1,4 +1,4 @@
-// bfloat16 rows times a weight in 4 bits on tcgen05: out = epilogue(X W^T).
+// bfloat16 rows, or 32-bit rows as three bfloat16 rows each (mx4.cu), times a weight in 4 bits on tcgen05: out = epilogue(X W^T).
 //
 // A code times its power of two is a bfloat16 number exactly, so what the tensor cores multiply is the weight as it is kept and the rows
 // as they are. The weight is the 128-row operand and comes out of tensor memory: converter warps take codes from shared memory, a weight
@@ -18,7 +18,8 @@
 // The tensor cores cut off what a sum has no bits for (14,336 values in a row: 1.7e-6 off, of one sign 1.6e-5), so 32-bit results leave
 // after 8,192 values at most and what follows is added to them with rounding (6e-7; leaving costs a tenth of that), to results in
 // memory, or in shared memory where a cluster or a gated unit joins them later. A result, and the stream or bias in it, is so
-// rounded once for each 8,192 values begun.
+// rounded once for each 8,192 values begun. Sums of 32-bit rows' parts leave after 2,048, always to shared memory, and are rounded into a
+// result once.
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
 #include <type_traits>
@@ -35,6 +36,7 @@ constexpr int MAX_CODES = 5, MAX_RING = 4, MAX_CLUSTER = 8;
 constexpr int MOST_ROWS = 256;              // of X in a tile
 constexpr int MOST_WAITING = 240;           // ... whose sums wait in shared memory of their own
 constexpr int SUM_STAGES = 32;              // of codes that one 32-bit sum runs over at most
+constexpr int SUM_STAGES_F32 = 8;           // ... of 32-bit rows
 constexpr int CONVERT_WARP = 2, CONVERT_WARPS = 8, X_WARP = CONVERT_WARP + CONVERT_WARPS;
 constexpr int THREADS = 32 * (X_WARP + 1);  // a warp that loads codes, one that multiplies, eight that convert, one that loads rows
 constexpr int BARRIERS = 512;
@@ -43,8 +45,10 @@ struct Params {
   const uint8_t* w_scales;
   Mx4Out o, more;   // where results go; what is added to them later
   int k_steps, k_stages;
-  int nt;  // rows of X of a whole tile, a multiple of 16
+  int nt;  // columns of a whole tile, a multiple of 16
+  int mt;  // ... and rows of the result: G columns make one
   int tiles_n, share;
+  bool joined;      // what leaves goes to shared memory and is joined later
   int sum_stages;   // stages of codes after which sums leave
   int sums_at;      // bytes into shared memory where sums that leave and are not results yet go: over the stages, where a block leaves once,
   int sums_bytes;   // else so many behind them
@@ -53,7 +57,8 @@ struct Params {
   int* err;
 };
 
-template <bool DUAL, int KC>
+// AGAIN: a block's sums leave several times, and wait in shared memory of their own
+template <bool DUAL, int KC, int G, bool AGAIN>
 __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                                                                 const Params p) {
   constexpr int BLOCKS = DUAL ? 2 : 1;  // runs of weight rows, each with its scales
@@ -76,8 +81,8 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.share > 1 ? (int)mx4_cluster_rank() : 0;
   const int tile = (int)blockIdx.x / p.share;
-  const int n0 = (tile % p.tiles_n) * FEATURES, m0 = (tile / p.tiles_n) * p.nt;
-  const int m_here = min(p.nt, p.o.m - m0);
+  const int n0 = (tile % p.tiles_n) * FEATURES, m0 = (tile / p.tiles_n) * p.mt;
+  const int m_here = min(p.mt, p.o.m - m0);
   const int ks0 = (int)((int64_t)p.k_stages * rank / p.share), ks1 = (int)((int64_t)p.k_stages * (rank + 1) / p.share);
   const int steps = (min(ks1 * STAGE_STEPS, p.k_steps) - ks0 * STAGE_STEPS) * (MX4_STEP / KC);  // of KC values
   const int second = DUAL ? p.o.n + n0 : n0 + HALF;  // weight row of the tile's second half
@@ -143,13 +148,13 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
         mbar_expect_tx(&full[ring.at], x_bytes);
 #pragma unroll
         for (int b = 0; b < BOXES; ++b)
-          tma_load_2d(smem + ring.at * x_bytes + b * box_bytes, &tm_x, &full[ring.at], k + b * BOX_K, m0);
+          tma_load_2d(smem + ring.at * x_bytes + b * box_bytes, &tm_x, &full[ring.at], k + b * BOX_K, m0 * G);
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------ products
     pdl_wait();
-    const uint32_t idesc = instr_desc((m_here + 15) & ~15);
+    const uint32_t idesc = instr_desc((m_here * G + 15) & ~15);
     const uint64_t x0 = smem_desc(smem_u32(smem));
     const uint32_t x_stride = x_bytes >> 4, box_stride = box_bytes >> 4;
     Mx4Ring ring, acc_ring;
@@ -248,9 +253,9 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
       const int half = ((m_here + 1) / 2 + 15) & ~15, first = set * half, last = set ? m_here : min(half, m_here);
       float* const sums = reinterpret_cast<float*>(smem + p.sums_at) + first * TILE_A;
       if (last > first) {
-        const bool alone = !DUAL && p.share == 1;
-        if (!alone || from == ks0) mx4_leave<1, false>(p.o, acc + first + lanes, m0 + first, last - first, n0, row, alone, sums, from > ks0);
-        else mx4_leave<1, false>(p.more, acc + first + lanes, m0 + first, last - first, n0, row, true, sums);
+        const uint32_t at = acc + first * G + lanes;
+        if (p.joined || from == ks0) mx4_leave<G, false>(p.o, at, m0 + first, last - first, n0, row, !p.joined, sums, AGAIN && from > ks0);
+        else mx4_leave<G, false>(p.more, at, m0 + first, last - first, n0, row, true, sums);
       }
       tc_fence_before();
       __syncwarp();
@@ -263,11 +268,11 @@ __global__ void __launch_bounds__(THREADS, 2) gemm_mx4_wide_kernel(const __grid_
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(acc, p.tmem_cols);
-  if (DUAL || p.share > 1) mx4_join<DUAL>(p.o, reinterpret_cast<const float*>(smem + p.sums_at), m0, m_here, n0, rank, p.share, *ok_flag != 0);
+  if (p.joined) mx4_join<DUAL>(p.o, reinterpret_cast<const float*>(smem + p.sums_at), m0, m_here, n0, rank, p.share, *ok_flag != 0);
 }
 
-template <bool DUAL, int KC>
-int launch(const CucaMx4Gemm* c, int nt) {
+template <bool DUAL, int KC, int G>
+int launch(const CucaMx4Gemm* c, int nt, int mt) {
   constexpr int CODE_STAGE = CODE_BYTES + (DUAL ? 2 : 1) * STAGE_STEPS * SCALE_BYTES;
   Params p;
   p.w_scales = c->w_scales;
@@ -276,9 +281,10 @@ int launch(const CucaMx4Gemm* c, int nt) {
   p.k_stages = (p.k_steps + STAGE_STEPS - 1) / STAGE_STEPS;
   p.err = c->err;
   p.nt = nt;
+  p.mt = mt;
   const int features = DUAL ? HALF : TILE_A;
   p.tiles_n = (int)((c->n + features - 1) / features);
-  const int64_t tiles = (int64_t)p.tiles_n * ((c->m + nt - 1) / nt);
+  const int64_t tiles = (int64_t)p.tiles_n * ((c->m + mt - 1) / mt);
   CUCA_REQUIRE(tiles * MAX_CLUSTER < (1ll << 31), "gemm_mx4: %lld rows by %lld features are too many", (long long)c->m, (long long)c->n);
   const bool two = nt <= 64;  // blocks an SM
   const int x_bytes = nt * KC * 2, budget = (two ? 108 : 222) * 1024;
@@ -286,13 +292,13 @@ int launch(const CucaMx4Gemm* c, int nt) {
   p.share = 1;
   while (p.share < MAX_CLUSTER && tiles * p.share * 2 <= slots && p.k_stages >= p.share * 4) p.share *= 2;
   const int stages = (p.k_stages + p.share - 1) / p.share;  // of a block, at most
-  const int sums = c->out_f32 ? (stages + SUM_STAGES - 1) / SUM_STAGES : 1;
+  const int most = G > 1 ? SUM_STAGES_F32 : SUM_STAGES, sums = c->out_f32 ? (stages + most - 1) / most : 1;
   p.sum_stages = (stages + sums - 1) / sums;
   p.more = p.o;
   p.more.bias = nullptr;
   p.more.epilogue = EPI_RESIDUAL;
-  const bool joined = DUAL || p.share > 1;  // what leaves goes to shared memory
-  p.sums_bytes = joined && sums > 1 ? nt * TILE_A * 4 : 0;
+  p.joined = DUAL || p.share > 1 || (G > 1 && sums > 1);
+  p.sums_bytes = p.joined && sums > 1 ? mt * TILE_A * 4 : 0;
   p.ring = ((two ? 256 : 512) - nt) / (KC / 2);
   if (p.ring > MAX_RING) p.ring = MAX_RING;
   while (p.ring > 2 && budget - p.sums_bytes - p.ring * x_bytes < 2 * CODE_STAGE) --p.ring;
@@ -302,33 +308,41 @@ int launch(const CucaMx4Gemm* c, int nt) {
   while (p.tmem_cols < nt + p.ring * (KC / 2)) p.tmem_cols *= 2;
   const int stage_bytes = p.codes * CODE_STAGE + p.ring * x_bytes, data = stage_bytes + p.sums_bytes;
   p.sums_at = p.sums_bytes ? stage_bytes : 0;
-  CUCA_REQUIRE(p.codes >= 2 && p.ring >= 2 && p.tmem_cols <= (two ? 256 : 512) && data - p.sums_at >= nt * TILE_A * 4, "gemm_mx4: no room for a tile");
+  CUCA_REQUIRE(p.codes >= 2 && p.ring >= 2 && p.tmem_cols <= (two ? 256 : 512) && data - p.sums_at >= mt * TILE_A * 4, "gemm_mx4: no room for a tile");
   CUtensorMap tm_w, tm_x;
   const uint64_t cols = (uint64_t)p.k_steps * 32;  // the codes as 16-bit elements
   CUCA_REQUIRE(cuca_tensor_map_2d(c->w, 2, (uint64_t)c->n * (DUAL ? 2 : 1), cols, cols, HALF, &tm_w) &&
-               cuca_tensor_map_2d(c->a, 2, (uint64_t)c->m, (uint64_t)c->k, (uint64_t)c->lda, nt, &tm_x), "gemm_mx4: tensor map failed");
-  constexpr auto kernel = gemm_mx4_wide_kernel<DUAL, KC>;
-  if (int e = mx4_configure<kernel>(227 * 1024)) return e;
+               cuca_tensor_map_2d(c->a, 2, (uint64_t)c->m * G, (uint64_t)c->k, (uint64_t)c->lda, nt, &tm_x), "gemm_mx4: tensor map failed");
   const dim3 grid((unsigned)(tiles * p.share));
   const int smem = data + 1024 + BARRIERS;
-  if (p.share > 1) cuca_launch_cluster(kernel, grid, dim3(THREADS), smem, c->stream, true, p.share, tm_w, tm_x, p);
-  else cuca_launch(kernel, grid, dim3(THREADS), smem, c->stream, true, tm_w, tm_x, p);
+  auto start = [&](auto again) {
+    constexpr auto kernel = gemm_mx4_wide_kernel<DUAL, KC, G, decltype(again)::value>;
+    if (int e = mx4_configure<kernel>(227 * 1024)) return e;
+    if (p.share > 1) cuca_launch_cluster(kernel, grid, dim3(THREADS), smem, c->stream, true, p.share, tm_w, tm_x, p);
+    else cuca_launch(kernel, grid, dim3(THREADS), smem, c->stream, true, tm_w, tm_x, p);
+    return 0;
+  };
+  if (int e = p.sums_bytes ? start(std::true_type{}) : start(std::false_type{})) return e;
   CUCA_CHECK_LAUNCH("gemm_mx4");
   return 0;
 }
 
-template <bool DUAL>
+template <bool DUAL, int G>
 int launch_tiles(const CucaMx4Gemm* c) {
   // 32-bit sums of many values that wait beside the stages leave room for fewer rows
   const int64_t features = (c->n + (DUAL ? HALF : TILE_A) - 1) / (DUAL ? HALF : TILE_A);
   const bool waits = c->out_f32 && c->k > SUM_STAGES * STAGE_STEPS * MX4_STEP &&
                      (DUAL || features * ((c->m + MOST_ROWS - 1) / MOST_ROWS) * 2 <= cuca_device_sms());
-  const int64_t most = waits ? MOST_WAITING : MOST_ROWS;
+  const int64_t most = (waits && G == 1 ? MOST_WAITING : MOST_ROWS) / G;
   const int64_t tiles = (c->m + most - 1) / most, rows = (c->m + tiles - 1) / tiles;  // tiles of equal height
-  const int nt = (int)(rows + 15) / 16 * 16;
-  return nt > 128 ? launch<DUAL, 64>(c, nt) : launch<DUAL, 128>(c, nt);
+  const int nt = (int)(rows * G + 15) / 16 * 16, mt = G > 1 ? (int)rows : nt;
+  return nt > 128 ? launch<DUAL, 64, G>(c, nt, mt) : launch<DUAL, 128, G>(c, nt, mt);
 }
 
 }  // namespace
 
-int cuca_gemm_mx4_wide(const CucaMx4Gemm* c) { return c->epilogue == EPI_SWIGLU ? launch_tiles<true>(c) : launch_tiles<false>(c); }
+// `parts`: X holds three rows for each of c->m
+int cuca_gemm_mx4_wide(const CucaMx4Gemm* c, bool parts) {
+  if (c->epilogue == EPI_SWIGLU) return parts ? launch_tiles<true, 3>(c) : launch_tiles<true, 1>(c);
+  return parts ? launch_tiles<false, 3>(c) : launch_tiles<false, 1>(c);
+}

@@ -147,10 +147,9 @@ __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams 
     *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(row, run >> 3, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
 }
 
-// Rows of 16 or 32 bits as eight rows in 4 bits each, whose values add up to theirs: digits of three bits (mx4_digit). After eight what is
-// left of a value is at most 2^-23 of its block's largest: of bfloat16 numbers nothing, where they are within 2^14 of it, and where
+// bfloat16 rows as eight rows in 4 bits each, whose values add up to theirs: digits of three bits (mx4_digit). After eight what is
+// left of a value is at most 2^-23 of its block's largest: nothing, where it is within 2^14 of it, and where
 // some are much larger than the rest the digits that these do not need go to the others.
-template <typename T>
 __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p) {
   pdl_trigger();
   pdl_wait();
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p)
   float v[DIGIT_RUN];
 #pragma unroll
   for (int j = 0; j < DIGIT_RUN; ++j) v[j] = 0.f;
-  if (live) load<T, DIGIT_RUN>(p, row, run * DIGIT_RUN, v);
+  if (live) load<__nv_bfloat16, DIGIT_RUN>(p, row, run * DIGIT_RUN, v);
 #pragma unroll
   for (int t = 0; t < MX4_DIGITS; ++t) {
     uint32_t byte, word;
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p)
     const uint32_t s1 = __shfl_down_sync(0xffffffffu, byte, 4), s2 = __shfl_down_sync(0xffffffffu, byte, 8),
                    s3 = __shfl_down_sync(0xffffffffu, byte, 12);
     if (live) {
-      const int64_t r = row * MX4_DIGITS + t;
+      const int64_t r = row * MX4_DIGITS + MX4_DIGITS - 1 - t;  // the smallest first
       *reinterpret_cast<uint32_t*>(p.codes + r * (p.steps * 64ll) + run * 4) = word;
       if ((run & 15) == 0)
         *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(r, run >> 4, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
@@ -177,18 +176,32 @@ __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p)
   }
 }
 
-// bfloat16 rows of any stride and alignment into rows that start on 16 bytes, the rest of a row zeros (for the copy engine)
-__global__ void __launch_bounds__(THREADS) mx4_align_kernel(const __nv_bfloat16* x, int64_t ldx, __nv_bfloat16* out, int ldo, int cols) {
+// Rows of any stride and alignment as bfloat16 rows that start on 16 bytes, what is left of a row zeros (for the copy engine). A row of 32
+// bits becomes three that add up to it, the smallest first: the bits that bfloat16 has room for, cut off, of the value, of what is left and of what is
+// left then. 24 bits are three times eight: nothing is lost from 2^-110 on, below it what lies under 2^-133. (Cut off, not rounded: no
+// part is larger than the value.) What is not finite is the first part alone.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) mx4_spread_kernel(const T* x, int64_t ldx, __nv_bfloat16* out, int ldo, int cols) {
+  constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
   pdl_trigger();
   pdl_wait();
-  const __nv_bfloat16* src = x + blockIdx.x * ldx;
-  __nv_bfloat16* dst = out + (int64_t)blockIdx.x * ldo;
-  for (int c = threadIdx.x * DIGIT_RUN; c < ldo; c += THREADS * DIGIT_RUN) {
-    uint32_t w[4] = {0, 0, 0, 0};
+  const T* src = x + blockIdx.x * ldx;
+  __nv_bfloat16* dst = out + (int64_t)blockIdx.x * PARTS * ldo;
+  for (int c = (blockIdx.y * THREADS + threadIdx.x) * DIGIT_RUN; c < ldo; c += gridDim.y * THREADS * DIGIT_RUN) {
+    uint32_t w[PARTS][DIGIT_RUN / 2];
 #pragma unroll
-    for (int j = 0; j < DIGIT_RUN; ++j)
-      if (c + j < cols) w[j >> 1] |= (uint32_t)__ldcg(reinterpret_cast<const unsigned short*>(src) + c + j) << (16 * (j & 1));
-    *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < DIGIT_RUN; ++j) {
+      float left = c + j < cols ? mx4_read(src + c + j) : 0.f;
+#pragma unroll
+      for (int t = 0; t < PARTS; ++t) {
+        const uint32_t part = left == left ? __float_as_uint(left) >> 16 : 0x7fffu;
+        w[t][j >> 1] = j & 1 ? w[t][j >> 1] | part << 16 : part;
+        left = fabsf(left) <= 3.402823466e38f ? left - __uint_as_float(part << 16) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < PARTS; ++t)
+      *reinterpret_cast<uint4*>(dst + (int64_t)(PARTS - 1 - t) * ldo + c) = make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
   }
 }
 
@@ -265,7 +278,7 @@ int launch_rows(const CucaMx4Rows* c, Form form) {
   const bool f32 = c->dtype == CUCA_F32;
   auto kernel = form == QUANTISE ? (f32 ? mx4_quantise_kernel<float> : mx4_quantise_kernel<__nv_bfloat16>)
                 : form == VALUES ? (f32 ? mx4_values_kernel<float> : mx4_values_kernel<__nv_bfloat16>)
-                                 : (f32 ? mx4_digits_kernel<float> : mx4_digits_kernel<__nv_bfloat16>);
+                                 : mx4_digits_kernel;
   const int64_t most = ((1ll << 31) - THREADS) / runs;  // rows of a launch
   for (int64_t at = 0; at < c->rows; at += most) {
     p.first = at;
@@ -282,8 +295,11 @@ int launch_rows(const CucaMx4Rows* c, Form form) {
 CUCA_API int cuca_mx4_quantise(const CucaMx4Rows* c) { return launch_rows(c, QUANTISE); }
 CUCA_API int cuca_mx4_values(const CucaMx4Rows* c) { return launch_rows(c, VALUES); }
 int cuca_mx4_digits(const CucaMx4Rows* c) { return launch_rows(c, DIGITS); }
-int cuca_mx4_align(const void* x, int64_t ldx, void* out, int ldo, int rows, int cols, cudaStream_t stream) {
-  cuca_launch(mx4_align_kernel, dim3(rows), dim3(THREADS), 0, stream, true, (const __nv_bfloat16*)x, ldx, (__nv_bfloat16*)out, ldo, cols);
+int cuca_mx4_spread(const void* x, int64_t ldx, bool f32, void* out, int ldo, int rows, int cols, cudaStream_t stream) {
+  int chunks = (ldo + THREADS * DIGIT_RUN - 1) / (THREADS * DIGIT_RUN);
+  const dim3 grid(rows, chunks < 64 ? chunks : 64);
+  if (f32) cuca_launch(mx4_spread_kernel<float>, grid, dim3(THREADS), 0, stream, true, (const float*)x, ldx, (__nv_bfloat16*)out, ldo, cols);
+  else cuca_launch(mx4_spread_kernel<__nv_bfloat16>, grid, dim3(THREADS), 0, stream, true, (const __nv_bfloat16*)x, ldx, (__nv_bfloat16*)out, ldo, cols);
   CUCA_CHECK_LAUNCH("gemm_mx4");
   return 0;
 }

@@ -16,7 +16,7 @@
 
 #define MX4_BLOCK 32
 #define MX4_STEP 128
-#define MX4_DIGITS 8  // rows in 4 bits that make up one of 16 or 32 bits (mx4.cu)
+#define MX4_DIGITS 8  // rows in 4 bits that make up a bfloat16 row (mx4.cu)
 
 // A launch, as Python packs it: one 64-bit word each, in this order (kernels/ops.py:mx4_quantise, mx4_values, gemm_mx4).
 struct CucaMx4Rows {

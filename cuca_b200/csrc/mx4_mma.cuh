@@ -119,16 +119,6 @@ struct Mx4Column {
   }
 };
 
-// Sixteen columns of this thread's lane as 16 / G results: G columns are one row of A (its digits, the smallest added first).
-template <int G>
-__device__ __forceinline__ void mx4_sum16(const uint32_t (&r)[16], float (&y)[16 / G]) {
-#pragma unroll
-  for (int i = 0; i < 16 / G; ++i) {
-    y[i] = __uint_as_float(r[i * G + G - 1]);
-#pragma unroll
-    for (int j = G - 2; j >= 0; --j) y[i] += __uint_as_float(r[i * G + j]);
-  }
-}
 __device__ __forceinline__ void mx4_ask16(uint32_t at, uint32_t (&r)[16]) {  // to be waited for
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -137,30 +127,66 @@ __device__ __forceinline__ void mx4_ask16(uint32_t at, uint32_t (&r)[16]) {  // 
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(at) : "memory");
 }
+// Results out of sixteens of columns: G columns are one row of A (its digits or parts, the smallest first), added up as they come.
+template <int G>
+struct Mx4Group {
+  static constexpr int LOADS = G == 3 ? 3 : 1, ROWS = LOADS * 16 / G;  // what whole rows take
+};
+template <int G, int LOAD>
+__device__ __forceinline__ void mx4_sum16(const uint32_t (&r)[16], float (&y)[Mx4Group<G>::ROWS]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int c = LOAD * 16 + j;
+    y[c / G] = c % G ? y[c / G] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
+  }
+}
+// `rows`: how many there are to have
+template <int G, int LOAD = 0>
+__device__ __forceinline__ void mx4_rows_of(uint32_t at, int rows, float (&y)[Mx4Group<G>::ROWS]) {
+  if constexpr (LOAD < Mx4Group<G>::LOADS) {
+    if (LOAD == 0 || LOAD * 16 < rows * G) {
+      uint32_t r[16];
+      mx4_ask16(at + LOAD * 16, r);
+      tmem_ld_wait();
+      mx4_sum16<G, LOAD>(r, y);
+      mx4_rows_of<G, LOAD + 1>(at, rows, y);
+    }
+  }
+}
 // A finished tile: lane `row` (0..127) of tensor memory holds weight row `row` of the tile, G columns `at`.. each of the m_here rows of A
 // from m0 on. Alone they are results, features from n0 on; else they go to shared memory, [row of A][128], for mx4_join (`again`: are added
 // to what this thread left there). GATED: the up part's accumulator lies `apart` columns further on, in shared memory `up` rows.
 template <int G, bool GATED>
 __device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, int m_here, int n0, int row, bool alone, float* sums,
                                           bool again = false, int apart = 0, int up = 0) {
-  constexpr int N = 16 / G;
+  constexpr int N = Mx4Group<G>::ROWS;
   const bool live = n0 + row < o.n;
   Mx4Column out(o, m0, live ? n0 + row : 0);
   for (int c = 0; c < m_here; c += N) {
-    uint32_t r[16], q[16];
-    mx4_ask16(at + c * G, r);
-    if (GATED) mx4_ask16(at + apart + c * G, q);
-    tmem_ld_wait();
     float v[N], u[N];
-    mx4_sum16<G>(r, v);
-    if (GATED) mx4_sum16<G>(q, u);
+    if constexpr (Mx4Group<G>::LOADS == 1) {
+      uint32_t r[16], q[16];
+      mx4_ask16(at + c * G, r);
+      if (GATED) mx4_ask16(at + apart + c * G, q);
+      tmem_ld_wait();
+      mx4_sum16<G, 0>(r, v);
+      if (GATED) mx4_sum16<G, 0>(q, u);
+    } else {
+      mx4_rows_of<G>(at + c * G, m_here - c, v);
+      if (GATED) mx4_rows_of<G>(at + apart + c * G, m_here - c, u);
+    }
     if (!alone) {
+      float* const sum = sums + c * TILE_A + row;
+      if (again) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (G == 1 || c + j < m_here) v[j] += sum[j * TILE_A];
+      }
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        if (c + j < m_here) {
-          float* const sum = sums + (c + j) * TILE_A + row;
-          *sum = again ? *sum + v[j] : v[j];
-          if (GATED) sum[up * TILE_A] = u[j];
+        if (G == 1 || c + j < m_here) {  // (where each column is a row there is room for whole sixteens of them)
+          sum[j * TILE_A] = v[j];
+          if (GATED) sum[(up + j) * TILE_A] = u[j];
         }
       }
     } else if (live) {

@@ -2044,8 +2044,9 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
     rows in 4 bits. Products are exact and summed in 32 bits. `epilogue`: EPI_STORE (plus `bias`; `out` 32-bit, or bfloat16 where
     `a` is not 32-bit), EPI_RESIDUAL (added to a 32-bit `out`, with `bias`), EPI_SWIGLU (silu(g) u of the stacked gate and up rows
     of `w`). `bias`: 32 or 16 bits. `out` must not overlap what is read. bfloat16 rows are multiplied as they are or, where there are few,
-    as digits that add up to them (`csrc/mx4.cu`), like 32-bit ones; a row that is not finite gives no finite results. Over more than
-    8,192 values a 32-bit result may be rounded once for each 8,192 begun."""
+    as digits that add up to them but for 2^-23 of the largest of 32 (`csrc/mx4.cu`); 32-bit rows as three bfloat16 parts that add up to
+    them (but for what lies under 2^-133). A row that is not finite gives no finite results. Over more than 8,192 values a 32-bit
+    result of bfloat16 rows may be rounded once for each 8,192 begun."""
     M, K = a.shape
     N, wk = w.shape
     if epilogue == EPI_SWIGLU:

@@ -87,3 +87,72 @@ def test_long_sums_in_32_bits_leave_after_8192_values(m, k, n, epilogue, one_sig
     elif stream is not None:
         want = want + stream[:, some].double()
     assert (out[:, some].double() - want).norm() < limit * want.norm()
+
+
+def _plain(xv, wv):
+    """The same product summed in 32 bits by PyTorch, in 64 bits."""
+    return (xv.float() @ wv.float().T).double()
+
+
+@pytest.mark.parametrize("k", [256, 4096])
+@pytest.mark.parametrize("larger", [1e3, 1e4, 1e9])
+@pytest.mark.parametrize("m", [1, 5, 64, 256, 300])
+def test_32_bit_rows_keep_their_bits_beside_larger_values(m, larger, k):
+    """Rows of 24 significant bits with one value of every 32 much larger, where the weight is zero: what counts is the others, and all of
+    their bits."""
+    n = 300
+    x, w = _normal(m, k, F32, m), _normal(n, k, F32, 2)
+    x[:, 5::32] *= larger
+    w[:, 5::32] = 0
+    out, xv, wv = _multiply("f32", x, w)
+    want = xv @ wv.T
+    assert (out.double() - want).norm() < _drift(min(k, 2048)) * want.norm()
+    rest = xv.clone()
+    rest[:, 5::32] = 0
+    _within(out, want, mx.chain_bound(rest, wv, k / 16 + 24) + 2.0 ** -24 * want.abs())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("m,k,n", [(1, 33, 300), (3, 130, 257), (5, 1010, 2050), (8, 4096, 512), (16, 14_336, 300), (24, 640, 200), (2, 14_336, 77),
+                                   (40, 4096, 320), (100, 2048, 130), (256, 4096, 512), (300, 14_336, 256)])
+def test_products_in_32_bits_by_their_2_norm(kind, m, k, n):
+    """As near to 64 bits as sums in 32 bits are, channels larger than others among the rows."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = (_normal(m, k, F32, m) * torch.exp(0.7 * torch.randn(k, generator=g, device="cuda"))).to(F32 if kind == "f32" else BF16)
+    out, xv, wv = _multiply(kind, x, _normal(n, k, F32, 2) / math.sqrt(k))
+    want = xv @ wv.T
+    assert (out.double() - want).norm() < _drift(min(k, 2048 if kind == "f32" else 8192)) * want.norm()
+
+
+def test_32_bit_rows_of_all_sizes():
+    """Numbers from the smallest on whose parts bfloat16 holds, up to the largest, times powers of two that bring them near one."""
+    k, n = 64, 40
+    for power in (-109, -60, 0, 100, 126):
+        x = _normal(7, k, F32, power % 97).clamp(-1.9, 1.9)
+        x = torch.where(x.abs() < 1, x.sign() + x, x) * 2.0 ** power  # 1 to 2 and their negatives
+        w = _normal(n, k, F32, 3) * 2.0 ** (-power / 2)
+        if power > 100:
+            w /= 1024  # (sums in range)
+        out, xv, wv = _multiply("f32", x, w)
+        _within(out, *mx.product(xv, wv, "store", F32, k / 16 + 24))
+
+
+def test_32_bit_rows_that_are_not_finite():
+    x, w = _normal(9, 96, F32, 1), _normal(33, 96, F32, 2)
+    x[2, 40], x[4, 3] = math.inf, -math.inf
+    x.view(torch.int32)[6, 70] = 0x7F800001  # a NaN of the lowest bits
+    out, xv, wv = _multiply("f32", x, w)
+    assert out[6].isnan().all() and not out[[2, 4]].isfinite().any()
+    good = [0, 1, 3, 5, 7, 8]
+    _within(out[good], *mx.product(xv[good], wv, "store", F32, 30))
+
+
+@pytest.mark.parametrize("epilogue", ["store", "residual", "swiglu"])
+@pytest.mark.parametrize("m,k,n", [(1, 2049, 200), (8, 4096, 1100), (17, 6100, 77), (85, 2500, 130), (86, 4100, 9500), (171, 9000, 96), (256, 2300, 640)])
+def test_32_bit_rows_whose_sums_leave_several_times(m, k, n, epilogue):
+    """Alone, shared and gated, tiles of 85 rows and of few; a bias and a stream are rounded into a result once."""
+    gated = epilogue == "swiglu"
+    x, w = _normal(m, k, F32, m), _normal(2 * n if gated else n, k, F32, n) / math.sqrt(k)
+    bias, stream = (None if gated else _normal(1, n, F32, 5)[0].contiguous()), (_normal(m, n, F32, 6) if epilogue == "residual" else None)
+    out, xv, wv = _multiply("f32", x, w, epilogue, F32, bias, stream)
+    _within(out, *mx.product(xv, wv, epilogue, F32, k / 16 + 24, bias, stream))
