@@ -13,11 +13,12 @@
 // its part of the features up in order out of the others': no workspace, equal bits in every run. Many tiles: a block takes tiles in turn,
 // the next one's loads under this one's results.
 //
-// Few bfloat16 rows come here too, as eight digits each (mx4.cu): G columns make one row of the result.
+// Few bfloat16 rows come here too, as twelve digits each (mx4.cu): G columns make one row of the result, and what
+// the digits left of a row, seldom anything, is multiplied on the ordinary pipes and added.
 //
 // Measured, K x features: 2,048 rows 4096 x 14336 gated 120 us (4.0 PFLOP/s; the tensor pipe busy for half of it: a stage takes 1,190
 // clocks of which its contractions need 768, and a tile's results are not hidden), 14336 x 4096 66 us (3.6); 8 rows 4096 x 6144 5.9 us;
-// 8 rows as digits 4096 x 14336 gated 16.0 us with the digits (3.9 TB/s), 14336 x 4096 13.5.
+// 8 rows as digits 4096 x 14336 gated 16.9 us with the digits (3.7 TB/s), 14336 x 4096 14.4.
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
 
@@ -28,7 +29,7 @@ constexpr int STAGE_STEPS = 2;              // of 128 values
 constexpr int MAX_STAGES = 8;
 constexpr int W_BYTES = TILE_A * STAGE_BYTES_K;
 constexpr int SCALE_BYTES = 512;            // of 128 rows and a step
-constexpr int MAX_CLUSTER = 4;              // (shares of K; eight took as long or longer: 14336 x 4096, 8 rows as digits 15.0 us, four 13.5)
+constexpr int MAX_CLUSTER = 4;              // (shares of K; eight took as long or longer: 14336 x 4096, 64 columns of digits 15.0 us, four 13.5)
 constexpr int MANY_ROWS = 256;              // more rows than these: two blocks of features
 constexpr int MANY_TILE = 192;              // ... and tiles of so many rows: two accumulators leave 128 columns for scales
 // A warp that loads weights, one that loads rows, one that multiplies, and the others read results: sixteen of tiles of many rows, whose
@@ -41,6 +42,8 @@ constexpr int BARRIERS = 512;
 struct Params {
   const uint8_t* a_scales;
   const uint8_t* w_scales;
+  const uint8_t* w;
+  Mx4Rest rest;    // of digits
   Mx4Out o;
   int k_steps, k_stages;
   int nt;          // rows of A of a whole tile, a multiple of 16
@@ -238,16 +241,28 @@ __global__ void __launch_bounds__(threads(SPANS), SPANS == 2 ? 1 : 2) gemm_mx4_c
     constexpr int PARTS = BLOCKS == 2 && !DUAL ? SETS / 2 : SETS;
     const int set = (warp - READ_WARP) >> 2, part = set % PARTS, block = set / PARTS, row = (warp & 3) * 32 + lane;
     const uint32_t at = acc + block * p.nt + ((uint32_t)((warp & 3) * 32) << 16);
+    Mx4RestOf rest{p.rest, p.w, p.w_scales, p.k_steps, ks0 * STAGE_STEPS, min(ks1 * STAGE_STEPS, p.k_steps), false};
+    if (G > 1) {  // while the products run: is there any?
+      const int flags = p.o.m * p.k_steps;
+      auto of = [](uint32_t word, int left) { return left >= 4 ? word : left > 0 ? word & ((1u << 8 * left) - 1) : 0u; };
+      uint32_t some = 0;
+      for (int i = lane * 16; i < flags; i += 512) {  // (there is memory to the end of 256)
+        const uint4 f = __ldcg(reinterpret_cast<const uint4*>(p.rest.flags + i));
+        some |= of(f.x, flags - i) | of(f.y, flags - i - 4) | of(f.z, flags - i - 8) | of(f.w, flags - i - 12);
+      }
+      rest.any = __any_sync(0xffffffffu, some != 0);
+    }
     float* sums = reinterpret_cast<float*>(smem) + block * (p.nt / G) * TILE_A;  // (of a cluster: every copy into the stages has been waited for)
     Mx4Ring acc_ring;
     for (int tile = first_tile; tile < p.tiles; tile += tile_step, acc_ring.next(1)) {
       const Tile t = tile_at(tile);
       if (!warp_wait(done, acc_ring.parity, p.err, abort_flag)) break;
       tc_fence_after();
-      const int each = (((t.nt + PARTS - 1) / PARTS + 15) & ~15) / G, first = part * each, last = min(first + each, t.m_here);
+      constexpr int UNIT = 16 * Mx4Group<G>::LOADS;
+      const int each = ((t.nt + PARTS - 1) / PARTS + UNIT - 1) / UNIT * UNIT / G, first = part * each, last = min(first + each, t.m_here);
       if (last > first && (block == 0 || t.scaled))
         mx4_leave<G, DUAL>(p.o, at + first * G, t.t0 + first, last - first, t.n0 + block * TILE_A, row, p.share == 1, sums + first * TILE_A,
-                           false, p.nt, p.nt / G);
+                           false, p.nt, p.nt / G, rest);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_free);
@@ -268,10 +283,11 @@ __global__ void __launch_bounds__(threads(SPANS), SPANS == 2 ? 1 : 2) gemm_mx4_c
 }
 
 template <int BLOCKS, bool DUAL, int SPANS, int G>
-int launch_spans(const CucaMx4Gemm* c) {
+int launch_spans(const CucaMx4Gemm* c, const Mx4Rest* rest) {
   const int64_t m = c->m * G;  // rows in 4 bits
   Params p;
-  p.a_scales = c->a_scales; p.w_scales = c->w_scales;
+  p.a_scales = c->a_scales; p.w_scales = c->w_scales; p.w = c->w;
+  p.rest = rest ? *rest : Mx4Rest{};
   p.o = Mx4Out{c->out, c->bias, c->ldo, (int)c->m, (int)c->n, (int)c->out_f32, (int)c->epilogue, (int)c->bias_f32};
   p.k_steps = (int)mx4_steps(c->k);
   p.k_stages = (p.k_steps + STAGE_STEPS - 1) / STAGE_STEPS;
@@ -312,15 +328,19 @@ int launch_spans(const CucaMx4Gemm* c) {
 }
 
 template <int G>
-int launch(const CucaMx4Gemm* c) {
+int launch(const CucaMx4Gemm* c, const Mx4Rest* rest) {
   const int64_t m = c->m * G;
   // a tile of more than 128 rows, or one that starts in the middle of 128, touches the scales of two runs of 128 rows
-  if (c->epilogue == EPI_SWIGLU) return m > 128 ? launch_spans<2, true, 2, G>(c) : launch_spans<2, true, 1, G>(c);
-  if (m > MANY_ROWS) return launch_spans<2, false, 2, G>(c);
-  return m > 128 ? launch_spans<1, false, 2, G>(c) : launch_spans<1, false, 1, G>(c);
+  if (c->epilogue == EPI_SWIGLU) return m > 128 ? launch_spans<2, true, 2, G>(c, rest) : launch_spans<2, true, 1, G>(c, rest);
+  if constexpr (G == 1) {
+    if (m > MANY_ROWS) return launch_spans<2, false, 2, G>(c, rest);
+  } else {
+    CUCA_REQUIRE(m <= MANY_TILE, "gemm_mx4: %lld rows as digits", (long long)c->m);  // a tile
+  }
+  return m > 128 ? launch_spans<1, false, 2, G>(c, rest) : launch_spans<1, false, 1, G>(c, rest);
 }
 
 }  // namespace
 
-// `digits`: A holds MX4_DIGITS rows for each of c->m
-int cuca_gemm_mx4_codes(const CucaMx4Gemm* c, bool digits) { return digits ? launch<MX4_DIGITS>(c) : launch<1>(c); }
+// `rest`: A holds MX4_DIGITS rows for each of c->m, and this is what they left of them; else null
+int cuca_gemm_mx4_codes(const CucaMx4Gemm* c, const Mx4Rest* rest) { return rest ? launch<MX4_DIGITS>(c, rest) : launch<1>(c, nullptr); }

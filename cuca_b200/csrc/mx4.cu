@@ -30,6 +30,8 @@ struct RowsParams {
   uint32_t magic, shift;  // i / runs = (i * magic >> 32) >> shift, for i below 2^31
   int cols, steps;
   int align;  // rows start on so many bytes: 32, 16 or less
+  uint8_t* rest_flags;  // of digits, as Mx4Rest
+  __nv_bfloat16* rest;
 };
 
 // Row of the launch and run of it that thread i has.
@@ -147,9 +149,11 @@ __global__ void __launch_bounds__(THREADS) mx4_quantise_kernel(const RowsParams 
     *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(row, run >> 3, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
 }
 
-// bfloat16 rows as eight rows in 4 bits each, whose values add up to theirs: digits of three bits (mx4_digit). After eight what is
-// left of a value is at most 2^-23 of its block's largest: nothing, where it is within 2^14 of it, and where
-// some are much larger than the rest the digits that these do not need go to the others.
+// bfloat16 rows as twelve rows in 4 bits each, whose values add up to theirs: digits of three bits (mx4_digit). After twelve what is
+// left of a value is at most 2^-35 of its block's largest: nothing, where it is within 2^27 of it. What is left all the same is a
+// bfloat16 number too (a multiple of the value's last place, and no larger than it) and is kept beside the digits, for the product
+// to add in 32 bits. (Of 32,768 normal values one
+// leaves something after eight digits; after twelve one in some six hundred times as many.)
 __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p) {
   pdl_trigger();
   pdl_wait();
@@ -161,18 +165,35 @@ __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p)
 #pragma unroll
   for (int j = 0; j < DIGIT_RUN; ++j) v[j] = 0.f;
   if (live) load<__nv_bfloat16, DIGIT_RUN>(p, row, run * DIGIT_RUN, v);
+  uint32_t byte = mx4_digit_power(v);
+  // the bytes of the step's four blocks, lowest first, for the step's first lane
+  uint32_t bytes = byte | __shfl_down_sync(0xffffffffu, byte, 4) << 8 | __shfl_down_sync(0xffffffffu, byte, 8) << 16 |
+                   __shfl_down_sync(0xffffffffu, byte, 12) << 24;
+  byte = min(byte, 254u);  // (of zeros)
 #pragma unroll
   for (int t = 0; t < MX4_DIGITS; ++t) {
-    uint32_t byte, word;
-    mx4_digit(v, byte, word);
-    const uint32_t s1 = __shfl_down_sync(0xffffffffu, byte, 4), s2 = __shfl_down_sync(0xffffffffu, byte, 8),
-                   s3 = __shfl_down_sync(0xffffffffu, byte, 12);
+    const uint32_t word = mx4_digit(v, byte);
     if (live) {
       const int64_t r = row * MX4_DIGITS + MX4_DIGITS - 1 - t;  // the smallest first
       *reinterpret_cast<uint32_t*>(p.codes + r * (p.steps * 64ll) + run * 4) = word;
-      if ((run & 15) == 0)
-        *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(r, run >> 4, p.steps)) = byte | s1 << 8 | s2 << 16 | s3 << 24;
+      if ((run & 15) == 0) *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_at(r, run >> 4, p.steps)) = bytes;
     }
+    byte = max((int)byte - 3, 1);
+    bytes = __vmaxu4(__vsubus4(bytes, 0x03030303u), 0x01010101u);
+  }
+  bool some = false;
+#pragma unroll
+  for (int j = 0; j < DIGIT_RUN; ++j) some = some || v[j] != 0.f;
+  // of this step, which sixteen lanes have
+  some = (__ballot_sync(0xffffffffu, some) >> (threadIdx.x & 16) & 0xffffu) != 0;
+  if (!live) return;
+  const int64_t step = row * p.steps + (run >> 4);
+  if ((run & 15) == 0) p.rest_flags[step] = some;
+  if (some) {
+    uint32_t w[DIGIT_RUN / 2];
+#pragma unroll
+    for (int j = 0; j < DIGIT_RUN; j += 2) w[j / 2] = __float_as_uint(v[j]) >> 16 | (__float_as_uint(v[j + 1]) & 0xffff0000u);
+    *reinterpret_cast<uint4*>(p.rest + step * MX4_STEP + (run & 15) * DIGIT_RUN) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -261,7 +282,7 @@ __global__ void __launch_bounds__(THREADS) mx4_values_kernel(const RowsParams p)
 
 enum Form { QUANTISE, VALUES, DIGITS };
 
-int launch_rows(const CucaMx4Rows* c, Form form) {
+int launch_rows(const CucaMx4Rows* c, Form form, const Mx4Rest& rest = {}) {
   const char* what = form == QUANTISE ? "mx4_quantise" : form == VALUES ? "mx4_values" : "gemm_mx4";
   CUCA_REQUIRE(c->dtype == CUCA_F32 || c->dtype == CUCA_BF16, "%s: unknown dtype %d", what, (int)c->dtype);
   CUCA_REQUIRE(c->rows >= 0 && c->cols > 0 && c->cols < (1ll << 30), "%s: %lld rows of %lld values", what, (long long)c->rows, (long long)c->cols);
@@ -269,7 +290,8 @@ int launch_rows(const CucaMx4Rows* c, Form form) {
   CUCA_REQUIRE((((uintptr_t)c->codes | (uintptr_t)c->scales) & 15) == 0, "%s: codes and scales must start on 16 bytes", what);
   const int64_t elem = c->dtype == CUCA_F32 ? 4 : 2, steps = mx4_steps(c->cols);
   const int64_t runs = steps * (MX4_STEP / (form == DIGITS ? DIGIT_RUN : RUN));
-  RowsParams p{c->x, c->x, c->codes, c->scales, c->ldx, 0, 0, (uint32_t)runs, 0, 0, (int)c->cols, (int)steps, 1};
+  RowsParams p{c->x, c->x, c->codes, c->scales, c->ldx, 0, 0, (uint32_t)runs, 0, 0, (int)c->cols, (int)steps, 1,
+               const_cast<uint8_t*>(rest.flags), const_cast<__nv_bfloat16*>(rest.values)};
   for (int align = 32; align >= 16 && p.align == 1; align /= 2)
     if ((uintptr_t)c->x % align == 0 && (c->ldx * elem % align == 0 || c->rows == 1)) p.align = align;
   // magic = ceil(2^(32 + shift) / runs) with 2^shift < runs <= 2^(shift + 1) is below 2^32 and off by less than one: exact below 2^31
@@ -294,7 +316,7 @@ int launch_rows(const CucaMx4Rows* c, Form form) {
 
 CUCA_API int cuca_mx4_quantise(const CucaMx4Rows* c) { return launch_rows(c, QUANTISE); }
 CUCA_API int cuca_mx4_values(const CucaMx4Rows* c) { return launch_rows(c, VALUES); }
-int cuca_mx4_digits(const CucaMx4Rows* c) { return launch_rows(c, DIGITS); }
+int cuca_mx4_digits(const CucaMx4Rows* c, const Mx4Rest& rest) { return launch_rows(c, DIGITS, rest); }
 int cuca_mx4_spread(const void* x, int64_t ldx, bool f32, void* out, int ldo, int rows, int cols, cudaStream_t stream) {
   int chunks = (ldo + THREADS * DIGIT_RUN - 1) / (THREADS * DIGIT_RUN);
   const dim3 grid(rows, chunks < 64 ? chunks : 64);

@@ -16,7 +16,7 @@
 
 #define MX4_BLOCK 32
 #define MX4_STEP 128
-#define MX4_DIGITS 8  // rows in 4 bits that make up a bfloat16 row (mx4.cu)
+#define MX4_DIGITS 12  // rows in 4 bits that make up a bfloat16 row (mx4.cu)
 
 // A launch, as Python packs it: one 64-bit word each, in this order (kernels/ops.py:mx4_quantise, mx4_values, gemm_mx4).
 struct CucaMx4Rows {
@@ -39,6 +39,11 @@ struct CucaMx4Gemm {
   void* scratch;  // what cuca_gemm_mx4_scratch asked for
   int* err;
   cudaStream_t stream;
+};
+// What the digits of bfloat16 rows leave of them (mx4.cu).
+struct Mx4Rest {
+  const uint8_t* flags;         // [rows, steps]: a step has anything left
+  const __nv_bfloat16* values;  // [rows, steps, 128], written where its flag is set
 };
 static_assert(sizeof(CucaMx4Rows) == 8 * 8 && sizeof(CucaMx4Gemm) == 18 * 8, "one 64-bit word each");
 
@@ -89,38 +94,30 @@ __device__ __forceinline__ uint32_t mx4_codes(const float* v) {
   return w;
 }
 
-// A digit of eight values, a quarter of a block whose other quarters the three neighbouring lanes have. With a = max |v| of the block,
-//
-//   e = max(ceil(log2 a) - 1, -126),   d = v / 2^e rounded to a multiple of 1/2 (at most 2 in magnitude),   v <- v - d 2^e,
-//
-// every step exact. What is left is at most 2^(e-2), so e falls by three or more a digit. A block that is not finite becomes NaN whole.
-__device__ __forceinline__ void mx4_digit(float (&v)[8], uint32_t& byte, uint32_t& word) {
-  float a = 0.f;
-  bool finite = true;
+// The first power of a block's digits, of which this lane and the three beside it have eight values each: with a = max |v|, the byte of
+// 2^e, e = max(ceil(log2 a) - 1, -126). A block that is not finite becomes NaN whole: byte 255, and zeros in place of its values.
+__device__ __forceinline__ uint32_t mx4_digit_power(float (&v)[8]) {
+  uint32_t most = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    a = fmaxf(a, fabsf(v[j]));  // (a NaN is passed over)
-    finite = finite && fabsf(v[j]) <= 3.402823466e38f;
-  }
-  uint32_t most = finite ? __float_as_uint(a) : 0x7f800000u;
+  for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
   most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
   most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-  word = 0;
-  if (most < 0x7f800000u) {
-    byte = max((int)(most >> 23) - ((most & 0x7fffffu) ? 0 : 1), 1);
-    const float down = mx4_power(254 - byte), up = mx4_power(byte);  // 2^-e, 2^e
-    float d[8];
+  if (most < 0x7f800000u) return max((int)(most >> 23) - ((most & 0x7fffffu) ? 0 : 1), 1);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      d[j] = __fadd_rn(__fmul_rn(v[j], down), 6291456.f) - 6291456.f;  // 1.5 * 2^22, whose last place is 1/2
-      v[j] = fmaf(-d[j], up, v[j]);
-    }
-    word = mx4_codes(d);
-  } else {
-    byte = 255;
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  return 255;
+}
+// A digit of eight values that are 2^(e+1) at most: d = v / 2^e rounded to a multiple of 1/2, v <- v - d 2^e, every step exact. What is
+// left is at most 2^(e-2), so the next digit's power is e - 3, whatever the values: digits need no more of each other than what is left.
+__device__ __forceinline__ uint32_t mx4_digit(float (&v)[8], uint32_t byte) {
+  const float down = mx4_power(254 - byte), up = mx4_power(byte);  // 2^-e, 2^e
+  float d[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  for (int j = 0; j < 8; ++j) {
+    d[j] = __fadd_rn(__fmul_rn(v[j], down), 6291456.f) - 6291456.f;  // 1.5 * 2^22, whose last place is 1/2
+    v[j] = fmaf(-d[j], up, v[j]);
   }
+  return mx4_codes(d);
 }
 
 // Eight codes as bfloat16 numbers times the power of two that a byte stands for, exactly, in their order.

@@ -130,7 +130,7 @@ __device__ __forceinline__ void mx4_ask16(uint32_t at, uint32_t (&r)[16]) {  // 
 // Results out of sixteens of columns: G columns are one row of A (its digits or parts, the smallest first), added up as they come.
 template <int G>
 struct Mx4Group {
-  static constexpr int LOADS = G == 3 ? 3 : 1, ROWS = LOADS * 16 / G;  // what whole rows take
+  static constexpr int LOADS = G == 1 ? 1 : 3, ROWS = LOADS * 16 / G;  // what whole rows take
 };
 template <int G, int LOAD>
 __device__ __forceinline__ void mx4_sum16(const uint32_t (&r)[16], float (&y)[Mx4Group<G>::ROWS]) {
@@ -153,12 +153,44 @@ __device__ __forceinline__ void mx4_rows_of(uint32_t at, int rows, float (&y)[Mx
     }
   }
 }
+// What the digits of a row left in steps s0..s1, times a weight row: sixteen codes' words a step, products exact, added up in 32 bits. Seldom
+// there is any: not fast.
+struct Mx4RestOf {
+  Mx4Rest rest;
+  const uint8_t* w;
+  const uint8_t* w_scales;
+  int steps, s0, s1;
+  bool any;
+};
+__device__ __noinline__ float mx4_rest_product(const Mx4RestOf r, int row, int n) {
+  float y = 0.f;
+  for (int s = r.s0; s < r.s1; ++s) {
+    const int64_t step = (int64_t)row * r.steps + s;
+    if (!__ldcg(r.rest.flags + step)) continue;
+    const uint4* x = reinterpret_cast<const uint4*>(r.rest.values + step * MX4_STEP);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w + ((int64_t)n * r.steps + s) * 64);
+    const uint32_t bytes = __ldcg(reinterpret_cast<const uint32_t*>(r.w_scales + mx4_scale_at(n, s, r.steps)));
+    for (int i = 0; i < 16; ++i) {
+      const uint4 q = __ldcg(x + i);
+      if (!(q.x | q.y | q.z | q.w)) continue;
+      const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+      uint32_t c[4];
+      mx4_to_bf16<true>(__ldcg(w + i), mx4_factor<true>(bytes >> (i >> 2) * 8 & 255), c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y = fmaf(__uint_as_float(v[j] << 16), __uint_as_float(c[j] << 16), y);
+        y = fmaf(__uint_as_float(v[j] & 0xffff0000u), __uint_as_float(c[j] & 0xffff0000u), y);
+      }
+    }
+  }
+  return y;
+}
 // A finished tile: lane `row` (0..127) of tensor memory holds weight row `row` of the tile, G columns `at`.. each of the m_here rows of A
 // from m0 on. Alone they are results, features from n0 on; else they go to shared memory, [row of A][128], for mx4_join (`again`: are added
-// to what this thread left there). GATED: the up part's accumulator lies `apart` columns further on, in shared memory `up` rows.
+// to what this thread left there). GATED: the up part's accumulator lies `apart` columns further on, in shared memory `up` rows. `rest`: of digits, what they left of these rows.
 template <int G, bool GATED>
 __device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, int m_here, int n0, int row, bool alone, float* sums,
-                                          bool again = false, int apart = 0, int up = 0) {
+                                          bool again = false, int apart = 0, int up = 0, const Mx4RestOf& rest = {}) {
   constexpr int N = Mx4Group<G>::ROWS;
   const bool live = n0 + row < o.n;
   Mx4Column out(o, m0, live ? n0 + row : 0);
@@ -174,6 +206,17 @@ __device__ __forceinline__ void mx4_leave(const Mx4Out& o, uint32_t at, int m0, 
     } else {
       mx4_rows_of<G>(at + c * G, m_here - c, v);
       if (GATED) mx4_rows_of<G>(at + apart + c * G, m_here - c, u);
+    }
+    if constexpr (G == MX4_DIGITS) {
+      if (rest.any && live) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (c + j < m_here) {
+            v[j] += mx4_rest_product(rest, m0 + c + j, n0 + row);
+            if (GATED) u[j] += mx4_rest_product(rest, m0 + c + j, o.n + n0 + row);
+          }
+        }
+      }
     }
     if (!alone) {
       float* const sum = sums + c * TILE_A + row;

@@ -2044,7 +2044,7 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
     rows in 4 bits. Products are exact and summed in 32 bits. `epilogue`: EPI_STORE (plus `bias`; `out` 32-bit, or bfloat16 where
     `a` is not 32-bit), EPI_RESIDUAL (added to a 32-bit `out`, with `bias`), EPI_SWIGLU (silu(g) u of the stacked gate and up rows
     of `w`). `bias`: 32 or 16 bits. `out` must not overlap what is read. bfloat16 rows are multiplied as they are or, where there are few,
-    as digits that add up to them but for 2^-23 of the largest of 32 (`csrc/mx4.cu`); 32-bit rows as three bfloat16 parts that add up to
+    as digits that add up to them (`csrc/mx4.cu`); 32-bit rows as three bfloat16 parts that add up to
     them (but for what lies under 2^-133). A row that is not finite gives no finite results. Over more than 8,192 values a 32-bit
     result of bfloat16 rows may be rounded once for each 8,192 begun."""
     M, K = a.shape
@@ -2081,7 +2081,7 @@ def gemm_mx4(a, w: Mx4Matrix, out, epilogue=EPI_STORE, bias=None, err=None) -> N
     scratch = None
     if kind != 2:
         # what the library makes of the rows first; the answer depends on the address only by where its 16 bytes start
-        key = kind, a_at & 15, lda & 7, M, N > 0, K, epilogue
+        key = kind, a_at & 15, lda & 7, M, N, K, epilogue
         need = _mx4_scratch.get(key)
         if need is None:
             if len(_mx4_scratch) >= 4096:

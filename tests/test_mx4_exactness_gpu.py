@@ -42,10 +42,9 @@ def _within(out, want, bound):
 
 @pytest.mark.parametrize("kind", ["bf16", "f32", "codes"])
 @pytest.mark.parametrize("m", [1, 3, 9, 20, 41, 70])
-@pytest.mark.parametrize("n", [5, 77, 130, 201])
-def test_ragged_tiles_that_share_a_long_sum(kind, m, n):
+@pytest.mark.parametrize("k,n", [(2050, 5), (2050, 77), (2050, 130), (2050, 201), (14_337, 1201)])
+def test_ragged_tiles_that_share_a_long_sum(kind, m, k, n):
     """Blocks of a cluster add up sums of ragged tiles: lanes of a warp leave that with different numbers of rows."""
-    k = 2050
     x, w = _normal(m, k, F32 if kind == "f32" else BF16, m), _normal(2 * n, k, F32, n) / math.sqrt(k)
     for epilogue in ("store", "swiglu"):
         out, xv, wv = _multiply(kind, x, w, epilogue)
@@ -114,7 +113,7 @@ def test_32_bit_rows_keep_their_bits_beside_larger_values(m, larger, k):
 
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("m,k,n", [(1, 33, 300), (3, 130, 257), (5, 1010, 2050), (8, 4096, 512), (16, 14_336, 300), (24, 640, 200), (2, 14_336, 77),
-                                   (40, 4096, 320), (100, 2048, 130), (256, 4096, 512), (300, 14_336, 256)])
+                                   (40, 4096, 320), (100, 2048, 130), (256, 4096, 512), (300, 14_336, 256), (1, 4096, 4100), (8, 14_336, 1300), (16, 2050, 9000)])
 def test_products_in_32_bits_by_their_2_norm(kind, m, k, n):
     """As near to 64 bits as sums in 32 bits are, channels larger than others among the rows."""
     g = torch.Generator(device="cuda").manual_seed(k)
@@ -156,3 +155,98 @@ def test_32_bit_rows_whose_sums_leave_several_times(m, k, n, epilogue):
     bias, stream = (None if gated else _normal(1, n, F32, 5)[0].contiguous()), (_normal(m, n, F32, 6) if epilogue == "residual" else None)
     out, xv, wv = _multiply("f32", x, w, epilogue, F32, bias, stream)
     _within(out, *mx.product(xv, wv, epilogue, F32, k / 16 + 24, bias, stream))
+
+
+def _small_beside_large(m, k, dtype, seed):
+    """Rows whose blocks hold values of four sizes, 2^40, 2^25, 2^12 and about one; the weights to go with them are zero for all but the last."""
+    x = _normal(m, k, F32, seed)
+    counts = torch.ones(k, dtype=torch.bool, device="cuda")
+    for at, power in ((3, 40), (4, 25), (17, 12), (30, 40), (31, 25)):
+        x[:, at::32] *= 2.0 ** power
+        counts[at::32] = False
+    return x.to(dtype), counts
+
+
+@pytest.mark.parametrize("epilogue", ["store", "swiglu"])
+@pytest.mark.parametrize("k,n", [(200, 130), (4096, 300), (2050, 201), (512, 9600), (4096, 4100), (2050, 9001), (200, 84_000), (14_337, 1201)])
+@pytest.mark.parametrize("m", [1, 3, 8, 9, 11, 16, 17, 24])
+def test_few_rows_keep_their_bits_beside_larger_values(m, k, n, epilogue):
+    """The products of few rows are exact too: a value's bits are all there, however much larger its block's others are."""
+    x, counts = _small_beside_large(m, k, BF16, m)
+    w = _normal(2 * n if epilogue == "swiglu" else n, k, F32, 2) / math.sqrt(k)
+    w[:, ~counts] = 0
+    out, xv, wv = _multiply("bf16", x, w, epilogue)
+    xv[:, ~counts] = 0
+    _within(out, *mx.product(xv, wv, epilogue, F32, 2.5 * k / 16 + 24))
+
+
+@pytest.mark.parametrize("m", [1, 5, 16])
+def test_few_rows_of_every_size_in_a_block(m):
+    """A block whose values go from 2^70 down to 2^-120 in steps of 2^6, in any order; the weight reads one of them at a time."""
+    k = 96
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = _normal(m, k, F32, m)
+    x = (x.sign() * (1 + x.abs() % 1)).to(BF16).float()
+    for b in range(3):
+        x[:, 32 * b:32 * b + 32] *= torch.exp2(70.0 - 6 * torch.randperm(32, generator=g, device="cuda"))
+    x = x.to(BF16)
+    for n in (96, 180_000):
+        w = torch.zeros(n, k, device="cuda")
+        w[torch.arange(n), torch.arange(n) % k] = 1
+        out, xv, wv = _multiply("bf16", x, w)
+        assert torch.equal(out.double(), xv @ wv.T)
+
+
+def test_few_rows_of_the_smallest_numbers():
+    """Numbers below 2^-126, times weights that bring them up."""
+    x = (_normal(4, 64, F32, 1) * 2.0 ** -128).to(BF16)
+    for n in (70, 270_000):
+        out, xv, wv = _multiply("bf16", x, _normal(n, 64, F32, 2) * 2.0 ** 100)
+        _within(out, *mx.product(xv, wv, "store", F32, 30))
+
+
+@pytest.mark.parametrize("m", [1, 4, 10, 11, 16])
+def test_few_rows_of_a_large_weight_every_way(m):
+    """Rows with gaps and off 16 bytes, results into columns of a wider matrix, every epilogue and result type, a bias of either type, values
+    and weights that are not finite, and a graph replayed on other rows."""
+    from cuca_b200.kernels import ops
+    k, n = 2056, 8200
+    w = _normal(n, k, F32, 2) / math.sqrt(k)
+    w[5] = 0
+    w[7, 100] = math.inf
+    q, held = ops.mx4_quantise(w), mx.held(w)
+    fine = [i for i in range(n) if i != 7]
+    for gap, shift in ((0, 0), (8, 0), (3, 1)):
+        memory = torch.zeros(m * (k + gap) + shift, dtype=BF16, device="cuda")
+        x = memory[shift:].view(m, k + gap)[:, :k]
+        x.copy_(_normal(m, k, BF16, m))
+        for out_dtype, bias_dtype in ((BF16, BF16), (F32, F32), (F32, BF16)):
+            bias = _normal(1, n, bias_dtype, 3)[0].contiguous()
+            wide = torch.full((m, n + 9), 7.0, dtype=out_dtype, device="cuda")
+            ops.gemm_mx4(x, q, wide[:, 3:3 + n], bias=bias)
+            assert (wide[:, :3] == 7).all() and (wide[:, 3 + n:] == 7).all() and wide[:, 10].isnan().all()
+            _within(wide[:, 3:3 + n][:, fine], *mx.product(x.double(), held[fine], "store", out_dtype, 2.5 * k / 16 + 24, bias[fine]))
+        gated = torch.empty(m, n // 2, dtype=BF16, device="cuda")
+        ops.gemm_mx4(x, q, gated, ops.EPI_SWIGLU)
+        assert gated[:, 7].isnan().all()
+        pair = [i for i in range(n // 2) if i != 7]
+        both = held[pair + [n // 2 + i for i in pair]]
+        _within(gated[:, pair], *mx.product(x.double(), both, "swiglu", BF16, 2.5 * k / 16 + 24))
+    stream = _normal(m, n, F32, 4)
+    out = stream.clone()
+    ops.gemm_mx4(x, q, out, ops.EPI_RESIDUAL, bias)
+    _within(out[:, fine], *mx.product(x.double(), held[fine], "store", F32, 2.5 * k / 16 + 24, bias[fine], stream[:, fine]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.gemm_mx4(x, q, out)
+        ops.gemm_mx4(x, q, gated, ops.EPI_SWIGLU)
+    for seed in (8, 9):
+        x.copy_(_normal(m, k, BF16, seed))
+        x[0, 40] = math.nan
+        x[0, 70] *= 2.0 ** 90  # what these digits leave is multiplied too
+        x[-1, 1000] = 0.5 if m == 1 else math.inf
+        graph.replay()
+        torch.cuda.synchronize()
+        assert out[0].isnan().all() and (m == 1 or not out[-1].isfinite().any())
+        if m > 2:
+            _within(out[1:-1][:, fine], *mx.product(x[1:-1].double(), held[fine], "store", F32, 2.5 * k / 16 + 24))
