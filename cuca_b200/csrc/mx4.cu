@@ -170,9 +170,10 @@ __global__ void __launch_bounds__(THREADS) mx4_digits_kernel(const RowsParams p)
   uint32_t bytes = byte | __shfl_down_sync(0xffffffffu, byte, 4) << 8 | __shfl_down_sync(0xffffffffu, byte, 8) << 16 |
                    __shfl_down_sync(0xffffffffu, byte, 12) << 24;
   byte = min(byte, 254u);  // (of zeros)
+  const bool none = byte == 254;  // a digit could be 2^128: values past 2^127 are left whole
 #pragma unroll
   for (int t = 0; t < MX4_DIGITS; ++t) {
-    const uint32_t word = mx4_digit(v, byte);
+    const uint32_t word = mx4_digit(v, byte, none);
     if (live) {
       const int64_t r = row * MX4_DIGITS + MX4_DIGITS - 1 - t;  // the smallest first
       *reinterpret_cast<uint32_t*>(p.codes + r * (p.steps * 64ll) + run * 4) = word;

@@ -109,8 +109,9 @@ __device__ __forceinline__ uint32_t mx4_digit_power(float (&v)[8]) {
 }
 // A digit of eight values that are 2^(e+1) at most: d = v / 2^e rounded to a multiple of 1/2, v <- v - d 2^e, every step exact. What is
 // left is at most 2^(e-2), so the next digit's power is e - 3, whatever the values: digits need no more of each other than what is left.
-__device__ __forceinline__ uint32_t mx4_digit(float (&v)[8], uint32_t byte) {
-  const float down = mx4_power(254 - byte), up = mx4_power(byte);  // 2^-e, 2^e
+// `none`: zeros, and everything is left.
+__device__ __forceinline__ uint32_t mx4_digit(float (&v)[8], uint32_t byte, bool none) {
+  const float down = none ? 0.f : mx4_power(254 - byte), up = mx4_power(byte);  // 2^-e, 2^e
   float d[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {

@@ -250,3 +250,15 @@ def test_few_rows_of_a_large_weight_every_way(m):
         assert out[0].isnan().all() and (m == 1 or not out[-1].isfinite().any())
         if m > 2:
             _within(out[1:-1][:, fine], *mx.product(x[1:-1].double(), held[fine], "store", F32, 2.5 * k / 16 + 24))
+
+
+@pytest.mark.parametrize("m", [1, 7, 16, 20])
+def test_few_rows_of_the_largest_numbers(m):
+    """The type's largest and lowest values come through weights of one: no part of them is past the range."""
+    k, n = 96, 180_000
+    x = _normal(m, k, BF16, m)
+    x[0, 3], x[0, 40], x[-1, 70] = torch.finfo(BF16).max, torch.finfo(BF16).min, 1.75 * 2.0 ** 127
+    w = torch.zeros(n, k, device="cuda")
+    w[torch.arange(n), torch.arange(n) % k] = 1
+    out, xv, wv = _multiply("bf16", x, w)
+    assert torch.equal(out.double(), xv @ wv.T)
