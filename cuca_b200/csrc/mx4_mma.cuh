@@ -75,9 +75,15 @@ struct Mx4Out {
   int64_t ldo;
   int m, n, out_f32, epilogue, bias_f32;
 };
-// silu(g) u: for bfloat16 results the approximate reciprocal and exponential, good to 2^-20
+// silu(g) u. For 32-bit results g / (1 + e^-|g|) u, times e^-|g| where g is negative, so that no exponential is past the range: good to 2^-21
+// down to where e^-|g| lies under 2^-126 and has fewer bits of its own. For bfloat16 results the approximate reciprocal and exponential:
+// good to 2^-20 and |g| 2^-23 more, which the rounded product in the exponent costs (2^-16 at -100); below -87.3, where silu lies under
+// 2^-119, they give zero. (The other form for these too: 2,048 gated rows in 4 bits of 4096 x 14336 took 125 us, 115.)
 __device__ __forceinline__ float mx4_gate(bool exact, float g, float u) {
-  if (exact) return g / (1.f + expf(-g)) * u;
+  if (exact) {
+    const float z = expf(-fabsf(g));
+    return (g < 0.f ? g * z : g) / (1.f + z) * u;
+  }
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(-1.4426950408889634f * g)));
   return g * r * u;

@@ -262,3 +262,27 @@ def test_few_rows_of_the_largest_numbers(m):
     w[torch.arange(n), torch.arange(n) % k] = 1
     out, xv, wv = _multiply("bf16", x, w)
     assert torch.equal(out.double(), xv @ wv.T)
+
+
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+@pytest.mark.parametrize("kind,m,n", [("bf16", 97, 40), ("bf16", 10, 131_072), ("f32", 50, 24), ("codes", 30, 24)])
+def test_gated_unit_over_the_whole_range(kind, m, n, out_dtype):
+    """silu(g) u for g from -120 to 120. 32-bit results are good to 2^-20 of themselves, but for the exponential's own last place where that lies
+    under 2^-126; bfloat16 ones to |g| 2^-23 more, and a sigmoid under 2^-126 may be taken as zero."""
+    if kind == "f32" and out_dtype == BF16:
+        pytest.skip("32-bit rows have 32-bit results")
+    k = 64
+    x = torch.zeros(m, k, device="cuda")
+    x[:, 0] = torch.linspace(-120, 120, m, device="cuda") if kind != "codes" else torch.tensor([-96.0, -64, -3, 0.5, 48, 96], device="cuda").repeat(5)
+    x[:, 32] = 1
+    w = torch.zeros(2 * n, k, device="cuda")
+    w[:n, 0] = 1
+    w[n:, 32] = torch.tensor([1.0, 2.0 ** 20, -1.5, 2.0 ** 60], device="cuda").repeat(n // 4)
+    out, xv, wv = _multiply(kind, x if kind == "f32" else x.to(BF16), w, "swiglu", out_dtype)
+    g, u = (xv @ wv.T).chunk(2, 1)
+    want = g * torch.sigmoid(g) * u
+    if out_dtype == BF16:
+        bound = want.abs() * (2.0 ** -8 + 2.0 ** -20 + g.abs() * 2.0 ** -23) + (g * u).abs() * 2.0 ** -126 + 2.0 ** -134
+    else:
+        bound = want.abs() * (2.0 ** -24 + 2.0 ** -20) + (g * u).abs() * 2.0 ** -148 + 2.0 ** -150
+    _within(out, want, bound)
