@@ -2,7 +2,7 @@
 """Decode and prefill throughput of the engine on one B200, on the Llama-3.1-8B shape with random weights.
 
     python bench.py [--gpus 1] [--steps K] [--warmup W] [--batch 8] [--layers L] [--impl reference]
-                    [--shape llama-3.1-8b | llama-2-13b | llama-3.2-1b]
+                    [--shape llama-3.1-8b | llama-2-13b | llama-3.2-1b] [--weight-dtype mxfp4] [--activation-dtype mxfp4]
 
 One JSON line: `value` is decoded tokens per second at batch 8 (K captured decode steps back to back on the
 device, timed with CUDA events); `e2e` is the same through the public entry point (`LocalModel.generate`, host
@@ -16,6 +16,9 @@ steps. For more than one GPU it prints one line saying so and exits with 2: this
 shape instead: 64 requests with prompts of 16 to 2,048 random ids and 128 tokens each under continuous batching
 through `LocalModel.generate`; `value` is then generated tokens per second from submission to the last token,
 and `points.decode_b64` / `roofline` describe the steady decode step of all 64 at head size 64.
+
+`--weight-dtype mxfp4 [--activation-dtype mxfp4]` measures any of these with the projections' weights, or weights and
+rows, in 4 bits; `metric` and `config` then say so.
 """
 from __future__ import annotations
 
@@ -435,6 +438,8 @@ def main() -> int:
                     help="instead of the bench: prefill and decode of this design beside a Llama of equal width, "
                          "feed-forward size and layer runs, at --sizes (1b,3b,8b layer sizes; a few layers each)")
     ap.add_argument("--sizes", default=None, help="with --design: which of 1b,3b,8b (all else)")
+    ap.add_argument("--weight-dtype", choices=["mxfp4"], default=None, help="the same line with the projections' weights in 4 bits")
+    ap.add_argument("--activation-dtype", choices=["mxfp4"], default=None, help="with --weight-dtype: what enters them in 4 bits too")
     args = ap.parse_args()
 
     if args.impl == "reference":
@@ -491,7 +496,8 @@ def main() -> int:
         model_config=cfg, random_weights=RandomWeights(seed=SEED, std=0.02), dtype="bfloat16", context_length=CONTEXT,
         kv_block_size=16, batching=BatchingConfig(max_sequences=max_batch, kv_tokens=kv_tokens,
                                                   max_step_tokens=max(STEP_TOKENS, max_batch),
-                                                  prefill_chunk=STEP_TOKENS)))
+                                                  prefill_chunk=STEP_TOKENS),
+        weight_dtype=args.weight_dtype, activation_dtype=args.activation_dtype))
     load_s = time.perf_counter() - t0
     core, sched, backend = model.core, model.scheduler, model.backend
     vocab = cfg["vocab_size"]
@@ -662,6 +668,9 @@ def main() -> int:
     step_bytes = roofline["bytes_per_step"]
     clocks.stop()
 
+    small = {k: v for k, v in (("weight_dtype", args.weight_dtype), ("activation_dtype", args.activation_dtype)) if v}
+    if small:  # another workload than the headline's, named as such
+        metric += ", " + ", ".join("%s %s" % kv for kv in small.items())
     line = {
         "metric": metric,
         "value": round(value, 1), "unit": "tokens/s", "n_gpus": 1, "steps": steps_of_value, "warmup": args.warmup,
@@ -676,6 +685,7 @@ def main() -> int:
             "l2": "no flush: a step reads %.1f GB, far above the 126 MB L2" % (step_bytes / 1e9),
             "parallelism": "1 GPU",
             "settle": "%.1f s idle between the prompts and a decode measurement's warm-up steps" % SETTLE_S,
+            **small,
         },
         "e2e": e2e, "gpu_launches": int(launches_per_step * (point_steps if mixed else args.steps)),
         "launches_per_step": launches_per_step,
