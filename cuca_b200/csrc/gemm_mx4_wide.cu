@@ -7,10 +7,11 @@
 //
 // A tile has 128 features, or 64 gate and 64 up rows of a gated unit, so that one conversion serves up to 256 rows either way.
 //
-// What bounds it: up to 128 rows the conversion, whose 17 instructions for eight codes take a scheduler 22 clocks, at most 46 codes a clock
-// and SM where the memory brings 44 (64 rows, 14336 x 4096: 19.5 us, without the conversion's arithmetic 15.7); many rows, the tensor
+// What bounds it: up to 128 rows in part the conversion, whose 17 instructions for eight codes take a scheduler 22 clocks, at most 46 codes a
+// clock and SM where the memory brings 44 (64 rows, 14336 x 4096: 19.0 us, without the conversion's arithmetic 15.7, of which a block's
+// start and the join are 6); many rows, the tensor
 // cores and their power: a tile of 256 rows converts 16 codes a clock (2,048 rows, 14336 x 4096: 166 us, 1.45 PFLOP/s; 4096 x 14336 gated
-// 396 us, 1.21: a tile's results, 7 us of 30, are not hidden). More converting warps or two tiles a block in turn were no faster.
+// 393 us, 1.22: a tile's results, 7 us of 30, are not hidden). More converting warps or two tiles a block in turn were no faster.
 // The multiplying warp is short of time too (a wait takes it 150 clocks, an instruction 60 where eight warps convert beside it), so
 // what it waits for is one barrier a step, on which the converted weights and the rows arrive, and a step is 128 values of a row
 // but for the largest tiles, whose rows' tiles would leave two steps in shared memory.
