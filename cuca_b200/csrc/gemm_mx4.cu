@@ -16,7 +16,8 @@ namespace {
 // ones 2048 x 2048 8 rows 7.7 and 6.2, 1024 x 5632 gated 8.2 and 6.7, 2048 x 6000 gated 11.8 and 8.2.
 bool as_digits(const CucaMx4Gemm* c) {
   const int64_t rows = c->n * (c->epilogue == EPI_SWIGLU ? 2 : 1);
-  return rows * c->k >= 1 << 24 && c->m <= (rows >= 5120 ? 16 : 10);
+  // (of longer rows what digits leave, up to 8 us a row and 128 values where all of them leave something, would come near a wait's two seconds)
+  return rows * c->k >= 1 << 24 && c->k <= 1 << 18 && c->m <= (rows >= 5120 ? 16 : 10);
 }
 
 enum Form { CODES, DIGITS, PARTS, ALIGNED, WIDE };

@@ -160,7 +160,8 @@ __device__ __forceinline__ void mx4_rows_of(uint32_t at, int rows, float (&y)[Mx
   }
 }
 // What the digits of a row left in steps s0..s1, times a weight row: sixteen codes' words a step, products exact, added up in 32 bits. Seldom
-// there is any: not fast.
+// there is any: not fast (8 rows of 4096 x 14336 gated of which every block leaves something 2.1 ms; all of a block's codes asked for at once 0.7,
+// but then the rows that leave nothing pay for the registers: 2 % of a model's step).
 struct Mx4RestOf {
   Mx4Rest rest;
   const uint8_t* w;
